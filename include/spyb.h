@@ -230,6 +230,101 @@ spyb_status spyb_prefill_selftest_wait_timeout(spyb_backend *backend, uint64_t l
  * kernels returned by themselves with such a code, accumulators came after their CTA had given up, and nothing of them is left for the next launch. */
 spyb_status spyb_prefill_selftest_handoff_timeout(spyb_backend *backend, uint64_t limit_ns, int32_t *error_code_out);
 
+/* ---- steps over many sequences of different lengths: caches in pages, attention over them, sampling (no reference counterpart: the reference keeps one
+ * sequence in one cache of n_ctx rows and samples greedily, model/src/llm/plugin/attention.cpp:228-262, model/include/llm/sampler/greedy.h:20-25).
+ * All pointers are device memory; the calls enqueue on the backend's stream and return (spyb_sync waits). What a call gives is a function of its operands alone,
+ * the same bits every time. Lengths, page tables and settings are read on the device when the kernels run, and whatever they hold, nothing
+ * outside the described buffers is touched. Descriptors are read during the call only. Calls on one backend come from one thread at a time (as spyb_submit's).
+ * Operands that are not described as optional must be there; what a call does not take is answered with SPYB_UNSUPPORTED before anything is enqueued. */
+
+/* Keys and values of all sequences, `page_size` positions a page. Element (page, position in the page, head, e) of either lies at page * page_stride +
+ * position * token_stride + head * head_stride + e, in elements; strides are multiples of 8, k and v 16-byte aligned. */
+typedef struct {
+    void   *k, *v;
+    int32_t number_type;          /* SPYB_FP16 */
+    int32_t n_pages, page_size, n_head_kv, head_dim;
+    int32_t reserved;
+    int64_t page_stride, token_stride, head_stride;
+} spyb_paged_cache;
+
+/* Which rows of a call are whose. Sequence s has the rows row_start[s] .. row_start[s+1]-1 (ascending; none is allowed) and n_kv[s] positions, these rows' among
+ * them: its rows are its last positions, row r is position n_kv[s] - row_start[s+1] + r. Position p lies in page page_table[s * table_stride + p / page_size].
+ * A negative position, one behind the table's row, and a page id outside 0 .. n_pages-1 are "not there": nothing is stored, nothing is seen.
+ * Rows from row_start[n_seq] to n_rows-1 (a padded batch) belong to nobody; their outputs are left as they were. */
+typedef struct {
+    const int32_t *row_start;     /* [n_seq + 1] */
+    const int32_t *n_kv;          /* [n_seq] */
+    const int32_t *page_table;    /* [n_seq][table_stride] */
+    int32_t n_seq, n_rows;        /* n_rows: rows that the call's buffers hold */
+    int32_t max_rows;             /* most rows of one sequence, if known (0: n_rows): chooses kernels; sequences with more rows are answered all the same */
+    int32_t table_stride;
+} spyb_paged_batch;
+
+/* Q and K rotated to their positions, K and V appended to the cache: what Rope, Rope, Copy, Copy do for one sequence (orchestration/include/operator/non-linear.h:191-207,
+ * backend/host/operator/view.cpp:83-227). Pair i of a head turns by position * freq_scale * freq_base^(-2 i / rope_dim), an angle in 64 bits; elements behind
+ * rope_dim are copied. q, k, v: [n_rows][heads][head_dim] with their own row strides (elements), in_type SPYB_FP32 or SPYB_FP16; rounded once, to nearest.
+ * q_out may be q itself where both are of one type and stride; it must not overlap k, v or the cache otherwise. Two rows of one call that share a page and
+ * a position in it leave either's values there. q == NULL (n_head = 0): K and V only. head_dim: a multiple of 8, at most 256; rope_dim: a multiple
+ * of 8, at most head_dim; pointers 16-byte aligned, row strides multiples of 8 (FP32: 4). */
+enum { SPYB_ROPE_NONE = -1, SPYB_ROPE_PAIRS = 0, SPYB_ROPE_HALVES = 2 };   /* pairs (2 i, 2 i + 1), or (i, i + rope_dim / 2) */
+typedef struct {
+    spyb_paged_cache cache;
+    spyb_paged_batch batch;
+    const void *q, *k, *v;
+    void   *q_out;
+    int64_t q_stride, k_stride, v_stride, q_out_stride;
+    int32_t in_type, q_out_type, n_head;
+    int32_t rope_mode, rope_dim;
+    float   freq_base, freq_scale;
+    int32_t reserved;
+} spyb_paged_append_desc;
+spyb_status spyb_paged_append(spyb_backend *backend, const spyb_paged_append_desc *desc);
+
+/* Attention of the rows over their sequences' pages, spyb_attention's operation for ragged batches: out = sum_j softmax_j(scale q . k_j) v_j over the positions j of
+ * the row's sequence that are there, not behind the row's own (causal != 0) and, with window > 0 (causal only), less than `window` positions back.
+ * A row that sees nothing is zeros. What is not seen has no influence, infinities and NaN included. Query head h reads K/V head h / (n_head / n_head_kv).
+ * q: fp16 [n_rows][n_head][head_dim]; out: the same layout in out_type SPYB_FP16 or SPYB_FP32 (strides of rows in elements, multiples of 8 (FP32: 4); 16-byte aligned pointers).
+ * scale = 0: 1 / sqrt(head_dim). head_dim 32, 64, 96 or 128. Scores, maxima, sums and accumulators are f32; probabilities are rounded to fp16 in front of
+ * the second product. out must not overlap q or the cache. */
+typedef struct {
+    spyb_paged_cache cache;
+    spyb_paged_batch batch;
+    const void *q;
+    void   *out;
+    int64_t q_stride, out_stride;
+    int32_t n_head, out_type, causal, window;
+    float   scale;
+    int32_t reserved;
+} spyb_paged_attention_desc;
+spyb_status spyb_paged_attention(spyb_backend *backend, const spyb_paged_attention_desc *desc);
+
+/* The next token of every row of logits [n_rows][n_vocab] (row_stride elements apart; SPYB_FP32 or SPYB_FP16): SamplerImpl<Greedy>::sample
+ * (model/include/llm/sampler/greedy.h:20-25) with the usual settings, one of each a row; a NULL array leaves the setting out.
+ *   w_i = exp((logit_i - largest) / temperature), in 64 bits; temperature NULL: 1; not above 0: the largest logit, the lowest index among equals
+ *   top_k   (0 < top_k < n_vocab): the top_k largest logits stay, the lowest indices among equals
+ *   top_p   (< 1): of these, in descending order, those in front of which less than top_p of their sum lies (never fewer than one)
+ *   min_p   (> 0): of these, those with w_i >= min_p
+ *   the token is the first index, ascending, up to which the weights that stayed sum to more than uniform[row] (in [0, 1)) times their sum.
+ * NaN and -inf are never drawn; where there is +inf, only +inf has weight, all the same. ids[row] = -1, probs[row] = 0 where there is nothing to draw.
+ * probs (optional): the token's share of the weights that stayed. n_vocab at most 2^20. uniform NULL reads as zeros. */
+typedef struct {
+    const void *logits;
+    int64_t row_stride;
+    int32_t number_type, n_rows, n_vocab, reserved;
+    const float   *temperature;
+    const int32_t *top_k;
+    const float   *top_p, *min_p, *uniform;
+    int32_t *ids;
+    float   *probs;
+} spyb_sample_desc;
+spyb_status spyb_sample(spyb_backend *backend, const spyb_sample_desc *desc);
+
+/* What the three calls above would answer to a descriptor, and why in `message` (up to `size` bytes with the closing 0; may be NULL with size 0): host
+ * arithmetic only, no GPU needed. */
+spyb_status spyb_paged_append_check(const spyb_paged_append_desc *desc, char *message, int32_t size);
+spyb_status spyb_paged_attention_check(const spyb_paged_attention_desc *desc, char *message, int32_t size);
+spyb_status spyb_sample_check(const spyb_sample_desc *desc, char *message, int32_t size);
+
 /* ---- whole-model path: the graph LLAMAModel::build_graph emits (model/src/llm/model/llama.cpp:86-264)
  * executed as a fixed plan of fused kernels. */
 typedef struct {

@@ -22,6 +22,7 @@ FP32, FP16, Q4_0, Q8_0, Q4_K, Q6_K, INT32 = 0, 1, 2, 8, 12, 14, 26
 OP = dict(Input=0, Nop=1, Dup=2, Copy=3, View=4, Reshape=5, GetRow=8, Transpose=9, Permute=10, Contiguous=11, Silu=13,
           Softmax=17, Add=18, Mul=20, MatMul=23, NormRMS=26, Rope=27)
 NODE_CONSTANT, NODE_IO, NODE_CACHE, NODE_DYNAMIC = 0, 1, 2, 6
+ROPE_NONE, ROPE_PAIRS, ROPE_HALVES = -1, 0, 2
 _BLOCK = {FP32: (1, 4), FP16: (1, 2), INT32: (1, 4), Q4_0: (32, 18), Q8_0: (32, 34), Q4_K: (256, 144), Q6_K: (256, 210)}
 
 
@@ -60,6 +61,32 @@ class ModelInfo(C.Structure):
                 ("kv_bytes_per_token", C.c_uint64)]
 
 
+class PagedCache(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("number_type", C.c_int32), ("n_pages", C.c_int32), ("page_size", C.c_int32), ("n_head_kv", C.c_int32),
+                ("head_dim", C.c_int32), ("reserved", C.c_int32), ("page_stride", C.c_int64), ("token_stride", C.c_int64), ("head_stride", C.c_int64)]
+
+
+class PagedBatch(C.Structure):
+    _fields_ = [("row_start", C.c_void_p), ("n_kv", C.c_void_p), ("page_table", C.c_void_p), ("n_seq", C.c_int32), ("n_rows", C.c_int32), ("max_rows", C.c_int32),
+                ("table_stride", C.c_int32)]
+
+
+class PagedAppendDesc(C.Structure):
+    _fields_ = [("cache", PagedCache), ("batch", PagedBatch), ("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p), ("q_out", C.c_void_p), ("q_stride", C.c_int64),
+                ("k_stride", C.c_int64), ("v_stride", C.c_int64), ("q_out_stride", C.c_int64), ("in_type", C.c_int32), ("q_out_type", C.c_int32), ("n_head", C.c_int32),
+                ("rope_mode", C.c_int32), ("rope_dim", C.c_int32), ("freq_base", C.c_float), ("freq_scale", C.c_float), ("reserved", C.c_int32)]
+
+
+class PagedAttentionDesc(C.Structure):
+    _fields_ = [("cache", PagedCache), ("batch", PagedBatch), ("q", C.c_void_p), ("out", C.c_void_p), ("q_stride", C.c_int64), ("out_stride", C.c_int64), ("n_head", C.c_int32),
+                ("out_type", C.c_int32), ("causal", C.c_int32), ("window", C.c_int32), ("scale", C.c_float), ("reserved", C.c_int32)]
+
+
+class SampleDesc(C.Structure):
+    _fields_ = [("logits", C.c_void_p), ("row_stride", C.c_int64), ("number_type", C.c_int32), ("n_rows", C.c_int32), ("n_vocab", C.c_int32), ("reserved", C.c_int32),
+                ("temperature", C.c_void_p), ("top_k", C.c_void_p), ("top_p", C.c_void_p), ("min_p", C.c_void_p), ("uniform", C.c_void_p), ("ids", C.c_void_p), ("probs", C.c_void_p)]
+
+
 CALLBACK = C.CFUNCTYPE(None, C.c_void_p)
 
 _lib = None
@@ -93,6 +120,12 @@ def lib():
         "spyb_block_dots": (i32, [vp, i32, vp, vp, i64, vp]),
         "spyb_read_tables": (i32, [vp, vp, vp]),
         "spyb_attention": (i32, [vp, vp, vp, vp, vp, i32, i32, i32, i32, i32, i32]),
+        "spyb_paged_append": (i32, [vp, C.POINTER(PagedAppendDesc)]),
+        "spyb_paged_attention": (i32, [vp, C.POINTER(PagedAttentionDesc)]),
+        "spyb_sample": (i32, [vp, C.POINTER(SampleDesc)]),
+        "spyb_paged_append_check": (i32, [C.POINTER(PagedAppendDesc), C.c_char_p, i32]),
+        "spyb_paged_attention_check": (i32, [C.POINTER(PagedAttentionDesc), C.c_char_p, i32]),
+        "spyb_sample_check": (i32, [C.POINTER(SampleDesc), C.c_char_p, i32]),
         "spyb_model_read_activation": (i32, [vp, i32, vp, u64]),
         "spyb_model_bench_kernel": (C.c_float, [vp, i32, i32, C.POINTER(u64)]),
         "spyb_model_load_gguf": (i32, [vp, C.c_char_p, i32, C.POINTER(vp)]),
@@ -165,6 +198,52 @@ def make_tensor(data_ptr, number_type: int, ne, nb=None, node_type: int = NODE_D
     return t
 
 
+def paged_cache(k_ptr, v_ptr, n_pages: int, page_size: int, n_head_kv: int, head_dim: int, token_major: bool = False, strides=None) -> PagedCache:
+    """fp16 keys and values in pages: [page][head][position][element], or [page][position][head][element] (token_major), or with the given strides
+    (page, position, head) in elements."""
+    c = PagedCache(k_ptr, v_ptr, FP16, n_pages, page_size, n_head_kv, head_dim, 0)
+    if strides is None:
+        strides = (page_size * n_head_kv * head_dim, n_head_kv * head_dim, head_dim) if token_major else (page_size * n_head_kv * head_dim, head_dim, page_size * head_dim)
+    c.page_stride, c.token_stride, c.head_stride = strides
+    return c
+
+
+def paged_batch(row_start_ptr, n_kv_ptr, page_table_ptr, n_seq: int, n_rows: int, table_stride: int, max_rows: int = 0) -> PagedBatch:
+    """Which rows are whose: int32 device arrays row_start [n_seq + 1], n_kv [n_seq], page_table [n_seq][table_stride]; max_rows: most rows of one sequence (0: unknown)."""
+    return PagedBatch(row_start_ptr, n_kv_ptr, page_table_ptr, n_seq, n_rows, max_rows, table_stride)
+
+
+def paged_append_desc(cache: PagedCache, batch: PagedBatch, q, k, v, q_out, n_head: int, in_type: int = FP32, q_out_type: int = FP16, row_stride=None, q_out_stride=None,
+                      rope_mode: int = ROPE_PAIRS, rope_dim=None, freq_base: float = 10000.0, freq_scale: float = 1.0) -> PagedAppendDesc:
+    """q, k, v: device pointers to rows of heads, `row_stride` elements apart (one for all three, or three of them; None: each its own width). q = q_out = None and
+    n_head = 0: keys and values only."""
+    hd, kv = cache.head_dim, cache.n_head_kv * cache.head_dim
+    qs, ks, vs = (n_head * hd, kv, kv) if row_stride is None else (row_stride,) * 3 if isinstance(row_stride, int) else row_stride
+    return PagedAppendDesc(cache, batch, q, k, v, q_out, qs, ks, vs, n_head * hd if q_out_stride is None else q_out_stride, in_type, q_out_type, n_head, rope_mode,
+                           hd if rope_dim is None else rope_dim, freq_base, freq_scale, 0)
+
+
+def paged_attention_desc(cache: PagedCache, batch: PagedBatch, q, out, n_head: int, out_type: int = FP16, causal: bool = True, window: int = 0, scale: float = 0.0,
+                         q_stride=None, out_stride=None) -> PagedAttentionDesc:
+    """q: fp16 [rows][n_head][head_dim]; out: the same layout in out_type; window: positions that a row sees at most (0: all); scale 0: 1 / sqrt(head_dim)."""
+    width = n_head * cache.head_dim
+    return PagedAttentionDesc(cache, batch, q, out, width if q_stride is None else q_stride, width if out_stride is None else out_stride, n_head, out_type, int(causal), window,
+                              scale, 0)
+
+
+def sample_desc(logits, number_type: int, n_rows: int, n_vocab: int, ids, uniform=None, temperature=None, top_k=None, top_p=None, min_p=None, probs=None,
+                row_stride=None) -> SampleDesc:
+    """logits [n_rows][n_vocab]; settings and uniform numbers: device arrays with one value a row, None leaves a setting out; ids int32, probs f32 (optional)."""
+    return SampleDesc(logits, n_vocab if row_stride is None else row_stride, number_type, n_rows, n_vocab, 0, temperature, top_k, top_p, min_p, uniform, ids, probs)
+
+
+def refusal(desc) -> str:
+    """Why paged_append, paged_attention or sample would not take this descriptor ("" if they would); no GPU needed."""
+    check = {PagedAppendDesc: lib().spyb_paged_append_check, PagedAttentionDesc: lib().spyb_paged_attention_check, SampleDesc: lib().spyb_sample_check}[type(desc)]
+    buf = C.create_string_buffer(256)
+    return "" if check(C.byref(desc), buf, len(buf)) == SUCCESS else buf.value.decode()
+
+
 def prefill_plan(weight_type: int, n_rows: int, k: int, n_cols: int, form=(0, 0, 0), n_sms: int = 148) -> tuple:
     """The form of the prompt GEMM for these sizes (no GPU needed): tokens a tile, CTAs a tile, last tiles whole (1) or shared (2). What is zero of
     `form` is by the sizes."""
@@ -181,6 +260,7 @@ class B200Backend:
                  use_graph: bool = True, arena_bytes: int = 0):
         self._l = lib()
         self._submit = self._l.spyb_submit
+        self._paged_append, self._paged_attention, self._sample = self._l.spyb_paged_append, self._l.spyb_paged_attention, self._l.spyb_sample
         cfg = Config(device_id, tp_size, tp_rank, int(use_pdl), int(use_graph), 0, arena_bytes)
         h = C.c_void_p()
         st = self._l.spyb_create(C.byref(cfg), C.byref(h))
@@ -253,6 +333,25 @@ class B200Backend:
             cb = CALLBACK(lambda _user: callback())
             self._callbacks.append(cb)   # keep alive until it has fired
         st = self._submit(self.h, C.byref(desc), cb, None)
+        if st != SUCCESS:
+            self._check(st)
+
+    # --- steps over many sequences: pages, attention over them, sampling (enqueued on the backend's stream, as submit; sync() waits)
+    def paged_append(self, desc: PagedAppendDesc) -> None:
+        """Rotates the rows' Q and K to their positions and stores K and V in their sequences' pages."""
+        st = self._paged_append(self.h, C.byref(desc))
+        if st != SUCCESS:
+            self._check(st)
+
+    def paged_attention(self, desc: PagedAttentionDesc) -> None:
+        """Attention of the rows over their sequences' pages."""
+        st = self._paged_attention(self.h, C.byref(desc))
+        if st != SUCCESS:
+            self._check(st)
+
+    def sample(self, desc: SampleDesc) -> None:
+        """The next token of every row of logits."""
+        st = self._sample(self.h, C.byref(desc))
         if st != SUCCESS:
             self._check(st)
 

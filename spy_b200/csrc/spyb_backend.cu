@@ -8,6 +8,7 @@
 
 #include "spyb_common.cuh"
 #include "spyb_internal.h"
+#include "spyb_paged.cuh"
 
 namespace spyb {
 
@@ -166,7 +167,9 @@ int32_t spyb_selftest_host(void) {
     const int ledger = smem_ledger_selftest();
     if (ledger != 0) { return ledger; }
     const int ring = attn_ring_selftest();
-    return ring != 0 ? ring : prefill_share_selftest();
+    if (ring != 0) { return ring; }
+    const int share = prefill_share_selftest();
+    return share != 0 ? share : paged_cut_selftest();
 }
 
 spyb_status spyb_create(const spyb_config *config, spyb_backend **out) {
@@ -235,6 +238,7 @@ void spyb_destroy(spyb_backend *be) {
     }
     for (void *p : be->owned) { cudaFree(p); }
     if (be->pf_handoff) { cudaFree(be->pf_handoff); }
+    if (be->paged_partial) { cudaFree(be->paged_partial); }
     if (be->d_silu_table) { cudaFree(be->d_silu_table); }
     if (be->d_exp_table) { cudaFree(be->d_exp_table); }
     if (be->h_error_flag) { cudaFreeHost(be->h_error_flag); }
@@ -856,11 +860,6 @@ bool pack_mask(const spyb_tensor &scores, const spyb_tensor &mask, MaskBits *out
         }
     }
     return other == 0;
-}
-
-void use_device(int device) {   // (most calls find it current)
-    int cur = -1;
-    if (cudaGetDevice(&cur) != cudaSuccess || cur != device) { cudaSetDevice(device); }
 }
 
 }  // namespace

@@ -65,6 +65,29 @@ inline cudaError_t upload(void *dst, const void *src, size_t bytes) {
     return err != cudaSuccess ? err : cudaStreamSynchronize(cudaStreamLegacy);
 }
 
+inline void use_device(int device) {   // (most calls find it current)
+    int cur = -1;
+    if (cudaGetDevice(&cur) != cudaSuccess || cur != device) { cudaSetDevice(device); }
+}
+
+// Why a descriptor is not taken: checks that need no backend
+struct Refusal {
+    char text[256] = "";
+    spyb_status because(const char *fmt, ...) {
+        va_list ap; va_start(ap, fmt); vsnprintf(text, sizeof(text), fmt, ap); va_end(ap);
+        return SPYB_UNSUPPORTED;
+    }
+    spyb_status answer(spyb_status st, char *message, int32_t size) const {
+        if (message != nullptr && size > 0) { snprintf(message, (size_t)size, "%s", st == SPYB_SUCCESS ? "" : text); }
+        return st;
+    }
+};
+inline bool aligned_to(const void *p, uintptr_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
+inline bool value_type(int t) { return t == SPYB_FP32 || t == SPYB_FP16; }
+
+// Shares of a circle by which the pairs of a head turn a position, of the setting that spyb_paged_append was asked for last.
+struct PagedTurns { float base = 0.f, scale = 0.f; int rot = 0; double turns[128] = {}; };
+
 }  // namespace spyb
 
 struct spyb_backend {
@@ -81,6 +104,9 @@ struct spyb_backend {
     int         *h_error_flag = nullptr;   // mapped pinned word the kernels set when a bounded wait runs out
     int         *d_error_flag = nullptr;   // its device address
     void        *pf_handoff = nullptr;     // prompt GEMMs, one after the other on the stream: PrefillGemm::handoff, and behind it the flags
+    float       *paged_partial = nullptr;  // paged attention, one call after the other on the stream: what the CTAs of a cut item found (made at first use),
+    unsigned    *paged_arrived = nullptr;  // and how many of them are done, by their first CTA; zero between launches
+    spyb::PagedTurns paged_turns;
     uint8_t     *noalloc_scratch = nullptr; // device address of the scratch array of spyb_matmul_noalloc (looked up once)
     float       *d_silu_table = nullptr;   // 65536 entries: xh / (1 + expf(-xh)) for the fp16 value xh
     float       *d_exp_table = nullptr;    // 65536 entries: expf(xh)
@@ -136,6 +162,17 @@ struct spyb_backend {
     void prefill_shared(spyb::PrefillGemm &g) const {   // what every prompt GEMM on this backend's stream has in common
         g.error_flag = d_error_flag; g.wait_limit_ns = wait_limit_ns;
         g.handoff = pf_handoff; g.handoff_flags = handoff_flags();
+    }
+    // room for two pieces of 256 rows x 128 elements (with their maxima and sums) of every SM; the small kernel's pieces are less
+    bool paged_workspace() {
+        if (paged_arrived != nullptr) { return true; }
+        const size_t piece = 256 * (128 + 2) * sizeof(float), words = 4 * (size_t)num_sms_total;
+        void *raw = nullptr;
+        if (cudaMalloc(&raw, 2 * num_sms_total * piece + words * sizeof(unsigned)) != cudaSuccess) { cudaGetLastError(); set_error("paged_attention: out of device memory for its workspace"); return false; }
+        unsigned *arrived = reinterpret_cast<unsigned *>(static_cast<uint8_t *>(raw) + 2 * num_sms_total * piece);
+        if (cudaMemsetAsync(arrived, 0, words * sizeof(unsigned), stream) != cudaSuccess) { cudaGetLastError(); cudaFree(raw); set_error("paged_attention: its workspace cannot be cleared"); return false; }
+        paged_partial = static_cast<float *>(raw); paged_arrived = arrived;
+        return true;
     }
     spyb::LaunchCfg launch_cfg(bool pdl) const {
         spyb::LaunchCfg c; c.stream = stream; c.pdl = pdl; c.num_sms = num_sms; c.mv_ctas_per_sm = mv_ctas_per_sm;

@@ -1,0 +1,166 @@
+// What the kernels over paged caches share: parameters, how a call's work is cut among its CTAs, and the joining of what several CTAs found for one tile of rows.
+#pragma once
+
+#include "spyb_common.cuh"
+#include "spyb_kernels.h"
+
+namespace spyb {
+
+struct PagedView {                        // a spyb_paged_cache and a spyb_paged_batch as the kernels read them
+    const int32_t *row_start = nullptr, *n_kv = nullptr, *page_table = nullptr;
+    int            n_seq = 0, n_rows = 0, table_stride = 0, n_pages = 0, page_size = 1;
+    int            n_kv_most = 0;         // positions that a row of the table can name
+    int64_t        page_stride = 0, token_stride = 0, head_stride = 0;
+};
+struct PagedAppend {
+    PagedView    view;
+    const void  *q = nullptr, *k = nullptr, *v = nullptr;
+    void        *q_out = nullptr;
+    __half      *k_cache = nullptr, *v_cache = nullptr;
+    int64_t      q_stride = 0, k_stride = 0, v_stride = 0, q_out_stride = 0;
+    int          n_head = 0, n_head_kv = 0, head_dim = 0, rot = 0, halves = 0;
+    double       turns[128] = {};         // pair i turns by this share of a full circle a position
+};
+struct PagedAttention {
+    PagedView    view;
+    const __half *q = nullptr, *k = nullptr, *v = nullptr;
+    void        *out = nullptr;
+    int64_t      q_stride = 0, out_stride = 0;
+    int          n_head_kv = 0, group = 1, causal = 1, window = 0, out_f32 = 0;
+    float        scale_log2 = 0.f;        // scale * log2(e): probabilities are powers of two
+    int          few_rows = 0;            // sequences of up to so many rows (of all query heads of a K/V head) are the small kernel's
+    float       *partial = nullptr;       // [CTAs][2][rows of a tile][head_dim + 2]
+    unsigned    *arrived = nullptr;       // [CTAs], zero between launches
+};
+int         paged_cut_selftest();   // host-only: 0 when the CTAs' pieces cover every item once, on any lengths
+cudaError_t launch_paged_append(const PagedAppend &p, int in_type, int q_out_type, const LaunchCfg &cfg);
+cudaError_t launch_paged_attention_rows(const PagedAttention &p, int head_dim, int row_tiles, int sms, const LaunchCfg &cfg);
+constexpr int PA_MAX_CTAS_PER_SM = 2;
+
+// ---------------------------------------------------------------------------------------------- cutting the work
+// The rows of a sequence that share a K/V head - token by token, its query heads side by side - are cut into tiles; a tile and a K/V head are an item, and the
+// positions that its rows see are counted in units of UNIT. All units of a call, item after item, are cut evenly among the CTAs: whatever the
+// lengths are, every SM has the same to read, and one long sequence uses the whole chip. An item on a cut is joined by the CTA that is done with it last.
+struct PagedSeq { int row0, rows, first, kv; };   // first row and number of rows, position of the first row, positions that are there
+struct PagedItem { int lo, hi, units; };          // positions [lo, hi) that some row of the tile sees (lo a multiple of ALIGN)
+
+__host__ __device__ __forceinline__ int pmin(int a, int b) { return a < b ? a : b; }
+__host__ __device__ __forceinline__ int pmax(int a, int b) { return a < b ? b : a; }
+__host__ __device__ __forceinline__ PagedSeq paged_seq(const PagedView &v, int s) {
+    const int a = pmax(0, pmin(v.row_start[s], v.n_rows)), end = pmax(a, pmin(v.row_start[s + 1], 1 << 24)), b = pmin(end, v.n_rows);
+    const int kv = pmin(pmax(0, v.n_kv[s]), 1 << 30);
+    return {a, b - a, kv - (end - a), pmin(kv, v.n_kv_most)};
+}
+template <int TILE, int UNIT, int ALIGN>
+__host__ __device__ __forceinline__ PagedItem paged_item(const PagedAttention &p, const PagedSeq &q, int tile) {
+    const int last = pmin(q.rows * p.group, (tile + 1) * TILE) - 1;
+    const int i0 = (int)((unsigned)(tile * TILE) / (unsigned)p.group), i1 = (int)((unsigned)last / (unsigned)p.group);
+    PagedItem t;
+    t.hi = p.causal ? pmin(q.kv, q.first + i1 + 1) : q.kv;
+    t.lo = p.causal && p.window > 0 ? pmax(0, q.first + i0 - p.window + 1) / ALIGN * ALIGN : 0;
+    t.units = pmax(1, (t.hi - t.lo + UNIT - 1) / UNIT);   // (an item without positions still has its zeros to write)
+    return t;
+}
+__host__ __device__ __forceinline__ bool paged_mine(const PagedAttention &p, const PagedSeq &q, bool few) {
+    return q.rows > 0 && ((int64_t)q.rows * p.group <= p.few_rows) == few;
+}
+template <int TILE, int UNIT, int ALIGN>
+__host__ __device__ __forceinline__ int64_t paged_seq_units(const PagedAttention &p, int s, bool few) {   // of one K/V head
+    const PagedSeq q = paged_seq(p.view, s);
+    if (!paged_mine(p, q, few)) { return 0; }
+    const int tiles = (q.rows * p.group + TILE - 1) / TILE;
+    int64_t n = 0;
+    for (int t = 0; t < tiles; ++t) { n += paged_item<TILE, UNIT, ALIGN>(p, q, t).units; }
+    return n;
+}
+
+// unit `rest` of a sequence whose K/V heads have `one` units each
+template <int TILE, int UNIT, int ALIGN>
+__host__ __device__ __forceinline__ void paged_find(const PagedAttention &p, const PagedSeq &q, int64_t one, int64_t rest, int &head, int &tile, int &off) {
+    head = (int)(rest / one); rest -= head * one;
+    for (tile = 0;; ++tile) {
+        const int u = paged_item<TILE, UNIT, ALIGN>(p, q, tile).units;
+        if (rest < u) { break; }
+        rest -= u;
+    }
+    off = (int)rest;
+}
+
+struct PagedPlace { int seq, head, tile, off; int64_t unit, end, total; int ctas; };   // where a CTA begins, its first unit and the one behind its last
+struct PagedPlanShared { int64_t warp[32]; int64_t total; int seq, head, tile, off; };
+__host__ __device__ __forceinline__ int64_t paged_cta_unit(int64_t total, int ctas, int c) { return total * c / ctas; }
+__host__ __device__ __forceinline__ int paged_unit_cta(int64_t total, int ctas, int64_t u) { return (int)(((u + 1) * ctas - 1) / total); }
+
+__host__ __device__ __forceinline__ int paged_ctas(int64_t total, int grid, int least) { const int64_t n = total / least; return n < 1 ? 1 : n < grid ? (int)n : grid; }
+
+// all NT threads of the CTA; `least`: units that a CTA takes at least
+template <int NT, int TILE, int UNIT, int ALIGN>
+__device__ PagedPlace paged_plan(const PagedAttention &p, bool few, int least, PagedPlanShared &sh) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    constexpr int NW = NT / 32;
+    int64_t total = 0, mine = 0;
+    for (int base = 0; base < p.view.n_seq; base += NT) {
+        const int s = base + tid;
+        mine = s < p.view.n_seq ? paged_seq_units<TILE, UNIT, ALIGN>(p, s, few) * p.n_head_kv : 0;
+        total += mine;
+    }
+    for (int o = 16; o > 0; o >>= 1) { total += __shfl_xor_sync(0xffffffffu, total, o); }
+    if (lane == 0) { sh.warp[warp] = total; }
+    __syncthreads();
+    total = 0;
+    for (int w = 0; w < NW; ++w) { total += sh.warp[w]; }
+    PagedPlace at;
+    at.total = total;
+    at.ctas = paged_ctas(total, gridDim.x, least);
+    at.unit = at.end = 0; at.seq = at.head = at.tile = at.off = 0;
+    if (total == 0 || (int)blockIdx.x >= at.ctas) { return at; }
+    at.unit = paged_cta_unit(total, at.ctas, blockIdx.x);
+    at.end = paged_cta_unit(total, at.ctas, blockIdx.x + 1);
+    int64_t before = 0;
+    for (int base = 0; base < p.view.n_seq; base += NT) {
+        const int s = base + tid;
+        if (p.view.n_seq > NT) { mine = s < p.view.n_seq ? paged_seq_units<TILE, UNIT, ALIGN>(p, s, few) * p.n_head_kv : 0; }
+        int64_t upto = mine;
+        for (int o = 1; o < 32; o <<= 1) { const int64_t v = __shfl_up_sync(0xffffffffu, upto, o); if (lane >= o) { upto += v; } }
+        __syncthreads();
+        if (lane == 31) { sh.warp[warp] = upto; }
+        __syncthreads();
+        int64_t all = 0;
+        for (int w = 0; w < NW; ++w) { const int64_t v = sh.warp[w]; upto += w < warp ? v : 0; all += v; }
+        const int64_t from = before + upto - mine;
+        if (from <= at.unit && at.unit < from + mine) {
+            sh.seq = s;
+            paged_find<TILE, UNIT, ALIGN>(p, paged_seq(p.view, s), mine / p.n_head_kv, at.unit - from, sh.head, sh.tile, sh.off);
+        }
+        before += all;
+        if (at.unit < before) { break; }   // (the same for all threads)
+    }
+    __syncthreads();
+    at.seq = sh.seq; at.head = sh.head; at.tile = sh.tile; at.off = sh.off;
+    return at;
+}
+
+// The item behind an item, the same for all threads; false behind the last one.
+template <int TILE>
+__host__ __device__ __forceinline__ bool paged_next(const PagedAttention &p, bool few, PagedSeq &q, int &seq, int &head, int &tile) {
+    if ((++tile) * TILE < q.rows * p.group) { return true; }
+    tile = 0;
+    if (++head < p.n_head_kv) { return true; }
+    head = 0;
+    while (++seq < p.view.n_seq) {
+        q = paged_seq(p.view, seq);
+        if (paged_mine(p, q, few)) { return true; }
+    }
+    return false;
+}
+
+// An item on a cut: its CTAs c0 .. c0 + parts - 1 leave what they found, and who is last joins it in their order. The first one's piece is the last of its own
+// stretch (place 1), every other one's the first of its own (place 0).
+struct PagedCut { int c0, parts; };
+__host__ __device__ __forceinline__ PagedCut paged_cut(const PagedPlace &at, int64_t item_begin, int units) {
+    const int a = paged_unit_cta(at.total, at.ctas, item_begin), b = paged_unit_cta(at.total, at.ctas, item_begin + units - 1);
+    return {a, b - a + 1};
+}
+__host__ __device__ __forceinline__ int64_t paged_slot(int c, int c0) { return 2 * (int64_t)c + (c == c0 ? 1 : 0); }
+
+}  // namespace spyb

@@ -1,0 +1,539 @@
+// The next token of every row of logits: temperature, top-k, top-p and min-p, drawn by a given uniform number.
+
+#include <algorithm>
+#include <cmath>
+
+#include <math_constants.h>
+
+#include "spyb_common.cuh"
+#include "spyb_internal.h"
+
+namespace spyb {
+namespace {
+
+// A cluster of CTAs has a row, each a slice of it in shared memory: the logits are read once. Which token a number falls on must not depend on how sums
+// are rounded, so weights are integers: w = round(2^S exp((x - largest) / T)), S = 45 for up to 2^17 tokens. Their sums are exact in any order, a histogram's
+// too, and a weight's error of 2^-46 moves a border of the sums by about 2^-37 at most. An exponential to 2^-50 costs 13 operations in 64 bits (64
+// a clock and SM), so it is taken where it is needed only:
+//   greedy            none
+//   top-k             a histogram of the logits' distances from the largest (counts) finds the few candidates; one CTA sorts them and does the rest
+//   top-p alone       the counts bracket the bin in which top_p is reached (a bin is 0.0156 wide, its weights are known to 0.8 %); one pass of
+//                     weights gives the sums around the bracket and a second histogram inside it, and the elements of its one bin are sorted
+//   draw              one pass of the weights that stayed; the warp on whose stretch the number falls walks it again
+// Candidates that do not fit a list (ties by the thousand, a top_k of thousands) take a binary search over (logit, index): slow, and as right.
+constexpr int SA_THREADS = 512, SA_WARPS = SA_THREADS / 32, SA_BINS = 2048, SA_LIST = 1024, SA_MAX_CLUSTER = 8;
+constexpr int SA_INDEX_BITS = 20;
+constexpr size_t SA_MAX_SLICE = 40960;    // logits that a CTA keeps in shared memory; longer slices are read again in every pass
+
+struct SampleParams {
+    const void    *logits;
+    int64_t        row_stride;
+    int            n_vocab, per, cached, frac_bits;   // per: logits of a slice; cached: kept in shared memory; frac_bits: S
+    const float   *temperature, *top_p, *min_p, *uniform;
+    const int32_t *top_k;
+    int32_t       *ids;
+    float         *probs;
+};
+
+__device__ __forceinline__ uint32_t ordered(float x) { const uint32_t b = __float_as_uint(x + 0.f); return b & 0x80000000u ? ~b : b | 0x80000000u; }   // (-0 and 0 are equals)
+__device__ __forceinline__ float unordered(uint32_t u) { return __uint_as_float(u & 0x80000000u ? u & 0x7fffffffu : ~u); }
+__device__ __forceinline__ uint64_t key_of(float x, int i) { return ((uint64_t)ordered(x) << SA_INDEX_BITS) | (uint32_t)((1 << SA_INDEX_BITS) - 1 - i); }   // descending: largest first, ties by index
+__device__ __forceinline__ int   index_of(uint64_t key) { return (1 << SA_INDEX_BITS) - 1 - (int)(key & ((1 << SA_INDEX_BITS) - 1)); }
+__device__ __forceinline__ float value_of(uint64_t key) { return unordered((uint32_t)(key >> SA_INDEX_BITS)); }
+__device__ __forceinline__ float as_float(float x) { return x; }
+__device__ __forceinline__ float as_float(__half x) { return __half2float(x); }
+
+__device__ __forceinline__ uint32_t rank_in_cluster() { uint32_t r; asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r)); return r; }
+__device__ __forceinline__ uint32_t cluster_ctas() { uint32_t r; asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r)); return r; }
+__device__ __forceinline__ uint4 cluster_load128(uint32_t addr) {
+    uint4 v;
+    asm volatile("ld.shared::cluster.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+    return v;
+}
+__device__ __forceinline__ uint32_t cluster_add(uint32_t addr, uint32_t n) {
+    uint32_t v;
+    asm volatile("atom.relaxed.cluster.shared::cluster.add.u32 %0, [%1], %2;" : "=r"(v) : "r"(addr), "r"(n) : "memory");
+    return v;
+}
+__device__ __forceinline__ uint64_t warp_sum64(uint64_t v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) { v += __shfl_xor_sync(0xffffffffu, v, o); }
+    return v;
+}
+__device__ __forceinline__ uint64_t warp_upto64(uint64_t v) {   // inclusive sums over the lanes
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) { const uint64_t u = __shfl_up_sync(0xffffffffu, v, o); if (lane >= o) { v += u; } }
+    return v;
+}
+
+struct SampleShared {
+    uint32_t count[SA_BINS];
+    uint32_t limb[3][SA_BINS];               // sums of weights in pieces of 15, 15 and the rest of their bits (up to 2^17 weights a CTA)
+    uint64_t list[SA_LIST];                  // the first CTA's: candidates
+    uint64_t scan[SA_WARPS];
+    uint64_t share[2][SA_MAX_CLUSTER];       // what every CTA of the cluster tells all others
+    uint64_t share2[SA_MAX_CLUSTER];
+    uint64_t cut, total;
+    double   table[32];                      // 2^(i / 32)
+    uint32_t n_list;
+    int      found, found2;
+};
+
+// the weight of a logit as an integer; `c` = log2(e) / T
+struct Weight {
+    const double *table;
+    double c, largest;
+    int    bits;
+    __device__ __forceinline__ uint64_t operator()(float x) const {
+        const double z = ((double)x - largest) * c;
+        if (!(z >= -(double)(bits + 1))) { return 0; }                                   // (-inf too)
+        const double magic = 6755399441055744.0;                                         // 1.5 x 2^52: the sum's low bits are the rounded integer
+        const double t = fma(z, 32.0, magic);
+        const int    k = __double2loint(t);
+        const double f = fma(t - magic, -1.0 / 32, z);                                   // |f| <= 1/64: the series of 2^f to the fifth term leaves 2e-15
+        double e = 1.3333558146428443e-3;
+        e = fma(e, f, 9.618129107628477e-3);
+        e = fma(e, f, 5.550410866482158e-2);
+        e = fma(e, f, 2.402265069591007e-1);
+        e = fma(e, f, 6.931471805599453e-1);
+        e = fma(e, f, 1.0);
+        e *= table[k & 31];
+        e = __hiloint2double(__double2hiint(e) + (((k >> 5) + bits) << 20), __double2loint(e));
+        return (uint64_t)(__double_as_longlong(e + 4503599627370496.0) & 0xfffffffffffffll);   // + 2^52: rounded to an integer (w < 2^51)
+    }
+};
+
+template <class T> struct Slice {
+    const T     *row;       // of the slice's first logit
+    const float *kept;      // in shared memory, or null
+    int          n, base;
+    bool         inf;       // the largest is +inf: 0 there, -inf elsewhere
+    __device__ __forceinline__ float operator()(int i) const {
+        float x;
+        if (kept != nullptr) { x = kept[i]; }
+        else { x = as_float(row[i]); x = x == x ? x : -CUDART_INF_F; }
+        return inf ? (x == CUDART_INF_F ? 0.f : -CUDART_INF_F) : x;
+    }
+};
+
+// inclusive sums over all threads in their order; *all: of all
+__device__ __forceinline__ uint64_t block_upto(uint64_t v, uint64_t *scan, uint64_t *all) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    uint64_t upto = warp_upto64(v);
+    __syncthreads();
+    if (lane == 31) { scan[warp] = upto; }
+    __syncthreads();
+    uint64_t sum = 0;
+#pragma unroll
+    for (int w = 0; w < SA_WARPS; ++w) { const uint64_t u = scan[w]; upto += w < warp ? u : 0; sum += u; }
+    *all = sum;
+    return upto;
+}
+// v of every CTA to all of the cluster (thread 0's counts), summed after the barrier
+__device__ __forceinline__ uint64_t cluster_total(uint64_t v, uint64_t *slots, uint32_t ctas, uint32_t rank) {
+    if (threadIdx.x < ctas) { cluster_store64(cluster_map(smem_u32(slots + rank), threadIdx.x), v); }
+    cluster_sync();
+    uint64_t sum = 0;
+    for (uint32_t i = 0; i < ctas; ++i) { sum += slots[i]; }
+    return sum;
+}
+// a list of up to SA_LIST keys, the largest first
+__device__ void sort_list(uint64_t *a, int n) {
+    int size = 32;
+    while (size < n) { size <<= 1; }
+    for (int i = n + threadIdx.x; i < size; i += SA_THREADS) { a[i] = 0; }
+    for (int k = 2; k <= size; k <<= 1) {
+        for (int j = k >> 1; j > 0; j >>= 1) {
+            __syncthreads();
+            for (int t = threadIdx.x; t < size / 2; t += SA_THREADS) {
+                const int i = 2 * t - (t & (j - 1)), l = i + j;
+                const uint64_t x = a[i], y = a[l];
+                if ((x < y) == ((i & k) == 0)) { a[i] = y; a[l] = x; }
+            }
+        }
+    }
+    __syncthreads();
+}
+
+template <class T>
+__global__ void __launch_bounds__(SA_THREADS) sample_kernel(const __grid_constant__ SampleParams p) {
+    extern __shared__ __align__(16) uint8_t dynamic[];
+    SampleShared &sh = *reinterpret_cast<SampleShared *>(dynamic);
+    float *slice = reinterpret_cast<float *>(dynamic + sizeof(SampleShared));
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const uint32_t rank = rank_in_cluster(), ctas = cluster_ctas();
+    const int row = blockIdx.x / ctas;
+    pdl_launch_dependents();
+    for (int i = tid; i < SA_BINS; i += SA_THREADS) { sh.count[i] = sh.limb[0][i] = sh.limb[1][i] = sh.limb[2][i] = 0; }
+    if (tid < 32) { sh.table[tid] = exp2((double)tid / 32); }
+    if (tid == 0) { sh.n_list = 0; sh.cut = 0; sh.found = sh.found2 = 0; }
+    asm volatile("barrier.cluster.arrive.release;" ::: "memory");   // (waited for in front of the first access to another CTA's memory)
+    pdl_wait();
+
+    Slice<T> x;
+    x.base = (int)rank * p.per;
+    x.n = max(0, min(p.per, p.n_vocab - x.base));
+    x.row = static_cast<const T *>(p.logits) + row * p.row_stride + x.base;
+    x.kept = p.cached ? slice : nullptr;
+    x.inf = false;
+    const float temp = p.temperature ? p.temperature[row] : 1.f, top_p = p.top_p ? p.top_p[row] : 1.f;
+    const float min_p = p.min_p ? p.min_p[row] : 0.f, uni = p.uniform ? p.uniform[row] : 0.f;
+    const int   top_k = p.top_k ? p.top_k[row] : 0;
+
+    // the slice, and its largest
+    uint64_t best = 0;
+    {
+        float m = -CUDART_INF_F;
+        int   at = -1;
+        auto take = [&](float v, int i) {
+            v = v == v ? v : -CUDART_INF_F;
+            if (p.cached) { slice[i] = v; }
+            if (v > m) { m = v; at = i; }
+        };
+        constexpr int VEC = 16 / sizeof(T);
+        if ((reinterpret_cast<uintptr_t>(x.row) & 15) == 0) {
+            const uint4 *src = reinterpret_cast<const uint4 *>(x.row);
+            const int n_vec = x.n / VEC;
+#pragma unroll 4
+            for (int i = tid; i < n_vec; i += SA_THREADS) {
+                const uint4 raw = __ldcs(src + i);
+                const T *v = reinterpret_cast<const T *>(&raw);
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) { take(as_float(v[e]), i * VEC + e); }
+            }
+            for (int i = n_vec * VEC + tid; i < x.n; i += SA_THREADS) { take(as_float(x.row[i]), i); }
+        } else {
+#pragma unroll 4
+            for (int i = tid; i < x.n; i += SA_THREADS) { take(as_float(x.row[i]), i); }
+        }
+        if (at >= 0) { best = key_of(m, x.base + at); }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) { best = max(best, __shfl_xor_sync(0xffffffffu, best, o)); }
+        if (lane == 0) { sh.scan[warp] = best; }
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < SA_WARPS; ++w) { best = max(best, sh.scan[w]); }
+        asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+        if (tid < (int)ctas) { cluster_store64(cluster_map(smem_u32(sh.share[0] + rank), tid), best); }
+        cluster_sync();
+        for (uint32_t i = 0; i < ctas; ++i) { best = max(best, sh.share[0][i]); }
+    }
+    const bool greedy = !(temp > 0.f);
+    if (best == 0 || greedy) {
+        if (rank == 0 && tid == 0) {
+            p.ids[row] = best == 0 ? -1 : index_of(best);
+            if (p.probs) { p.probs[row] = best == 0 ? 0.f : 1.f; }
+        }
+        return;
+    }
+    float largest = value_of(best);
+    if (largest == CUDART_INF_F) { x.inf = true; largest = 0.f; }
+    Weight weight;
+    weight.table = sh.table; weight.bits = p.frac_bits; weight.largest = largest;
+    weight.c = fmin(1.4426950408889634073599 / (double)temp, 1e30);
+    const double one = exp2((double)p.frac_bits);
+    const uint64_t least = min_p > 0.f ? (uint64_t)max(1.0, ceil((double)fminf(min_p, 1.f) * one)) : 1;
+    const float  bin_scale = (float)(weight.c * (SA_BINS / (double)(p.frac_bits + 1)));
+    auto bin_of = [&](float v) { return (largest - v) * bin_scale; };        // not below SA_BINS (or NaN): no weight
+    const bool by_k = top_k > 0 && top_k < p.n_vocab, by_p = top_p < 1.f;
+    auto reach = [&](uint64_t total) { return max((uint64_t)1, (uint64_t)ceil((double)max(top_p, 0.f) * (double)total)); };   // a token stays while less than this is in front of it
+    uint64_t cut = 0;                        // keys from here on stay
+    bool     search = false;                 // ... by the slow way
+
+    // gives the first CTA all elements that `wanted` names; false when they do not fit (all CTAs know)
+    auto gather = [&](auto wanted) {
+        const uint32_t counter = cluster_map(smem_u32(&sh.n_list), 0), list = cluster_map(smem_u32(sh.list), 0);
+        for (int i0 = warp * 32; i0 < x.n; i0 += SA_THREADS) {
+            const int i = i0 + lane;
+            const float v = i < x.n ? x(i) : -CUDART_INF_F;
+            const bool in = i < x.n && wanted(v);
+            const unsigned mask = __ballot_sync(0xffffffffu, in);
+            if (mask == 0) { continue; }
+            uint32_t at = 0;
+            if (lane == 0) { at = cluster_add(counter, __popc(mask)); }
+            at = __shfl_sync(0xffffffffu, at, 0) + __popc(mask & ((1u << lane) - 1));
+            if (in && at < SA_LIST) { cluster_store64(list + at * 8, key_of(v, x.base + i)); }
+        }
+        cluster_sync();
+    };
+    // the sum over all keys from `from` on that are not below `low`
+    auto sum_from = [&](uint64_t from, bool counts, int turn) {
+        uint64_t s = 0;
+        for (int i = tid; i < x.n; i += SA_THREADS) {
+            const float v = x(i);
+            if (v != -CUDART_INF_F && key_of(v, x.base + i) >= from) { s += counts ? 1 : weight(v); }
+        }
+        uint64_t all;
+        block_upto(s, sh.scan, &all);
+        return cluster_total(all, sh.share[turn & 1], ctas, rank);
+    };
+
+    if (by_k || by_p) {
+        __syncthreads();
+        for (int i = tid; i < x.n; i += SA_THREADS) {
+            const float b = bin_of(x(i));
+            if (b < (float)SA_BINS) { atomicAdd(&sh.count[(int)b], 1u); }
+        }
+        cluster_sync();
+        uint4 n4 = make_uint4(0, 0, 0, 0);               // four bins a thread, of the whole row
+        for (uint32_t r = 0; r < ctas; ++r) {
+            const uint4 v = cluster_load128(cluster_map(smem_u32(sh.count) + tid * 16, r));
+            n4.x += v.x; n4.y += v.y; n4.z += v.z; n4.w += v.w;
+        }
+        if (by_k) {
+            uint64_t all;
+            const uint64_t upto = block_upto((uint64_t)n4.x + n4.y + n4.z + n4.w, sh.scan, &all);
+            const uint64_t before = upto - n4.x - n4.y - n4.z - n4.w, want = min((uint64_t)top_k, all);
+            if (before < want && want <= upto) {
+                uint64_t c = before + n4.x; int b = tid * 4;
+                if (c < want) { c += n4.y; ++b; }
+                if (c < want) { c += n4.z; ++b; }
+                if (c < want) { c += n4.w; ++b; }
+                sh.found = b; sh.found2 = (int)min(c, (uint64_t)SA_LIST + 1);
+            }
+            __syncthreads();
+            const int last_bin = sh.found, n = sh.found2;
+            if (n <= SA_LIST) {
+                gather([&](float v) { return bin_of(v) < (float)(last_bin + 1); });
+                if (rank != 0) { return; }
+                // everything else is the first CTA's: sorted, cut from the end, put back into the order of indices, drawn
+                sort_list(sh.list, n);
+                const int n1 = min(n, top_k);
+                uint64_t w0 = 0, w1 = 0, k0 = 0, k1 = 0, all_w;
+                if (2 * tid < n1) { k0 = sh.list[2 * tid]; w0 = weight(value_of(k0)); }
+                if (2 * tid + 1 < n1) { k1 = sh.list[2 * tid + 1]; w1 = weight(value_of(k1)); }
+                const uint64_t up = block_upto(w0 + w1, sh.scan, &all_w);
+                const uint64_t stop = by_p ? reach(all_w) : ~0ull;
+                const bool in0 = 2 * tid < n1 && up - w1 - w0 < stop && w0 >= least, in1 = 2 * tid + 1 < n1 && up - w1 < stop && w1 >= least;
+                uint64_t kept;
+                const uint64_t kept_upto = block_upto((in0 ? 1 : 0) + (in1 ? 1 : 0), sh.scan, &kept);   // (a prefix of the list)
+                (void)kept_upto;
+                uint64_t sum;
+                block_upto((in0 ? w0 : 0) + (in1 ? w1 : 0), sh.scan, &sum);
+                // by index: the key's low bits, ascending as descending complements; the weights are found again from their place in the sorted list
+                uint64_t *by_index = sh.list, *weights = reinterpret_cast<uint64_t *>(sh.limb);
+                __syncthreads();
+                constexpr uint64_t low = (1 << SA_INDEX_BITS) - 1;
+                if (in0) { by_index[2 * tid] = ((k0 & low) << 11 | (2 * tid)) + 1; weights[2 * tid] = w0; }
+                if (in1) { by_index[2 * tid + 1] = ((k1 & low) << 11 | (2 * tid + 1)) + 1; weights[2 * tid + 1] = w1; }
+                sort_list(by_index, (int)kept);
+                uint64_t v0 = 0, v1 = 0, p0 = 0, p1 = 0, ignore;
+                if (2 * tid < (int)kept) { p0 = by_index[2 * tid] - 1; v0 = weights[p0 & 2047]; }
+                if (2 * tid + 1 < (int)kept) { p1 = by_index[2 * tid + 1] - 1; v1 = weights[p1 & 2047]; }
+                const uint64_t upto2 = block_upto(v0 + v1, sh.scan, &ignore);
+                const uint64_t t = min((uint64_t)((double)(uni > 0.f ? uni : 0.f) * (double)sum), sum - 1);
+                const bool hit0 = v0 > 0 && upto2 - v1 - v0 <= t && t < upto2 - v1, hit1 = v1 > 0 && upto2 - v1 <= t && t < upto2;
+                if (hit0 || hit1) {
+                    p.ids[row] = (int)(low - ((hit0 ? p0 : p1) >> 11));
+                    if (p.probs) { p.probs[row] = (float)((double)(hit0 ? v0 : v1) / (double)sum); }
+                }
+                return;
+            }
+            search = true;
+        } else {
+            // what the bins weigh, to 0.8 %: the bins in which top_p may be reached
+            const float step = -(float)(p.frac_bits + 1) / SA_BINS;     // log2 of a weight, a bin
+            const float w[4] = {exp2f(step * (4 * tid + 0.5f)), exp2f(step * (4 * tid + 1.5f)), exp2f(step * (4 * tid + 2.5f)), exp2f(step * (4 * tid + 3.5f))};
+            const uint32_t n[4] = {n4.x, n4.y, n4.z, n4.w};
+            uint64_t m[4], all;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) { m[e] = (uint64_t)((double)w[e] * n[e] * 1099511627776.0); }   // x 2^40
+            const uint64_t upto = block_upto(m[0] + m[1] + m[2] + m[3], sh.scan, &all);
+            const double   goal = (double)max(top_p, 0.f) * (double)all;
+            const uint64_t lo = (uint64_t)(0.98 * goal), hi = min((uint64_t)(1.02 * goal), all);
+            uint64_t c = upto - m[0] - m[1] - m[2] - m[3];
+            if (tid == 0) { sh.found = 0; sh.found2 = SA_BINS - 1; }
+            __syncthreads();
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                if (c < lo && lo <= c + m[e]) { sh.found = 4 * tid + e; }
+                if (c < hi && hi <= c + m[e]) { sh.found2 = min(4 * tid + e + 1, SA_BINS - 1); }
+                c += m[e];
+            }
+            __syncthreads();
+            const int   first = sh.found, last = sh.found2;
+            const float sub_scale = (float)SA_BINS / (float)(last + 1 - first);
+            auto sub_of = [&](float b) { return min(SA_BINS - 1, (int)((b - (float)first) * sub_scale)); };
+            uint64_t front = 0, rest = 0;
+            for (int i = tid; i < x.n; i += SA_THREADS) {
+                const float v = x(i), b = bin_of(v);
+                const uint64_t ww = weight(v);
+                if (b < (float)first) { front += ww; }
+                else if (b < (float)(last + 1)) {
+                    const int s = sub_of(b);
+                    rest += ww;
+                    atomicAdd(&sh.limb[0][s], (uint32_t)(ww & 0x7fff));
+                    atomicAdd(&sh.limb[1][s], (uint32_t)(ww >> 15) & 0x7fff);
+                    if (ww >> 30) { atomicAdd(&sh.limb[2][s], (uint32_t)(ww >> 30)); }
+                } else { rest += ww; }
+            }
+            uint64_t mine, others;
+            block_upto(front, sh.scan, &mine);
+            block_upto(rest, sh.scan, &others);
+            if (tid < (int)ctas) { cluster_store64(cluster_map(smem_u32(sh.share[1] + rank), tid), mine); cluster_store64(cluster_map(smem_u32(sh.share2 + rank), tid), others); }
+            cluster_sync();
+            front = rest = 0;
+            for (uint32_t r = 0; r < ctas; ++r) { front += sh.share[1][r]; rest += sh.share2[r]; }
+            uint64_t q[4] = {0, 0, 0, 0};
+            for (uint32_t r = 0; r < ctas; ++r) {
+                const uint4 a = cluster_load128(cluster_map(smem_u32(sh.limb[0]) + tid * 16, r)), b = cluster_load128(cluster_map(smem_u32(sh.limb[1]) + tid * 16, r)),
+                            d = cluster_load128(cluster_map(smem_u32(sh.limb[2]) + tid * 16, r));
+                q[0] += a.x + ((uint64_t)b.x << 15) + ((uint64_t)d.x << 30); q[1] += a.y + ((uint64_t)b.y << 15) + ((uint64_t)d.y << 30);
+                q[2] += a.z + ((uint64_t)b.z << 15) + ((uint64_t)d.z << 30); q[3] += a.w + ((uint64_t)b.w << 15) + ((uint64_t)d.w << 30);
+            }
+            const uint64_t stop = reach(front + rest);
+            const uint64_t upto_s = block_upto(q[0] + q[1] + q[2] + q[3], sh.scan, &all);
+            if (tid == 0) { sh.found = -1; }
+            __syncthreads();
+            c = front + upto_s - q[0] - q[1] - q[2] - q[3];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                if (c < stop && stop <= c + q[e]) { sh.found = 4 * tid + e; sh.total = c; }
+                c += q[e];
+            }
+            __syncthreads();
+            const int sub = sh.found;
+            if (sub < 0) { search = true; }              // (not reached inside the bracket)
+            else {
+                gather([&](float v) { const float b = bin_of(v); return b >= (float)first && b < (float)(last + 1) && sub_of(b) == sub; });
+                // the first CTA finds the last one that stays and tells all
+                if (rank == 0) {
+                    const int nn = (int)min(sh.n_list, (uint32_t)SA_LIST + 1);
+                    uint64_t found = 0;
+                    if (nn <= SA_LIST) {
+                        sort_list(sh.list, nn);
+                        uint64_t w0 = 0, w1 = 0, ignore;
+                        if (2 * tid < nn) { w0 = weight(value_of(sh.list[2 * tid])); }
+                        if (2 * tid + 1 < nn) { w1 = weight(value_of(sh.list[2 * tid + 1])); }
+                        const uint64_t up = sh.total + block_upto(w0 + w1, sh.scan, &ignore);
+                        uint64_t n_in;
+                        block_upto((2 * tid < nn && up - w1 - w0 < stop ? 1 : 0) + (2 * tid + 1 < nn && up - w1 < stop ? 1 : 0), sh.scan, &n_in);
+                        found = n_in > 0 ? sh.list[n_in - 1] : 0;
+                    }
+                    if (tid < (int)ctas) { cluster_store64(cluster_map(smem_u32(&sh.cut), tid), found); }
+                }
+                cluster_sync();
+                cut = sh.cut;
+                search = cut == 0;
+            }
+        }
+    }
+    if (search) {
+        int turn = 0;
+        cluster_sync();                                   // (nobody reads the shares of an earlier exchange any more)
+        if (by_k) {
+            for (int bit = 31 + SA_INDEX_BITS; bit >= 0; --bit) {
+                if (sum_from(cut | 1ull << bit, true, turn++) >= (uint64_t)top_k) { cut |= 1ull << bit; }
+            }
+        }
+        if (by_p) {
+            const uint64_t floor = cut, stop = reach(sum_from(floor, false, turn++));
+            cut = 0;
+            for (int bit = 31 + SA_INDEX_BITS; bit >= 0; --bit) {
+                if (sum_from(max(floor, cut | (uint64_t)1 << bit), false, turn++) >= stop) { cut |= 1ull << bit; }
+            }
+            cut = max(cut, floor);
+        }
+    }
+
+    // draw: warps have contiguous stretches
+    const int stretch = ((x.n + SA_WARPS - 1) / SA_WARPS + 31) & ~31, from = min(warp * stretch, x.n), to = min(from + stretch, x.n);
+    auto stays = [&](int i, float v) {
+        if (key_of(v, x.base + i) < cut) { return (uint64_t)0; }
+        const uint64_t w = weight(v);
+        return w >= least ? w : (uint64_t)0;
+    };
+    uint64_t s = 0;
+    for (int i = from + lane; i < to; i += 32) { s += stays(i, x(i)); }
+    s = warp_sum64(s);
+    __syncthreads();
+    if (lane == 0) { sh.scan[warp] = s; }
+    __syncthreads();
+    uint64_t mine = 0, before = 0;
+#pragma unroll
+    for (int w = 0; w < SA_WARPS; ++w) { const uint64_t u = sh.scan[w]; before += w < warp ? u : 0; mine += u; }
+    cluster_sync();                                       // (shares of earlier exchanges are read)
+    const uint64_t total = cluster_total(mine, sh.share[0], ctas, rank);
+    for (uint32_t r = 0; r < rank; ++r) { before += sh.share[0][r]; }
+    const uint64_t t = min((uint64_t)((double)(uni > 0.f ? uni : 0.f) * (double)total), total - 1);
+    if (before <= t && t < before + s) {
+        uint64_t c = before;
+        for (int i0 = from; i0 < to; i0 += 32) {
+            const int i = i0 + lane;
+            const uint64_t w = i < to ? stays(i, x(i)) : 0, upto = c + warp_upto64(w);
+            const unsigned hit = __ballot_sync(0xffffffffu, t < upto);
+            if (hit) {
+                if (lane == __ffs(hit) - 1) {
+                    p.ids[row] = x.base + i;
+                    if (p.probs) { p.probs[row] = (float)((double)w / (double)total); }
+                }
+                break;
+            }
+            c = __shfl_sync(0xffffffffu, upto, 31);
+        }
+    }
+}
+
+template <class T>
+cudaError_t launch_sample(SampleParams &p, int n_rows, const LaunchCfg &cfg) {
+    // CTAs of a row: slices of about 4096 logits (8 for 32 000 and more); slices that fit are kept
+    int ctas = 1;
+    while (ctas < SA_MAX_CLUSTER && p.n_vocab > 4096 * ctas) { ctas *= 2; }
+    p.per = ((p.n_vocab + ctas - 1) / ctas + 31) & ~31;
+    p.cached = (size_t)p.per <= SA_MAX_SLICE;
+    const size_t smem = sizeof(SampleShared) + (p.cached ? (size_t)p.per * 4 : 0);
+    const void *kernel = reinterpret_cast<const void *>(sample_kernel<T>);
+    const cudaError_t err = allow_dynamic_smem(kernel, smem);
+    if (err != cudaSuccess) { return err; }
+    cudaLaunchConfig_t lc = {};
+    lc.gridDim = dim3((unsigned)n_rows * ctas); lc.blockDim = dim3(SA_THREADS); lc.dynamicSmemBytes = smem; lc.stream = cfg.stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = ctas; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    lc.attrs = attr; lc.numAttrs = cfg.pdl ? 2 : 1;
+    void *args[] = {&p};
+    return cudaLaunchKernelExC(&lc, kernel, args);
+}
+
+}  // namespace
+}  // namespace spyb
+
+using namespace spyb;
+
+static spyb_status check_sample(Refusal &no, const spyb_sample_desc &d) {
+    if (!value_type(d.number_type)) { return no.because("sample: logits of type %d", d.number_type); }
+    if (d.n_rows < 0 || d.n_rows > (1 << 24) || d.n_vocab < 1 || d.n_vocab > (1 << SA_INDEX_BITS) || (d.n_rows > 1 && d.row_stride < d.n_vocab)) {
+        return no.because("sample: %d rows of %d logits, %lld apart", d.n_rows, d.n_vocab, (long long)d.row_stride);
+    }
+    if (d.logits == nullptr || d.ids == nullptr) { return no.because("sample: logits and ids must be there"); }
+    const void *const words[] = {d.temperature, d.top_k, d.top_p, d.min_p, d.uniform, d.ids, d.probs};
+    bool aligned = aligned_to(d.logits, d.number_type == SPYB_FP32 ? 4 : 2);
+    for (const void *w : words) { aligned &= aligned_to(w, 4); }
+    if (!aligned) { return no.because("sample: operands must be aligned to their elements"); }
+    return SPYB_SUCCESS;
+}
+
+extern "C" spyb_status spyb_sample_check(const spyb_sample_desc *d, char *message, int32_t size) {
+    Refusal no;
+    return d == nullptr ? SPYB_FAIL : no.answer(check_sample(no, *d), message, size);
+}
+
+extern "C" spyb_status spyb_sample(spyb_backend *be, const spyb_sample_desc *d) {
+    if (be == nullptr || d == nullptr) { return SPYB_FAIL; }
+    Refusal no;
+    if (check_sample(no, *d) != SPYB_SUCCESS) { be->set_error("%s", no.text); return SPYB_UNSUPPORTED; }
+    if (d->n_rows == 0) { return SPYB_SUCCESS; }
+    use_device(be->config.device_id);
+    SampleParams p;
+    p.logits = d->logits; p.row_stride = d->row_stride; p.n_vocab = d->n_vocab;
+    int log2_vocab = 0;
+    while ((1 << log2_vocab) < d->n_vocab) { ++log2_vocab; }
+    p.frac_bits = std::min(45, 62 - log2_vocab);
+    p.temperature = d->temperature; p.top_k = d->top_k; p.top_p = d->top_p; p.min_p = d->min_p; p.uniform = d->uniform; p.ids = d->ids; p.probs = d->probs;
+    const LaunchCfg cfg = be->launch_cfg(be->config.use_pdl != 0);
+    SPYB_CUDA(be, d->number_type == SPYB_FP32 ? launch_sample<float>(p, d->n_rows, cfg) : launch_sample<__half>(p, d->n_rows, cfg));
+    return SPYB_SUCCESS;
+}

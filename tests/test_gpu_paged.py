@@ -1,0 +1,572 @@
+"""GPU: the operators over paged caches and the sampler against plain numpy in 64 bits.
+
+Tolerances: a rounding is off by half a step at most, relative 2^-11 for fp16 (2^-25 absolutely among its smallest values) and 2^-24 for f32; what follows from it
+is derived where it is used."""
+import numpy as np
+import pytest
+
+from spy_b200 import backend as B
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def be():
+    b = B.B200Backend(0)
+    yield b
+    b.close()
+
+
+class Device:
+    """Arrays on the device that go when the test is over."""
+
+    def __init__(self, be):
+        self.be, self.held = be, []
+
+    def __call__(self, a):
+        a = np.ascontiguousarray(a)
+        p = self.be.upload(a)
+        self.held.append((p, max(1, a.nbytes)))
+        return p
+
+    def back(self, p, like):
+        return self.be.download(p, like.shape, like.dtype)
+
+    def free(self):
+        self.be.sync()
+        for p, n in self.held:
+            self.be.dealloc_memory(p, n)
+
+
+@pytest.fixture
+def dev(be):
+    d = Device(be)
+    yield d
+    d.free()
+
+
+class Pool:
+    """Pages in random order with NaN wherever nothing is stored; `k` and `v`: what each sequence has stored, [position][head][element]."""
+
+    def __init__(self, rng, n_kv, heads, head_dim, page, token_major=False, strides=None, spare=2, fill=np.nan):
+        self.page, self.heads, self.hd, self.n_kv, self.token_major = page, heads, head_dim, list(n_kv), token_major
+        need = [-(-max(0, n) // page) for n in n_kv]
+        self.n_pages = sum(need) + spare
+        order = rng.permutation(self.n_pages)
+        self.table = np.full((len(n_kv), max(1, max(need))), -1, dtype=np.int32)
+        at = 0
+        for s, n in enumerate(need):
+            self.table[s, :n] = order[at:at + n]
+            at += n
+        if strides is None:
+            strides = (page * heads * head_dim, heads * head_dim, head_dim) if token_major else (page * heads * head_dim, head_dim, page * head_dim)
+        self.strides = strides
+        self.size = self.n_pages * strides[0] + (page - 1) * strides[1] + (heads - 1) * strides[2] + head_dim
+        self.k, self.v = (np.full(self.size, fill, dtype=np.float16) for _ in range(2))
+
+    def view(self, a):
+        return np.lib.stride_tricks.as_strided(a, (self.n_pages, self.page, self.heads, self.hd), tuple(2 * s for s in self.strides) + (2,))
+
+    def put(self, s, k, v):
+        pos = np.arange(len(k))
+        for a, x in ((self.k, k), (self.v, v)):
+            self.view(a)[self.table[s, pos // self.page], pos % self.page] = x
+
+    def get(self, a, s, n=None):
+        n = max(0, self.n_kv[s]) if n is None else n
+        pos = np.arange(n)
+        return self.view(a)[self.table[s, pos // self.page], pos % self.page]
+
+    def cache(self, pk, pv):
+        return B.paged_cache(pk, pv, self.n_pages, self.page, self.heads, self.hd, strides=self.strides)
+
+
+def plain_attention(q, k, v, first, scale, causal, window, there):
+    """q [rows][heads][e]; k, v [positions][kv heads][e], f64. Returns out, and per element how far fp16 probabilities and f32 sums may move it."""
+    rows, h, hd = q.shape
+    n, h_kv, _ = k.shape
+    out, off = np.zeros(q.shape), np.zeros(q.shape)
+    for i in range(rows):
+        j = np.arange(n)
+        seen = there.copy()
+        if causal:
+            seen &= j <= first + i
+            if window:
+                seen &= j > first + i - window
+        if not seen.any():
+            continue
+        for x in range(h):
+            kk, vv = k[seen][:, x // (h // h_kv)], v[seen][:, x // (h // h_kv)]
+            t = kk @ q[i, x] * scale
+            w = np.exp(t - t.max())
+            w /= w.sum()
+            out[i, x] = w @ vv
+            with np.errstate(invalid="ignore"):
+                # scores: f32 sums of exact products (head_dim terms), scaled, subtracted, 2^x: relative error of a probability
+                d_score = (hd + 8) * 2.0 ** -24 * (np.abs(kk) @ np.abs(q[i, x])).max() * abs(scale) + 2.0 ** -20
+                # probabilities to fp16, twice (sum and product use the same ones), their smallest absolutely; f32 sums
+                rel = 2 * (2.0 ** -11 + d_score) + (len(w) / 16 + 40) * 2.0 ** -24
+                off[i, x] = rel * (w @ np.abs(vv)) + len(w) * 2.0 ** -24 * np.abs(vv).max()
+    return out, off
+
+
+def run_attention(be, dev, pool, row_start, q, out0, **kw):
+    n_rows, h, hd = q.shape
+    row_start = np.asarray(row_start, dtype=np.int32)
+    c = pool.cache(dev(pool.k), dev(pool.v))
+    b = B.paged_batch(dev(row_start), dev(np.array(pool.n_kv, dtype=np.int32)), dev(pool.table), len(pool.n_kv), n_rows, pool.table.shape[1], kw.pop("max_rows", 0))
+    po = dev(out0)
+    d = B.paged_attention_desc(c, b, dev(q), po, h, out_type=B.FP32 if out0.dtype == np.float32 else B.FP16, **kw)
+    be.paged_attention(d)
+    got = dev.back(po, out0)
+    be.paged_attention(d)                                    # the same bits every time
+    again = dev.back(po, out0)
+    assert np.array_equal(got.view(np.uint8), again.view(np.uint8))
+    return got
+
+
+def check_attention(be, dev, rng, rows, n_kv, h, h_kv, hd, page, causal=True, window=0, scale=0.0, out=np.float16, token_major=False, pad=0, spread=1.0, max_rows=0, drop=None, strides=None):
+    pool = Pool(rng, n_kv, h_kv, hd, page, token_major, strides)
+    for s, n in enumerate(n_kv):
+        pool.put(s, *(rng.standard_normal((2, max(0, n), h_kv, hd)).astype(np.float16)))
+    if drop is not None:
+        pool.table[rng.random(pool.table.shape) < drop] = -1
+        pool.table[rng.random(pool.table.shape) < drop / 2] = pool.n_pages + 5
+    starts = np.concatenate([[0], np.cumsum(rows)])
+    q = (spread * rng.standard_normal((starts[-1] + pad, h, hd))).astype(np.float16)
+    out0 = np.full(q.shape, 7.5, dtype=out)
+    got = run_attention(be, dev, pool, starts, q, out0, causal=causal, window=window, scale=scale, max_rows=max_rows)
+    for s, n in enumerate(n_kv):
+        pos = np.arange(max(0, n))
+        pages = pool.table[s, pos // page]
+        there = (pages >= 0) & (pages < pool.n_pages)
+        safe = np.where(there, pages, 0)
+        k, v = (np.where(there[:, None, None], pool.view(a)[safe, pos % page], 0).astype(np.float64) for a in (pool.k, pool.v))
+        a, b = starts[s], starts[s + 1]
+        want, off = plain_attention(q[a:b].astype(np.float64), k, v, n - rows[s], scale or hd ** -0.5, causal, window, there)
+        tol = off + (np.abs(want) * 2.0 ** -11 + 2.0 ** -25 if out == np.float16 else np.abs(want) * 2.0 ** -24)
+        err = np.abs(got[a:b].astype(np.float64) - want)
+        assert (err <= tol).all(), (s, float((err / np.maximum(tol, 1e-30)).max()), np.unravel_index(np.argmax(err - tol), err.shape))
+        assert (got[a:b][~np.any(off > 0, axis=2)] == 0).all()
+    assert (got[starts[-1]:] == 7.5).all()                   # rows behind the last sequence
+
+
+@pytest.mark.parametrize("hd", [32, 64, 96, 128])
+@pytest.mark.parametrize("h,h_kv", [(4, 4), (6, 2), (5, 1), (8, 1)])
+def test_single_tokens(be, dev, hd, h, h_kv):
+    rng = np.random.default_rng(hd * 100 + h * 10 + h_kv)
+    check_attention(be, dev, rng, [1] * 7, [1, 2, 15, 16, 17, 300, 1031], h, h_kv, hd, 16, pad=2, max_rows=1)
+
+
+@pytest.mark.parametrize("page", [1, 3, 8, 24, 64, 200, 256])
+@pytest.mark.parametrize("token_major", [False, True])
+def test_pages_of_all_sizes(be, dev, page, token_major):
+    rng = np.random.default_rng(page)
+    check_attention(be, dev, rng, [1, 3, 40, 0, 1], [77, 130, 290, 55, 1], 4, 2, 64, page, token_major=token_major)
+    check_attention(be, dev, rng, [140, 2], [333, 64], 4, 1, 128, page, token_major=token_major)
+
+
+@pytest.mark.parametrize("rows,n_kv", [([1], [0]), ([0], [5]), ([3], [2]), ([5, 1, 0, 2], [5, 0, 9, 1]), ([130], [130]), ([129], [500]), ([257], [260]), ([64, 1, 64], [64, 700, 200])])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_short_and_empty(be, dev, rows, n_kv, hd):
+    """No positions at all, more rows than positions (rows without a key are zeros), no rows, whole prompts."""
+    rng = np.random.default_rng(len(rows) + rows[0])
+    check_attention(be, dev, rng, rows, n_kv, 4, 2, hd, 16, pad=3)
+
+
+@pytest.mark.parametrize("window", [1, 2, 17, 64, 128, 129, 1000])
+@pytest.mark.parametrize("rows", [1, 5, 150])
+def test_windows(be, dev, window, rows):
+    rng = np.random.default_rng(window)
+    check_attention(be, dev, rng, [rows, 1, rows], [700, 90, rows], 6, 2, 64, 16, window=window)
+
+
+@pytest.mark.parametrize("hd", [32, 64, 96, 128])
+@pytest.mark.parametrize("rows", [1, 9, 200])
+def test_without_causal_order_and_with_other_scales(be, dev, hd, rows):
+    rng = np.random.default_rng(hd + rows)
+    check_attention(be, dev, rng, [rows, rows], [310, 40], 4, 2, hd, 32, causal=False, scale=0.3)
+    check_attention(be, dev, rng, [rows], [310], 4, 4, hd, 32, scale=-0.1, out=np.float32)
+
+
+@pytest.mark.parametrize("rows", [1, 4, 33, 300])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_f32_outputs_and_sharp_rows(be, dev, rows, hd):
+    rng = np.random.default_rng(rows)
+    check_attention(be, dev, rng, [rows, rows], [900, rows], 8, 2, hd, 16, out=np.float32, spread=6.0)
+
+
+@pytest.mark.parametrize("rows", [1, 6, 160])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_pages_that_are_not_there(be, dev, rows, hd):
+    rng = np.random.default_rng(rows * hd)
+    for drop in (0.3, 0.9, 1.0):
+        check_attention(be, dev, rng, [rows, rows, 1], [400, 170, 333], 4, 2, hd, 16, drop=drop)
+
+
+@pytest.mark.parametrize("rows", [2, 30, 200])
+@pytest.mark.parametrize("hd", [32, 64, 128])
+@pytest.mark.parametrize("value", [np.inf, -np.inf, np.nan])
+def test_values_that_are_not_finite_reach_only_who_sees_them(be, dev, rows, hd, value):
+    """A K or V element of a later position, of one outside the window, behind the sequence's end or in a free page has no influence."""
+    rng = np.random.default_rng(rows + hd)
+    n, h, h_kv, window = 230 + rows, 4, 2, 90
+    pool = Pool(rng, [n], h_kv, hd, 16, fill=value)
+    k, v = rng.standard_normal((2, n, h_kv, hd)).astype(np.float16)
+    bad_v, bad_k, old = n - rows + rows // 2, n - 1, n - rows - window - 3       # seen by the rows behind it in its window, by the last one, by nobody
+    v[bad_v, 0, 5] = value
+    k[bad_k, 1, 3] = value
+    v[old, :, :] = value
+    k[old, :, :] = value
+    pool.put(0, k, v)
+    q = rng.standard_normal((rows, h, hd)).astype(np.float16)
+    got = run_attention(be, dev, pool, [0, rows], q, np.zeros(q.shape, dtype=np.float32), window=window)
+    first = n - rows
+    good_k, good_v = k.astype(np.float64), v.astype(np.float64)
+    for a in (good_k, good_v):
+        a[~np.isfinite(a)] = 0
+    want, off = plain_attention(q.astype(np.float64), good_k, good_v, first, hd ** -0.5, True, window, np.ones(n, dtype=bool))
+    err = np.abs(got - want)
+    clean = np.ones(q.shape, dtype=bool)
+    seeing = slice(bad_v - first, bad_v - first + window)
+    clean[seeing, :2, 5] = False                              # the rows that see the bad V, in that element
+    clean[rows - 1, 2:, :] = False                            # the row that sees the bad K
+    assert (err[clean] <= (off + np.abs(want) * 2.0 ** -24)[clean]).all()
+    dirty = got[seeing, :2, 5]
+    assert (np.isnan(dirty) if np.isnan(value) else (dirty == value) | np.isnan(dirty)).all()
+
+
+def test_whole_chip_on_one_head_and_cut_items(be, dev):
+    """One K/V head and a long context: every CTA has a piece of the same item."""
+    rng = np.random.default_rng(5)
+    check_attention(be, dev, rng, [1], [40000], 2, 1, 64, 64, max_rows=1)
+    check_attention(be, dev, rng, [40], [9000], 2, 1, 128, 64)
+
+
+def test_more_sequences_than_threads(be, dev):
+    rng = np.random.default_rng(6)
+    n = 700
+    rows = rng.integers(0, 3, n).tolist()
+    check_attention(be, dev, rng, rows, [int(x) for x in rng.integers(0, 60, n)], 2, 1, 32, 16)
+    check_attention(be, dev, rng, rows, [int(x) for x in rng.integers(0, 60, n)], 24, 1, 64, 16)
+
+
+def test_shared_pages_and_other_strides(be, dev):
+    """Two sequences with the same first pages; heads and positions with room between them."""
+    rng = np.random.default_rng(7)
+    check_attention(be, dev, rng, [1, 50], [200, 150], 4, 2, 64, 16, strides=(16 * 2 * 96 + 40, 72 + 72, 72))
+    pool = Pool(rng, [100, 100], 2, 64, 16)
+    pool.table[1, :4] = pool.table[0, :4]
+    k, v = rng.standard_normal((2, 100, 2, 64)).astype(np.float16)
+    pool.put(1, k, v)
+    pool.put(0, k, v)
+    q = rng.standard_normal((2, 4, 64)).astype(np.float16)
+    q[1] = q[0]
+    got = run_attention(be, dev, pool, [0, 1, 2], q, np.zeros(q.shape, dtype=np.float16))
+    assert np.array_equal(got[0], got[1])
+
+
+def test_lengths_that_make_no_sense_touch_nothing_else(be, dev):
+    """Negative lengths, lengths beyond the table, rows beyond the buffer: answered inside the described buffers (margins around them stay)."""
+    rng = np.random.default_rng(8)
+    pool = Pool(rng, [64, 64, 64], 2, 64, 16, fill=0.5)
+    pool.n_kv = [-5, 100000, 70]
+    margin = np.full((4 + 6 + 4, 4, 64), 3.0, dtype=np.float16)
+    po = dev(margin)
+    b = B.paged_batch(dev(np.array([0, 2, 5, 50], dtype=np.int32)), dev(np.array(pool.n_kv, dtype=np.int32)), dev(pool.table), 3, 6, pool.table.shape[1])
+    c = pool.cache(dev(pool.k), dev(pool.v))
+    be.paged_attention(B.paged_attention_desc(c, b, dev(rng.standard_normal((6, 4, 64)).astype(np.float16)), po + 4 * 4 * 64 * 2, 4))
+    got = dev.back(po, margin)
+    assert (got[:4] == 3).all() and (got[10:] == 3).all()
+    assert (got[4:6] == 0).all()                              # no positions
+    assert np.allclose(got[6:9], 0.5, atol=2.0 ** -11)
+
+
+# ---------------------------------------------------------------------------------------------- append
+def plain_rope(x, pos, mode, rot, base, scale):
+    out = x.copy()
+    i = np.arange(rot // 2)
+    angle = (pos[:, None] * (scale * np.float64(np.float32(base)) ** (-2.0 * i / rot)))[:, None, :]
+    a, b = (2 * i, 2 * i + 1) if mode == B.ROPE_PAIRS else (i, i + rot // 2)
+    out[..., a] = x[..., a] * np.cos(angle) - x[..., b] * np.sin(angle)
+    out[..., b] = x[..., a] * np.sin(angle) + x[..., b] * np.cos(angle)
+    return out
+
+
+def rope_off(x, mode, rot):
+    """|a| + |b| of an element's pair: angle to 2^-26 of a circle, sine, cosine and the two products to f32."""
+    s = np.abs(x).copy()
+    i = np.arange(rot // 2)
+    a, b = (2 * i, 2 * i + 1) if mode == B.ROPE_PAIRS else (i, i + rot // 2)
+    s[..., a] = s[..., b] = np.abs(x[..., a]) + np.abs(x[..., b])
+    return s * (2 * np.pi * 2.0 ** -26 + 4 * 2.0 ** -24)
+
+
+def check_append(be, dev, rng, rows, n_kv, h, h_kv, hd, page, mode=B.ROPE_PAIRS, rot=None, base=10000.0, scale=1.0, dtype=np.float32, q_type=np.float16, token_major=False, pad=0, in_place=False, drop=0):
+    rot = hd if rot is None else rot
+    pool = Pool(rng, n_kv, h_kv, hd, page, token_major, fill=0.25)
+    if drop:
+        pool.table[rng.random(pool.table.shape) < drop] = -1
+        pool.table[rng.random(pool.table.shape) < drop / 2] = pool.n_pages
+    starts = np.concatenate([[0], np.cumsum(rows)]).astype(np.int32)
+    n_rows, width = int(starts[-1]) + pad, (h + 2 * h_kv) * hd + 8
+    x = rng.standard_normal((n_rows, width)).astype(dtype)
+    px, pk, pv = dev(x), dev(pool.k), dev(pool.v)
+    q0 = np.full((n_rows, h, hd), -9, dtype=q_type)
+    pq = px if in_place else dev(q0)
+    e = x.itemsize * hd
+    types = {np.float32: B.FP32, np.float16: B.FP16}
+    d = B.paged_append_desc(pool.cache(pk, pv), B.paged_batch(dev(starts), dev(np.array(n_kv, dtype=np.int32)), dev(pool.table), len(rows), n_rows, pool.table.shape[1]),
+                            px if h else None, px + h * e, px + (h + h_kv) * e, pq if h else None, h, in_type=types[dtype], q_out_type=types[q_type], row_stride=width,
+                            q_out_stride=width if in_place else None, rope_mode=mode, rope_dim=rot, freq_base=base, freq_scale=scale)
+    be.paged_append(d)
+    got_k, got_v = dev.back(pk, pool.k), dev.back(pv, pool.v)
+    got_q = dev.back(px, x)[:, :h * hd].reshape(n_rows, h, hd) if in_place else dev.back(pq, q0)
+    want_k, want_v = pool.k.copy(), pool.v.copy()
+    untouched = np.ones((n_rows,), dtype=bool)
+    half = lambda a: np.abs(a) * 2.0 ** -11 + 2.0 ** -25  # noqa: E731
+    for s, n in enumerate(n_kv):
+        a, b = starts[s], starts[s + 1]
+        pos = np.arange(n - rows[s], n)
+        full = x[a:b, :(h + 2 * h_kv) * hd].reshape(b - a, h + 2 * h_kv, hd).astype(np.float64)
+        turned = full if mode == B.ROPE_NONE else plain_rope(full, pos, mode, rot, base, scale)
+        off = 0 * full if mode == B.ROPE_NONE else rope_off(full, mode, rot)
+        ok = pos >= 0
+        untouched[a:b] = ~ok
+        if h:
+            err = np.abs(got_q[a:b][ok].astype(np.float64) - turned[ok, :h])
+            tol = off[ok, :h] + (half(turned[ok, :h]) if q_type == np.float16 else np.abs(turned[ok, :h]) * 2.0 ** -24)
+            assert (err <= tol).all(), float((err / tol).max())
+        pages = pool.table[s, pos[ok] // page] if ok.any() else np.zeros(0, dtype=int)
+        there = (pages >= 0) & (pages < pool.n_pages)
+        at = (pages[there], pos[ok][there] % page)
+        for got, want, lo, exact in ((got_k, want_k, h, False), (got_v, want_v, h + h_kv, True)):
+            value = (full if exact else turned)[ok][there][:, lo:lo + h_kv]
+            have = pool.view(got)[at].astype(np.float64)
+            assert (np.abs(have - value) <= half(value) + (0 if exact else off[ok][there][:, lo:lo + h_kv])).all()
+            pool.view(want)[at] = pool.view(got)[at]
+    assert np.array_equal(got_k, want_k) and np.array_equal(got_v, want_v)         # nothing else was stored
+    untouched[starts[-1]:] = True
+    if h:
+        before = x[:, :h * hd].reshape(n_rows, h, hd) if in_place else q0
+        assert np.array_equal(got_q[untouched], before[untouched])
+
+
+@pytest.mark.parametrize("mode", [B.ROPE_NONE, B.ROPE_PAIRS, B.ROPE_HALVES])
+@pytest.mark.parametrize("hd,rot", [(8, 8), (24, 16), (64, 64), (96, 48), (128, 128), (256, 256)])
+@pytest.mark.parametrize("dtype", [np.float32, np.float16])
+def test_append(be, dev, mode, hd, rot, dtype):
+    rng = np.random.default_rng(hd + rot)
+    check_append(be, dev, rng, [1, 20, 0, 3], [400, 20, 7, 100001], 6, 2, hd, 16, mode=mode, rot=rot, dtype=dtype, pad=2)
+    check_append(be, dev, rng, [1], [33], 3, 3, hd, 5, mode=mode, rot=rot, dtype=dtype, q_type=np.float32, token_major=True, base=500000.0, scale=0.25)
+
+
+def test_append_in_place_without_q_and_with_missing_pages(be, dev):
+    rng = np.random.default_rng(11)
+    check_append(be, dev, rng, [5, 2], [50, 2], 4, 2, 64, 16, q_type=np.float32, in_place=True)
+    check_append(be, dev, rng, [5, 2], [50, 2], 4, 2, 64, 16, mode=B.ROPE_HALVES, dtype=np.float16, in_place=True)
+    check_append(be, dev, rng, [5, 2], [50, 2], 0, 2, 64, 16)
+    check_append(be, dev, rng, [40, 30], [300, 30], 4, 2, 64, 8, drop=0.5)
+    check_append(be, dev, rng, [6, 1], [4, 0], 4, 2, 64, 8)                              # rows with negative positions
+
+
+def test_append_of_many_sequences(be, dev):
+    rng = np.random.default_rng(12)
+    rows = rng.integers(0, 4, 1500).tolist()
+    check_append(be, dev, rng, rows, [r + int(x) for r, x in zip(rows, rng.integers(0, 30, 1500))], 2, 1, 64, 16, pad=5)
+
+
+def test_nothing_to_do(be, dev):
+    """No sequences, no rows."""
+    c = B.paged_cache(dev(np.zeros(4096, np.float16)), dev(np.zeros(4096, np.float16)), 2, 16, 1, 64)
+    z = dev(np.zeros(64, np.float32))
+    for n_seq, n_rows in ((0, 3), (2, 0)):
+        b = B.paged_batch(z, z, z, n_seq, n_rows, 1)
+        be.paged_attention(B.paged_attention_desc(c, b, z, z, 1))
+        be.paged_append(B.paged_append_desc(c, b, z, z, z, z, 1))
+    be.sample(B.sample_desc(z, B.FP32, 0, 5, z))
+    be.sync()
+
+
+# ---------------------------------------------------------------------------------------------- sample
+def plain_sample(x, t, k, p, least, u):
+    x = np.where(np.isnan(x), -np.inf, x.astype(np.float64))
+    if x.max() == -np.inf:
+        return -1, 0.0
+    if not t > 0:
+        return int(np.argmax(x)), 1.0
+    if x.max() == np.inf:
+        x = np.where(x == np.inf, 0.0, -np.inf)
+    with np.errstate(invalid="ignore"):
+        w = np.where(x == -np.inf, 0.0, np.exp((x - x.max()) / np.float64(t)))
+    order = np.lexsort((np.arange(len(x)), -x))
+    if 0 < k < len(x):
+        order = order[:k]
+    if p < 1:
+        sums = np.concatenate([[0.0], np.cumsum(w[order])])
+        stay = sums[:-1] < np.float64(p) * sums[-1]
+        stay[0] = True
+        order = order[stay]
+    if least > 0:
+        order = order[w[order] >= min(np.float64(least), 1.0)]
+    order = np.sort(order)
+    sums = np.cumsum(w[order])
+    at = int(np.searchsorted(sums, np.float64(max(u, 0.0)) * sums[-1], side="right"))
+    at = min(at, int(np.nonzero(w[order] > 0)[0][-1]))
+    return int(order[at]), float(w[order][at] / sums[-1])
+
+
+def check_sample(be, dev, x, t=None, k=None, p=None, least=None, u=None, stride=None, offset=0):
+    n, v = x.shape
+    store = np.full(n * (stride or v) + offset, 50.0, dtype=x.dtype)
+    for r in range(n):
+        store[offset + r * (stride or v):][:v] = x[r]
+    arrays = {"temperature": (t, np.float32), "top_k": (k, np.int32), "top_p": (p, np.float32), "min_p": (least, np.float32), "uniform": (u, np.float32)}
+    host = {name: None if a is None else np.broadcast_to(np.asarray(a, dtype=dt), (n,)).copy() for name, (a, dt) in arrays.items()}
+    ids, probs = np.full(n + 1, -77, dtype=np.int32), np.full(n + 1, -77, dtype=np.float32)
+    pi, pp = dev(ids), dev(probs)
+    d = B.sample_desc(dev(store) + offset * x.itemsize, B.FP32 if x.dtype == np.float32 else B.FP16, n, v, pi, probs=pp, row_stride=stride, **{m: None if a is None else dev(a) for m, a in host.items()})
+    be.sample(d)
+    got_i, got_p = dev.back(pi, ids), dev.back(pp, probs)
+    default = {"temperature": 1.0, "top_k": 0, "top_p": 1.0, "min_p": 0.0, "uniform": 0.0}
+    for r in range(n):
+        with np.errstate(over="ignore"):
+            want = plain_sample(x[r], *(default[m] if host[m] is None else host[m][r] for m in ("temperature", "top_k", "top_p", "min_p", "uniform")))
+        assert got_i[r] == want[0], (r, got_i[r], want)
+        assert abs(got_p[r] - want[1]) <= 2.0 ** -23 * want[1]                        # one rounding to f32, weights to 2^-40
+    assert got_i[n] == -77 and got_p[n] == -77
+
+
+@pytest.mark.parametrize("v", [1, 2, 31, 100, 1000, 4097, 32000, 50001])
+@pytest.mark.parametrize("dtype", [np.float32, np.float16])
+def test_sample_settings(be, dev, v, dtype):
+    rng = np.random.default_rng(v)
+    n = 24
+    x = (3 * rng.standard_normal((n, v))).astype(dtype)
+    u = rng.random(n).astype(np.float32)
+    r = np.arange(n)
+    check_sample(be, dev, x, u=u)
+    check_sample(be, dev, x, t=np.where(r % 3 == 0, 0, 0.5 + r / 20), u=u)
+    check_sample(be, dev, x, t=0.8, k=r * r, u=u)
+    check_sample(be, dev, x, t=1.1, p=(r + 1) / n, u=u)
+    check_sample(be, dev, x, least=r / n, u=u)
+    check_sample(be, dev, x, t=0.3 + r / 10, k=np.where(r % 2, 0, 40), p=np.where(r % 3, 0.9, 1.0), least=np.where(r % 5, 0.02, 0), u=u, stride=v + 3, offset=1)
+
+
+def test_sample_many_candidates(be, dev):
+    """Candidates that do not fit a list: a large top_k, flat rows, ties by the thousand."""
+    rng = np.random.default_rng(3)
+    u = rng.random(6).astype(np.float32)
+    x = (2 * rng.standard_normal((6, 20000))).astype(np.float32)
+    check_sample(be, dev, x, k=[1023, 1024, 1025, 5000, 19999, 20000], u=u)
+    check_sample(be, dev, x, k=[1023, 1024, 1025, 5000, 19999, 20000], p=0.6, least=1e-4, u=u)
+    check_sample(be, dev, 1e-3 * x, p=[0.01, 0.2, 0.5, 0.9, 0.999, 0.3], t=3.0, u=u)
+    ties = np.round(x)
+    check_sample(be, dev, ties, p=[0.01, 0.25, 0.5, 0.9, 0.999, 0.3], u=u)
+    check_sample(be, dev, ties, k=[1, 2, 500, 3000, 9000, 15000], u=u)
+    check_sample(be, dev, np.zeros_like(x), p=0.5, u=u)
+    check_sample(be, dev, np.zeros_like(x), k=7, u=u)
+    check_sample(be, dev, np.zeros_like(x), k=3000, p=0.5, least=0.5, u=u)
+
+
+def test_sample_what_is_not_finite(be, dev):
+    inf, nan = np.inf, np.nan
+    rows = [[1, 2, nan, 0], [-inf, -inf, -inf, -inf], [nan, nan, nan, nan], [-inf, 3, -inf, 3], [inf, 1, inf, -inf], [inf, nan, inf, inf], [-1e30, -1e30, 1e30, 1e30], [3e38, -3e38, 3e38, 0]]
+    x = np.array(rows, dtype=np.float32)
+    for u in (0.0, 0.4, 0.5, 0.75, 1 - 2.0 ** -24, 1.0, -1.0, nan):
+        check_sample(be, dev, x, u=0.0 if u != u else u) if u == u else None
+        for extra in ({}, {"t": 0.0}, {"t": 1e-3}, {"t": 1e3}, {"k": 1}, {"k": 3, "p": 0.5}, {"p": 0.0}, {"p": 0.7}, {"least": 1.0}, {"least": 5.0}):
+            check_sample(be, dev, x, u=0.0 if u != u else u, **extra)
+
+
+def test_sample_large_vocabulary(be, dev):
+    """Slices that do not stay in shared memory."""
+    rng = np.random.default_rng(4)
+    x = (3 * rng.standard_normal((2, (1 << 20) - 5))).astype(np.float32)
+    u = rng.random(2).astype(np.float32)
+    for k in ({}, {"t": 0.0}, {"k": 50, "p": 0.9}, {"p": 0.8}, {"least": 0.01}):
+        check_sample(be, dev, x, u=u, **k)
+
+
+def test_sample_draws_by_weight(be, dev):
+    """Evenly spaced numbers draw each token by its share."""
+    x = np.log(np.array([0.5, 0.25, 0.125, 0.125], dtype=np.float64)).astype(np.float32)
+    n = 4096
+    u = ((np.arange(n) + 0.5) / n).astype(np.float32)
+    ids = np.zeros(n, dtype=np.int32)
+    pi = dev(ids)
+    be.sample(B.sample_desc(dev(np.broadcast_to(x, (n, 4)).copy()), B.FP32, n, 4, pi, uniform=dev(u)))
+    count = np.bincount(dev.back(pi, ids), minlength=4)
+    assert np.abs(count - np.array([2048, 1024, 512, 512])).max() <= 1
+
+
+# ---------------------------------------------------------------------------------------------- together
+def test_a_serving_loop(be, dev):
+    """Requests of different lengths come in chunks beside running ones: append, attend, sample, feed the token back; against one plain cache a request."""
+    rng = np.random.default_rng(21)
+    h, h_kv, hd, v, page = 4, 2, 64, 500, 16
+    d, width = 128, (h + 2 * h_kv) * hd
+    embed, w_qkv, w_out = rng.standard_normal((v, d)), rng.standard_normal((d, width)) * d ** -0.5, rng.standard_normal((h * hd, v)) * 0.2
+    prompts = [rng.integers(0, v, n).tolist() for n in (37, 5, 1, 90)]
+    total, n_seq = 128, len(prompts)
+    pool = Pool(rng, [total] * n_seq, h_kv, hd, page)
+    pk, pv, pt = dev(pool.k), dev(pool.v), dev(pool.table)
+    done, history = [0] * n_seq, [([], []) for _ in prompts]
+    for step in range(12):
+        rows = [min(32, len(t) - n) for t, n in zip(prompts, done)]                    # chunks of at most 32
+        starts = np.concatenate([[0], np.cumsum(rows)]).astype(np.int32)
+        n_kv = np.array([n + r for n, r in zip(done, rows)], dtype=np.int32)
+        x = np.concatenate([embed[t[n:n + r]] for t, n, r in zip(prompts, done, rows)]) @ w_qkv
+        x = x.astype(np.float32)
+        px, n_rows = dev(x), int(starts[-1])
+        pq, po = dev(np.zeros((n_rows, h, hd), np.float16)), dev(np.zeros((n_rows, h, hd), np.float32))
+        batch = B.paged_batch(dev(starts), dev(n_kv), pt, n_seq, n_rows, pool.table.shape[1], max(rows))
+        cache = pool.cache(pk, pv)
+        be.paged_append(B.paged_append_desc(cache, batch, px, px + 4 * h * hd, px + 4 * (h + h_kv) * hd, pq, h, row_stride=width))
+        be.paged_attention(B.paged_attention_desc(cache, batch, pq, po, h, out_type=B.FP32))
+        out = dev.back(po, np.zeros((n_rows, h, hd), np.float32))
+        for s in range(n_seq):
+            a, b = starts[s], starts[s + 1]
+            full = x[a:b].reshape(-1, h + 2 * h_kv, hd).astype(np.float64)
+            turned = plain_rope(full, np.arange(done[s], n_kv[s]), B.ROPE_PAIRS, hd, 10000.0, 1.0)
+            history[s][0].extend(turned[:, h:h + h_kv])
+            history[s][1].extend(full[:, h + h_kv:])
+            want, off = plain_attention(turned[:, :h], np.array(history[s][0]), np.array(history[s][1]), done[s], hd ** -0.5, True, 0, np.ones(n_kv[s], dtype=bool))
+            # Q, K and V were rounded to fp16 on their way: a score is off by 2 x 2^-11 of the sum of its products' sizes, a probability by twice that, a value by 2^-11
+            size = hd ** -0.5 * np.abs(turned[:, :h]).sum(-1).max() * np.abs(np.array(history[s][0])).max()
+            assert np.all(np.abs(out[a:b] - want) <= off + (2 * 2 * 2.0 ** -11 * size + 2.0 ** -10) * np.abs(np.array(history[s][1])).max())
+        last = starts[1:] - 1
+        logits = (out.reshape(n_rows, -1)[last] @ w_out).astype(np.float32)
+        u = rng.random(n_seq).astype(np.float32)
+        pi = dev(np.zeros(n_seq, np.int32))
+        be.sample(B.sample_desc(dev(logits), B.FP32, n_seq, v, pi, uniform=dev(u), top_k=dev(np.full(n_seq, 20, np.int32)), temperature=dev(np.full(n_seq, 0.8, np.float32))))
+        ids = dev.back(pi, np.zeros(n_seq, np.int32))
+        for s in range(n_seq):
+            assert ids[s] == plain_sample(logits[s], np.float32(0.8), 20, 1.0, 0.0, u[s])[0]
+            done[s] = int(n_kv[s])
+            if done[s] == len(prompts[s]):
+                prompts[s].append(int(ids[s]))
+    assert all(len(t) > n for t, n in zip(prompts, (37, 5, 1, 90)))
+
+
+def test_results_do_not_depend_on_programmatic_launch(dev):
+    """Append, attention and sampling back to back on one stream, with and without kernels that start beside their predecessors."""
+    got = []
+    for pdl in (True, False):
+        b = B.B200Backend(0, use_pdl=pdl)
+        d, rng = Device(b), np.random.default_rng(31)
+        pool = Pool(rng, [300, 20, 90], 2, 64, 16, fill=0.0)
+        pool.put(0, *rng.standard_normal((2, 299, 2, 64)).astype(np.float16))
+        cache = pool.cache(d(pool.k), d(pool.v))
+        batch = B.paged_batch(d(np.array([0, 1, 21, 60], np.int32)), d(np.array([300, 20, 39], np.int32)), d(pool.table), 3, 60, pool.table.shape[1])
+        x = d(rng.standard_normal((60, 8 * 64)).astype(np.float32))
+        q, o, ids = d(np.zeros((60, 4, 64), np.float16)), np.zeros((60, 4 * 64), np.float32), np.zeros(60, np.int32)
+        po, pi = d(o), d(ids)
+        for _ in range(20):
+            b.paged_append(B.paged_append_desc(cache, batch, x, x + 4 * 256, x + 4 * 384, q, 4, row_stride=512))
+            b.paged_attention(B.paged_attention_desc(cache, batch, q, po, 4, out_type=B.FP32))
+            b.sample(B.sample_desc(po, B.FP32, 60, 256, pi))
+        got.append((d.back(po, o), d.back(pi, ids)))
+        d.free()
+        b.close()
+    assert np.array_equal(got[0][0], got[1][0]) and np.array_equal(got[0][1], got[1][1])
