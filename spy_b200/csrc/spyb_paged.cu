@@ -657,8 +657,13 @@ spyb_status spyb_paged_attention(spyb_backend *be, const spyb_paged_attention_de
     p.scale_log2 = (float)((double)scale * 1.4426950408889634073599);
     p.partial = be->paged_partial; p.arrived = be->paged_arrived;
     const int64_t most = (int64_t)(d->batch.max_rows > 0 ? std::min(d->batch.max_rows, d->batch.n_rows) : d->batch.n_rows) * p.group;
+    const LaunchCfg cfg = be->launch_cfg(be->config.use_pdl != 0);
     p.few_rows = 1 << 30;
-    SPYB_CUDA(be, launch_paged_attention_rows(p, hd, most <= 16 ? 1 : 2, be->num_sms_total, be->launch_cfg(be->config.use_pdl != 0)));
+    if (most > PA_FEW_ROWS && paged_tc_can(p.view, hd)) {
+        p.few_rows = p.view.n_seq == 1 ? 0 : PA_FEW_ROWS;
+        SPYB_CUDA(be, launch_paged_attention_tc(p, hd, be->num_sms_total, cfg, be->wait_limit_ns));
+    }
+    if (p.few_rows > 0) { SPYB_CUDA(be, launch_paged_attention_rows(p, hd, most <= 16 ? 1 : 2, be->num_sms_total, cfg)); }
     return SPYB_SUCCESS;
 }
 

@@ -35,6 +35,9 @@ struct PagedAttention {
 int         paged_cut_selftest();   // host-only: 0 when the CTAs' pieces cover every item once, on any lengths
 cudaError_t launch_paged_append(const PagedAppend &p, int in_type, int q_out_type, const LaunchCfg &cfg);
 cudaError_t launch_paged_attention_rows(const PagedAttention &p, int head_dim, int row_tiles, int sms, const LaunchCfg &cfg);
+bool        paged_tc_can(const PagedView &v, int head_dim);   // the tensor-memory kernel takes these pages and heads
+cudaError_t launch_paged_attention_tc(const PagedAttention &p, int head_dim, int sms, const LaunchCfg &cfg, uint64_t wait_limit);
+constexpr int PA_FEW_ROWS = 32;          // sequences of up to so many rows (times query heads of a K/V head) are the small kernel's
 constexpr int PA_MAX_CTAS_PER_SM = 2;
 
 // ---------------------------------------------------------------------------------------------- cutting the work

@@ -1,0 +1,592 @@
+// Attention of many rows a sequence (chunks of prompts, groups of query heads) over paged caches on the tcgen05 tensor cores.
+//
+// Rows and positions go in tiles: 256 rows - two tiles of 128, each with a warpgroup of its own - against 128 positions at a time. S = Q K^T and O += P V are
+// tcgen05 MMAs, 128 x 128 x 16 and 128 x head_dim x 16; S, P (fp16, in place of S) and O live in tensor memory, a row a lane, so that a row's maximum and sum stay in
+// one thread. While one tile's probabilities are made (16 powers of two a clock and SM, as many clocks as its two products take), the other tile's
+// products run. K and V come page by page through tensor maps, in pieces of as many positions as divide the page size, into the 128-byte
+// swizzle of the operands: K row by row (K-major), V as it lies (its positions are the product's inner dimension: MN-major), no transposition anywhere.
+//   warps 0-3, 4-7   probabilities of tile 0 / 1, rescaling, output          warp 8   issues the MMAs
+//   warp 9           copies                                                   warp 10  clears and checks the V tiles that not all rows see whole
+// Probabilities are taken against a maximum that follows the true one when that is 2^8 above it: O is rescaled in the first steps and hardly ever after.
+
+#include <algorithm>
+
+#include <cuda.h>
+#include <math_constants.h>
+
+#include "spyb_internal.h"
+#include "spyb_paged.cuh"
+#include "spyb_tc.cuh"
+
+namespace spyb {
+namespace {
+
+constexpr int PT_THREADS = 384, PT_ROWS = 128, PT_TILE = 2 * PT_ROWS, PT_KEYS = 128;
+constexpr int PT_REGS_SOFTMAX = 208, PT_REGS_OTHERS = 88;   // 256 x 208 + 128 x 88 = 384 x 168, what the block is launched with
+constexpr uint32_t PT_HALF = PT_KEYS * 128;              // bytes of 128 rows x 64 elements
+
+template <int HD> struct TcShape {
+    static constexpr uint32_t OPERAND = PT_KEYS * HD * 2;                      // a tile of Q, K or V
+    static constexpr int SLOTS = HD == 128 ? 5 : 8;                            // K and V tiles in flight
+    static constexpr uint32_t SMEM = (2 + SLOTS) * OPERAND + 1024;             // (+ alignment)
+};
+struct TcShared {
+    uint64_t full[8], empty[8];                          // a slot's copies have landed; its last MMA is done
+    uint64_t clean[8];                                   // of the last V tiles: what nobody sees is cleared
+    uint64_t q_ready[2], s_ready[2], p_ready[2], o_ready[2];
+    uint32_t tmem;
+    uint32_t there[8];                                   // of the last tiles: which groups of eight positions are there
+    int      poison[8];                                  // of the last stretches: a V tile that some rows see in part holds values that are not finite
+    int      last[2];
+    PagedPlanShared plan;
+};
+
+__device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap *map, uint32_t bar, int x, int token, int head, int page) {
+    asm volatile("cp.async.bulk.tensor.4d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3,%4,%5,%6}], [%2];"
+                 ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(token), "r"(head), "r"(page) : "memory");
+}
+// operands in the 128-byte swizzle: rows of 128 bytes, groups of eight rows 1024 bytes apart; `far`: from one 64-element half of an MN-major operand to the next
+__device__ __forceinline__ uint64_t swizzled_desc(uint32_t addr, uint32_t far) {
+    return (uint64_t)((addr & 0x3FFFFu) >> 4) | ((uint64_t)(far >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+__device__ __forceinline__ void mma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+                 ::"r"(d_tmem), "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate) : "memory");
+}
+#define SPYB_R32(r) "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), \
+    "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), \
+    "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+#define SPYB_I32(r) "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), \
+    "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), \
+    "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t *r) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+                 : SPYB_R32(r) : "r"(taddr) : "memory");
+}
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t *r) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};"
+                 ::SPYB_I32(r), "r"(taddr) : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ float max3(float a, float b, float c) { float d; asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c)); return d; }
+__device__ __forceinline__ float exp2_fast(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) { uint32_t r; asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo)); return r; }
+__device__ __forceinline__ uint32_t not_finite(uint32_t h2) { return ((h2 & 0x7c007c00u) + 0x04000400u) & 0x80008000u; }
+__device__ __forceinline__ void group_sync(int t) { asm volatile("bar.sync %0, 128;" ::"r"(1 + t) : "memory"); }
+
+// One stretch of an item: positions [j0 x 128, j1 x 128) of its tiles' rows. Every role walks the same stretches.
+struct Stretch {
+    PagedSeq  q;
+    PagedItem it;
+    int seq, head, tile, off, todo;
+    int rows[2], pos_first[2], pos_last[2];          // of the two tiles
+    int from[2], to[2];                              // 128-position steps (of the item) in which a tile sees anything, within this stretch
+
+    __device__ __forceinline__ void describe(const PagedAttention &p, const PagedPlace &at) {
+        it = paged_item<PT_TILE, PT_KEYS, PT_KEYS>(p, q, tile);
+        todo = (int)min((int64_t)(it.units - off), at.end - at.unit);
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            const int r0 = tile * PT_TILE + t * PT_ROWS;
+            rows[t] = max(0, min(PT_ROWS, q.rows * p.group - r0));
+            pos_first[t] = q.first + (int)((unsigned)r0 / (unsigned)p.group);
+            pos_last[t] = q.first + (int)((unsigned)(r0 + max(rows[t], 1) - 1) / (unsigned)p.group);
+            const int hi = p.causal ? min(it.hi, pos_last[t] + 1) : it.hi, lo = p.causal && p.window > 0 ? max(it.lo, pos_first[t] - p.window + 1) : it.lo;
+            from[t] = max(off, (max(lo, it.lo) - it.lo) / PT_KEYS);
+            to[t] = rows[t] == 0 || hi <= it.lo ? off : min(off + todo, (hi - it.lo + PT_KEYS - 1) / PT_KEYS);
+            if (to[t] <= from[t]) { from[t] = to[t] = off; }
+        }
+    }
+    __device__ __forceinline__ bool active(int t, int step) const { return step >= from[t] && step < to[t]; }
+    __device__ __forceinline__ bool needed(int step) const { return active(0, step) || active(1, step); }
+    // all rows of tile t see all positions of the step (if their pages are there)
+    __device__ __forceinline__ bool whole(const PagedAttention &p, int t, int step) const {
+        const int j = it.lo + step * PT_KEYS;
+        return j + PT_KEYS <= it.hi && (!p.causal || (j + PT_KEYS - 1 <= pos_first[t] && (p.window <= 0 || j > pos_last[t] - p.window)));
+    }
+    __device__ __forceinline__ bool next(const PagedAttention &p, PagedPlace &at) {
+        at.unit += todo;
+        if (at.unit >= at.end) { return false; }
+        off = 0;
+        return paged_next<PT_TILE>(p, false, q, seq, head, tile);
+    }
+};
+
+template <int HD>
+__global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_constant__ PagedAttention p, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
+                                                                  const int box, int *error_flag, const uint64_t wait_limit) {
+    using Shape = TcShape<HD>;
+    constexpr int SLOTS = Shape::SLOTS;
+    extern __shared__ uint8_t raw[];
+    __shared__ TcShared sh;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const uint32_t base = (smem_u32(raw) + 1023) & ~1023u, q_addr = base, ring = base + 2 * Shape::OPERAND;
+    const uint32_t full = smem_u32(sh.full), empty = smem_u32(sh.empty), clean = smem_u32(sh.clean);
+    const uint32_t q_ready = smem_u32(sh.q_ready), s_ready = smem_u32(sh.s_ready), p_ready = smem_u32(sh.p_ready), o_ready = smem_u32(sh.o_ready);
+    if (tid == 0) {
+        for (int i = 0; i < 8; ++i) { mbar_init(full + 8 * i, 1); mbar_init(empty + 8 * i, 1); mbar_init(clean + 8 * i, 1); sh.poison[i] = 0; }
+        for (int t = 0; t < 2; ++t) { mbar_init(q_ready + 8 * t, 4); mbar_init(s_ready + 8 * t, 1); mbar_init(p_ready + 8 * t, 4); mbar_init(o_ready + 8 * t, 1); }
+        mbar_init_fence();
+    }
+    pdl_launch_dependents();
+    pdl_wait();
+    PagedPlace at = paged_plan<PT_THREADS, PT_TILE, PT_KEYS, PT_KEYS>(p, false, 2, sh.plan);
+    if (at.unit >= at.end) { return; }
+    if (warp == 8) { asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&sh.tmem)) : "memory"); }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = sh.tmem;
+    uint64_t limit = wait_limit;
+    Stretch x;
+    x.seq = at.seq; x.head = at.head; x.tile = at.tile; x.off = at.off;
+    x.q = paged_seq(p.view, at.seq);
+
+    if (warp < 8) {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(PT_REGS_SOFTMAX));
+        // ---------------------------------------------------------------------------------- probabilities, output
+        const int t = warp >> 2, row = tid & 127;
+        const uint32_t lanes = (uint32_t)(warp & 3) << 21;                                   // (32 lanes a warp, in the address's upper half)
+        const uint32_t s_tmem = tmem + lanes + t * PT_KEYS, o_tmem = tmem + lanes + 2 * PT_KEYS + t * HD;
+        const float scale = fabsf(p.scale_log2);
+        const uint32_t flip = p.scale_log2 < 0.f ? 0x80008000u : 0u;                         // the scale's sign goes into Q
+        uint32_t s_phase = 0, o_phase = 0, tiles = 0, stretch = 0;
+        auto load_q = [&]() {
+            // rows of this warp, two at a time (hd 64: four): 16-byte pieces into the swizzle
+            constexpr int PIECES = HD / 8, AT_ONCE = 32 / PIECES;
+#pragma unroll 4
+            for (int i = 0; i < 32 / AT_ONCE; ++i) {
+                const int r = (warp & 3) * 32 + i * AT_ONCE + lane / PIECES, c = lane % PIECES;
+                uint4 v = make_uint4(0, 0, 0, 0);
+                if (r < x.rows[t]) {
+                    const int pr = x.tile * PT_TILE + t * PT_ROWS + r, token = (int)((unsigned)pr / (unsigned)p.group), g = pr - token * p.group;
+                    v = *reinterpret_cast<const uint4 *>(p.q + (int64_t)(x.q.row0 + token) * p.q_stride + (x.head * p.group + g) * HD + c * 8);
+                    v.x ^= flip; v.y ^= flip; v.z ^= flip; v.w ^= flip;
+                }
+                sts128(q_addr + t * Shape::OPERAND + (c >> 3) * PT_HALF + r * 128 + (((c & 7) ^ (r & 7)) << 4), v);
+            }
+            fence_async_smem();
+            __syncwarp();
+            if (lane == 0) { mbar_arrive(q_ready + 8 * t); }
+        };
+        x.describe(p, at);
+        load_q();
+        for (;;) {
+            float m = -CUDART_INF_F, l = 0.f;
+            const int pr = x.tile * PT_TILE + t * PT_ROWS + min(row, max(x.rows[t], 1) - 1);
+            const int token = (int)((unsigned)pr / (unsigned)p.group), g = pr - token * p.group, pos = x.q.first + token;
+            for (int step = x.off; step < x.off + x.todo; ++step) {
+                if (!x.needed(step)) { continue; }
+                ++tiles;
+                if (!x.active(t, step)) { continue; }
+                mbar_wait_lean(s_ready + 8 * t, s_phase, limit);
+                s_phase ^= 1;
+                tc_fence_after();
+                uint32_t s[128];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) { tmem_ld32(s_tmem + 32 * i, s + 32 * i); }
+                tmem_ld_wait();
+                const uint32_t there = *reinterpret_cast<volatile uint32_t *>(&sh.there[(tiles - 1) & 7]);
+                if (!x.whole(p, t, step) || there != 0xffffu) {
+                    const int j0 = x.it.lo + step * PT_KEYS;
+                    const int c1 = (p.causal ? min(x.it.hi, pos + 1) : x.it.hi) - j0, c0 = p.causal && p.window > 0 ? pos - p.window + 1 - j0 : 0;
+#pragma unroll
+                    for (int c = 0; c < 128; ++c) {
+                        if (!(c >= c0 && c < c1 && ((there >> (c >> 3)) & 1))) { s[c] = 0xff800000u; }
+                    }
+                }
+                float top = __uint_as_float(s[0]);
+#pragma unroll
+                for (int c = 1; c < 127; c += 2) { top = max3(top, __uint_as_float(s[c]), __uint_as_float(s[c + 1])); }
+                top = fmaxf(top, __uint_as_float(s[127])) * scale;
+                if (__any_sync(0xffffffffu, top > m + 8.f)) {
+                    const float to = fmaxf(m, top), f = to == m ? 1.f : exp2_fast(m - to);
+                    m = to; l *= f;
+                    if (step != x.from[t]) {
+#pragma unroll 1
+                        for (int i = 0; i < HD / 32; ++i) {
+                            uint32_t o[32];
+                            tmem_ld32(o_tmem + 32 * i, o);
+                            tmem_ld_wait();
+#pragma unroll
+                            for (int c = 0; c < 32; ++c) { o[c] = __float_as_uint(__uint_as_float(o[c]) * f); }
+                            tmem_st32(o_tmem + 32 * i, o);
+                        }
+                    }
+                }
+                const float neg = m == -CUDART_INF_F ? 0.f : -m;
+                const uint64_t neg2 = f2_pack(neg, neg), scale2 = f2_pack(scale, scale);
+                uint64_t sum[2] = {0, 0};
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    uint32_t h[32];
+#pragma unroll
+                    for (int c = 0; c < 32; ++c) {
+                        const int k = 64 * i + 2 * c;
+                        float a, b;
+                        f2_unpack(f2_fma(f2_pack_bits(s[k], s[k + 1]), scale2, neg2), a, b);
+                        a = exp2_fast(a); b = exp2_fast(b);
+                        sum[c & 1] = f2_add(sum[c & 1], f2_pack(a, b));
+                        h[c] = pack_f16(a, b);
+                    }
+                    tmem_st32(s_tmem + 32 * i, h);
+                }
+                float a, b;
+                f2_unpack(f2_add(sum[0], sum[1]), a, b);
+                l += a + b;
+                tmem_st_wait();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) { mbar_arrive(p_ready + 8 * t); }
+            }
+            // this stretch's findings; the next one's Q goes first (all S of this one are there)
+            const Stretch done = x;
+            const PagedPlace was = at;
+            const bool any = done.to[t] > done.from[t];
+            if (!any) { mbar_wait_lean(o_ready + 8 * t, o_phase, limit); }       // (so that nobody is two stretches ahead of the MMAs)
+            const bool more = x.next(p, at);
+            if (more) { x.describe(p, at); load_q(); }
+            if (any) { mbar_wait_lean(o_ready + 8 * t, o_phase, limit); tc_fence_after(); }
+            o_phase ^= 1;
+            const PagedCut cut = paged_cut(was, was.unit - done.off, done.it.units);
+            float4 *part = reinterpret_cast<float4 *>(p.partial) + (paged_slot(blockIdx.x, cut.c0) * 2 + t) * (PT_ROWS * (HD + 2) / 4);     // [HD / 4][128] x 4, [128], [128]
+            const float inv = cut.parts > 1 ? 1.f : l == 0.f ? 0.f : 1.f / l;
+            const bool mine = row < done.rows[t];
+            const bool poisoned = any && *reinterpret_cast<volatile int *>(&sh.poison[stretch & 7]) == (int)stretch + 1;
+            const int64_t to_row = (int64_t)(done.q.row0 + token) * p.out_stride + (done.head * p.group + g) * HD;
+#pragma unroll 1
+            for (int i = 0; i < HD / 32; ++i) {
+                uint32_t o[32];
+                if (any) { tmem_ld32(o_tmem + 32 * i, o); tmem_ld_wait(); }
+                else {
+#pragma unroll
+                    for (int c = 0; c < 32; ++c) { o[c] = 0; }
+                }
+                if (poisoned && mine) {
+                    // values that are not finite were taken out of the V tiles that not all rows see whole: back to the rows that see them
+                    for (int step = done.from[t]; step < done.to[t]; ++step) {
+                        if (done.whole(p, 0, step) && done.whole(p, 1, step)) { continue; }
+                        const int j0 = done.it.lo + step * PT_KEYS, ja = max(j0, p.causal && p.window > 0 ? pos - p.window + 1 : 0), jb = min(j0 + PT_KEYS, p.causal ? min(done.it.hi, pos + 1) : done.it.hi);
+                        for (int j = ja; j < jb; ++j) {
+                            const int page = p.view.page_table[(int64_t)done.seq * p.view.table_stride + j / p.view.page_size];
+                            if (page < 0 || page >= p.view.n_pages) { continue; }
+                            const __half *v = p.v + page * p.view.page_stride + (j % p.view.page_size) * p.view.token_stride + done.head * p.view.head_stride + 32 * i;
+#pragma unroll
+                            for (int c = 0; c < 32; ++c) {
+                                const float y = __half2float(v[c]);
+                                if (!isfinite(y)) { o[c] = __float_as_uint(__uint_as_float(o[c]) + y); }
+                            }
+                        }
+                    }
+                }
+                if (cut.parts > 1) {
+#pragma unroll
+                    for (int c = 0; c < 8; ++c) {
+                        part[(8 * i + c) * PT_ROWS + row] = make_float4(__uint_as_float(o[4 * c]), __uint_as_float(o[4 * c + 1]), __uint_as_float(o[4 * c + 2]), __uint_as_float(o[4 * c + 3]));
+                    }
+                } else if (mine) {
+                    if (p.out_f32) {
+                        float4 *dst = reinterpret_cast<float4 *>(static_cast<float *>(p.out) + to_row + 32 * i);
+#pragma unroll
+                        for (int c = 0; c < 8; ++c) {
+                            dst[c] = make_float4(__uint_as_float(o[4 * c]) * inv, __uint_as_float(o[4 * c + 1]) * inv, __uint_as_float(o[4 * c + 2]) * inv, __uint_as_float(o[4 * c + 3]) * inv);
+                        }
+                    } else {
+                        uint4 *dst = reinterpret_cast<uint4 *>(static_cast<__half *>(p.out) + to_row + 32 * i);
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) {
+                            uint32_t h[4];
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) { h[e] = pack_f16(__uint_as_float(o[8 * c + 2 * e]) * inv, __uint_as_float(o[8 * c + 2 * e + 1]) * inv); }
+                            dst[c] = make_uint4(h[0], h[1], h[2], h[3]);
+                        }
+                    }
+                }
+            }
+            tc_fence_before();
+            if (cut.parts > 1) {
+                float *stats = reinterpret_cast<float *>(part + PT_ROWS * HD / 4);
+                stats[row] = m; stats[PT_ROWS + row] = l;
+                group_sync(t);
+                if (row == 0) {
+                    __threadfence();
+                    unsigned *arrived = p.arrived + 2 * cut.c0 + t;
+                    const bool last = atomicAdd(arrived, 1u) == (unsigned)cut.parts - 1;
+                    if (last) { *arrived = 0; __threadfence(); }
+                    sh.last[t] = last;
+                }
+                group_sync(t);
+                if (sh.last[t]) {
+                    const float4 *all = reinterpret_cast<const float4 *>(p.partial);
+                    auto piece = [&](int i) { return all + (paged_slot(cut.c0 + i, cut.c0) * 2 + t) * (PT_ROWS * (HD + 2) / 4); };
+                    if (mine) {
+                        float top = -CUDART_INF_F, sum = 0.f;
+                        for (int i = 0; i < cut.parts; ++i) { top = fmaxf(top, __ldcg(reinterpret_cast<const float *>(piece(i) + PT_ROWS * HD / 4) + row)); }
+                        const float ref = top == -CUDART_INF_F ? 0.f : top;
+#pragma unroll 1
+                        for (int c8 = 0; c8 < HD / 32; ++c8) {
+                            float4 v[8];
+#pragma unroll
+                            for (int c = 0; c < 8; ++c) { v[c] = make_float4(0.f, 0.f, 0.f, 0.f); }
+                            sum = 0.f;
+                            for (int i = 0; i < cut.parts; ++i) {
+                                const float4 *from = piece(i);
+                                const float *st = reinterpret_cast<const float *>(from + PT_ROWS * HD / 4);
+                                const float f = exp2_fast(__ldcg(st + row) - ref);
+                                sum += f * __ldcg(st + PT_ROWS + row);
+#pragma unroll
+                                for (int c = 0; c < 8; ++c) {
+                                    const float4 u = __ldcg(from + (8 * c8 + c) * PT_ROWS + row);
+                                    v[c].x += f * u.x; v[c].y += f * u.y; v[c].z += f * u.z; v[c].w += f * u.w;
+                                }
+                            }
+                            const float inv_all = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
+                            for (int c = 0; c < 8; ++c) {
+                                const float4 u = make_float4(v[c].x * inv_all, v[c].y * inv_all, v[c].z * inv_all, v[c].w * inv_all);
+                                if (p.out_f32) { *reinterpret_cast<float4 *>(static_cast<float *>(p.out) + to_row + 32 * c8 + 4 * c) = u; }
+                                else { *reinterpret_cast<uint2 *>(static_cast<__half *>(p.out) + to_row + 32 * c8 + 4 * c) = make_uint2(pack_f16(u.x, u.y), pack_f16(u.z, u.w)); }
+                            }
+                        }
+                    }
+                }
+            }
+            ++stretch;
+            if (!more) { break; }
+        }
+    } else {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PT_REGS_OTHERS));
+        // K and V tiles take slots in turn: K of step 0, V of step 0, K of step 1, ...
+        uint32_t slot = 0, phase = 0;
+        auto advance = [&]() { if (++slot == SLOTS) { slot = 0; phase ^= 1; } };
+        if (warp == 9) {
+            // ------------------------------------------------------------------------------ copies
+            constexpr int halves = HD / 64;                                                 // a tile's boxes are 64 elements wide
+            uint32_t tiles = 0;
+            for (;;) {
+                x.describe(p, at);
+                const int32_t *table = p.view.page_table + (int64_t)x.seq * p.view.table_stride;
+                for (int step = x.off; step < x.off + x.todo; ++step) {
+                    if (!x.needed(step)) { continue; }
+                    const int j0 = x.it.lo + step * PT_KEYS;
+                    const int group = lane % 16 * 8, in_box = group & (box - 1);            // this lane's eight positions, their place in their box
+                    const int j = j0 + group;
+                    int page = p.view.n_pages, token = 0;
+                    if (j < x.it.hi) {
+                        const int e = table[j / p.view.page_size];
+                        if (e >= 0 && e < p.view.n_pages) { page = e; token = j % p.view.page_size; }
+                    }
+                    const uint32_t there = __ballot_sync(0xffffffffu, page < p.view.n_pages) & 0xffffu;
+#pragma unroll
+                    for (int kv = 0; kv < 2; ++kv) {
+                        mbar_wait_lean(empty + 8 * slot, phase ^ 1, limit);
+                        const uint32_t bar = full + 8 * slot, dst = ring + slot * Shape::OPERAND;
+                        if (lane == 0) {
+                            if (kv == 0) { sh.there[tiles & 7] = there; }
+                            mbar_expect_tx(bar, Shape::OPERAND);
+                        }
+                        __syncwarp();
+                        if (in_box == 0 && lane < 16 * halves) {
+                            const int half = lane >> 4;
+                            tma_load(dst + half * PT_HALF + group * 128, kv == 0 ? &k_map : &v_map, bar, half * 64, token, x.head, page);
+                        }
+                        __syncwarp();
+                        advance();
+                    }
+                    ++tiles;
+                }
+                if (!x.next(p, at)) { break; }
+            }
+            if (limit == 0) {   // something gave up: what is on its way lands before the CTA ends
+                uint64_t again = wait_limit;
+                for (int i = 0; i < SLOTS; ++i) {
+                    if (slot == 0) { slot = SLOTS; phase ^= 1; }
+                    --slot;
+                    if (2 * tiles > (uint32_t)i) { mbar_wait_lean(full + 8 * slot, phase, again); }
+                }
+            }
+        } else if (warp == 10) {
+            // ------------------------------------------------------------------------------ V tiles that not all rows see whole
+            uint32_t tiles = 0, stretch = 0;
+            for (;;) {
+                x.describe(p, at);
+                for (int step = x.off; step < x.off + x.todo; ++step) {
+                    if (!x.needed(step)) { continue; }
+                    advance();                                                               // (K)
+                    mbar_wait_lean(full + 8 * slot, phase, limit);
+                    const int j0 = x.it.lo + step * PT_KEYS;
+                    if (!(x.whole(p, 0, step) && (x.rows[1] == 0 || x.whole(p, 1, step)))) {
+                        const int first = p.causal && p.window > 0 ? max(0, x.pos_first[0] - p.window + 1) : 0;   // positions that some row sees
+                        uint32_t bad = 0;
+                        const uint32_t v_addr = ring + slot * Shape::OPERAND;
+#pragma unroll 4
+                        for (int i = 0; i < PT_KEYS * HD / 8 / 32; ++i) {
+                            const int piece = i * 32 + lane, r = (piece >> 3) & 127;         // (half, row, piece of the row)
+                            const uint32_t a = v_addr + piece * 16;
+                            uint4 v = lds128(a);
+                            if (j0 + r >= x.it.hi || j0 + r < first) { sts128(a, make_uint4(0, 0, 0, 0)); }
+                            else if (not_finite(v.x) | not_finite(v.y) | not_finite(v.z) | not_finite(v.w)) {
+                                uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) {
+                                    if ((w[e] & 0x7c00u) == 0x7c00u) { w[e] &= 0xffff0000u; }
+                                    if ((w[e] & 0x7c000000u) == 0x7c000000u) { w[e] &= 0xffffu; }
+                                }
+                                sts128(a, make_uint4(w[0], w[1], w[2], w[3]));
+                                bad = 1;
+                            }
+                        }
+                        if (__any_sync(0xffffffffu, bad) && lane == 0) { *reinterpret_cast<volatile int *>(&sh.poison[stretch & 7]) = (int)stretch + 1; }
+                        fence_async_smem();
+                    }
+                    __syncwarp();
+                    if (lane == 0) { mbar_arrive(clean + 8 * (tiles & 7)); }
+                    advance();
+                    ++tiles;
+                }
+                ++stretch;
+                if (!x.next(p, at)) { break; }
+            }
+        } else if (warp == 8) {
+            // ------------------------------------------------------------------------------ MMAs
+            constexpr uint32_t idesc_s = idesc_f16(PT_KEYS), idesc_o = idesc_f16(HD) | (1u << 16);   // (bit 16: B is MN-major)
+            uint32_t q_phase = 0, p_phase[2] = {0, 0};
+            uint32_t v_slot = 0, v_phase = 0, tiles = 0;
+            auto scores = [&](int t, uint32_t k_slot) {
+                if (elect_one()) {
+                    const uint64_t a = swizzled_desc(q_addr + t * Shape::OPERAND, 16), b = swizzled_desc(ring + k_slot * Shape::OPERAND, 16);
+#pragma unroll
+                    for (int k = 0; k < HD / 16; ++k) {
+                        const uint64_t step = ((k >> 2) * PT_HALF + (k & 3) * 32) >> 4;
+                        mma_f16_ss(tmem + t * PT_KEYS, a + step, b + step, idesc_s, k != 0);
+                    }
+                    mma_commit(s_ready + 8 * t);
+                }
+                __syncwarp();
+            };
+            for (;;) {
+                x.describe(p, at);
+#pragma unroll
+                for (int t = 0; t < 2; ++t) { mbar_wait_lean(q_ready + 8 * t, q_phase, limit); }
+                q_phase ^= 1;
+                tc_fence_after();
+                if (elect_one()) {
+#pragma unroll
+                    for (int t = 0; t < 2; ++t) { if (x.to[t] <= x.from[t]) { mma_commit(o_ready + 8 * t); } }
+                }
+                __syncwarp();
+                const int begin = min(x.to[0] > x.from[0] ? x.from[0] : 1 << 30, x.to[1] > x.from[1] ? x.from[1] : 1 << 30), end = max(x.to[0], x.to[1]);
+                for (int step = begin; step < end; ++step) {        // (the steps between are needed, all of them: the tiles' ranges overlap)
+                    if (step == begin) {
+                        mbar_wait_lean(full + 8 * slot, phase, limit);
+                        tc_fence_after();
+                        if (x.active(0, step)) { scores(0, slot); }
+                        if (x.active(1, step)) { scores(1, slot); }
+                        if (elect_one()) { mma_commit(empty + 8 * slot); }
+                        __syncwarp();
+                        advance();
+                    }
+                    v_slot = slot; v_phase = phase;
+                    advance();
+                    mbar_wait_lean(full + 8 * v_slot, v_phase, limit);
+                    mbar_wait_lean(clean + 8 * (tiles & 7), (tiles >> 3) & 1, limit);
+                    ++tiles;
+                    const bool ahead = step + 1 < end;
+                    if (ahead) { mbar_wait_lean(full + 8 * slot, phase, limit); }
+#pragma unroll
+                    for (int t = 0; t < 2; ++t) {
+                        if (x.active(t, step)) {
+                            mbar_wait_lean(p_ready + 8 * t, p_phase[t], limit);
+                            p_phase[t] ^= 1;
+                            tc_fence_after();
+                            if (elect_one()) {
+                                const uint64_t b = swizzled_desc(ring + v_slot * Shape::OPERAND, PT_HALF);
+#pragma unroll
+                                for (int k = 0; k < PT_KEYS / 16; ++k) {
+                                    mma_f16_ts(tmem + 2 * PT_KEYS + t * HD, tmem + t * PT_KEYS + 8 * k, b + ((k * 2048) >> 4), idesc_o, step != x.from[t] || k != 0);
+                                }
+                                if (step + 1 == x.to[t]) { mma_commit(o_ready + 8 * t); }
+                            }
+                            __syncwarp();
+                        }
+                        if (ahead && x.active(t, step + 1)) { scores(t, slot); }
+                    }
+                    if (elect_one()) {
+                        mma_commit(empty + 8 * v_slot);
+                        if (ahead) { mma_commit(empty + 8 * slot); }
+                    }
+                    __syncwarp();
+                    if (ahead) { advance(); }
+                }
+                if (!x.next(p, at)) { break; }
+            }
+        }
+    }
+    if (limit == 0 && lane == 0) { pf_report(error_flag, 7); }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 8) {
+        tc_fence_after();
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+    }
+}
+
+using EncodeTiled = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
+                                 CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeTiled encoder() {
+    static const EncodeTiled fn = [] {
+        void *f = nullptr;
+        cudaDriverEntryPointQueryResult found;
+        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &f, 12000, cudaEnableDefault, &found) != cudaSuccess || found != cudaDriverEntryPointSuccess) { cudaGetLastError(); f = nullptr; }
+        return reinterpret_cast<EncodeTiled>(f);
+    }();
+    return fn;
+}
+// pages of one pool: [page][head][position][element] whatever the order of the strides; boxes of `box` positions x 64 elements
+bool page_map(CUtensorMap *map, const __half *pool, const PagedView &v, int heads, int head_dim, int box) {
+    if (encoder() == nullptr) { return false; }
+    const cuuint64_t dims[4] = {(cuuint64_t)head_dim, (cuuint64_t)v.page_size, (cuuint64_t)heads, (cuuint64_t)v.n_pages};
+    const cuuint64_t strides[3] = {(cuuint64_t)v.token_stride * 2, (cuuint64_t)v.head_stride * 2, (cuuint64_t)v.page_stride * 2};
+    const cuuint32_t boxes[4] = {64, (cuuint32_t)box, 1, 1}, ones[4] = {1, 1, 1, 1};
+    return encoder()(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<__half *>(pool), dims, strides, boxes, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                     CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+// the warpgroups' registers after their split are what the block is launched with: fewer, and the split would wait for ever
+template <int HD> cudaError_t registers_suffice() {
+    static const cudaError_t answer = [] {
+        cudaFuncAttributes a;
+        const cudaError_t err = cudaFuncGetAttributes(&a, paged_tc_kernel<HD>);
+        return err != cudaSuccess ? err : a.numRegs * PT_THREADS >= 256 * PT_REGS_SOFTMAX + 128 * PT_REGS_OTHERS ? cudaSuccess : cudaErrorInvalidConfiguration;
+    }();
+    return answer;
+}
+template <int HD>
+cudaError_t launch_tc(const PagedAttention &p, const CUtensorMap &k, const CUtensorMap &v, int box, int sms, const LaunchCfg &cfg, uint64_t wait_limit) {
+    cudaError_t err = registers_suffice<HD>();
+    if (err != cudaSuccess) { return err; }
+    err = allow_dynamic_smem(reinterpret_cast<const void *>(paged_tc_kernel<HD>), TcShape<HD>::SMEM);
+    if (err != cudaSuccess) { return err; }
+    return launch_maybe_pdl(paged_tc_kernel<HD>, dim3(sms), PT_THREADS, TcShape<HD>::SMEM, cfg.stream, cfg.pdl, p, k, v, box, cfg.error_flag, wait_limit);
+}
+
+}  // namespace
+
+int paged_tc_box(int page_size) {   // positions of a box: the largest power of two up to 128 that divides the page size
+    int box = 1;
+    while (box < PT_KEYS && page_size % (2 * box) == 0) { box *= 2; }
+    return box;
+}
+bool paged_tc_can(const PagedView &v, int head_dim) {
+    return (head_dim == 64 || head_dim == 128) && paged_tc_box(v.page_size) >= 8 && v.token_stride > 0 && v.head_stride > 0 && v.page_stride > 0 &&
+           std::max({v.token_stride, v.head_stride, v.page_stride}) < (1ll << 38) && encoder() != nullptr;
+}
+cudaError_t launch_paged_attention_tc(const PagedAttention &p, int head_dim, int sms, const LaunchCfg &cfg, uint64_t wait_limit) {
+    CUtensorMap k, v;
+    const int box = paged_tc_box(p.view.page_size);
+    if (!page_map(&k, p.k, p.view, p.n_head_kv, head_dim, box) || !page_map(&v, p.v, p.view, p.n_head_kv, head_dim, box)) { return cudaErrorInvalidValue; }
+    return head_dim == 128 ? launch_tc<128>(p, k, v, box, sms, cfg, wait_limit) : launch_tc<64>(p, k, v, box, sms, cfg, wait_limit);
+}
+
+}  // namespace spyb
