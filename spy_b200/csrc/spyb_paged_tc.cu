@@ -34,6 +34,7 @@ struct TcShared {
     uint64_t full[8], empty[8];                          // a slot's copies have landed; its last MMA is done
     uint64_t clean[8];                                   // of the last V tiles: what nobody sees is cleared
     uint64_t q_ready[2], s_ready[2], p_ready[2], o_ready[2];
+    uint64_t passed[2];                                  // the MMAs have come to a stretch in which the tile sees nothing
     uint32_t tmem;
     uint32_t there[8];                                   // of the last tiles: which groups of eight positions are there
     int      poison[8];                                  // of the last stretches: a V tile that some rows see in part holds values that are not finite
@@ -67,6 +68,11 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t *r) {
 __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t *r) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};"
                  ::SPYB_I32(r), "r"(taddr) : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t *r) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};"
+                 ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]),
+                   "r"(r[15]), "r"(taddr) : "memory");
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ float max3(float a, float b, float c) { float d; asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c)); return d; }
@@ -123,10 +129,10 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const uint32_t base = (smem_u32(raw) + 1023) & ~1023u, q_addr = base, ring = base + 2 * Shape::OPERAND;
     const uint32_t full = smem_u32(sh.full), empty = smem_u32(sh.empty), clean = smem_u32(sh.clean);
-    const uint32_t q_ready = smem_u32(sh.q_ready), s_ready = smem_u32(sh.s_ready), p_ready = smem_u32(sh.p_ready), o_ready = smem_u32(sh.o_ready);
+    const uint32_t q_ready = smem_u32(sh.q_ready), s_ready = smem_u32(sh.s_ready), p_ready = smem_u32(sh.p_ready), o_ready = smem_u32(sh.o_ready), passed = smem_u32(sh.passed);
     if (tid == 0) {
         for (int i = 0; i < 8; ++i) { mbar_init(full + 8 * i, 1); mbar_init(empty + 8 * i, 1); mbar_init(clean + 8 * i, 1); sh.poison[i] = 0; }
-        for (int t = 0; t < 2; ++t) { mbar_init(q_ready + 8 * t, 4); mbar_init(s_ready + 8 * t, 1); mbar_init(p_ready + 8 * t, 4); mbar_init(o_ready + 8 * t, 1); }
+        for (int t = 0; t < 2; ++t) { mbar_init(q_ready + 8 * t, 4); mbar_init(s_ready + 8 * t, 1); mbar_init(p_ready + 8 * t, 4); mbar_init(o_ready + 8 * t, 1); mbar_init(passed + 8 * t, 1); }
         mbar_init_fence();
     }
     pdl_launch_dependents();
@@ -151,7 +157,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
         const uint32_t s_tmem = tmem + lanes + t * PT_KEYS, o_tmem = tmem + lanes + 2 * PT_KEYS + t * HD;
         const float scale = fabsf(p.scale_log2);
         const uint32_t flip = p.scale_log2 < 0.f ? 0x80008000u : 0u;                         // the scale's sign goes into Q
-        uint32_t s_phase = 0, o_phase = 0, tiles = 0, stretch = 0;
+        uint32_t s_phase = 0, o_phase = 0, passed_phase = 0, tiles = 0, stretch = 0;
         auto load_q = [&]() {
             // rows of this warp, two at a time (hd 64: four): 16-byte pieces into the swizzle
             constexpr int PIECES = HD / 8, AT_ONCE = 32 / PIECES;
@@ -183,23 +189,33 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
                 mbar_wait_lean(s_ready + 8 * t, s_phase, limit);
                 s_phase ^= 1;
                 tc_fence_after();
-                uint32_t s[128];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) { tmem_ld32(s_tmem + 32 * i, s + 32 * i); }
-                tmem_ld_wait();
+                // the row's scores, twice: for their maximum, and (two pieces of 32 in flight) for the powers. To keep all 128 costs registers that spill
+                uint32_t s[2][32];
+                float top = -CUDART_INF_F;
+                tmem_ld32(s_tmem, s[0]);
                 const uint32_t there = *reinterpret_cast<volatile uint32_t *>(&sh.there[(tiles - 1) & 7]);
-                if (!x.whole(p, t, step) || there != 0xffffu) {
-                    const int j0 = x.it.lo + step * PT_KEYS;
-                    const int c1 = (p.causal ? min(x.it.hi, pos + 1) : x.it.hi) - j0, c0 = p.causal && p.window > 0 ? pos - p.window + 1 - j0 : 0;
+                const bool plain = there == 0xffffu && x.whole(p, t, step);
+                const int j0 = x.it.lo + step * PT_KEYS;
+                const int c1 = (p.causal ? min(x.it.hi, pos + 1) : x.it.hi) - j0, c0 = p.causal && p.window > 0 ? pos - p.window + 1 - j0 : 0;
 #pragma unroll
-                    for (int c = 0; c < 128; ++c) {
-                        if (!(c >= c0 && c < c1 && ((there >> (c >> 3)) & 1))) { s[c] = 0xff800000u; }
+                for (int i = 0; i < 4; ++i) {
+                    uint32_t *v = s[i & 1];
+                    tmem_ld_wait();
+                    if (i < 3) { tmem_ld32(s_tmem + 32 * (i + 1), s[(i + 1) & 1]); }
+                    if (!plain) {
+#pragma unroll
+                        for (int c = 0; c < 32; ++c) {
+                            const int k = 32 * i + c;
+                            if (!(k >= c0 && k < c1 && ((there >> (k >> 3)) & 1))) { v[c] = 0xff800000u; }
+                        }
+                        tmem_st32(s_tmem + 32 * i, v);
                     }
-                }
-                float top = __uint_as_float(s[0]);
 #pragma unroll
-                for (int c = 1; c < 127; c += 2) { top = max3(top, __uint_as_float(s[c]), __uint_as_float(s[c + 1])); }
-                top = fmaxf(top, __uint_as_float(s[127])) * scale;
+                    for (int c = 0; c < 32; c += 2) { top = max3(top, __uint_as_float(v[c]), __uint_as_float(v[c + 1])); }
+                }
+                if (!plain) { tmem_st_wait(); }
+                tmem_ld32(s_tmem, s[0]);
+                top *= scale;
                 if (__any_sync(0xffffffffu, top > m + 8.f)) {
                     const float to = fmaxf(m, top), f = to == m ? 1.f : exp2_fast(m - to);
                     m = to; l *= f;
@@ -219,18 +235,20 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
                 const uint64_t neg2 = f2_pack(neg, neg), scale2 = f2_pack(scale, scale);
                 uint64_t sum[2] = {0, 0};
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    uint32_t h[32];
+                for (int i = 0; i < 4; ++i) {
+                    const uint32_t *v = s[i & 1];
+                    tmem_ld_wait();
+                    if (i < 3) { tmem_ld32(s_tmem + 32 * (i + 1), s[(i + 1) & 1]); }
+                    uint32_t h[16];
 #pragma unroll
-                    for (int c = 0; c < 32; ++c) {
-                        const int k = 64 * i + 2 * c;
+                    for (int c = 0; c < 16; ++c) {
                         float a, b;
-                        f2_unpack(f2_fma(f2_pack_bits(s[k], s[k + 1]), scale2, neg2), a, b);
+                        f2_unpack(f2_fma(f2_pack_bits(v[2 * c], v[2 * c + 1]), scale2, neg2), a, b);
                         a = exp2_fast(a); b = exp2_fast(b);
                         sum[c & 1] = f2_add(sum[c & 1], f2_pack(a, b));
                         h[c] = pack_f16(a, b);
                     }
-                    tmem_st32(s_tmem + 32 * i, h);
+                    tmem_st16(s_tmem + 16 * i, h);               // (over scores that are read)
                 }
                 float a, b;
                 f2_unpack(f2_add(sum[0], sum[1]), a, b);
@@ -244,11 +262,11 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
             const Stretch done = x;
             const PagedPlace was = at;
             const bool any = done.to[t] > done.from[t];
-            if (!any) { mbar_wait_lean(o_ready + 8 * t, o_phase, limit); }       // (so that nobody is two stretches ahead of the MMAs)
+            // nobody gets two stretches ahead of the MMAs (a barrier of its own: the O of the stretch before may not have been waited for yet)
+            if (!any) { mbar_wait_lean(passed + 8 * t, passed_phase, limit); passed_phase ^= 1; }
             const bool more = x.next(p, at);
             if (more) { x.describe(p, at); load_q(); }
-            if (any) { mbar_wait_lean(o_ready + 8 * t, o_phase, limit); tc_fence_after(); }
-            o_phase ^= 1;
+            if (any) { mbar_wait_lean(o_ready + 8 * t, o_phase, limit); o_phase ^= 1; tc_fence_after(); }
             const PagedCut cut = paged_cut(was, was.unit - done.off, done.it.units);
             float4 *part = reinterpret_cast<float4 *>(p.partial) + (paged_slot(blockIdx.x, cut.c0) * 2 + t) * (PT_ROWS * (HD + 2) / 4);     // [HD / 4][128] x 4, [128], [128]
             const float inv = cut.parts > 1 ? 1.f : l == 0.f ? 0.f : 1.f / l;
@@ -471,9 +489,9 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
                 for (int t = 0; t < 2; ++t) { mbar_wait_lean(q_ready + 8 * t, q_phase, limit); }
                 q_phase ^= 1;
                 tc_fence_after();
-                if (elect_one()) {
+                if (lane == 0) {
 #pragma unroll
-                    for (int t = 0; t < 2; ++t) { if (x.to[t] <= x.from[t]) { mma_commit(o_ready + 8 * t); } }
+                    for (int t = 0; t < 2; ++t) { if (x.to[t] <= x.from[t]) { mbar_arrive(passed + 8 * t); } }
                 }
                 __syncwarp();
                 const int begin = min(x.to[0] > x.from[0] ? x.from[0] : 1 << 30, x.to[1] > x.from[1] ? x.from[1] : 1 << 30), end = max(x.to[0], x.to[1]);

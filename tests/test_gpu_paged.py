@@ -243,6 +243,28 @@ def test_whole_chip_on_one_head_and_cut_items(be, dev):
     check_attention(be, dev, rng, [40], [9000], 2, 1, 128, 64)
 
 
+@pytest.mark.parametrize("hd", [64, 128])
+def test_items_with_one_tile_between_others(be, dev, hd):
+    """Many items a CTA, every other one with a second tile that has no rows or sees nothing: the order of the stretches' hand-overs, over and over."""
+    rng = np.random.default_rng(hd)
+    rows, n_kv, h = [300, 60, 513, 40, 300], [300, 700, 513, 40, 20], 40
+    starts = np.concatenate([[0], np.cumsum(rows)]).astype(np.int32)
+    pool = Pool(rng, n_kv, h, hd, 16, fill=0.0)
+    for s, n in enumerate(n_kv):
+        pool.put(s, *rng.standard_normal((2, n, h, hd)).astype(np.float16))
+    q = rng.standard_normal((starts[-1], h, hd)).astype(np.float16)
+    out = np.zeros(q.shape, dtype=np.float16)
+    po = dev(out)
+    d = B.paged_attention_desc(pool.cache(dev(pool.k), dev(pool.v)), B.paged_batch(dev(starts), dev(np.array(n_kv, np.int32)), dev(pool.table), 5, int(starts[-1]), pool.table.shape[1]), dev(q), po, h, window=200)
+    for _ in range(300):
+        be.paged_attention(d)
+    got = dev.back(po, out)
+    for s in (0, 2, 4):
+        k, v = (pool.get(a, s).astype(np.float64)[:, :2] for a in (pool.k, pool.v))
+        want, off = plain_attention(q[starts[s]:starts[s + 1], :2].astype(np.float64), k, v, n_kv[s] - rows[s], hd ** -0.5, True, 200, np.ones(n_kv[s], dtype=bool))
+        assert (np.abs(got[starts[s]:starts[s + 1], :2] - want) <= off + np.abs(want) * 2.0 ** -11 + 2.0 ** -25).all()
+
+
 def test_more_sequences_than_threads(be, dev):
     rng = np.random.default_rng(6)
     n = 700
