@@ -6,7 +6,7 @@
 // products run. K and V come page by page through tensor maps, in pieces of as many positions as divide the page size, into the 128-byte
 // swizzle of the operands: K row by row (K-major), V as it lies (its positions are the product's inner dimension: MN-major), no transposition anywhere.
 //   warps 0-3, 4-7   probabilities of tile 0 / 1, rescaling, output          warp 8   issues the MMAs
-//   warp 9           copies                                                   warp 10  clears and checks the V tiles that not all rows see whole
+//   warp 9           copies                                                   warps 10, 11  clear and check the V tiles that not all rows see whole
 // Probabilities are taken against a maximum that follows the true one when that is 2^8 above it: O is rescaled in the first steps and hardly ever after.
 
 #include <algorithm>
@@ -65,10 +65,6 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t *r) {
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
                  : SPYB_R32(r) : "r"(taddr) : "memory");
 }
-__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t *r) {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};"
-                 ::SPYB_I32(r), "r"(taddr) : "memory");
-}
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t *r) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};"
                  ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]),
@@ -81,35 +77,36 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) { uint32_t r; a
 __device__ __forceinline__ uint32_t not_finite(uint32_t h2) { return ((h2 & 0x7c007c00u) + 0x04000400u) & 0x80008000u; }
 __device__ __forceinline__ void group_sync(int t) { asm volatile("bar.sync %0, 128;" ::"r"(1 + t) : "memory"); }
 
-// One stretch of an item: positions [j0 x 128, j1 x 128) of its tiles' rows. Every role walks the same stretches.
+// One stretch of an item: `todo` steps of 128 positions from step `off` of the item on. Every role walks the same stretches.
+struct Tile {
+    int rows, pos_first, pos_last;                   // of 128 rows: how many there are, positions of the first and the last
+    int from, to;                                    // steps (of the item) in which it sees anything, within the stretch
+    // all rows see all positions of the step (if their pages are there)
+    __device__ __forceinline__ bool whole(const PagedAttention &p, const PagedItem &it, int step) const {
+        const int j = it.lo + step * PT_KEYS;
+        return j + PT_KEYS <= it.hi && (!p.causal || (j + PT_KEYS - 1 <= pos_first && (p.window <= 0 || j > pos_last - p.window)));
+    }
+};
 struct Stretch {
     PagedSeq  q;
     PagedItem it;
     int seq, head, tile, off, todo;
-    int rows[2], pos_first[2], pos_last[2];          // of the two tiles
-    int from[2], to[2];                              // 128-position steps (of the item) in which a tile sees anything, within this stretch
 
+    __device__ __forceinline__ Tile half(const PagedAttention &p, int t) const {
+        Tile h;
+        const int r0 = tile * PT_TILE + t * PT_ROWS;
+        h.rows = max(0, min(PT_ROWS, q.rows * p.group - r0));
+        h.pos_first = q.first + (int)((unsigned)r0 / (unsigned)p.group);
+        h.pos_last = q.first + (int)((unsigned)(r0 + max(h.rows, 1) - 1) / (unsigned)p.group);
+        const int hi = p.causal ? min(it.hi, h.pos_last + 1) : it.hi, lo = p.causal && p.window > 0 ? max(it.lo, h.pos_first - p.window + 1) : it.lo;
+        h.from = max(off, (max(lo, it.lo) - it.lo) / PT_KEYS);
+        h.to = h.rows == 0 || hi <= it.lo ? off : min(off + todo, (hi - it.lo + PT_KEYS - 1) / PT_KEYS);
+        if (h.to <= h.from) { h.from = h.to = off; }
+        return h;
+    }
     __device__ __forceinline__ void describe(const PagedAttention &p, const PagedPlace &at) {
         it = paged_item<PT_TILE, PT_KEYS, PT_KEYS>(p, q, tile);
         todo = (int)min((int64_t)(it.units - off), at.end - at.unit);
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-            const int r0 = tile * PT_TILE + t * PT_ROWS;
-            rows[t] = max(0, min(PT_ROWS, q.rows * p.group - r0));
-            pos_first[t] = q.first + (int)((unsigned)r0 / (unsigned)p.group);
-            pos_last[t] = q.first + (int)((unsigned)(r0 + max(rows[t], 1) - 1) / (unsigned)p.group);
-            const int hi = p.causal ? min(it.hi, pos_last[t] + 1) : it.hi, lo = p.causal && p.window > 0 ? max(it.lo, pos_first[t] - p.window + 1) : it.lo;
-            from[t] = max(off, (max(lo, it.lo) - it.lo) / PT_KEYS);
-            to[t] = rows[t] == 0 || hi <= it.lo ? off : min(off + todo, (hi - it.lo + PT_KEYS - 1) / PT_KEYS);
-            if (to[t] <= from[t]) { from[t] = to[t] = off; }
-        }
-    }
-    __device__ __forceinline__ bool active(int t, int step) const { return step >= from[t] && step < to[t]; }
-    __device__ __forceinline__ bool needed(int step) const { return active(0, step) || active(1, step); }
-    // all rows of tile t see all positions of the step (if their pages are there)
-    __device__ __forceinline__ bool whole(const PagedAttention &p, int t, int step) const {
-        const int j = it.lo + step * PT_KEYS;
-        return j + PT_KEYS <= it.hi && (!p.causal || (j + PT_KEYS - 1 <= pos_first[t] && (p.window <= 0 || j > pos_last[t] - p.window)));
     }
     __device__ __forceinline__ bool next(const PagedAttention &p, PagedPlace &at) {
         at.unit += todo;
@@ -118,6 +115,13 @@ struct Stretch {
         return paged_next<PT_TILE>(p, false, q, seq, head, tile);
     }
 };
+// steps in which either tile sees something: one run, for the second one's positions begin at the first one's end at the latest
+struct Steps { int begin, end; };
+__device__ __forceinline__ Steps steps_of(const Tile &a, const Tile &b) {
+    if (a.to <= a.from) { return {b.from, b.to}; }
+    if (b.to <= b.from) { return {a.from, a.to}; }
+    return {min(a.from, b.from), max(a.to, b.to)};
+}
 
 template <int HD>
 __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_constant__ PagedAttention p, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
@@ -131,7 +135,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
     const uint32_t full = smem_u32(sh.full), empty = smem_u32(sh.empty), clean = smem_u32(sh.clean);
     const uint32_t q_ready = smem_u32(sh.q_ready), s_ready = smem_u32(sh.s_ready), p_ready = smem_u32(sh.p_ready), o_ready = smem_u32(sh.o_ready), passed = smem_u32(sh.passed);
     if (tid == 0) {
-        for (int i = 0; i < 8; ++i) { mbar_init(full + 8 * i, 1); mbar_init(empty + 8 * i, 1); mbar_init(clean + 8 * i, 1); sh.poison[i] = 0; }
+        for (int i = 0; i < 8; ++i) { mbar_init(full + 8 * i, 1); mbar_init(empty + 8 * i, 1); mbar_init(clean + 8 * i, 2); sh.poison[i] = 0; }
         for (int t = 0; t < 2; ++t) { mbar_init(q_ready + 8 * t, 4); mbar_init(s_ready + 8 * t, 1); mbar_init(p_ready + 8 * t, 4); mbar_init(o_ready + 8 * t, 1); mbar_init(passed + 8 * t, 1); }
         mbar_init_fence();
     }
@@ -158,6 +162,13 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
         const float scale = fabsf(p.scale_log2);
         const uint32_t flip = p.scale_log2 < 0.f ? 0x80008000u : 0u;                         // the scale's sign goes into Q
         uint32_t s_phase = 0, o_phase = 0, passed_phase = 0, tiles = 0, stretch = 0;
+        Tile own;
+        Steps steps;
+        auto describe = [&]() {
+            x.describe(p, at);
+            own = x.half(p, t);
+            steps = steps_of(own, x.half(p, 1 - t));
+        };
         auto load_q = [&]() {
             // rows of this warp, two at a time (hd 64: four): 16-byte pieces into the swizzle
             constexpr int PIECES = HD / 8, AT_ONCE = 32 / PIECES;
@@ -165,7 +176,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
             for (int i = 0; i < 32 / AT_ONCE; ++i) {
                 const int r = (warp & 3) * 32 + i * AT_ONCE + lane / PIECES, c = lane % PIECES;
                 uint4 v = make_uint4(0, 0, 0, 0);
-                if (r < x.rows[t]) {
+                if (r < own.rows) {
                     const int pr = x.tile * PT_TILE + t * PT_ROWS + r, token = (int)((unsigned)pr / (unsigned)p.group), g = pr - token * p.group;
                     v = *reinterpret_cast<const uint4 *>(p.q + (int64_t)(x.q.row0 + token) * p.q_stride + (x.head * p.group + g) * HD + c * 8);
                     v.x ^= flip; v.y ^= flip; v.z ^= flip; v.w ^= flip;
@@ -176,58 +187,50 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
             __syncwarp();
             if (lane == 0) { mbar_arrive(q_ready + 8 * t); }
         };
-        x.describe(p, at);
+        describe();
         load_q();
         for (;;) {
             float m = -CUDART_INF_F, l = 0.f;
-            const int pr = x.tile * PT_TILE + t * PT_ROWS + min(row, max(x.rows[t], 1) - 1);
+            const int pr = x.tile * PT_TILE + t * PT_ROWS + min(row, max(own.rows, 1) - 1);
             const int token = (int)((unsigned)pr / (unsigned)p.group), g = pr - token * p.group, pos = x.q.first + token;
-            for (int step = x.off; step < x.off + x.todo; ++step) {
-                if (!x.needed(step)) { continue; }
-                ++tiles;
-                if (!x.active(t, step)) { continue; }
+            for (int step = own.from; step < own.to; ++step) {
                 mbar_wait_lean(s_ready + 8 * t, s_phase, limit);
                 s_phase ^= 1;
                 tc_fence_after();
-                // the row's scores, twice: for their maximum, and (two pieces of 32 in flight) for the powers. To keep all 128 costs registers that spill
-                uint32_t s[2][32];
-                float top = -CUDART_INF_F;
-                tmem_ld32(s_tmem, s[0]);
-                const uint32_t there = *reinterpret_cast<volatile uint32_t *>(&sh.there[(tiles - 1) & 7]);
-                const bool plain = there == 0xffffu && x.whole(p, t, step);
-                const int j0 = x.it.lo + step * PT_KEYS;
-                const int c1 = (p.causal ? min(x.it.hi, pos + 1) : x.it.hi) - j0, c0 = p.causal && p.window > 0 ? pos - p.window + 1 - j0 : 0;
+                uint32_t s[128];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    uint32_t *v = s[i & 1];
-                    tmem_ld_wait();
-                    if (i < 3) { tmem_ld32(s_tmem + 32 * (i + 1), s[(i + 1) & 1]); }
-                    if (!plain) {
+                for (int i = 0; i < 4; ++i) { tmem_ld32(s_tmem + 32 * i, s + 32 * i); }
+                const uint32_t there = *reinterpret_cast<volatile uint32_t *>(&sh.there[(tiles + step - steps.begin) & 7]);
+                tmem_ld_wait();
+                if (there != 0xffffu || !own.whole(p, x.it, step)) {
+                    const int j0 = x.it.lo + step * PT_KEYS;
+                    const int c1 = (p.causal ? min(x.it.hi, pos + 1) : x.it.hi) - j0, c0 = p.causal && p.window > 0 ? pos - p.window + 1 - j0 : 0;
 #pragma unroll
-                        for (int c = 0; c < 32; ++c) {
-                            const int k = 32 * i + c;
-                            if (!(k >= c0 && k < c1 && ((there >> (k >> 3)) & 1))) { v[c] = 0xff800000u; }
-                        }
-                        tmem_st32(s_tmem + 32 * i, v);
+                    for (int c = 0; c < 128; ++c) {
+                        if (!(c >= c0 && c < c1 && ((there >> (c >> 3)) & 1))) { s[c] = 0xff800000u; }
                     }
-#pragma unroll
-                    for (int c = 0; c < 32; c += 2) { top = max3(top, __uint_as_float(v[c]), __uint_as_float(v[c + 1])); }
                 }
-                if (!plain) { tmem_st_wait(); }
-                tmem_ld32(s_tmem, s[0]);
-                top *= scale;
+                float tops[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) { tops[i] = fmaxf(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])); }
+#pragma unroll
+                for (int c = 8; c < 128; c += 8) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) { tops[i] = max3(tops[i], __uint_as_float(s[c + 2 * i]), __uint_as_float(s[c + 2 * i + 1])); }
+                }
+                const float top = fmaxf(max3(tops[0], tops[1], tops[2]), tops[3]) * scale;
                 if (__any_sync(0xffffffffu, top > m + 8.f)) {
                     const float to = fmaxf(m, top), f = to == m ? 1.f : exp2_fast(m - to);
                     m = to; l *= f;
-                    if (step != x.from[t]) {
+                    if (step != own.from) {
 #pragma unroll 1
-                        for (int i = 0; i < HD / 32; ++i) {
-                            uint32_t o[32];
-                            tmem_ld32(o_tmem + 32 * i, o);
+                        for (int i = 0; i < HD / 16; ++i) {
+                            uint32_t o[16];
+                            tmem_ld16(o_tmem + 16 * i, o);
                             tmem_ld_wait();
 #pragma unroll
-                            for (int c = 0; c < 32; ++c) { o[c] = __float_as_uint(__uint_as_float(o[c]) * f); }
-                            tmem_st32(o_tmem + 32 * i, o);
+                            for (int c = 0; c < 16; ++c) { o[c] = __float_as_uint(__uint_as_float(o[c]) * f); }
+                            tmem_st16(o_tmem + 16 * i, o);
                         }
                     }
                 }
@@ -236,19 +239,16 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
                 uint64_t sum[2] = {0, 0};
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const uint32_t *v = s[i & 1];
-                    tmem_ld_wait();
-                    if (i < 3) { tmem_ld32(s_tmem + 32 * (i + 1), s[(i + 1) & 1]); }
                     uint32_t h[16];
 #pragma unroll
                     for (int c = 0; c < 16; ++c) {
                         float a, b;
-                        f2_unpack(f2_fma(f2_pack_bits(v[2 * c], v[2 * c + 1]), scale2, neg2), a, b);
+                        f2_unpack(f2_fma(f2_pack_bits(s[32 * i + 2 * c], s[32 * i + 2 * c + 1]), scale2, neg2), a, b);
                         a = exp2_fast(a); b = exp2_fast(b);
                         sum[c & 1] = f2_add(sum[c & 1], f2_pack(a, b));
                         h[c] = pack_f16(a, b);
                     }
-                    tmem_st16(s_tmem + 16 * i, h);               // (over scores that are read)
+                    tmem_st16(s_tmem + 16 * i, h);
                 }
                 float a, b;
                 f2_unpack(f2_add(sum[0], sum[1]), a, b);
@@ -258,19 +258,21 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
                 __syncwarp();
                 if (lane == 0) { mbar_arrive(p_ready + 8 * t); }
             }
+            tiles += steps.end - steps.begin;
             // this stretch's findings; the next one's Q goes first (all S of this one are there)
             const Stretch done = x;
+            const Tile done_own = own, done_other = x.half(p, 1 - t);
             const PagedPlace was = at;
-            const bool any = done.to[t] > done.from[t];
+            const bool any = own.to > own.from;
             // nobody gets two stretches ahead of the MMAs (a barrier of its own: the O of the stretch before may not have been waited for yet)
             if (!any) { mbar_wait_lean(passed + 8 * t, passed_phase, limit); passed_phase ^= 1; }
             const bool more = x.next(p, at);
-            if (more) { x.describe(p, at); load_q(); }
+            if (more) { describe(); load_q(); }
             if (any) { mbar_wait_lean(o_ready + 8 * t, o_phase, limit); o_phase ^= 1; tc_fence_after(); }
             const PagedCut cut = paged_cut(was, was.unit - done.off, done.it.units);
             float4 *part = reinterpret_cast<float4 *>(p.partial) + (paged_slot(blockIdx.x, cut.c0) * 2 + t) * (PT_ROWS * (HD + 2) / 4);     // [HD / 4][128] x 4, [128], [128]
             const float inv = cut.parts > 1 ? 1.f : l == 0.f ? 0.f : 1.f / l;
-            const bool mine = row < done.rows[t];
+            const bool mine = row < done_own.rows;
             const bool poisoned = any && *reinterpret_cast<volatile int *>(&sh.poison[stretch & 7]) == (int)stretch + 1;
             const int64_t to_row = (int64_t)(done.q.row0 + token) * p.out_stride + (done.head * p.group + g) * HD;
 #pragma unroll 1
@@ -283,8 +285,8 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
                 }
                 if (poisoned && mine) {
                     // values that are not finite were taken out of the V tiles that not all rows see whole: back to the rows that see them
-                    for (int step = done.from[t]; step < done.to[t]; ++step) {
-                        if (done.whole(p, 0, step) && done.whole(p, 1, step)) { continue; }
+                    for (int step = done_own.from; step < done_own.to; ++step) {
+                        if (done_own.whole(p, done.it, step) && done_other.whole(p, done.it, step)) { continue; }
                         const int j0 = done.it.lo + step * PT_KEYS, ja = max(j0, p.causal && p.window > 0 ? pos - p.window + 1 : 0), jb = min(j0 + PT_KEYS, p.causal ? min(done.it.hi, pos + 1) : done.it.hi);
                         for (int j = ja; j < jb; ++j) {
                             const int page = p.view.page_table[(int64_t)done.seq * p.view.table_stride + j / p.view.page_size];
@@ -381,21 +383,23 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
         if (warp == 9) {
             // ------------------------------------------------------------------------------ copies
             constexpr int halves = HD / 64;                                                 // a tile's boxes are 64 elements wide
+            const int group = lane % 16 * 8, half = lane >> 4;                              // this lane's eight positions of a tile, and half
+            const bool issues = (group & (box - 1)) == 0 && half < halves;
             uint32_t tiles = 0;
             for (;;) {
                 x.describe(p, at);
+                const Steps steps = steps_of(x.half(p, 0), x.half(p, 1));
                 const int32_t *table = p.view.page_table + (int64_t)x.seq * p.view.table_stride;
-                for (int step = x.off; step < x.off + x.todo; ++step) {
-                    if (!x.needed(step)) { continue; }
-                    const int j0 = x.it.lo + step * PT_KEYS;
-                    const int group = lane % 16 * 8, in_box = group & (box - 1);            // this lane's eight positions, their place in their box
-                    const int j = j0 + group;
-                    int page = p.view.n_pages, token = 0;
-                    if (j < x.it.hi) {
-                        const int e = table[j / p.view.page_size];
-                        if (e >= 0 && e < p.view.n_pages) { page = e; token = j % p.view.page_size; }
-                    }
-                    const uint32_t there = __ballot_sync(0xffffffffu, page < p.view.n_pages) & 0xffffu;
+                auto page_of = [&](int step) {                                              // (one step ahead: the table's latency is hidden)
+                    const int j = x.it.lo + step * PT_KEYS + group;
+                    return step < steps.end && j < x.it.hi ? table[j / p.view.page_size] : -1;
+                };
+                int e = page_of(steps.begin);
+                for (int step = steps.begin; step < steps.end; ++step) {
+                    const bool ok = e >= 0 && e < p.view.n_pages;
+                    const int page = ok ? e : p.view.n_pages, token = ok ? (x.it.lo + step * PT_KEYS + group) % p.view.page_size : 0;
+                    const uint32_t there = __ballot_sync(0xffffffffu, ok) & 0xffffu;
+                    e = page_of(step + 1);
 #pragma unroll
                     for (int kv = 0; kv < 2; ++kv) {
                         mbar_wait_lean(empty + 8 * slot, phase ^ 1, limit);
@@ -405,10 +409,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
                             mbar_expect_tx(bar, Shape::OPERAND);
                         }
                         __syncwarp();
-                        if (in_box == 0 && lane < 16 * halves) {
-                            const int half = lane >> 4;
-                            tma_load(dst + half * PT_HALF + group * 128, kv == 0 ? &k_map : &v_map, bar, half * 64, token, x.head, page);
-                        }
+                        if (issues) { tma_load(dst + half * PT_HALF + group * 128, kv == 0 ? &k_map : &v_map, bar, half * 64, token, x.head, page); }
                         __syncwarp();
                         advance();
                     }
@@ -424,38 +425,47 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
                     if (2 * tiles > (uint32_t)i) { mbar_wait_lean(full + 8 * slot, phase, again); }
                 }
             }
-        } else if (warp == 10) {
-            // ------------------------------------------------------------------------------ V tiles that not all rows see whole
+        } else if (warp >= 10) {
+            // ------------------------------------------------------------------------------ V tiles that not all rows see whole, half of the rows a warp
             uint32_t tiles = 0, stretch = 0;
+            const int r0 = (warp - 10) * (PT_KEYS / 2);
             for (;;) {
                 x.describe(p, at);
-                for (int step = x.off; step < x.off + x.todo; ++step) {
-                    if (!x.needed(step)) { continue; }
+                const Tile a = x.half(p, 0), b = x.half(p, 1);
+                const Steps steps = steps_of(a, b);
+                for (int step = steps.begin; step < steps.end; ++step) {
                     advance();                                                               // (K)
                     mbar_wait_lean(full + 8 * slot, phase, limit);
-                    const int j0 = x.it.lo + step * PT_KEYS;
-                    if (!(x.whole(p, 0, step) && (x.rows[1] == 0 || x.whole(p, 1, step)))) {
-                        const int first = p.causal && p.window > 0 ? max(0, x.pos_first[0] - p.window + 1) : 0;   // positions that some row sees
-                        uint32_t bad = 0;
+                    if (!(a.whole(p, x.it, step) && (b.rows == 0 || b.whole(p, x.it, step)))) {
+                        const int j0 = x.it.lo + step * PT_KEYS;
+                        const int first = p.causal && p.window > 0 ? max(0, a.pos_first - p.window + 1) - j0 : 0, end = x.it.hi - j0;   // rows that some query sees
                         const uint32_t v_addr = ring + slot * Shape::OPERAND;
-#pragma unroll 4
-                        for (int i = 0; i < PT_KEYS * HD / 8 / 32; ++i) {
-                            const int piece = i * 32 + lane, r = (piece >> 3) & 127;         // (half, row, piece of the row)
-                            const uint32_t a = v_addr + piece * 16;
-                            uint4 v = lds128(a);
-                            if (j0 + r >= x.it.hi || j0 + r < first) { sts128(a, make_uint4(0, 0, 0, 0)); }
-                            else if (not_finite(v.x) | not_finite(v.y) | not_finite(v.z) | not_finite(v.w)) {
+                        uint32_t bad = 0;
+                        auto piece = [&](int i) {                                            // (half, row, piece of the row)
+                            const int at = i * 32 + lane;
+                            return (at >> 9) * PT_HALF + r0 * 128 + (at & 511) * 16;
+                        };
+#pragma unroll 8
+                        for (int i = 0; i < PT_KEYS / 2 * HD / 8 / 32; ++i) {
+                            const int r = r0 + (((i * 32 + lane) & 511) >> 3);
+                            const uint4 v = lds128(v_addr + piece(i));
+                            if (r >= end || r < first) { sts128(v_addr + piece(i), make_uint4(0, 0, 0, 0)); }
+                            else { bad |= not_finite(v.x) | not_finite(v.y) | not_finite(v.z) | not_finite(v.w); }
+                        }
+                        if (__any_sync(0xffffffffu, bad)) {
+#pragma unroll 1
+                            for (int i = 0; i < PT_KEYS / 2 * HD / 8 / 32; ++i) {
+                                const uint4 v = lds128(v_addr + piece(i));
                                 uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
                                 for (int e = 0; e < 4; ++e) {
                                     if ((w[e] & 0x7c00u) == 0x7c00u) { w[e] &= 0xffff0000u; }
                                     if ((w[e] & 0x7c000000u) == 0x7c000000u) { w[e] &= 0xffffu; }
                                 }
-                                sts128(a, make_uint4(w[0], w[1], w[2], w[3]));
-                                bad = 1;
+                                sts128(v_addr + piece(i), make_uint4(w[0], w[1], w[2], w[3]));
                             }
+                            if (lane == 0) { *reinterpret_cast<volatile int *>(&sh.poison[stretch & 7]) = (int)stretch + 1; }
                         }
-                        if (__any_sync(0xffffffffu, bad) && lane == 0) { *reinterpret_cast<volatile int *>(&sh.poison[stretch & 7]) = (int)stretch + 1; }
                         fence_async_smem();
                     }
                     __syncwarp();
@@ -489,18 +499,20 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
                 for (int t = 0; t < 2; ++t) { mbar_wait_lean(q_ready + 8 * t, q_phase, limit); }
                 q_phase ^= 1;
                 tc_fence_after();
+                const Tile halves[2] = {x.half(p, 0), x.half(p, 1)};
+                const Steps steps = steps_of(halves[0], halves[1]);
+                auto active = [&](int t, int step) { return step >= halves[t].from && step < halves[t].to; };
                 if (lane == 0) {
 #pragma unroll
-                    for (int t = 0; t < 2; ++t) { if (x.to[t] <= x.from[t]) { mbar_arrive(passed + 8 * t); } }
+                    for (int t = 0; t < 2; ++t) { if (halves[t].to <= halves[t].from) { mbar_arrive(passed + 8 * t); } }
                 }
                 __syncwarp();
-                const int begin = min(x.to[0] > x.from[0] ? x.from[0] : 1 << 30, x.to[1] > x.from[1] ? x.from[1] : 1 << 30), end = max(x.to[0], x.to[1]);
-                for (int step = begin; step < end; ++step) {        // (the steps between are needed, all of them: the tiles' ranges overlap)
-                    if (step == begin) {
+                for (int step = steps.begin; step < steps.end; ++step) {
+                    if (step == steps.begin) {
                         mbar_wait_lean(full + 8 * slot, phase, limit);
                         tc_fence_after();
-                        if (x.active(0, step)) { scores(0, slot); }
-                        if (x.active(1, step)) { scores(1, slot); }
+                        if (active(0, step)) { scores(0, slot); }
+                        if (active(1, step)) { scores(1, slot); }
                         if (elect_one()) { mma_commit(empty + 8 * slot); }
                         __syncwarp();
                         advance();
@@ -510,11 +522,11 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
                     mbar_wait_lean(full + 8 * v_slot, v_phase, limit);
                     mbar_wait_lean(clean + 8 * (tiles & 7), (tiles >> 3) & 1, limit);
                     ++tiles;
-                    const bool ahead = step + 1 < end;
+                    const bool ahead = step + 1 < steps.end;
                     if (ahead) { mbar_wait_lean(full + 8 * slot, phase, limit); }
 #pragma unroll
                     for (int t = 0; t < 2; ++t) {
-                        if (x.active(t, step)) {
+                        if (active(t, step)) {
                             mbar_wait_lean(p_ready + 8 * t, p_phase[t], limit);
                             p_phase[t] ^= 1;
                             tc_fence_after();
@@ -522,13 +534,13 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
                                 const uint64_t b = swizzled_desc(ring + v_slot * Shape::OPERAND, PT_HALF);
 #pragma unroll
                                 for (int k = 0; k < PT_KEYS / 16; ++k) {
-                                    mma_f16_ts(tmem + 2 * PT_KEYS + t * HD, tmem + t * PT_KEYS + 8 * k, b + ((k * 2048) >> 4), idesc_o, step != x.from[t] || k != 0);
+                                    mma_f16_ts(tmem + 2 * PT_KEYS + t * HD, tmem + t * PT_KEYS + 8 * k, b + ((k * 2048) >> 4), idesc_o, step != halves[t].from || k != 0);
                                 }
-                                if (step + 1 == x.to[t]) { mma_commit(o_ready + 8 * t); }
+                                if (step + 1 == halves[t].to) { mma_commit(o_ready + 8 * t); }
                             }
                             __syncwarp();
                         }
-                        if (ahead && x.active(t, step + 1)) { scores(t, slot); }
+                        if (ahead && active(t, step + 1)) { scores(t, slot); }
                     }
                     if (elect_one()) {
                         mma_commit(empty + 8 * v_slot);
