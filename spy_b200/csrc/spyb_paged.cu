@@ -547,13 +547,15 @@ template <int TILE, int UNIT, int ALIGN> static int cut_selftest(uint32_t seed) 
         const int grid = 1 + rnd(300), least = 1 + rnd(4);
         for (int few = 0; few < 2; ++few) {
             PagedPlace at = {};
-            for (int s = 0; s < n_seq; ++s) { at.total += paged_seq_units<TILE, UNIT, ALIGN>(p, s, few) * p.n_head_kv; }
-            at.ctas = paged_ctas(at.total, grid, least);
-            if (at.total == 0) { continue; }
-            std::vector<uint8_t> seen((size_t)at.total), place((size_t)2 * at.ctas);
-            std::vector<int> arrived(at.ctas), wanted(at.ctas);
-            for (int c = 0; c < at.ctas; ++c) {
-                at.unit = paged_cta_unit(at.total, at.ctas, c); at.end = paged_cta_unit(at.total, at.ctas, c + 1);
+            int64_t total = 0;
+            for (int s = 0; s < n_seq; ++s) { total += paged_seq_units<TILE, UNIT, ALIGN>(p, s, few) * p.n_head_kv; }
+            if (total == 0) { continue; }
+            const int ctas = paged_ctas(total, grid, least);
+            at.share = paged_share(total, ctas);
+            std::vector<uint8_t> seen((size_t)total), place((size_t)2 * ctas);
+            std::vector<int> arrived(ctas), wanted(ctas);
+            for (int c = 0; c < ctas; ++c) {
+                at.unit = paged_cta_unit(at.share, c); at.end = paged_cta_unit(at.share, c + 1);
                 if (at.unit >= at.end) { return 1; }
                 int64_t rest = at.unit;
                 int s = 0;
@@ -572,7 +574,7 @@ template <int TILE, int UNIT, int ALIGN> static int cut_selftest(uint32_t seed) 
                     if (it.lo < 0 || it.lo % ALIGN != 0 || it.hi > p.view.n_kv_most || off >= it.units || (int64_t)it.units * UNIT + it.lo < it.hi) { return 4; }
                     const int todo = (int)std::min<int64_t>(it.units - off, at.end - at.unit);
                     const PagedCut cut = paged_cut(at, at.unit - off, it.units);
-                    if ((cut.parts == 1) != (todo == it.units) || cut.c0 < 0 || cut.c0 + cut.parts > at.ctas || c < cut.c0 || c >= cut.c0 + cut.parts) { return 5; }
+                    if ((cut.parts == 1) != (todo == it.units) || cut.c0 < 0 || cut.c0 + cut.parts > ctas || c < cut.c0 || c >= cut.c0 + cut.parts) { return 5; }
                     if (cut.parts > 1) {
                         if (place[(size_t)paged_slot(c, cut.c0)]++) { return 6; }
                         if ((c == cut.c0) != (off == 0)) { return 7; }
@@ -586,7 +588,7 @@ template <int TILE, int UNIT, int ALIGN> static int cut_selftest(uint32_t seed) 
                 }
             }
             for (uint8_t x : seen) { if (x != 1) { return 10; } }
-            for (int c = 0; c < at.ctas; ++c) { if (arrived[c] != wanted[c]) { return 11; } }
+            for (int c = 0; c < ctas; ++c) { if (arrived[c] != wanted[c]) { return 11; } }
         }
     }
     return 0;
@@ -659,7 +661,7 @@ spyb_status spyb_paged_attention(spyb_backend *be, const spyb_paged_attention_de
     const int64_t most = (int64_t)(d->batch.max_rows > 0 ? std::min(d->batch.max_rows, d->batch.n_rows) : d->batch.n_rows) * p.group;
     const LaunchCfg cfg = be->launch_cfg(be->config.use_pdl != 0);
     p.few_rows = 1 << 30;
-    if (most > PA_FEW_ROWS && paged_tc_can(p.view, hd)) {
+    if (most > PA_FEW_ROWS && scale >= 0.f && paged_tc_can(p.view, hd)) {
         p.few_rows = p.view.n_seq == 1 ? 0 : PA_FEW_ROWS;
         SPYB_CUDA(be, launch_paged_attention_tc(p, hd, be->num_sms_total, cfg, be->wait_limit_ns));
     }

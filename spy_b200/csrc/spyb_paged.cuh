@@ -77,10 +77,13 @@ __host__ __device__ __forceinline__ int64_t paged_seq_units(const PagedAttention
     return n;
 }
 
+__host__ __device__ __forceinline__ int64_t paged_div(int64_t a, int64_t b) {   // (a division of 64 bits costs some 100 instructions)
+    return ((a | b) >> 32) == 0 ? (int64_t)((uint32_t)a / (uint32_t)b) : a / b;
+}
 // unit `rest` of a sequence whose K/V heads have `one` units each
 template <int TILE, int UNIT, int ALIGN>
 __host__ __device__ __forceinline__ void paged_find(const PagedAttention &p, const PagedSeq &q, int64_t one, int64_t rest, int &head, int &tile, int &off) {
-    head = (int)(rest / one); rest -= head * one;
+    head = (int)paged_div(rest, one); rest -= head * one;
     for (tile = 0;; ++tile) {
         const int u = paged_item<TILE, UNIT, ALIGN>(p, q, tile).units;
         if (rest < u) { break; }
@@ -89,12 +92,20 @@ __host__ __device__ __forceinline__ void paged_find(const PagedAttention &p, con
     off = (int)rest;
 }
 
-struct PagedPlace { int seq, head, tile, off; int64_t unit, end, total; int ctas; };   // where a CTA begins, its first unit and the one behind its last
-struct PagedPlanShared { int64_t warp[32]; int64_t total; int seq, head, tile, off; };
-__host__ __device__ __forceinline__ int64_t paged_cta_unit(int64_t total, int ctas, int c) { return total * c / ctas; }
-__host__ __device__ __forceinline__ int paged_unit_cta(int64_t total, int ctas, int64_t u) { return (int)(((u + 1) * ctas - 1) / total); }
-
-__host__ __device__ __forceinline__ int paged_ctas(int64_t total, int grid, int least) { const int64_t n = total / least; return n < 1 ? 1 : n < grid ? (int)n : grid; }
+// All units cut into `ctas` stretches, the first `longer` of them one longer than the others
+struct PagedShare { int64_t total, each; int ctas, longer; };
+__host__ __device__ __forceinline__ PagedShare paged_share(int64_t total, int ctas) {
+    const int64_t each = paged_div(total, ctas);
+    return {total, each, ctas, (int)(total - each * ctas)};
+}
+__host__ __device__ __forceinline__ int64_t paged_cta_unit(const PagedShare &s, int c) { return s.each * c + pmin(c, s.longer); }
+__host__ __device__ __forceinline__ int paged_unit_cta(const PagedShare &s, int64_t u) {
+    const int64_t head = (s.each + 1) * s.longer;
+    return u < head ? (int)paged_div(u, s.each + 1) : s.longer + (int)paged_div(u - head, s.each);
+}
+struct PagedPlace { PagedShare share; int seq, head, tile, off; int64_t unit, end; };   // where a CTA begins, its first unit and the one behind its last
+struct PagedPlanShared { int64_t warp[32]; int seq, head, tile, off; };
+__host__ __device__ __forceinline__ int paged_ctas(int64_t total, int grid, int least) { const int64_t n = paged_div(total, least); return n < 1 ? 1 : n < grid ? (int)n : grid; }
 
 // all NT threads of the CTA; `least`: units that a CTA takes at least
 template <int NT, int TILE, int UNIT, int ALIGN>
@@ -113,12 +124,11 @@ __device__ PagedPlace paged_plan(const PagedAttention &p, bool few, int least, P
     total = 0;
     for (int w = 0; w < NW; ++w) { total += sh.warp[w]; }
     PagedPlace at;
-    at.total = total;
-    at.ctas = paged_ctas(total, gridDim.x, least);
+    at.share = paged_share(total, paged_ctas(total, gridDim.x, least));
     at.unit = at.end = 0; at.seq = at.head = at.tile = at.off = 0;
-    if (total == 0 || (int)blockIdx.x >= at.ctas) { return at; }
-    at.unit = paged_cta_unit(total, at.ctas, blockIdx.x);
-    at.end = paged_cta_unit(total, at.ctas, blockIdx.x + 1);
+    if (total == 0 || (int)blockIdx.x >= at.share.ctas) { return at; }
+    at.unit = paged_cta_unit(at.share, blockIdx.x);
+    at.end = paged_cta_unit(at.share, blockIdx.x + 1);
     int64_t before = 0;
     for (int base = 0; base < p.view.n_seq; base += NT) {
         const int s = base + tid;
@@ -133,7 +143,7 @@ __device__ PagedPlace paged_plan(const PagedAttention &p, bool few, int least, P
         const int64_t from = before + upto - mine;
         if (from <= at.unit && at.unit < from + mine) {
             sh.seq = s;
-            paged_find<TILE, UNIT, ALIGN>(p, paged_seq(p.view, s), mine / p.n_head_kv, at.unit - from, sh.head, sh.tile, sh.off);
+            paged_find<TILE, UNIT, ALIGN>(p, paged_seq(p.view, s), paged_div(mine, p.n_head_kv), at.unit - from, sh.head, sh.tile, sh.off);
         }
         before += all;
         if (at.unit < before) { break; }   // (the same for all threads)
@@ -161,7 +171,7 @@ __host__ __device__ __forceinline__ bool paged_next(const PagedAttention &p, boo
 // stretch (place 1), every other one's the first of its own (place 0).
 struct PagedCut { int c0, parts; };
 __host__ __device__ __forceinline__ PagedCut paged_cut(const PagedPlace &at, int64_t item_begin, int units) {
-    const int a = paged_unit_cta(at.total, at.ctas, item_begin), b = paged_unit_cta(at.total, at.ctas, item_begin + units - 1);
+    const int a = paged_unit_cta(at.share, item_begin), b = paged_unit_cta(at.share, item_begin + units - 1);
     return {a, b - a + 1};
 }
 __host__ __device__ __forceinline__ int64_t paged_slot(int c, int c0) { return 2 * (int64_t)c + (c == c0 ? 1 : 0); }

@@ -33,8 +33,7 @@ template <int HD> struct TcShape {
 struct TcShared {
     uint64_t full[8], empty[8];                          // a slot's copies have landed; its last MMA is done
     uint64_t clean[8];                                   // of the last V tiles: what nobody sees is cleared
-    uint64_t q_ready[2], s_ready[2], p_ready[2], o_ready[2];
-    uint64_t passed[2];                                  // the MMAs have come to a stretch in which the tile sees nothing
+    uint64_t q_ready[2], q_free[2], s_ready[2], p_ready[2], o_ready[2];   // of the two tiles, in stretches in which they see anything
     uint32_t tmem;
     uint32_t there[8];                                   // of the last tiles: which groups of eight positions are there
     int      poison[8];                                  // of the last stretches: a V tile that some rows see in part holds values that are not finite
@@ -133,10 +132,10 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const uint32_t base = (smem_u32(raw) + 1023) & ~1023u, q_addr = base, ring = base + 2 * Shape::OPERAND;
     const uint32_t full = smem_u32(sh.full), empty = smem_u32(sh.empty), clean = smem_u32(sh.clean);
-    const uint32_t q_ready = smem_u32(sh.q_ready), s_ready = smem_u32(sh.s_ready), p_ready = smem_u32(sh.p_ready), o_ready = smem_u32(sh.o_ready), passed = smem_u32(sh.passed);
+    const uint32_t q_ready = smem_u32(sh.q_ready), s_ready = smem_u32(sh.s_ready), p_ready = smem_u32(sh.p_ready), o_ready = smem_u32(sh.o_ready), q_free = smem_u32(sh.q_free);
     if (tid == 0) {
         for (int i = 0; i < 8; ++i) { mbar_init(full + 8 * i, 1); mbar_init(empty + 8 * i, 1); mbar_init(clean + 8 * i, 2); sh.poison[i] = 0; }
-        for (int t = 0; t < 2; ++t) { mbar_init(q_ready + 8 * t, 4); mbar_init(s_ready + 8 * t, 1); mbar_init(p_ready + 8 * t, 4); mbar_init(o_ready + 8 * t, 1); mbar_init(passed + 8 * t, 1); }
+        for (int t = 0; t < 2; ++t) { mbar_init(q_ready + 8 * t, 1); mbar_init(q_free + 8 * t, 1); mbar_init(s_ready + 8 * t, 1); mbar_init(p_ready + 8 * t, 4); mbar_init(o_ready + 8 * t, 1); }
         mbar_init_fence();
     }
     pdl_launch_dependents();
@@ -159,9 +158,8 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
         const int t = warp >> 2, row = tid & 127;
         const uint32_t lanes = (uint32_t)(warp & 3) << 21;                                   // (32 lanes a warp, in the address's upper half)
         const uint32_t s_tmem = tmem + lanes + t * PT_KEYS, o_tmem = tmem + lanes + 2 * PT_KEYS + t * HD;
-        const float scale = fabsf(p.scale_log2);
-        const uint32_t flip = p.scale_log2 < 0.f ? 0x80008000u : 0u;                         // the scale's sign goes into Q
-        uint32_t s_phase = 0, o_phase = 0, passed_phase = 0, tiles = 0, stretch = 0;
+        const float scale = p.scale_log2;
+        uint32_t s_phase = 0, o_phase = 0, tiles = 0, stretch = 0;
         Tile own;
         Steps steps;
         auto describe = [&]() {
@@ -169,26 +167,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
             own = x.half(p, t);
             steps = steps_of(own, x.half(p, 1 - t));
         };
-        auto load_q = [&]() {
-            // rows of this warp, two at a time (hd 64: four): 16-byte pieces into the swizzle
-            constexpr int PIECES = HD / 8, AT_ONCE = 32 / PIECES;
-#pragma unroll 4
-            for (int i = 0; i < 32 / AT_ONCE; ++i) {
-                const int r = (warp & 3) * 32 + i * AT_ONCE + lane / PIECES, c = lane % PIECES;
-                uint4 v = make_uint4(0, 0, 0, 0);
-                if (r < own.rows) {
-                    const int pr = x.tile * PT_TILE + t * PT_ROWS + r, token = (int)((unsigned)pr / (unsigned)p.group), g = pr - token * p.group;
-                    v = *reinterpret_cast<const uint4 *>(p.q + (int64_t)(x.q.row0 + token) * p.q_stride + (x.head * p.group + g) * HD + c * 8);
-                    v.x ^= flip; v.y ^= flip; v.z ^= flip; v.w ^= flip;
-                }
-                sts128(q_addr + t * Shape::OPERAND + (c >> 3) * PT_HALF + r * 128 + (((c & 7) ^ (r & 7)) << 4), v);
-            }
-            fence_async_smem();
-            __syncwarp();
-            if (lane == 0) { mbar_arrive(q_ready + 8 * t); }
-        };
         describe();
-        load_q();
         for (;;) {
             float m = -CUDART_INF_F, l = 0.f;
             const int pr = x.tile * PT_TILE + t * PT_ROWS + min(row, max(own.rows, 1) - 1);
@@ -210,16 +189,50 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
                         if (!(c >= c0 && c < c1 && ((there >> (c >> 3)) & 1))) { s[c] = 0xff800000u; }
                     }
                 }
-                float tops[4];
+                float tops[4], top;
+                auto largest = [&](int i) {                   // of columns 32 i .. 32 i + 31
 #pragma unroll
-                for (int i = 0; i < 4; ++i) { tops[i] = fmaxf(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])); }
+                    for (int c = 0; c < 32; c += 8) {
 #pragma unroll
-                for (int c = 8; c < 128; c += 8) {
+                        for (int e = 0; e < 4; ++e) { tops[e] = max3(tops[e], __uint_as_float(s[32 * i + c + 2 * e]), __uint_as_float(s[32 * i + c + 2 * e + 1])); }
+                    }
+                };
+                auto powers = [&](bool also_largest) {        // the row's probabilities against m, into tensor memory; their sum
+                    const float neg = m == -CUDART_INF_F ? 0.f : -m;
+                    const uint64_t neg2 = f2_pack(neg, neg), scale2 = f2_pack(scale, scale);
+                    uint64_t sum[2] = {0, 0};
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) { tops[i] = max3(tops[i], __uint_as_float(s[c + 2 * i]), __uint_as_float(s[c + 2 * i + 1])); }
+                    for (int i = 0; i < 4; ++i) {
+                        uint32_t h[16];
+#pragma unroll
+                        for (int c = 0; c < 16; ++c) {
+                            float a, b;
+                            f2_unpack(f2_fma(f2_pack_bits(s[32 * i + 2 * c], s[32 * i + 2 * c + 1]), scale2, neg2), a, b);
+                            a = exp2_fast(a); b = exp2_fast(b);
+                            sum[c & 1] = f2_add(sum[c & 1], f2_pack(a, b));
+                            h[c] = pack_f16(a, b);
+                        }
+                        tmem_st16(s_tmem + 16 * i, h);
+                        if (also_largest) { largest(i); }
+                    }
+                    float a, b;
+                    f2_unpack(f2_add(sum[0], sum[1]), a, b);
+                    return a + b;
+                };
+                tops[0] = tops[1] = tops[2] = tops[3] = -CUDART_INF_F;
+                bool again = step == own.from;
+                if (!again) {
+                    // the maximum of the steps before does, nearly always: powers at once, and whether it did
+                    const float sum = powers(true);
+                    top = fmaxf(max3(tops[0], tops[1], tops[2]), tops[3]) * scale;
+                    again = __any_sync(0xffffffffu, top > m + 8.f);
+                    if (!again) { l += sum; }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) { largest(i); }
+                    top = fmaxf(max3(tops[0], tops[1], tops[2]), tops[3]) * scale;
                 }
-                const float top = fmaxf(max3(tops[0], tops[1], tops[2]), tops[3]) * scale;
-                if (__any_sync(0xffffffffu, top > m + 8.f)) {
+                if (again) {
                     const float to = fmaxf(m, top), f = to == m ? 1.f : exp2_fast(m - to);
                     m = to; l *= f;
                     if (step != own.from) {
@@ -233,41 +246,21 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
                             tmem_st16(o_tmem + 16 * i, o);
                         }
                     }
+                    l += powers(false);
                 }
-                const float neg = m == -CUDART_INF_F ? 0.f : -m;
-                const uint64_t neg2 = f2_pack(neg, neg), scale2 = f2_pack(scale, scale);
-                uint64_t sum[2] = {0, 0};
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    uint32_t h[16];
-#pragma unroll
-                    for (int c = 0; c < 16; ++c) {
-                        float a, b;
-                        f2_unpack(f2_fma(f2_pack_bits(s[32 * i + 2 * c], s[32 * i + 2 * c + 1]), scale2, neg2), a, b);
-                        a = exp2_fast(a); b = exp2_fast(b);
-                        sum[c & 1] = f2_add(sum[c & 1], f2_pack(a, b));
-                        h[c] = pack_f16(a, b);
-                    }
-                    tmem_st16(s_tmem + 16 * i, h);
-                }
-                float a, b;
-                f2_unpack(f2_add(sum[0], sum[1]), a, b);
-                l += a + b;
                 tmem_st_wait();
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) { mbar_arrive(p_ready + 8 * t); }
             }
             tiles += steps.end - steps.begin;
-            // this stretch's findings; the next one's Q goes first (all S of this one are there)
+            // this stretch's findings
             const Stretch done = x;
             const Tile done_own = own, done_other = x.half(p, 1 - t);
             const PagedPlace was = at;
             const bool any = own.to > own.from;
-            // nobody gets two stretches ahead of the MMAs (a barrier of its own: the O of the stretch before may not have been waited for yet)
-            if (!any) { mbar_wait_lean(passed + 8 * t, passed_phase, limit); passed_phase ^= 1; }
             const bool more = x.next(p, at);
-            if (more) { describe(); load_q(); }
+            if (more) { describe(); }
             if (any) { mbar_wait_lean(o_ready + 8 * t, o_phase, limit); o_phase ^= 1; tc_fence_after(); }
             const PagedCut cut = paged_cut(was, was.unit - done.off, done.it.units);
             float4 *part = reinterpret_cast<float4 *>(p.partial) + (paged_slot(blockIdx.x, cut.c0) * 2 + t) * (PT_ROWS * (HD + 2) / 4);     // [HD / 4][128] x 4, [128], [128]
@@ -342,32 +335,33 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
                     auto piece = [&](int i) { return all + (paged_slot(cut.c0 + i, cut.c0) * 2 + t) * (PT_ROWS * (HD + 2) / 4); };
                     if (mine) {
                         float top = -CUDART_INF_F, sum = 0.f;
+#pragma unroll 4
                         for (int i = 0; i < cut.parts; ++i) { top = fmaxf(top, __ldcg(reinterpret_cast<const float *>(piece(i) + PT_ROWS * HD / 4) + row)); }
                         const float ref = top == -CUDART_INF_F ? 0.f : top;
+                        float4 v[HD / 4];
+#pragma unroll
+                        for (int c = 0; c < HD / 4; ++c) { v[c] = make_float4(0.f, 0.f, 0.f, 0.f); }
 #pragma unroll 1
-                        for (int c8 = 0; c8 < HD / 32; ++c8) {
-                            float4 v[8];
+                        for (int i = 0; i < cut.parts; ++i) {
+                            const float4 *from = piece(i);
+                            const float *st = reinterpret_cast<const float *>(from + PT_ROWS * HD / 4);
+                            const float f = exp2_fast(__ldcg(st + row) - ref);
+                            sum += f * __ldcg(st + PT_ROWS + row);
 #pragma unroll
-                            for (int c = 0; c < 8; ++c) { v[c] = make_float4(0.f, 0.f, 0.f, 0.f); }
-                            sum = 0.f;
-                            for (int i = 0; i < cut.parts; ++i) {
-                                const float4 *from = piece(i);
-                                const float *st = reinterpret_cast<const float *>(from + PT_ROWS * HD / 4);
-                                const float f = exp2_fast(__ldcg(st + row) - ref);
-                                sum += f * __ldcg(st + PT_ROWS + row);
-#pragma unroll
-                                for (int c = 0; c < 8; ++c) {
-                                    const float4 u = __ldcg(from + (8 * c8 + c) * PT_ROWS + row);
-                                    v[c].x += f * u.x; v[c].y += f * u.y; v[c].z += f * u.z; v[c].w += f * u.w;
-                                }
+                            for (int c = 0; c < HD / 4; ++c) {
+                                const float4 u = __ldcg(from + c * PT_ROWS + row);
+                                v[c].x += f * u.x; v[c].y += f * u.y; v[c].z += f * u.z; v[c].w += f * u.w;
                             }
-                            const float inv_all = sum == 0.f ? 0.f : 1.f / sum;
+                        }
+                        const float inv_all = sum == 0.f ? 0.f : 1.f / sum;
 #pragma unroll
-                            for (int c = 0; c < 8; ++c) {
-                                const float4 u = make_float4(v[c].x * inv_all, v[c].y * inv_all, v[c].z * inv_all, v[c].w * inv_all);
-                                if (p.out_f32) { *reinterpret_cast<float4 *>(static_cast<float *>(p.out) + to_row + 32 * c8 + 4 * c) = u; }
-                                else { *reinterpret_cast<uint2 *>(static_cast<__half *>(p.out) + to_row + 32 * c8 + 4 * c) = make_uint2(pack_f16(u.x, u.y), pack_f16(u.z, u.w)); }
-                            }
+                        for (int c = 0; c < HD / 4; c += 2) {
+                            const float4 a = make_float4(v[c].x * inv_all, v[c].y * inv_all, v[c].z * inv_all, v[c].w * inv_all);
+                            const float4 b = make_float4(v[c + 1].x * inv_all, v[c + 1].y * inv_all, v[c + 1].z * inv_all, v[c + 1].w * inv_all);
+                            if (p.out_f32) {
+                                float4 *dst = reinterpret_cast<float4 *>(static_cast<float *>(p.out) + to_row + 4 * c);
+                                dst[0] = a; dst[1] = b;
+                            } else { *reinterpret_cast<uint4 *>(static_cast<__half *>(p.out) + to_row + 4 * c) = make_uint4(pack_f16(a.x, a.y), pack_f16(a.z, a.w), pack_f16(b.x, b.y), pack_f16(b.z, b.w)); }
                         }
                     }
                 }
@@ -426,13 +420,36 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
                 }
             }
         } else if (warp >= 10) {
-            // ------------------------------------------------------------------------------ V tiles that not all rows see whole, half of the rows a warp
-            uint32_t tiles = 0, stretch = 0;
-            const int r0 = (warp - 10) * (PT_KEYS / 2);
+            // ------------------------------------------------------------------------------ Q of a tile each; V tiles that not all rows see whole, half of the rows each
+            uint32_t tiles = 0, stretch = 0, q_phase = 1;
+            const int t = warp - 10;
+            const int v_row0 = t * (PT_KEYS / 2);
             for (;;) {
                 x.describe(p, at);
                 const Tile a = x.half(p, 0), b = x.half(p, 1);
                 const Steps steps = steps_of(a, b);
+                if (t == 0 ? a.to > a.from : b.to > b.from) {
+                    mbar_wait_lean(q_free + 8 * t, q_phase, limit);
+                    q_phase ^= 1;
+                    constexpr int PIECES = HD / 8, AT_ONCE = 32 / PIECES;                    // pieces of 16 bytes of a row, rows at once
+                    const int rows = t == 0 ? a.rows : b.rows, c = lane % PIECES;
+                    const unsigned r0 = (unsigned)(x.tile * PT_TILE + t * PT_ROWS + lane / PIECES), group = (unsigned)p.group;
+                    int token = (int)(r0 / group), g = (int)(r0 - (unsigned)token * group);
+                    const int more_tokens = AT_ONCE / p.group, more_heads = AT_ONCE - more_tokens * p.group;
+                    const __half *src = p.q + (int64_t)x.q.row0 * p.q_stride + x.head * p.group * HD + c * 8;
+#pragma unroll 4
+                    for (int r = lane / PIECES; r < PT_ROWS; r += AT_ONCE) {
+                        const bool in = r < rows;
+                        const uint32_t dst = q_addr + t * Shape::OPERAND + (c >> 3) * PT_HALF + r * 128 + (((c & 7) ^ (r & 7)) << 4);
+                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(in ? src + token * p.q_stride + g * HD : p.q), "r"(in ? 16 : 0) : "memory");
+                        token += more_tokens; g += more_heads;
+                        if (g >= p.group) { g -= p.group; ++token; }
+                    }
+                    asm volatile("cp.async.wait_all;" ::: "memory");
+                    fence_async_smem();
+                    __syncwarp();
+                    if (lane == 0) { mbar_arrive(q_ready + 8 * t); }
+                }
                 for (int step = steps.begin; step < steps.end; ++step) {
                     advance();                                                               // (K)
                     mbar_wait_lean(full + 8 * slot, phase, limit);
@@ -443,11 +460,11 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
                         uint32_t bad = 0;
                         auto piece = [&](int i) {                                            // (half, row, piece of the row)
                             const int at = i * 32 + lane;
-                            return (at >> 9) * PT_HALF + r0 * 128 + (at & 511) * 16;
+                            return (at >> 9) * PT_HALF + v_row0 * 128 + (at & 511) * 16;
                         };
 #pragma unroll 8
                         for (int i = 0; i < PT_KEYS / 2 * HD / 8 / 32; ++i) {
-                            const int r = r0 + (((i * 32 + lane) & 511) >> 3);
+                            const int r = v_row0 + (((i * 32 + lane) & 511) >> 3);
                             const uint4 v = lds128(v_addr + piece(i));
                             if (r >= end || r < first) { sts128(v_addr + piece(i), make_uint4(0, 0, 0, 0)); }
                             else { bad |= not_finite(v.x) | not_finite(v.y) | not_finite(v.z) | not_finite(v.w); }
@@ -479,9 +496,9 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
         } else if (warp == 8) {
             // ------------------------------------------------------------------------------ MMAs
             constexpr uint32_t idesc_s = idesc_f16(PT_KEYS), idesc_o = idesc_f16(HD) | (1u << 16);   // (bit 16: B is MN-major)
-            uint32_t q_phase = 0, p_phase[2] = {0, 0};
+            uint32_t q_phase[2] = {0, 0}, p_phase[2] = {0, 0};
             uint32_t v_slot = 0, v_phase = 0, tiles = 0;
-            auto scores = [&](int t, uint32_t k_slot) {
+            auto scores = [&](int t, uint32_t k_slot, bool last) {
                 if (elect_one()) {
                     const uint64_t a = swizzled_desc(q_addr + t * Shape::OPERAND, 16), b = swizzled_desc(ring + k_slot * Shape::OPERAND, 16);
 #pragma unroll
@@ -490,29 +507,26 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
                         mma_f16_ss(tmem + t * PT_KEYS, a + step, b + step, idesc_s, k != 0);
                     }
                     mma_commit(s_ready + 8 * t);
+                    if (last) { mma_commit(q_free + 8 * t); }
                 }
                 __syncwarp();
             };
             for (;;) {
                 x.describe(p, at);
-#pragma unroll
-                for (int t = 0; t < 2; ++t) { mbar_wait_lean(q_ready + 8 * t, q_phase, limit); }
-                q_phase ^= 1;
-                tc_fence_after();
                 const Tile halves[2] = {x.half(p, 0), x.half(p, 1)};
                 const Steps steps = steps_of(halves[0], halves[1]);
                 auto active = [&](int t, int step) { return step >= halves[t].from && step < halves[t].to; };
-                if (lane == 0) {
 #pragma unroll
-                    for (int t = 0; t < 2; ++t) { if (halves[t].to <= halves[t].from) { mbar_arrive(passed + 8 * t); } }
+                for (int t = 0; t < 2; ++t) {
+                    if (halves[t].to > halves[t].from) { mbar_wait_lean(q_ready + 8 * t, q_phase[t], limit); q_phase[t] ^= 1; }
                 }
-                __syncwarp();
+                tc_fence_after();
                 for (int step = steps.begin; step < steps.end; ++step) {
                     if (step == steps.begin) {
                         mbar_wait_lean(full + 8 * slot, phase, limit);
                         tc_fence_after();
-                        if (active(0, step)) { scores(0, slot); }
-                        if (active(1, step)) { scores(1, slot); }
+                        if (active(0, step)) { scores(0, slot, step + 1 == halves[0].to); }
+                        if (active(1, step)) { scores(1, slot, step + 1 == halves[1].to); }
                         if (elect_one()) { mma_commit(empty + 8 * slot); }
                         __syncwarp();
                         advance();
@@ -540,7 +554,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
                             }
                             __syncwarp();
                         }
-                        if (ahead && active(t, step + 1)) { scores(t, slot); }
+                        if (ahead && active(t, step + 1)) { scores(t, slot, step + 2 == halves[t].to); }
                     }
                     if (elect_one()) {
                         mma_commit(empty + 8 * v_slot);
