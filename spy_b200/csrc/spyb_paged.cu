@@ -145,12 +145,12 @@ __global__ void __launch_bounds__(PR_WARPS * 32) paged_rows_kernel(const __grid_
     const uint32_t ring = smem_u32(smem) + warp * PR_STAGES * STAGE;
     pdl_launch_dependents();
     pdl_wait();
-    PagedPlace at = paged_plan<NT, TILE, PR_UNIT, PR_BLOCK>(p, true, 1, plan);
+    PagedPlace at = paged_plan<NT, PR_UNIT, PR_BLOCK>(p, true, 1, plan);
     if (at.unit >= at.end) { return; }
     PagedSeq q = paged_seq(p.view, at.seq);
     int seq = at.seq, head = at.head, tile = at.tile, off = at.off;
     for (;;) {
-        const PagedItem it = paged_item<TILE, PR_UNIT, PR_BLOCK>(p, q, tile);
+        const PagedItem it = paged_item<PR_UNIT, PR_BLOCK>(p, q, tile);
         const int todo = (int)min((int64_t)(it.units - off), at.end - at.unit);
         const int ka = it.lo + off * PR_UNIT, kb = min(it.hi, ka + todo * PR_UNIT);
         const int n_block = kb > ka ? (kb - ka + PR_BLOCK - 1) / PR_BLOCK : 0;
@@ -423,7 +423,7 @@ __global__ void __launch_bounds__(PR_WARPS * 32) paged_rows_kernel(const __grid_
         at.unit += todo;
         if (at.unit >= at.end) { return; }
         off = 0;
-        if (!paged_next<TILE>(p, true, q, seq, head, tile)) { return; }
+        if (!paged_next(p, true, q, seq, head, tile)) { return; }
         __syncthreads();   // (the ring takes the findings' place again)
     }
 }
@@ -533,7 +533,7 @@ PagedView view_of(const spyb_paged_cache &c, const spyb_paged_batch &b) {
 
 // Host check of how the work is cut: on any lengths, also ones that make no sense, the CTAs' pieces cover every unit of every item once, and every CTA of an item has a place of
 // its own for what it finds. 0 = passed.
-template <int TILE, int UNIT, int ALIGN> static int cut_selftest(uint32_t seed) {
+template <int UNIT, int ALIGN> static int cut_selftest(uint32_t seed, int tile_rows) {
     auto rnd = [&](int n) { seed = seed * 1664525u + 1013904223u; return (int)((seed >> 8) % (uint32_t)n); };
     for (int turn = 0; turn < 400; ++turn) {
         const int n_seq = 1 + rnd(12), most_rows = 1 + rnd(turn % 3 == 0 ? 3 : 60), most_kv = 1 + rnd(3000);
@@ -543,12 +543,12 @@ template <int TILE, int UNIT, int ALIGN> static int cut_selftest(uint32_t seed) 
         PagedAttention p;
         p.view.row_start = start.data(); p.view.n_kv = kv.data(); p.view.n_seq = n_seq; p.view.n_rows = std::max(1, start[n_seq] - rnd(2)); p.view.page_size = 1 + rnd(40);
         p.view.table_stride = 1 + rnd(80); p.view.n_kv_most = p.view.table_stride * p.view.page_size;
-        p.n_head_kv = 1 + rnd(5); p.group = 1 + rnd(8); p.causal = rnd(4) != 0; p.window = p.causal && rnd(2) ? 1 + rnd(500) : 0; p.few_rows = rnd(3) == 0 ? 1 << 30 : rnd(40);
+        p.n_head_kv = 1 + rnd(5); p.group = 1 + rnd(8); p.tile_rows = tile_rows > 0 ? tile_rows : 2 * (128 / p.group) * p.group; p.causal = rnd(4) != 0; p.window = p.causal && rnd(2) ? 1 + rnd(500) : 0; p.few_rows = rnd(3) == 0 ? 1 << 30 : rnd(40);
         const int grid = 1 + rnd(300), least = 1 + rnd(4);
         for (int few = 0; few < 2; ++few) {
             PagedPlace at = {};
             int64_t total = 0;
-            for (int s = 0; s < n_seq; ++s) { total += paged_seq_units<TILE, UNIT, ALIGN>(p, s, few) * p.n_head_kv; }
+            for (int s = 0; s < n_seq; ++s) { total += paged_seq_units<UNIT, ALIGN>(p, s, few) * p.n_head_kv; }
             if (total == 0) { continue; }
             const int ctas = paged_ctas(total, grid, least);
             at.share = paged_share(total, ctas);
@@ -560,17 +560,17 @@ template <int TILE, int UNIT, int ALIGN> static int cut_selftest(uint32_t seed) 
                 int64_t rest = at.unit;
                 int s = 0;
                 for (;; ++s) {
-                    const int64_t n = s < n_seq ? paged_seq_units<TILE, UNIT, ALIGN>(p, s, few) * p.n_head_kv : 0;
+                    const int64_t n = s < n_seq ? paged_seq_units<UNIT, ALIGN>(p, s, few) * p.n_head_kv : 0;
                     if (s >= n_seq) { return 2; }
                     if (rest < n) { break; }
                     rest -= n;
                 }
                 PagedSeq q = paged_seq(p.view, s);
                 int head, tile, off;
-                paged_find<TILE, UNIT, ALIGN>(p, q, paged_seq_units<TILE, UNIT, ALIGN>(p, s, few), rest, head, tile, off);
+                paged_find<UNIT, ALIGN>(p, q, paged_seq_units<UNIT, ALIGN>(p, s, few), rest, head, tile, off);
                 for (;;) {
-                    const PagedItem it = paged_item<TILE, UNIT, ALIGN>(p, q, tile);
-                    if (q.row0 < 0 || q.rows < 1 || q.row0 + q.rows > p.view.n_rows || head >= p.n_head_kv || tile * TILE >= q.rows * p.group) { return 3; }
+                    const PagedItem it = paged_item<UNIT, ALIGN>(p, q, tile);
+                    if (q.row0 < 0 || q.rows < 1 || q.row0 + q.rows > p.view.n_rows || head >= p.n_head_kv || tile * p.tile_rows >= q.rows * p.group) { return 3; }
                     if (it.lo < 0 || it.lo % ALIGN != 0 || it.hi > p.view.n_kv_most || off >= it.units || (int64_t)it.units * UNIT + it.lo < it.hi) { return 4; }
                     const int todo = (int)std::min<int64_t>(it.units - off, at.end - at.unit);
                     const PagedCut cut = paged_cut(at, at.unit - off, it.units);
@@ -584,7 +584,7 @@ template <int TILE, int UNIT, int ALIGN> static int cut_selftest(uint32_t seed) 
                     at.unit += todo;
                     if (at.unit >= at.end) { break; }
                     off = 0;
-                    if (!paged_next<TILE>(p, few, q, s, head, tile)) { return 9; }
+                    if (!paged_next(p, few, q, s, head, tile)) { return 9; }
                 }
             }
             for (uint8_t x : seen) { if (x != 1) { return 10; } }
@@ -594,9 +594,9 @@ template <int TILE, int UNIT, int ALIGN> static int cut_selftest(uint32_t seed) 
     return 0;
 }
 int paged_cut_selftest() {
-    int bad = cut_selftest<16, 64, 16>(1);
-    if (bad == 0) { bad = cut_selftest<32, 64, 16>(2); }
-    if (bad == 0) { bad = cut_selftest<256, 128, 128>(3); }
+    int bad = cut_selftest<64, 16>(1, 16);
+    if (bad == 0) { bad = cut_selftest<64, 16>(2, 32); }
+    if (bad == 0) { bad = cut_selftest<128, 128>(3, 0); }
     return bad == 0 ? 0 : 100 + bad;
 }
 
@@ -661,11 +661,15 @@ spyb_status spyb_paged_attention(spyb_backend *be, const spyb_paged_attention_de
     const int64_t most = (int64_t)(d->batch.max_rows > 0 ? std::min(d->batch.max_rows, d->batch.n_rows) : d->batch.n_rows) * p.group;
     const LaunchCfg cfg = be->launch_cfg(be->config.use_pdl != 0);
     p.few_rows = 1 << 30;
-    if (most > PA_FEW_ROWS && scale >= 0.f && paged_tc_can(p.view, hd)) {
+    if (most > PA_FEW_ROWS && scale >= 0.f) {
+        cudaError_t err = cudaSuccess;
         p.few_rows = p.view.n_seq == 1 ? 0 : PA_FEW_ROWS;
-        SPYB_CUDA(be, launch_paged_attention_tc(p, hd, be->num_sms_total, cfg, be->wait_limit_ns));
+        if (!launch_paged_attention_tc(p, hd, d->n_head, be->num_sms_total, cfg, be->wait_limit_ns, &err)) { p.few_rows = 1 << 30; }
+        SPYB_CUDA(be, err);
     }
-    if (p.few_rows > 0) { SPYB_CUDA(be, launch_paged_attention_rows(p, hd, most <= 16 ? 1 : 2, be->num_sms_total, cfg)); }
+    const int row_tiles = most <= 16 ? 1 : 2;
+    p.tile_rows = 16 * row_tiles;
+    if (p.few_rows > 0) { SPYB_CUDA(be, launch_paged_attention_rows(p, hd, row_tiles, be->num_sms_total, cfg)); }
     return SPYB_SUCCESS;
 }
 

@@ -28,6 +28,7 @@ struct PagedAttention {
     int64_t      q_stride = 0, out_stride = 0;
     int          n_head_kv = 0, group = 1, causal = 1, window = 0, out_f32 = 0;
     float        scale_log2 = 0.f;        // scale * log2(e): probabilities are powers of two
+    int          tile_rows = 16;          // rows of a tile, counting every query head of its K/V head
     int          few_rows = 0;            // sequences of up to so many rows (of all query heads of a K/V head) are the small kernel's
     float       *partial = nullptr;       // [CTAs][2][rows of a tile][head_dim + 2]
     unsigned    *arrived = nullptr;       // [CTAs], zero between launches
@@ -35,8 +36,8 @@ struct PagedAttention {
 int         paged_cut_selftest();   // host-only: 0 when the CTAs' pieces cover every item once, on any lengths
 cudaError_t launch_paged_append(const PagedAppend &p, int in_type, int q_out_type, const LaunchCfg &cfg);
 cudaError_t launch_paged_attention_rows(const PagedAttention &p, int head_dim, int row_tiles, int sms, const LaunchCfg &cfg);
-bool        paged_tc_can(const PagedView &v, int head_dim);   // the tensor-memory kernel takes these pages and heads
-cudaError_t launch_paged_attention_tc(const PagedAttention &p, int head_dim, int sms, const LaunchCfg &cfg, uint64_t wait_limit);
+// the kernel on tensor memory; false where it does not take these pages, heads or strides (nothing is launched then)
+bool        launch_paged_attention_tc(const PagedAttention &p, int head_dim, int n_head, int sms, const LaunchCfg &cfg, uint64_t wait_limit, cudaError_t *err);
 constexpr int PA_FEW_ROWS = 32;          // sequences of up to so many rows (times query heads of a K/V head) are the small kernel's
 constexpr int PA_MAX_CTAS_PER_SM = 2;
 
@@ -54,10 +55,10 @@ __host__ __device__ __forceinline__ PagedSeq paged_seq(const PagedView &v, int s
     const int kv = pmin(pmax(0, v.n_kv[s]), 1 << 30);
     return {a, b - a, kv - (end - a), pmin(kv, v.n_kv_most)};
 }
-template <int TILE, int UNIT, int ALIGN>
+template <int UNIT, int ALIGN>
 __host__ __device__ __forceinline__ PagedItem paged_item(const PagedAttention &p, const PagedSeq &q, int tile) {
-    const int last = pmin(q.rows * p.group, (tile + 1) * TILE) - 1;
-    const int i0 = (int)((unsigned)(tile * TILE) / (unsigned)p.group), i1 = (int)((unsigned)last / (unsigned)p.group);
+    const int last = pmin(q.rows * p.group, (tile + 1) * p.tile_rows) - 1;
+    const int i0 = (int)((unsigned)(tile * p.tile_rows) / (unsigned)p.group), i1 = (int)((unsigned)last / (unsigned)p.group);
     PagedItem t;
     t.hi = p.causal ? pmin(q.kv, q.first + i1 + 1) : q.kv;
     t.lo = p.causal && p.window > 0 ? pmax(0, q.first + i0 - p.window + 1) / ALIGN * ALIGN : 0;
@@ -67,13 +68,13 @@ __host__ __device__ __forceinline__ PagedItem paged_item(const PagedAttention &p
 __host__ __device__ __forceinline__ bool paged_mine(const PagedAttention &p, const PagedSeq &q, bool few) {
     return q.rows > 0 && ((int64_t)q.rows * p.group <= p.few_rows) == few;
 }
-template <int TILE, int UNIT, int ALIGN>
-__host__ __device__ __forceinline__ int64_t paged_seq_units(const PagedAttention &p, int s, bool few) {   // of one K/V head
+template <int UNIT, int ALIGN>
+__host__ __device__ __forceinline__ int64_t paged_seq_units(const PagedAttention &p, int s, bool few, int first = 0, int step = 1) {   // of one K/V head; of every step-th tile
     const PagedSeq q = paged_seq(p.view, s);
     if (!paged_mine(p, q, few)) { return 0; }
-    const int tiles = (q.rows * p.group + TILE - 1) / TILE;
+    const int tiles = (q.rows * p.group + p.tile_rows - 1) / p.tile_rows;
     int64_t n = 0;
-    for (int t = 0; t < tiles; ++t) { n += paged_item<TILE, UNIT, ALIGN>(p, q, t).units; }
+    for (int t = first; t < tiles; t += step) { n += paged_item<UNIT, ALIGN>(p, q, t).units; }
     return n;
 }
 
@@ -81,11 +82,11 @@ __host__ __device__ __forceinline__ int64_t paged_div(int64_t a, int64_t b) {   
     return ((a | b) >> 32) == 0 ? (int64_t)((uint32_t)a / (uint32_t)b) : a / b;
 }
 // unit `rest` of a sequence whose K/V heads have `one` units each
-template <int TILE, int UNIT, int ALIGN>
+template <int UNIT, int ALIGN>
 __host__ __device__ __forceinline__ void paged_find(const PagedAttention &p, const PagedSeq &q, int64_t one, int64_t rest, int &head, int &tile, int &off) {
     head = (int)paged_div(rest, one); rest -= head * one;
     for (tile = 0;; ++tile) {
-        const int u = paged_item<TILE, UNIT, ALIGN>(p, q, tile).units;
+        const int u = paged_item<UNIT, ALIGN>(p, q, tile).units;
         if (rest < u) { break; }
         rest -= u;
     }
@@ -104,21 +105,30 @@ __host__ __device__ __forceinline__ int paged_unit_cta(const PagedShare &s, int6
     return u < head ? (int)paged_div(u, s.each + 1) : s.longer + (int)paged_div(u - head, s.each);
 }
 struct PagedPlace { PagedShare share; int seq, head, tile, off; int64_t unit, end; };   // where a CTA begins, its first unit and the one behind its last
-struct PagedPlanShared { int64_t warp[32]; int seq, head, tile, off; };
+struct PagedPlanShared { int64_t warp[32], one, rest; int seq; };
 __host__ __device__ __forceinline__ int paged_ctas(int64_t total, int grid, int least) { const int64_t n = paged_div(total, least); return n < 1 ? 1 : n < grid ? (int)n : grid; }
 
 // all NT threads of the CTA; `least`: units that a CTA takes at least
-template <int NT, int TILE, int UNIT, int ALIGN>
+template <int NT, int UNIT, int ALIGN>
 __device__ PagedPlace paged_plan(const PagedAttention &p, bool few, int least, PagedPlanShared &sh) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     constexpr int NW = NT / 32;
+    // few sequences have a warp each, whose lanes share the tiles; many have a thread each
+    const bool by_warp = p.view.n_seq <= NW;
     int64_t total = 0, mine = 0;
-    for (int base = 0; base < p.view.n_seq; base += NT) {
-        const int s = base + tid;
-        mine = s < p.view.n_seq ? paged_seq_units<TILE, UNIT, ALIGN>(p, s, few) * p.n_head_kv : 0;
-        total += mine;
+    if (by_warp) {
+        if (warp < p.view.n_seq) { mine = paged_seq_units<UNIT, ALIGN>(p, warp, few, lane, 32); }
+        for (int o = 16; o > 0; o >>= 1) { mine += __shfl_xor_sync(0xffffffffu, mine, o); }
+        mine *= p.n_head_kv;
+        total = mine;
+    } else {
+        for (int base = 0; base < p.view.n_seq; base += NT) {
+            const int s = base + tid;
+            mine = s < p.view.n_seq ? paged_seq_units<UNIT, ALIGN>(p, s, few) * p.n_head_kv : 0;
+            total += mine;
+        }
+        for (int o = 16; o > 0; o >>= 1) { total += __shfl_xor_sync(0xffffffffu, total, o); }
     }
-    for (int o = 16; o > 0; o >>= 1) { total += __shfl_xor_sync(0xffffffffu, total, o); }
     if (lane == 0) { sh.warp[warp] = total; }
     __syncthreads();
     total = 0;
@@ -129,34 +139,53 @@ __device__ PagedPlace paged_plan(const PagedAttention &p, bool few, int least, P
     if (total == 0 || (int)blockIdx.x >= at.share.ctas) { return at; }
     at.unit = paged_cta_unit(at.share, blockIdx.x);
     at.end = paged_cta_unit(at.share, blockIdx.x + 1);
-    int64_t before = 0;
-    for (int base = 0; base < p.view.n_seq; base += NT) {
-        const int s = base + tid;
-        if (p.view.n_seq > NT) { mine = s < p.view.n_seq ? paged_seq_units<TILE, UNIT, ALIGN>(p, s, few) * p.n_head_kv : 0; }
-        int64_t upto = mine;
-        for (int o = 1; o < 32; o <<= 1) { const int64_t v = __shfl_up_sync(0xffffffffu, upto, o); if (lane >= o) { upto += v; } }
-        __syncthreads();
-        if (lane == 31) { sh.warp[warp] = upto; }
-        __syncthreads();
-        int64_t all = 0;
-        for (int w = 0; w < NW; ++w) { const int64_t v = sh.warp[w]; upto += w < warp ? v : 0; all += v; }
-        const int64_t from = before + upto - mine;
-        if (from <= at.unit && at.unit < from + mine) {
-            sh.seq = s;
-            paged_find<TILE, UNIT, ALIGN>(p, paged_seq(p.view, s), paged_div(mine, p.n_head_kv), at.unit - from, sh.head, sh.tile, sh.off);
+    if (by_warp) {
+        int64_t from = 0;
+        for (int w = 0; w < warp; ++w) { from += sh.warp[w]; }
+        if (from <= at.unit && at.unit < from + mine && lane == 0) { sh.seq = warp; sh.one = paged_div(mine, p.n_head_kv); sh.rest = at.unit - from; }
+    } else {
+        int64_t before = 0;
+        for (int base = 0; base < p.view.n_seq; base += NT) {
+            const int s = base + tid;
+            if (p.view.n_seq > NT) { mine = s < p.view.n_seq ? paged_seq_units<UNIT, ALIGN>(p, s, few) * p.n_head_kv : 0; }
+            int64_t upto = mine;
+            for (int o = 1; o < 32; o <<= 1) { const int64_t v = __shfl_up_sync(0xffffffffu, upto, o); if (lane >= o) { upto += v; } }
+            __syncthreads();
+            if (lane == 31) { sh.warp[warp] = upto; }
+            __syncthreads();
+            int64_t all = 0;
+            for (int w = 0; w < NW; ++w) { const int64_t v = sh.warp[w]; upto += w < warp ? v : 0; all += v; }
+            const int64_t from = before + upto - mine;
+            if (from <= at.unit && at.unit < from + mine) { sh.seq = s; sh.one = paged_div(mine, p.n_head_kv); sh.rest = at.unit - from; }
+            before += all;
+            if (at.unit < before) { break; }   // (the same for all threads)
         }
-        before += all;
-        if (at.unit < before) { break; }   // (the same for all threads)
     }
     __syncthreads();
-    at.seq = sh.seq; at.head = sh.head; at.tile = sh.tile; at.off = sh.off;
+    at.seq = sh.seq;
+    at.head = (int)paged_div(sh.rest, sh.one);
+    int64_t rest = sh.rest - at.head * sh.one;
+    const PagedSeq q = paged_seq(p.view, at.seq);
+    const int tiles = (q.rows * p.group + p.tile_rows - 1) / p.tile_rows;
+    for (int base = 0; base < tiles; base += 32) {       // 32 tiles at a time, every warp for itself
+        const int u = base + lane < tiles ? paged_item<UNIT, ALIGN>(p, q, base + lane).units : 0;
+        int upto = u;
+        for (int o = 1; o < 32; o <<= 1) { const int v = __shfl_up_sync(0xffffffffu, upto, o); if (lane >= o) { upto += v; } }
+        const unsigned hit = __ballot_sync(0xffffffffu, rest < upto);
+        if (hit) {
+            const int l = __ffs(hit) - 1;
+            at.tile = base + l;
+            at.off = (int)rest - (__shfl_sync(0xffffffffu, upto, l) - __shfl_sync(0xffffffffu, u, l));
+            break;
+        }
+        rest -= __shfl_sync(0xffffffffu, upto, 31);
+    }
     return at;
 }
 
 // The item behind an item, the same for all threads; false behind the last one.
-template <int TILE>
 __host__ __device__ __forceinline__ bool paged_next(const PagedAttention &p, bool few, PagedSeq &q, int &seq, int &head, int &tile) {
-    if ((++tile) * TILE < q.rows * p.group) { return true; }
+    if ((++tile) * p.tile_rows < q.rows * p.group) { return true; }
     tile = 0;
     if (++head < p.n_head_kv) { return true; }
     head = 0;

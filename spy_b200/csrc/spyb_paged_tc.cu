@@ -1,6 +1,7 @@
 // Attention of many rows a sequence (chunks of prompts, groups of query heads) over paged caches on the tcgen05 tensor cores.
 //
-// Rows and positions go in tiles: 256 rows - two tiles of 128, each with a warpgroup of its own - against 128 positions at a time. S = Q K^T and O += P V are
+// Rows and positions go in tiles: up to 256 rows - two tiles of as many whole tokens (with all query heads of the K/V head) as 128 rows hold, each with a warpgroup of its
+// own - against 128 positions at a time. S = Q K^T and O += P V are
 // tcgen05 MMAs, 128 x 128 x 16 and 128 x head_dim x 16; S, P (fp16, in place of S) and O live in tensor memory, a row a lane, so that a row's maximum and sum stay in
 // one thread. While one tile's probabilities are made (16 powers of two a clock and SM, as many clocks as its two products take), the other tile's
 // products run. K and V come page by page through tensor maps, in pieces of as many positions as divide the page size, into the 128-byte
@@ -21,7 +22,7 @@
 namespace spyb {
 namespace {
 
-constexpr int PT_THREADS = 384, PT_ROWS = 128, PT_TILE = 2 * PT_ROWS, PT_KEYS = 128;
+constexpr int PT_THREADS = 384, PT_ROWS = 128, PT_KEYS = 128;
 constexpr int PT_REGS_SOFTMAX = 208, PT_REGS_OTHERS = 88;   // 256 x 208 + 128 x 88 = 384 x 168, what the block is launched with
 constexpr uint32_t PT_HALF = PT_KEYS * 128;              // bytes of 128 rows x 64 elements
 
@@ -44,6 +45,10 @@ struct TcShared {
 __device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap *map, uint32_t bar, int x, int token, int head, int page) {
     asm volatile("cp.async.bulk.tensor.4d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3,%4,%5,%6}], [%2];"
                  ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(token), "r"(head), "r"(page) : "memory");
+}
+__device__ __forceinline__ void tma_load3(uint32_t dst, const CUtensorMap *map, uint32_t bar, int x, int head, int row) {
+    asm volatile("cp.async.bulk.tensor.3d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3,%4,%5}], [%2];"
+                 ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(head), "r"(row) : "memory");
 }
 // operands in the 128-byte swizzle: rows of 128 bytes, groups of eight rows 1024 bytes apart; `far`: from one 64-element half of an MN-major operand to the next
 __device__ __forceinline__ uint64_t swizzled_desc(uint32_t addr, uint32_t far) {
@@ -93,8 +98,8 @@ struct Stretch {
 
     __device__ __forceinline__ Tile half(const PagedAttention &p, int t) const {
         Tile h;
-        const int r0 = tile * PT_TILE + t * PT_ROWS;
-        h.rows = max(0, min(PT_ROWS, q.rows * p.group - r0));
+        const int r0 = tile * p.tile_rows + t * (p.tile_rows / 2);
+        h.rows = max(0, min(p.tile_rows / 2, q.rows * p.group - r0));
         h.pos_first = q.first + (int)((unsigned)r0 / (unsigned)p.group);
         h.pos_last = q.first + (int)((unsigned)(r0 + max(h.rows, 1) - 1) / (unsigned)p.group);
         const int hi = p.causal ? min(it.hi, h.pos_last + 1) : it.hi, lo = p.causal && p.window > 0 ? max(it.lo, h.pos_first - p.window + 1) : it.lo;
@@ -104,14 +109,14 @@ struct Stretch {
         return h;
     }
     __device__ __forceinline__ void describe(const PagedAttention &p, const PagedPlace &at) {
-        it = paged_item<PT_TILE, PT_KEYS, PT_KEYS>(p, q, tile);
+        it = paged_item<PT_KEYS, PT_KEYS>(p, q, tile);
         todo = (int)min((int64_t)(it.units - off), at.end - at.unit);
     }
     __device__ __forceinline__ bool next(const PagedAttention &p, PagedPlace &at) {
         at.unit += todo;
         if (at.unit >= at.end) { return false; }
         off = 0;
-        return paged_next<PT_TILE>(p, false, q, seq, head, tile);
+        return paged_next(p, false, q, seq, head, tile);
     }
 };
 // steps in which either tile sees something: one run, for the second one's positions begin at the first one's end at the latest
@@ -123,7 +128,7 @@ __device__ __forceinline__ Steps steps_of(const Tile &a, const Tile &b) {
 }
 
 template <int HD>
-__global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_constant__ PagedAttention p, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
+__global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_constant__ PagedAttention p, const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
                                                                   const int box, int *error_flag, const uint64_t wait_limit) {
     using Shape = TcShape<HD>;
     constexpr int SLOTS = Shape::SLOTS;
@@ -140,7 +145,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
     }
     pdl_launch_dependents();
     pdl_wait();
-    PagedPlace at = paged_plan<PT_THREADS, PT_TILE, PT_KEYS, PT_KEYS>(p, false, 2, sh.plan);
+    PagedPlace at = paged_plan<PT_THREADS, PT_KEYS, PT_KEYS>(p, false, 2, sh.plan);
     if (at.unit >= at.end) { return; }
     if (warp == 8) { asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&sh.tmem)) : "memory"); }
     tc_fence_before();
@@ -159,6 +164,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
         const uint32_t lanes = (uint32_t)(warp & 3) << 21;                                   // (32 lanes a warp, in the address's upper half)
         const uint32_t s_tmem = tmem + lanes + t * PT_KEYS, o_tmem = tmem + lanes + 2 * PT_KEYS + t * HD;
         const float scale = p.scale_log2;
+        const int half_tokens = PT_ROWS / p.group, row_token = (int)((unsigned)row / (unsigned)p.group), g = row - row_token * p.group;   // a tile has whole tokens
         uint32_t s_phase = 0, o_phase = 0, tiles = 0, stretch = 0;
         Tile own;
         Steps steps;
@@ -170,8 +176,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
         describe();
         for (;;) {
             float m = -CUDART_INF_F, l = 0.f;
-            const int pr = x.tile * PT_TILE + t * PT_ROWS + min(row, max(own.rows, 1) - 1);
-            const int token = (int)((unsigned)pr / (unsigned)p.group), g = pr - token * p.group, pos = x.q.first + token;
+            const int token = (2 * x.tile + t) * half_tokens + row_token, pos = x.q.first + token;   // (of rows that are there)
             for (int step = own.from; step < own.to; ++step) {
                 mbar_wait_lean(s_ready + 8 * t, s_phase, limit);
                 s_phase ^= 1;
@@ -265,7 +270,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
             const PagedCut cut = paged_cut(was, was.unit - done.off, done.it.units);
             float4 *part = reinterpret_cast<float4 *>(p.partial) + (paged_slot(blockIdx.x, cut.c0) * 2 + t) * (PT_ROWS * (HD + 2) / 4);     // [HD / 4][128] x 4, [128], [128]
             const float inv = cut.parts > 1 ? 1.f : l == 0.f ? 0.f : 1.f / l;
-            const bool mine = row < done_own.rows;
+            const bool mine = row < done_own.rows;                       // (rows behind the last whole token are nobody's)
             const bool poisoned = any && *reinterpret_cast<volatile int *>(&sh.poison[stretch & 7]) == (int)stretch + 1;
             const int64_t to_row = (int64_t)(done.q.row0 + token) * p.out_stride + (done.head * p.group + g) * HD;
 #pragma unroll 1
@@ -422,6 +427,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
         } else if (warp >= 10) {
             // ------------------------------------------------------------------------------ Q of a tile each; V tiles that not all rows see whole, half of the rows each
             uint32_t tiles = 0, stretch = 0, q_phase = 1;
+            bool asked = false;
             const int t = warp - 10;
             const int v_row0 = t * (PT_KEYS / 2);
             for (;;) {
@@ -430,25 +436,15 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
                 const Steps steps = steps_of(a, b);
                 if (t == 0 ? a.to > a.from : b.to > b.from) {
                     mbar_wait_lean(q_free + 8 * t, q_phase, limit);
-                    q_phase ^= 1;
-                    constexpr int PIECES = HD / 8, AT_ONCE = 32 / PIECES;                    // pieces of 16 bytes of a row, rows at once
-                    const int rows = t == 0 ? a.rows : b.rows, c = lane % PIECES;
-                    const unsigned r0 = (unsigned)(x.tile * PT_TILE + t * PT_ROWS + lane / PIECES), group = (unsigned)p.group;
-                    int token = (int)(r0 / group), g = (int)(r0 - (unsigned)token * group);
-                    const int more_tokens = AT_ONCE / p.group, more_heads = AT_ONCE - more_tokens * p.group;
-                    const __half *src = p.q + (int64_t)x.q.row0 * p.q_stride + x.head * p.group * HD + c * 8;
-#pragma unroll 4
-                    for (int r = lane / PIECES; r < PT_ROWS; r += AT_ONCE) {
-                        const bool in = r < rows;
-                        const uint32_t dst = q_addr + t * Shape::OPERAND + (c >> 3) * PT_HALF + r * 128 + (((c & 7) ^ (r & 7)) << 4);
-                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(in ? src + token * p.q_stride + g * HD : p.q), "r"(in ? 16 : 0) : "memory");
-                        token += more_tokens; g += more_heads;
-                        if (g >= p.group) { g -= p.group; ++token; }
+                    q_phase ^= 1; asked = true;
+                    // whole tokens, token by token their heads: what lies behind the sequence's rows is other sequences' or nothing, and goes nowhere
+                    if (elect_one()) {
+                        const int tokens = PT_ROWS / p.group, row = x.q.row0 + (2 * x.tile + t) * tokens;
+                        mbar_expect_tx(q_ready + 8 * t, tokens * p.group * HD * 2);
+#pragma unroll
+                        for (int h = 0; h < HD / 64; ++h) { tma_load3(q_addr + t * Shape::OPERAND + h * PT_HALF, &q_map, q_ready + 8 * t, h * 64, x.head * p.group, row); }
                     }
-                    asm volatile("cp.async.wait_all;" ::: "memory");
-                    fence_async_smem();
                     __syncwarp();
-                    if (lane == 0) { mbar_arrive(q_ready + 8 * t); }
                 }
                 for (int step = steps.begin; step < steps.end; ++step) {
                     advance();                                                               // (K)
@@ -492,6 +488,10 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
                 }
                 ++stretch;
                 if (!x.next(p, at)) { break; }
+            }
+            if (limit == 0 && asked) {   // (something gave up: what is on its way lands before the CTA ends)
+                uint64_t again = wait_limit;
+                mbar_wait_lean(q_ready + 8 * t, q_phase, again);
             }
         } else if (warp == 8) {
             // ------------------------------------------------------------------------------ MMAs
@@ -588,14 +588,23 @@ EncodeTiled encoder() {
     }();
     return fn;
 }
+bool tensor_map(CUtensorMap *map, const __half *data, int n, const cuuint64_t *dims, const cuuint64_t *strides, const cuuint32_t *box) {
+    const cuuint32_t ones[4] = {1, 1, 1, 1};
+    return encoder() != nullptr && encoder()(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, n, const_cast<__half *>(data), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                                             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
 // pages of one pool: [page][head][position][element] whatever the order of the strides; boxes of `box` positions x 64 elements
 bool page_map(CUtensorMap *map, const __half *pool, const PagedView &v, int heads, int head_dim, int box) {
-    if (encoder() == nullptr) { return false; }
     const cuuint64_t dims[4] = {(cuuint64_t)head_dim, (cuuint64_t)v.page_size, (cuuint64_t)heads, (cuuint64_t)v.n_pages};
     const cuuint64_t strides[3] = {(cuuint64_t)v.token_stride * 2, (cuuint64_t)v.head_stride * 2, (cuuint64_t)v.page_stride * 2};
-    const cuuint32_t boxes[4] = {64, (cuuint32_t)box, 1, 1}, ones[4] = {1, 1, 1, 1};
-    return encoder()(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<__half *>(pool), dims, strides, boxes, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                     CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+    const cuuint32_t boxes[4] = {64, (cuuint32_t)box, 1, 1};
+    return tensor_map(map, pool, 4, dims, strides, boxes);
+}
+// Q: [row][head][element], boxes of whole tokens of a group of heads
+bool query_map(CUtensorMap *map, const PagedAttention &p, int n_head, int head_dim) {
+    const cuuint64_t dims[3] = {(cuuint64_t)head_dim, (cuuint64_t)n_head, (cuuint64_t)p.view.n_rows}, strides[2] = {(cuuint64_t)head_dim * 2, (cuuint64_t)p.q_stride * 2};
+    const cuuint32_t boxes[3] = {64, (cuuint32_t)p.group, (cuuint32_t)(PT_ROWS / p.group)};
+    return tensor_map(map, p.q, 3, dims, strides, boxes);
 }
 // the warpgroups' registers after their split are what the block is launched with: fewer, and the split would wait for ever
 template <int HD> cudaError_t registers_suffice() {
@@ -607,30 +616,32 @@ template <int HD> cudaError_t registers_suffice() {
     return answer;
 }
 template <int HD>
-cudaError_t launch_tc(const PagedAttention &p, const CUtensorMap &k, const CUtensorMap &v, int box, int sms, const LaunchCfg &cfg, uint64_t wait_limit) {
+cudaError_t launch_tc(const PagedAttention &p, const CUtensorMap &q, const CUtensorMap &k, const CUtensorMap &v, int box, int sms, const LaunchCfg &cfg, uint64_t wait_limit) {
     cudaError_t err = registers_suffice<HD>();
     if (err != cudaSuccess) { return err; }
     err = allow_dynamic_smem(reinterpret_cast<const void *>(paged_tc_kernel<HD>), TcShape<HD>::SMEM);
     if (err != cudaSuccess) { return err; }
-    return launch_maybe_pdl(paged_tc_kernel<HD>, dim3(sms), PT_THREADS, TcShape<HD>::SMEM, cfg.stream, cfg.pdl, p, k, v, box, cfg.error_flag, wait_limit);
+    return launch_maybe_pdl(paged_tc_kernel<HD>, dim3(sms), PT_THREADS, TcShape<HD>::SMEM, cfg.stream, cfg.pdl, p, q, k, v, box, cfg.error_flag, wait_limit);
 }
 
 }  // namespace
 
-int paged_tc_box(int page_size) {   // positions of a box: the largest power of two up to 128 that divides the page size
+static int paged_tc_box(int page_size) {   // positions of a box: the largest power of two up to 128 that divides the page size
     int box = 1;
     while (box < PT_KEYS && page_size % (2 * box) == 0) { box *= 2; }
     return box;
 }
-bool paged_tc_can(const PagedView &v, int head_dim) {
-    return (head_dim == 64 || head_dim == 128) && paged_tc_box(v.page_size) >= 8 && v.token_stride > 0 && v.head_stride > 0 && v.page_stride > 0 &&
-           std::max({v.token_stride, v.head_stride, v.page_stride}) < (1ll << 38) && encoder() != nullptr;
-}
-cudaError_t launch_paged_attention_tc(const PagedAttention &p, int head_dim, int sms, const LaunchCfg &cfg, uint64_t wait_limit) {
-    CUtensorMap k, v;
-    const int box = paged_tc_box(p.view.page_size);
-    if (!page_map(&k, p.k, p.view, p.n_head_kv, head_dim, box) || !page_map(&v, p.v, p.view, p.n_head_kv, head_dim, box)) { return cudaErrorInvalidValue; }
-    return head_dim == 128 ? launch_tc<128>(p, k, v, box, sms, cfg, wait_limit) : launch_tc<64>(p, k, v, box, sms, cfg, wait_limit);
+bool launch_paged_attention_tc(const PagedAttention &given, int head_dim, int n_head, int sms, const LaunchCfg &cfg, uint64_t wait_limit, cudaError_t *err) {
+    const int box = paged_tc_box(given.view.page_size);
+    const PagedView &view = given.view;
+    const int64_t most = std::max({view.token_stride, view.head_stride, view.page_stride, given.q_stride}), least = std::min({view.token_stride, view.head_stride, view.page_stride, given.q_stride});
+    if ((head_dim != 64 && head_dim != 128) || box < 8 || given.group > PT_ROWS || least <= 0 || most >= (1ll << 38)) { return false; }
+    PagedAttention p = given;
+    p.tile_rows = 2 * (PT_ROWS / p.group) * p.group;
+    CUtensorMap q, k, v;
+    if (!query_map(&q, p, n_head, head_dim) || !page_map(&k, p.k, p.view, p.n_head_kv, head_dim, box) || !page_map(&v, p.v, p.view, p.n_head_kv, head_dim, box)) { return false; }
+    *err = head_dim == 128 ? launch_tc<128>(p, q, k, v, box, sms, cfg, wait_limit) : launch_tc<64>(p, q, k, v, box, sms, cfg, wait_limit);
+    return true;
 }
 
 }  // namespace spyb
