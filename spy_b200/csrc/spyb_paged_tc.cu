@@ -34,12 +34,13 @@ template <int HD> struct TcShape {
 struct TcShared {
     uint64_t full[8], empty[8];                          // a slot's copies have landed; its last MMA is done
     uint64_t clean[8];                                   // of the last V tiles: what nobody sees is cleared
-    uint64_t q_ready[2], q_free[2], s_ready[2], p_ready[2], o_ready[2];   // of the two tiles, in stretches in which they see anything
+    uint64_t q_ready[2], q_free[2], s_ready[2], p_ready[2][2], o_ready[2];   // of the two tiles, in stretches in which they see anything; (P) of their first 96 positions and the rest
     uint32_t tmem;
     uint32_t there[8];                                   // of the last tiles: which groups of eight positions are there
     int      poison[8];                                  // of the last stretches: a V tile that some rows see in part holds values that are not finite
-    int      last[2];
+    int      last[2], more[2];
     PagedPlanShared plan;
+    uint64_t walk[2][24];                                // the probability warpgroups' Walk: in registers it would push scores out of them
 };
 
 __device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap *map, uint32_t bar, int x, int token, int head, int page) {
@@ -79,6 +80,9 @@ __device__ __forceinline__ float max3(float a, float b, float c) { float d; asm(
 __device__ __forceinline__ float exp2_fast(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
 __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) { uint32_t r; asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo)); return r; }
 __device__ __forceinline__ uint32_t not_finite(uint32_t h2) { return ((h2 & 0x7c007c00u) + 0x04000400u) & 0x80008000u; }
+// the tiles make their probabilities in turn: together they would share the unit for powers of two, and then wait together for their products
+__device__ __forceinline__ void turn_wait(int t) { asm volatile("bar.sync %0, 256;" ::"r"(3 + t) : "memory"); }
+__device__ __forceinline__ void turn_give(int t) { asm volatile("bar.arrive %0, 256;" ::"r"(3 + t) : "memory"); }
 __device__ __forceinline__ void group_sync(int t) { asm volatile("bar.sync %0, 128;" ::"r"(1 + t) : "memory"); }
 
 // One stretch of an item: `todo` steps of 128 positions from step `off` of the item on. Every role walks the same stretches.
@@ -119,6 +123,8 @@ struct Stretch {
         return paged_next(p, false, q, seq, head, tile);
     }
 };
+struct Walk { Stretch x; PagedPlace at; };
+static_assert(sizeof(Walk) <= sizeof(TcShared::walk[0]), "room for the walk");
 // steps in which either tile sees something: one run, for the second one's positions begin at the first one's end at the latest
 struct Steps { int begin, end; };
 __device__ __forceinline__ Steps steps_of(const Tile &a, const Tile &b) {
@@ -140,7 +146,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
     const uint32_t q_ready = smem_u32(sh.q_ready), s_ready = smem_u32(sh.s_ready), p_ready = smem_u32(sh.p_ready), o_ready = smem_u32(sh.o_ready), q_free = smem_u32(sh.q_free);
     if (tid == 0) {
         for (int i = 0; i < 8; ++i) { mbar_init(full + 8 * i, 1); mbar_init(empty + 8 * i, 1); mbar_init(clean + 8 * i, 2); sh.poison[i] = 0; }
-        for (int t = 0; t < 2; ++t) { mbar_init(q_ready + 8 * t, 1); mbar_init(q_free + 8 * t, 1); mbar_init(s_ready + 8 * t, 1); mbar_init(p_ready + 8 * t, 4); mbar_init(o_ready + 8 * t, 1); }
+        for (int t = 0; t < 2; ++t) { mbar_init(q_ready + 8 * t, 1); mbar_init(q_free + 8 * t, 1); mbar_init(s_ready + 8 * t, 1); mbar_init(p_ready + 16 * t, 4); mbar_init(p_ready + 16 * t + 8, 4); mbar_init(o_ready + 8 * t, 1); }
         mbar_init_fence();
     }
     pdl_launch_dependents();
@@ -166,17 +172,15 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
         const float scale = p.scale_log2;
         const int half_tokens = PT_ROWS / p.group, row_token = (int)((unsigned)row / (unsigned)p.group), g = row - row_token * p.group;   // a tile has whole tokens
         uint32_t s_phase = 0, o_phase = 0, tiles = 0, stretch = 0;
-        Tile own;
-        Steps steps;
-        auto describe = [&]() {
-            x.describe(p, at);
-            own = x.half(p, t);
-            steps = steps_of(own, x.half(p, 1 - t));
-        };
-        describe();
+        Walk &w = *reinterpret_cast<Walk *>(sh.walk[t]);
+        if (row == 0) { x.describe(p, at); w.x = x; w.at = at; }
+        group_sync(t);
         for (;;) {
             float m = -CUDART_INF_F, l = 0.f;
-            const int token = (2 * x.tile + t) * half_tokens + row_token, pos = x.q.first + token;   // (of rows that are there)
+            const Tile own = w.x.half(p, t);
+            const Tile other = w.x.half(p, 1 - t);
+            const Steps steps = steps_of(own, other), both = {max(own.from, other.from), min(own.to, other.to)};
+            const int token = (2 * w.x.tile + t) * half_tokens + row_token, pos = w.x.q.first + token;   // (of rows that are there)
             for (int step = own.from; step < own.to; ++step) {
                 mbar_wait_lean(s_ready + 8 * t, s_phase, limit);
                 s_phase ^= 1;
@@ -185,59 +189,26 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
 #pragma unroll
                 for (int i = 0; i < 4; ++i) { tmem_ld32(s_tmem + 32 * i, s + 32 * i); }
                 const uint32_t there = *reinterpret_cast<volatile uint32_t *>(&sh.there[(tiles + step - steps.begin) & 7]);
+                const bool plain = there == 0xffffu && own.whole(p, w.x.it, step);
                 tmem_ld_wait();
-                if (there != 0xffffu || !own.whole(p, x.it, step)) {
-                    const int j0 = x.it.lo + step * PT_KEYS;
-                    const int c1 = (p.causal ? min(x.it.hi, pos + 1) : x.it.hi) - j0, c0 = p.causal && p.window > 0 ? pos - p.window + 1 - j0 : 0;
+                if (!plain) {
+                    const int j0 = w.x.it.lo + step * PT_KEYS;
+                    const int c1 = (p.causal ? min(w.x.it.hi, pos + 1) : w.x.it.hi) - j0, c0 = p.causal && p.window > 0 ? pos - p.window + 1 - j0 : 0;
 #pragma unroll
                     for (int c = 0; c < 128; ++c) {
                         if (!(c >= c0 && c < c1 && ((there >> (c >> 3)) & 1))) { s[c] = 0xff800000u; }
                     }
                 }
-                float tops[4], top;
-                auto largest = [&](int i) {                   // of columns 32 i .. 32 i + 31
+                float tops[4];
 #pragma unroll
-                    for (int c = 0; c < 32; c += 8) {
+                for (int e = 0; e < 4; ++e) { tops[e] = fmaxf(__uint_as_float(s[2 * e]), __uint_as_float(s[2 * e + 1])); }
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) { tops[e] = max3(tops[e], __uint_as_float(s[32 * i + c + 2 * e]), __uint_as_float(s[32 * i + c + 2 * e + 1])); }
-                    }
-                };
-                auto powers = [&](bool also_largest) {        // the row's probabilities against m, into tensor memory; their sum
-                    const float neg = m == -CUDART_INF_F ? 0.f : -m;
-                    const uint64_t neg2 = f2_pack(neg, neg), scale2 = f2_pack(scale, scale);
-                    uint64_t sum[2] = {0, 0};
+                for (int c = 8; c < 128; c += 8) {
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        uint32_t h[16];
-#pragma unroll
-                        for (int c = 0; c < 16; ++c) {
-                            float a, b;
-                            f2_unpack(f2_fma(f2_pack_bits(s[32 * i + 2 * c], s[32 * i + 2 * c + 1]), scale2, neg2), a, b);
-                            a = exp2_fast(a); b = exp2_fast(b);
-                            sum[c & 1] = f2_add(sum[c & 1], f2_pack(a, b));
-                            h[c] = pack_f16(a, b);
-                        }
-                        tmem_st16(s_tmem + 16 * i, h);
-                        if (also_largest) { largest(i); }
-                    }
-                    float a, b;
-                    f2_unpack(f2_add(sum[0], sum[1]), a, b);
-                    return a + b;
-                };
-                tops[0] = tops[1] = tops[2] = tops[3] = -CUDART_INF_F;
-                bool again = step == own.from;
-                if (!again) {
-                    // the maximum of the steps before does, nearly always: powers at once, and whether it did
-                    const float sum = powers(true);
-                    top = fmaxf(max3(tops[0], tops[1], tops[2]), tops[3]) * scale;
-                    again = __any_sync(0xffffffffu, top > m + 8.f);
-                    if (!again) { l += sum; }
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) { largest(i); }
-                    top = fmaxf(max3(tops[0], tops[1], tops[2]), tops[3]) * scale;
+                    for (int e = 0; e < 4; ++e) { tops[e] = max3(tops[e], __uint_as_float(s[c + 2 * e]), __uint_as_float(s[c + 2 * e + 1])); }
                 }
-                if (again) {
+                const float top = fmaxf(max3(tops[0], tops[1], tops[2]), tops[3]) * scale;
+                if (__any_sync(0xffffffffu, top > m + 8.f)) {
                     const float to = fmaxf(m, top), f = to == m ? 1.f : exp2_fast(m - to);
                     m = to; l *= f;
                     if (step != own.from) {
@@ -251,28 +222,50 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
                             tmem_st16(o_tmem + 16 * i, o);
                         }
                     }
-                    l += powers(false);
                 }
-                tmem_st_wait();
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) { mbar_arrive(p_ready + 8 * t); }
+                const uint64_t scale2 = f2_pack(scale, scale);
+                const float neg = m == -CUDART_INF_F ? 0.f : -m;
+                const uint64_t neg2 = f2_pack(neg, neg);
+                uint64_t sum[2] = {0, 0};
+                auto powers = [&](int i) {                    // probabilities of these columns against m, into tensor memory over scores that are read
+                    uint32_t h[16];
+#pragma unroll
+                    for (int c = 0; c < 16; ++c) {
+                        float a, b;
+                        f2_unpack(f2_fma(f2_pack_bits(s[32 * i + 2 * c], s[32 * i + 2 * c + 1]), scale2, neg2), a, b);
+                        a = exp2_fast(a); b = exp2_fast(b);
+                        sum[c & 1] = f2_add(sum[c & 1], f2_pack(a, b));
+                        h[c] = pack_f16(a, b);
+                    }
+                    tmem_st16(s_tmem + 16 * i, h);
+                };
+                auto hand_over = [&](int half) {
+                    tmem_st_wait();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) { mbar_arrive(p_ready + 16 * t + 8 * half); }
+                };
+                const bool in_turn = step >= both.begin && step < both.end;
+                if (in_turn && (t == 1 || step > both.begin)) { turn_wait(t); }
+                powers(0); powers(1); powers(2);
+                hand_over(0);                                 // (their products run beside the last powers)
+                powers(3);
+                if (in_turn && (t == 0 || step + 1 < both.end)) { turn_give(1 - t); }
+                hand_over(1);
+                float a, b;
+                f2_unpack(f2_add(sum[0], sum[1]), a, b);
+                l += a + b;
             }
             tiles += steps.end - steps.begin;
             // this stretch's findings
-            const Stretch done = x;
-            const Tile done_own = own, done_other = x.half(p, 1 - t);
-            const PagedPlace was = at;
             const bool any = own.to > own.from;
-            const bool more = x.next(p, at);
-            if (more) { describe(); }
             if (any) { mbar_wait_lean(o_ready + 8 * t, o_phase, limit); o_phase ^= 1; tc_fence_after(); }
-            const PagedCut cut = paged_cut(was, was.unit - done.off, done.it.units);
+            const PagedCut cut = paged_cut(w.at, w.at.unit - w.x.off, w.x.it.units);
             float4 *part = reinterpret_cast<float4 *>(p.partial) + (paged_slot(blockIdx.x, cut.c0) * 2 + t) * (PT_ROWS * (HD + 2) / 4);     // [HD / 4][128] x 4, [128], [128]
             const float inv = cut.parts > 1 ? 1.f : l == 0.f ? 0.f : 1.f / l;
-            const bool mine = row < done_own.rows;                       // (rows behind the last whole token are nobody's)
+            const bool mine = row < own.rows;                       // (rows behind the last whole token are nobody's)
             const bool poisoned = any && *reinterpret_cast<volatile int *>(&sh.poison[stretch & 7]) == (int)stretch + 1;
-            const int64_t to_row = (int64_t)(done.q.row0 + token) * p.out_stride + (done.head * p.group + g) * HD;
+            const int64_t to_row = (int64_t)(w.x.q.row0 + token) * p.out_stride + (w.x.head * p.group + g) * HD;
 #pragma unroll 1
             for (int i = 0; i < HD / 32; ++i) {
                 uint32_t o[32];
@@ -283,8 +276,9 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
                 }
                 if (poisoned && mine) {
                     // values that are not finite were taken out of the V tiles that not all rows see whole: back to the rows that see them
-                    for (int step = done_own.from; step < done_own.to; ++step) {
-                        if (done_own.whole(p, done.it, step) && done_other.whole(p, done.it, step)) { continue; }
+                    const Stretch done = w.x;
+                    for (int step = own.from; step < own.to; ++step) {
+                        if (own.whole(p, done.it, step) && other.whole(p, done.it, step)) { continue; }
                         const int j0 = done.it.lo + step * PT_KEYS, ja = max(j0, p.causal && p.window > 0 ? pos - p.window + 1 : 0), jb = min(j0 + PT_KEYS, p.causal ? min(done.it.hi, pos + 1) : done.it.hi);
                         for (int j = ja; j < jb; ++j) {
                             const int page = p.view.page_table[(int64_t)done.seq * p.view.table_stride + j / p.view.page_size];
@@ -343,36 +337,48 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
 #pragma unroll 4
                         for (int i = 0; i < cut.parts; ++i) { top = fmaxf(top, __ldcg(reinterpret_cast<const float *>(piece(i) + PT_ROWS * HD / 4) + row)); }
                         const float ref = top == -CUDART_INF_F ? 0.f : top;
-                        float4 v[HD / 4];
-#pragma unroll
-                        for (int c = 0; c < HD / 4; ++c) { v[c] = make_float4(0.f, 0.f, 0.f, 0.f); }
 #pragma unroll 1
-                        for (int i = 0; i < cut.parts; ++i) {
-                            const float4 *from = piece(i);
-                            const float *st = reinterpret_cast<const float *>(from + PT_ROWS * HD / 4);
-                            const float f = exp2_fast(__ldcg(st + row) - ref);
-                            sum += f * __ldcg(st + PT_ROWS + row);
+                        for (int c0 = 0; c0 < HD / 4; c0 += 16) {
+                            float4 v[16];
 #pragma unroll
-                            for (int c = 0; c < HD / 4; ++c) {
-                                const float4 u = __ldcg(from + c * PT_ROWS + row);
-                                v[c].x += f * u.x; v[c].y += f * u.y; v[c].z += f * u.z; v[c].w += f * u.w;
+                            for (int c = 0; c < 16; ++c) { v[c] = make_float4(0.f, 0.f, 0.f, 0.f); }
+                            sum = 0.f;
+#pragma unroll 1
+                            for (int i = 0; i < cut.parts; ++i) {
+                                const float4 *from = piece(i);
+                                const float *st = reinterpret_cast<const float *>(from + PT_ROWS * HD / 4);
+                                const float f = exp2_fast(__ldcg(st + row) - ref);
+                                sum += f * __ldcg(st + PT_ROWS + row);
+#pragma unroll
+                                for (int c = 0; c < 16; ++c) {
+                                    const float4 u = __ldcg(from + (c0 + c) * PT_ROWS + row);
+                                    v[c].x += f * u.x; v[c].y += f * u.y; v[c].z += f * u.z; v[c].w += f * u.w;
+                                }
                             }
-                        }
-                        const float inv_all = sum == 0.f ? 0.f : 1.f / sum;
+                            const float inv_all = sum == 0.f ? 0.f : 1.f / sum;
 #pragma unroll
-                        for (int c = 0; c < HD / 4; c += 2) {
-                            const float4 a = make_float4(v[c].x * inv_all, v[c].y * inv_all, v[c].z * inv_all, v[c].w * inv_all);
-                            const float4 b = make_float4(v[c + 1].x * inv_all, v[c + 1].y * inv_all, v[c + 1].z * inv_all, v[c + 1].w * inv_all);
-                            if (p.out_f32) {
-                                float4 *dst = reinterpret_cast<float4 *>(static_cast<float *>(p.out) + to_row + 4 * c);
-                                dst[0] = a; dst[1] = b;
-                            } else { *reinterpret_cast<uint4 *>(static_cast<__half *>(p.out) + to_row + 4 * c) = make_uint4(pack_f16(a.x, a.y), pack_f16(a.z, a.w), pack_f16(b.x, b.y), pack_f16(b.z, b.w)); }
+                            for (int c = 0; c < 16; c += 2) {
+                                const float4 a = make_float4(v[c].x * inv_all, v[c].y * inv_all, v[c].z * inv_all, v[c].w * inv_all);
+                                const float4 b = make_float4(v[c + 1].x * inv_all, v[c + 1].y * inv_all, v[c + 1].z * inv_all, v[c + 1].w * inv_all);
+                                if (p.out_f32) {
+                                    float4 *dst = reinterpret_cast<float4 *>(static_cast<float *>(p.out) + to_row + 4 * (c0 + c));
+                                    dst[0] = a; dst[1] = b;
+                                } else { *reinterpret_cast<uint4 *>(static_cast<__half *>(p.out) + to_row + 4 * (c0 + c)) = make_uint4(pack_f16(a.x, a.y), pack_f16(a.z, a.w), pack_f16(b.x, b.y), pack_f16(b.z, b.w)); }
+                            }
                         }
                     }
                 }
             }
             ++stretch;
-            if (!more) { break; }
+            group_sync(t);
+            if (row == 0) {
+                x = w.x; at = w.at;
+                const bool more = x.next(p, at);
+                if (more) { x.describe(p, at); w.x = x; w.at = at; }
+                sh.more[t] = more;
+            }
+            group_sync(t);
+            if (!sh.more[t]) { break; }
         }
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PT_REGS_OTHERS));
@@ -541,18 +547,21 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
 #pragma unroll
                     for (int t = 0; t < 2; ++t) {
                         if (active(t, step)) {
-                            mbar_wait_lean(p_ready + 8 * t, p_phase[t], limit);
-                            p_phase[t] ^= 1;
-                            tc_fence_after();
-                            if (elect_one()) {
-                                const uint64_t b = swizzled_desc(ring + v_slot * Shape::OPERAND, PT_HALF);
 #pragma unroll
-                                for (int k = 0; k < PT_KEYS / 16; ++k) {
-                                    mma_f16_ts(tmem + 2 * PT_KEYS + t * HD, tmem + t * PT_KEYS + 8 * k, b + ((k * 2048) >> 4), idesc_o, step != halves[t].from || k != 0);
+                            for (int half = 0; half < 2; ++half) {
+                                mbar_wait_lean(p_ready + 16 * t + 8 * half, p_phase[t], limit);
+                                tc_fence_after();
+                                if (elect_one()) {
+                                    const uint64_t b = swizzled_desc(ring + v_slot * Shape::OPERAND, PT_HALF);
+#pragma unroll
+                                    for (int k = 6 * half; k < 6 + 2 * half; ++k) {
+                                        mma_f16_ts(tmem + 2 * PT_KEYS + t * HD, tmem + t * PT_KEYS + 8 * k, b + ((k * 2048) >> 4), idesc_o, step != halves[t].from || k != 0);
+                                    }
+                                    if (half == 1 && step + 1 == halves[t].to) { mma_commit(o_ready + 8 * t); }
                                 }
-                                if (step + 1 == halves[t].to) { mma_commit(o_ready + 8 * t); }
+                                __syncwarp();
                             }
-                            __syncwarp();
+                            p_phase[t] ^= 1;
                         }
                         if (ahead && active(t, step + 1)) { scores(t, slot, step + 2 == halves[t].to); }
                     }
