@@ -11,28 +11,31 @@
 namespace spyb {
 namespace {
 
-// A cluster of CTAs has a row, each a slice of it in shared memory: the logits are read once. Which token a number falls on must not depend on how sums
-// are rounded, so weights are integers: w = round(2^S exp((x - largest) / T)), S = 45 for up to 2^17 tokens. Their sums are exact in any order, a histogram's
-// too, and a weight's error of 2^-46 moves a border of the sums by about 2^-37 at most. An exponential to 2^-50 costs 13 operations in 64 bits (64
-// a clock and SM), so it is taken where it is needed only:
+// A cluster of CTAs has a row, each a slice of it in shared memory: the logits are read once, by bulk copies. Which token a number falls on must not depend on how
+// sums are rounded, so weights are integers: w = round(2^S exp((x - largest) / T)), S = 45 for up to 2^17 tokens. Their sums are exact in any order,
+// a histogram's too, and a weight's error of 2^-46 moves a border of the sums by about 2^-37 at most. An exponential to 2^-48 costs 13 operations in 64 bits
+// (64 a clock and SM), so it is taken where it is needed only:
 //   greedy            none
-//   top-k             a histogram of the logits' distances from the largest (counts) finds the few candidates; one CTA sorts them and does the rest
-//   top-p alone       the counts bracket the bin in which top_p is reached (a bin is 0.0156 wide, its weights are known to 0.8 %); one pass of
-//                     weights gives the sums around the bracket and a second histogram inside it, and the elements of its one bin are sorted
+//   top-k             the k-th largest of the threads' own maxima is a lower bound of the k-th largest logit (one histogram of their distances from the
+//                     largest); threads whose maximum reaches it give their candidates to the first CTA, which ranks them and does the rest
+//   top-p alone       a histogram of all distances (counts) brackets the bin in which top_p is reached (a bin is 0.0156 wide, its weights are known to 0.8 %);
+//                     one pass of weights gives the sums around the bracket and a second histogram inside it, and the elements of its one bin are sorted
 //   draw              one pass of the weights that stayed; the warp on whose stretch the number falls walks it again
 // Candidates that do not fit a list (ties by the thousand, a top_k of thousands) take a binary search over (logit, index): slow, and as right.
-constexpr int SA_THREADS = 512, SA_WARPS = SA_THREADS / 32, SA_BINS = 2048, SA_LIST = 1024, SA_MAX_CLUSTER = 8;
+constexpr int SA_THREADS = 512, SA_WARPS = SA_THREADS / 32, SA_BINS = 2048, SA_LIST = 1024, SA_RANKED = 256, SA_MAX_CLUSTER = 8, SA_PIECES = 4;
 constexpr int SA_INDEX_BITS = 20;
 constexpr size_t SA_MAX_SLICE = 40960;    // logits that a CTA keeps in shared memory; longer slices are read again in every pass
 
 struct SampleParams {
     const void    *logits;
     int64_t        row_stride;
-    int            n_vocab, per, cached, frac_bits;   // per: logits of a slice; cached: kept in shared memory; frac_bits: S
+    int            n_vocab, per, frac_bits;     // per: logits of a slice (a multiple of 128); frac_bits: S
     const float   *temperature, *top_p, *min_p, *uniform;
     const int32_t *top_k;
     int32_t       *ids;
     float         *probs;
+    int           *error_flag;
+    uint64_t       wait_limit;
 };
 
 __device__ __forceinline__ uint32_t ordered(float x) { const uint32_t b = __float_as_uint(x + 0.f); return b & 0x80000000u ? ~b : b | 0x80000000u; }   // (-0 and 0 are equals)
@@ -48,6 +51,11 @@ __device__ __forceinline__ uint32_t cluster_ctas() { uint32_t r; asm volatile("m
 __device__ __forceinline__ uint4 cluster_load128(uint32_t addr) {
     uint4 v;
     asm volatile("ld.shared::cluster.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+    return v;
+}
+__device__ __forceinline__ uint32_t cluster_load32(uint32_t addr) {
+    uint32_t v;
+    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
     return v;
 }
 __device__ __forceinline__ uint32_t cluster_add(uint32_t addr, uint32_t n) {
@@ -74,6 +82,7 @@ struct SampleShared {
     uint64_t scan[SA_WARPS];
     uint64_t share[2][SA_MAX_CLUSTER];       // what every CTA of the cluster tells all others
     uint64_t share2[SA_MAX_CLUSTER];
+    uint64_t arrived[SA_PIECES];             // barriers of the slice's pieces
     uint64_t cut, total;
     double   table[32];                      // 2^(i / 32)
     uint32_t n_list;
@@ -84,10 +93,11 @@ struct SampleShared {
 struct Weight {
     const double *table;
     double c, largest;
+    float  least;               // no logit below it has weight: it stands for them, and for -inf
+    bool   edge;                // ... if f32 has such a number near enough; else the exponent itself is bounded
     int    bits;
     __device__ __forceinline__ uint64_t operator()(float x) const {
-        const double z = ((double)x - largest) * c;
-        if (!(z >= -(double)(bits + 1))) { return 0; }                                   // (-inf too)
+        const double z = edge ? fmax(((double)x - largest) * c, -60.0) : ((double)fmaxf(x, least) - largest) * c;   // (NaN reads as no weight)
         const double magic = 6755399441055744.0;                                         // 1.5 x 2^52: the sum's low bits are the rounded integer
         const double t = fma(z, 32.0, magic);
         const int    k = __double2loint(t);
@@ -104,16 +114,30 @@ struct Weight {
     }
 };
 
-template <class T> struct Slice {
+// A slice of the row: in shared memory (NaN is -inf there, and where the largest is +inf it is 0 and all else -inf), or read from where it lies
+template <class T, bool KEPT> struct Slice {
     const T     *row;       // of the slice's first logit
-    const float *kept;      // in shared memory, or null
+    const float *kept;
     int          n, base;
-    bool         inf;       // the largest is +inf: 0 there, -inf elsewhere
+    bool         inf;
     __device__ __forceinline__ float operator()(int i) const {
-        float x;
-        if (kept != nullptr) { x = kept[i]; }
-        else { x = as_float(row[i]); x = x == x ? x : -CUDART_INF_F; }
+        if (KEPT) { return kept[i]; }
+        float x = as_float(row[i]);
+        x = x == x ? x : -CUDART_INF_F;
         return inf ? (x == CUDART_INF_F ? 0.f : -CUDART_INF_F) : x;
+    }
+    // f(logit, place) for this thread's share, four at a time where they are kept (the slice is padded with -inf to whole fours)
+    template <class F> __device__ __forceinline__ void each(const F &f) const { stretch(0, n, threadIdx.x, SA_THREADS, f); }
+    template <class F> __device__ __forceinline__ void stretch(int from, int to, int first, int step, const F &f) const {   // from: a multiple of 4
+        if (KEPT) {
+#pragma unroll 2
+            for (int i = from + 4 * first; i < to; i += 4 * step) {
+                const float4 v = *reinterpret_cast<const float4 *>(kept + i);
+                f(v.x, i); f(v.y, i + 1); f(v.z, i + 2); f(v.w, i + 3);
+            }
+        } else {
+            for (int i = from + first; i < to; i += step) { f((*this)(i), i); }
+        }
     }
 };
 
@@ -130,6 +154,16 @@ __device__ __forceinline__ uint64_t block_upto(uint64_t v, uint64_t *scan, uint6
     *all = sum;
     return upto;
 }
+__device__ __forceinline__ uint64_t block_sum(uint64_t v, uint64_t *scan) {
+    v = warp_sum64(v);
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) { scan[threadIdx.x >> 5] = v; }
+    __syncthreads();
+    uint64_t sum = 0;
+#pragma unroll
+    for (int w = 0; w < SA_WARPS; ++w) { sum += scan[w]; }
+    return sum;
+}
 // v of every CTA to all of the cluster (thread 0's counts), summed after the barrier
 __device__ __forceinline__ uint64_t cluster_total(uint64_t v, uint64_t *slots, uint32_t ctas, uint32_t rank) {
     if (threadIdx.x < ctas) { cluster_store64(cluster_map(smem_u32(slots + rank), threadIdx.x), v); }
@@ -139,7 +173,7 @@ __device__ __forceinline__ uint64_t cluster_total(uint64_t v, uint64_t *slots, u
     return sum;
 }
 // a list of up to SA_LIST keys, the largest first
-__device__ void sort_list(uint64_t *a, int n) {
+__device__ __noinline__ void sort_list(uint64_t *a, int n) {
     int size = 32;
     while (size < n) { size <<= 1; }
     for (int i = n + threadIdx.x; i < size; i += SA_THREADS) { a[i] = 0; }
@@ -155,59 +189,109 @@ __device__ void sort_list(uint64_t *a, int n) {
     }
     __syncthreads();
 }
+__device__ __forceinline__ uint64_t of_total(float share, uint64_t total) {   // the sum on which the number falls, below the total
+    return min((uint64_t)((double)(share > 0.f ? share : 0.f) * (double)total), total - 1);
+}
 
-template <class T>
-__global__ void __launch_bounds__(SA_THREADS) sample_kernel(const __grid_constant__ SampleParams p) {
+template <class T, bool KEPT>
+__global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(const __grid_constant__ SampleParams p) {
     extern __shared__ __align__(16) uint8_t dynamic[];
     SampleShared &sh = *reinterpret_cast<SampleShared *>(dynamic);
     float *slice = reinterpret_cast<float *>(dynamic + sizeof(SampleShared));
+    static_assert(sizeof(SampleShared) % 16 == 0, "the slice is read in pieces of 16 bytes");
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const uint32_t rank = rank_in_cluster(), ctas = cluster_ctas();
     const int row = blockIdx.x / ctas;
     pdl_launch_dependents();
-    for (int i = tid; i < SA_BINS; i += SA_THREADS) { sh.count[i] = sh.limb[0][i] = sh.limb[1][i] = sh.limb[2][i] = 0; }
-    if (tid < 32) { sh.table[tid] = exp2((double)tid / 32); }
-    if (tid == 0) { sh.n_list = 0; sh.cut = 0; sh.found = sh.found2 = 0; }
+    if (tid == 0) {
+        for (int i = 0; i < SA_PIECES; ++i) { mbar_init(smem_u32(sh.arrived + i), 1); }
+        mbar_init_fence();
+        sh.n_list = 0; sh.cut = 0; sh.found = sh.found2 = 0;
+    }
+    *reinterpret_cast<uint4 *>(sh.count + 4 * tid) = make_uint4(0, 0, 0, 0);
     asm volatile("barrier.cluster.arrive.release;" ::: "memory");   // (waited for in front of the first access to another CTA's memory)
     pdl_wait();
 
-    Slice<T> x;
+    Slice<T, KEPT> x;
     x.base = (int)rank * p.per;
     x.n = max(0, min(p.per, p.n_vocab - x.base));
     x.row = static_cast<const T *>(p.logits) + row * p.row_stride + x.base;
-    x.kept = p.cached ? slice : nullptr;
+    x.kept = slice;
     x.inf = false;
+    // pieces of the slice by bulk copies, from whole 16 bytes on
+    const bool bulk = KEPT && sizeof(T) == 4 && (reinterpret_cast<uintptr_t>(x.row) & 15) == 0;
+    const int  whole = bulk ? x.n & ~3 : 0, piece = (whole / SA_PIECES + 3) & ~3;
+    if (bulk && tid == 0) {
+        for (int i = 0; i < SA_PIECES; ++i) {
+            const int from = min(i * piece, whole), n = min(piece, whole - from);
+            if (n > 0) {
+                const uint32_t bar = smem_u32(sh.arrived + i);
+                mbar_expect_tx(bar, n * 4);
+                bulk_copy_g2s(smem_u32(slice + from), x.row + from, n * 4, bar);
+            }
+        }
+    }
+    if (tid < 32) { sh.table[tid] = exp2((double)tid / 32); }
     const float temp = p.temperature ? p.temperature[row] : 1.f, top_p = p.top_p ? p.top_p[row] : 1.f;
     const float min_p = p.min_p ? p.min_p[row] : 0.f, uni = p.uniform ? p.uniform[row] : 0.f;
     const int   top_k = p.top_k ? p.top_k[row] : 0;
 
-    // the slice, and its largest
+    // this thread's largest (of the elements that Slice::each gives it), the row's, and where that is
+    float own = -CUDART_INF_F;
     uint64_t best = 0;
     {
-        float m = -CUDART_INF_F;
-        int   at = -1;
-        auto take = [&](float v, int i) {
-            v = v == v ? v : -CUDART_INF_F;
-            if (p.cached) { slice[i] = v; }
-            if (v > m) { m = v; at = i; }
+        int at = -1;                                       // the first of the four that own is in
+        auto take4 = [&](float4 v, int i) {
+            const float m = fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w));
+            if (m > own) { own = m; at = i; }
         };
-        constexpr int VEC = 16 / sizeof(T);
-        if ((reinterpret_cast<uintptr_t>(x.row) & 15) == 0) {
-            const uint4 *src = reinterpret_cast<const uint4 *>(x.row);
-            const int n_vec = x.n / VEC;
-#pragma unroll 4
-            for (int i = tid; i < n_vec; i += SA_THREADS) {
-                const uint4 raw = __ldcs(src + i);
-                const T *v = reinterpret_cast<const T *>(&raw);
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) { take(as_float(v[e]), i * VEC + e); }
+        if (bulk) {
+            __syncthreads();                               // (the barriers are there)
+            bool ok = true;
+            for (int q = 0; q < SA_PIECES; ++q) {
+                const int from = min(q * piece, whole), to = min(from + piece, whole);
+                if (from < to) { ok &= mbar_wait_prompt(smem_u32(sh.arrived + q), 0, p.wait_limit); }
+                // every thread meets the fours that it meets in the passes to come
+                const int first = (from / 4 - tid + SA_THREADS - 1) / SA_THREADS * SA_THREADS + tid;
+                for (int i = 4 * max(first, tid); i < to; i += 4 * SA_THREADS) {
+                    float4 v = *reinterpret_cast<const float4 *>(slice + i);
+                    if (!(v.x == v.x && v.y == v.y && v.z == v.z && v.w == v.w)) {
+                        v = make_float4(v.x == v.x ? v.x : -CUDART_INF_F, v.y == v.y ? v.y : -CUDART_INF_F, v.z == v.z ? v.z : -CUDART_INF_F, v.w == v.w ? v.w : -CUDART_INF_F);
+                        *reinterpret_cast<float4 *>(slice + i) = v;
+                    }
+                    take4(v, i);
+                }
             }
-            for (int i = n_vec * VEC + tid; i < x.n; i += SA_THREADS) { take(as_float(x.row[i]), i); }
+            if (!ok) {   // reported; what is on its way lands first, or is given a last chance to
+                for (int q = 0; q < SA_PIECES; ++q) { if (min(q * piece, whole) < whole) { mbar_wait_bounded(smem_u32(sh.arrived + q), 0, p.wait_limit); } }
+                if (lane == 0 && p.error_flag != nullptr) { atomicExch(p.error_flag, 1); }
+            }
+            if (whole < x.n && tid == (whole / 4) % SA_THREADS) {
+                float v[4];
+                for (int e = 0; e < 4; ++e) { v[e] = whole + e < x.n ? as_float(x.row[whole + e]) : -CUDART_INF_F; v[e] = v[e] == v[e] ? v[e] : -CUDART_INF_F; }
+                *reinterpret_cast<float4 *>(slice + whole) = make_float4(v[0], v[1], v[2], v[3]);
+                take4(make_float4(v[0], v[1], v[2], v[3]), whole);
+            }
+        } else if (KEPT) {
+#pragma unroll 2
+            for (int i = 4 * tid; i < x.n; i += 4 * SA_THREADS) {
+                float v[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) { v[e] = i + e < x.n ? as_float(x.row[i + e]) : -CUDART_INF_F; v[e] = v[e] == v[e] ? v[e] : -CUDART_INF_F; }
+                *reinterpret_cast<float4 *>(slice + i) = make_float4(v[0], v[1], v[2], v[3]);
+                take4(make_float4(v[0], v[1], v[2], v[3]), i);
+            }
         } else {
 #pragma unroll 4
-            for (int i = tid; i < x.n; i += SA_THREADS) { take(as_float(x.row[i]), i); }
+            for (int i = tid; i < x.n; i += SA_THREADS) {
+                const float v = x(i);
+                if (v > own) { own = v; at = i; }
+            }
         }
-        if (at >= 0) { best = key_of(m, x.base + at); }
+        if (at >= 0) {
+            if (KEPT) { at = slice[at] == own ? at : slice[at + 1] == own ? at + 1 : slice[at + 2] == own ? at + 2 : at + 3; }
+            best = key_of(own, x.base + at);
+        }
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) { best = max(best, __shfl_xor_sync(0xffffffffu, best, o)); }
         if (lane == 0) { sh.scan[warp] = best; }
@@ -228,10 +312,19 @@ __global__ void __launch_bounds__(SA_THREADS) sample_kernel(const __grid_constan
         return;
     }
     float largest = value_of(best);
-    if (largest == CUDART_INF_F) { x.inf = true; largest = 0.f; }
+    if (largest == CUDART_INF_F) {
+        x.inf = true; largest = 0.f;
+        own = own == CUDART_INF_F ? 0.f : -CUDART_INF_F;
+        if (KEPT) {
+            for (int i = tid; i < ((x.n + 3) & ~3); i += SA_THREADS) { slice[i] = slice[i] == CUDART_INF_F ? 0.f : -CUDART_INF_F; }
+            __syncthreads();
+        }
+    }
     Weight weight;
     weight.table = sh.table; weight.bits = p.frac_bits; weight.largest = largest;
-    weight.c = fmin(1.4426950408889634073599 / (double)temp, 1e30);
+    weight.c = fmax(fmin(1.4426950408889634073599 / (double)temp, 1e30), 1e-30);
+    const double lowest = (double)largest - 60 / weight.c;                                  // weight 2^-60, and with it all below, rounds to 0
+    weight.edge = lowest < -3.4e38 || fabs((double)largest) * weight.c > 8e6; weight.least = weight.edge ? 0.f : (float)lowest;   // (f32 spacing: 2^-23 of the largest)
     const double one = exp2((double)p.frac_bits);
     const uint64_t least = min_p > 0.f ? (uint64_t)max(1.0, ceil((double)fminf(min_p, 1.f) * one)) : 1;
     const float  bin_scale = (float)(weight.c * (SA_BINS / (double)(p.frac_bits + 1)));
@@ -241,47 +334,60 @@ __global__ void __launch_bounds__(SA_THREADS) sample_kernel(const __grid_constan
     uint64_t cut = 0;                        // keys from here on stay
     bool     search = false;                 // ... by the slow way
 
-    // gives the first CTA all elements that `wanted` names; false when they do not fit (all CTAs know)
-    auto gather = [&](auto wanted) {
-        const uint32_t counter = cluster_map(smem_u32(&sh.n_list), 0), list = cluster_map(smem_u32(sh.list), 0);
-        for (int i0 = warp * 32; i0 < x.n; i0 += SA_THREADS) {
-            const int i = i0 + lane;
-            const float v = i < x.n ? x(i) : -CUDART_INF_F;
-            const bool in = i < x.n && wanted(v);
-            const unsigned mask = __ballot_sync(0xffffffffu, in);
-            if (mask == 0) { continue; }
-            uint32_t at = 0;
-            if (lane == 0) { at = cluster_add(counter, __popc(mask)); }
-            at = __shfl_sync(0xffffffffu, at, 0) + __popc(mask & ((1u << lane) - 1));
-            if (in && at < SA_LIST) { cluster_store64(list + at * 8, key_of(v, x.base + i)); }
-        }
+    // the whole row's counts, four bins a thread
+    auto counts = [&]() {
         cluster_sync();
-    };
-    // the sum over all keys from `from` on that are not below `low`
-    auto sum_from = [&](uint64_t from, bool counts, int turn) {
-        uint64_t s = 0;
-        for (int i = tid; i < x.n; i += SA_THREADS) {
-            const float v = x(i);
-            if (v != -CUDART_INF_F && key_of(v, x.base + i) >= from) { s += counts ? 1 : weight(v); }
-        }
-        uint64_t all;
-        block_upto(s, sh.scan, &all);
-        return cluster_total(all, sh.share[turn & 1], ctas, rank);
-    };
-
-    if (by_k || by_p) {
-        __syncthreads();
-        for (int i = tid; i < x.n; i += SA_THREADS) {
-            const float b = bin_of(x(i));
-            if (b < (float)SA_BINS) { atomicAdd(&sh.count[(int)b], 1u); }
-        }
-        cluster_sync();
-        uint4 n4 = make_uint4(0, 0, 0, 0);               // four bins a thread, of the whole row
+        uint4 n4 = make_uint4(0, 0, 0, 0);
         for (uint32_t r = 0; r < ctas; ++r) {
             const uint4 v = cluster_load128(cluster_map(smem_u32(sh.count) + tid * 16, r));
             n4.x += v.x; n4.y += v.y; n4.z += v.z; n4.w += v.w;
         }
-        if (by_k) {
+        return n4;
+    };
+    auto count_all = [&]() {
+        x.each([&](float v, int) {
+            const float b = bin_of(v);
+            if (b < (float)SA_BINS) { atomicAdd(&sh.count[(int)b], 1u); }
+        });
+    };
+    // elements that `wanted` names, of the threads whose largest is wanted, to the first CTA; how many there are (more than SA_LIST: they do not fit)
+    auto gather = [&](bool mine, auto wanted) {
+        const uint32_t counter = cluster_map(smem_u32(&sh.n_list), 0), list = cluster_map(smem_u32(sh.list), 0);
+        if (mine) {
+            x.each([&](float v, int i) {
+                if (!wanted(v)) { return; }
+                const uint32_t at = cluster_add(counter, 1);
+                if (at < SA_LIST) { cluster_store64(list + at * 8, key_of(v, x.base + i)); }
+            });
+        }
+        cluster_sync();
+        return cluster_load32(counter);
+    };
+    // the sum over all keys from `from` on
+    auto sum_from = [&](uint64_t from, bool counting, int turn) {
+        uint64_t s = 0;
+        x.each([&](float v, int i) {
+            if (v != -CUDART_INF_F && key_of(v, x.base + i) >= from) { s += counting ? 1 : weight(v); }
+        });
+        return cluster_total(block_sum(s, sh.scan), sh.share[turn & 1], ctas, rank);
+    };
+
+    if (by_k) {
+        const bool quick = top_k <= (int)(SA_THREADS * ctas) / 8;            // by the threads' maxima first
+        for (int all_of_them = quick ? 0 : 1; all_of_them < 2; ++all_of_them) {
+            if (all_of_them) {
+                if (quick) {
+                    cluster_sync();                                           // (nobody reads the first counts any more)
+                    *reinterpret_cast<uint4 *>(sh.count + 4 * tid) = make_uint4(0, 0, 0, 0);
+                    if (tid == 0) { sh.n_list = 0; }
+                    __syncthreads();
+                }
+                count_all();
+            } else {
+                const float b = bin_of(own);
+                if (b < (float)SA_BINS) { atomicAdd(&sh.count[(int)b], 1u); }
+            }
+            const uint4 n4 = counts();
             uint64_t all;
             const uint64_t upto = block_upto((uint64_t)n4.x + n4.y + n4.z + n4.w, sh.scan, &all);
             const uint64_t before = upto - n4.x - n4.y - n4.z - n4.w, want = min((uint64_t)top_k, all);
@@ -293,130 +399,172 @@ __global__ void __launch_bounds__(SA_THREADS) sample_kernel(const __grid_constan
                 sh.found = b; sh.found2 = (int)min(c, (uint64_t)SA_LIST + 1);
             }
             __syncthreads();
-            const int last_bin = sh.found, n = sh.found2;
-            if (n <= SA_LIST) {
-                gather([&](float v) { return bin_of(v) < (float)(last_bin + 1); });
-                if (rank != 0) { return; }
-                // everything else is the first CTA's: sorted, cut from the end, put back into the order of indices, drawn
-                sort_list(sh.list, n);
-                const int n1 = min(n, top_k);
-                uint64_t w0 = 0, w1 = 0, k0 = 0, k1 = 0, all_w;
-                if (2 * tid < n1) { k0 = sh.list[2 * tid]; w0 = weight(value_of(k0)); }
-                if (2 * tid + 1 < n1) { k1 = sh.list[2 * tid + 1]; w1 = weight(value_of(k1)); }
-                const uint64_t up = block_upto(w0 + w1, sh.scan, &all_w);
-                const uint64_t stop = by_p ? reach(all_w) : ~0ull;
-                const bool in0 = 2 * tid < n1 && up - w1 - w0 < stop && w0 >= least, in1 = 2 * tid + 1 < n1 && up - w1 < stop && w1 >= least;
-                uint64_t kept;
-                const uint64_t kept_upto = block_upto((in0 ? 1 : 0) + (in1 ? 1 : 0), sh.scan, &kept);   // (a prefix of the list)
-                (void)kept_upto;
-                uint64_t sum;
-                block_upto((in0 ? w0 : 0) + (in1 ? w1 : 0), sh.scan, &sum);
-                // by index: the key's low bits, ascending as descending complements; the weights are found again from their place in the sorted list
-                uint64_t *by_index = sh.list, *weights = reinterpret_cast<uint64_t *>(sh.limb);
+            const float last_bin = (float)(sh.found + 1);
+            uint32_t n = SA_LIST + 1;
+            if (all_of_them ? sh.found2 <= SA_LIST : all >= (uint64_t)top_k) {
+                n = gather(bin_of(own) < last_bin, [&](float v) { return bin_of(v) < last_bin; });
+            }
+            if (n > SA_LIST) { continue; }
+            cluster_sync();                                                   // (all have read how many there are)
+            if (rank != 0) { return; }
+            // everything else is the first CTA's
+            const int n_list = (int)n;
+            if (n_list <= SA_RANKED) {
+                // few candidates: a group of threads ranks each, by counting and weighing what is in front of it - first in the order of weights, then of indices
+                int per = 512 / SA_RANKED;
+                while (per < 32 && n_list * per * 2 <= SA_THREADS) { per *= 2; }
+                const int i = tid / per, part = tid & (per - 1);
+                const bool is = i < n_list;
+                const uint64_t key = is ? sh.list[i] : 0;
+                uint64_t *weights = reinterpret_cast<uint64_t *>(sh.limb);
+                uint64_t w = 0;
+                if (is) { w = weight(value_of(key)); if (part == 0) { weights[i] = w; } }
                 __syncthreads();
+                auto group_sum = [&](uint64_t v) {
+                    for (int o = 1; o < per; o <<= 1) { v += __shfl_xor_sync(0xffffffffu, v, o); }
+                    return v;
+                };
+                uint64_t in_front = 0, before_w = 0;
+                if (is) {
+                    for (int j = part; j < n_list; j += per) { if (sh.list[j] > key) { ++in_front; before_w += weights[j]; } }
+                }
+                in_front = group_sum(in_front); before_w = group_sum(before_w);
+                bool stays = is && in_front < (uint64_t)top_k;
+                const uint64_t total_k = block_sum(stays && part == 0 ? w : 0, sh.scan);
+                stays = stays && (!by_p || before_w < reach(total_k)) && w >= least;
+                if (is && part == 0 && !stays) { weights[i] = 0; }
+                const uint64_t sum = block_sum(stays && part == 0 ? w : 0, sh.scan);          // (its barriers are between the writes above and the reads below)
+                const uint64_t t = of_total(uni, sum);
+                uint64_t upto_w = 0;
                 constexpr uint64_t low = (1 << SA_INDEX_BITS) - 1;
-                if (in0) { by_index[2 * tid] = ((k0 & low) << 11 | (2 * tid)) + 1; weights[2 * tid] = w0; }
-                if (in1) { by_index[2 * tid + 1] = ((k1 & low) << 11 | (2 * tid + 1)) + 1; weights[2 * tid + 1] = w1; }
-                sort_list(by_index, (int)kept);
-                uint64_t v0 = 0, v1 = 0, p0 = 0, p1 = 0, ignore;
-                if (2 * tid < (int)kept) { p0 = by_index[2 * tid] - 1; v0 = weights[p0 & 2047]; }
-                if (2 * tid + 1 < (int)kept) { p1 = by_index[2 * tid + 1] - 1; v1 = weights[p1 & 2047]; }
-                const uint64_t upto2 = block_upto(v0 + v1, sh.scan, &ignore);
-                const uint64_t t = min((uint64_t)((double)(uni > 0.f ? uni : 0.f) * (double)sum), sum - 1);
-                const bool hit0 = v0 > 0 && upto2 - v1 - v0 <= t && t < upto2 - v1, hit1 = v1 > 0 && upto2 - v1 <= t && t < upto2;
-                if (hit0 || hit1) {
-                    p.ids[row] = (int)(low - ((hit0 ? p0 : p1) >> 11));
-                    if (p.probs) { p.probs[row] = (float)((double)(hit0 ? v0 : v1) / (double)sum); }
+                if (stays) {
+                    for (int j = part; j < n_list; j += per) { if ((sh.list[j] & low) > (key & low)) { upto_w += weights[j]; } }
+                }
+                upto_w = group_sum(upto_w);
+                if (stays && part == 0 && upto_w <= t && t < upto_w + w) {
+                    p.ids[row] = index_of(key);
+                    if (p.probs) { p.probs[row] = (float)((double)w / (double)sum); }
                 }
                 return;
             }
-            search = true;
-        } else {
-            // what the bins weigh, to 0.8 %: the bins in which top_p may be reached
-            const float step = -(float)(p.frac_bits + 1) / SA_BINS;     // log2 of a weight, a bin
-            const float w[4] = {exp2f(step * (4 * tid + 0.5f)), exp2f(step * (4 * tid + 1.5f)), exp2f(step * (4 * tid + 2.5f)), exp2f(step * (4 * tid + 3.5f))};
-            const uint32_t n[4] = {n4.x, n4.y, n4.z, n4.w};
-            uint64_t m[4], all;
+            // sorted, cut from the end, put back into the order of indices, drawn
+            sort_list(sh.list, n_list);
+            const int n1 = min(n_list, top_k);
+            uint64_t w0 = 0, w1 = 0, k0 = 0, k1 = 0, all_w;
+            if (2 * tid < n1) { k0 = sh.list[2 * tid]; w0 = weight(value_of(k0)); }
+            if (2 * tid + 1 < n1) { k1 = sh.list[2 * tid + 1]; w1 = weight(value_of(k1)); }
+            const uint64_t up = block_upto(w0 + w1, sh.scan, &all_w);
+            const uint64_t stop = by_p ? reach(all_w) : ~0ull;
+            const bool in0 = 2 * tid < n1 && up - w1 - w0 < stop && w0 >= least, in1 = 2 * tid + 1 < n1 && up - w1 < stop && w1 >= least;
+            const uint64_t kept = block_sum((in0 ? 1 : 0) + (in1 ? 1 : 0), sh.scan);          // (a prefix of the list)
+            const uint64_t sum = block_sum((in0 ? w0 : 0) + (in1 ? w1 : 0), sh.scan);
+            // by index: the key's low bits, ascending as descending complements; the weights are found again from their place in the sorted list
+            uint64_t *by_index = sh.list, *weights = reinterpret_cast<uint64_t *>(sh.limb);
+            __syncthreads();
+            constexpr uint64_t low = (1 << SA_INDEX_BITS) - 1;
+            if (in0) { by_index[2 * tid] = ((k0 & low) << 11 | (2 * tid)) + 1; weights[2 * tid] = w0; }
+            if (in1) { by_index[2 * tid + 1] = ((k1 & low) << 11 | (2 * tid + 1)) + 1; weights[2 * tid + 1] = w1; }
+            sort_list(by_index, (int)kept);
+            uint64_t v0 = 0, v1 = 0, p0 = 0, p1 = 0, ignore;
+            if (2 * tid < (int)kept) { p0 = by_index[2 * tid] - 1; v0 = weights[p0 & 2047]; }
+            if (2 * tid + 1 < (int)kept) { p1 = by_index[2 * tid + 1] - 1; v1 = weights[p1 & 2047]; }
+            const uint64_t upto2 = block_upto(v0 + v1, sh.scan, &ignore);
+            const uint64_t t = of_total(uni, sum);
+            const bool hit0 = v0 > 0 && upto2 - v1 - v0 <= t && t < upto2 - v1, hit1 = v1 > 0 && upto2 - v1 <= t && t < upto2;
+            if (hit0 || hit1) {
+                p.ids[row] = (int)(low - ((hit0 ? p0 : p1) >> 11));
+                if (p.probs) { p.probs[row] = (float)((double)(hit0 ? v0 : v1) / (double)sum); }
+            }
+            return;
+        }
+        search = true;
+    } else if (by_p) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) { m[e] = (uint64_t)((double)w[e] * n[e] * 1099511627776.0); }   // x 2^40
-            const uint64_t upto = block_upto(m[0] + m[1] + m[2] + m[3], sh.scan, &all);
-            const double   goal = (double)max(top_p, 0.f) * (double)all;
-            const uint64_t lo = (uint64_t)(0.98 * goal), hi = min((uint64_t)(1.02 * goal), all);
-            uint64_t c = upto - m[0] - m[1] - m[2] - m[3];
-            if (tid == 0) { sh.found = 0; sh.found2 = SA_BINS - 1; }
-            __syncthreads();
+        for (int i = 0; i < 3; ++i) { *reinterpret_cast<uint4 *>(sh.limb[i] + 4 * tid) = make_uint4(0, 0, 0, 0); }
+        count_all();
+        const uint4 n4 = counts();
+        // what the bins weigh, to 0.8 %: the bins in which top_p may be reached
+        const float step = -(float)(p.frac_bits + 1) / SA_BINS;     // log2 of a weight, a bin
+        const float w[4] = {exp2f(step * (4 * tid + 0.5f)), exp2f(step * (4 * tid + 1.5f)), exp2f(step * (4 * tid + 2.5f)), exp2f(step * (4 * tid + 3.5f))};
+        const uint32_t n[4] = {n4.x, n4.y, n4.z, n4.w};
+        uint64_t m[4], all;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                if (c < lo && lo <= c + m[e]) { sh.found = 4 * tid + e; }
-                if (c < hi && hi <= c + m[e]) { sh.found2 = min(4 * tid + e + 1, SA_BINS - 1); }
-                c += m[e];
-            }
-            __syncthreads();
-            const int   first = sh.found, last = sh.found2;
-            const float sub_scale = (float)SA_BINS / (float)(last + 1 - first);
-            auto sub_of = [&](float b) { return min(SA_BINS - 1, (int)((b - (float)first) * sub_scale)); };
-            uint64_t front = 0, rest = 0;
-            for (int i = tid; i < x.n; i += SA_THREADS) {
-                const float v = x(i), b = bin_of(v);
-                const uint64_t ww = weight(v);
-                if (b < (float)first) { front += ww; }
-                else if (b < (float)(last + 1)) {
-                    const int s = sub_of(b);
-                    rest += ww;
-                    atomicAdd(&sh.limb[0][s], (uint32_t)(ww & 0x7fff));
-                    atomicAdd(&sh.limb[1][s], (uint32_t)(ww >> 15) & 0x7fff);
-                    if (ww >> 30) { atomicAdd(&sh.limb[2][s], (uint32_t)(ww >> 30)); }
-                } else { rest += ww; }
-            }
-            uint64_t mine, others;
-            block_upto(front, sh.scan, &mine);
-            block_upto(rest, sh.scan, &others);
-            if (tid < (int)ctas) { cluster_store64(cluster_map(smem_u32(sh.share[1] + rank), tid), mine); cluster_store64(cluster_map(smem_u32(sh.share2 + rank), tid), others); }
-            cluster_sync();
-            front = rest = 0;
-            for (uint32_t r = 0; r < ctas; ++r) { front += sh.share[1][r]; rest += sh.share2[r]; }
-            uint64_t q[4] = {0, 0, 0, 0};
-            for (uint32_t r = 0; r < ctas; ++r) {
-                const uint4 a = cluster_load128(cluster_map(smem_u32(sh.limb[0]) + tid * 16, r)), b = cluster_load128(cluster_map(smem_u32(sh.limb[1]) + tid * 16, r)),
-                            d = cluster_load128(cluster_map(smem_u32(sh.limb[2]) + tid * 16, r));
-                q[0] += a.x + ((uint64_t)b.x << 15) + ((uint64_t)d.x << 30); q[1] += a.y + ((uint64_t)b.y << 15) + ((uint64_t)d.y << 30);
-                q[2] += a.z + ((uint64_t)b.z << 15) + ((uint64_t)d.z << 30); q[3] += a.w + ((uint64_t)b.w << 15) + ((uint64_t)d.w << 30);
-            }
-            const uint64_t stop = reach(front + rest);
-            const uint64_t upto_s = block_upto(q[0] + q[1] + q[2] + q[3], sh.scan, &all);
-            if (tid == 0) { sh.found = -1; }
-            __syncthreads();
-            c = front + upto_s - q[0] - q[1] - q[2] - q[3];
+        for (int e = 0; e < 4; ++e) { m[e] = (uint64_t)((double)w[e] * n[e] * 1099511627776.0); }   // x 2^40
+        const uint64_t upto = block_upto(m[0] + m[1] + m[2] + m[3], sh.scan, &all);
+        const double   goal = (double)max(top_p, 0.f) * (double)all;
+        const uint64_t lo = (uint64_t)(0.98 * goal), hi = min((uint64_t)(1.02 * goal), all);
+        uint64_t c = upto - m[0] - m[1] - m[2] - m[3];
+        if (tid == 0) { sh.found = 0; sh.found2 = SA_BINS - 1; }
+        __syncthreads();
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                if (c < stop && stop <= c + q[e]) { sh.found = 4 * tid + e; sh.total = c; }
-                c += q[e];
+        for (int e = 0; e < 4; ++e) {
+            if (c < lo && lo <= c + m[e]) { sh.found = 4 * tid + e; }
+            if (c < hi && hi <= c + m[e]) { sh.found2 = min(4 * tid + e + 1, SA_BINS - 1); }
+            c += m[e];
+        }
+        __syncthreads();
+        const float first = (float)sh.found, behind = (float)(sh.found2 + 1);
+        const float sub_scale = (float)SA_BINS / (behind - first);
+        auto sub_of = [&](float b) { return min(SA_BINS - 1, (int)((b - first) * sub_scale)); };
+        uint64_t front = 0, total = 0;
+        x.each([&](float v, int) {
+            const float b = bin_of(v);
+            const uint64_t ww = weight(v);
+            total += ww;
+            front += b < first ? ww : 0;
+            if (b >= first && b < behind) {
+                const int s = sub_of(b);
+                atomicAdd(&sh.limb[0][s], (uint32_t)(ww & 0x7fff));
+                atomicAdd(&sh.limb[1][s], (uint32_t)(ww >> 15) & 0x7fff);
+                if (ww >> 30) { atomicAdd(&sh.limb[2][s], (uint32_t)(ww >> 30)); }
             }
-            __syncthreads();
-            const int sub = sh.found;
-            if (sub < 0) { search = true; }              // (not reached inside the bracket)
-            else {
-                gather([&](float v) { const float b = bin_of(v); return b >= (float)first && b < (float)(last + 1) && sub_of(b) == sub; });
-                // the first CTA finds the last one that stays and tells all
-                if (rank == 0) {
-                    const int nn = (int)min(sh.n_list, (uint32_t)SA_LIST + 1);
-                    uint64_t found = 0;
-                    if (nn <= SA_LIST) {
-                        sort_list(sh.list, nn);
-                        uint64_t w0 = 0, w1 = 0, ignore;
-                        if (2 * tid < nn) { w0 = weight(value_of(sh.list[2 * tid])); }
-                        if (2 * tid + 1 < nn) { w1 = weight(value_of(sh.list[2 * tid + 1])); }
-                        const uint64_t up = sh.total + block_upto(w0 + w1, sh.scan, &ignore);
-                        uint64_t n_in;
-                        block_upto((2 * tid < nn && up - w1 - w0 < stop ? 1 : 0) + (2 * tid + 1 < nn && up - w1 < stop ? 1 : 0), sh.scan, &n_in);
-                        found = n_in > 0 ? sh.list[n_in - 1] : 0;
-                    }
-                    if (tid < (int)ctas) { cluster_store64(cluster_map(smem_u32(&sh.cut), tid), found); }
+        });
+        front = block_sum(front, sh.scan);
+        total = block_sum(total, sh.scan);
+        if (tid < (int)ctas) { cluster_store64(cluster_map(smem_u32(sh.share[1] + rank), tid), front); cluster_store64(cluster_map(smem_u32(sh.share2 + rank), tid), total); }
+        cluster_sync();
+        front = total = 0;
+        for (uint32_t r = 0; r < ctas; ++r) { front += sh.share[1][r]; total += sh.share2[r]; }
+        uint64_t q[4] = {0, 0, 0, 0};
+        for (uint32_t r = 0; r < ctas; ++r) {
+            const uint4 a = cluster_load128(cluster_map(smem_u32(sh.limb[0]) + tid * 16, r)), b = cluster_load128(cluster_map(smem_u32(sh.limb[1]) + tid * 16, r)),
+                        d = cluster_load128(cluster_map(smem_u32(sh.limb[2]) + tid * 16, r));
+            q[0] += a.x + ((uint64_t)b.x << 15) + ((uint64_t)d.x << 30); q[1] += a.y + ((uint64_t)b.y << 15) + ((uint64_t)d.y << 30);
+            q[2] += a.z + ((uint64_t)b.z << 15) + ((uint64_t)d.z << 30); q[3] += a.w + ((uint64_t)b.w << 15) + ((uint64_t)d.w << 30);
+        }
+        const uint64_t stop = reach(total);
+        const uint64_t upto_s = block_upto(q[0] + q[1] + q[2] + q[3], sh.scan, &all);
+        if (tid == 0) { sh.found = -1; }
+        __syncthreads();
+        c = front + upto_s - q[0] - q[1] - q[2] - q[3];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            if (c < stop && stop <= c + q[e]) { sh.found = 4 * tid + e; sh.total = c; }
+            c += q[e];
+        }
+        __syncthreads();
+        const int sub = sh.found;
+        if (sub < 0) { search = true; }              // (not reached inside the bracket)
+        else {
+            const uint32_t n_in_bin = gather(bin_of(own) < behind, [&](float v) { const float b = bin_of(v); return b >= first && b < behind && sub_of(b) == sub; });
+            // the first CTA finds the last one that stays and tells all
+            if (rank == 0) {
+                const int nn = (int)min(n_in_bin, (uint32_t)SA_LIST + 1);
+                uint64_t found = 0;
+                if (nn <= SA_LIST) {
+                    sort_list(sh.list, nn);
+                    uint64_t w0 = 0, w1 = 0, ignore;
+                    if (2 * tid < nn) { w0 = weight(value_of(sh.list[2 * tid])); }
+                    if (2 * tid + 1 < nn) { w1 = weight(value_of(sh.list[2 * tid + 1])); }
+                    const uint64_t up = sh.total + block_upto(w0 + w1, sh.scan, &ignore);
+                    const uint64_t n_in = block_sum((2 * tid < nn && up - w1 - w0 < stop ? 1 : 0) + (2 * tid + 1 < nn && up - w1 < stop ? 1 : 0), sh.scan);
+                    found = n_in > 0 ? sh.list[n_in - 1] : 0;
                 }
-                cluster_sync();
-                cut = sh.cut;
-                search = cut == 0;
+                if (tid < (int)ctas) { cluster_store64(cluster_map(smem_u32(&sh.cut), tid), found); }
             }
+            cluster_sync();
+            cut = sh.cut;
+            search = cut == 0;
         }
     }
     if (search) {
@@ -424,28 +572,32 @@ __global__ void __launch_bounds__(SA_THREADS) sample_kernel(const __grid_constan
         cluster_sync();                                   // (nobody reads the shares of an earlier exchange any more)
         if (by_k) {
             for (int bit = 31 + SA_INDEX_BITS; bit >= 0; --bit) {
-                if (sum_from(cut | 1ull << bit, true, turn++) >= (uint64_t)top_k) { cut |= 1ull << bit; }
+                if (sum_from(cut | (uint64_t)1 << bit, true, turn++) >= (uint64_t)top_k) { cut |= (uint64_t)1 << bit; }
             }
         }
         if (by_p) {
             const uint64_t floor = cut, stop = reach(sum_from(floor, false, turn++));
             cut = 0;
             for (int bit = 31 + SA_INDEX_BITS; bit >= 0; --bit) {
-                if (sum_from(max(floor, cut | (uint64_t)1 << bit), false, turn++) >= stop) { cut |= 1ull << bit; }
+                if (sum_from(max(floor, cut | (uint64_t)1 << bit), false, turn++) >= stop) { cut |= (uint64_t)1 << bit; }
             }
             cut = max(cut, floor);
         }
     }
 
     // draw: warps have contiguous stretches
-    const int stretch = ((x.n + SA_WARPS - 1) / SA_WARPS + 31) & ~31, from = min(warp * stretch, x.n), to = min(from + stretch, x.n);
-    auto stays = [&](int i, float v) {
-        if (key_of(v, x.base + i) < cut) { return (uint64_t)0; }
+    const int stretch = ((x.n + SA_WARPS - 1) / SA_WARPS + 127) & ~127, from = min(warp * stretch, x.n), to = min(from + stretch, x.n);
+    const float cut_value = cut == 0 ? -CUDART_INF_F : value_of(cut);
+    const int   cut_index = cut == 0 ? p.n_vocab : index_of(cut);
+    auto stays = [&](float v, int i) {
         const uint64_t w = weight(v);
-        return w >= least ? w : (uint64_t)0;
+        return (v > cut_value || (v == cut_value && x.base + i <= cut_index)) && w >= least ? w : (uint64_t)0;
     };
     uint64_t s = 0;
-    for (int i = from + lane; i < to; i += 32) { s += stays(i, x(i)); }
+    if (cut == 0 && least == 1) { x.stretch(from, to, lane, 32, [&](float v, int) { s += weight(v); }); }
+    else {
+        x.stretch(from, to, lane, 32, [&](float v, int i) { if (v >= cut_value) { s += stays(v, i); } });
+    }
     s = warp_sum64(s);
     __syncthreads();
     if (lane == 0) { sh.scan[warp] = s; }
@@ -456,12 +608,12 @@ __global__ void __launch_bounds__(SA_THREADS) sample_kernel(const __grid_constan
     cluster_sync();                                       // (shares of earlier exchanges are read)
     const uint64_t total = cluster_total(mine, sh.share[0], ctas, rank);
     for (uint32_t r = 0; r < rank; ++r) { before += sh.share[0][r]; }
-    const uint64_t t = min((uint64_t)((double)(uni > 0.f ? uni : 0.f) * (double)total), total - 1);
+    const uint64_t t = of_total(uni, total);
     if (before <= t && t < before + s) {
         uint64_t c = before;
         for (int i0 = from; i0 < to; i0 += 32) {
             const int i = i0 + lane;
-            const uint64_t w = i < to ? stays(i, x(i)) : 0, upto = c + warp_upto64(w);
+            const uint64_t w = i < to ? stays(x(i), i) : 0, upto = c + warp_upto64(w);
             const unsigned hit = __ballot_sync(0xffffffffu, t < upto);
             if (hit) {
                 if (lane == __ffs(hit) - 1) {
@@ -475,15 +627,10 @@ __global__ void __launch_bounds__(SA_THREADS) sample_kernel(const __grid_constan
     }
 }
 
-template <class T>
-cudaError_t launch_sample(SampleParams &p, int n_rows, const LaunchCfg &cfg) {
-    // CTAs of a row: slices of about 4096 logits (8 for 32 000 and more); slices that fit are kept
-    int ctas = 1;
-    while (ctas < SA_MAX_CLUSTER && p.n_vocab > 4096 * ctas) { ctas *= 2; }
-    p.per = ((p.n_vocab + ctas - 1) / ctas + 31) & ~31;
-    p.cached = (size_t)p.per <= SA_MAX_SLICE;
-    const size_t smem = sizeof(SampleShared) + (p.cached ? (size_t)p.per * 4 : 0);
-    const void *kernel = reinterpret_cast<const void *>(sample_kernel<T>);
+template <class T, bool KEPT>
+cudaError_t launch_sample(SampleParams &p, int n_rows, int ctas, const LaunchCfg &cfg) {
+    const size_t smem = sizeof(SampleShared) + (KEPT ? (size_t)p.per * 4 : 0);
+    const void *kernel = reinterpret_cast<const void *>(sample_kernel<T, KEPT>);
     const cudaError_t err = allow_dynamic_smem(kernel, smem);
     if (err != cudaSuccess) { return err; }
     cudaLaunchConfig_t lc = {};
@@ -496,6 +643,14 @@ cudaError_t launch_sample(SampleParams &p, int n_rows, const LaunchCfg &cfg) {
     lc.attrs = attr; lc.numAttrs = cfg.pdl ? 2 : 1;
     void *args[] = {&p};
     return cudaLaunchKernelExC(&lc, kernel, args);
+}
+template <class T>
+cudaError_t launch_sample(SampleParams &p, int n_rows, int sms, const LaunchCfg &cfg) {
+    // slices of up to 16384 logits, so that an SM holds two CTAs; smaller ones while there are SMs without a CTA
+    int ctas = 1;
+    while (ctas < SA_MAX_CLUSTER && (p.n_vocab > 16384 * ctas || (n_rows * ctas < sms && p.n_vocab > 2048 * ctas))) { ctas *= 2; }
+    p.per = ((p.n_vocab + ctas - 1) / ctas + 127) & ~127;
+    return (size_t)p.per <= SA_MAX_SLICE ? launch_sample<T, true>(p, n_rows, ctas, cfg) : launch_sample<T, false>(p, n_rows, ctas, cfg);
 }
 
 }  // namespace
@@ -533,7 +688,8 @@ extern "C" spyb_status spyb_sample(spyb_backend *be, const spyb_sample_desc *d) 
     while ((1 << log2_vocab) < d->n_vocab) { ++log2_vocab; }
     p.frac_bits = std::min(45, 62 - log2_vocab);
     p.temperature = d->temperature; p.top_k = d->top_k; p.top_p = d->top_p; p.min_p = d->min_p; p.uniform = d->uniform; p.ids = d->ids; p.probs = d->probs;
+    p.error_flag = be->d_error_flag; p.wait_limit = be->wait_limit_ns;
     const LaunchCfg cfg = be->launch_cfg(be->config.use_pdl != 0);
-    SPYB_CUDA(be, d->number_type == SPYB_FP32 ? launch_sample<float>(p, d->n_rows, cfg) : launch_sample<__half>(p, d->n_rows, cfg));
+    SPYB_CUDA(be, d->number_type == SPYB_FP32 ? launch_sample<float>(p, d->n_rows, be->num_sms_total, cfg) : launch_sample<__half>(p, d->n_rows, be->num_sms_total, cfg));
     return SPYB_SUCCESS;
 }
