@@ -16,8 +16,8 @@ namespace {
 // a histogram's too, and a weight's error of 2^-46 moves a border of the sums by about 2^-37 at most. An exponential to 2^-48 costs 13 operations in 64 bits
 // (64 a clock and SM), so it is taken where it is needed only:
 //   greedy            none
-//   top-k             the k-th largest of the threads' own maxima is a lower bound of the k-th largest logit (one histogram of their distances from the
-//                     largest); threads whose maximum reaches it give their candidates to the first CTA, which ranks them and does the rest
+//   top-k             every CTA takes its share of k among its threads' own maxima (a histogram of their distances from its largest); the lowest such
+//                     threshold has at least k logits above it. Threads whose maximum reaches it give theirs to the first CTA, which ranks them and does the rest
 //   top-p alone       a histogram of all distances (counts) brackets the bin in which top_p is reached (a bin is 0.0156 wide, its weights are known to 0.8 %);
 //                     one pass of weights gives the sums around the bracket and a second histogram inside it, and the elements of its one bin are sorted
 //   draw              one pass of the weights that stayed; the warp on whose stretch the number falls walks it again
@@ -81,11 +81,11 @@ struct SampleShared {
     uint64_t list[SA_LIST];                  // the first CTA's: candidates
     uint64_t scan[SA_WARPS];
     uint64_t share[2][SA_MAX_CLUSTER];       // what every CTA of the cluster tells all others
-    uint64_t share2[SA_MAX_CLUSTER];
+    uint64_t share2[SA_MAX_CLUSTER], told[SA_MAX_CLUSTER];
     uint64_t arrived[SA_PIECES];             // barriers of the slice's pieces
     uint64_t cut, total;
     double   table[32];                      // 2^(i / 32)
-    uint32_t n_list;
+    uint32_t n_list, n_own;
     int      found, found2;
 };
 
@@ -206,7 +206,7 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(const __grid_cons
     if (tid == 0) {
         for (int i = 0; i < SA_PIECES; ++i) { mbar_init(smem_u32(sh.arrived + i), 1); }
         mbar_init_fence();
-        sh.n_list = 0; sh.cut = 0; sh.found = sh.found2 = 0;
+        sh.n_list = sh.n_own = 0; sh.cut = 0; sh.found = sh.found2 = 0;
     }
     *reinterpret_cast<uint4 *>(sh.count + 4 * tid) = make_uint4(0, 0, 0, 0);
     asm volatile("barrier.cluster.arrive.release;" ::: "memory");   // (waited for in front of the first access to another CTA's memory)
@@ -237,8 +237,11 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(const __grid_cons
     const int   top_k = p.top_k ? p.top_k[row] : 0;
 
     // this thread's largest (of the elements that Slice::each gives it), the row's, and where that is
-    float own = -CUDART_INF_F;
+    float own = -CUDART_INF_F, from_here = CUDART_INF_F;      // (top-k: nothing below from_here is among the k largest)
     uint64_t best = 0;
+    const bool greedy = !(temp > 0.f), by_k = !greedy && top_k > 0 && top_k < p.n_vocab, by_p = top_p < 1.f;
+    const bool quick = by_k && top_k <= 32 * (int)ctas;        // by the threads' maxima first
+    const uint64_t need = ctas > 1 ? (top_k + ctas - 2) / (ctas - 1) : top_k;
     {
         int at = -1;                                       // the first of the four that own is in
         auto take4 = [&](float4 v, int i) {
@@ -298,12 +301,28 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(const __grid_cons
         __syncthreads();
 #pragma unroll
         for (int w = 0; w < SA_WARPS; ++w) { best = max(best, sh.scan[w]); }
+        // this CTA's threshold: its largest minus so many 64ths that `need` of its threads' maxima lie above
+        float threshold = -CUDART_INF_F;
+        if (quick) {
+            const float top = best == 0 ? -CUDART_INF_F : value_of(best), b = (top - own) * 64.f;
+            if (b < (float)SA_BINS) { atomicAdd(&sh.count[(int)b], 1u); }
+            __syncthreads();
+            const uint4 n4 = *reinterpret_cast<const uint4 *>(sh.count + 4 * tid);
+            uint64_t all;
+            const uint64_t upto = block_upto((uint64_t)n4.x + n4.y + n4.z + n4.w, sh.scan, &all), before = upto - n4.x - n4.y - n4.z - n4.w;
+            if (before < need && need <= upto) { sh.found = 4 * tid + 3; }
+            __syncthreads();
+            // (a slice's end may lack them: it is left out, and the others' shares suffice)
+            threshold = all >= need ? top - (float)(sh.found + 2) * (1.f / 64) : ctas > 1 && rank == ctas - 1 ? CUDART_INF_F : -CUDART_INF_F;
+        }
         asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
-        if (tid < (int)ctas) { cluster_store64(cluster_map(smem_u32(sh.share[0] + rank), tid), best); }
+        if (tid < (int)ctas) {
+            cluster_store64(cluster_map(smem_u32(sh.share[0] + rank), tid), best);
+            cluster_store64(cluster_map(smem_u32(sh.share2 + rank), tid), __float_as_uint(threshold));
+        }
         cluster_sync();
-        for (uint32_t i = 0; i < ctas; ++i) { best = max(best, sh.share[0][i]); }
+        for (uint32_t i = 0; i < ctas; ++i) { best = max(best, sh.share[0][i]); from_here = fminf(from_here, __uint_as_float((uint32_t)sh.share2[i])); }
     }
-    const bool greedy = !(temp > 0.f);
     if (best == 0 || greedy) {
         if (rank == 0 && tid == 0) {
             p.ids[row] = best == 0 ? -1 : index_of(best);
@@ -315,6 +334,7 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(const __grid_cons
     if (largest == CUDART_INF_F) {
         x.inf = true; largest = 0.f;
         own = own == CUDART_INF_F ? 0.f : -CUDART_INF_F;
+        from_here = 0.f;
         if (KEPT) {
             for (int i = tid; i < ((x.n + 3) & ~3); i += SA_THREADS) { slice[i] = slice[i] == CUDART_INF_F ? 0.f : -CUDART_INF_F; }
             __syncthreads();
@@ -323,25 +343,29 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(const __grid_cons
     Weight weight;
     weight.table = sh.table; weight.bits = p.frac_bits; weight.largest = largest;
     weight.c = fmax(fmin(1.4426950408889634073599 / (double)temp, 1e30), 1e-30);
-    const double lowest = (double)largest - 60 / weight.c;                                  // weight 2^-60, and with it all below, rounds to 0
+    const double lowest = (double)largest - 60 * fmin(fmax(0.69314718055994530942 * (double)temp, 1e-30), 1e30);   // weight 2^-60, and with it all below, rounds to 0
     weight.edge = lowest < -3.4e38 || fabs((double)largest) * weight.c > 8e6; weight.least = weight.edge ? 0.f : (float)lowest;   // (f32 spacing: 2^-23 of the largest)
-    const double one = exp2((double)p.frac_bits);
+    const double one = __hiloint2double((1023 + p.frac_bits) << 20, 0);
     const uint64_t least = min_p > 0.f ? (uint64_t)max(1.0, ceil((double)fminf(min_p, 1.f) * one)) : 1;
     const float  bin_scale = (float)(weight.c * (SA_BINS / (double)(p.frac_bits + 1)));
     auto bin_of = [&](float v) { return (largest - v) * bin_scale; };        // not below SA_BINS (or NaN): no weight
-    const bool by_k = top_k > 0 && top_k < p.n_vocab, by_p = top_p < 1.f;
     auto reach = [&](uint64_t total) { return max((uint64_t)1, (uint64_t)ceil((double)max(top_p, 0.f) * (double)total)); };   // a token stays while less than this is in front of it
     uint64_t cut = 0;                        // keys from here on stay
     bool     search = false;                 // ... by the slow way
 
+    // every CTA's four bins of a thread (all loads in flight together)
+    auto row_sum = [&](const uint32_t *bins, auto add) {
+        uint4 v[SA_MAX_CLUSTER];
+#pragma unroll
+        for (uint32_t r = 0; r < SA_MAX_CLUSTER; ++r) { if (r < ctas) { v[r] = cluster_load128(cluster_map(smem_u32(bins) + tid * 16, r)); } }
+#pragma unroll
+        for (uint32_t r = 0; r < SA_MAX_CLUSTER; ++r) { if (r < ctas) { add(v[r]); } }
+    };
     // the whole row's counts, four bins a thread
     auto counts = [&]() {
         cluster_sync();
         uint4 n4 = make_uint4(0, 0, 0, 0);
-        for (uint32_t r = 0; r < ctas; ++r) {
-            const uint4 v = cluster_load128(cluster_map(smem_u32(sh.count) + tid * 16, r));
-            n4.x += v.x; n4.y += v.y; n4.z += v.z; n4.w += v.w;
-        }
+        row_sum(sh.count, [&](uint4 v) { n4.x += v.x; n4.y += v.y; n4.z += v.z; n4.w += v.w; });
         return n4;
     };
     auto count_all = [&]() {
@@ -350,18 +374,53 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(const __grid_cons
             if (b < (float)SA_BINS) { atomicAdd(&sh.count[(int)b], 1u); }
         });
     };
-    // elements that `wanted` names, of the threads whose largest is wanted, to the first CTA; how many there are (more than SA_LIST: they do not fit)
+    // Elements that `wanted` names, of the threads whose largest is wanted, to the first CTA: how many there are (more than SA_LIST: they do not fit), and where. Every
+    // CTA has its part of the list, so that nobody waits for a place in it; the first one closes the gaps
+    uint64_t *const compact = reinterpret_cast<uint64_t *>(sh.limb), *const weights = compact + SA_LIST;
+    uint64_t *candidates = sh.list;
     auto gather = [&](bool mine, auto wanted) {
-        const uint32_t counter = cluster_map(smem_u32(&sh.n_list), 0), list = cluster_map(smem_u32(sh.list), 0);
+        const uint32_t part = SA_LIST / ctas, list = cluster_map(smem_u32(sh.list), 0) + rank * part * 8;
         if (mine) {
             x.each([&](float v, int i) {
                 if (!wanted(v)) { return; }
-                const uint32_t at = cluster_add(counter, 1);
-                if (at < SA_LIST) { cluster_store64(list + at * 8, key_of(v, x.base + i)); }
+                const uint32_t at = atomicAdd(&sh.n_own, 1u);
+                if (at < part) { cluster_store64(list + at * 8, key_of(v, x.base + i)); }
             });
         }
+        __syncthreads();
+        if (tid < (int)ctas) { cluster_store64(cluster_map(smem_u32(sh.told + rank), tid), sh.n_own); }
         cluster_sync();
-        return cluster_load32(counter);
+        uint32_t n = 0;
+        bool fits = true;
+        for (uint32_t r = 0; r < ctas; ++r) { const uint32_t c = (uint32_t)sh.told[r]; fits &= c <= part; n += c; }
+        if (!fits) { return (uint32_t)SA_LIST + 1; }
+        if (rank == 0 && ctas > 1) {
+            for (uint32_t e = tid; e < SA_LIST; e += SA_THREADS) {
+                const uint32_t r = e / part, o = e - r * part;
+                if (o < (uint32_t)sh.told[r]) {
+                    uint32_t before = 0;
+                    for (uint32_t k = 0; k < r; ++k) { before += (uint32_t)sh.told[k]; }
+                    compact[before + o] = sh.list[e];
+                }
+            }
+            candidates = compact;
+            __syncthreads();
+        }
+        return n;
+    };
+    // the same where places are given out one by one: candidates may all lie in one slice
+    auto gather_one_by_one = [&](auto wanted) {
+        const uint32_t counter = cluster_map(smem_u32(&sh.n_list), 0), list = cluster_map(smem_u32(sh.list), 0);
+        x.each([&](float v, int i) {
+            if (!wanted(v)) { return; }
+            const uint32_t at = cluster_add(counter, 1);
+            if (at < SA_LIST) { cluster_store64(list + at * 8, key_of(v, x.base + i)); }
+        });
+        cluster_sync();
+        const uint32_t n = cluster_load32(counter);
+        candidates = sh.list;
+        cluster_sync();                                   // (all have read how many there are)
+        return n;
     };
     // the sum over all keys from `from` on
     auto sum_from = [&](uint64_t from, bool counting, int turn) {
@@ -373,20 +432,12 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(const __grid_cons
     };
 
     if (by_k) {
-        const bool quick = top_k <= (int)(SA_THREADS * ctas) / 8;            // by the threads' maxima first
-        for (int all_of_them = quick ? 0 : 1; all_of_them < 2; ++all_of_them) {
-            if (all_of_them) {
-                if (quick) {
-                    cluster_sync();                                           // (nobody reads the first counts any more)
-                    *reinterpret_cast<uint4 *>(sh.count + 4 * tid) = make_uint4(0, 0, 0, 0);
-                    if (tid == 0) { sh.n_list = 0; }
-                    __syncthreads();
-                }
-                count_all();
-            } else {
-                const float b = bin_of(own);
-                if (b < (float)SA_BINS) { atomicAdd(&sh.count[(int)b], 1u); }
-            }
+        uint32_t n = SA_LIST + 1;
+        if (quick) { n = gather(own >= from_here, [&](float v) { return v >= from_here; }); }
+        if (n > SA_LIST) {                                // from a histogram of all the row
+            if (quick) { *reinterpret_cast<uint4 *>(sh.count + 4 * tid) = make_uint4(0, 0, 0, 0); }
+            __syncthreads();
+            count_all();
             const uint4 n4 = counts();
             uint64_t all;
             const uint64_t upto = block_upto((uint64_t)n4.x + n4.y + n4.z + n4.w, sh.scan, &all);
@@ -399,13 +450,10 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(const __grid_cons
                 sh.found = b; sh.found2 = (int)min(c, (uint64_t)SA_LIST + 1);
             }
             __syncthreads();
-            const float last_bin = (float)(sh.found + 1);
-            uint32_t n = SA_LIST + 1;
-            if (all_of_them ? sh.found2 <= SA_LIST : all >= (uint64_t)top_k) {
-                n = gather(bin_of(own) < last_bin, [&](float v) { return bin_of(v) < last_bin; });
-            }
-            if (n > SA_LIST) { continue; }
-            cluster_sync();                                                   // (all have read how many there are)
+            const float behind = (float)(sh.found + 1);
+            if (sh.found2 <= SA_LIST) { n = gather_one_by_one([&](float v) { return bin_of(v) < behind; }); }
+        }
+        if (n <= SA_LIST) {
             if (rank != 0) { return; }
             // everything else is the first CTA's
             const int n_list = (int)n;
@@ -415,8 +463,7 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(const __grid_cons
                 while (per < 32 && n_list * per * 2 <= SA_THREADS) { per *= 2; }
                 const int i = tid / per, part = tid & (per - 1);
                 const bool is = i < n_list;
-                const uint64_t key = is ? sh.list[i] : 0;
-                uint64_t *weights = reinterpret_cast<uint64_t *>(sh.limb);
+                const uint64_t key = is ? candidates[i] : 0;
                 uint64_t w = 0;
                 if (is) { w = weight(value_of(key)); if (part == 0) { weights[i] = w; } }
                 __syncthreads();
@@ -426,7 +473,7 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(const __grid_cons
                 };
                 uint64_t in_front = 0, before_w = 0;
                 if (is) {
-                    for (int j = part; j < n_list; j += per) { if (sh.list[j] > key) { ++in_front; before_w += weights[j]; } }
+                    for (int j = part; j < n_list; j += per) { if (candidates[j] > key) { ++in_front; before_w += weights[j]; } }
                 }
                 in_front = group_sum(in_front); before_w = group_sum(before_w);
                 bool stays = is && in_front < (uint64_t)top_k;
@@ -438,7 +485,7 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(const __grid_cons
                 uint64_t upto_w = 0;
                 constexpr uint64_t low = (1 << SA_INDEX_BITS) - 1;
                 if (stays) {
-                    for (int j = part; j < n_list; j += per) { if ((sh.list[j] & low) > (key & low)) { upto_w += weights[j]; } }
+                    for (int j = part; j < n_list; j += per) { if ((candidates[j] & low) > (key & low)) { upto_w += weights[j]; } }
                 }
                 upto_w = group_sum(upto_w);
                 if (stays && part == 0 && upto_w <= t && t < upto_w + w) {
@@ -448,18 +495,18 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(const __grid_cons
                 return;
             }
             // sorted, cut from the end, put back into the order of indices, drawn
-            sort_list(sh.list, n_list);
+            sort_list(candidates, n_list);
             const int n1 = min(n_list, top_k);
             uint64_t w0 = 0, w1 = 0, k0 = 0, k1 = 0, all_w;
-            if (2 * tid < n1) { k0 = sh.list[2 * tid]; w0 = weight(value_of(k0)); }
-            if (2 * tid + 1 < n1) { k1 = sh.list[2 * tid + 1]; w1 = weight(value_of(k1)); }
+            if (2 * tid < n1) { k0 = candidates[2 * tid]; w0 = weight(value_of(k0)); }
+            if (2 * tid + 1 < n1) { k1 = candidates[2 * tid + 1]; w1 = weight(value_of(k1)); }
             const uint64_t up = block_upto(w0 + w1, sh.scan, &all_w);
             const uint64_t stop = by_p ? reach(all_w) : ~0ull;
             const bool in0 = 2 * tid < n1 && up - w1 - w0 < stop && w0 >= least, in1 = 2 * tid + 1 < n1 && up - w1 < stop && w1 >= least;
             const uint64_t kept = block_sum((in0 ? 1 : 0) + (in1 ? 1 : 0), sh.scan);          // (a prefix of the list)
             const uint64_t sum = block_sum((in0 ? w0 : 0) + (in1 ? w1 : 0), sh.scan);
             // by index: the key's low bits, ascending as descending complements; the weights are found again from their place in the sorted list
-            uint64_t *by_index = sh.list, *weights = reinterpret_cast<uint64_t *>(sh.limb);
+            uint64_t *by_index = candidates;
             __syncthreads();
             constexpr uint64_t low = (1 << SA_INDEX_BITS) - 1;
             if (in0) { by_index[2 * tid] = ((k0 & low) << 11 | (2 * tid)) + 1; weights[2 * tid] = w0; }
@@ -526,12 +573,7 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(const __grid_cons
         front = total = 0;
         for (uint32_t r = 0; r < ctas; ++r) { front += sh.share[1][r]; total += sh.share2[r]; }
         uint64_t q[4] = {0, 0, 0, 0};
-        for (uint32_t r = 0; r < ctas; ++r) {
-            const uint4 a = cluster_load128(cluster_map(smem_u32(sh.limb[0]) + tid * 16, r)), b = cluster_load128(cluster_map(smem_u32(sh.limb[1]) + tid * 16, r)),
-                        d = cluster_load128(cluster_map(smem_u32(sh.limb[2]) + tid * 16, r));
-            q[0] += a.x + ((uint64_t)b.x << 15) + ((uint64_t)d.x << 30); q[1] += a.y + ((uint64_t)b.y << 15) + ((uint64_t)d.y << 30);
-            q[2] += a.z + ((uint64_t)b.z << 15) + ((uint64_t)d.z << 30); q[3] += a.w + ((uint64_t)b.w << 15) + ((uint64_t)d.w << 30);
-        }
+        for (int i = 0; i < 3; ++i) { row_sum(sh.limb[i], [&](uint4 v) { q[0] += (uint64_t)v.x << 15 * i; q[1] += (uint64_t)v.y << 15 * i; q[2] += (uint64_t)v.z << 15 * i; q[3] += (uint64_t)v.w << 15 * i; }); }
         const uint64_t stop = reach(total);
         const uint64_t upto_s = block_upto(q[0] + q[1] + q[2] + q[3], sh.scan, &all);
         if (tid == 0) { sh.found = -1; }
@@ -549,16 +591,16 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(const __grid_cons
             const uint32_t n_in_bin = gather(bin_of(own) < behind, [&](float v) { const float b = bin_of(v); return b >= first && b < behind && sub_of(b) == sub; });
             // the first CTA finds the last one that stays and tells all
             if (rank == 0) {
-                const int nn = (int)min(n_in_bin, (uint32_t)SA_LIST + 1);
+                const int nn = (int)n_in_bin;
                 uint64_t found = 0;
                 if (nn <= SA_LIST) {
-                    sort_list(sh.list, nn);
+                    sort_list(candidates, nn);
                     uint64_t w0 = 0, w1 = 0, ignore;
-                    if (2 * tid < nn) { w0 = weight(value_of(sh.list[2 * tid])); }
-                    if (2 * tid + 1 < nn) { w1 = weight(value_of(sh.list[2 * tid + 1])); }
+                    if (2 * tid < nn) { w0 = weight(value_of(candidates[2 * tid])); }
+                    if (2 * tid + 1 < nn) { w1 = weight(value_of(candidates[2 * tid + 1])); }
                     const uint64_t up = sh.total + block_upto(w0 + w1, sh.scan, &ignore);
                     const uint64_t n_in = block_sum((2 * tid < nn && up - w1 - w0 < stop ? 1 : 0) + (2 * tid + 1 < nn && up - w1 < stop ? 1 : 0), sh.scan);
-                    found = n_in > 0 ? sh.list[n_in - 1] : 0;
+                    found = n_in > 0 ? candidates[n_in - 1] : 0;
                 }
                 if (tid < (int)ctas) { cluster_store64(cluster_map(smem_u32(&sh.cut), tid), found); }
             }
