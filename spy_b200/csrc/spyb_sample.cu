@@ -18,11 +18,11 @@ namespace {
 //   greedy            none
 //   top-k             every CTA takes its share of k among its threads' own maxima (a histogram of their distances from its largest); the lowest such
 //                     threshold has at least k logits above it. Threads whose maximum reaches it give theirs to the first CTA, which ranks them and does the rest
-//   top-p alone       a histogram of all distances (counts) brackets the bin in which top_p is reached (a bin is 0.0156 wide, its weights are known to 0.8 %);
+//   top-p alone       a histogram of all distances (counts) brackets the bin in which top_p is reached (a bin is 0.031 wide, its weights are known to 1.6 %);
 //                     one pass of weights gives the sums around the bracket and a second histogram inside it, and the elements of its one bin are sorted
 //   draw              one pass of the weights that stayed; the warp on whose stretch the number falls walks it again
 // Candidates that do not fit a list (ties by the thousand, a top_k of thousands) take a binary search over (logit, index): slow, and as right.
-constexpr int SA_THREADS = 512, SA_WARPS = SA_THREADS / 32, SA_BINS = 2048, SA_LIST = 1024, SA_RANKED = 256, SA_MAX_CLUSTER = 8, SA_PIECES = 4;
+constexpr int SA_THREADS = 512, SA_WARPS = SA_THREADS / 32, SA_BINS = 1024, SA_SUB = SA_THREADS, SA_LIST = 1024, SA_RANKED = 256, SA_MAX_CLUSTER = 8, SA_PIECES = 4;
 constexpr int SA_INDEX_BITS = 20;
 constexpr size_t SA_MAX_SLICE = 40960;    // logits that a CTA keeps in shared memory; longer slices are read again in every pass
 
@@ -48,9 +48,9 @@ __device__ __forceinline__ float as_float(__half x) { return __half2float(x); }
 
 __device__ __forceinline__ uint32_t rank_in_cluster() { uint32_t r; asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r)); return r; }
 __device__ __forceinline__ uint32_t cluster_ctas() { uint32_t r; asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r)); return r; }
-__device__ __forceinline__ uint4 cluster_load128(uint32_t addr) {
-    uint4 v;
-    asm volatile("ld.shared::cluster.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+__device__ __forceinline__ uint64_t cluster_load64(uint32_t addr) {
+    uint64_t v;
+    asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(addr) : "memory");
     return v;
 }
 __device__ __forceinline__ uint32_t cluster_load32(uint32_t addr) {
@@ -77,7 +77,8 @@ __device__ __forceinline__ uint64_t warp_upto64(uint64_t v) {   // inclusive sum
 
 struct SampleShared {
     uint32_t count[SA_BINS];
-    uint32_t limb[3][SA_BINS];               // sums of weights in pieces of 15, 15 and the rest of their bits (up to 2^17 weights a CTA)
+    uint32_t limb[3][SA_SUB];                // sums of weights in pieces of 15, 15 and the rest of their bits (up to 2^17 weights a CTA)
+    uint64_t compact[SA_LIST], weights[SA_LIST];
     uint64_t list[SA_LIST];                  // the first CTA's: candidates
     uint64_t scan[SA_WARPS];
     uint64_t share[2][SA_MAX_CLUSTER];       // what every CTA of the cluster tells all others
@@ -96,21 +97,39 @@ struct Weight {
     float  least;               // no logit below it has weight: it stands for them, and for -inf
     bool   edge;                // ... if f32 has such a number near enough; else the exponent itself is bounded
     int    bits;
-    __device__ __forceinline__ uint64_t operator()(float x) const {
-        const double z = edge ? fmax(((double)x - largest) * c, -60.0) : ((double)fmaxf(x, least) - largest) * c;   // (NaN reads as no weight)
+    // N at a time: their steps side by side, for an operation in 64 bits has a long way
+    template <int N> __device__ __forceinline__ void of(const float (&x)[N], uint64_t (&w)[N]) const {
         const double magic = 6755399441055744.0;                                         // 1.5 x 2^52: the sum's low bits are the rounded integer
-        const double t = fma(z, 32.0, magic);
-        const int    k = __double2loint(t);
-        const double f = fma(t - magic, -1.0 / 32, z);                                   // |f| <= 1/64: the series of 2^f to the fifth term leaves 2e-15
-        double e = 1.3333558146428443e-3;
-        e = fma(e, f, 9.618129107628477e-3);
-        e = fma(e, f, 5.550410866482158e-2);
-        e = fma(e, f, 2.402265069591007e-1);
-        e = fma(e, f, 6.931471805599453e-1);
-        e = fma(e, f, 1.0);
-        e *= table[k & 31];
-        e = __hiloint2double(__double2hiint(e) + (((k >> 5) + bits) << 20), __double2loint(e));
-        return (uint64_t)(__double_as_longlong(e + 4503599627370496.0) & 0xfffffffffffffll);   // + 2^52: rounded to an integer (w < 2^51)
+        double z[N], t[N], f[N], e[N];
+#pragma unroll
+        for (int i = 0; i < N; ++i) { z[i] = edge ? fmax(((double)x[i] - largest) * c, -60.0) : ((double)fmaxf(x[i], least) - largest) * c; }   // (NaN reads as no weight)
+#pragma unroll
+        for (int i = 0; i < N; ++i) { t[i] = fma(z[i], 32.0, magic); }
+#pragma unroll
+        for (int i = 0; i < N; ++i) { f[i] = fma(t[i] - magic, -1.0 / 32, z[i]); }       // |f| <= 1/64: the series of 2^f to the fifth term leaves 2e-15
+#pragma unroll
+        for (int i = 0; i < N; ++i) { e[i] = fma(1.3333558146428443e-3, f[i], 9.618129107628477e-3); }
+#pragma unroll
+        for (int i = 0; i < N; ++i) { e[i] = fma(e[i], f[i], 5.550410866482158e-2); }
+#pragma unroll
+        for (int i = 0; i < N; ++i) { e[i] = fma(e[i], f[i], 2.402265069591007e-1); }
+#pragma unroll
+        for (int i = 0; i < N; ++i) { e[i] = fma(e[i], f[i], 6.931471805599453e-1); }
+#pragma unroll
+        for (int i = 0; i < N; ++i) { e[i] = fma(e[i], f[i], 1.0); }
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int k = __double2loint(t[i]);
+            e[i] *= table[k & 31];
+            e[i] = __hiloint2double(__double2hiint(e[i]) + (((k >> 5) + bits) << 20), __double2loint(e[i]));
+            w[i] = (uint64_t)(__double_as_longlong(e[i] + 4503599627370496.0) & 0xfffffffffffffll);   // + 2^52: rounded to an integer (w < 2^51)
+        }
+    }
+    __device__ __forceinline__ uint64_t operator()(float x) const {
+        const float one[1] = {x};
+        uint64_t w[1];
+        of(one, w);
+        return w[0];
     }
 };
 
@@ -126,18 +145,26 @@ template <class T, bool KEPT> struct Slice {
         x = x == x ? x : -CUDART_INF_F;
         return inf ? (x == CUDART_INF_F ? 0.f : -CUDART_INF_F) : x;
     }
-    // f(logit, place) for this thread's share, four at a time where they are kept (the slice is padded with -inf to whole fours)
-    template <class F> __device__ __forceinline__ void each(const F &f) const { stretch(0, n, threadIdx.x, SA_THREADS, f); }
+    // f(four logits, place of the first) for this thread's share; -inf behind the slice's end
+    template <class F> __device__ __forceinline__ void fours(const F &f) const { stretch(0, n, threadIdx.x, SA_THREADS, f); }
     template <class F> __device__ __forceinline__ void stretch(int from, int to, int first, int step, const F &f) const {   // from: a multiple of 4
-        if (KEPT) {
-#pragma unroll 2
-            for (int i = from + 4 * first; i < to; i += 4 * step) {
-                const float4 v = *reinterpret_cast<const float4 *>(kept + i);
-                f(v.x, i); f(v.y, i + 1); f(v.z, i + 2); f(v.w, i + 3);
+        for (int i = from + 4 * first; i < to; i += 4 * step) {
+            float v[4];
+            if (KEPT) {
+                const float4 u = *reinterpret_cast<const float4 *>(kept + i);
+                v[0] = u.x; v[1] = u.y; v[2] = u.z; v[3] = u.w;
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) { v[e] = i + e < n ? (*this)(i + e) : -CUDART_INF_F; }
             }
-        } else {
-            for (int i = from + first; i < to; i += step) { f((*this)(i), i); }
+            f(v, i);
         }
+    }
+    template <class F> __device__ __forceinline__ void each(const F &f) const {   // f(logit, place)
+        fours([&](const float (&v)[4], int i) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) { f(v[e], i + e); }
+        });
     }
 };
 
@@ -208,7 +235,7 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(const __grid_cons
         mbar_init_fence();
         sh.n_list = sh.n_own = 0; sh.cut = 0; sh.found = sh.found2 = 0;
     }
-    *reinterpret_cast<uint4 *>(sh.count + 4 * tid) = make_uint4(0, 0, 0, 0);
+    *reinterpret_cast<uint2 *>(sh.count + 2 * tid) = make_uint2(0, 0);
     asm volatile("barrier.cluster.arrive.release;" ::: "memory");   // (waited for in front of the first access to another CTA's memory)
     pdl_wait();
 
@@ -285,14 +312,10 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(const __grid_cons
                 take4(make_float4(v[0], v[1], v[2], v[3]), i);
             }
         } else {
-#pragma unroll 4
-            for (int i = tid; i < x.n; i += SA_THREADS) {
-                const float v = x(i);
-                if (v > own) { own = v; at = i; }
-            }
+            x.fours([&](const float (&v)[4], int i) { take4(make_float4(v[0], v[1], v[2], v[3]), i); });
         }
         if (at >= 0) {
-            if (KEPT) { at = slice[at] == own ? at : slice[at + 1] == own ? at + 1 : slice[at + 2] == own ? at + 2 : at + 3; }
+            at = x(at) == own ? at : x(at + 1) == own ? at + 1 : x(at + 2) == own ? at + 2 : at + 3;
             best = key_of(own, x.base + at);
         }
 #pragma unroll
@@ -301,19 +324,19 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(const __grid_cons
         __syncthreads();
 #pragma unroll
         for (int w = 0; w < SA_WARPS; ++w) { best = max(best, sh.scan[w]); }
-        // this CTA's threshold: its largest minus so many 64ths that `need` of its threads' maxima lie above
+        // this CTA's threshold: its largest minus so many 32nds that `need` of its threads' maxima lie above
         float threshold = -CUDART_INF_F;
         if (quick) {
-            const float top = best == 0 ? -CUDART_INF_F : value_of(best), b = (top - own) * 64.f;
+            const float top = best == 0 ? -CUDART_INF_F : value_of(best), b = (top - own) * 32.f;
             if (b < (float)SA_BINS) { atomicAdd(&sh.count[(int)b], 1u); }
             __syncthreads();
-            const uint4 n4 = *reinterpret_cast<const uint4 *>(sh.count + 4 * tid);
+            const uint2 n2 = *reinterpret_cast<const uint2 *>(sh.count + 2 * tid);
             uint64_t all;
-            const uint64_t upto = block_upto((uint64_t)n4.x + n4.y + n4.z + n4.w, sh.scan, &all), before = upto - n4.x - n4.y - n4.z - n4.w;
-            if (before < need && need <= upto) { sh.found = 4 * tid + 3; }
+            const uint64_t upto = block_upto((uint64_t)n2.x + n2.y, sh.scan, &all), before = upto - n2.x - n2.y;
+            if (before < need && need <= upto) { sh.found = 2 * tid + 1; }
             __syncthreads();
             // (a slice's end may lack them: it is left out, and the others' shares suffice)
-            threshold = all >= need ? top - (float)(sh.found + 2) * (1.f / 64) : ctas > 1 && rank == ctas - 1 ? CUDART_INF_F : -CUDART_INF_F;
+            threshold = all >= need ? top - (float)(sh.found + 2) * (1.f / 32) : ctas > 1 && rank == ctas - 1 ? CUDART_INF_F : -CUDART_INF_F;
         }
         asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
         if (tid < (int)ctas) {
@@ -353,20 +376,16 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(const __grid_cons
     uint64_t cut = 0;                        // keys from here on stay
     bool     search = false;                 // ... by the slow way
 
-    // every CTA's four bins of a thread (all loads in flight together)
-    auto row_sum = [&](const uint32_t *bins, auto add) {
-        uint4 v[SA_MAX_CLUSTER];
-#pragma unroll
-        for (uint32_t r = 0; r < SA_MAX_CLUSTER; ++r) { if (r < ctas) { v[r] = cluster_load128(cluster_map(smem_u32(bins) + tid * 16, r)); } }
-#pragma unroll
-        for (uint32_t r = 0; r < SA_MAX_CLUSTER; ++r) { if (r < ctas) { add(v[r]); } }
-    };
-    // the whole row's counts, four bins a thread
+    // the whole row's counts, two bins a thread (all CTAs' in flight together)
     auto counts = [&]() {
         cluster_sync();
-        uint4 n4 = make_uint4(0, 0, 0, 0);
-        row_sum(sh.count, [&](uint4 v) { n4.x += v.x; n4.y += v.y; n4.z += v.z; n4.w += v.w; });
-        return n4;
+        uint64_t v[SA_MAX_CLUSTER];
+        uint2 n2 = make_uint2(0, 0);
+#pragma unroll
+        for (uint32_t r = 0; r < SA_MAX_CLUSTER; ++r) { v[r] = r < ctas ? cluster_load64(cluster_map(smem_u32(sh.count) + tid * 8, r)) : 0; }
+#pragma unroll
+        for (uint32_t r = 0; r < SA_MAX_CLUSTER; ++r) { n2.x += (uint32_t)v[r]; n2.y += (uint32_t)(v[r] >> 32); }
+        return n2;
     };
     auto count_all = [&]() {
         x.each([&](float v, int) {
@@ -376,7 +395,7 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(const __grid_cons
     };
     // Elements that `wanted` names, of the threads whose largest is wanted, to the first CTA: how many there are (more than SA_LIST: they do not fit), and where. Every
     // CTA has its part of the list, so that nobody waits for a place in it; the first one closes the gaps
-    uint64_t *const compact = reinterpret_cast<uint64_t *>(sh.limb), *const weights = compact + SA_LIST;
+    uint64_t *const compact = sh.compact, *const weights = sh.weights;
     uint64_t *candidates = sh.list;
     auto gather = [&](bool mine, auto wanted) {
         const uint32_t part = SA_LIST / ctas, list = cluster_map(smem_u32(sh.list), 0) + rank * part * 8;
@@ -435,18 +454,16 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(const __grid_cons
         uint32_t n = SA_LIST + 1;
         if (quick) { n = gather(own >= from_here, [&](float v) { return v >= from_here; }); }
         if (n > SA_LIST) {                                // from a histogram of all the row
-            if (quick) { *reinterpret_cast<uint4 *>(sh.count + 4 * tid) = make_uint4(0, 0, 0, 0); }
+            if (quick) { *reinterpret_cast<uint2 *>(sh.count + 2 * tid) = make_uint2(0, 0); }
             __syncthreads();
             count_all();
-            const uint4 n4 = counts();
+            const uint2 n2 = counts();
             uint64_t all;
-            const uint64_t upto = block_upto((uint64_t)n4.x + n4.y + n4.z + n4.w, sh.scan, &all);
-            const uint64_t before = upto - n4.x - n4.y - n4.z - n4.w, want = min((uint64_t)top_k, all);
+            const uint64_t upto = block_upto((uint64_t)n2.x + n2.y, sh.scan, &all);
+            const uint64_t before = upto - n2.x - n2.y, want = min((uint64_t)top_k, all);
             if (before < want && want <= upto) {
-                uint64_t c = before + n4.x; int b = tid * 4;
-                if (c < want) { c += n4.y; ++b; }
-                if (c < want) { c += n4.z; ++b; }
-                if (c < want) { c += n4.w; ++b; }
+                uint64_t c = before + n2.x; int b = tid * 2;
+                if (c < want) { c += n2.y; ++b; }
                 sh.found = b; sh.found2 = (int)min(c, (uint64_t)SA_LIST + 1);
             }
             __syncthreads();
@@ -526,44 +543,39 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(const __grid_cons
         }
         search = true;
     } else if (by_p) {
-#pragma unroll
-        for (int i = 0; i < 3; ++i) { *reinterpret_cast<uint4 *>(sh.limb[i] + 4 * tid) = make_uint4(0, 0, 0, 0); }
+        sh.limb[0][tid] = sh.limb[1][tid] = sh.limb[2][tid] = 0;
         count_all();
-        const uint4 n4 = counts();
-        // what the bins weigh, to 0.8 %: the bins in which top_p may be reached
+        const uint2 n2 = counts();
+        // what the bins weigh, to 1.6 %: the bins in which top_p may be reached
         const float step = -(float)(p.frac_bits + 1) / SA_BINS;     // log2 of a weight, a bin
-        const float w[4] = {exp2f(step * (4 * tid + 0.5f)), exp2f(step * (4 * tid + 1.5f)), exp2f(step * (4 * tid + 2.5f)), exp2f(step * (4 * tid + 3.5f))};
-        const uint32_t n[4] = {n4.x, n4.y, n4.z, n4.w};
-        uint64_t m[4], all;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) { m[e] = (uint64_t)((double)w[e] * n[e] * 1099511627776.0); }   // x 2^40
-        const uint64_t upto = block_upto(m[0] + m[1] + m[2] + m[3], sh.scan, &all);
+        uint64_t all;
+        const uint64_t m0 = (uint64_t)((double)exp2f(step * (2 * tid + 0.5f)) * n2.x * 1099511627776.0), m1 = (uint64_t)((double)exp2f(step * (2 * tid + 1.5f)) * n2.y * 1099511627776.0);   // x 2^40
+        const uint64_t upto = block_upto(m0 + m1, sh.scan, &all), before_b = upto - m0 - m1;
         const double   goal = (double)max(top_p, 0.f) * (double)all;
-        const uint64_t lo = (uint64_t)(0.98 * goal), hi = min((uint64_t)(1.02 * goal), all);
-        uint64_t c = upto - m[0] - m[1] - m[2] - m[3];
+        const uint64_t lo = (uint64_t)(0.965 * goal), hi = min((uint64_t)(1.035 * goal), all);
         if (tid == 0) { sh.found = 0; sh.found2 = SA_BINS - 1; }
         __syncthreads();
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            if (c < lo && lo <= c + m[e]) { sh.found = 4 * tid + e; }
-            if (c < hi && hi <= c + m[e]) { sh.found2 = min(4 * tid + e + 1, SA_BINS - 1); }
-            c += m[e];
-        }
+        if (before_b < lo && lo <= upto) { sh.found = lo <= before_b + m0 ? 2 * tid : 2 * tid + 1; }
+        if (before_b < hi && hi <= upto) { sh.found2 = min(hi <= before_b + m0 ? 2 * tid + 1 : 2 * tid + 2, SA_BINS - 1); }
         __syncthreads();
         const float first = (float)sh.found, behind = (float)(sh.found2 + 1);
-        const float sub_scale = (float)SA_BINS / (behind - first);
-        auto sub_of = [&](float b) { return min(SA_BINS - 1, (int)((b - first) * sub_scale)); };
+        const float sub_scale = (float)SA_SUB / (behind - first);
+        auto sub_of = [&](float b) { return min(SA_SUB - 1, (int)((b - first) * sub_scale)); };
         uint64_t front = 0, total = 0;
-        x.each([&](float v, int) {
-            const float b = bin_of(v);
-            const uint64_t ww = weight(v);
-            total += ww;
-            front += b < first ? ww : 0;
-            if (b >= first && b < behind) {
-                const int s = sub_of(b);
-                atomicAdd(&sh.limb[0][s], (uint32_t)(ww & 0x7fff));
-                atomicAdd(&sh.limb[1][s], (uint32_t)(ww >> 15) & 0x7fff);
-                if (ww >> 30) { atomicAdd(&sh.limb[2][s], (uint32_t)(ww >> 30)); }
+        x.fours([&](const float (&v)[4], int) {
+            uint64_t ww[4];
+            weight.of(v, ww);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float b = bin_of(v[e]);
+                total += ww[e];
+                front += b < first ? ww[e] : 0;
+                if (b >= first && b < behind) {
+                    const int s = sub_of(b);
+                    atomicAdd(&sh.limb[0][s], (uint32_t)(ww[e] & 0x7fff));
+                    atomicAdd(&sh.limb[1][s], (uint32_t)(ww[e] >> 15) & 0x7fff);
+                    if (ww[e] >> 30) { atomicAdd(&sh.limb[2][s], (uint32_t)(ww[e] >> 30)); }
+                }
             }
         });
         front = block_sum(front, sh.scan);
@@ -572,18 +584,20 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(const __grid_cons
         cluster_sync();
         front = total = 0;
         for (uint32_t r = 0; r < ctas; ++r) { front += sh.share[1][r]; total += sh.share2[r]; }
-        uint64_t q[4] = {0, 0, 0, 0};
-        for (int i = 0; i < 3; ++i) { row_sum(sh.limb[i], [&](uint4 v) { q[0] += (uint64_t)v.x << 15 * i; q[1] += (uint64_t)v.y << 15 * i; q[2] += (uint64_t)v.z << 15 * i; q[3] += (uint64_t)v.w << 15 * i; }); }
+        uint64_t mass = 0;                               // of this thread's bin of the bracket
+#pragma unroll
+        for (int i = 0; i < 3; ++i) {
+            uint32_t v[SA_MAX_CLUSTER];
+#pragma unroll
+            for (uint32_t r = 0; r < SA_MAX_CLUSTER; ++r) { v[r] = r < ctas ? cluster_load32(cluster_map(smem_u32(sh.limb[i]) + tid * 4, r)) : 0; }
+#pragma unroll
+            for (uint32_t r = 0; r < SA_MAX_CLUSTER; ++r) { mass += (uint64_t)v[r] << 15 * i; }
+        }
         const uint64_t stop = reach(total);
-        const uint64_t upto_s = block_upto(q[0] + q[1] + q[2] + q[3], sh.scan, &all);
+        const uint64_t upto_s = front + block_upto(mass, sh.scan, &all);
         if (tid == 0) { sh.found = -1; }
         __syncthreads();
-        c = front + upto_s - q[0] - q[1] - q[2] - q[3];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            if (c < stop && stop <= c + q[e]) { sh.found = 4 * tid + e; sh.total = c; }
-            c += q[e];
-        }
+        if (upto_s - mass < stop && stop <= upto_s) { sh.found = tid; sh.total = upto_s - mass; }
         __syncthreads();
         const int sub = sh.found;
         if (sub < 0) { search = true; }              // (not reached inside the bracket)
@@ -631,15 +645,17 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(const __grid_cons
     const int stretch = ((x.n + SA_WARPS - 1) / SA_WARPS + 127) & ~127, from = min(warp * stretch, x.n), to = min(from + stretch, x.n);
     const float cut_value = cut == 0 ? -CUDART_INF_F : value_of(cut);
     const int   cut_index = cut == 0 ? p.n_vocab : index_of(cut);
-    auto stays = [&](float v, int i) {
-        const uint64_t w = weight(v);
+    auto stays = [&](float v, int i, uint64_t w) {
         return (v > cut_value || (v == cut_value && x.base + i <= cut_index)) && w >= least ? w : (uint64_t)0;
     };
     uint64_t s = 0;
-    if (cut == 0 && least == 1) { x.stretch(from, to, lane, 32, [&](float v, int) { s += weight(v); }); }
-    else {
-        x.stretch(from, to, lane, 32, [&](float v, int i) { if (v >= cut_value) { s += stays(v, i); } });
-    }
+    x.stretch(from, to, lane, 32, [&](const float (&v)[4], int i) {
+        if (fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])) < cut_value) { return; }
+        uint64_t w[4];
+        weight.of(v, w);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) { s += stays(v[e], i + e, w[e]); }
+    });
     s = warp_sum64(s);
     __syncthreads();
     if (lane == 0) { sh.scan[warp] = s; }
@@ -655,7 +671,7 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(const __grid_cons
         uint64_t c = before;
         for (int i0 = from; i0 < to; i0 += 32) {
             const int i = i0 + lane;
-            const uint64_t w = i < to ? stays(x(i), i) : 0, upto = c + warp_upto64(w);
+            const uint64_t w = i < to ? stays(x(i), i, weight(x(i))) : 0, upto = c + warp_upto64(w);
             const unsigned hit = __ballot_sync(0xffffffffu, t < upto);
             if (hit) {
                 if (lane == __ffs(hit) - 1) {
