@@ -12,9 +12,9 @@ namespace spyb {
 namespace {
 
 // A cluster of CTAs has a row, each a slice of it in shared memory: the logits are read once, by bulk copies. Which token a number falls on must not depend on how
-// sums are rounded, so weights are integers: w = round(2^S exp((x - largest) / T)), S = 45 for up to 2^17 tokens. Their sums are exact in any order,
-// a histogram's too, and a weight's error of 2^-46 moves a border of the sums by about 2^-37 at most. An exponential to 2^-48 costs 13 operations in 64 bits
-// (64 a clock and SM), so it is taken where it is needed only:
+// sums are rounded, so weights are integers: w = 2^S exp((x - largest) / T), S = 45 for up to 2^17 tokens. Their sums are exact in any order,
+// a histogram's too, and errors of 2^-34 of each weight, as often up as down, move a border of N weights' sums by some 2^-34 / sqrt(N) of the whole. An exponential to so many bits costs some 35
+// instructions, so it is taken where it is needed only:
 //   greedy            none
 //   top-k             every CTA takes its share of k among its threads' own maxima (a histogram of their distances from its largest); the lowest such
 //                     threshold has at least k logits above it. Threads whose maximum reaches it give theirs to the first CTA, which ranks them and does the rest
@@ -85,44 +85,67 @@ struct SampleShared {
     uint64_t share2[SA_MAX_CLUSTER], told[SA_MAX_CLUSTER];
     uint64_t arrived[SA_PIECES];             // barriers of the slice's pieces
     uint64_t cut, total;
-    double   table[32];                      // 2^(i / 32)
+    uint64_t table[1024];                    // Weight's
     uint32_t n_list, n_own;
     int      found, found2;
 };
 
-// the weight of a logit as an integer; `c` = log2(e) / T
+// The weight of a logit as an integer, 2^S 2^-z with z = (largest - x) c, c = log2(e) / T, to 2^-34 of itself and a unit. (An operation in 64 bits takes eight clocks of a
+// quarter of an SM, one in f32 one: with them the pass took 7 us longer per 37 rows of 128 000.) z is taken apart as r / 1024 + f + e without an error that counts:
+//   p + p' = x c, by FMA; A = largest c in 64 bits, A = a + a' with a a multiple of 2^-14; r = round(1024 (a - p));
+//   f = (a - r / 1024) - p: the first difference is exact (multiples of 2^-14 below 2^10), the second too (|f| <= 2^-11); e = a' - p'.
+// 2^-(r / 1024) is a table's 2^46-fold and a shift, 2^-(f + e) = 1 + y with |y| < 2^-11.5, y to 2^-36 in f32.
+// Where |A| is too large for that (1000 and more: tiny temperatures, huge logits), the same in 64 bits.
 struct Weight {
-    const double *table;
-    double c, largest;
+    const uint64_t *table;      // 2^46 2^-(j / 1024)
+    float  c_hi, c_lo, a_hi, a_lo;
     float  least;               // no logit below it has weight: it stands for them, and for -inf
-    bool   edge;                // ... if f32 has such a number near enough; else the exponent itself is bounded
-    int    bits;
-    // N at a time: their steps side by side, for an operation in 64 bits has a long way
+    bool   wide;                // in 64 bits
+    double c, largest;
+    int    shift;               // 46 - S
+    __device__ __forceinline__ void set(const uint64_t *powers, float top, double scale, int bits) {
+        table = powers; c = scale; largest = top; shift = 46 - bits;
+        const double a = largest * c, lowest = largest - 56 / c;                         // (2^-56 is no unit: rounds to nothing)
+        wide = !(fabs(a) < 960.0 && lowest > -3.4e38);
+        least = wide ? 0.f : (float)lowest;
+        c_hi = (float)c; c_lo = (float)(c - c_hi);
+        a_hi = (float)(rint(a * 16384.0) * (1.0 / 16384)); a_lo = (float)(a - a_hi);
+    }
+    static __device__ __noinline__ uint64_t in_64_bits(const uint64_t *table, double z, int shift) {
+        z = fmin(z, 56.0);                                                               // (NaN reads as no weight)
+        const double r = rint(z * 1024.0), f = (r * (1.0 / 1024) - z) * 0.69314718055994530942;
+        const int    k = (int)r;
+        const double t = (double)table[k & 1023] * (1.0 + f * (1.0 + f * (0.5 + f * (1.0 / 6))));
+        return (uint64_t)(t + 0.5) >> ((k >> 10) + shift);
+    }
     template <int N> __device__ __forceinline__ void of(const float (&x)[N], uint64_t (&w)[N]) const {
-        const double magic = 6755399441055744.0;                                         // 1.5 x 2^52: the sum's low bits are the rounded integer
-        double z[N], t[N], f[N], e[N];
+        if (wide) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) { z[i] = edge ? fmax(((double)x[i] - largest) * c, -60.0) : ((double)fmaxf(x[i], least) - largest) * c; }   // (NaN reads as no weight)
-#pragma unroll
-        for (int i = 0; i < N; ++i) { t[i] = fma(z[i], 32.0, magic); }
-#pragma unroll
-        for (int i = 0; i < N; ++i) { f[i] = fma(t[i] - magic, -1.0 / 32, z[i]); }       // |f| <= 1/64: the series of 2^f to the fifth term leaves 2e-15
-#pragma unroll
-        for (int i = 0; i < N; ++i) { e[i] = fma(1.3333558146428443e-3, f[i], 9.618129107628477e-3); }
-#pragma unroll
-        for (int i = 0; i < N; ++i) { e[i] = fma(e[i], f[i], 5.550410866482158e-2); }
-#pragma unroll
-        for (int i = 0; i < N; ++i) { e[i] = fma(e[i], f[i], 2.402265069591007e-1); }
-#pragma unroll
-        for (int i = 0; i < N; ++i) { e[i] = fma(e[i], f[i], 6.931471805599453e-1); }
-#pragma unroll
-        for (int i = 0; i < N; ++i) { e[i] = fma(e[i], f[i], 1.0); }
+            for (int i = 0; i < N; ++i) { w[i] = in_64_bits(table, (largest - (double)x[i]) * c, shift); }
+            return;
+        }
+        float p[N], e[N], t[N], f[N], y[N];
+        uint64_t full[N];
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const int k = __double2loint(t[i]);
-            e[i] *= table[k & 31];
-            e[i] = __hiloint2double(__double2hiint(e[i]) + (((k >> 5) + bits) << 20), __double2loint(e[i]));
-            w[i] = (uint64_t)(__double_as_longlong(e[i] + 4503599627370496.0) & 0xfffffffffffffll);   // + 2^52: rounded to an integer (w < 2^51)
+            const float v = fmaxf(x[i], least);                                          // (NaN reads as no weight)
+            p[i] = __fmul_rn(v, c_hi);
+            e[i] = fmaf(v, c_lo, fmaf(v, c_hi, -p[i]));
+            t[i] = __fadd_rn(fmaf(v, -1024.f * c_hi, 1024.f * a_hi), 12582912.f);
+        }
+#pragma unroll
+        for (int i = 0; i < N; ++i) { full[i] = table[__float_as_uint(t[i]) & 1023]; }
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const float r = __fsub_rn(t[i], 12582912.f);
+            f[i] = __fadd_rn(__fsub_rn(fmaf(r, -1.f / 1024, a_hi), p[i]), __fsub_rn(a_lo, e[i]));
+            y[i] = f[i] * fmaf(f[i], 0.2402265f, -0.69314718f);
+        }
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const float whole = __fsub_rn(__uint_as_float((uint32_t)(full[i] >> 23) | 0x4b000000u), 8388608.f);   // 2^23 2^-(j / 1024), cut
+            const int   more = (int)(__float_as_uint(__fadd_rn(whole * y[i], 1.5f * 8192)) - 0x46400000u);        // their product in units of 2^-10 (2^-33 of the largest weight)
+            w[i] = (full[i] + (int64_t)more * 8192) >> (((__float_as_uint(t[i]) >> 10) & 63) + shift);
         }
     }
     __device__ __forceinline__ uint64_t operator()(float x) const {
@@ -258,11 +281,14 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(const __grid_cons
             }
         }
     }
-    if (tid < 32) { sh.table[tid] = exp2((double)tid / 32); }
     const float temp = p.temperature ? p.temperature[row] : 1.f, top_p = p.top_p ? p.top_p[row] : 1.f;
     const float min_p = p.min_p ? p.min_p[row] : 0.f, uni = p.uniform ? p.uniform[row] : 0.f;
     const int   top_k = p.top_k ? p.top_k[row] : 0;
 
+    // (while the slice comes; the powers' table is needed by whoever weighs)
+    if (!(p.temperature && !(p.temperature[row] > 0.f))) {
+        for (int i = tid; i < 1024; i += SA_THREADS) { sh.table[i] = (uint64_t)(exp2(-(double)i / 1024) * 70368744177664.0 + 0.5); }
+    }
     // this thread's largest (of the elements that Slice::each gives it), the row's, and where that is
     float own = -CUDART_INF_F, from_here = CUDART_INF_F;      // (top-k: nothing below from_here is among the k largest)
     uint64_t best = 0;
@@ -285,7 +311,8 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(const __grid_cons
                 const int first = (from / 4 - tid + SA_THREADS - 1) / SA_THREADS * SA_THREADS + tid;
                 for (int i = 4 * max(first, tid); i < to; i += 4 * SA_THREADS) {
                     float4 v = *reinterpret_cast<const float4 *>(slice + i);
-                    if (!(v.x == v.x && v.y == v.y && v.z == v.z && v.w == v.w)) {
+                    const float all = (v.x + v.y) + (v.z + v.w);     // (NaN if one of them is)
+                    if (!(all == all)) {
                         v = make_float4(v.x == v.x ? v.x : -CUDART_INF_F, v.y == v.y ? v.y : -CUDART_INF_F, v.z == v.z ? v.z : -CUDART_INF_F, v.w == v.w ? v.w : -CUDART_INF_F);
                         *reinterpret_cast<float4 *>(slice + i) = v;
                     }
@@ -364,10 +391,7 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(const __grid_cons
         }
     }
     Weight weight;
-    weight.table = sh.table; weight.bits = p.frac_bits; weight.largest = largest;
-    weight.c = fmax(fmin(1.4426950408889634073599 / (double)temp, 1e30), 1e-30);
-    const double lowest = (double)largest - 60 * fmin(fmax(0.69314718055994530942 * (double)temp, 1e-30), 1e30);   // weight 2^-60, and with it all below, rounds to 0
-    weight.edge = lowest < -3.4e38 || fabs((double)largest) * weight.c > 8e6; weight.least = weight.edge ? 0.f : (float)lowest;   // (f32 spacing: 2^-23 of the largest)
+    weight.set(sh.table, largest, fmax(fmin(1.4426950408889634073599 / (double)temp, 1e30), 1e-30), p.frac_bits);
     const double one = __hiloint2double((1023 + p.frac_bits) << 20, 0);
     const uint64_t least = min_p > 0.f ? (uint64_t)max(1.0, ceil((double)fminf(min_p, 1.f) * one)) : 1;
     const float  bin_scale = (float)(weight.c * (SA_BINS / (double)(p.frac_bits + 1)));
@@ -646,16 +670,24 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(const __grid_cons
     const float cut_value = cut == 0 ? -CUDART_INF_F : value_of(cut);
     const int   cut_index = cut == 0 ? p.n_vocab : index_of(cut);
     auto stays = [&](float v, int i, uint64_t w) {
-        return (v > cut_value || (v == cut_value && x.base + i <= cut_index)) && w >= least ? w : (uint64_t)0;
+        return v >= cut_value && !(v == cut_value && x.base + i > cut_index) && w >= least ? w : (uint64_t)0;
     };
     uint64_t s = 0;
-    x.stretch(from, to, lane, 32, [&](const float (&v)[4], int i) {
-        if (fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])) < cut_value) { return; }
-        uint64_t w[4];
-        weight.of(v, w);
+    if (cut == 0 && least == 1) {                         // (all of them)
+        x.stretch(from, to, lane, 32, [&](const float (&v)[4], int) {
+            uint64_t w[4];
+            weight.of(v, w);
+            s += (w[0] + w[1]) + (w[2] + w[3]);
+        });
+    } else {
+        x.stretch(from, to, lane, 32, [&](const float (&v)[4], int i) {
+            if (fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])) < cut_value) { return; }
+            uint64_t w[4];
+            weight.of(v, w);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) { s += stays(v[e], i + e, w[e]); }
-    });
+            for (int e = 0; e < 4; ++e) { s += stays(v[e], i + e, w[e]); }
+        });
+    }
     s = warp_sum64(s);
     __syncthreads();
     if (lane == 0) { sh.scan[warp] = s; }
