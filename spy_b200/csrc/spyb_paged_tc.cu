@@ -29,18 +29,44 @@ constexpr uint32_t PT_HALF = PT_KEYS * 128;              // bytes of 128 rows x 
 template <int HD> struct TcShape {
     static constexpr uint32_t OPERAND = PT_KEYS * HD * 2;                      // a tile of Q, K or V
     static constexpr int SLOTS = HD == 128 ? 5 : 8;                            // K and V tiles in flight
-    static constexpr uint32_t SMEM = (2 + SLOTS) * OPERAND + 1024;             // (+ alignment)
+    static constexpr int Q_BUFFERS = HD == 128 ? 1 : 2;                        // (heads of 64: the next stretch's Q comes while this one's is in use)
+    static constexpr uint32_t SMEM = (2 * Q_BUFFERS + SLOTS) * OPERAND + 1024; // (+ alignment)
+    // tensor memory: S of both tiles, then O of both; P over S, or for heads of 64, whose O leaves room, beside it: the next S is made while P is
+    static constexpr bool P_APART = HD == 64;
+    static constexpr uint32_t P_COLUMN = P_APART ? 256 : 0, P_STEP = P_APART ? 64 : 128, O_COLUMN = P_APART ? 384 : 256;
 };
+struct Tile {
+    int rows, pos_first, pos_last;                   // of up to 128 rows: how many there are, positions of the first and the last
+    int from, to;                                    // steps (of the item) in which it sees anything, within the stretch
+};
+// One stretch of an item: `todo` steps of 128 positions from step `off` of the item on (todo = 0: behind the last one). The copying warp finds them one after the other
+// for all roles.
+struct Entry {
+    int todo, off, lo, hi;                           // positions [lo, hi) of the item
+    int seq, head, tile, row0, first;                // first row of the sequence, its position
+    int begin, end;                                  // steps in which either tile sees something: one run, for the second one's positions begin at the first one's end at the latest
+    int c0, parts;                                   // the CTAs of the item
+    Tile half[2];
+    // all rows of a tile see all positions of the step (if their pages are there)
+    __device__ __forceinline__ bool whole(const PagedAttention &p, const Tile &h, int step) const {
+        const int j = lo + step * PT_KEYS;
+        return j + PT_KEYS <= hi && (!p.causal || (j + PT_KEYS - 1 <= h.pos_first && (p.window <= 0 || j > h.pos_last - p.window)));
+    }
+};
+constexpr int PT_ENTRIES = 4, PT_READERS = 11;       // stretches known ahead; warps that read them: eight for probabilities, one for MMAs, two for Q and V
 struct TcShared {
     uint64_t full[8], empty[8];                          // a slot's copies have landed; its last MMA is done
     uint64_t clean[8];                                   // of the last V tiles: what nobody sees is cleared
-    uint64_t q_ready[2], q_free[2], s_ready[2], p_ready[2][2], o_ready[2];   // of the two tiles, in stretches in which they see anything; (P) of their first 96 positions and the rest
+    uint64_t q_ready[2][2], q_free[2][2];                // of the two tiles and their buffers, in stretches in which they see anything
+    uint64_t s_ready[2], s_free[2], p_ready[2][2], p_free[2], o_ready[2];   // (P ready) of the first 96 positions and the rest; (free) where P lies apart
+    uint64_t known[PT_ENTRIES], read[PT_ENTRIES];        // an entry is there; all have read it
+    uint64_t joined[2];                                  // all threads of a tile have come so far
     uint32_t tmem;
     uint32_t there[8];                                   // of the last tiles: which groups of eight positions are there
     int      poison[8];                                  // of the last stretches: a V tile that some rows see in part holds values that are not finite
-    int      last[2], more[2];
+    int      last[2];
+    Entry    entry[PT_ENTRIES];
     PagedPlanShared plan;
-    uint64_t walk[2][24];                                // the probability warpgroups' Walk: in registers it would push scores out of them
 };
 
 __device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap *map, uint32_t bar, int x, int token, int head, int page) {
@@ -80,58 +106,43 @@ __device__ __forceinline__ float max3(float a, float b, float c) { float d; asm(
 __device__ __forceinline__ float exp2_fast(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
 __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) { uint32_t r; asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo)); return r; }
 __device__ __forceinline__ uint32_t not_finite(uint32_t h2) { return ((h2 & 0x7c007c00u) + 0x04000400u) & 0x80008000u; }
-// the tiles make their probabilities in turn: together they would share the unit for powers of two, and then wait together for their products
-__device__ __forceinline__ void turn_wait(int t) { asm volatile("bar.sync %0, 256;" ::"r"(3 + t) : "memory"); }
-__device__ __forceinline__ void turn_give(int t) { asm volatile("bar.arrive %0, 256;" ::"r"(3 + t) : "memory"); }
-__device__ __forceinline__ void group_sync(int t) { asm volatile("bar.sync %0, 128;" ::"r"(1 + t) : "memory"); }
-
-// One stretch of an item: `todo` steps of 128 positions from step `off` of the item on. Every role walks the same stretches.
-struct Tile {
-    int rows, pos_first, pos_last;                   // of 128 rows: how many there are, positions of the first and the last
-    int from, to;                                    // steps (of the item) in which it sees anything, within the stretch
-    // all rows see all positions of the step (if their pages are there)
-    __device__ __forceinline__ bool whole(const PagedAttention &p, const PagedItem &it, int step) const {
-        const int j = it.lo + step * PT_KEYS;
-        return j + PT_KEYS <= it.hi && (!p.causal || (j + PT_KEYS - 1 <= pos_first && (p.window <= 0 || j > pos_last - p.window)));
-    }
-};
-struct Stretch {
+struct Walker {                                      // the copying warp's place in the work
     PagedSeq  q;
-    PagedItem it;
-    int seq, head, tile, off, todo;
+    PagedPlace at;
+    int seq, head, tile, off;
 
-    __device__ __forceinline__ Tile half(const PagedAttention &p, int t) const {
+    __device__ __forceinline__ Tile half(const PagedAttention &p, const Entry &e, int t) const {
         Tile h;
         const int r0 = tile * p.tile_rows + t * (p.tile_rows / 2);
         h.rows = max(0, min(p.tile_rows / 2, q.rows * p.group - r0));
         h.pos_first = q.first + (int)((unsigned)r0 / (unsigned)p.group);
         h.pos_last = q.first + (int)((unsigned)(r0 + max(h.rows, 1) - 1) / (unsigned)p.group);
-        const int hi = p.causal ? min(it.hi, h.pos_last + 1) : it.hi, lo = p.causal && p.window > 0 ? max(it.lo, h.pos_first - p.window + 1) : it.lo;
-        h.from = max(off, (max(lo, it.lo) - it.lo) / PT_KEYS);
-        h.to = h.rows == 0 || hi <= it.lo ? off : min(off + todo, (hi - it.lo + PT_KEYS - 1) / PT_KEYS);
+        const int hi = p.causal ? min(e.hi, h.pos_last + 1) : e.hi, lo = p.causal && p.window > 0 ? max(e.lo, h.pos_first - p.window + 1) : e.lo;
+        h.from = max(off, (lo - e.lo) / PT_KEYS);
+        h.to = h.rows == 0 || hi <= e.lo ? off : min(off + e.todo, (hi - e.lo + PT_KEYS - 1) / PT_KEYS);
         if (h.to <= h.from) { h.from = h.to = off; }
         return h;
     }
-    __device__ __forceinline__ void describe(const PagedAttention &p, const PagedPlace &at) {
-        it = paged_item<PT_KEYS, PT_KEYS>(p, q, tile);
-        todo = (int)min((int64_t)(it.units - off), at.end - at.unit);
+    __device__ __forceinline__ Entry entry(const PagedAttention &p) const {
+        const PagedItem it = paged_item<PT_KEYS, PT_KEYS>(p, q, tile);
+        Entry e;
+        e.todo = (int)min((int64_t)(it.units - off), at.end - at.unit);
+        e.off = off; e.lo = it.lo; e.hi = it.hi; e.seq = seq; e.head = head; e.tile = tile; e.row0 = q.row0; e.first = q.first;
+        const Tile a = half(p, e, 0), b = half(p, e, 1);
+        e.half[0] = a; e.half[1] = b;
+        e.begin = a.to <= a.from ? b.from : b.to <= b.from ? a.from : min(a.from, b.from);
+        e.end = a.to <= a.from ? b.to : b.to <= b.from ? a.to : max(a.to, b.to);
+        const PagedCut cut = paged_cut(at, at.unit - off, it.units);
+        e.c0 = cut.c0; e.parts = cut.parts;
+        return e;
     }
-    __device__ __forceinline__ bool next(const PagedAttention &p, PagedPlace &at) {
+    __device__ __forceinline__ bool next(const PagedAttention &p, int todo) {
         at.unit += todo;
         if (at.unit >= at.end) { return false; }
         off = 0;
         return paged_next(p, false, q, seq, head, tile);
     }
 };
-struct Walk { Stretch x; PagedPlace at; };
-static_assert(sizeof(Walk) <= sizeof(TcShared::walk[0]), "room for the walk");
-// steps in which either tile sees something: one run, for the second one's positions begin at the first one's end at the latest
-struct Steps { int begin, end; };
-__device__ __forceinline__ Steps steps_of(const Tile &a, const Tile &b) {
-    if (a.to <= a.from) { return {b.from, b.to}; }
-    if (b.to <= b.from) { return {a.from, a.to}; }
-    return {min(a.from, b.from), max(a.to, b.to)};
-}
 
 template <int HD>
 __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_constant__ PagedAttention p, const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
@@ -141,93 +152,87 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
     extern __shared__ uint8_t raw[];
     __shared__ TcShared sh;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const uint32_t base = (smem_u32(raw) + 1023) & ~1023u, q_addr = base, ring = base + 2 * Shape::OPERAND;
-    const uint32_t full = smem_u32(sh.full), empty = smem_u32(sh.empty), clean = smem_u32(sh.clean);
-    const uint32_t q_ready = smem_u32(sh.q_ready), s_ready = smem_u32(sh.s_ready), p_ready = smem_u32(sh.p_ready), o_ready = smem_u32(sh.o_ready), q_free = smem_u32(sh.q_free);
+    const uint32_t base = (smem_u32(raw) + 1023) & ~1023u, q_addr = base, ring = base + 2 * Shape::Q_BUFFERS * Shape::OPERAND;
+    const uint32_t full = smem_u32(sh.full), empty = smem_u32(sh.empty), clean = smem_u32(sh.clean), known = smem_u32(sh.known), read = smem_u32(sh.read), joined = smem_u32(sh.joined);
+    const uint32_t q_ready = smem_u32(sh.q_ready), q_free = smem_u32(sh.q_free), s_ready = smem_u32(sh.s_ready), s_free = smem_u32(sh.s_free), p_ready = smem_u32(sh.p_ready),
+                   o_ready = smem_u32(sh.o_ready), p_free = smem_u32(sh.p_free);
     if (tid == 0) {
         for (int i = 0; i < 8; ++i) { mbar_init(full + 8 * i, 1); mbar_init(empty + 8 * i, 1); mbar_init(clean + 8 * i, 2); sh.poison[i] = 0; }
-        for (int t = 0; t < 2; ++t) { mbar_init(q_ready + 8 * t, 1); mbar_init(q_free + 8 * t, 1); mbar_init(s_ready + 8 * t, 1); mbar_init(p_ready + 16 * t, 4); mbar_init(p_ready + 16 * t + 8, 4); mbar_init(o_ready + 8 * t, 1); }
+        for (int i = 0; i < 4; ++i) { mbar_init(q_ready + 8 * i, 1); mbar_init(q_free + 8 * i, 1); mbar_init(p_ready + 8 * i, 4); }
+        for (int t = 0; t < 2; ++t) { mbar_init(s_ready + 8 * t, 1); mbar_init(s_free + 8 * t, 4); mbar_init(o_ready + 8 * t, 1); mbar_init(p_free + 8 * t, 1); mbar_init(joined + 8 * t, 4); }
+        for (int i = 0; i < PT_ENTRIES; ++i) { mbar_init(known + 8 * i, 1); mbar_init(read + 8 * i, PT_READERS); }
         mbar_init_fence();
     }
     pdl_launch_dependents();
     pdl_wait();
-    PagedPlace at = paged_plan<PT_THREADS, PT_KEYS, PT_KEYS>(p, false, 2, sh.plan);
-    if (at.unit >= at.end) { return; }
+    Walker walk;
+    walk.at = paged_plan<PT_THREADS, PT_KEYS, PT_KEYS>(p, false, 2, sh.plan);
+    if (walk.at.unit >= walk.at.end) { return; }
     if (warp == 8) { asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&sh.tmem)) : "memory"); }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = sh.tmem;
     uint64_t limit = wait_limit;
-    Stretch x;
-    x.seq = at.seq; x.head = at.head; x.tile = at.tile; x.off = at.off;
-    x.q = paged_seq(p.view, at.seq);
+    uint32_t stretch = 0;
+    // the next entry; false behind the last one, or when a wait gave up (the roles then end one after the other: nobody waits without a limit)
+    auto next_entry = [&]() {
+        mbar_wait_lean(known + 8 * (stretch & (PT_ENTRIES - 1)), (stretch / PT_ENTRIES) & 1, limit);
+        return limit != 0 && sh.entry[stretch & (PT_ENTRIES - 1)].todo != 0;
+    };
+    auto entry_read = [&](bool by_me) {
+        if (by_me) { mbar_arrive(read + 8 * (stretch & (PT_ENTRIES - 1))); }
+        ++stretch;
+    };
 
     if (warp < 8) {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(PT_REGS_SOFTMAX));
         // ---------------------------------------------------------------------------------- probabilities, output
         const int t = warp >> 2, row = tid & 127;
         const uint32_t lanes = (uint32_t)(warp & 3) << 21;                                   // (32 lanes a warp, in the address's upper half)
-        const uint32_t s_tmem = tmem + lanes + t * PT_KEYS, o_tmem = tmem + lanes + 2 * PT_KEYS + t * HD;
+        const uint32_t s_tmem = tmem + lanes + t * PT_KEYS, p_tmem = tmem + lanes + Shape::P_COLUMN + t * Shape::P_STEP, o_tmem = tmem + lanes + Shape::O_COLUMN + t * HD;
         const float scale = p.scale_log2;
         const int half_tokens = PT_ROWS / p.group, row_token = (int)((unsigned)row / (unsigned)p.group), g = row - row_token * p.group;   // a tile has whole tokens
-        uint32_t s_phase = 0, o_phase = 0, tiles = 0, stretch = 0;
-        Walk &w = *reinterpret_cast<Walk *>(sh.walk[t]);
-        if (row == 0) { x.describe(p, at); w.x = x; w.at = at; }
-        group_sync(t);
-        for (;;) {
+        uint32_t s_phase = 0, o_phase = 0, joined_phase = 0, p_phase = 1, tiles = 0;
+        auto all_of_tile = [&]() {                            // the tile's four warps
+            __syncwarp();
+            if (lane == 0) { mbar_arrive(joined + 8 * t); }
+            mbar_wait_lean(joined + 8 * t, joined_phase, limit);
+            joined_phase ^= 1;
+        };
+        while (next_entry()) {
+            const Entry &en = sh.entry[stretch & (PT_ENTRIES - 1)];
             float m = -CUDART_INF_F, l = 0.f;
-            const Tile own = w.x.half(p, t);
-            const Tile other = w.x.half(p, 1 - t);
-            const Steps steps = steps_of(own, other), both = {max(own.from, other.from), min(own.to, other.to)};
-            const int token = (2 * w.x.tile + t) * half_tokens + row_token, pos = w.x.q.first + token;   // (of rows that are there)
+            const Tile own = en.half[t];
+            const int token = (2 * en.tile + t) * half_tokens + row_token, pos = en.first + token;   // (of rows that are there)
             for (int step = own.from; step < own.to; ++step) {
                 mbar_wait_lean(s_ready + 8 * t, s_phase, limit);
                 s_phase ^= 1;
                 tc_fence_after();
                 uint32_t s[128];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) { tmem_ld32(s_tmem + 32 * i, s + 32 * i); }
-                const uint32_t there = *reinterpret_cast<volatile uint32_t *>(&sh.there[(tiles + step - steps.begin) & 7]);
-                const bool plain = there == 0xffffu && own.whole(p, w.x.it, step);
+                tmem_ld32(s_tmem, s);
+                const uint32_t there = *reinterpret_cast<volatile uint32_t *>(&sh.there[(tiles + step - en.begin) & 7]);
+                const bool plain = there == 0xffffu && en.whole(p, own, step);
                 tmem_ld_wait();
+#pragma unroll
+                for (int i = 1; i < 4; ++i) { tmem_ld32(s_tmem + 32 * i, s + 32 * i); }
                 if (!plain) {
-                    const int j0 = w.x.it.lo + step * PT_KEYS;
-                    const int c1 = (p.causal ? min(w.x.it.hi, pos + 1) : w.x.it.hi) - j0, c0 = p.causal && p.window > 0 ? pos - p.window + 1 - j0 : 0;
+                    const int j0 = en.lo + step * PT_KEYS;
+                    const int c1 = (p.causal ? min(en.hi, pos + 1) : en.hi) - j0, c0 = p.causal && p.window > 0 ? pos - p.window + 1 - j0 : 0;
+                    tmem_ld_wait();
 #pragma unroll
-                    for (int c = 0; c < 128; ++c) {
-                        if (!(c >= c0 && c < c1 && ((there >> (c >> 3)) & 1))) { s[c] = 0xff800000u; }
-                    }
-                }
-                float tops[4];
+                    for (int i = 0; i < 4; ++i) {
+                        const int a = min(max(c0 - 32 * i, 0), 32), b = min(max(c1 - 32 * i, 0), 32);
+                        uint32_t seen = ((there >> 4 * i & 15) * 0x00204081u & 0x01010101u) * 0xffu;      // (four groups of eight)
+                        seen &= (b == 32 ? 0xffffffffu : (1u << b) - 1) & (a == 32 ? 0u : 0xffffffffu << a);
+                        if (__all_sync(0xffffffffu, seen == 0xffffffffu)) { continue; }
 #pragma unroll
-                for (int e = 0; e < 4; ++e) { tops[e] = fmaxf(__uint_as_float(s[2 * e]), __uint_as_float(s[2 * e + 1])); }
-#pragma unroll
-                for (int c = 8; c < 128; c += 8) {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) { tops[e] = max3(tops[e], __uint_as_float(s[c + 2 * e]), __uint_as_float(s[c + 2 * e + 1])); }
-                }
-                const float top = fmaxf(max3(tops[0], tops[1], tops[2]), tops[3]) * scale;
-                if (__any_sync(0xffffffffu, top > m + 8.f)) {
-                    const float to = fmaxf(m, top), f = to == m ? 1.f : exp2_fast(m - to);
-                    m = to; l *= f;
-                    if (step != own.from) {
-#pragma unroll 1
-                        for (int i = 0; i < HD / 16; ++i) {
-                            uint32_t o[16];
-                            tmem_ld16(o_tmem + 16 * i, o);
-                            tmem_ld_wait();
-#pragma unroll
-                            for (int c = 0; c < 16; ++c) { o[c] = __float_as_uint(__uint_as_float(o[c]) * f); }
-                            tmem_st16(o_tmem + 16 * i, o);
-                        }
+                        for (int c = 0; c < 32; ++c) { if (!(seen >> c & 1)) { s[32 * i + c] = 0xff800000u; } }
                     }
                 }
                 const uint64_t scale2 = f2_pack(scale, scale);
-                const float neg = m == -CUDART_INF_F ? 0.f : -m;
-                const uint64_t neg2 = f2_pack(neg, neg);
-                uint64_t sum[2] = {0, 0};
-                auto powers = [&](int i) {                    // probabilities of these columns against m, into tensor memory over scores that are read
+                uint64_t neg2 = 0, sum[2] = {0, 0};
+                auto powers = [&](int i) {                    // probabilities of these columns against m, into tensor memory
                     uint32_t h[16];
 #pragma unroll
                     for (int c = 0; c < 16; ++c) {
@@ -237,35 +242,72 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
                         sum[c & 1] = f2_add(sum[c & 1], f2_pack(a, b));
                         h[c] = pack_f16(a, b);
                     }
-                    tmem_st16(s_tmem + 16 * i, h);
+                    tmem_st16(p_tmem + 16 * i, h);
                 };
-                auto hand_over = [&](int half) {
+                auto hand_over = [&](int part) {
                     tmem_st_wait();
                     tc_fence_before();
                     __syncwarp();
-                    if (lane == 0) { mbar_arrive(p_ready + 16 * t + 8 * half); }
+                    if (lane == 0) { mbar_arrive(p_ready + 16 * t + 8 * part); }
                 };
-                const bool in_turn = step >= both.begin && step < both.end;
-                if (in_turn && (t == 1 || step > both.begin)) { turn_wait(t); }
-                powers(0); powers(1); powers(2);
+                if (Shape::P_APART) { mbar_wait_lean(p_free + 8 * t, p_phase, limit); p_phase ^= 1; tc_fence_after(); }   // (P's products of the step before; else S is made behind them)
+                // Powers against the maximum of the steps before, which nearly always does; whether it did shows beside them. (Not the stretch's first time round.)
+                bool fresh = step == own.from;
+                for (;;) {
+                    const float neg = m == -CUDART_INF_F ? 0.f : -m;
+                    neg2 = f2_pack(neg, neg);
+                    sum[0] = sum[1] = 0;
+                    if (!fresh) { powers(0); }
+                    tmem_ld_wait();
+                    if (!fresh) { powers(1); }
+                    float tops[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) { tops[e] = fmaxf(__uint_as_float(s[2 * e]), __uint_as_float(s[2 * e + 1])); }
+#pragma unroll
+                    for (int c = 8; c < 128; c += 8) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) { tops[e] = max3(tops[e], __uint_as_float(s[c + 2 * e]), __uint_as_float(s[c + 2 * e + 1])); }
+                    }
+                    const float top = fmaxf(max3(tops[0], tops[1], tops[2]), tops[3]) * scale;
+                    if (__any_sync(0xffffffffu, top > m + 8.f)) {
+                        const float to = fmaxf(m, top), f = to == m ? 1.f : exp2_fast(m - to);
+                        m = to; l *= f;
+                        if (step != own.from) {
+#pragma unroll 1
+                            for (int i = 0; i < HD / 16; ++i) {
+                                uint32_t o[16];
+                                tmem_ld16(o_tmem + 16 * i, o);
+                                tmem_ld_wait();
+#pragma unroll
+                                for (int c = 0; c < 16; ++c) { o[c] = __float_as_uint(__uint_as_float(o[c]) * f); }
+                                tmem_st16(o_tmem + 16 * i, o);
+                            }
+                        }
+                    } else if (!fresh) { break; }
+                    fresh = false;
+                }
+                if (Shape::P_APART) {                         // (S is in registers)
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) { mbar_arrive(s_free + 8 * t); }
+                }
+                powers(2);
                 hand_over(0);                                 // (their products run beside the last powers)
                 powers(3);
-                if (in_turn && (t == 0 || step + 1 < both.end)) { turn_give(1 - t); }
                 hand_over(1);
                 float a, b;
                 f2_unpack(f2_add(sum[0], sum[1]), a, b);
                 l += a + b;
             }
-            tiles += steps.end - steps.begin;
+            tiles += en.end - en.begin;
             // this stretch's findings
-            const bool any = own.to > own.from;
+            const bool any = own.to > own.from, mine = row < own.rows;      // (rows behind the last whole token are nobody's)
+            const int  parts = en.parts, c0 = en.c0;
             if (any) { mbar_wait_lean(o_ready + 8 * t, o_phase, limit); o_phase ^= 1; tc_fence_after(); }
-            const PagedCut cut = paged_cut(w.at, w.at.unit - w.x.off, w.x.it.units);
-            float4 *part = reinterpret_cast<float4 *>(p.partial) + (paged_slot(blockIdx.x, cut.c0) * 2 + t) * (PT_ROWS * (HD + 2) / 4);     // [HD / 4][128] x 4, [128], [128]
-            const float inv = cut.parts > 1 ? 1.f : l == 0.f ? 0.f : 1.f / l;
-            const bool mine = row < own.rows;                       // (rows behind the last whole token are nobody's)
+            float4 *part = reinterpret_cast<float4 *>(p.partial) + (paged_slot(blockIdx.x, c0) * 2 + t) * (PT_ROWS * (HD + 2) / 4);     // [HD / 4][128] x 4, [128], [128]
+            const float inv = parts > 1 ? 1.f : l == 0.f ? 0.f : 1.f / l;
             const bool poisoned = any && *reinterpret_cast<volatile int *>(&sh.poison[stretch & 7]) == (int)stretch + 1;
-            const int64_t to_row = (int64_t)(w.x.q.row0 + token) * p.out_stride + (w.x.head * p.group + g) * HD;
+            const int64_t to_row = (int64_t)(en.row0 + token) * p.out_stride + (en.head * p.group + g) * HD;
 #pragma unroll 1
             for (int i = 0; i < HD / 32; ++i) {
                 uint32_t o[32];
@@ -276,14 +318,14 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
                 }
                 if (poisoned && mine) {
                     // values that are not finite were taken out of the V tiles that not all rows see whole: back to the rows that see them
-                    const Stretch done = w.x;
+                    const Tile other = en.half[1 - t];
                     for (int step = own.from; step < own.to; ++step) {
-                        if (own.whole(p, done.it, step) && other.whole(p, done.it, step)) { continue; }
-                        const int j0 = done.it.lo + step * PT_KEYS, ja = max(j0, p.causal && p.window > 0 ? pos - p.window + 1 : 0), jb = min(j0 + PT_KEYS, p.causal ? min(done.it.hi, pos + 1) : done.it.hi);
+                        if (en.whole(p, own, step) && en.whole(p, other, step)) { continue; }
+                        const int j0 = en.lo + step * PT_KEYS, ja = max(j0, p.causal && p.window > 0 ? pos - p.window + 1 : 0), jb = min(j0 + PT_KEYS, p.causal ? min(en.hi, pos + 1) : en.hi);
                         for (int j = ja; j < jb; ++j) {
-                            const int page = p.view.page_table[(int64_t)done.seq * p.view.table_stride + j / p.view.page_size];
+                            const int page = p.view.page_table[(int64_t)en.seq * p.view.table_stride + j / p.view.page_size];
                             if (page < 0 || page >= p.view.n_pages) { continue; }
-                            const __half *v = p.v + page * p.view.page_stride + (j % p.view.page_size) * p.view.token_stride + done.head * p.view.head_stride + 32 * i;
+                            const __half *v = p.v + page * p.view.page_stride + (j % p.view.page_size) * p.view.token_stride + en.head * p.view.head_stride + 32 * i;
 #pragma unroll
                             for (int c = 0; c < 32; ++c) {
                                 const float y = __half2float(v[c]);
@@ -292,7 +334,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
                         }
                     }
                 }
-                if (cut.parts > 1) {
+                if (parts > 1) {
 #pragma unroll
                     for (int c = 0; c < 8; ++c) {
                         part[(8 * i + c) * PT_ROWS + row] = make_float4(__uint_as_float(o[4 * c]), __uint_as_float(o[4 * c + 1]), __uint_as_float(o[4 * c + 2]), __uint_as_float(o[4 * c + 3]));
@@ -317,41 +359,42 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
                 }
             }
             tc_fence_before();
-            if (cut.parts > 1) {
+            if (parts > 1) {
                 float *stats = reinterpret_cast<float *>(part + PT_ROWS * HD / 4);
                 stats[row] = m; stats[PT_ROWS + row] = l;
-                group_sync(t);
+                __threadfence();
+                all_of_tile();
                 if (row == 0) {
                     __threadfence();
-                    unsigned *arrived = p.arrived + 2 * cut.c0 + t;
-                    const bool last = atomicAdd(arrived, 1u) == (unsigned)cut.parts - 1;
+                    unsigned *arrived = p.arrived + 2 * c0 + t;
+                    const bool last = atomicAdd(arrived, 1u) == (unsigned)parts - 1;
                     if (last) { *arrived = 0; __threadfence(); }
-                    sh.last[t] = last;
+                    *reinterpret_cast<volatile int *>(&sh.last[t]) = last;
                 }
-                group_sync(t);
-                if (sh.last[t]) {
+                all_of_tile();
+                if (*reinterpret_cast<volatile int *>(&sh.last[t])) {
                     const float4 *all = reinterpret_cast<const float4 *>(p.partial);
-                    auto piece = [&](int i) { return all + (paged_slot(cut.c0 + i, cut.c0) * 2 + t) * (PT_ROWS * (HD + 2) / 4); };
+                    auto piece = [&](int i) { return all + (paged_slot(c0 + i, c0) * 2 + t) * (PT_ROWS * (HD + 2) / 4); };
                     if (mine) {
                         float top = -CUDART_INF_F, sum = 0.f;
 #pragma unroll 4
-                        for (int i = 0; i < cut.parts; ++i) { top = fmaxf(top, __ldcg(reinterpret_cast<const float *>(piece(i) + PT_ROWS * HD / 4) + row)); }
+                        for (int i = 0; i < parts; ++i) { top = fmaxf(top, __ldcg(reinterpret_cast<const float *>(piece(i) + PT_ROWS * HD / 4) + row)); }
                         const float ref = top == -CUDART_INF_F ? 0.f : top;
 #pragma unroll 1
-                        for (int c0 = 0; c0 < HD / 4; c0 += 16) {
+                        for (int q4 = 0; q4 < HD / 4; q4 += 16) {
                             float4 v[16];
 #pragma unroll
                             for (int c = 0; c < 16; ++c) { v[c] = make_float4(0.f, 0.f, 0.f, 0.f); }
                             sum = 0.f;
 #pragma unroll 1
-                            for (int i = 0; i < cut.parts; ++i) {
+                            for (int i = 0; i < parts; ++i) {
                                 const float4 *from = piece(i);
                                 const float *st = reinterpret_cast<const float *>(from + PT_ROWS * HD / 4);
                                 const float f = exp2_fast(__ldcg(st + row) - ref);
                                 sum += f * __ldcg(st + PT_ROWS + row);
 #pragma unroll
                                 for (int c = 0; c < 16; ++c) {
-                                    const float4 u = __ldcg(from + (c0 + c) * PT_ROWS + row);
+                                    const float4 u = __ldcg(from + (q4 + c) * PT_ROWS + row);
                                     v[c].x += f * u.x; v[c].y += f * u.y; v[c].z += f * u.z; v[c].w += f * u.w;
                                 }
                             }
@@ -361,24 +404,16 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
                                 const float4 a = make_float4(v[c].x * inv_all, v[c].y * inv_all, v[c].z * inv_all, v[c].w * inv_all);
                                 const float4 b = make_float4(v[c + 1].x * inv_all, v[c + 1].y * inv_all, v[c + 1].z * inv_all, v[c + 1].w * inv_all);
                                 if (p.out_f32) {
-                                    float4 *dst = reinterpret_cast<float4 *>(static_cast<float *>(p.out) + to_row + 4 * (c0 + c));
+                                    float4 *dst = reinterpret_cast<float4 *>(static_cast<float *>(p.out) + to_row + 4 * (q4 + c));
                                     dst[0] = a; dst[1] = b;
-                                } else { *reinterpret_cast<uint4 *>(static_cast<__half *>(p.out) + to_row + 4 * (c0 + c)) = make_uint4(pack_f16(a.x, a.y), pack_f16(a.z, a.w), pack_f16(b.x, b.y), pack_f16(b.z, b.w)); }
+                                } else { *reinterpret_cast<uint4 *>(static_cast<__half *>(p.out) + to_row + 4 * (q4 + c)) = make_uint4(pack_f16(a.x, a.y), pack_f16(a.z, a.w), pack_f16(b.x, b.y), pack_f16(b.z, b.w)); }
                             }
                         }
                     }
                 }
             }
-            ++stretch;
-            group_sync(t);
-            if (row == 0) {
-                x = w.x; at = w.at;
-                const bool more = x.next(p, at);
-                if (more) { x.describe(p, at); w.x = x; w.at = at; }
-                sh.more[t] = more;
-            }
-            group_sync(t);
-            if (!sh.more[t]) { break; }
+            __syncwarp();
+            entry_read(lane == 0);
         }
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PT_REGS_OTHERS));
@@ -386,42 +421,53 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
         uint32_t slot = 0, phase = 0;
         auto advance = [&]() { if (++slot == SLOTS) { slot = 0; phase ^= 1; } };
         if (warp == 9) {
-            // ------------------------------------------------------------------------------ copies
+            // ------------------------------------------------------------------------------ the stretches, and their copies
             constexpr int halves = HD / 64;                                                 // a tile's boxes are 64 elements wide
             const int group = lane % 16 * 8, half = lane >> 4;                              // this lane's eight positions of a tile, and half
             const bool issues = (group & (box - 1)) == 0 && half < halves;
             uint32_t tiles = 0;
+            walk.seq = walk.at.seq; walk.head = walk.at.head; walk.tile = walk.at.tile; walk.off = walk.at.off;
+            walk.q = paged_seq(p.view, walk.seq);
+            auto put = [&](const Entry &e) {
+                const uint32_t i = stretch & (PT_ENTRIES - 1);
+                mbar_wait_lean(read + 8 * i, ((stretch / PT_ENTRIES) & 1) ^ 1, limit);
+                if (lane == 0) { sh.entry[i] = e; mbar_arrive(known + 8 * i); }
+                ++stretch;
+            };
             for (;;) {
-                x.describe(p, at);
-                const Steps steps = steps_of(x.half(p, 0), x.half(p, 1));
-                const int32_t *table = p.view.page_table + (int64_t)x.seq * p.view.table_stride;
+                const Entry e = walk.entry(p);
+                put(e);
+                if (limit == 0) { break; }
+                const int32_t *table = p.view.page_table + (int64_t)e.seq * p.view.table_stride;
                 auto page_of = [&](int step) {                                              // (one step ahead: the table's latency is hidden)
-                    const int j = x.it.lo + step * PT_KEYS + group;
-                    return step < steps.end && j < x.it.hi ? table[j / p.view.page_size] : -1;
+                    const int j = e.lo + step * PT_KEYS + group;
+                    return step < e.end && j < e.hi ? table[j / p.view.page_size] : -1;
                 };
-                int e = page_of(steps.begin);
-                for (int step = steps.begin; step < steps.end; ++step) {
-                    const bool ok = e >= 0 && e < p.view.n_pages;
-                    const int page = ok ? e : p.view.n_pages, token = ok ? (x.it.lo + step * PT_KEYS + group) % p.view.page_size : 0;
+                int named = page_of(e.begin);
+                for (int step = e.begin; step < e.end; ++step) {
+                    const bool ok = named >= 0 && named < p.view.n_pages;
+                    const int page = ok ? named : p.view.n_pages, token = ok ? (e.lo + step * PT_KEYS + group) % p.view.page_size : 0;
                     const uint32_t there = __ballot_sync(0xffffffffu, ok) & 0xffffu;
-                    e = page_of(step + 1);
+                    named = page_of(step + 1);
 #pragma unroll
                     for (int kv = 0; kv < 2; ++kv) {
                         mbar_wait_lean(empty + 8 * slot, phase ^ 1, limit);
                         const uint32_t bar = full + 8 * slot, dst = ring + slot * Shape::OPERAND;
                         if (lane == 0) {
-                            if (kv == 0) { sh.there[tiles & 7] = there; }
+                            if (kv == 0) { *reinterpret_cast<volatile uint32_t *>(&sh.there[tiles & 7]) = there; }
                             mbar_expect_tx(bar, Shape::OPERAND);
                         }
                         __syncwarp();
-                        if (issues) { tma_load(dst + half * PT_HALF + group * 128, kv == 0 ? &k_map : &v_map, bar, half * 64, token, x.head, page); }
+                        if (issues) { tma_load(dst + half * PT_HALF + group * 128, kv == 0 ? &k_map : &v_map, bar, half * 64, token, e.head, page); }
                         __syncwarp();
                         advance();
                     }
                     ++tiles;
                 }
-                if (!x.next(p, at)) { break; }
+                if (!walk.next(p, e.todo)) { break; }
             }
+            Entry over = {};
+            put(over);
             if (limit == 0) {   // something gave up: what is on its way lands before the CTA ends
                 uint64_t again = wait_limit;
                 for (int i = 0; i < SLOTS; ++i) {
@@ -432,32 +478,30 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
             }
         } else if (warp >= 10) {
             // ------------------------------------------------------------------------------ Q of a tile each; V tiles that not all rows see whole, half of the rows each
-            uint32_t tiles = 0, stretch = 0, q_phase = 1;
-            bool asked = false;
-            const int t = warp - 10;
-            const int v_row0 = t * (PT_KEYS / 2);
-            for (;;) {
-                x.describe(p, at);
-                const Tile a = x.half(p, 0), b = x.half(p, 1);
-                const Steps steps = steps_of(a, b);
+            uint32_t tiles = 0, q_count = 0;
+            const int t = warp - 10, v_row0 = t * (PT_KEYS / 2);
+            while (next_entry()) {
+                const Entry &en = sh.entry[stretch & (PT_ENTRIES - 1)];
+                const Tile a = en.half[0], b = en.half[1];
                 if (t == 0 ? a.to > a.from : b.to > b.from) {
-                    mbar_wait_lean(q_free + 8 * t, q_phase, limit);
-                    q_phase ^= 1; asked = true;
+                    const uint32_t buffer = q_count % Shape::Q_BUFFERS, bar = 16 * t + 8 * buffer;
+                    mbar_wait_lean(q_free + bar, (q_count / Shape::Q_BUFFERS & 1) ^ 1, limit);
+                    ++q_count;
                     // whole tokens, token by token their heads: what lies behind the sequence's rows is other sequences' or nothing, and goes nowhere
                     if (elect_one()) {
-                        const int tokens = PT_ROWS / p.group, row = x.q.row0 + (2 * x.tile + t) * tokens;
-                        mbar_expect_tx(q_ready + 8 * t, tokens * p.group * HD * 2);
+                        const int tokens = PT_ROWS / p.group, row = en.row0 + (2 * en.tile + t) * tokens;
+                        mbar_expect_tx(q_ready + bar, tokens * p.group * HD * 2);
 #pragma unroll
-                        for (int h = 0; h < HD / 64; ++h) { tma_load3(q_addr + t * Shape::OPERAND + h * PT_HALF, &q_map, q_ready + 8 * t, h * 64, x.head * p.group, row); }
+                        for (int h = 0; h < HD / 64; ++h) { tma_load3(q_addr + (2 * buffer + t) * Shape::OPERAND + h * PT_HALF, &q_map, q_ready + bar, h * 64, en.head * p.group, row); }
                     }
                     __syncwarp();
                 }
-                for (int step = steps.begin; step < steps.end; ++step) {
+                for (int step = en.begin; step < en.end; ++step) {
                     advance();                                                               // (K)
                     mbar_wait_lean(full + 8 * slot, phase, limit);
-                    if (!(a.whole(p, x.it, step) && (b.rows == 0 || b.whole(p, x.it, step)))) {
-                        const int j0 = x.it.lo + step * PT_KEYS;
-                        const int first = p.causal && p.window > 0 ? max(0, a.pos_first - p.window + 1) - j0 : 0, end = x.it.hi - j0;   // rows that some query sees
+                    if (!(en.whole(p, a, step) && (b.rows == 0 || en.whole(p, b, step)))) {
+                        const int j0 = en.lo + step * PT_KEYS;
+                        const int first = p.causal && p.window > 0 ? max(0, a.pos_first - p.window + 1) - j0 : 0, end = en.hi - j0;   // rows that some query sees
                         const uint32_t v_addr = ring + slot * Shape::OPERAND;
                         uint32_t bad = 0;
                         auto piece = [&](int i) {                                            // (half, row, piece of the row)
@@ -492,87 +536,99 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
                     advance();
                     ++tiles;
                 }
-                ++stretch;
-                if (!x.next(p, at)) { break; }
+                __syncwarp();
+                entry_read(lane == 0);
             }
-            if (limit == 0 && asked) {   // (something gave up: what is on its way lands before the CTA ends)
-                uint64_t again = wait_limit;
-                mbar_wait_lean(q_ready + 8 * t, q_phase, again);
+            if (limit == 0 && q_count > 0) {   // (something gave up: what is on its way lands before the CTA ends)
+                for (uint32_t i = 1; i <= Shape::Q_BUFFERS && i <= q_count; ++i) {
+                    uint64_t again = wait_limit;
+                    const uint32_t n = q_count - i;
+                    mbar_wait_lean(q_ready + 16 * t + 8 * (n % Shape::Q_BUFFERS), n / Shape::Q_BUFFERS & 1, again);
+                }
             }
         } else if (warp == 8) {
             // ------------------------------------------------------------------------------ MMAs
             constexpr uint32_t idesc_s = idesc_f16(PT_KEYS), idesc_o = idesc_f16(HD) | (1u << 16);   // (bit 16: B is MN-major)
-            uint32_t q_phase[2] = {0, 0}, p_phase[2] = {0, 0};
-            uint32_t v_slot = 0, v_phase = 0, tiles = 0;
+            uint32_t q_count[2] = {0, 0}, s_count[2] = {0, 0}, p_phase[2] = {0, 0}, tiles = 0;
             auto scores = [&](int t, uint32_t k_slot, bool last) {
+                if (Shape::P_APART) { mbar_wait_lean(s_free + 8 * t, (s_count[t] & 1) ^ 1, limit); tc_fence_after(); }   // (else P's products, in order, are what frees S)
+                ++s_count[t];
+                const uint32_t buffer = (q_count[t] - 1) % Shape::Q_BUFFERS;
                 if (elect_one()) {
-                    const uint64_t a = swizzled_desc(q_addr + t * Shape::OPERAND, 16), b = swizzled_desc(ring + k_slot * Shape::OPERAND, 16);
+                    const uint64_t a = swizzled_desc(q_addr + (2 * buffer + t) * Shape::OPERAND, 16), b = swizzled_desc(ring + k_slot * Shape::OPERAND, 16);
 #pragma unroll
                     for (int k = 0; k < HD / 16; ++k) {
                         const uint64_t step = ((k >> 2) * PT_HALF + (k & 3) * 32) >> 4;
                         mma_f16_ss(tmem + t * PT_KEYS, a + step, b + step, idesc_s, k != 0);
                     }
                     mma_commit(s_ready + 8 * t);
-                    if (last) { mma_commit(q_free + 8 * t); }
+                    if (last) { mma_commit(q_free + 16 * t + 8 * buffer); }
                 }
                 __syncwarp();
             };
-            for (;;) {
-                x.describe(p, at);
-                const Tile halves[2] = {x.half(p, 0), x.half(p, 1)};
-                const Steps steps = steps_of(halves[0], halves[1]);
-                auto active = [&](int t, int step) { return step >= halves[t].from && step < halves[t].to; };
+            while (next_entry()) {
+                const Entry &en = sh.entry[stretch & (PT_ENTRIES - 1)];
+                const int begin = en.begin, end = en.end, from[2] = {en.half[0].from, en.half[1].from}, to[2] = {en.half[0].to, en.half[1].to};
+                __syncwarp();
+                entry_read(lane == 0);
+                auto active = [&](int t, int step) { return step >= from[t] && step < to[t]; };
 #pragma unroll
                 for (int t = 0; t < 2; ++t) {
-                    if (halves[t].to > halves[t].from) { mbar_wait_lean(q_ready + 8 * t, q_phase[t], limit); q_phase[t] ^= 1; }
+                    if (to[t] > from[t]) { mbar_wait_lean(q_ready + 16 * t + 8 * (q_count[t] % Shape::Q_BUFFERS), q_count[t] / Shape::Q_BUFFERS & 1, limit); ++q_count[t]; }
                 }
                 tc_fence_after();
-                for (int step = steps.begin; step < steps.end; ++step) {
-                    if (step == steps.begin) {
+                for (int step = begin; step < end; ++step) {
+                    if (step == begin) {
                         mbar_wait_lean(full + 8 * slot, phase, limit);
                         tc_fence_after();
-                        if (active(0, step)) { scores(0, slot, step + 1 == halves[0].to); }
-                        if (active(1, step)) { scores(1, slot, step + 1 == halves[1].to); }
+#pragma unroll
+                        for (int t = 0; t < 2; ++t) { if (active(t, step)) { scores(t, slot, step + 1 == to[t]); } }
                         if (elect_one()) { mma_commit(empty + 8 * slot); }
                         __syncwarp();
                         advance();
                     }
-                    v_slot = slot; v_phase = phase;
+                    const uint32_t v_slot = slot, v_phase = phase;
                     advance();
+                    const bool ahead = step + 1 < end;
+                    if (ahead) { mbar_wait_lean(full + 8 * slot, phase, limit); }
+                    if (Shape::P_APART && ahead) {
+#pragma unroll
+                        for (int t = 0; t < 2; ++t) { if (active(t, step + 1)) { scores(t, slot, step + 2 == to[t]); } }
+                        if (elect_one()) { mma_commit(empty + 8 * slot); }
+                        __syncwarp();
+                    }
                     mbar_wait_lean(full + 8 * v_slot, v_phase, limit);
                     mbar_wait_lean(clean + 8 * (tiles & 7), (tiles >> 3) & 1, limit);
                     ++tiles;
-                    const bool ahead = step + 1 < steps.end;
-                    if (ahead) { mbar_wait_lean(full + 8 * slot, phase, limit); }
 #pragma unroll
                     for (int t = 0; t < 2; ++t) {
                         if (active(t, step)) {
 #pragma unroll
-                            for (int half = 0; half < 2; ++half) {
-                                mbar_wait_lean(p_ready + 16 * t + 8 * half, p_phase[t], limit);
+                            for (int part = 0; part < 2; ++part) {
+                                mbar_wait_lean(p_ready + 16 * t + 8 * part, p_phase[t], limit);
                                 tc_fence_after();
                                 if (elect_one()) {
                                     const uint64_t b = swizzled_desc(ring + v_slot * Shape::OPERAND, PT_HALF);
 #pragma unroll
-                                    for (int k = 6 * half; k < 6 + 2 * half; ++k) {
-                                        mma_f16_ts(tmem + 2 * PT_KEYS + t * HD, tmem + t * PT_KEYS + 8 * k, b + ((k * 2048) >> 4), idesc_o, step != halves[t].from || k != 0);
+                                    for (int k = 6 * part; k < 6 + 2 * part; ++k) {
+                                        mma_f16_ts(tmem + Shape::O_COLUMN + t * HD, tmem + Shape::P_COLUMN + t * Shape::P_STEP + 8 * k, b + ((k * 2048) >> 4), idesc_o, step != from[t] || k != 0);
                                     }
-                                    if (half == 1 && step + 1 == halves[t].to) { mma_commit(o_ready + 8 * t); }
+                                    if (part == 1 && Shape::P_APART) { mma_commit(p_free + 8 * t); }
+                                    if (part == 1 && step + 1 == to[t]) { mma_commit(o_ready + 8 * t); }
                                 }
                                 __syncwarp();
                             }
                             p_phase[t] ^= 1;
                         }
-                        if (ahead && active(t, step + 1)) { scores(t, slot, step + 2 == halves[t].to); }
+                        if (!Shape::P_APART && ahead && active(t, step + 1)) { scores(t, slot, step + 2 == to[t]); }
                     }
                     if (elect_one()) {
                         mma_commit(empty + 8 * v_slot);
-                        if (ahead) { mma_commit(empty + 8 * slot); }
+                        if (!Shape::P_APART && ahead) { mma_commit(empty + 8 * slot); }
                     }
                     __syncwarp();
                     if (ahead) { advance(); }
                 }
-                if (!x.next(p, at)) { break; }
             }
         }
     }
