@@ -106,6 +106,12 @@ __device__ __forceinline__ float max3(float a, float b, float c) { float d; asm(
 __device__ __forceinline__ float exp2_fast(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
 __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) { uint32_t r; asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo)); return r; }
 __device__ __forceinline__ uint32_t not_finite(uint32_t h2) { return ((h2 & 0x7c007c00u) + 0x04000400u) & 0x80008000u; }
+// A wait by a whole warp. Its lanes may see the phase's end at different times, and what follows - an elected lane, tensor-memory accesses - is the whole warp's:
+// two groups of lanes would elect one each, and products and their completions would count twice.
+__device__ __forceinline__ void wait_for(uint32_t bar, uint32_t parity, uint64_t &limit) {
+    mbar_wait_lean(bar, parity, limit);
+    __syncwarp();
+}
 struct Walker {                                      // the copying warp's place in the work
     PagedSeq  q;
     PagedPlace at;
@@ -177,7 +183,8 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
     uint32_t stretch = 0;
     // the next entry; false behind the last one, or when a wait gave up (the roles then end one after the other: nobody waits without a limit)
     auto next_entry = [&]() {
-        mbar_wait_lean(known + 8 * (stretch & (PT_ENTRIES - 1)), (stretch / PT_ENTRIES) & 1, limit);
+        wait_for(known + 8 * (stretch & (PT_ENTRIES - 1)), (stretch / PT_ENTRIES) & 1, limit);
+        if (!__all_sync(0xffffffffu, limit != 0)) { limit = 0; }
         return limit != 0 && sh.entry[stretch & (PT_ENTRIES - 1)].todo != 0;
     };
     auto entry_read = [&](bool by_me) {
@@ -197,7 +204,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
         auto all_of_tile = [&]() {                            // the tile's four warps
             __syncwarp();
             if (lane == 0) { mbar_arrive(joined + 8 * t); }
-            mbar_wait_lean(joined + 8 * t, joined_phase, limit);
+            wait_for(joined + 8 * t, joined_phase, limit);
             joined_phase ^= 1;
         };
         while (next_entry()) {
@@ -206,7 +213,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
             const Tile own = en.half[t];
             const int token = (2 * en.tile + t) * half_tokens + row_token, pos = en.first + token;   // (of rows that are there)
             for (int step = own.from; step < own.to; ++step) {
-                mbar_wait_lean(s_ready + 8 * t, s_phase, limit);
+                wait_for(s_ready + 8 * t, s_phase, limit);
                 s_phase ^= 1;
                 tc_fence_after();
                 uint32_t s[128];
@@ -250,7 +257,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
                     __syncwarp();
                     if (lane == 0) { mbar_arrive(p_ready + 16 * t + 8 * part); }
                 };
-                if (Shape::P_APART) { mbar_wait_lean(p_free + 8 * t, p_phase, limit); p_phase ^= 1; tc_fence_after(); }   // (P's products of the step before; else S is made behind them)
+                if (Shape::P_APART) { wait_for(p_free + 8 * t, p_phase, limit); p_phase ^= 1; tc_fence_after(); }   // (P's products of the step before; else S is made behind them)
                 // Powers against the maximum of the steps before, which nearly always does; whether it did shows beside them. (Not the stretch's first time round.)
                 bool fresh = step == own.from;
                 for (;;) {
@@ -303,7 +310,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
             // this stretch's findings
             const bool any = own.to > own.from, mine = row < own.rows;      // (rows behind the last whole token are nobody's)
             const int  parts = en.parts, c0 = en.c0;
-            if (any) { mbar_wait_lean(o_ready + 8 * t, o_phase, limit); o_phase ^= 1; tc_fence_after(); }
+            if (any) { wait_for(o_ready + 8 * t, o_phase, limit); o_phase ^= 1; tc_fence_after(); }
             float4 *part = reinterpret_cast<float4 *>(p.partial) + (paged_slot(blockIdx.x, c0) * 2 + t) * (PT_ROWS * (HD + 2) / 4);     // [HD / 4][128] x 4, [128], [128]
             const float inv = parts > 1 ? 1.f : l == 0.f ? 0.f : 1.f / l;
             const bool poisoned = any && *reinterpret_cast<volatile int *>(&sh.poison[stretch & 7]) == (int)stretch + 1;
@@ -430,14 +437,14 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
             walk.q = paged_seq(p.view, walk.seq);
             auto put = [&](const Entry &e) {
                 const uint32_t i = stretch & (PT_ENTRIES - 1);
-                mbar_wait_lean(read + 8 * i, ((stretch / PT_ENTRIES) & 1) ^ 1, limit);
+                wait_for(read + 8 * i, ((stretch / PT_ENTRIES) & 1) ^ 1, limit);
                 if (lane == 0) { sh.entry[i] = e; mbar_arrive(known + 8 * i); }
                 ++stretch;
             };
             for (;;) {
                 const Entry e = walk.entry(p);
                 put(e);
-                if (limit == 0) { break; }
+                if (!__all_sync(0xffffffffu, limit != 0)) { limit = 0; break; }
                 const int32_t *table = p.view.page_table + (int64_t)e.seq * p.view.table_stride;
                 auto page_of = [&](int step) {                                              // (one step ahead: the table's latency is hidden)
                     const int j = e.lo + step * PT_KEYS + group;
@@ -451,7 +458,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
                     named = page_of(step + 1);
 #pragma unroll
                     for (int kv = 0; kv < 2; ++kv) {
-                        mbar_wait_lean(empty + 8 * slot, phase ^ 1, limit);
+                        wait_for(empty + 8 * slot, phase ^ 1, limit);
                         const uint32_t bar = full + 8 * slot, dst = ring + slot * Shape::OPERAND;
                         if (lane == 0) {
                             if (kv == 0) { *reinterpret_cast<volatile uint32_t *>(&sh.there[tiles & 7]) = there; }
@@ -473,7 +480,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
                 for (int i = 0; i < SLOTS; ++i) {
                     if (slot == 0) { slot = SLOTS; phase ^= 1; }
                     --slot;
-                    if (2 * tiles > (uint32_t)i) { mbar_wait_lean(full + 8 * slot, phase, again); }
+                    if (2 * tiles > (uint32_t)i) { wait_for(full + 8 * slot, phase, again); }
                 }
             }
         } else if (warp >= 10) {
@@ -485,7 +492,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
                 const Tile a = en.half[0], b = en.half[1];
                 if (t == 0 ? a.to > a.from : b.to > b.from) {
                     const uint32_t buffer = q_count % Shape::Q_BUFFERS, bar = 16 * t + 8 * buffer;
-                    mbar_wait_lean(q_free + bar, (q_count / Shape::Q_BUFFERS & 1) ^ 1, limit);
+                    wait_for(q_free + bar, (q_count / Shape::Q_BUFFERS & 1) ^ 1, limit);
                     ++q_count;
                     // whole tokens, token by token their heads: what lies behind the sequence's rows is other sequences' or nothing, and goes nowhere
                     if (elect_one()) {
@@ -497,8 +504,10 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
                     __syncwarp();
                 }
                 for (int step = en.begin; step < en.end; ++step) {
-                    advance();                                                               // (K)
-                    mbar_wait_lean(full + 8 * slot, phase, limit);
+                    // K as well, though nothing is done to it: copies land in any order, and a slot's phase that nobody waited for could be taken for the one after the next
+                    wait_for(full + 8 * slot, phase, limit);
+                    advance();
+                    wait_for(full + 8 * slot, phase, limit);
                     if (!(en.whole(p, a, step) && (b.rows == 0 || en.whole(p, b, step)))) {
                         const int j0 = en.lo + step * PT_KEYS;
                         const int first = p.causal && p.window > 0 ? max(0, a.pos_first - p.window + 1) - j0 : 0, end = en.hi - j0;   // rows that some query sees
@@ -543,7 +552,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
                 for (uint32_t i = 1; i <= Shape::Q_BUFFERS && i <= q_count; ++i) {
                     uint64_t again = wait_limit;
                     const uint32_t n = q_count - i;
-                    mbar_wait_lean(q_ready + 16 * t + 8 * (n % Shape::Q_BUFFERS), n / Shape::Q_BUFFERS & 1, again);
+                    wait_for(q_ready + 16 * t + 8 * (n % Shape::Q_BUFFERS), n / Shape::Q_BUFFERS & 1, again);
                 }
             }
         } else if (warp == 8) {
@@ -551,7 +560,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
             constexpr uint32_t idesc_s = idesc_f16(PT_KEYS), idesc_o = idesc_f16(HD) | (1u << 16);   // (bit 16: B is MN-major)
             uint32_t q_count[2] = {0, 0}, s_count[2] = {0, 0}, p_phase[2] = {0, 0}, tiles = 0;
             auto scores = [&](int t, uint32_t k_slot, bool last) {
-                if (Shape::P_APART) { mbar_wait_lean(s_free + 8 * t, (s_count[t] & 1) ^ 1, limit); tc_fence_after(); }   // (else P's products, in order, are what frees S)
+                if (Shape::P_APART) { wait_for(s_free + 8 * t, (s_count[t] & 1) ^ 1, limit); tc_fence_after(); }   // (else P's products, in order, are what frees S)
                 ++s_count[t];
                 const uint32_t buffer = (q_count[t] - 1) % Shape::Q_BUFFERS;
                 if (elect_one()) {
@@ -574,12 +583,12 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
                 auto active = [&](int t, int step) { return step >= from[t] && step < to[t]; };
 #pragma unroll
                 for (int t = 0; t < 2; ++t) {
-                    if (to[t] > from[t]) { mbar_wait_lean(q_ready + 16 * t + 8 * (q_count[t] % Shape::Q_BUFFERS), q_count[t] / Shape::Q_BUFFERS & 1, limit); ++q_count[t]; }
+                    if (to[t] > from[t]) { wait_for(q_ready + 16 * t + 8 * (q_count[t] % Shape::Q_BUFFERS), q_count[t] / Shape::Q_BUFFERS & 1, limit); ++q_count[t]; }
                 }
                 tc_fence_after();
                 for (int step = begin; step < end; ++step) {
                     if (step == begin) {
-                        mbar_wait_lean(full + 8 * slot, phase, limit);
+                        wait_for(full + 8 * slot, phase, limit);
                         tc_fence_after();
 #pragma unroll
                         for (int t = 0; t < 2; ++t) { if (active(t, step)) { scores(t, slot, step + 1 == to[t]); } }
@@ -590,22 +599,22 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
                     const uint32_t v_slot = slot, v_phase = phase;
                     advance();
                     const bool ahead = step + 1 < end;
-                    if (ahead) { mbar_wait_lean(full + 8 * slot, phase, limit); }
+                    if (ahead) { wait_for(full + 8 * slot, phase, limit); }
                     if (Shape::P_APART && ahead) {
 #pragma unroll
                         for (int t = 0; t < 2; ++t) { if (active(t, step + 1)) { scores(t, slot, step + 2 == to[t]); } }
                         if (elect_one()) { mma_commit(empty + 8 * slot); }
                         __syncwarp();
                     }
-                    mbar_wait_lean(full + 8 * v_slot, v_phase, limit);
-                    mbar_wait_lean(clean + 8 * (tiles & 7), (tiles >> 3) & 1, limit);
+                    wait_for(full + 8 * v_slot, v_phase, limit);
+                    wait_for(clean + 8 * (tiles & 7), (tiles >> 3) & 1, limit);
                     ++tiles;
 #pragma unroll
                     for (int t = 0; t < 2; ++t) {
                         if (active(t, step)) {
 #pragma unroll
                             for (int part = 0; part < 2; ++part) {
-                                mbar_wait_lean(p_ready + 16 * t + 8 * part, p_phase[t], limit);
+                                wait_for(p_ready + 16 * t + 8 * part, p_phase[t], limit);
                                 tc_fence_after();
                                 if (elect_one()) {
                                     const uint64_t b = swizzled_desc(ring + v_slot * Shape::OPERAND, PT_HALF);

@@ -265,6 +265,26 @@ def test_items_with_one_tile_between_others(be, dev, hd):
         assert (np.abs(got[starts[s]:starts[s + 1], :2] - want) <= off + np.abs(want) * 2.0 ** -11 + 2.0 ** -25).all()
 
 
+def test_long_contexts_over_and_over(be, dev):
+    """Copies from cold memory land in any order: no role may take one phase of a ring slot for another (a wait that ran out shows as an error)."""
+    import torch
+
+    n, h_kv, hd, page = 90000, 8, 128, 64
+    pools = torch.randn((2, n // page + 1, h_kv, page, hd), device="cuda", dtype=torch.float16)
+    q = torch.randn((5, 40, hd), device="cuda", dtype=torch.float16)
+    out = torch.empty((8,) + tuple(q.shape), device="cuda", dtype=torch.float16)
+    table = torch.randperm(pools.shape[1], device="cuda").int()
+    start, n_kv = torch.tensor([0, 5], device="cuda", dtype=torch.int32), torch.tensor([n], device="cuda", dtype=torch.int32)
+    torch.cuda.synchronize()
+    c = B.paged_cache(pools[0].data_ptr(), pools[1].data_ptr(), pools.shape[1], page, h_kv, hd)
+    b = B.paged_batch(start.data_ptr(), n_kv.data_ptr(), table.data_ptr(), 1, 5, table.numel())
+    d = [B.paged_attention_desc(c, b, q.data_ptr(), o.data_ptr(), 40) for o in out]
+    for i in range(600):
+        be.paged_attention(d[i % 8])
+    be.sync()
+    assert all(torch.equal(o, out[0]) for o in out)
+
+
 def test_more_sequences_than_threads(be, dev):
     rng = np.random.default_rng(6)
     n = 700
