@@ -134,7 +134,8 @@ template <int HD, int MT> struct RowsSmem {       // the ring, and in its place 
     static constexpr int BYTES = MASKS + PR_WARPS * PR_STAGES * 4;
 };
 
-template <int HD, int MT>
+// IN_PAGE: a block's positions lie in one page (pages of a multiple of 16)
+template <int HD, int MT, bool IN_PAGE>
 __global__ void __launch_bounds__(PR_WARPS * 32) paged_rows_kernel(const __grid_constant__ PagedAttention p) {
     constexpr int TILE = 16 * MT, ROW = RowsShape<HD>::ROW, STAGE = RowsShape<HD>::STAGE, NT = PR_WARPS * 32;
     extern __shared__ __align__(128) uint8_t smem[];
@@ -158,25 +159,43 @@ __global__ void __launch_bounds__(PR_WARPS * 32) paged_rows_kernel(const __grid_
         const int32_t *table = p.view.page_table + (int64_t)seq * p.view.table_stride;
         const __half *kbase = p.k + head * p.view.head_stride, *vbase = p.v + head * p.view.head_stride;
 
-        auto page_of = [&](int b) {          // (lanes 0..15 and 16..31 alike) page of this lane's position in block b, or -1
-            const int j = ka + b * PR_BLOCK + (lane & 15);
-            return b < n_block && j < kb ? table[j / p.view.page_size] : -1;
+        auto page_of = [&](int b) {          // page of block b, or (lanes 0..15 and 16..31 alike) of this lane's position in it; -1: none
+            const int j = ka + b * PR_BLOCK + (IN_PAGE ? 0 : lane & 15);
+            return b < n_block && j < kb ? table[p.page_shift >= 0 ? j >> p.page_shift : j / p.view.page_size] : -1;
         };
         auto issue = [&](int b, int stage, int page) {
-            const int j = ka + b * PR_BLOCK + (lane & 15);
+            const int j = ka + b * PR_BLOCK + (IN_PAGE ? 0 : lane & 15);
             const bool ok = page >= 0 && page < p.view.n_pages;
-            const int64_t cell = ok ? page * p.view.page_stride + (j % p.view.page_size) * p.view.token_stride : 0;
-            const unsigned mask = __ballot_sync(0xffffffffu, ok) & 0xffffu;
+            const int in_page = p.page_shift >= 0 ? j & (p.view.page_size - 1) : j % p.view.page_size;
+            const int64_t cell = ok ? page * p.view.page_stride + in_page * p.view.token_stride : 0;
+            const unsigned mask = IN_PAGE ? (ok ? (kb - j >= PR_BLOCK ? 0xffffu : (1u << (kb - j)) - 1) : 0u) : __ballot_sync(0xffffffffu, ok) & 0xffffu;
             const uint32_t dst = ring + stage * STAGE;
             constexpr int PIECES = HD / 8;
+            if (IN_PAGE && 32 % PIECES == 0) {
+                constexpr int AT_ONCE = 32 / PIECES;
+                const int r0 = lane / PIECES, c = lane % PIECES;
+                int64_t o = cell + r0 * p.view.token_stride + c * 8;
+                const int64_t more = AT_ONCE * p.view.token_stride;
 #pragma unroll
-            for (int i = 0; i < PIECES / 2; ++i) {
-                const int x = i * 32 + lane, r = x / PIECES, c = x - r * PIECES;
-                const int64_t o = __shfl_sync(0xffffffffu, cell, r) + c * 8;
-                const bool in = (mask >> r) & 1;
-                const uint32_t d = dst + r * ROW + ((c ^ (r & 7)) << 4);
-                cp_async16(d, kbase + o, in);
-                cp_async16(d + PR_BLOCK * ROW, vbase + o, in);
+                for (int i = 0; i < PIECES / 2; ++i) {
+                    const int r = i * AT_ONCE + r0;
+                    const bool in = (mask >> r) & 1;
+                    const uint32_t d = dst + r * ROW + ((c ^ (r & 7)) << 4);
+                    const int64_t at = in ? o : 0;
+                    cp_async16(d, kbase + at, in);
+                    cp_async16(d + PR_BLOCK * ROW, vbase + at, in);
+                    o += more;
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < PIECES / 2; ++i) {
+                    const int x = i * 32 + lane, r = x / PIECES, c = x - r * PIECES;
+                    const bool in = (mask >> r) & 1;
+                    const int64_t row = IN_PAGE ? cell + r * p.view.token_stride : __shfl_sync(0xffffffffu, cell, r), o = in ? row + c * 8 : 0;
+                    const uint32_t d = dst + r * ROW + ((c ^ (r & 7)) << 4);
+                    cp_async16(d, kbase + o, in);
+                    cp_async16(d + PR_BLOCK * ROW, vbase + o, in);
+                }
             }
             if (lane == 0) { there[stage] = mask; }
             cp_commit();
@@ -208,10 +227,10 @@ __global__ void __launch_bounds__(PR_WARPS * 32) paged_rows_kernel(const __grid_
             }
         }
         const int pos_first = q.first + (int)((unsigned)(tile * TILE) / (unsigned)p.group), pos_last = q.first + (int)((unsigned)(tile * TILE + packed - 1) / (unsigned)p.group);
-        float o[MT][HD / 8][4], mx[MT][2], sum[MT][2];
+        float o[MT][HD / 8][4], mx[MT][2], sum[MT][2], base[MT][2], over[MT][2];   // (base: the maximum, or 0 for none; over: scores beyond it move the maximum)
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
-            mx[m][0] = mx[m][1] = -CUDART_INF_F; sum[m][0] = sum[m][1] = 0.f;
+            mx[m][0] = mx[m][1] = over[m][0] = over[m][1] = -CUDART_INF_F; sum[m][0] = sum[m][1] = base[m][0] = base[m][1] = 0.f;
 #pragma unroll
             for (int n = 0; n < HD / 8; ++n) { o[m][n][0] = o[m][n][1] = o[m][n][2] = o[m][n][3] = 0.f; }
         }
@@ -244,6 +263,7 @@ __global__ void __launch_bounds__(PR_WARPS * 32) paged_rows_kernel(const __grid_
 #pragma unroll
                 for (int m = 0; m < MT; ++m) { mma16816(sc[m][0], qf[m][ks], kf[0], kf[1]); mma16816(sc[m][1], qf[m][ks], kf[2], kf[3]); }
             }
+            // scores against the maximum, in powers of two
             bool above = false;
 #pragma unroll
             for (int m = 0; m < MT; ++m) {
@@ -252,13 +272,13 @@ __global__ void __launch_bounds__(PR_WARPS * 32) paged_rows_kernel(const __grid_
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         float &x = sc[m][n][e];
-                        x *= p.scale_log2;
+                        x = fmaf(x, p.scale_log2, -base[m][e >> 1]);
                         if (!whole) {
                             const int jj = n * 8 + (lane & 3) * 2 + (e & 1), d = pos[m][e >> 1] - (j0 + jj);
                             const bool seen = ((mask >> jj) & 1) && (!p.causal || (d >= 0 && (p.window <= 0 || d < p.window)));
                             x = seen ? x : -CUDART_INF_F;
                         }
-                        above |= x > mx[m][e >> 1] + 8.f;
+                        above |= x > over[m][e >> 1];
                     }
                 }
             }
@@ -270,8 +290,13 @@ __global__ void __launch_bounds__(PR_WARPS * 32) paged_rows_kernel(const __grid_
                         float v = fmaxf(fmaxf(sc[m][0][2 * hf], sc[m][0][2 * hf + 1]), fmaxf(sc[m][1][2 * hf], sc[m][1][2 * hf + 1]));
                         v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 1));
                         v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 2));
-                        const float to = fmaxf(mx[m][hf], v), f = to == mx[m][hf] ? 1.f : ex2(mx[m][hf] - to);   // (2^-inf = 0 at the first)
+                        const float to = fmaxf(mx[m][hf], base[m][hf] + v), f = to == mx[m][hf] ? 1.f : ex2(mx[m][hf] - to);   // (2^-inf = 0 at the first)
+                        const float from = base[m][hf];
                         mx[m][hf] = to; sum[m][hf] *= f;
+                        base[m][hf] = to == -CUDART_INF_F ? 0.f : to;
+                        over[m][hf] = to == -CUDART_INF_F ? to : 8.f;
+#pragma unroll
+                        for (int n = 0; n < 2; ++n) { sc[m][n][2 * hf] += from - base[m][hf]; sc[m][n][2 * hf + 1] += from - base[m][hf]; }
 #pragma unroll
                         for (int n = 0; n < HD / 8; ++n) { o[m][n][2 * hf] *= f; o[m][n][2 * hf + 1] *= f; }
                     }
@@ -282,15 +307,11 @@ __global__ void __launch_bounds__(PR_WARPS * 32) paged_rows_kernel(const __grid_
             for (int m = 0; m < MT; ++m) {
 #pragma unroll
                 for (int hf = 0; hf < 2; ++hf) {
-                    const float base = mx[m][hf] == -CUDART_INF_F ? 0.f : mx[m][hf];
 #pragma unroll
                     for (int n = 0; n < 2; ++n) {
-                        float a = ex2(sc[m][n][2 * hf] - base), c = ex2(sc[m][n][2 * hf + 1] - base);
-                        // what is summed is what is multiplied: the rounded probabilities, so that their errors cancel in the quotient's constant part
-                        const uint32_t h = pack2(a, c);
-                        const float2 back = __half22float2(*reinterpret_cast<const __half2 *>(&h));
-                        sum[m][hf] += back.x + back.y;
-                        pf[m][2 * n + hf] = h;
+                        const float a = ex2(sc[m][n][2 * hf]), c = ex2(sc[m][n][2 * hf + 1]);
+                        sum[m][hf] += a + c;
+                        pf[m][2 * n + hf] = pack2(a, c);
                     }
                 }
             }
@@ -428,12 +449,19 @@ __global__ void __launch_bounds__(PR_WARPS * 32) paged_rows_kernel(const __grid_
     }
 }
 
-template <int HD, int MT>
-cudaError_t launch_rows(const PagedAttention &p, int sms, const LaunchCfg &cfg) {
-    const void *kernel = reinterpret_cast<const void *>(paged_rows_kernel<HD, MT>);
+template <int HD, int MT, bool IN_PAGE>
+cudaError_t launch_rows_as(const PagedAttention &p, int sms, const LaunchCfg &cfg) {
+    const void *kernel = reinterpret_cast<const void *>(paged_rows_kernel<HD, MT, IN_PAGE>);
     const cudaError_t err = allow_dynamic_smem(kernel, (size_t)RowsSmem<HD, MT>::BYTES);
     if (err != cudaSuccess) { return err; }
-    return launch_maybe_pdl(paged_rows_kernel<HD, MT>, dim3(PA_MAX_CTAS_PER_SM * sms), PR_WARPS * 32, (size_t)RowsSmem<HD, MT>::BYTES, cfg.stream, cfg.pdl, p);
+    return launch_maybe_pdl(paged_rows_kernel<HD, MT, IN_PAGE>, dim3(PA_MAX_CTAS_PER_SM * sms), PR_WARPS * 32, (size_t)RowsSmem<HD, MT>::BYTES, cfg.stream, cfg.pdl, p);
+}
+template <int HD, int MT>
+cudaError_t launch_rows(PagedAttention p, int sms, const LaunchCfg &cfg) {
+    const int page = p.view.page_size;
+    p.page_shift = -1;
+    for (int s = 0; s < 31; ++s) { if (page == 1 << s) { p.page_shift = s; } }
+    return page % PR_BLOCK == 0 ? launch_rows_as<HD, MT, true>(p, sms, cfg) : launch_rows_as<HD, MT, false>(p, sms, cfg);
 }
 
 }  // namespace

@@ -29,6 +29,7 @@ struct PagedAttention {
     int          n_head_kv = 0, group = 1, causal = 1, window = 0, out_f32 = 0;
     float        scale_log2 = 0.f;        // scale * log2(e): probabilities are powers of two
     int          tile_rows = 16;          // rows of a tile, counting every query head of its K/V head
+    int          page_shift = -1;         // log2 of the page size, if it is a power of two
     int          few_rows = 0;            // sequences of up to so many rows (of all query heads of a K/V head) are the small kernel's
     float       *partial = nullptr;       // [CTAs][2][rows of a tile][head_dim + 2]
     unsigned    *arrived = nullptr;       // [CTAs], zero between launches
@@ -38,7 +39,7 @@ cudaError_t launch_paged_append(const PagedAppend &p, int in_type, int q_out_typ
 cudaError_t launch_paged_attention_rows(const PagedAttention &p, int head_dim, int row_tiles, int sms, const LaunchCfg &cfg);
 // the kernel on tensor memory; false where it does not take these pages, heads or strides (nothing is launched then)
 bool        launch_paged_attention_tc(const PagedAttention &p, int head_dim, int n_head, int sms, const LaunchCfg &cfg, uint64_t wait_limit, cudaError_t *err);
-constexpr int PA_FEW_ROWS = 32;          // sequences of up to so many rows (times query heads of a K/V head) are the small kernel's
+constexpr int PA_FEW_ROWS = 16;          // sequences of up to so many rows (times query heads of a K/V head) are the small kernel's
 constexpr int PA_MAX_CTAS_PER_SM = 2;
 
 // ---------------------------------------------------------------------------------------------- cutting the work
