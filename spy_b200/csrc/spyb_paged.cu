@@ -129,11 +129,10 @@ template <int HD> struct RowsShape {
     static constexpr int STAGE = 2 * PR_BLOCK * ROW;
     static constexpr int RING = PR_WARPS * PR_STAGES * STAGE;
 };
-template <int HD, int MT> struct RowsSmem {       // the ring, and in its place the warps' findings; the masks of the ring's stages
-    static constexpr int FOUND = PR_WARPS * 16 * MT * (HD + 2) * 4, MASKS = RowsShape<HD>::RING > FOUND ? RowsShape<HD>::RING : FOUND;
-    static constexpr int BYTES = MASKS + PR_WARPS * PR_STAGES * 4;
+template <int HD, int MT> struct RowsSmem {       // the ring; what the warps found: beside it for up to EARLY rows, in its place for more; the masks of the ring's stages
+    static constexpr int EARLY = MT == 1 ? 8 : 0, FOUND = PR_WARPS * 16 * MT * (HD + 2) * 4, RING = RowsShape<HD>::RING > FOUND ? RowsShape<HD>::RING : FOUND;
+    static constexpr int MASKS = RING + PR_WARPS * EARLY * (HD + 2) * 4, BYTES = MASKS + PR_WARPS * PR_STAGES * 4;
 };
-
 // IN_PAGE: a block's positions lie in one page (pages of a multiple of 16)
 template <int HD, int MT, bool IN_PAGE>
 __global__ void __launch_bounds__(PR_WARPS * 32) paged_rows_kernel(const __grid_constant__ PagedAttention p) {
@@ -150,15 +149,19 @@ __global__ void __launch_bounds__(PR_WARPS * 32) paged_rows_kernel(const __grid_
     if (at.unit >= at.end) { return; }
     PagedSeq q = paged_seq(p.view, at.seq);
     int seq = at.seq, head = at.head, tile = at.tile, off = at.off;
-    for (;;) {
-        const PagedItem it = paged_item<PR_UNIT, PR_BLOCK>(p, q, tile);
-        const int todo = (int)min((int64_t)(it.units - off), at.end - at.unit);
-        const int ka = it.lo + off * PR_UNIT, kb = min(it.hi, ka + todo * PR_UNIT);
-        const int n_block = kb > ka ? (kb - ka + PR_BLOCK - 1) / PR_BLOCK : 0;
-        const int packed = min(TILE, q.rows * p.group - tile * TILE);         // rows of this tile
-        const int32_t *table = p.view.page_table + (int64_t)seq * p.view.table_stride;
-        const __half *kbase = p.k + head * p.view.head_stride, *vbase = p.v + head * p.view.head_stride;
-
+    PagedItem it;
+    int todo, ka, kb, n_block, packed;        // of the item that comes next: units of this CTA, positions [ka, kb), blocks of them; rows of the tile
+    const int32_t *table;
+    const __half *kbase, *vbase;
+    auto describe = [&]() {
+        it = paged_item<PR_UNIT, PR_BLOCK>(p, q, tile);
+        todo = (int)min((int64_t)(it.units - off), at.end - at.unit);
+        ka = it.lo + off * PR_UNIT; kb = min(it.hi, ka + todo * PR_UNIT);
+        n_block = kb > ka ? (kb - ka + PR_BLOCK - 1) / PR_BLOCK : 0;
+        packed = min(TILE, q.rows * p.group - tile * TILE);
+        table = p.view.page_table + (int64_t)seq * p.view.table_stride;
+        kbase = p.k + head * p.view.head_stride; vbase = p.v + head * p.view.head_stride;
+    };
         auto page_of = [&](int b) {          // page of block b, or (lanes 0..15 and 16..31 alike) of this lane's position in it; -1: none
             const int j = ka + b * PR_BLOCK + (IN_PAGE ? 0 : lane & 15);
             return b < n_block && j < kb ? table[p.page_shift >= 0 ? j >> p.page_shift : j / p.view.page_size] : -1;
@@ -201,16 +204,17 @@ __global__ void __launch_bounds__(PR_WARPS * 32) paged_rows_kernel(const __grid_
             cp_commit();
         };
 
-        // the first blocks are on their way while Q comes
-        int page = page_of(warp);
+    int page = -1;                            // of the block that is issued next
+    uint32_t qf[MT][HD / 16][4];
+    int pos[MT][2];
+    auto start = [&]() {                      // the item's first blocks are on their way while its Q comes
+        page = page_of(warp);
 #pragma unroll
         for (int i = 0; i < PR_STAGES - 1; ++i) {
             const int next = page_of(warp + (i + 1) * PR_WARPS);
             if (warp + i * PR_WARPS < n_block) { issue(warp + i * PR_WARPS, i, page); } else { cp_commit(); }
             page = next;
         }
-        uint32_t qf[MT][HD / 16][4];
-        int pos[MT][2];
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
 #pragma unroll
@@ -226,6 +230,10 @@ __global__ void __launch_bounds__(PR_WARPS * 32) paged_rows_kernel(const __grid_
                 }
             }
         }
+    };
+    describe();
+    start();
+    for (;;) {
         const int pos_first = q.first + (int)((unsigned)(tile * TILE) / (unsigned)p.group), pos_last = q.first + (int)((unsigned)(tile * TILE + packed - 1) / (unsigned)p.group);
         float o[MT][HD / 8][4], mx[MT][2], sum[MT][2], base[MT][2], over[MT][2];   // (base: the maximum, or 0 for none; over: scores beyond it move the maximum)
 #pragma unroll
@@ -360,9 +368,18 @@ __global__ void __launch_bounds__(PR_WARPS * 32) paged_rows_kernel(const __grid_
             stage = stage == PR_STAGES - 1 ? 0 : stage + 1;
         }
         cp_wait<0>();
-        __syncthreads();
-        // the warps' findings side by side in shared memory, in place of the ring
-        float *mo = reinterpret_cast<float *>(smem), *mm = mo + PR_WARPS * TILE * HD, *ml = mm + PR_WARPS * TILE;
+        __syncwarp();
+        // What is known of this item; the next one's copies start before its findings are joined, where these have a place of their own
+        const int done = packed, done_tile = tile, done_row0 = q.row0, done_head = head;
+        const PagedCut cut = paged_cut(at, at.unit - off, it.units);
+        at.unit += todo;
+        off = 0;
+        const bool more = at.unit < at.end && paged_next(p, true, q, seq, head, tile), early = done <= RowsSmem<HD, MT>::EARLY;
+        if (more) { describe(); }
+        if (more && early) { start(); }
+        if (!early) { __syncthreads(); }
+        const int room = early ? RowsSmem<HD, MT>::EARLY : TILE;              // rows of a warp's findings
+        float *mo = reinterpret_cast<float *>(smem + (early ? RowsSmem<HD, MT>::RING : 0)), *mm = mo + PR_WARPS * room * HD, *ml = mm + PR_WARPS * room;
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
 #pragma unroll
@@ -371,38 +388,37 @@ __global__ void __launch_bounds__(PR_WARPS * 32) paged_rows_kernel(const __grid_
                 l += __shfl_xor_sync(0xffffffffu, l, 1);
                 l += __shfl_xor_sync(0xffffffffu, l, 2);
                 const int r = m * 16 + hf * 8 + (lane >> 2);
-                if (r < packed) {
-                    float *dst = mo + (warp * TILE + r) * HD + (lane & 3) * 2;
+                if (r < done) {
+                    float *dst = mo + (warp * room + r) * HD + (lane & 3) * 2;
 #pragma unroll
                     for (int n = 0; n < HD / 8; ++n) { *reinterpret_cast<float2 *>(dst + n * 8) = make_float2(o[m][n][2 * hf], o[m][n][2 * hf + 1]); }
-                    if ((lane & 3) == 0) { mm[warp * TILE + r] = mx[m][hf]; ml[warp * TILE + r] = l; }
+                    if ((lane & 3) == 0) { mm[warp * room + r] = mx[m][hf]; ml[warp * room + r] = l; }
                 }
             }
         }
         __syncthreads();
-        const PagedCut cut = paged_cut(at, at.unit - off, it.units);
         constexpr int PART = TILE * (HD + 2);
         float *part = p.partial + paged_slot(blockIdx.x, cut.c0) * PART;
         auto put = [&](int r, int c, float4 v) {   // four elements of a finished row
-            const int pr = tile * TILE + r, token = (int)((unsigned)pr / (unsigned)p.group), g = pr - token * p.group;
-            const int64_t o2 = (int64_t)(q.row0 + token) * p.out_stride + (head * p.group + g) * HD + c;
+            const int pr = done_tile * TILE + r, token = (int)((unsigned)pr / (unsigned)p.group), g = pr - token * p.group;
+            const int64_t o2 = (int64_t)(done_row0 + token) * p.out_stride + (done_head * p.group + g) * HD + c;
             const float w[4] = {v.x, v.y, v.z, v.w};
             if (p.out_f32) { store4(static_cast<float *>(p.out) + o2, w); } else { store4(static_cast<__half *>(p.out) + o2, w); }
         };
-        for (int x = tid; x < packed * (HD / 4); x += NT) {
+        for (int x = tid; x < done * (HD / 4); x += NT) {
             const int r = x / (HD / 4), c = (x - r * (HD / 4)) * 4;
             float m = -CUDART_INF_F;
 #pragma unroll
-            for (int w = 0; w < PR_WARPS; ++w) { m = fmaxf(m, mm[w * TILE + r]); }
+            for (int w = 0; w < PR_WARPS; ++w) { m = fmaxf(m, mm[w * room + r]); }
             const float base = m == -CUDART_INF_F ? 0.f : m;
             float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
             float l = 0.f;
 #pragma unroll
             for (int w = 0; w < PR_WARPS; ++w) {
-                const float f = ex2(mm[w * TILE + r] - base);
-                const float4 u = *reinterpret_cast<const float4 *>(mo + (w * TILE + r) * HD + c);
+                const float f = ex2(mm[w * room + r] - base);
+                const float4 u = *reinterpret_cast<const float4 *>(mo + (w * room + r) * HD + c);
                 v.x += f * u.x; v.y += f * u.y; v.z += f * u.z; v.w += f * u.w;
-                l += f * ml[w * TILE + r];
+                l += f * ml[w * room + r];
             }
             if (cut.parts == 1) {
                 const float inv = l == 0.f ? 0.f : 1.f / l;
@@ -422,7 +438,7 @@ __global__ void __launch_bounds__(PR_WARPS * 32) paged_rows_kernel(const __grid_
             }
             __syncthreads();
             if (last_one) {
-                for (int x = tid; x < packed * (HD / 4); x += NT) {
+                for (int x = tid; x < done * (HD / 4); x += NT) {
                     const int r = x / (HD / 4), c = (x - r * (HD / 4)) * 4;
                     float m = -CUDART_INF_F, l = 0.f;
                     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -441,11 +457,9 @@ __global__ void __launch_bounds__(PR_WARPS * 32) paged_rows_kernel(const __grid_
                 }
             }
         }
-        at.unit += todo;
-        if (at.unit >= at.end) { return; }
-        off = 0;
-        if (!paged_next(p, true, q, seq, head, tile)) { return; }
-        __syncthreads();   // (the ring takes the findings' place again)
+        if (!more) { return; }
+        __syncthreads();                      // (the findings' place is free again)
+        if (!early) { start(); }
     }
 }
 
