@@ -104,7 +104,7 @@ __global__ void __launch_bounds__(AP_THREADS) paged_append_kernel(const __grid_c
 // asynchronous copies, scores and values by mma.sync on up to 32 rows, a running maximum and sum in registers - and the warps of a CTA, then the CTAs
 // of an item are joined at the end. The maximum that probabilities are taken against follows the true one only when that is 2^8 above it: the
 // accumulators are hardly ever rescaled, and p <= 2^8 is as exact in fp16 as p <= 1.
-constexpr int PR_WARPS = 4, PR_STAGES = 3, PR_BLOCK = 16, PR_UNIT = PR_WARPS * PR_BLOCK;
+constexpr int PR_WARPS = 4, PR_BLOCK = 16, PR_UNIT = PR_WARPS * PR_BLOCK;
 
 __device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
@@ -127,16 +127,17 @@ __device__ __forceinline__ bool not_finite2(uint32_t h2) { return (h2 & 0x7c00u)
 template <int HD> struct RowsShape {
     static constexpr int ROW = HD <= 64 ? 128 : 256;                 // bytes of a position in shared memory (16-byte pieces swizzled within eight)
     static constexpr int STAGE = 2 * PR_BLOCK * ROW;
-    static constexpr int RING = PR_WARPS * PR_STAGES * STAGE;
+    static constexpr int STAGES = 3 * 256 / ROW;                     // (as many bytes on their way for short positions as for long ones)
+    static constexpr int RING = PR_WARPS * STAGES * STAGE;
 };
 template <int HD, int MT> struct RowsSmem {       // the ring; what the warps found: beside it for up to EARLY rows, in its place for more; the masks of the ring's stages
     static constexpr int EARLY = MT == 1 ? 8 : 0, FOUND = PR_WARPS * 16 * MT * (HD + 2) * 4, RING = RowsShape<HD>::RING > FOUND ? RowsShape<HD>::RING : FOUND;
-    static constexpr int MASKS = RING + PR_WARPS * EARLY * (HD + 2) * 4, BYTES = MASKS + PR_WARPS * PR_STAGES * 4;
+    static constexpr int MASKS = RING + PR_WARPS * EARLY * (HD + 2) * 4, BYTES = MASKS + PR_WARPS * RowsShape<HD>::STAGES * 4;
 };
 // IN_PAGE: a block's positions lie in one page (pages of a multiple of 16)
 template <int HD, int MT, bool IN_PAGE>
 __global__ void __launch_bounds__(PR_WARPS * 32) paged_rows_kernel(const __grid_constant__ PagedAttention p) {
-    constexpr int TILE = 16 * MT, ROW = RowsShape<HD>::ROW, STAGE = RowsShape<HD>::STAGE, NT = PR_WARPS * 32;
+    constexpr int PR_STAGES = RowsShape<HD>::STAGES, TILE = 16 * MT, ROW = RowsShape<HD>::ROW, STAGE = RowsShape<HD>::STAGE, NT = PR_WARPS * 32;
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ PagedPlanShared plan;
     __shared__ int last_one;
