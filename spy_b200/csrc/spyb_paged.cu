@@ -205,14 +205,24 @@ __global__ void __launch_bounds__(PR_WARPS * 32) paged_rows_kernel(const __grid_
             cp_commit();
         };
 
-    int page = -1;                            // of the block that is issued next
+    // Pages of blocks inside one: a lane's is that of every 32nd block of this warp, the next 32 are read while these are in use; a block's is told by its lane
+    int page = -1, ids = -1, ids_next = -1, issued = 0;   // (page: of the block that is issued next)
+    auto next_page = [&](int b) {             // of block b, the `issued`-th of this warp
+        if (!IN_PAGE) { return page_of(b); }
+        const int l = issued & 31;
+        if (l == 0) { ids = ids_next; ids_next = page_of(warp + (issued + 32 + lane) * PR_WARPS); }
+        ++issued;
+        return __shfl_sync(0xffffffffu, ids, l);
+    };
     uint32_t qf[MT][HD / 16][4];
     int pos[MT][2];
     auto start = [&]() {                      // the item's first blocks are on their way while its Q comes
-        page = page_of(warp);
+        issued = 0;
+        if (IN_PAGE) { ids_next = page_of(warp + lane * PR_WARPS); }
+        page = next_page(warp);
 #pragma unroll
         for (int i = 0; i < PR_STAGES - 1; ++i) {
-            const int next = page_of(warp + (i + 1) * PR_WARPS);
+            const int next = next_page(warp + (i + 1) * PR_WARPS);
             if (warp + i * PR_WARPS < n_block) { issue(warp + i * PR_WARPS, i, page); } else { cp_commit(); }
             page = next;
         }
@@ -246,7 +256,7 @@ __global__ void __launch_bounds__(PR_WARPS * 32) paged_rows_kernel(const __grid_
         int stage = 0;
         for (int b = warp; b < n_block; b += PR_WARPS) {
             {
-                const int ahead = b + (PR_STAGES - 1) * PR_WARPS, next = page_of(ahead + PR_WARPS);
+                const int ahead = b + (PR_STAGES - 1) * PR_WARPS, next = next_page(ahead + PR_WARPS);
                 const int to = stage == 0 ? PR_STAGES - 1 : stage - 1;
                 __syncwarp();
                 if (ahead < n_block) { issue(ahead, to, page); } else { cp_commit(); }
