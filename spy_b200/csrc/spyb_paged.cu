@@ -127,11 +127,12 @@ __device__ __forceinline__ bool not_finite2(uint32_t h2) { return (h2 & 0x7c00u)
 template <int HD> struct RowsShape {
     static constexpr int ROW = HD <= 64 ? 128 : 256;                 // bytes of a position in shared memory (16-byte pieces swizzled within eight)
     static constexpr int STAGE = 2 * PR_BLOCK * ROW;
-    static constexpr int STAGES = 3 * 256 / ROW;                     // (as many bytes on their way for short positions as for long ones)
+    static constexpr int STAGES = ROW == 128 ? 4 : 3;                // (short positions: three CTAs an SM; a warp's time a block is what their instructions wait for one another)
     static constexpr int RING = PR_WARPS * STAGES * STAGE;
 };
 template <int HD, int MT> struct RowsSmem {       // the ring; what the warps found: beside it for up to EARLY rows, in its place for more; the masks of the ring's stages
     static constexpr int EARLY = MT == 1 ? 8 : 0, FOUND = PR_WARPS * 16 * MT * (HD + 2) * 4, RING = RowsShape<HD>::RING > FOUND ? RowsShape<HD>::RING : FOUND;
+    static constexpr int CTAS = MT == 1 && HD <= 64 ? 3 : 2;         // of an SM
     static constexpr int MASKS = RING + PR_WARPS * EARLY * (HD + 2) * 4, BYTES = MASKS + PR_WARPS * RowsShape<HD>::STAGES * 4;
 };
 // IN_PAGE: a block's positions lie in one page (pages of a multiple of 16)
@@ -205,10 +206,12 @@ __global__ void __launch_bounds__(PR_WARPS * 32) paged_rows_kernel(const __grid_
             cp_commit();
         };
 
-    // Pages of blocks inside one: a lane's is that of every 32nd block of this warp, the next 32 are read while these are in use; a block's is told by its lane
+    // Short positions in one page: a lane has the page of every 32nd block of this warp, the next 32 are read while these are in use; a block's is told by its lane. (Long
+    // positions' blocks take longer than the table's latency: one page ahead, 64 single tokens 103.0 us against 104.5.)
+    constexpr bool BATCH = IN_PAGE && HD <= 64;
     int page = -1, ids = -1, ids_next = -1, issued = 0;   // (page: of the block that is issued next)
     auto next_page = [&](int b) {             // of block b, the `issued`-th of this warp
-        if (!IN_PAGE) { return page_of(b); }
+        if (!BATCH) { return page_of(b); }
         const int l = issued & 31;
         if (l == 0) { ids = ids_next; ids_next = page_of(warp + (issued + 32 + lane) * PR_WARPS); }
         ++issued;
@@ -218,7 +221,7 @@ __global__ void __launch_bounds__(PR_WARPS * 32) paged_rows_kernel(const __grid_
     int pos[MT][2];
     auto start = [&]() {                      // the item's first blocks are on their way while its Q comes
         issued = 0;
-        if (IN_PAGE) { ids_next = page_of(warp + lane * PR_WARPS); }
+        if (BATCH) { ids_next = page_of(warp + lane * PR_WARPS); }
         page = next_page(warp);
 #pragma unroll
         for (int i = 0; i < PR_STAGES - 1; ++i) {
@@ -479,7 +482,7 @@ cudaError_t launch_rows_as(const PagedAttention &p, int sms, const LaunchCfg &cf
     const void *kernel = reinterpret_cast<const void *>(paged_rows_kernel<HD, MT, IN_PAGE>);
     const cudaError_t err = allow_dynamic_smem(kernel, (size_t)RowsSmem<HD, MT>::BYTES);
     if (err != cudaSuccess) { return err; }
-    return launch_maybe_pdl(paged_rows_kernel<HD, MT, IN_PAGE>, dim3(PA_MAX_CTAS_PER_SM * sms), PR_WARPS * 32, (size_t)RowsSmem<HD, MT>::BYTES, cfg.stream, cfg.pdl, p);
+    return launch_maybe_pdl(paged_rows_kernel<HD, MT, IN_PAGE>, dim3(RowsSmem<HD, MT>::CTAS * sms), PR_WARPS * 32, (size_t)RowsSmem<HD, MT>::BYTES, cfg.stream, cfg.pdl, p);
 }
 template <int HD, int MT>
 cudaError_t launch_rows(PagedAttention p, int sms, const LaunchCfg &cfg) {

@@ -40,7 +40,6 @@ cudaError_t launch_paged_attention_rows(const PagedAttention &p, int head_dim, i
 // the kernel on tensor memory; false where it does not take these pages, heads or strides (nothing is launched then)
 bool        launch_paged_attention_tc(const PagedAttention &p, int head_dim, int n_head, int sms, const LaunchCfg &cfg, uint64_t wait_limit, cudaError_t *err);
 constexpr int PA_FEW_ROWS = 16;          // sequences of up to so many rows (times query heads of a K/V head) are the small kernel's
-constexpr int PA_MAX_CTAS_PER_SM = 2;
 
 // ---------------------------------------------------------------------------------------------- cutting the work
 // The rows of a sequence that share a K/V head - token by token, its query heads side by side - are cut into tiles; a tile and a K/V head are an item, and the
