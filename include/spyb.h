@@ -395,6 +395,19 @@ spyb_status spyb_model_set_sequences(spyb_model *model, int32_t n_seq);
 spyb_status spyb_model_select_sequence(spyb_model *model, int32_t seq);
 spyb_status spyb_model_decode_batch(spyb_model *model, const int32_t *first_tokens, int32_t n_seq, int32_t n_past, int32_t n_steps,
                                     int32_t *ids_host, float *logits_host);
+/* spyb_model_decode and spyb_model_decode_batch with drawn tokens in place of the largest logits': each step's ids are spyb_sample's on the step's logits with
+ * these settings (host arrays, read during the call; temperature, top_k, top_p and min_p have one value a sequence, `uniform` one a step and sequence,
+ * [n_steps][n_seq]; NULL leaves a setting out, a missing `uniform` reads as zeros). temperature 0 gives spyb_model_decode's ids. Where a row of logits leaves
+ * nothing to draw the id is -1 and the sequence goes on with token 0. Vocabularies of up to 2^20 tokens; the same on every rank of a sharded model. */
+typedef struct {
+    const float   *temperature;
+    const int32_t *top_k;
+    const float   *top_p, *min_p, *uniform;
+} spyb_sampling;
+spyb_status spyb_model_decode_sampled(spyb_model *model, int32_t first_token, int32_t n_past, int32_t n_steps, const spyb_sampling *sampling,
+                                      int32_t *ids_host, float *logits_host);
+spyb_status spyb_model_decode_batch_sampled(spyb_model *model, const int32_t *first_tokens, int32_t n_seq, int32_t n_past, int32_t n_steps,
+                                            const spyb_sampling *sampling, int32_t *ids_host, float *logits_host);
 /* device time in milliseconds of the most recent spyb_model_decode / spyb_model_eval call,
  * measured with CUDA events on the backend's stream; number of kernels that call launched */
 float   spyb_model_last_ms(const spyb_model *model);

@@ -87,6 +87,10 @@ class SampleDesc(C.Structure):
                 ("temperature", C.c_void_p), ("top_k", C.c_void_p), ("top_p", C.c_void_p), ("min_p", C.c_void_p), ("uniform", C.c_void_p), ("ids", C.c_void_p), ("probs", C.c_void_p)]
 
 
+class Sampling(C.Structure):
+    _fields_ = [("temperature", C.c_void_p), ("top_k", C.c_void_p), ("top_p", C.c_void_p), ("min_p", C.c_void_p), ("uniform", C.c_void_p)]
+
+
 CALLBACK = C.CFUNCTYPE(None, C.c_void_p)
 
 _lib = None
@@ -138,6 +142,8 @@ def lib():
         "spyb_model_set_sequences": (i32, [vp, i32]),
         "spyb_model_select_sequence": (i32, [vp, i32]),
         "spyb_model_decode_batch": (i32, [vp, vp, i32, i32, i32, vp, vp]),
+        "spyb_model_decode_sampled": (i32, [vp, i32, i32, i32, C.POINTER(Sampling), vp, vp]),
+        "spyb_model_decode_batch_sampled": (i32, [vp, vp, i32, i32, i32, C.POINTER(Sampling), vp, vp]),
         "spyb_model_last_ms": (C.c_float, [vp]),
         "spyb_model_last_launches": (i64, [vp]),
         "spyb_model_tap_xq": (i32, [vp, vp]),
@@ -507,6 +513,33 @@ class LlamaModel:
         logits = np.empty((n_steps, n_seq, self.info.n_vocab), dtype=np.float32) if want_logits else None
         self.backend._check(self._l.spyb_model_decode_batch(self.h, _np_ptr(first), n_seq, n_past, n_steps, _np_ptr(ids),
                                                             _np_ptr(logits) if want_logits else None))
+        return ids, logits
+
+    @staticmethod
+    def _sampling(n_steps: int, n_seq: int, uniform, temperature, top_k, top_p, min_p):
+        def row(a, dtype, shape):
+            return None if a is None else np.ascontiguousarray(np.broadcast_to(np.asarray(a, dtype=dtype), shape))
+        arrays = (row(temperature, np.float32, (n_seq,)), row(top_k, np.int32, (n_seq,)), row(top_p, np.float32, (n_seq,)), row(min_p, np.float32, (n_seq,)),
+                  row(uniform, np.float32, (n_steps, n_seq)))
+        return Sampling(*(None if a is None else _np_ptr(a) for a in arrays)), arrays
+
+    def decode_sampled(self, first_token: int, n_past: int, n_steps: int, uniform=None, temperature=None, top_k=None, top_p=None, min_p=None, want_logits: bool = False):
+        """decode with drawn tokens: uniform holds one number in [0, 1) a step, the settings are scalars (None leaves one out); returns (ids, logits or None)."""
+        how, keep = self._sampling(n_steps, 1, None if uniform is None else np.reshape(uniform, (n_steps, 1)), temperature, top_k, top_p, min_p)
+        ids = np.zeros(n_steps, dtype=np.int32)
+        logits = np.empty((n_steps, self.info.n_vocab), dtype=np.float32) if want_logits else None
+        self.backend._check(self._l.spyb_model_decode_sampled(self.h, int(first_token), n_past, n_steps, C.byref(how), _np_ptr(ids), _np_ptr(logits) if want_logits else None))
+        return ids, logits
+
+    def decode_batch_sampled(self, first_tokens, n_past: int, n_steps: int, uniform=None, temperature=None, top_k=None, top_p=None, min_p=None, want_logits: bool = False):
+        """decode_batch with drawn tokens: uniform [n_steps, n_seq] in [0, 1), settings as scalars or one a sequence (None leaves one out)."""
+        first = np.ascontiguousarray(first_tokens, dtype=np.int32)
+        n_seq = len(first)
+        how, keep = self._sampling(n_steps, n_seq, uniform, temperature, top_k, top_p, min_p)
+        ids = np.zeros((n_steps, n_seq), dtype=np.int32)
+        logits = np.empty((n_steps, n_seq, self.info.n_vocab), dtype=np.float32) if want_logits else None
+        self.backend._check(self._l.spyb_model_decode_batch_sampled(self.h, _np_ptr(first), n_seq, n_past, n_steps, C.byref(how), _np_ptr(ids),
+                                                                    _np_ptr(logits) if want_logits else None))
         return ids, logits
 
     def generate(self, prompt, n_predict: int, want_logits: bool = True):

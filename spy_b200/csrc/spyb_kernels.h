@@ -277,6 +277,7 @@ cudaError_t launch_argmax_embed_batch(const float *logits, int64_t n_vocab, int 
                                       int64_t d_model, float *x_out, int64_t x_stride, int *pos_counter, cudaStream_t s);
 cudaError_t launch_argmax_embed(const float *logits, int64_t n_vocab, int32_t *token_out, int32_t *history, int *pos_counter,
                                 const uint8_t *embd, int embd_type, int64_t d_model, float *x_out, const LaunchCfg &cfg);
+cudaError_t launch_take_tokens(const int32_t *ids, int32_t *tokens, int n, int *pos_counter, cudaStream_t s);
 cudaError_t launch_embed(const int32_t *ids, int n_ids, const uint8_t *embd, int embd_type, int64_t d_model, float *x_out, cudaStream_t s);
 
 // ---- one decode step as a single persistent kernel (spyb_step.cu)

@@ -214,6 +214,9 @@ struct spyb_model {
     float   *logits_batch = nullptr;
     int32_t *batch_tokens = nullptr, *batch_ids = nullptr;
     int64_t  batch_ids_cap = 0;
+    // settings, uniform numbers and ids of sampled steps, four bytes each
+    uint32_t *sampling = nullptr;
+    int64_t  sampling_cap = 0;
     // Captured steps: a captured step holds the cache addresses of its sequence and the attention kernel of its form. The least recently used
     // goes when there are MAX_STEP_GRAPHS.
     struct StepGraph { cudaGraphExec_t exec; int kind, seq, form; int64_t launches; uint64_t used; };
@@ -707,6 +710,52 @@ spyb_status run_decode_step(spyb_model *m, int64_t *launches) {
     ++*launches;
     return SPYB_SUCCESS;
 }
+
+// Steps whose tokens are drawn (spyb_sampling): the sampler's descriptor of step 0, whose uniform numbers and ids are n_seq words behind the last step's.
+// The caller's host arrays are read before this returns.
+spyb_status prepare_sampling(spyb_model *m, const spyb_sampling &how, const float *logits, int n_seq, int n_steps, spyb_sample_desc *d) {
+    spyb_backend *be = m->be;
+    *d = {};
+    d->number_type = SPYB_FP32; d->n_rows = n_seq; d->n_vocab = m->info.n_vocab; d->row_stride = m->info.n_vocab; d->logits = logits;
+    const int64_t each = n_seq, all = (int64_t)n_seq * n_steps, need = 4 * each + 2 * all;
+    if (need > m->sampling_cap) {
+        if (dev_alloc(m, &m->sampling, (size_t)need) != SPYB_SUCCESS) { return SPYB_FAIL; }
+        m->sampling_cap = need;
+    }
+    uint32_t *next = m->sampling;
+    cudaError_t err = cudaSuccess;
+    auto take = [&](const void *host, int64_t n) -> const void * {
+        uint32_t *at = next;
+        next += n;
+        if (host == nullptr) { return nullptr; }
+        if (err == cudaSuccess) { err = cudaMemcpyAsync(at, host, (size_t)n * 4, cudaMemcpyHostToDevice, be->stream); }
+        return at;
+    };
+    d->temperature = static_cast<const float *>(take(how.temperature, each));
+    d->top_k       = static_cast<const int32_t *>(take(how.top_k, each));
+    d->top_p       = static_cast<const float *>(take(how.top_p, each));
+    d->min_p       = static_cast<const float *>(take(how.min_p, each));
+    d->uniform     = static_cast<const float *>(take(how.uniform, all));
+    d->ids         = reinterpret_cast<int32_t *>(next);
+    SPYB_CUDA(be, err);
+    SPYB_CUDA(be, cudaStreamSynchronize(be->stream));
+    char why[128];
+    if (spyb_sample_check(d, why, sizeof why) != SPYB_SUCCESS) { be->set_error("%s", why); return SPYB_UNSUPPORTED; }
+    return SPYB_SUCCESS;
+}
+// The step's ids from its logits, and the tokens that the next one starts from; d is the next step's then.
+spyb_status sample_step(spyb_model *m, spyb_sample_desc *d, int32_t *tokens, int *pos_counter, int64_t *launches) {
+    if (spyb_sample(m->be, d) != SPYB_SUCCESS) { return SPYB_FAIL; }
+    SPYB_CUDA(m->be, launch_take_tokens(d->ids, tokens, d->n_rows, pos_counter, m->be->stream));
+    *launches += 2;
+    d->ids += d->n_rows;
+    if (d->uniform != nullptr) { d->uniform += d->n_rows; }
+    return SPYB_SUCCESS;
+}
+
+spyb_status decode(spyb_model *m, int32_t first_token, int32_t n_past, int32_t n_steps, const spyb_sampling *how, int32_t *ids_host, float *logits_host);
+spyb_status decode_batch(spyb_model *m, const int32_t *first_tokens, int32_t n_seq, int32_t n_past, int32_t n_steps, const spyb_sampling *how, int32_t *ids_host,
+                         float *logits_host);
 
 }  // namespace
 
@@ -1253,46 +1302,11 @@ spyb_status spyb_model_eval(spyb_model *m, const int32_t *tokens, int32_t n_toke
 }
 
 spyb_status spyb_model_decode(spyb_model *m, int32_t first_token, int32_t n_past, int32_t n_steps, int32_t *ids_host, float *logits_host) {
-    if (m == nullptr || n_steps < 1 || ids_host == nullptr) { return SPYB_FAIL; }
-    spyb_backend *be = m->be;
-    cudaSetDevice(be->config.device_id);
-    if (n_past < 0 || n_past + n_steps > m->info.n_ctx) { be->set_error("decode would exceed the context length (%d + %d > %d)", n_past, n_steps, m->info.n_ctx); return SPYB_FAIL; }
-    if (first_token < 0 || first_token >= m->info.n_vocab) { be->set_error("token id %d out of range", first_token); return SPYB_FAIL; }
-    m->h_pos_pinned[0] = n_past; m->h_pos_pinned[1] = 0; *m->h_tok_pinned = first_token;   // [1] = 0: rows end at the token itself
-    m->h_pos_pinned[2] = ++m->epoch;   // the argmax kernel advances the device copy once per step
-    m->epoch += n_steps - 1;
-    SPYB_CUDA(be, cudaMemcpyAsync(m->d_pos, m->h_pos_pinned, 12, cudaMemcpyHostToDevice, be->stream));
-    SPYB_CUDA(be, cudaMemcpyAsync(m->d_tokens_in, m->h_tok_pinned, 4, cudaMemcpyHostToDevice, be->stream));
-    SPYB_CUDA(be, launch_embed(m->d_tokens_in, 1, m->embd, m->embd_type, m->info.d_model, m->x, be->stream));
+    return decode(m, first_token, n_past, n_steps, nullptr, ids_host, logits_host);
+}
 
-    const bool use_graph = be->config.use_graph != 0 && (m->info.tp_size == 1 || std::getenv("SPYB_TP_NO_GRAPH") == nullptr);   // the all-reduces of the prompt pass have warmed NCCL up before the capture
-    // one decode step captured once per sequence and form of the attention, when the first step of that form comes (a capture leaves the steps in
-    // front of it running); positions and the token live in device memory, so the same graph replays for every later step
-    auto step_at = [&](int pos) {
-        m->att_form = step_form(m, pos);
-        return use_graph ? captured_step(m, GRAPH_DECODE, [&](int64_t *n) { return run_decode_step(m, n); }) : nullptr;
-    };
-    if (step_at(n_past) == nullptr && use_graph) { return SPYB_FAIL; }
-    int64_t per_step = m->step_ok ? 2 : (int64_t)m->layers.size() * 5 + 2;
-    SPYB_CUDA(be, cudaEventRecord(m->ev0, be->stream));
-    for (int s = 0; s < n_steps; ++s) {
-        const spyb_model::StepGraph *step = step_at(n_past + s);
-        if (step == nullptr && use_graph) { cudaStreamSynchronize(be->stream); return SPYB_FAIL; }
-        if (use_graph) { SPYB_CUDA(be, cudaGraphLaunch(step->exec, be->stream)); }
-        else { int64_t n = 0; if (run_decode_step(m, &n) != SPYB_SUCCESS) { return SPYB_FAIL; } per_step = n; }
-        if (logits_host != nullptr) {
-            // parity mode: logits of every step come back (argmax_embed does not modify them)
-            SPYB_CUDA(be, cudaMemcpyAsync(logits_host + (size_t)s * m->info.n_vocab, m->logits, (size_t)m->info.n_vocab * 4, cudaMemcpyDeviceToHost, be->stream));
-            SPYB_CUDA(be, cudaStreamSynchronize(be->stream));
-        }
-    }
-    SPYB_CUDA(be, cudaEventRecord(m->ev1, be->stream));
-    SPYB_CUDA(be, cudaMemcpyAsync(ids_host, m->d_history + n_past, (size_t)n_steps * 4, cudaMemcpyDeviceToHost, be->stream));
-    SPYB_CUDA(be, cudaStreamSynchronize(be->stream));
-    if (be->device_error()) { return SPYB_FAIL; }
-    SPYB_CUDA(be, cudaEventElapsedTime(&m->last_ms, m->ev0, m->ev1));
-    m->last_launches = per_step * n_steps;
-    return SPYB_SUCCESS;
+spyb_status spyb_model_decode_sampled(spyb_model *m, int32_t first_token, int32_t n_past, int32_t n_steps, const spyb_sampling *how, int32_t *ids_host, float *logits_host) {
+    return how == nullptr ? SPYB_FAIL : decode(m, first_token, n_past, n_steps, how, ids_host, logits_host);
 }
 
 #ifndef SPYB_NO_MEASUREMENT_AIDS
@@ -1422,6 +1436,114 @@ spyb_status spyb_model_select_sequence(spyb_model *m, int32_t seq) {
 
 spyb_status spyb_model_decode_batch(spyb_model *m, const int32_t *first_tokens, int32_t n_seq, int32_t n_past, int32_t n_steps, int32_t *ids_host,
                                     float *logits_host) {
+    return decode_batch(m, first_tokens, n_seq, n_past, n_steps, nullptr, ids_host, logits_host);
+}
+
+spyb_status spyb_model_decode_batch_sampled(spyb_model *m, const int32_t *first_tokens, int32_t n_seq, int32_t n_past, int32_t n_steps, const spyb_sampling *how,
+                                            int32_t *ids_host, float *logits_host) {
+    return how == nullptr ? SPYB_FAIL : decode_batch(m, first_tokens, n_seq, n_past, n_steps, how, ids_host, logits_host);
+}
+
+float   spyb_model_last_ms(const spyb_model *m) { return m ? m->last_ms : 0.f; }
+int64_t spyb_model_last_launches(const spyb_model *m) { return m ? m->last_launches : 0; }
+
+spyb_status spyb_model_read_activation(spyb_model *m, int32_t which, void *host, uint64_t bytes) {
+    if (m == nullptr || host == nullptr) { return SPYB_FAIL; }
+    const void *src = nullptr; uint64_t avail = 0;
+    switch (which) {
+    case 0: src = m->q;      avail = (uint64_t)8 * m->dl * 2; break;
+    case 1: src = m->att;    avail = (uint64_t)8 * m->info.d_model * 4; break;
+    case 2: src = m->x;      avail = (uint64_t)8 * m->info.d_model * 4; break;
+    case 3: src = m->act;    avail = (uint64_t)8 * m->info.n_ff * 4; break;
+    case 4: src = m->logits; avail = (uint64_t)m->info.n_vocab * 4; break;
+    default: m->be->set_error("read_activation: unknown buffer %d", which); return SPYB_FAIL;
+    }
+    if (bytes > avail) { m->be->set_error("read_activation: %llu bytes requested, %llu available", (unsigned long long)bytes, (unsigned long long)avail); return SPYB_FAIL; }
+    SPYB_CUDA(m->be, cudaStreamSynchronize(m->be->stream));
+    SPYB_CUDA(m->be, cudaMemcpy(host, src, bytes, cudaMemcpyDeviceToHost));
+    return SPYB_SUCCESS;
+}
+
+#ifndef SPYB_NO_MEASUREMENT_AIDS
+int32_t spyb_model_read_timeline(spyb_model *m, uint64_t *stamps_host, int32_t max_kernels) {
+    if (m == nullptr || m->d_stamps == nullptr || stamps_host == nullptr) { return 0; }
+    const int n = std::min<int>(max_kernels, 5 * (int)m->layers.size() + 1);
+    if (cudaMemcpy(stamps_host, m->d_stamps, (size_t)n * 8 * sizeof(uint64_t), cudaMemcpyDeviceToHost) != cudaSuccess) { return 0; }
+    return n;
+}
+
+int32_t spyb_model_read_step_timeline(spyb_model *m, uint64_t *stamps_host, int32_t max_points) {
+    if (m == nullptr || m->d_step_stamps == nullptr || stamps_host == nullptr) { return 0; }
+    const int n = std::min<int>(max_points, m->step_stamp_count);
+    if (cudaMemcpy(stamps_host, m->d_step_stamps, (size_t)n * 2 * sizeof(uint64_t), cudaMemcpyDeviceToHost) != cudaSuccess) { return 0; }
+    return n;
+}
+#endif
+
+spyb_status spyb_model_tap_xq(spyb_model *m, void *blocks_host) {
+    if (m == nullptr || blocks_host == nullptr) { return SPYB_FAIL; }
+    SPYB_CUDA(m->be, cudaMemcpy(blocks_host, m->d_tap, (size_t)m->info.d_model / 32 * 34, cudaMemcpyDeviceToHost));
+    return SPYB_SUCCESS;
+}
+
+}  // extern "C"
+
+namespace {
+spyb_status decode(spyb_model *m, int32_t first_token, int32_t n_past, int32_t n_steps, const spyb_sampling *how, int32_t *ids_host, float *logits_host) {
+    if (m == nullptr || n_steps < 1 || ids_host == nullptr) { return SPYB_FAIL; }
+    spyb_backend *be = m->be;
+    cudaSetDevice(be->config.device_id);
+    if (n_past < 0 || n_past + n_steps > m->info.n_ctx) { be->set_error("decode would exceed the context length (%d + %d > %d)", n_past, n_steps, m->info.n_ctx); return SPYB_FAIL; }
+    if (first_token < 0 || first_token >= m->info.n_vocab) { be->set_error("token id %d out of range", first_token); return SPYB_FAIL; }
+    spyb_sample_desc draw;
+    if (how != nullptr) {
+        const spyb_status st = prepare_sampling(m, *how, m->logits, 1, n_steps, &draw);
+        if (st != SPYB_SUCCESS) { return st; }
+    }
+    const int32_t *drawn = how != nullptr ? draw.ids : nullptr;
+    m->h_pos_pinned[0] = n_past; m->h_pos_pinned[1] = 0; *m->h_tok_pinned = first_token;   // [1] = 0: rows end at the token itself
+    m->h_pos_pinned[2] = ++m->epoch;   // the argmax kernel advances the device copy once per step
+    m->epoch += n_steps - 1;
+    SPYB_CUDA(be, cudaMemcpyAsync(m->d_pos, m->h_pos_pinned, 12, cudaMemcpyHostToDevice, be->stream));
+    SPYB_CUDA(be, cudaMemcpyAsync(m->d_tokens_in, m->h_tok_pinned, 4, cudaMemcpyHostToDevice, be->stream));
+    SPYB_CUDA(be, launch_embed(m->d_tokens_in, 1, m->embd, m->embd_type, m->info.d_model, m->x, be->stream));
+
+    const bool use_graph = be->config.use_graph != 0 && (m->info.tp_size == 1 || std::getenv("SPYB_TP_NO_GRAPH") == nullptr);   // the all-reduces of the prompt pass have warmed NCCL up before the capture
+    // one decode step captured once per sequence and form of the attention, when the first step of that form comes (a capture leaves the steps in
+    // front of it running); positions and the token live in device memory, so the same graph replays for every later step
+    auto step_at = [&](int pos) {
+        m->att_form = step_form(m, pos);
+        return use_graph ? captured_step(m, GRAPH_DECODE, [&](int64_t *n) { return run_decode_step(m, n); }) : nullptr;
+    };
+    if (step_at(n_past) == nullptr && use_graph) { return SPYB_FAIL; }
+    int64_t extra = 0, per_step = m->step_ok ? 2 : (int64_t)m->layers.size() * 5 + 2;
+    SPYB_CUDA(be, cudaEventRecord(m->ev0, be->stream));
+    for (int s = 0; s < n_steps; ++s) {
+        const spyb_model::StepGraph *step = step_at(n_past + s);
+        if (step == nullptr && use_graph) { cudaStreamSynchronize(be->stream); return SPYB_FAIL; }
+        if (use_graph) { SPYB_CUDA(be, cudaGraphLaunch(step->exec, be->stream)); }
+        else { int64_t n = 0; if (run_decode_step(m, &n) != SPYB_SUCCESS) { return SPYB_FAIL; } per_step = n; }
+        if (how != nullptr) {   // (the step has embedded the largest logit's token for the next one: the drawn token takes its place)
+            if (sample_step(m, &draw, m->d_tokens_in, nullptr, &extra) != SPYB_SUCCESS) { return SPYB_FAIL; }
+            SPYB_CUDA(be, launch_embed(m->d_tokens_in, 1, m->embd, m->embd_type, m->info.d_model, m->x, be->stream)); ++extra;
+        }
+        if (logits_host != nullptr) {
+            // parity mode: logits of every step come back (argmax_embed does not modify them)
+            SPYB_CUDA(be, cudaMemcpyAsync(logits_host + (size_t)s * m->info.n_vocab, m->logits, (size_t)m->info.n_vocab * 4, cudaMemcpyDeviceToHost, be->stream));
+            SPYB_CUDA(be, cudaStreamSynchronize(be->stream));
+        }
+    }
+    SPYB_CUDA(be, cudaEventRecord(m->ev1, be->stream));
+    SPYB_CUDA(be, cudaMemcpyAsync(ids_host, drawn != nullptr ? drawn : m->d_history + n_past, (size_t)n_steps * 4, cudaMemcpyDeviceToHost, be->stream));
+    SPYB_CUDA(be, cudaStreamSynchronize(be->stream));
+    if (be->device_error()) { return SPYB_FAIL; }
+    SPYB_CUDA(be, cudaEventElapsedTime(&m->last_ms, m->ev0, m->ev1));
+    m->last_launches = per_step * n_steps + extra;
+    return SPYB_SUCCESS;
+}
+
+spyb_status decode_batch(spyb_model *m, const int32_t *first_tokens, int32_t n_seq, int32_t n_past, int32_t n_steps, const spyb_sampling *how, int32_t *ids_host,
+                         float *logits_host) {
     if (m == nullptr || first_tokens == nullptr || ids_host == nullptr || n_steps < 1) { return SPYB_FAIL; }
     spyb_backend *be = m->be;
     cudaSetDevice(be->config.device_id);
@@ -1433,6 +1555,12 @@ spyb_status spyb_model_decode_batch(spyb_model *m, const int32_t *first_tokens, 
         if (dev_alloc(m, &m->batch_ids, (size_t)need) != SPYB_SUCCESS) { return SPYB_FAIL; }
         m->batch_ids_cap = need;
     }
+    spyb_sample_desc draw;
+    if (how != nullptr) {
+        const spyb_status st = prepare_sampling(m, *how, m->logits_batch, n_seq, n_steps, &draw);
+        if (st != SPYB_SUCCESS) { return st; }
+    }
+    const int32_t *drawn = how != nullptr ? draw.ids : nullptr;
     const int V = m->info.n_vocab, d = m->info.d_model;
     const int group = m->kq ? KQ_MAX_COLUMNS : std::min(TMAX, std::min(matvec_max_columns(d / 32), matvec_max_columns(m->info.n_ff / 32)));   // columns per pass through the layers
     SPYB_CUDA(be, cudaStreamSynchronize(be->stream));
@@ -1486,61 +1614,22 @@ spyb_status spyb_model_decode_batch(spyb_model *m, const int32_t *first_tokens, 
             if (run_layers(m, T, false, &launches, g0) != SPYB_SUCCESS) { return SPYB_FAIL; }
             if (run_head_columns(m, T, m->logits_batch + (int64_t)g0 * V, &launches) != SPYB_SUCCESS) { return SPYB_FAIL; }
         }
-        SPYB_CUDA(be, launch_argmax_embed_batch(m->logits_batch, V, n_seq, m->batch_tokens, m->batch_ids + (int64_t)step * n_seq, nullptr, 0, d, nullptr, 0, m->d_pos, be->stream));
-        launches += 2;
+        if (how != nullptr) {
+            if (sample_step(m, &draw, m->batch_tokens, m->d_pos, &launches) != SPYB_SUCCESS) { return SPYB_FAIL; }
+        } else {
+            SPYB_CUDA(be, launch_argmax_embed_batch(m->logits_batch, V, n_seq, m->batch_tokens, m->batch_ids + (int64_t)step * n_seq, nullptr, 0, d, nullptr, 0, m->d_pos, be->stream));
+            launches += 2;
+        }
         if (logits_host != nullptr) {
             SPYB_CUDA(be, cudaMemcpyAsync(logits_host + (int64_t)step * n_seq * V, m->logits_batch, (size_t)n_seq * V * 4, cudaMemcpyDeviceToHost, be->stream));
         }
     }
     SPYB_CUDA(be, cudaEventRecord(m->ev1, be->stream));
-    SPYB_CUDA(be, cudaMemcpyAsync(ids_host, m->batch_ids, (size_t)need * 4, cudaMemcpyDeviceToHost, be->stream));
+    SPYB_CUDA(be, cudaMemcpyAsync(ids_host, drawn != nullptr ? drawn : m->batch_ids, (size_t)need * 4, cudaMemcpyDeviceToHost, be->stream));
     SPYB_CUDA(be, cudaStreamSynchronize(be->stream));
     if (be->device_error()) { return SPYB_FAIL; }
     SPYB_CUDA(be, cudaEventElapsedTime(&m->last_ms, m->ev0, m->ev1));
     m->last_launches = launches;
     return SPYB_SUCCESS;
 }
-
-float   spyb_model_last_ms(const spyb_model *m) { return m ? m->last_ms : 0.f; }
-int64_t spyb_model_last_launches(const spyb_model *m) { return m ? m->last_launches : 0; }
-
-spyb_status spyb_model_read_activation(spyb_model *m, int32_t which, void *host, uint64_t bytes) {
-    if (m == nullptr || host == nullptr) { return SPYB_FAIL; }
-    const void *src = nullptr; uint64_t avail = 0;
-    switch (which) {
-    case 0: src = m->q;      avail = (uint64_t)8 * m->dl * 2; break;
-    case 1: src = m->att;    avail = (uint64_t)8 * m->info.d_model * 4; break;
-    case 2: src = m->x;      avail = (uint64_t)8 * m->info.d_model * 4; break;
-    case 3: src = m->act;    avail = (uint64_t)8 * m->info.n_ff * 4; break;
-    case 4: src = m->logits; avail = (uint64_t)m->info.n_vocab * 4; break;
-    default: m->be->set_error("read_activation: unknown buffer %d", which); return SPYB_FAIL;
-    }
-    if (bytes > avail) { m->be->set_error("read_activation: %llu bytes requested, %llu available", (unsigned long long)bytes, (unsigned long long)avail); return SPYB_FAIL; }
-    SPYB_CUDA(m->be, cudaStreamSynchronize(m->be->stream));
-    SPYB_CUDA(m->be, cudaMemcpy(host, src, bytes, cudaMemcpyDeviceToHost));
-    return SPYB_SUCCESS;
-}
-
-#ifndef SPYB_NO_MEASUREMENT_AIDS
-int32_t spyb_model_read_timeline(spyb_model *m, uint64_t *stamps_host, int32_t max_kernels) {
-    if (m == nullptr || m->d_stamps == nullptr || stamps_host == nullptr) { return 0; }
-    const int n = std::min<int>(max_kernels, 5 * (int)m->layers.size() + 1);
-    if (cudaMemcpy(stamps_host, m->d_stamps, (size_t)n * 8 * sizeof(uint64_t), cudaMemcpyDeviceToHost) != cudaSuccess) { return 0; }
-    return n;
-}
-
-int32_t spyb_model_read_step_timeline(spyb_model *m, uint64_t *stamps_host, int32_t max_points) {
-    if (m == nullptr || m->d_step_stamps == nullptr || stamps_host == nullptr) { return 0; }
-    const int n = std::min<int>(max_points, m->step_stamp_count);
-    if (cudaMemcpy(stamps_host, m->d_step_stamps, (size_t)n * 2 * sizeof(uint64_t), cudaMemcpyDeviceToHost) != cudaSuccess) { return 0; }
-    return n;
-}
-#endif
-
-spyb_status spyb_model_tap_xq(spyb_model *m, void *blocks_host) {
-    if (m == nullptr || blocks_host == nullptr) { return SPYB_FAIL; }
-    SPYB_CUDA(m->be, cudaMemcpy(blocks_host, m->d_tap, (size_t)m->info.d_model / 32 * 34, cudaMemcpyDeviceToHost));
-    return SPYB_SUCCESS;
-}
-
-}  // extern "C"
+}  // namespace

@@ -1836,4 +1836,15 @@ cudaError_t launch_argmax_embed_batch(const float *logits, int64_t n_vocab, int 
     return cudaGetLastError();
 }
 
+// Sampled ids become the next step's tokens: -1 (nothing to draw) goes on with token 0, as the greedy kernels do with a row of NaN. Advances the position
+// where pos_counter is given. One CTA, a few words: bound by its launch.
+__global__ void take_tokens_kernel(const int32_t *ids, int32_t *tokens, int n, int *pos_counter) {
+    for (int i = threadIdx.x; i < n; i += blockDim.x) { tokens[i] = max(ids[i], 0); }
+    if (pos_counter != nullptr && threadIdx.x == 0) { pos_counter[0] += 1; pos_counter[2] += 1; }
+}
+cudaError_t launch_take_tokens(const int32_t *ids, int32_t *tokens, int n, int *pos_counter, cudaStream_t s) {
+    take_tokens_kernel<<<1, 64, 0, s>>>(ids, tokens, n, pos_counter);
+    return cudaGetLastError();
+}
+
 }  // namespace spyb

@@ -6,6 +6,7 @@ import numpy as np
 import pytest
 
 from spy_b200 import backend as B
+from spy_b200 import gguf_io, quants
 
 pytestmark = pytest.mark.gpu
 
@@ -612,3 +613,113 @@ def test_results_do_not_depend_on_programmatic_launch(dev):
         d.free()
         b.close()
     assert np.array_equal(got[0][0], got[1][0]) and np.array_equal(got[0][1], got[1][1])
+
+
+# ---------------------------------------------------------------------------------------------- a model's decoding loop with drawn tokens
+def sampled_model(path, kq=False, nothing=False):
+    cfg = gguf_io.LlamaConfig(n_layer=2, d_model=256, n_head=2, n_ff=512, n_vocab=400, weight_std=0.06,
+                              **(dict(wtype=quants.Q4_K, overrides={"attn_v": quants.Q6_K, "ffn_down": quants.Q6_K, "output": quants.Q6_K}) if kq else {}))
+    gguf_io.make_llama_gguf(path, cfg, seed=61)
+    if nothing:                                                                       # every scale of the output matrix is NaN: so are all logits
+        blocks = bytes(gguf_io.read_gguf(path)[1]["output.weight"][2])
+        raw = np.memmap(path, dtype=np.uint8, mode="r+")
+        at = raw.tobytes().find(blocks)
+        raw[at:at + len(blocks)].reshape(-1, 18)[:, 0:2] = (0x00, 0x7e)
+        raw.flush()
+    return cfg
+
+
+def drawn(logits, uniform, temperature, top_k, top_p, min_p):
+    return np.array([plain_sample(x, np.float32(temperature), top_k, np.float32(top_p), np.float32(min_p), u)[0] for x, u in zip(logits, uniform)])
+
+
+@pytest.mark.parametrize("use_graph", [True, False])
+@pytest.mark.parametrize("kq", [False, True])
+def test_model_decode_sampled(use_graph, kq, tmp_models):
+    path = str(tmp_models / f"sampled{int(kq)}.gguf")
+    cfg = sampled_model(path, kq)
+    rng = np.random.default_rng(5)
+    prompt, n_steps = rng.integers(3, cfg.n_vocab, size=9), 20
+    b = B.B200Backend(0, use_graph=use_graph)
+    m = B.LlamaModel(b, path, n_ctx=64)
+    first = int(np.argmax(m.eval(prompt, 0)))
+    greedy = m.decode(first, 9, n_steps, want_logits=True)
+    for settings in ({}, {"temperature": 0.0}):                                       # (temperature 1 and no uniform numbers: the first index with any weight)
+        ids, logits = m.decode_sampled(first, 9, n_steps, want_logits=True, **settings)
+        if settings:
+            assert np.array_equal(ids, greedy[0]) and np.array_equal(logits, greedy[1])
+        else:
+            assert np.array_equal(ids, drawn(logits, np.zeros(n_steps), 1, 0, 1, 0))
+    for t, k, p, least in ((1.0, 0, 1.0, 0.0), (0.7, 30, 0.9, 0.01), (3.0, 0, 0.95, 0.0)):
+        u = rng.random(n_steps).astype(np.float32)
+        ids, logits = m.decode_sampled(first, 9, n_steps, uniform=u, temperature=t, top_k=k, top_p=p, min_p=least, want_logits=True)
+        assert np.array_equal(ids, drawn(logits, u, t, k, p, least))
+        again = m.decode_sampled(first, 9, n_steps, uniform=u, temperature=t, top_k=k, top_p=p, min_p=least)[0]
+        assert np.array_equal(ids, again)
+        last, feed = [], [first, *ids[:-1]]
+        for s, token in enumerate(feed):                                              # each step's logits are those of the tokens that were drawn
+            last.append(m.eval(np.array([token], dtype=np.int32), 9 + s))
+        assert np.array_equal(np.array(last), logits)
+        m.eval(prompt, 0)
+    again = m.decode(first, 9, n_steps)[0]
+    assert np.array_equal(again, greedy[0])
+    m.close()
+    b.close()
+
+
+@pytest.mark.parametrize("n_seq", [1, 5, 18])
+def test_model_decode_batch_sampled(n_seq, tmp_models):
+    """Every sequence draws what it would draw alone, with its own settings; batches on the mat-vec passes and on the GEMMs."""
+    path = str(tmp_models / "sampled0.gguf")
+    cfg = sampled_model(path)
+    rng = np.random.default_rng(n_seq)
+    n_prompt, n_steps = 11, 12
+    t, k = (0.4 + rng.random(n_seq)).astype(np.float32), rng.integers(0, 50, size=n_seq).astype(np.int32)
+    u = rng.random((n_steps, n_seq)).astype(np.float32)
+    t[0] = 0
+    b = B.B200Backend(0)
+    m = B.LlamaModel(b, path, n_ctx=64)
+    m.set_sequences(n_seq)
+    prompts, first, want = rng.integers(3, cfg.n_vocab, size=(n_seq, n_prompt)), [], []
+    for c in range(n_seq):
+        m.select_sequence(c)
+        first.append(int(np.argmax(m.eval(prompts[c], 0))))
+        want.append(m.decode_sampled(first[c], n_prompt, n_steps, uniform=u[:, c], temperature=t[c], top_k=k[c], top_p=0.9, want_logits=True))
+    ids, logits = m.decode_batch_sampled(first, n_prompt, n_steps, uniform=u, temperature=t, top_k=k, top_p=0.9, want_logits=True)
+    for c in range(n_seq):
+        assert np.array_equal(ids[:, c], want[c][0]) and np.array_equal(logits[:, c], want[c][1]), c
+        assert np.array_equal(ids[:, c], drawn(logits[:, c], u[:, c], t[c], k[c], 0.9, 0)), c
+    m.close()
+    b.close()
+
+
+def test_model_decode_sampled_with_nothing_to_draw(tmp_models):
+    path = str(tmp_models / "sampled_nan.gguf")
+    sampled_model(path, nothing=True)
+    b = B.B200Backend(0)
+    m = B.LlamaModel(b, path, n_ctx=32)
+    m.set_sequences(2)
+    for c in range(2):
+        m.select_sequence(c)
+        assert np.isnan(m.eval(np.array([5, 6], dtype=np.int32), 0)).all()
+        assert np.array_equal(m.decode_sampled(7, 2, 3)[0], [-1] * 3)
+    assert np.array_equal(m.decode_batch_sampled([7, 8], 2, 3)[0], [[-1, -1]] * 3)
+    m.close()
+    b.close()
+
+
+def test_model_decode_sampled_refuses(tmp_models):
+    path = str(tmp_models / "sampled0.gguf")
+    cfg = sampled_model(path)
+    b = B.B200Backend(0)
+    m = B.LlamaModel(b, path, n_ctx=32)
+    m.set_sequences(2)
+    for bad in (lambda: m.decode_sampled(5, 30, 3), lambda: m.decode_sampled(cfg.n_vocab, 0, 3), lambda: m.decode_batch_sampled([1, 2, 3], 0, 2), lambda: m.decode_batch_sampled([1, -2], 0, 2),
+                lambda: m.decode_batch_sampled([1, 2], -1, 2)):
+        with pytest.raises(B.SpybError):
+            bad()
+    ids = np.zeros(3, np.int32)
+    assert b._l.spyb_model_decode_sampled(m.h, 5, 0, 3, None, B._np_ptr(ids), None) != B.SUCCESS
+    assert m.decode_sampled(5, 0, 3, temperature=0.0)[0].tolist() == m.decode(5, 0, 3)[0].tolist()
+    m.close()
+    b.close()
