@@ -218,6 +218,9 @@ spyb_status spyb_create(const spyb_config *config, spyb_backend **out) {
               cudaMalloc(reinterpret_cast<void **>(&be->d_exp_table), 65536 * 4) == cudaSuccess &&
               upload(be->d_silu_table, silu.data(), 65536 * 4) == cudaSuccess &&
               upload(be->d_exp_table, ex.data(), 65536 * 4) == cudaSuccess;
+    std::vector<uint64_t> powers(1024);
+    for (int j = 0; j < 1024; ++j) { powers[j] = (uint64_t)std::floor(std::exp2(46.0 - j / 1024.0) + 0.5); }
+    ok = ok && cudaMalloc(reinterpret_cast<void **>(&be->d_power_table), 1024 * 8) == cudaSuccess && upload(be->d_power_table, powers.data(), 1024 * 8) == cudaSuccess;
     if (!ok) { spyb_destroy(be); return SPYB_FAIL; }
     const size_t handoff = (size_t)be->num_sms_total * (PF_HANDOFF_BYTES + PF_HANDOFF_FLAGS * sizeof(unsigned));
     if (cudaMalloc(&be->pf_handoff, handoff) != cudaSuccess) { cudaGetLastError(); be->pf_handoff = nullptr; }   // (the GEMMs go without)
@@ -241,6 +244,7 @@ void spyb_destroy(spyb_backend *be) {
     if (be->paged_partial) { cudaFree(be->paged_partial); }
     if (be->d_silu_table) { cudaFree(be->d_silu_table); }
     if (be->d_exp_table) { cudaFree(be->d_exp_table); }
+    if (be->d_power_table) { cudaFree(be->d_power_table); }
     if (be->h_error_flag) { cudaFreeHost(be->h_error_flag); }
     be->arena.destroy();
     if (be->stream) { cudaStreamDestroy(be->stream); }

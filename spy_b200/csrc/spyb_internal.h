@@ -110,6 +110,7 @@ struct spyb_backend {
     uint8_t     *noalloc_scratch = nullptr; // device address of the scratch array of spyb_matmul_noalloc (looked up once)
     float       *d_silu_table = nullptr;   // 65536 entries: xh / (1 + expf(-xh)) for the fp16 value xh
     float       *d_exp_table = nullptr;    // 65536 entries: expf(xh)
+    uint64_t    *d_power_table = nullptr;  // 1024 entries: 2^46 2^-(j / 1024), the sampler's
 
     std::mutex  err_mutex;
     std::string last_error;

@@ -34,6 +34,7 @@ struct SampleParams {
     const int32_t *top_k;
     int32_t       *ids;
     float         *probs;
+    const uint64_t *powers;                     // 2^46 2^-(j / 1024), j = 0 .. 1023, to the nearest
     int           *error_flag;
     uint64_t       wait_limit;
 };
@@ -85,6 +86,9 @@ struct SampleShared {
     uint64_t share2[SA_MAX_CLUSTER], told[SA_MAX_CLUSTER];
     uint64_t arrived[SA_PIECES];             // barriers of the slice's pieces
     uint64_t cut, total;
+    double   c, edge;                        // of this row: Weight's, found by one thread while the slice comes (64 bits are slow: see Weight)
+    uint64_t least;                          // the smallest weight that min_p leaves
+    float    bin_scale, unused;
     uint64_t table[1024];                    // Weight's
     uint32_t n_list, n_own;
     int      found, found2;
@@ -103,9 +107,9 @@ struct Weight {
     bool   wide;                // in 64 bits
     double c, largest;
     int    shift;               // 46 - S
-    __device__ __forceinline__ void set(const uint64_t *powers, float top, double scale, int bits) {
+    __device__ __forceinline__ void set(const uint64_t *powers, float top, double scale, double edge, int bits) {   // edge: 56 / c (2^-56 is no unit: rounds to nothing)
         table = powers; c = scale; largest = top; shift = 46 - bits;
-        const double a = largest * c, lowest = largest - 56 / c;                         // (2^-56 is no unit: rounds to nothing)
+        const double a = largest * c, lowest = largest - edge;
         wide = !(fabs(a) < 960.0 && lowest > -3.4e38);
         least = wide ? 0.f : (float)lowest;
         c_hi = (float)c; c_lo = (float)(c - c_hi);
@@ -259,6 +263,8 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(const __grid_cons
         sh.n_list = sh.n_own = 0; sh.cut = 0; sh.found = sh.found2 = 0;
     }
     *reinterpret_cast<uint2 *>(sh.count + 2 * tid) = make_uint2(0, 0);
+    static_assert(2 * SA_THREADS == 1024, "a thread brings two of the table's powers");
+    const uint4 powers = __ldg(reinterpret_cast<const uint4 *>(p.powers) + tid);
     asm volatile("barrier.cluster.arrive.release;" ::: "memory");   // (waited for in front of the first access to another CTA's memory)
     pdl_wait();
 
@@ -285,9 +291,12 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(const __grid_cons
     const float min_p = p.min_p ? p.min_p[row] : 0.f, uni = p.uniform ? p.uniform[row] : 0.f;
     const int   top_k = p.top_k ? p.top_k[row] : 0;
 
-    // (while the slice comes; the powers' table is needed by whoever weighs)
-    if (!(p.temperature && !(p.temperature[row] > 0.f))) {
-        for (int i = tid; i < 1024; i += SA_THREADS) { sh.table[i] = (uint64_t)(exp2(-(double)i / 1024) * 70368744177664.0 + 0.5); }
+    *reinterpret_cast<uint4 *>(sh.table + 2 * tid) = powers;
+    if (tid == SA_THREADS - 1) {
+        const double c = fmax(fmin(1.4426950408889634073599 / (double)temp, 1e30), 1e-30);
+        sh.c = c; sh.edge = 56 / c;
+        sh.least = min_p > 0.f ? (uint64_t)max(1.0, ceil((double)fminf(min_p, 1.f) * __hiloint2double((1023 + p.frac_bits) << 20, 0))) : 1;
+        sh.bin_scale = (float)(c * (SA_BINS / (double)(p.frac_bits + 1)));
     }
     // this thread's largest (of the elements that Slice::each gives it), the row's, and where that is
     float own = -CUDART_INF_F, from_here = CUDART_INF_F;      // (top-k: nothing below from_here is among the k largest)
@@ -391,10 +400,9 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(const __grid_cons
         }
     }
     Weight weight;
-    weight.set(sh.table, largest, fmax(fmin(1.4426950408889634073599 / (double)temp, 1e30), 1e-30), p.frac_bits);
-    const double one = __hiloint2double((1023 + p.frac_bits) << 20, 0);
-    const uint64_t least = min_p > 0.f ? (uint64_t)max(1.0, ceil((double)fminf(min_p, 1.f) * one)) : 1;
-    const float  bin_scale = (float)(weight.c * (SA_BINS / (double)(p.frac_bits + 1)));
+    weight.set(sh.table, largest, sh.c, sh.edge, p.frac_bits);
+    const uint64_t least = sh.least;
+    const float    bin_scale = sh.bin_scale;
     auto bin_of = [&](float v) { return (largest - v) * bin_scale; };        // not below SA_BINS (or NaN): no weight
     auto reach = [&](uint64_t total) { return max((uint64_t)1, (uint64_t)ceil((double)max(top_p, 0.f) * (double)total)); };   // a token stays while less than this is in front of it
     uint64_t cut = 0;                        // keys from here on stay
@@ -778,7 +786,7 @@ extern "C" spyb_status spyb_sample(spyb_backend *be, const spyb_sample_desc *d) 
     while ((1 << log2_vocab) < d->n_vocab) { ++log2_vocab; }
     p.frac_bits = std::min(45, 62 - log2_vocab);
     p.temperature = d->temperature; p.top_k = d->top_k; p.top_p = d->top_p; p.min_p = d->min_p; p.uniform = d->uniform; p.ids = d->ids; p.probs = d->probs;
-    p.error_flag = be->d_error_flag; p.wait_limit = be->wait_limit_ns;
+    p.powers = be->d_power_table; p.error_flag = be->d_error_flag; p.wait_limit = be->wait_limit_ns;
     const LaunchCfg cfg = be->launch_cfg(be->config.use_pdl != 0);
     SPYB_CUDA(be, d->number_type == SPYB_FP32 ? launch_sample<float>(p, d->n_rows, be->num_sms_total, cfg) : launch_sample<__half>(p, d->n_rows, be->num_sms_total, cfg));
     return SPYB_SUCCESS;
