@@ -723,7 +723,7 @@ spyb_status spyb_paged_attention(spyb_backend *be, const spyb_paged_attention_de
         if (!launch_paged_attention_tc(p, hd, d->n_head, be->num_sms_total, cfg, be->wait_limit_ns, &err)) { p.few_rows = 1 << 30; }
         SPYB_CUDA(be, err);
     }
-    const int row_tiles = most <= 16 ? 1 : 2;
+    const int row_tiles = std::min<int64_t>(most, p.few_rows) <= 16 ? 1 : 2;
     p.tile_rows = 16 * row_tiles;
     if (p.few_rows > 0) { SPYB_CUDA(be, launch_paged_attention_rows(p, hd, row_tiles, be->num_sms_total, cfg)); }
     return SPYB_SUCCESS;
