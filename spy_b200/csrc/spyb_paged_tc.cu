@@ -11,6 +11,7 @@
 // Probabilities are taken against a maximum that follows the true one when that is 2^8 above it: O is rescaled in the first steps and hardly ever after.
 
 #include <algorithm>
+#include <type_traits>
 
 #include <cuda.h>
 #include <math_constants.h>
@@ -318,6 +319,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
 #pragma unroll 1
             for (int i = 0; i < HD / 32; ++i) {
                 uint32_t o[32];
+                __syncwarp();
                 if (any) { tmem_ld32(o_tmem + 32 * i, o); tmem_ld_wait(); }
                 else {
 #pragma unroll
@@ -341,7 +343,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
                         }
                     }
                 }
-                if (parts > 1) {
+                if (parts > 1 && mine) {
 #pragma unroll
                     for (int c = 0; c < 8; ++c) {
                         part[(8 * i + c) * PT_ROWS + row] = make_float4(__uint_as_float(o[4 * c]), __uint_as_float(o[4 * c + 1]), __uint_as_float(o[4 * c + 2]), __uint_as_float(o[4 * c + 3]));
@@ -366,7 +368,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
                 }
             }
             tc_fence_before();
-            if (parts > 1) {
+            if (parts > 1 && own.rows > 0) {
                 float *stats = reinterpret_cast<float *>(part + PT_ROWS * HD / 4);
                 stats[row] = m; stats[PT_ROWS + row] = l;
                 __threadfence();
@@ -380,42 +382,68 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
                 }
                 all_of_tile();
                 if (*reinterpret_cast<volatile int *>(&sh.last[t])) {
-                    const float4 *all = reinterpret_cast<const float4 *>(p.partial);
-                    auto piece = [&](int i) { return all + (paged_slot(c0 + i, c0) * 2 + t) * (PT_ROWS * (HD + 2) / 4); };
-                    if (mine) {
-                        float top = -CUDART_INF_F, sum = 0.f;
-#pragma unroll 4
-                        for (int i = 0; i < parts; ++i) { top = fmaxf(top, __ldcg(reinterpret_cast<const float *>(piece(i) + PT_ROWS * HD / 4) + row)); }
+                    // Few rows have several threads each, so that all of them load: row `row & (rows - 1)`, every share-th four elements. Either way 16 loads of 16
+                    // bytes a thread are in flight: of one CTA's piece, or where rows are few and their CTAs many, of four
+                    int rows = PT_ROWS;
+                    while (rows > 4 && rows / 2 >= own.rows) { rows /= 2; }
+                    const int r = row & (rows - 1), share = PT_ROWS / rows, token_in = (int)((unsigned)r / (unsigned)p.group);
+                    const float4 *const all = reinterpret_cast<const float4 *>(p.partial) + t * (PT_ROWS * (HD + 2) / 4);
+                    auto piece = [&](int i) { return all + paged_slot(c0 + i, c0) * (2 * PT_ROWS * (HD + 2) / 4); };
+                    const int64_t out_row = (int64_t)(en.row0 + (2 * en.tile + t) * half_tokens + token_in) * p.out_stride + (en.head * p.group + r - token_in * p.group) * HD;
+                    auto join = [&](auto fours, auto ahead) {
+                        constexpr int FOURS = decltype(fours)::value, AHEAD = decltype(ahead)::value;
+                        float top = -CUDART_INF_F;
+#pragma unroll 8
+                        for (int i = 0; i < parts; ++i) { top = fmaxf(top, __ldcg(reinterpret_cast<const float *>(piece(i) + PT_ROWS * HD / 4) + r)); }
                         const float ref = top == -CUDART_INF_F ? 0.f : top;
 #pragma unroll 1
-                        for (int q4 = 0; q4 < HD / 4; q4 += 16) {
-                            float4 v[16];
+                        for (int q4 = row / rows; q4 < HD / 4; q4 += FOURS * share) {
+                            float4 v[FOURS];
 #pragma unroll
-                            for (int c = 0; c < 16; ++c) { v[c] = make_float4(0.f, 0.f, 0.f, 0.f); }
-                            sum = 0.f;
+                            for (int c = 0; c < FOURS; ++c) { v[c] = make_float4(0.f, 0.f, 0.f, 0.f); }
+                            float sum = 0.f;
 #pragma unroll 1
-                            for (int i = 0; i < parts; ++i) {
-                                const float4 *from = piece(i);
-                                const float *st = reinterpret_cast<const float *>(from + PT_ROWS * HD / 4);
-                                const float f = exp2_fast(__ldcg(st + row) - ref);
-                                sum += f * __ldcg(st + PT_ROWS + row);
+                            for (int i0 = 0; i0 < parts; i0 += AHEAD) {
+                                float4 u[AHEAD][FOURS];
+                                float  pm[AHEAD], pl[AHEAD];
 #pragma unroll
-                                for (int c = 0; c < 16; ++c) {
-                                    const float4 u = __ldcg(from + (q4 + c) * PT_ROWS + row);
-                                    v[c].x += f * u.x; v[c].y += f * u.y; v[c].z += f * u.z; v[c].w += f * u.w;
+                                for (int j = 0; j < AHEAD; ++j) {
+                                    const bool is = i0 + j < parts;
+                                    const float4 *from = piece(is ? i0 + j : 0);
+                                    const float *st = reinterpret_cast<const float *>(from + PT_ROWS * HD / 4);
+                                    pm[j] = is ? __ldcg(st + r) : -CUDART_INF_F;
+                                    pl[j] = is ? __ldcg(st + PT_ROWS + r) : 0.f;
+#pragma unroll
+                                    for (int c = 0; c < FOURS; ++c) { u[j][c] = is && q4 + c * share < HD / 4 ? __ldcg(from + (q4 + c * share) * PT_ROWS + r) : make_float4(0.f, 0.f, 0.f, 0.f); }
+                                }
+#pragma unroll
+                                for (int j = 0; j < AHEAD; ++j) {
+                                    const float f = exp2_fast(pm[j] - ref);
+                                    sum += f * pl[j];
+#pragma unroll
+                                    for (int c = 0; c < FOURS; ++c) { v[c].x += f * u[j][c].x; v[c].y += f * u[j][c].y; v[c].z += f * u[j][c].z; v[c].w += f * u[j][c].w; }
                                 }
                             }
                             const float inv_all = sum == 0.f ? 0.f : 1.f / sum;
 #pragma unroll
-                            for (int c = 0; c < 16; c += 2) {
-                                const float4 a = make_float4(v[c].x * inv_all, v[c].y * inv_all, v[c].z * inv_all, v[c].w * inv_all);
-                                const float4 b = make_float4(v[c + 1].x * inv_all, v[c + 1].y * inv_all, v[c + 1].z * inv_all, v[c + 1].w * inv_all);
-                                if (p.out_f32) {
-                                    float4 *dst = reinterpret_cast<float4 *>(static_cast<float *>(p.out) + to_row + 4 * (q4 + c));
-                                    dst[0] = a; dst[1] = b;
-                                } else { *reinterpret_cast<uint4 *>(static_cast<__half *>(p.out) + to_row + 4 * (q4 + c)) = make_uint4(pack_f16(a.x, a.y), pack_f16(a.z, a.w), pack_f16(b.x, b.y), pack_f16(b.z, b.w)); }
+                            for (int c = 0; c < FOURS; ++c) { v[c] = make_float4(v[c].x * inv_all, v[c].y * inv_all, v[c].z * inv_all, v[c].w * inv_all); }
+                            __half *const out16 = static_cast<__half *>(p.out) + out_row;
+#pragma unroll
+                            for (int c = 0; c < FOURS; ++c) {
+                                const int at = q4 + c * share;
+                                if (at >= HD / 4) { break; }
+                                if (p.out_f32) { *reinterpret_cast<float4 *>(static_cast<float *>(p.out) + out_row + 4 * at) = v[c]; }
+                                else if (FOURS < 16) { *reinterpret_cast<uint2 *>(out16 + 4 * at) = make_uint2(pack_f16(v[c].x, v[c].y), pack_f16(v[c].z, v[c].w)); }
+                                else if (c % 2 == 0) {
+                                    const float4 b = v[(c + 1) % FOURS];
+                                    *reinterpret_cast<uint4 *>(out16 + 4 * at) = make_uint4(pack_f16(v[c].x, v[c].y), pack_f16(v[c].z, v[c].w), pack_f16(b.x, b.y), pack_f16(b.z, b.w));
+                                }
                             }
                         }
+                    };
+                    if (r < own.rows) {
+                        if (share == 1) { join(std::integral_constant<int, 16>(), std::integral_constant<int, 1>()); }
+                        else { join(std::integral_constant<int, 4>(), std::integral_constant<int, 4>()); }
                     }
                 }
             }
