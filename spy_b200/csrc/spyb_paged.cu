@@ -17,6 +17,8 @@ namespace {
 // Memory bound: every element is read once and written once, (4 + 2) or (2 + 2) bytes. A CTA has one row; a thread has eight elements of a head - a 16-byte piece of
 // the output, or half of two pieces where the pairs are halves - in every 8th or 16th head, so that its (up to) four angles are made once a row. Angles are
 // position x share of a circle in 64 bits, reduced to half a turn either way: in f32 a position of 100 000 leaves an angle 0.004 of uncertainty.
+// Measured: 8900 rows of 120 heads of 128 elements (f32, 852 MB) 155 us, 5.5 TB/s; one row 3.7 us and 96 rows 6 to 8 us, a launch and a chain of four dependent loads
+// (whose row, which position, which page, the row itself).
 constexpr int AP_THREADS = 256;
 
 __device__ __forceinline__ int sequence_of(const PagedView &v, int row) {   // the last s with row_start[s] <= row, by a whole warp; -1 and n_seq: nobody's
@@ -104,6 +106,10 @@ __global__ void __launch_bounds__(AP_THREADS) paged_append_kernel(const __grid_c
 // asynchronous copies, scores and values by mma.sync on up to 32 rows, a running maximum and sum in registers - and the warps of a CTA, then the CTAs
 // of an item are joined at the end. The maximum that probabilities are taken against follows the true one only when that is 2^8 above it: the
 // accumulators are hardly ever rescaled, and p <= 2^8 is as exact in fp16 as p <= 1.
+// Measured: three sequences of 100 000 positions, 40 query heads on 8 of 128 elements (1.2 GB) 191 us, 6.3 TB/s; 64 sequences of up to 4096, 32 on 8: 103 us, 5.3 TB/s,
+// heads of 64: 65 us, 4.2 TB/s; one of 4000, 32 on 32 (66 MB): 21 us. What is above the memory's time: some 6 us until the first block is there (lengths, the plan, the
+// page table, the block, one after the other), the join of items on a cut (3 to 4 us), and each warp's chain of copy, scores, powers and values with eight to
+// twelve warps an SM.
 constexpr int PR_WARPS = 4, PR_BLOCK = 16, PR_UNIT = PR_WARPS * PR_BLOCK;
 
 __device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
@@ -132,10 +138,11 @@ template <int HD> struct RowsShape {
 };
 template <int HD, int MT> struct RowsSmem {       // the ring; what the warps found: beside it for up to EARLY rows, in its place for more; the masks of the ring's stages
     static constexpr int EARLY = MT == 1 ? 8 : 0, FOUND = PR_WARPS * 16 * MT * (HD + 2) * 4, RING = RowsShape<HD>::RING > FOUND ? RowsShape<HD>::RING : FOUND;
-    static constexpr int CTAS = MT == 1 && HD <= 64 ? 3 : 2;         // of an SM
+    static constexpr int CTAS = MT == 1 && HD <= 64 ? 3 : 2;         // of an SM (64 single tokens, heads of 64: 65 us with three, 79 with two; longer heads' rings leave room for two)
     static constexpr int MASKS = RING + PR_WARPS * EARLY * (HD + 2) * 4, BYTES = MASKS + PR_WARPS * RowsShape<HD>::STAGES * 4;
 };
-// IN_PAGE: a block's positions lie in one page (pages of a multiple of 16)
+// IN_PAGE: a block's positions lie in one page (pages of a multiple of 16), heads of up to 64: 64 single tokens 64.8 us against 66.6. (Longer heads' blocks take longer than
+// the table's latency: 103.2 us against 102.8, they go without.)
 template <int HD, int MT, bool IN_PAGE>
 __global__ void __launch_bounds__(PR_WARPS * 32) paged_rows_kernel(const __grid_constant__ PagedAttention p) {
     constexpr int PR_STAGES = RowsShape<HD>::STAGES, TILE = 16 * MT, ROW = RowsShape<HD>::ROW, STAGE = RowsShape<HD>::STAGE, NT = PR_WARPS * 32;
@@ -206,12 +213,10 @@ __global__ void __launch_bounds__(PR_WARPS * 32) paged_rows_kernel(const __grid_
             cp_commit();
         };
 
-    // Short positions in one page: a lane has the page of every 32nd block of this warp, the next 32 are read while these are in use; a block's is told by its lane. (Long
-    // positions' blocks take longer than the table's latency: one page ahead, 64 single tokens 103.0 us against 104.5.)
-    constexpr bool BATCH = IN_PAGE && HD <= 64;
+    // IN_PAGE: a lane has the page of every 32nd block of this warp, the next 32 are read while these are in use; a block's is told by its lane
     int page = -1, ids = -1, ids_next = -1, issued = 0;   // (page: of the block that is issued next)
     auto next_page = [&](int b) {             // of block b, the `issued`-th of this warp
-        if (!BATCH) { return page_of(b); }
+        if (!IN_PAGE) { return page_of(b); }
         const int l = issued & 31;
         if (l == 0) { ids = ids_next; ids_next = page_of(warp + (issued + 32 + lane) * PR_WARPS); }
         ++issued;
@@ -221,7 +226,7 @@ __global__ void __launch_bounds__(PR_WARPS * 32) paged_rows_kernel(const __grid_
     int pos[MT][2];
     auto start = [&]() {                      // the item's first blocks are on their way while its Q comes
         issued = 0;
-        if (BATCH) { ids_next = page_of(warp + lane * PR_WARPS); }
+        if (IN_PAGE) { ids_next = page_of(warp + lane * PR_WARPS); }
         page = next_page(warp);
 #pragma unroll
         for (int i = 0; i < PR_STAGES - 1; ++i) {
@@ -489,14 +494,17 @@ cudaError_t launch_rows(PagedAttention p, int sms, const LaunchCfg &cfg) {
     const int page = p.view.page_size;
     p.page_shift = -1;
     for (int s = 0; s < 31; ++s) { if (page == 1 << s) { p.page_shift = s; } }
-    return page % PR_BLOCK == 0 ? launch_rows_as<HD, MT, true>(p, sms, cfg) : launch_rows_as<HD, MT, false>(p, sms, cfg);
+    if constexpr (HD <= 64) {
+        if (page % PR_BLOCK == 0) { return launch_rows_as<HD, MT, true>(p, sms, cfg); }
+    }
+    return launch_rows_as<HD, MT, false>(p, sms, cfg);
 }
 
 }  // namespace
 
 cudaError_t launch_paged_append(const PagedAppend &p, int in_type, int q_out_type, const LaunchCfg &cfg) {
     const int total = p.n_head + 2 * p.n_head_kv, slots = AP_THREADS / (p.head_dim / 8), loops = (total + slots - 1) / slots;
-    // few rows: a row's heads are spread over CTAs
+    // few rows: a row's heads are spread over CTAs (one row of 96 heads 5.8 us against 6.0 in one CTA, 300 rows of 56 heads 9.7 against 9.9)
     const int split = std::max(1, std::min(loops, 296 / std::max(1, p.view.n_rows)));
     const dim3 grid(p.view.n_rows, split);
     if (in_type == SPYB_FP32) {

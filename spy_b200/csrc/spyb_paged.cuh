@@ -39,7 +39,10 @@ cudaError_t launch_paged_append(const PagedAppend &p, int in_type, int q_out_typ
 cudaError_t launch_paged_attention_rows(const PagedAttention &p, int head_dim, int row_tiles, int sms, const LaunchCfg &cfg);
 // the kernel on tensor memory; false where it does not take these pages, heads or strides (nothing is launched then)
 bool        launch_paged_attention_tc(const PagedAttention &p, int head_dim, int n_head, int sms, const LaunchCfg &cfg, uint64_t wait_limit, cudaError_t *err);
-constexpr int PA_FEW_ROWS = 16;          // sequences of up to so many rows (times query heads of a K/V head) are the small kernel's
+// Sequences of up to so many rows (times query heads of a K/V head) are the small kernel's, whose tile of 16 rows costs them nothing but the memory's time; a second tile
+// doubles its instructions. 24 sequences of up to 9000 positions, four query heads a K/V head: 3 and 4 rows (12 and 16 in all) 95 and 98 us there against
+// 118 and 118 on tensor memory, 5 and 8 rows (20 and 32) 144 and 156 against 118 and 118.
+constexpr int PA_FEW_ROWS = 16;
 
 // ---------------------------------------------------------------------------------------------- cutting the work
 // The rows of a sequence that share a K/V head - token by token, its query heads side by side - are cut into tiles; a tile and a K/V head are an item, and the

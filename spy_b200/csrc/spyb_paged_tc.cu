@@ -9,6 +9,13 @@
 //   warps 0-3, 4-7   probabilities of tile 0 / 1, rescaling, output          warp 8   issues the MMAs
 //   warp 9           copies                                                   warps 10, 11  clear and check the V tiles that not all rows see whole
 // Probabilities are taken against a maximum that follows the true one when that is 2^8 above it: O is rescaled in the first steps and hardly ever after.
+// Measured (heads of 128): 8192 tokens of a prompt, 32 heads, 570 us, 965 TFLOP/s of the 1640 of a matrix product; 512 tokens at 32 768 positions 281 us, 970;
+// 1500 at 9111, 40 heads, 247 us, 1040; 512 at 3968 55 us, 577; five tokens of 24 sequences of up to 9000, 119 us, 3.9 TB/s. Heads of 64 have half the
+// products for as many powers: 8192 tokens 524 us, 524 TFLOP/s. A step of 256 rows and 128 positions takes 2.4 us, in which 16 powers a clock alone take 1.1; the chain of
+// a tile - S, reading it, maximum, powers, P, product - is what bounds it, two tiles hide each other's. Beside the steps: 7 us until the first (lengths, the plan, page
+// table, Q and K), some 4 us from one stretch to the next and for the join of an item on a cut, which is what holds short contexts back (512 tokens at 1024: 35 us).
+// Tried and left out: powers by polynomials on the FMA units for some of the columns (slower: their instructions are what is short), the two tiles taking turns by
+// barriers (no gain), both tiles on one tile's rows by every second step where only one has rows (24 x 5 rows 122 us against 119: memory bounds those steps).
 
 #include <algorithm>
 #include <type_traits>
@@ -30,7 +37,7 @@ constexpr uint32_t PT_HALF = PT_KEYS * 128;              // bytes of 128 rows x 
 template <int HD> struct TcShape {
     static constexpr uint32_t OPERAND = PT_KEYS * HD * 2;                      // a tile of Q, K or V
     static constexpr int SLOTS = HD == 128 ? 5 : 8;                            // K and V tiles in flight
-    static constexpr int Q_BUFFERS = HD == 128 ? 1 : 2;                        // (heads of 64: the next stretch's Q comes while this one's is in use)
+    static constexpr int Q_BUFFERS = HD == 128 ? 1 : 2;                        // (heads of 64: the next stretch's Q comes while this one's is in use; there is room for it)
     static constexpr uint32_t SMEM = (2 * Q_BUFFERS + SLOTS) * OPERAND + 1024; // (+ alignment)
     // tensor memory: S of both tiles, then O of both; P over S, or for heads of 64, whose O leaves room, beside it: the next S is made while P is
     static constexpr bool P_APART = HD == 64;
@@ -173,6 +180,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
     pdl_launch_dependents();
     pdl_wait();
     Walker walk;
+    // (at least two steps a CTA: 512 tokens at 512 positions 21.7 us, against 24.9 from one step on and 29.1 from four; 4 x 20 rows at 700 positions 23.4, 25.6, 28.3)
     walk.at = paged_plan<PT_THREADS, PT_KEYS, PT_KEYS>(p, false, 2, sh.plan);
     if (walk.at.unit >= walk.at.end) { return; }
     if (warp == 8) { asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&sh.tmem)) : "memory"); }
@@ -383,7 +391,8 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
                 all_of_tile();
                 if (*reinterpret_cast<volatile int *>(&sh.last[t])) {
                     // Few rows have several threads each, so that all of them load: row `row & (rows - 1)`, every share-th four elements. Either way 16 loads of 16
-                    // bytes a thread are in flight: of one CTA's piece, or where rows are few and their CTAs many, of four
+                    // bytes a thread are in flight: of one CTA's piece, or where rows are few, and their CTAs often many, of four (five rows at 100 000 positions, 18 CTAs
+                    // an item: 96 us against 113 in the first way; a tile of 128 rows has few CTAs an item: a chunk of 512 rows 55 us in the first way, 58 in the second)
                     int rows = PT_ROWS;
                     while (rows > 4 && rows / 2 >= own.rows) { rows /= 2; }
                     const int r = row & (rows - 1), share = PT_ROWS / rows, token_in = (int)((unsigned)r / (unsigned)p.group);
