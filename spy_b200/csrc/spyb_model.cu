@@ -717,7 +717,7 @@ spyb_status prepare_sampling(spyb_model *m, const spyb_sampling &how, const floa
     spyb_backend *be = m->be;
     *d = {};
     d->number_type = SPYB_FP32; d->n_rows = n_seq; d->n_vocab = m->info.n_vocab; d->row_stride = m->info.n_vocab; d->logits = logits;
-    const int64_t each = n_seq, all = (int64_t)n_seq * n_steps, need = 4 * each + 2 * all;
+    const int64_t each = n_seq, all = (int64_t)n_seq * n_steps, need = 4 * each + 2 * each * m->info.n_ctx;   // (n_steps is n_ctx at most)
     if (need > m->sampling_cap) {
         if (dev_alloc(m, &m->sampling, (size_t)need) != SPYB_SUCCESS) { return SPYB_FAIL; }
         m->sampling_cap = need;

@@ -183,7 +183,8 @@ __global__ void __launch_bounds__(PR_WARPS * 32) paged_rows_kernel(const __grid_
             const unsigned mask = IN_PAGE ? (ok ? (kb - j >= PR_BLOCK ? 0xffffu : (1u << (kb - j)) - 1) : 0u) : __ballot_sync(0xffffffffu, ok) & 0xffffu;
             const uint32_t dst = ring + stage * STAGE;
             constexpr int PIECES = HD / 8;
-            if (IN_PAGE && 32 % PIECES == 0) {
+            if constexpr (IN_PAGE) {
+                static_assert(32 % PIECES == 0, "a row's pieces are lanes side by side");
                 constexpr int AT_ONCE = 32 / PIECES;
                 const int r0 = lane / PIECES, c = lane % PIECES;
                 int64_t o = cell + r0 * p.view.token_stride + c * 8;
@@ -203,7 +204,7 @@ __global__ void __launch_bounds__(PR_WARPS * 32) paged_rows_kernel(const __grid_
                 for (int i = 0; i < PIECES / 2; ++i) {
                     const int x = i * 32 + lane, r = x / PIECES, c = x - r * PIECES;
                     const bool in = (mask >> r) & 1;
-                    const int64_t row = IN_PAGE ? cell + r * p.view.token_stride : __shfl_sync(0xffffffffu, cell, r), o = in ? row + c * 8 : 0;
+                    const int64_t row = __shfl_sync(0xffffffffu, cell, r), o = in ? row + c * 8 : 0;
                     const uint32_t d = dst + r * ROW + ((c ^ (r & 7)) << 4);
                     cp_async16(d, kbase + o, in);
                     cp_async16(d + PR_BLOCK * ROW, vbase + o, in);

@@ -61,6 +61,7 @@ struct Entry {
         return j + PT_KEYS <= hi && (!p.causal || (j + PT_KEYS - 1 <= h.pos_first && (p.window <= 0 || j > h.pos_last - p.window)));
     }
 };
+constexpr uint64_t PT_LANDING_NS = 1000000000;       // when a wait gave up: what is on its way has this long to land (whatever the limit of the waits)
 constexpr int PT_ENTRIES = 4, PT_READERS = 11;       // stretches known ahead; warps that read them: eight for probabilities, one for MMAs, two for Q and V
 struct TcShared {
     uint64_t full[8], empty[8];                          // a slot's copies have landed; its last MMA is done
@@ -69,6 +70,7 @@ struct TcShared {
     uint64_t s_ready[2], s_free[2], p_ready[2][2], p_free[2], o_ready[2];   // (P ready) of the first 96 positions and the rest; (free) where P lies apart
     uint64_t known[PT_ENTRIES], read[PT_ENTRIES];        // an entry is there; all have read it
     uint64_t joined[2];                                  // all threads of a tile have come so far
+    uint64_t over;                                       // (something gave up) the last MMA is done
     uint32_t tmem;
     uint32_t there[8];                                   // of the last tiles: which groups of eight positions are there
     int      poison[8];                                  // of the last stretches: a V tile that some rows see in part holds values that are not finite
@@ -174,6 +176,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
         for (int i = 0; i < 8; ++i) { mbar_init(full + 8 * i, 1); mbar_init(empty + 8 * i, 1); mbar_init(clean + 8 * i, 2); sh.poison[i] = 0; }
         for (int i = 0; i < 4; ++i) { mbar_init(q_ready + 8 * i, 1); mbar_init(q_free + 8 * i, 1); mbar_init(p_ready + 8 * i, 4); }
         for (int t = 0; t < 2; ++t) { mbar_init(s_ready + 8 * t, 1); mbar_init(s_free + 8 * t, 4); mbar_init(o_ready + 8 * t, 1); mbar_init(p_free + 8 * t, 1); mbar_init(joined + 8 * t, 4); }
+        mbar_init(smem_u32(&sh.over), 1);
         for (int i = 0; i < PT_ENTRIES; ++i) { mbar_init(known + 8 * i, 1); mbar_init(read + 8 * i, PT_READERS); }
         mbar_init_fence();
     }
@@ -469,7 +472,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
             constexpr int halves = HD / 64;                                                 // a tile's boxes are 64 elements wide
             const int group = lane % 16 * 8, half = lane >> 4;                              // this lane's eight positions of a tile, and half
             const bool issues = (group & (box - 1)) == 0 && half < halves;
-            uint32_t tiles = 0;
+            uint32_t copies = 0;
             walk.seq = walk.at.seq; walk.head = walk.at.head; walk.tile = walk.at.tile; walk.off = walk.at.off;
             walk.q = paged_seq(p.view, walk.seq);
             auto put = [&](const Entry &e) {
@@ -496,28 +499,30 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
 #pragma unroll
                     for (int kv = 0; kv < 2; ++kv) {
                         wait_for(empty + 8 * slot, phase ^ 1, limit);
+                        if (!__all_sync(0xffffffffu, limit != 0)) { limit = 0; break; }
                         const uint32_t bar = full + 8 * slot, dst = ring + slot * Shape::OPERAND;
                         if (lane == 0) {
-                            if (kv == 0) { *reinterpret_cast<volatile uint32_t *>(&sh.there[tiles & 7]) = there; }
+                            if (kv == 0) { *reinterpret_cast<volatile uint32_t *>(&sh.there[copies / 2 & 7]) = there; }
                             mbar_expect_tx(bar, Shape::OPERAND);
                         }
                         __syncwarp();
                         if (issues) { tma_load(dst + half * PT_HALF + group * 128, kv == 0 ? &k_map : &v_map, bar, half * 64, token, e.head, page); }
                         __syncwarp();
                         advance();
+                        ++copies;
                     }
-                    ++tiles;
+                    if (limit == 0) { break; }
                 }
                 if (!walk.next(p, e.todo)) { break; }
             }
             Entry over = {};
             put(over);
             if (limit == 0) {   // something gave up: what is on its way lands before the CTA ends
-                uint64_t again = wait_limit;
-                for (int i = 0; i < SLOTS; ++i) {
+                uint64_t again = PT_LANDING_NS;
+                for (uint32_t i = 0; i < SLOTS && i < copies; ++i) {
                     if (slot == 0) { slot = SLOTS; phase ^= 1; }
                     --slot;
-                    if (2 * tiles > (uint32_t)i) { wait_for(full + 8 * slot, phase, again); }
+                    wait_for(full + 8 * slot, phase, again);
                 }
             }
         } else if (warp >= 10) {
@@ -530,6 +535,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
                 if (t == 0 ? a.to > a.from : b.to > b.from) {
                     const uint32_t buffer = q_count % Shape::Q_BUFFERS, bar = 16 * t + 8 * buffer;
                     wait_for(q_free + bar, (q_count / Shape::Q_BUFFERS & 1) ^ 1, limit);
+                    if (!__all_sync(0xffffffffu, limit != 0)) { limit = 0; break; }
                     ++q_count;
                     // whole tokens, token by token their heads: what lies behind the sequence's rows is other sequences' or nothing, and goes nowhere
                     if (elect_one()) {
@@ -587,7 +593,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
             }
             if (limit == 0 && q_count > 0) {   // (something gave up: what is on its way lands before the CTA ends)
                 for (uint32_t i = 1; i <= Shape::Q_BUFFERS && i <= q_count; ++i) {
-                    uint64_t again = wait_limit;
+                    uint64_t again = PT_LANDING_NS;
                     const uint32_t n = q_count - i;
                     wait_for(q_ready + 16 * t + 8 * (n % Shape::Q_BUFFERS), n / Shape::Q_BUFFERS & 1, again);
                 }
@@ -675,6 +681,12 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
                     __syncwarp();
                     if (ahead) { advance(); }
                 }
+            }
+            if (limit == 0) {   // (something gave up: what was issued is done before the CTA ends)
+                if (elect_one()) { mma_commit(smem_u32(&sh.over)); }
+                __syncwarp();
+                uint64_t again = PT_LANDING_NS;
+                wait_for(smem_u32(&sh.over), 0, again);
             }
         }
     }

@@ -333,7 +333,7 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(const __grid_cons
                 }
             }
             if (!ok) {   // reported; what is on its way lands first, or is given a last chance to
-                for (int q = 0; q < SA_PIECES; ++q) { if (min(q * piece, whole) < whole) { mbar_wait_bounded(smem_u32(sh.arrived + q), 0, p.wait_limit); } }
+                for (int q = 0; q < SA_PIECES; ++q) { if (min(q * piece, whole) < whole) { mbar_wait_bounded(smem_u32(sh.arrived + q), 0, 1000000000); } }
                 if (lane == 0 && p.error_flag != nullptr) { atomicExch(p.error_flag, 1); }
             }
             if (whole < x.n && tid == (whole / 4) % SA_THREADS) {

@@ -723,3 +723,70 @@ def test_model_decode_sampled_refuses(tmp_models):
     assert m.decode_sampled(5, 0, 3, temperature=0.0)[0].tolist() == m.decode(5, 0, 3)[0].tolist()
     m.close()
     b.close()
+
+
+# ---------------------------------------------------------------------------------------------- far pages, several backends
+@pytest.mark.parametrize("hd,h", [(128, 2), (64, 4), (96, 2)])
+def test_pages_beyond_32_bits(be, dev, hd, h):
+    """Elements more than 2^32 behind the pool's first: the same bits as with pages side by side."""
+    import torch
+
+    rng = np.random.default_rng(hd)
+    n, page, far = 40, 16, (1 << 31) + 64
+    pool = Pool(rng, [n], 1, hd, page)
+    pool.table[0, :3] = [2, 0, 1]
+    x = rng.standard_normal((n, (h + 2) * hd)).astype(np.float32)
+    q = rng.standard_normal((n, h, hd)).astype(np.float16)
+    store = torch.full((2 * far + (1 << 18),), 3.0, dtype=torch.float16, device="cuda")
+    torch.cuda.synchronize()
+    px, pq, pt, pk, pv = dev(x), dev(q), dev(pool.table[:, :3].copy()), dev(np.full(3 * page * hd, 3, np.float16)), dev(np.full(3 * page * hd, 3, np.float16))
+    near = B.paged_cache(pk, pv, 3, page, 1, hd)
+    base = store.data_ptr()
+    got = []
+    for c in (near, B.paged_cache(base, base + (1 << 18), 3, page, 1, hd, strides=(far, hd, page * hd))):
+        batch = B.paged_batch(dev(np.array([0, n], np.int32)), dev(np.array([n], np.int32)), pt, 1, n, 3)
+        turned = dev(np.zeros((n, h, hd), np.float16))
+        be.paged_append(B.paged_append_desc(c, batch, px, px + 4 * h * hd, px + 4 * (h + 1) * hd, turned, h, row_stride=(h + 2) * hd))
+        out = np.zeros((n + 1, h, hd), np.float32)
+        po = dev(out)
+        be.paged_attention(B.paged_attention_desc(c, batch, pq, po, h, out_type=B.FP32))
+        one = B.paged_batch(dev(np.array([0, 1], np.int32)), dev(np.array([n], np.int32)), pt, 1, 1, 3)
+        be.paged_attention(B.paged_attention_desc(c, one, pq, po + 4 * n * h * hd, h, out_type=B.FP32))
+        got.append(dev.back(po, out))
+    assert got[0].any(axis=(1, 2)).all() and np.array_equal(got[0].view(np.uint32), got[1].view(np.uint32))
+    k = np.empty(3 * page * hd, np.float16)
+    assert np.array_equal(store[2 * far:2 * far + page * hd].cpu().numpy(), dev.back(pk, k)[2 * page * hd:])
+
+
+def test_two_backends_at_once(dev):
+    import threading
+
+    rng = np.random.default_rng(9)
+    pool = Pool(rng, [700, 60, 3000], 2, 128, 16)
+    for s, n in enumerate((700, 60, 3000)):
+        pool.put(s, *rng.standard_normal((2, n, 2, 128)).astype(np.float16))
+    q = rng.standard_normal((141, 8, 128)).astype(np.float16)
+    x = rng.standard_normal((5, 40000)).astype(np.float32)
+    results = [None] * 3
+
+    def work(i):
+        b = B.B200Backend(0)
+        d = Device(b)
+        batch = B.paged_batch(d(np.array([0, 130, 140, 141], np.int32)), d(np.array([700, 60, 3000], np.int32)), d(pool.table), 3, 141, pool.table.shape[1])
+        po, ids = d(np.zeros(q.shape, np.float16)), d(np.zeros(5, np.int32))
+        attention = B.paged_attention_desc(pool.cache(d(pool.k), d(pool.v)), batch, d(q), po, 8)
+        sample = B.sample_desc(d(x), B.FP32, 5, 40000, ids, uniform=d(np.linspace(0, 0.9, 5).astype(np.float32)), top_p=d(np.full(5, 0.9, np.float32)))
+        for _ in range(100):
+            b.paged_attention(attention)
+            b.sample(sample)
+        results[i] = (d.back(po, np.zeros(q.shape, np.float16)), d.back(ids, np.zeros(5, np.int32)))
+        d.free()
+        b.close()
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    work(2)
+    assert all(np.array_equal(r[0], results[2][0]) and np.array_equal(r[1], results[2][1]) for r in results[:2])
