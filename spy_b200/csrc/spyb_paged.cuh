@@ -35,7 +35,7 @@ struct PagedAttention {
     unsigned    *arrived = nullptr;       // [CTAs], zero between launches
 };
 int         paged_cut_selftest();   // host-only: 0 when the CTAs' pieces cover every item once, on any lengths
-cudaError_t launch_paged_append(const PagedAppend &p, int in_type, int q_out_type, const LaunchCfg &cfg);
+cudaError_t launch_paged_append(const PagedAppend &p, int in_type, int q_out_type, int sms, const LaunchCfg &cfg);
 cudaError_t launch_paged_attention_rows(const PagedAttention &p, int head_dim, int row_tiles, int sms, const LaunchCfg &cfg);
 // the kernel on tensor memory; false where it does not take these pages, heads or strides (nothing is launched then)
 bool        launch_paged_attention_tc(const PagedAttention &p, int head_dim, int n_head, int sms, const LaunchCfg &cfg, uint64_t wait_limit, cudaError_t *err);
