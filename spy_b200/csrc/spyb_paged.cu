@@ -17,8 +17,8 @@ namespace {
 // Memory bound: every element is read once and written once, (4 + 2) or (2 + 2) bytes. A CTA has one row; a thread has eight elements of a head - a 16-byte piece of
 // the output, or half of two pieces where the pairs are halves - in every 8th or 16th head, so that its (up to) four angles are made once a row. Angles are
 // position x share of a circle in 64 bits, reduced to half a turn either way: in f32 a position of 100 000 leaves an angle 0.004 of uncertainty.
-// Measured: 8900 rows of 120 heads of 128 elements (f32, 852 MB) 155 us, 5.5 TB/s; one row 3.7 us and 96 rows 6 to 8 us, a launch and a chain of four dependent loads
-// (whose row, which position, which page, the row itself).
+// Measured: 9246 rows of 120 heads of 128 elements (f32, 852 MB) 149 us, 5.7 TB/s; one row 3.5 us and 96 rows 6 to 7 us, a launch and a chain of dependent loads
+// (whose row, which position, which page), beside which the row's first elements come.
 constexpr int AP_THREADS = 256;
 
 __device__ __forceinline__ int sequence_of(const PagedView &v, int row) {   // the last s with row_start[s] <= row, by a whole warp; -1 and n_seq: nobody's
