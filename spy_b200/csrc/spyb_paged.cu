@@ -409,7 +409,7 @@ __global__ void __launch_bounds__(PR_WARPS * 32) paged_rows_kernel(const __grid_
         // What is known of this item; the next one's copies start before its findings are joined, where these have a place of their own
         const int done = packed, done_tile = tile, done_row0 = q.row0, done_head = head;
         const PagedCut cut = paged_cut(at, at.unit - off, it.units);
-        at.unit += todo;
+        at.unit += todo + p.start_units;
         off = 0;
         const bool more = at.unit < at.end && paged_next(p, true, q, seq, head, tile), early = done <= RowsSmem<HD, MT>::EARLY;
         if (more) { describe(); }
@@ -510,7 +510,7 @@ cudaError_t launch_rows_as(const PagedAttention &p, int sms, const LaunchCfg &cf
 template <int HD, int MT>
 cudaError_t launch_rows(PagedAttention p, int sms, const LaunchCfg &cfg) {
     const int page = p.view.page_size;
-    p.page_shift = -1;
+    p.page_shift = -1; p.start_units = PA_START;
     for (int s = 0; s < 31; ++s) { if (page == 1 << s) { p.page_shift = s; } }
     if constexpr (HD <= 64) {
         if (page % PR_BLOCK == 0) { return launch_rows_as<HD, MT, true>(p, sms, cfg); }
@@ -627,6 +627,7 @@ template <int UNIT, int ALIGN> static int cut_selftest(uint32_t seed, int tile_r
         p.view.row_start = start.data(); p.view.n_kv = kv.data(); p.view.n_seq = n_seq; p.view.n_rows = std::max(1, start[n_seq] - rnd(2)); p.view.page_size = 1 + rnd(40);
         p.view.table_stride = 1 + rnd(80); p.view.n_kv_most = p.view.table_stride * p.view.page_size;
         p.n_head_kv = 1 + rnd(5); p.group = 1 + rnd(8); p.tile_rows = tile_rows > 0 ? tile_rows : 2 * (128 / p.group) * p.group; p.causal = rnd(4) != 0; p.window = p.causal && rnd(2) ? 1 + rnd(500) : 0; p.few_rows = rnd(3) == 0 ? 1 << 30 : rnd(40);
+        p.start_units = rnd(2) * rnd(5);
         const int grid = 1 + rnd(300), least = 1 + rnd(4);
         for (int few = 0; few < 2; ++few) {
             PagedPlace at = {};
@@ -635,7 +636,7 @@ template <int UNIT, int ALIGN> static int cut_selftest(uint32_t seed, int tile_r
             if (total == 0) { continue; }
             const int ctas = paged_ctas(total, grid, least);
             at.share = paged_share(total, ctas);
-            std::vector<uint8_t> seen((size_t)total), place((size_t)2 * ctas);
+            std::vector<uint8_t> seen((size_t)total), real((size_t)total), place((size_t)2 * ctas);
             std::vector<int> arrived(ctas), wanted(ctas);
             for (int c = 0; c < ctas; ++c) {
                 at.unit = paged_cta_unit(at.share, c); at.end = paged_cta_unit(at.share, c + 1);
@@ -649,8 +650,11 @@ template <int UNIT, int ALIGN> static int cut_selftest(uint32_t seed, int tile_r
                     rest -= n;
                 }
                 PagedSeq q = paged_seq(p.view, s);
-                int head, tile, off;
-                paged_find<UNIT, ALIGN>(p, q, paged_seq_units<UNIT, ALIGN>(p, s, few), rest, head, tile, off);
+                int head, tile;
+                paged_find<UNIT, ALIGN>(p, q, paged_seq_units<UNIT, ALIGN>(p, s, few), rest, head, tile, at.off);
+                paged_begin(p, at);
+                if (at.unit >= at.end) { continue; }
+                int off = at.off;
                 for (;;) {
                     const PagedItem it = paged_item<UNIT, ALIGN>(p, q, tile);
                     if (q.row0 < 0 || q.rows < 1 || q.row0 + q.rows > p.view.n_rows || head >= p.n_head_kv || tile * p.tile_rows >= q.rows * p.group) { return 3; }
@@ -663,14 +667,22 @@ template <int UNIT, int ALIGN> static int cut_selftest(uint32_t seed, int tile_r
                         if ((c == cut.c0) != (off == 0)) { return 7; }
                         ++arrived[cut.c0]; wanted[cut.c0] = cut.parts;
                     }
+                    if (at.unit - off + it.units > total) { return 12; }
+                    for (int u = 0; u < it.units; ++u) { real[(size_t)(at.unit - off + u)] = 1; }
                     for (int u = 0; u < todo; ++u) { if (seen[(size_t)(at.unit + u)]++) { return 8; } }
-                    at.unit += todo;
+                    at.unit += todo + p.start_units;
                     if (at.unit >= at.end) { break; }
                     off = 0;
                     if (!paged_next(p, few, q, s, head, tile)) { return 9; }
                 }
             }
-            for (uint8_t x : seen) { if (x != 1) { return 10; } }
+            int64_t items = 0, work = 0;
+            for (int s = 0; s < n_seq; ++s) {
+                const PagedSeq q = paged_seq(p.view, s);
+                if (paged_mine(p, q, few)) { items += (int64_t)((q.rows * p.group + p.tile_rows - 1) / p.tile_rows) * p.n_head_kv; }
+            }
+            for (size_t u = 0; u < seen.size(); ++u) { work += seen[u]; if (seen[u] != real[u]) { return 10; } }
+            if (work != total - items * p.start_units) { return 13; }
             for (int c = 0; c < ctas; ++c) { if (arrived[c] != wanted[c]) { return 11; } }
         }
     }

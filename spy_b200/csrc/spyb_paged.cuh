@@ -30,6 +30,7 @@ struct PagedAttention {
     float        scale_log2 = 0.f;        // scale * log2(e): probabilities are powers of two
     int          tile_rows = 16;          // rows of a tile, counting every query head of its K/V head
     int          page_shift = -1;         // log2 of the page size, if it is a power of two
+    int          start_units = 0;         // what going on to an item costs beside its units, in units (PA_START)
     int          few_rows = 0;            // sequences of up to so many rows (of all query heads of a K/V head) are the small kernel's
     float       *partial = nullptr;       // [CTAs][2][rows of a tile][head_dim + 2]
     unsigned    *arrived = nullptr;       // [CTAs], zero between launches
@@ -48,6 +49,12 @@ constexpr int PA_FEW_ROWS = 16;
 // The rows of a sequence that share a K/V head - token by token, its query heads side by side - are cut into tiles; a tile and a K/V head are an item, and the
 // positions that its rows see are counted in units of UNIT. All units of a call, item after item, are cut evenly among the CTAs: whatever the
 // lengths are, every SM has the same to read, and one long sequence uses the whole chip. An item on a cut is joined by the CTA that is done with it last.
+// A CTA that goes on from one item to the next loses the time of some units (its findings go out, the next item's Q and first block come): an item counts PA_START units
+// more than it has. Without them the CTAs with two pieces of items end 10 us behind the others. Small kernel, of 64 positions, none / 1 / 2 / 4: 64 single tokens of up to
+// 4096 positions 103.1 / 97.8 / 91.3 / 92.8 us, heads of 64 65.1 / 61.9 / 53.5 / 53.4, 16 of up to 8000 64.0 / 53.3 / 51.0 / 50.4, 100 of up to 300 - / - / 27.5 / 29.0.
+// Tensor memory, of 128: 24 x 5 rows of up to 9000 117.5 / 109.7 / 110.6 / 113.2, 512 rows at 3968 54.7 / 53.1 / 52.2 / 52.4, prompts of 6 under a window
+// 225.8 / 209.0 / 211.3 / 218.9, 512 at 1024 34.5 / 27.3 / 28.4 / 30.0.
+constexpr int PA_START = 2;
 struct PagedSeq { int row0, rows, first, kv; };   // first row and number of rows, position of the first row, positions that are there
 struct PagedItem { int lo, hi, units; };          // positions [lo, hi) that some row of the tile sees (lo a multiple of ALIGN)
 
@@ -77,7 +84,7 @@ __host__ __device__ __forceinline__ int64_t paged_seq_units(const PagedAttention
     if (!paged_mine(p, q, few)) { return 0; }
     const int tiles = (q.rows * p.group + p.tile_rows - 1) / p.tile_rows;
     int64_t n = 0;
-    for (int t = first; t < tiles; t += step) { n += paged_item<UNIT, ALIGN>(p, q, t).units; }
+    for (int t = first; t < tiles; t += step) { n += paged_item<UNIT, ALIGN>(p, q, t).units + p.start_units; }
     return n;
 }
 
@@ -89,11 +96,11 @@ template <int UNIT, int ALIGN>
 __host__ __device__ __forceinline__ void paged_find(const PagedAttention &p, const PagedSeq &q, int64_t one, int64_t rest, int &head, int &tile, int &off) {
     head = (int)paged_div(rest, one); rest -= head * one;
     for (tile = 0;; ++tile) {
-        const int u = paged_item<UNIT, ALIGN>(p, q, tile).units;
+        const int u = paged_item<UNIT, ALIGN>(p, q, tile).units + p.start_units;
         if (rest < u) { break; }
         rest -= u;
     }
-    off = (int)rest;
+    off = (int)rest;                                      // (of the item with its beginning)
 }
 
 // All units cut into `ctas` stretches, the first `longer` of them one longer than the others
@@ -108,6 +115,12 @@ __host__ __device__ __forceinline__ int paged_unit_cta(const PagedShare &s, int6
     return u < head ? (int)paged_div(u, s.each + 1) : s.longer + (int)paged_div(u - head, s.each);
 }
 struct PagedPlace { PagedShare share; int seq, head, tile, off; int64_t unit, end; };   // where a CTA begins, its first unit and the one behind its last
+// A CTA's stretch begins at a unit that is work: beginnings of items, which are counted but nobody's, are stepped over (in the middle of a stretch by whoever goes on to the
+// next item). A stretch of nothing else is empty.
+__host__ __device__ __forceinline__ void paged_begin(const PagedAttention &p, PagedPlace &at) {
+    at.unit += pmax(0, p.start_units - at.off);
+    at.off = pmax(0, at.off - p.start_units);
+}
 struct PagedPlanShared { int64_t warp[32], one, rest; int seq; };
 __host__ __device__ __forceinline__ int paged_ctas(int64_t total, int grid, int least) { const int64_t n = paged_div(total, least); return n < 1 ? 1 : n < grid ? (int)n : grid; }
 
@@ -171,7 +184,7 @@ __device__ PagedPlace paged_plan(const PagedAttention &p, bool few, int least, P
     const PagedSeq q = paged_seq(p.view, at.seq);
     const int tiles = (q.rows * p.group + p.tile_rows - 1) / p.tile_rows;
     for (int base = 0; base < tiles; base += 32) {       // 32 tiles at a time, every warp for itself
-        const int u = base + lane < tiles ? paged_item<UNIT, ALIGN>(p, q, base + lane).units : 0;
+        const int u = base + lane < tiles ? paged_item<UNIT, ALIGN>(p, q, base + lane).units + p.start_units : 0;
         int upto = u;
         for (int o = 1; o < 32; o <<= 1) { const int v = __shfl_up_sync(0xffffffffu, upto, o); if (lane >= o) { upto += v; } }
         const unsigned hit = __ballot_sync(0xffffffffu, rest < upto);
@@ -183,6 +196,7 @@ __device__ PagedPlace paged_plan(const PagedAttention &p, bool few, int least, P
         }
         rest -= __shfl_sync(0xffffffffu, upto, 31);
     }
+    paged_begin(p, at);
     return at;
 }
 

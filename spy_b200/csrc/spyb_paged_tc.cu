@@ -153,7 +153,7 @@ struct Walker {                                      // the copying warp's place
         return e;
     }
     __device__ __forceinline__ bool next(const PagedAttention &p, int todo) {
-        at.unit += todo;
+        at.unit += todo + p.start_units;
         if (at.unit >= at.end) { return false; }
         off = 0;
         return paged_next(p, false, q, seq, head, tile);
@@ -183,8 +183,8 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
     pdl_launch_dependents();
     pdl_wait();
     Walker walk;
-    // (at least two steps a CTA: 512 tokens at 512 positions 21.7 us, against 24.9 from one step on and 29.1 from four; 4 x 20 rows at 700 positions 23.4, 25.6, 28.3)
-    walk.at = paged_plan<PT_THREADS, PT_KEYS, PT_KEYS>(p, false, 2, sh.plan);
+    // (at least four units a CTA, items' beginnings among them: 512 tokens at 512 positions 20.8 us, 23.8 from two on; 4 x 20 rows at 700 positions 24.5 and 22.8)
+    walk.at = paged_plan<PT_THREADS, PT_KEYS, PT_KEYS>(p, false, 4, sh.plan);
     if (walk.at.unit >= walk.at.end) { return; }
     if (warp == 8) { asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&sh.tmem)) : "memory"); }
     tc_fence_before();
@@ -761,6 +761,7 @@ bool launch_paged_attention_tc(const PagedAttention &given, int head_dim, int n_
     if ((head_dim != 64 && head_dim != 128) || box < 8 || given.group > PT_ROWS || least <= 0 || most >= (1ll << 38)) { return false; }
     PagedAttention p = given;
     p.tile_rows = 2 * (PT_ROWS / p.group) * p.group;
+    p.start_units = PA_START;
     CUtensorMap q, k, v;
     if (!query_map(&q, p, n_head, head_dim) || !page_map(&k, p.k, p.view, p.n_head_kv, head_dim, box) || !page_map(&v, p.v, p.view, p.n_head_kv, head_dim, box)) { return false; }
     *err = head_dim == 128 ? launch_tc<128>(p, q, k, v, box, sms, cfg, wait_limit) : launch_tc<64>(p, q, k, v, box, sms, cfg, wait_limit);
