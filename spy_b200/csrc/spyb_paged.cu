@@ -479,15 +479,30 @@ __global__ void __launch_bounds__(PR_WARPS * 32) paged_rows_kernel(const __grid_
                     const int r = x / (HD / 4), c = (x - r * (HD / 4)) * 4;
                     float m = -CUDART_INF_F, l = 0.f;
                     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-                    for (int i = 0; i < cut.parts; ++i) { m = fmaxf(m, __ldcg(p.partial + paged_slot(cut.c0 + i, cut.c0) * PART + TILE * HD + r)); }
-                    const float base = m == -CUDART_INF_F ? 0.f : m;
-#pragma unroll 4
-                    for (int i = 0; i < cut.parts; ++i) {
-                        const float *from = p.partial + paged_slot(cut.c0 + i, cut.c0) * PART;
-                        const float f = ex2(__ldcg(from + TILE * HD + r) - base);
-                        const float4 u = __ldcg(reinterpret_cast<const float4 *>(from + r * HD + c));
-                        v.x += f * u.x; v.y += f * u.y; v.z += f * u.z; v.w += f * u.w;
-                        l += f * __ldcg(from + TILE * HD + TILE + r);
+                    // eight CTAs' findings are in flight together; what came before is scaled to the new maximum
+#pragma unroll 1
+                    for (int i0 = 0; i0 < cut.parts; i0 += 8) {
+                        float  pm[8], pl[8], top = m;
+                        float4 u[8];
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) {
+                            const bool is = i0 + j < cut.parts;
+                            const float *from = p.partial + paged_slot(cut.c0 + (is ? i0 + j : 0), cut.c0) * PART;
+                            pm[j] = is ? __ldcg(from + TILE * HD + r) : -CUDART_INF_F;
+                            pl[j] = is ? __ldcg(from + TILE * HD + TILE + r) : 0.f;
+                            u[j] = is ? __ldcg(reinterpret_cast<const float4 *>(from + r * HD + c)) : make_float4(0.f, 0.f, 0.f, 0.f);
+                        }
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) { top = fmaxf(top, pm[j]); }
+                        const float base = top == -CUDART_INF_F ? 0.f : top, before = ex2(m - base);
+                        m = top; l *= before;
+                        v = make_float4(v.x * before, v.y * before, v.z * before, v.w * before);
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) {
+                            const float f = ex2(pm[j] - base);
+                            v.x += f * u[j].x; v.y += f * u[j].y; v.z += f * u[j].z; v.w += f * u[j].w;
+                            l += f * pl[j];
+                        }
                     }
                     const float inv = l == 0.f ? 0.f : 1.f / l;
                     put(r, c, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
