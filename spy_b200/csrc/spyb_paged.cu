@@ -123,10 +123,10 @@ __global__ void __launch_bounds__(AP_THREADS) paged_append_kernel(const __grid_c
 // asynchronous copies, scores and values by mma.sync on up to 32 rows, a running maximum and sum in registers - and the warps of a CTA, then the CTAs
 // of an item are joined at the end. The maximum that probabilities are taken against follows the true one only when that is 2^8 above it: the
 // accumulators are hardly ever rescaled, and p <= 2^8 is as exact in fp16 as p <= 1.
-// Measured: three sequences of 100 000 positions, 40 query heads on 8 of 128 elements (1.2 GB) 191 us, 6.3 TB/s; 64 sequences of up to 4096, 32 on 8: 103 us, 5.3 TB/s,
-// heads of 64: 65 us, 4.2 TB/s; one of 4000, 32 on 32 (66 MB): 21 us. What is above the memory's time: some 6 us until the first block is there (lengths, the plan, the
-// page table, the block, one after the other), the join of items on a cut (3 to 4 us), and each warp's chain of copy, scores, powers and values with eight to
-// twelve warps an SM.
+// Measured: three sequences of 100 000 positions, 40 query heads on 8 of 128 elements (1.2 GB) 192 to 199 us, 6.1 to 6.3 TB/s; 64 sequences of up to 4096, 32 on 8: 91 us,
+// 6.0 TB/s, heads of 64: 54 us, 5.1 TB/s; one of 4000, 32 on 32 (66 MB): 19.7 us. What is above the memory's time: some 6 us until the first block is there (lengths, the
+// plan, the page table, the block, one after the other), the join of items on a cut (2 to 3 us), and each warp's chain of copy, scores, powers and values with
+// eight to twelve warps an SM.
 constexpr int PR_WARPS = 4, PR_BLOCK = 16, PR_UNIT = PR_WARPS * PR_BLOCK;
 
 __device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
@@ -155,7 +155,7 @@ template <int HD> struct RowsShape {
 };
 template <int HD, int MT> struct RowsSmem {       // the ring; what the warps found: beside it for up to EARLY rows, in its place for more; the masks of the ring's stages
     static constexpr int EARLY = MT == 1 ? 8 : 0, FOUND = PR_WARPS * 16 * MT * (HD + 2) * 4, RING = RowsShape<HD>::RING > FOUND ? RowsShape<HD>::RING : FOUND;
-    static constexpr int CTAS = MT == 1 && HD <= 64 ? 3 : 2;         // of an SM (64 single tokens, heads of 64: 65 us with three, 79 with two; longer heads' rings leave room for two)
+    static constexpr int CTAS = MT == 1 && HD <= 64 ? 3 : 2;         // of an SM (64 single tokens, heads of 64, before the cut counted items' beginnings: 65 us with three, 79 with two; longer heads' rings leave room for two)
     static constexpr int MASKS = RING + PR_WARPS * EARLY * (HD + 2) * 4, BYTES = MASKS + PR_WARPS * RowsShape<HD>::STAGES * 4;
 };
 // IN_PAGE: a block's positions lie in one page (pages of a multiple of 16), heads of up to 64: 64 single tokens 64.8 us against 66.6. (Longer heads' blocks take longer than

@@ -10,10 +10,10 @@
 //   warp 9           copies                                                   warps 10, 11  clear and check the V tiles that not all rows see whole
 // Probabilities are taken against a maximum that follows the true one when that is 2^8 above it: O is rescaled in the first steps and hardly ever after.
 // Measured (heads of 128): 8192 tokens of a prompt, 32 heads, 570 us, 965 TFLOP/s of the 1640 of a matrix product; 512 tokens at 32 768 positions 281 us, 970;
-// 1500 at 9111, 40 heads, 247 us, 1040; 512 at 3968 55 us, 577; five tokens of 24 sequences of up to 9000, 119 us, 3.9 TB/s. Heads of 64 have half the
+// 1500 at 9111, 40 heads, 247 us, 1040; 512 at 3968 52 to 55 us, 595; five tokens of 24 sequences of up to 9000, 111 us, 4.2 TB/s. Heads of 64 have half the
 // products for as many powers: 8192 tokens 524 us, 524 TFLOP/s. A step of 256 rows and 128 positions takes 2.4 us, in which 16 powers a clock alone take 1.1; the chain of
 // a tile - S, reading it, maximum, powers, P, product - is what bounds it, two tiles hide each other's. Beside the steps: 7 us until the first (lengths, the plan, page
-// table, Q and K), some 4 us from one stretch to the next and for the join of an item on a cut, which is what holds short contexts back (512 tokens at 1024: 35 us).
+// table, Q and K), 5 us from one stretch to the next and 6 for the join of an item on a cut, which is what holds short contexts back (512 tokens at 1024: 28 us).
 // Tried and left out: powers by polynomials on the FMA units for some of the columns (slower: their instructions are what is short), the two tiles taking turns by
 // barriers (no gain), both tiles on one tile's rows by every second step where only one has rows (24 x 5 rows 122 us against 119: memory bounds those steps).
 
