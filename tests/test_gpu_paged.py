@@ -126,10 +126,11 @@ def run_attention(be, dev, pool, row_start, q, out0, **kw):
     return got
 
 
-def check_attention(be, dev, rng, rows, n_kv, h, h_kv, hd, page, causal=True, window=0, scale=0.0, out=np.float16, token_major=False, pad=0, spread=1.0, max_rows=0, drop=None, strides=None):
+def check_attention(be, dev, rng, rows, n_kv, h, h_kv, hd, page, causal=True, window=0, scale=0.0, out=np.float16, token_major=False, pad=0, spread=1.0, max_rows=0, drop=None, strides=None, share=0):
     pool = Pool(rng, n_kv, h_kv, hd, page, token_major, strides)
     for s, n in enumerate(n_kv):
         pool.put(s, *(rng.standard_normal((2, max(0, n), h_kv, hd)).astype(np.float16)))
+    pool.table[1:, :share] = pool.table[0, :share]             # (a common beginning)
     if drop is not None:
         pool.table[rng.random(pool.table.shape) < drop] = -1
         pool.table[rng.random(pool.table.shape) < drop / 2] = pool.n_pages + 5
@@ -726,6 +727,13 @@ def test_model_decode_sampled_refuses(tmp_models):
 
 
 # ---------------------------------------------------------------------------------------------- far pages, several backends
+@pytest.mark.parametrize("hd", [64, 96, 128])
+def test_sequences_that_share_pages(be, dev, hd):
+    rng = np.random.default_rng(hd + 1)
+    check_attention(be, dev, rng, [1, 1, 1, 1], [200, 130, 64, 300], 4, 2, hd, 16, share=4, max_rows=1)
+    check_attention(be, dev, rng, [150, 1, 40, 7], [200, 130, 104, 300], 4, 2, hd, 16, share=4)
+
+
 @pytest.mark.parametrize("hd,h", [(128, 2), (64, 4), (96, 2)])
 def test_pages_beyond_32_bits(be, dev, hd, h):
     """Elements more than 2^32 behind the pool's first: the same bits as with pages side by side."""
