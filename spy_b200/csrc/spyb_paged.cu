@@ -2,6 +2,7 @@
 // head dimensions without a tensor-memory kernel), and the entry points of both operators.
 
 #include <algorithm>
+#include <climits>
 #include <cmath>
 #include <vector>
 
@@ -643,6 +644,8 @@ template <int UNIT, int ALIGN> static int cut_selftest(uint32_t seed, int tile_r
         p.view.table_stride = 1 + rnd(80); p.view.n_kv_most = p.view.table_stride * p.view.page_size;
         p.n_head_kv = 1 + rnd(5); p.group = 1 + rnd(8); p.tile_rows = tile_rows > 0 ? tile_rows : 2 * (128 / p.group) * p.group; p.causal = rnd(4) != 0; p.window = p.causal && rnd(2) ? 1 + rnd(500) : 0; p.few_rows = rnd(3) == 0 ? 1 << 30 : rnd(40);
         p.start_units = rnd(2) * rnd(5);
+        const bool all_seen = p.window > 0 && turn % 4 == 1;   // a window as long as an int can say is none
+        if (all_seen) { p.window = paged_window(INT_MAX - rnd(3)); }
         const int grid = 1 + rnd(300), least = 1 + rnd(4);
         for (int few = 0; few < 2; ++few) {
             PagedPlace at = {};
@@ -673,6 +676,7 @@ template <int UNIT, int ALIGN> static int cut_selftest(uint32_t seed, int tile_r
                 for (;;) {
                     const PagedItem it = paged_item<UNIT, ALIGN>(p, q, tile);
                     if (q.row0 < 0 || q.rows < 1 || q.row0 + q.rows > p.view.n_rows || head >= p.n_head_kv || tile * p.tile_rows >= q.rows * p.group) { return 3; }
+                    if (all_seen && it.lo != 0) { return 14; }
                     if (it.lo < 0 || it.lo % ALIGN != 0 || it.hi > p.view.n_kv_most || off >= it.units || (int64_t)it.units * UNIT + it.lo < it.hi) { return 4; }
                     const int todo = (int)std::min<int64_t>(it.units - off, at.end - at.unit);
                     const PagedCut cut = paged_cut(at, at.unit - off, it.units);
@@ -764,7 +768,7 @@ spyb_status spyb_paged_attention(spyb_backend *be, const spyb_paged_attention_de
     p.q = static_cast<const __half *>(d->q); p.out = d->out;
     p.k = static_cast<const __half *>(d->cache.k); p.v = static_cast<const __half *>(d->cache.v);
     p.q_stride = d->q_stride; p.out_stride = d->out_stride; p.n_head_kv = d->cache.n_head_kv; p.group = d->n_head / d->cache.n_head_kv;
-    p.causal = d->causal != 0; p.window = d->window; p.out_f32 = d->out_type == SPYB_FP32;
+    p.causal = d->causal != 0; p.window = paged_window(d->window); p.out_f32 = d->out_type == SPYB_FP32;
     const float scale = d->scale == 0.f ? 1.0f / std::sqrt((float)hd) : d->scale;
     p.scale_log2 = (float)((double)scale * 1.4426950408889634073599);
     p.partial = be->paged_partial; p.arrived = be->paged_arrived;

@@ -60,6 +60,8 @@ struct PagedItem { int lo, hi, units; };          // positions [lo, hi) that som
 
 __host__ __device__ __forceinline__ int pmin(int a, int b) { return a < b ? a : b; }
 __host__ __device__ __forceinline__ int pmax(int a, int b) { return a < b ? b : a; }
+// Positions are below 2^30: a window of as many hides nothing, and a position minus a window stays in 32 bits also for rows in front of position 0
+inline int paged_window(int window) { return pmin(window, 1 << 30); }
 __host__ __device__ __forceinline__ PagedSeq paged_seq(const PagedView &v, int s) {
     const int a = pmax(0, pmin(v.row_start[s], v.n_rows)), end = pmax(a, pmin(v.row_start[s + 1], 1 << 24)), b = pmin(end, v.n_rows);
     const int kv = pmin(pmax(0, v.n_kv[s]), 1 << 30);

@@ -798,3 +798,13 @@ def test_two_backends_at_once(dev):
         t.join()
     work(2)
     assert all(np.array_equal(r[0], results[2][0]) and np.array_equal(r[1], results[2][1]) for r in results[:2])
+
+
+# ---------------------------------------------------------------------------------------------- what the descriptors allow at their ends
+@pytest.mark.parametrize("rows", [5, 8, 150])
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 30 + 5, 2 ** 30])
+def test_windows_as_long_as_an_int_can_say(be, dev, rows, window):
+    """Rows in front of position 0 beside a window that hides nothing: the rows behind see all of their past."""
+    rng = np.random.default_rng(rows)
+    check_attention(be, dev, rng, [rows, 1, rows], [2, 300, rows - 4], 4, 2, 64, 16, window=window)
+    check_attention(be, dev, rng, [rows], [rows // 2], 4, 4, 128, 16, window=window)
