@@ -1176,7 +1176,7 @@ spyb_status spyb_model_eval(spyb_model *m, const int32_t *tokens, int32_t n_toke
     if (m == nullptr || tokens == nullptr || n_tokens < 1) { return SPYB_FAIL; }
     spyb_backend *be = m->be;
     cudaSetDevice(be->config.device_id);
-    if (n_past < 0 || n_past + n_tokens > m->info.n_ctx) { be->set_error("the number of tokens exceeds the context length (%d + %d > %d)", n_past, n_tokens, m->info.n_ctx); return SPYB_FAIL; }
+    if (n_past < 0 || n_tokens > m->info.n_ctx - n_past) { be->set_error("the number of tokens exceeds the context length (%d + %d > %d)", n_past, n_tokens, m->info.n_ctx); return SPYB_FAIL; }
     for (int i = 0; i < n_tokens; ++i) { if (tokens[i] < 0 || tokens[i] >= m->info.n_vocab) { be->set_error("token id %d out of range", tokens[i]); return SPYB_FAIL; } }
     int64_t launches = 0;
     if (n_tokens == 1 && be->config.use_graph != 0 && (m->info.tp_size == 1 || std::getenv("SPYB_TP_NO_GRAPH") == nullptr)) {
@@ -1493,7 +1493,7 @@ spyb_status decode(spyb_model *m, int32_t first_token, int32_t n_past, int32_t n
     if (m == nullptr || n_steps < 1 || ids_host == nullptr) { return SPYB_FAIL; }
     spyb_backend *be = m->be;
     cudaSetDevice(be->config.device_id);
-    if (n_past < 0 || n_past + n_steps > m->info.n_ctx) { be->set_error("decode would exceed the context length (%d + %d > %d)", n_past, n_steps, m->info.n_ctx); return SPYB_FAIL; }
+    if (n_past < 0 || n_steps > m->info.n_ctx - n_past) { be->set_error("decode would exceed the context length (%d + %d > %d)", n_past, n_steps, m->info.n_ctx); return SPYB_FAIL; }
     if (first_token < 0 || first_token >= m->info.n_vocab) { be->set_error("token id %d out of range", first_token); return SPYB_FAIL; }
     spyb_sample_desc draw;
     if (how != nullptr) {
@@ -1548,7 +1548,7 @@ spyb_status decode_batch(spyb_model *m, const int32_t *first_tokens, int32_t n_s
     spyb_backend *be = m->be;
     cudaSetDevice(be->config.device_id);
     if (n_seq < 1 || n_seq > m->n_seq || m->logits_batch == nullptr) { be->set_error("decode_batch: %d sequences, %d prepared by spyb_model_set_sequences", n_seq, m->n_seq); return SPYB_FAIL; }
-    if (n_past < 0 || n_past + n_steps > m->info.n_ctx) { be->set_error("decode would exceed the context length (%d + %d > %d)", n_past, n_steps, m->info.n_ctx); return SPYB_FAIL; }
+    if (n_past < 0 || n_steps > m->info.n_ctx - n_past) { be->set_error("decode would exceed the context length (%d + %d > %d)", n_past, n_steps, m->info.n_ctx); return SPYB_FAIL; }
     for (int c = 0; c < n_seq; ++c) { if (first_tokens[c] < 0 || first_tokens[c] >= m->info.n_vocab) { be->set_error("token id %d out of range", first_tokens[c]); return SPYB_FAIL; } }
     const int64_t need = (int64_t)n_steps * n_seq;
     if (need > m->batch_ids_cap) {

@@ -808,3 +808,26 @@ def test_windows_as_long_as_an_int_can_say(be, dev, rows, window):
     rng = np.random.default_rng(rows)
     check_attention(be, dev, rng, [rows, 1, rows], [2, 300, rows - 4], 4, 2, 64, 16, window=window)
     check_attention(be, dev, rng, [rows], [rows // 2], 4, 4, 128, 16, window=window)
+
+
+def test_numbers_of_steps_beyond_32_bits_are_refused(tmp_models):
+    """n_past + n_steps that leaves 32 bits is beyond the context too."""
+    path = str(tmp_models / "sampled0.gguf")
+    sampled_model(path)
+    b = B.B200Backend(0)
+    m = B.LlamaModel(b, path, n_ctx=32)
+    m.set_sequences(2)
+    most, ids, first = 2 ** 31 - 1, np.zeros(8, np.int32), np.array([1, 2], np.int32)
+    how, keep = B.LlamaModel._sampling(1, 1, None, 1.0, None, None, None)
+    i, f = B._np_ptr(ids), B._np_ptr(first)
+    for past in (1, 32, most):
+        assert b._l.spyb_model_decode(m.h, 5, past, most, i, None) != B.SUCCESS
+        assert b._l.spyb_model_decode_sampled(m.h, 5, past, most, B.C.byref(how), i, None) != B.SUCCESS
+        assert b._l.spyb_model_decode_batch(m.h, f, 2, past, most, i, None) != B.SUCCESS
+        assert b._l.spyb_model_decode_batch_sampled(m.h, f, 2, past, most, B.C.byref(how), i, None) != B.SUCCESS
+        assert b._l.spyb_model_eval(m.h, f, most, past, None) != B.SUCCESS
+    with pytest.raises(B.SpybError):
+        m.decode(5, 31, 2)
+    assert m.decode_sampled(5, 31, 1, temperature=0.0)[0].tolist() == m.decode(5, 31, 1)[0].tolist()
+    m.close()
+    b.close()
