@@ -103,7 +103,7 @@ struct SampleShared {
 //   p + p' = x c, by FMA; A = largest c in 64 bits, A = a + a' with a a multiple of 2^-14; r = round(1024 (a - p));
 //   f = (a - r / 1024) - p: the first difference is exact (multiples of 2^-14 below 2^10), the second too (|f| <= 2^-11); e = a' - p'.
 // 2^-(r / 1024) is a table's 2^46-fold and a shift, 2^-(f + e) = 1 + y with |y| < 2^-11.5, y to 2^-36 in f32.
-// Where |A| is too large for that (1000 and more: tiny temperatures, huge logits), the same in 64 bits.
+// Where |A| is too large for that (1000 and more: tiny temperatures, huge logits), or c itself for f32, the same in 64 bits.
 struct Weight {
     const uint64_t *table;      // 2^46 2^-(j / 1024)
     float  c_hi, c_lo, a_hi, a_lo;
@@ -114,7 +114,7 @@ struct Weight {
     __device__ __forceinline__ void set(const uint64_t *powers, float top, double scale, double edge, int bits) {   // edge: 56 / c (2^-56 is no unit: rounds to nothing)
         table = powers; c = scale; largest = top; shift = 46 - bits;
         const double a = largest * c, lowest = largest - edge;
-        wide = !(fabs(a) < 960.0 && lowest > -3.4e38);
+        wide = !(fabs(a) < 960.0 && lowest > -3.4e38 && c > 1e-30 && c < 1e30);
         least = wide ? 0.f : (float)lowest;
         c_hi = (float)c; c_lo = (float)(c - c_hi);
         a_hi = (float)(rint(a * 16384.0) * (1.0 / 16384)); a_lo = (float)(a - a_hi);
@@ -297,10 +297,10 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(const __grid_cons
 
     *reinterpret_cast<uint4 *>(sh.table + 2 * tid) = powers;
     if (tid == SA_THREADS - 1) {
-        const double c = fmax(fmin(1.4426950408889634073599 / (double)temp, 1e30), 1e-30);
+        const double c = 1.4426950408889634073599 / (double)temp;      // (4e-39 to 1e45, or 0)
         sh.c = c; sh.edge = 56 / c;
         sh.least = min_p > 0.f ? (uint64_t)max(1.0, ceil((double)fminf(min_p, 1.f) * __hiloint2double((1023 + p.frac_bits) << 20, 0))) : 1;
-        sh.bin_scale = (float)(c * (SA_BINS / (double)(p.frac_bits + 1)));
+        sh.bin_scale = (float)fmin(c * (2 * SA_BINS / (double)(p.frac_bits + 1)), 3e38);   // of halves (cut: bins hold more than they should, and the slow search decides)
     }
     // this thread's largest (of the elements that Slice::each gives it), the row's, and where that is
     float own = -CUDART_INF_F, from_here = CUDART_INF_F;      // (top-k: nothing below from_here is among the k largest)
@@ -407,7 +407,8 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(const __grid_cons
     weight.set(sh.table, largest, sh.c, sh.edge, p.frac_bits);
     const uint64_t least = sh.least;
     const float    bin_scale = sh.bin_scale;
-    auto bin_of = [&](float v) { return (largest - v) * bin_scale; };        // not below SA_BINS (or NaN): no weight
+    const float half_largest = 0.5f * largest;
+    auto bin_of = [&](float v) { return fmaf(v, -0.5f, half_largest) * bin_scale; };   // not below SA_BINS (or NaN): no weight (halves: a difference may leave f32)
     auto reach = [&](uint64_t total) { return max((uint64_t)1, (uint64_t)ceil((double)max(top_p, 0.f) * (double)total)); };   // a token stays while less than this is in front of it
     uint64_t cut = 0;                        // keys from here on stay
     bool     search = false;                 // ... by the slow way

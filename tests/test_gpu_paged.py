@@ -831,3 +831,16 @@ def test_numbers_of_steps_beyond_32_bits_are_refused(tmp_models):
     assert m.decode_sampled(5, 31, 1, temperature=0.0)[0].tolist() == m.decode(5, 31, 1)[0].tolist()
     m.close()
     b.close()
+
+
+@pytest.mark.parametrize("t", [1.5e-45, 1e-38, 3e-31, 1e-20, 1e20, 1e31, 3e38, np.inf])
+def test_sample_temperatures_of_all_sizes(be, dev, t):
+    """Logits as many times smaller or larger: weights are those of logit / temperature at ordinary sizes."""
+    rng = np.random.default_rng(17)
+    n, v = 6, 700
+    scale = min(max(t, 2.0 ** -149), 1e38)
+    x = np.clip(scale * np.clip(2 * rng.standard_normal((n, v)), -3.3, 3.3), -3.3e38, 3.3e38).astype(np.float32)
+    x[0, ::3] = -np.inf
+    u = (0.05 + 0.9 * rng.random(n)).astype(np.float32)
+    for extra in ({}, {"k": 5}, {"k": 300}, {"k": 650, "p": 0.9}, {"p": 0.3}, {"p": 0.95}, {"least": 0.1}):
+        check_sample(be, dev, x, t=t, u=u, **extra)
