@@ -304,7 +304,8 @@ spyb_status spyb_paged_attention(spyb_backend *backend, const spyb_paged_attenti
  *   top_k   (0 < top_k < n_vocab): the top_k largest logits stay, the lowest indices among equals
  *   top_p   (< 1): of these, in descending order, those in front of which less than top_p of their sum lies (never fewer than one)
  *   min_p   (> 0): of these, those with w_i >= min_p
- *   the token is the first index, ascending, up to which the weights that stayed sum to more than uniform[row] (in [0, 1)) times their sum.
+ *   the token is the first index, ascending, up to which the weights that stayed sum to more than uniform[row] (in [0, 1)) times their sum: at 0 the first
+ *   whose weight is not 0 in 64 bits, however small
  * NaN and -inf are never drawn; where there is +inf, only +inf has weight, all the same. ids[row] = -1, probs[row] = 0 where there is nothing to draw.
  * probs (optional): the token's share of the weights that stayed. n_vocab at most 2^20. uniform NULL reads as zeros. */
 typedef struct {

@@ -20,7 +20,7 @@ namespace {
 //                     threshold has at least k logits above it. Threads whose maximum reaches it give theirs to the first CTA, which ranks them and does the rest
 //   top-p alone       a histogram of all distances (counts) brackets the bin in which top_p is reached (a bin is 0.031 wide, its weights are known to 1.6 %);
 //                     one pass of weights gives the sums around the bracket and a second histogram inside it, and the elements of its one bin are sorted
-//   draw              one pass of the weights that stayed; the warp on whose stretch the number falls walks it again
+//   draw              one pass of the weights that stayed; the warp on whose stretch the number falls walks it again. Numbers below 2^-20: see SA_FINE
 // Candidates that do not fit a list (ties by the thousand, a top_k of thousands) take a binary search over (logit, index): slow, and as right.
 // Measured: 192 rows of 128 000 f32 logits (98 MB: 15 us of memory) greedy 36 us, top-k with the other settings 75, temperature alone 98, settings that differ by row
 // 134; one row of 32 000: 4.9, 11.7, 8.6. Two CTAs an SM are all that their slices leave room for, so 192 rows go in five to six waves, and a wave takes as long as a
@@ -251,6 +251,104 @@ __device__ __forceinline__ uint64_t of_total(float share, uint64_t total) {   //
     return min((uint64_t)((double)(share > 0.f ? share : 0.f) * (double)total), total - 1);
 }
 
+// Uniform numbers below SA_FINE fall among weights that are no unit, down to what 64 bits hold: at 0 on the first index whose weight is not 0 there. Such rows - one in a
+// million of evenly spread numbers - are drawn by weights in floating point of 64 bits. What stays is found as ever, but for min_p, which is asked of these weights.
+// (A function of its own, and its exponential too: the registers of what runs for all other rows stay theirs.)
+constexpr float SA_FINE = 1.f / (1 << 20);
+__device__ __noinline__ double fine_weight(float x, float largest, float temp) {
+    if (x == -CUDART_INF_F) { return 0.0; }
+    const double z = ((double)x - (double)largest) / (double)temp;
+    if (z > -700) { return exp(z); }
+    const double half = exp(0.5 * z);
+    return half * half;                                   // (exp may be off by a step, and 0 in place of the smallest numbers; a product is rounded)
+}
+__device__ __forceinline__ double fine_upto(double v) {   // inclusive sums over the lanes
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) { const double u = __shfl_up_sync(0xffffffffu, v, o); if (lane >= o) { v += u; } }
+    return v;
+}
+// The list's: weights in the order `by_index`'s entries name them, by one thread
+__device__ __noinline__ void fine_draw_list(const SampleParams &p, int row, const uint64_t *by_index, const uint64_t *weights, int n, float uni) {
+    double total = 0, upto = 0;
+    for (int i = 0; i < n; ++i) { total += __longlong_as_double((long long)weights[(by_index[i] - 1) & 2047]); }
+    const double t = (uni > 0.f ? (double)uni : 0.0) * total;
+    for (int i = 0; i < n; ++i) {
+        const double w = __longlong_as_double((long long)weights[(by_index[i] - 1) & 2047]);
+        upto += w;
+        if (upto > t || i == n - 1) {
+            p.ids[row] = (1 << SA_INDEX_BITS) - 1 - (int)((by_index[i] - 1) >> 11);
+            if (p.probs) { p.probs[row] = (float)(w / total); }
+            return;
+        }
+    }
+}
+// All of the row. Sums of CTAs, of a CTA's warps and of a warp's lanes are not rounded alike: each step takes the first part whose sum passes the number, or the last that has
+// any weight.
+template <class T, bool KEPT>
+__device__ __noinline__ void fine_draw(const SampleParams &p, SampleShared &sh, const Slice<T, KEPT> x, int row, float largest, float temp, float min_p, float uni, float cut_value, int cut_index, uint32_t rank, uint32_t ctas) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int stretch = ((x.n + SA_WARPS - 1) / SA_WARPS + 127) & ~127, from = min(warp * stretch, x.n), to = min(from + stretch, x.n);
+    const double least = min_p > 0.f ? (double)fminf(min_p, 1.f) : 0.0;
+    auto weight = [&](int i) {
+        const float v = i < to ? x(i) : -CUDART_INF_F;
+        if (!(v >= cut_value) || (v == cut_value && x.base + i > cut_index)) { return 0.0; }
+        const double w = fine_weight(v, largest, temp);
+        return w >= least ? w : 0.0;
+    };
+    double s = 0;
+    for (int i = from + lane; i < to; i += 32) { s += weight(i); }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) { s += __shfl_xor_sync(0xffffffffu, s, o); }
+    __syncthreads();
+    if (lane == 0) { sh.scan[warp] = (uint64_t)__double_as_longlong(s); }
+    __syncthreads();
+    double mine = 0;
+    for (int w = 0; w < SA_WARPS; ++w) { mine += __longlong_as_double((long long)sh.scan[w]); }
+    cluster_sync();                                       // (shares of earlier exchanges are read)
+    if (threadIdx.x < ctas) { cluster_store64(cluster_map(smem_u32(sh.share[0] + rank), threadIdx.x), (uint64_t)__double_as_longlong(mine)); }
+    cluster_sync();
+    double total = 0, before = 0;
+    for (uint32_t r = 0; r < ctas; ++r) { total += __longlong_as_double((long long)sh.share[0][r]); }
+    const double t = (uni > 0.f ? (double)uni : 0.0) * total;                 // (below the total, which is 1 at least)
+    uint32_t at = 0;
+    for (;; ++at) {
+        const double next = before + __longlong_as_double((long long)sh.share[0][at]);
+        if (next > t || at == ctas - 1) { break; }
+        before = next;
+    }
+    if (at != rank) { return; }
+    int    who = -1;
+    double start = before;
+    for (int w = 0; w < SA_WARPS; ++w) {
+        const double v = __longlong_as_double((long long)sh.scan[w]);
+        if (v > 0) {
+            who = w; start = before;
+            if (before + v > t) { break; }
+        }
+        before += v;
+    }
+    if (who != warp) { return; }
+    before = start;
+    int    last = -1;
+    double last_w = 0;
+    for (int i0 = from; i0 < to; i0 += 32) {
+        const double   w = weight(i0 + lane), upto = before + fine_upto(w);
+        const unsigned any = __ballot_sync(0xffffffffu, w > 0), hit = __ballot_sync(0xffffffffu, w > 0 && upto > t);
+        if (any) {
+            const int l = hit ? __ffs(hit) - 1 : 31 - __clz(any);
+            last = i0 + l;
+            last_w = __shfl_sync(0xffffffffu, w, l);
+            if (hit) { break; }
+        }
+        before = __shfl_sync(0xffffffffu, upto, 31);
+    }
+    if (lane == 0 && last >= 0) {
+        p.ids[row] = x.base + last;
+        if (p.probs) { p.probs[row] = (float)(last_w / total); }
+    }
+}
+
 template <class T, bool KEPT>
 __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(const __grid_constant__ SampleParams p) {
     extern __shared__ __align__(16) uint8_t dynamic[];
@@ -405,6 +503,7 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(const __grid_cons
     }
     Weight weight;
     weight.set(sh.table, largest, sh.c, sh.edge, p.frac_bits);
+    const bool     fine = !(uni >= SA_FINE);
     const uint64_t least = sh.least;
     const float    bin_scale = sh.bin_scale;
     const float half_largest = 0.5f * largest;
@@ -505,13 +604,14 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(const __grid_cons
             }
             __syncthreads();
             const float behind = (float)(sh.found + 1);
-            if (sh.found2 <= SA_LIST) { n = gather_one_by_one([&](float v) { return bin_of(v) < behind; }); }
+            // (a drawing to the bottom asks for what has no unit, too, and so is in no bin)
+            if (sh.found2 <= SA_LIST && !(fine && all < (uint64_t)top_k)) { n = gather_one_by_one([&](float v) { return bin_of(v) < behind; }); }
         }
         if (n <= SA_LIST) {
             if (rank != 0) { return; }
             // everything else is the first CTA's
             const int n_list = (int)n;
-            if (n_list <= SA_RANKED) {
+            if (n_list <= SA_RANKED && !fine) {
                 // few candidates: a group of threads ranks each, by counting and weighing what is in front of it - first in the order of weights, then of indices
                 int per = 512 / SA_RANKED;
                 while (per < 32 && n_list * per * 2 <= SA_THREADS) { per *= 2; }
@@ -556,7 +656,12 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(const __grid_cons
             if (2 * tid + 1 < n1) { k1 = candidates[2 * tid + 1]; w1 = weight(value_of(k1)); }
             const uint64_t up = block_upto(w0 + w1, sh.scan, &all_w);
             const uint64_t stop = by_p ? reach(all_w) : ~0ull;
-            const bool in0 = 2 * tid < n1 && up - w1 - w0 < stop && w0 >= least, in1 = 2 * tid + 1 < n1 && up - w1 < stop && w1 >= least;
+            bool in0 = 2 * tid < n1 && up - w1 - w0 < stop, in1 = 2 * tid + 1 < n1 && up - w1 < stop;
+            if (fine) {
+                const double floor = min_p > 0.f ? (double)fminf(min_p, 1.f) : 0.0, d0 = in0 ? fine_weight(value_of(k0), largest, temp) : 0.0, d1 = in1 ? fine_weight(value_of(k1), largest, temp) : 0.0;
+                in0 = d0 > 0 && d0 >= floor; in1 = d1 > 0 && d1 >= floor;
+                w0 = (uint64_t)__double_as_longlong(d0); w1 = (uint64_t)__double_as_longlong(d1);
+            } else { in0 = in0 && w0 >= least; in1 = in1 && w1 >= least; }
             const uint64_t kept = block_sum((in0 ? 1 : 0) + (in1 ? 1 : 0), sh.scan);          // (a prefix of the list)
             const uint64_t sum = block_sum((in0 ? w0 : 0) + (in1 ? w1 : 0), sh.scan);
             // by index: the key's low bits, ascending as descending complements; the weights are found again from their place in the sorted list
@@ -566,6 +671,10 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(const __grid_cons
             if (in0) { by_index[2 * tid] = ((k0 & low) << 11 | (2 * tid)) + 1; weights[2 * tid] = w0; }
             if (in1) { by_index[2 * tid + 1] = ((k1 & low) << 11 | (2 * tid + 1)) + 1; weights[2 * tid + 1] = w1; }
             sort_list(by_index, (int)kept);
+            if (fine) {
+                if (tid == 0) { fine_draw_list(p, row, by_index, weights, (int)kept, uni); }
+                return;
+            }
             uint64_t v0 = 0, v1 = 0, p0 = 0, p1 = 0, ignore;
             if (2 * tid < (int)kept) { p0 = by_index[2 * tid] - 1; v0 = weights[p0 & 2047]; }
             if (2 * tid + 1 < (int)kept) { p1 = by_index[2 * tid + 1] - 1; v1 = weights[p1 & 2047]; }
@@ -682,6 +791,7 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(const __grid_cons
     const int stretch = ((x.n + SA_WARPS - 1) / SA_WARPS + 127) & ~127, from = min(warp * stretch, x.n), to = min(from + stretch, x.n);
     const float cut_value = cut == 0 ? -CUDART_INF_F : value_of(cut);
     const int   cut_index = cut == 0 ? p.n_vocab : index_of(cut);
+    if (fine) { fine_draw<T, KEPT>(p, sh, x, row, largest, temp, min_p, uni, cut_value, cut_index, rank, ctas); return; }
     auto stays = [&](float v, int i, uint64_t w) {
         return v >= cut_value && !(v == cut_value && x.base + i > cut_index) && w >= least ? w : (uint64_t)0;
     };

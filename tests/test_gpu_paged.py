@@ -844,3 +844,44 @@ def test_sample_temperatures_of_all_sizes(be, dev, t):
     u = (0.05 + 0.9 * rng.random(n)).astype(np.float32)
     for extra in ({}, {"k": 5}, {"k": 300}, {"k": 650, "p": 0.9}, {"p": 0.3}, {"p": 0.95}, {"least": 0.1}):
         check_sample(be, dev, x, t=t, u=u, **extra)
+
+
+def check_low(be, dev, x, u, t, **settings):
+    """check_sample for numbers near 0: shares down to the smallest that 64 bits hold, rounded to f32."""
+    n, v = x.shape
+    ids, probs = np.zeros(n, dtype=np.int32), np.zeros(n, dtype=np.float32)
+    pi, pp = dev(ids), dev(probs)
+    types = {"top_k": np.int32}
+    host = {m: np.broadcast_to(np.asarray(a, dtype=types.get(m, np.float32)), (n,)).copy() for m, a in dict(settings, temperature=t).items()}
+    pu = None if u is None else dev(np.broadcast_to(np.float32(u), (n,)).copy())
+    be.sample(B.sample_desc(dev(x), B.FP32 if x.dtype == np.float32 else B.FP16, n, v, pi, probs=pp, uniform=pu, **{m: dev(a) for m, a in host.items()}))
+    got_i, got_p = dev.back(pi, ids), dev.back(pp, probs)
+    full = dict({"top_k": np.zeros(n, int), "top_p": np.ones(n), "min_p": np.zeros(n)}, **host)
+    for r in range(n):
+        want = plain_sample(x[r], full["temperature"][r], full["top_k"][r], full["top_p"][r], full["min_p"][r], np.float32(u or 0))
+        assert got_i[r] == want[0], (r, got_i[r], want, u, settings)
+        assert abs(got_p[r] - want[1]) <= 2.0 ** -23 * want[1] + 2.0 ** -150          # (half a step of the smallest f32)
+
+
+@pytest.mark.parametrize("v,dtype", [(50, np.float32), (3000, np.float16), (32000, np.float32), (50001, np.float16), ((1 << 20) - 5, np.float32)])
+@pytest.mark.parametrize("t", [0.3, 0.5, 1.0, 0.01])
+def test_sample_uniform_numbers_near_zero(be, dev, v, dtype, t):
+    """A number of 0 falls on the first token that has any weight in 64 bits, however small; numbers near it among weights that are no unit of the integers."""
+    rng = np.random.default_rng(v)
+    n = 4 if v < 10 ** 6 else 1
+    x = (3 * rng.standard_normal((n, v))).astype(dtype)
+    x[0, 2:v // 3] -= 40
+    for u in (None, 0.0, -1.0, 1e-30, 1e-12, 1e-9, 3e-8, 2.0 ** -24, 9e-7):
+        for s in ({}, {"top_k": 7}, {"top_k": min(v - 1, 700)}, {"top_k": v // 2, "min_p": 1e-25}, {"top_p": 0.9}, {"top_p": 1 - 2.0 ** -24}, {"min_p": 1e-20}, {"min_p": 1e-5}, {"top_k": 40, "top_p": 0.95, "min_p": 0.01}):
+            if v > 10 ** 6 and (u not in (None, 1e-12) or "top_k" in s and s["top_k"] > 7):
+                continue
+            check_low(be, dev, x, u, t, **s)
+
+
+def test_sample_nothing_but_far_tokens_in_front(be, dev):
+    """Shares of 1e-30 and of nothing in front of the largest; equal tokens; +inf; -inf."""
+    x = np.array([[-600, 0, 1], [-2000, -1000, 0], [-np.inf, -69, 0], [5, 5, 5], [1, np.inf, np.inf], [np.nan, -745, 0]], dtype=np.float32)
+    for u in (None, 0.0, 1e-38, 1e-31, 9e-7):
+        for s in ({}, {"top_k": 2}, {"top_p": 0.5}, {"min_p": 1e-35}, {"min_p": 1.0}):
+            check_low(be, dev, x, u, 1.0, **s)
+            check_low(be, dev, x, u, np.inf, **s)
