@@ -224,6 +224,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
             float m = -CUDART_INF_F, l = 0.f;
             const Tile own = en.half[t];
             const int token = (2 * en.tile + t) * half_tokens + row_token, pos = en.first + token;   // (of rows that are there)
+            const bool mine = row < own.rows;                 // others hold what was there before, or another sequence's Q: they decide nothing
             for (int step = own.from; step < own.to; ++step) {
                 wait_for(s_ready + 8 * t, s_phase, limit);
                 s_phase ^= 1;
@@ -288,7 +289,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
                         for (int e = 0; e < 4; ++e) { tops[e] = max3(tops[e], __uint_as_float(s[c + 2 * e]), __uint_as_float(s[c + 2 * e + 1])); }
                     }
                     const float top = fmaxf(max3(tops[0], tops[1], tops[2]), tops[3]) * scale;
-                    if (__any_sync(0xffffffffu, top > m + 8.f)) {
+                    if (__any_sync(0xffffffffu, mine && top > m + 8.f)) {
                         const float to = fmaxf(m, top), f = to == m ? 1.f : exp2_fast(m - to);
                         m = to; l *= f;
                         if (step != own.from) {
@@ -320,7 +321,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
             }
             tiles += en.end - en.begin;
             // this stretch's findings
-            const bool any = own.to > own.from, mine = row < own.rows;      // (rows behind the last whole token are nobody's)
+            const bool any = own.to > own.from;
             const int  parts = en.parts, c0 = en.c0;
             if (any) { wait_for(o_ready + 8 * t, o_phase, limit); o_phase ^= 1; tc_fence_after(); }
             float4 *part = reinterpret_cast<float4 *>(p.partial) + (paged_slot(blockIdx.x, c0) * 2 + t) * (PT_ROWS * (HD + 2) / 4);     // [HD / 4][128] x 4, [128], [128]

@@ -885,3 +885,42 @@ def test_sample_nothing_but_far_tokens_in_front(be, dev):
         for s in ({}, {"top_k": 2}, {"top_p": 0.5}, {"min_p": 1e-35}, {"min_p": 1.0}):
             check_low(be, dev, x, u, 1.0, **s)
             check_low(be, dev, x, u, np.inf, **s)
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("group", [3, 5, 12])
+def test_rows_of_nobody_decide_nothing(be, dev, hd, group):
+    """The same bits whatever an earlier kernel left in shared memory (a tile of 128 rows holds whole tokens: groups of 5 leave three rows over), and whatever Q the padding and
+    the other sequences have."""
+    rng = np.random.default_rng(hd + group)
+    rows, n_kv = [130, 9, 61], [900, 400, 61]
+    pool = Pool(rng, n_kv, 1, hd, 16, fill=0.0)
+    for s, n in enumerate(n_kv):
+        pool.put(s, *rng.standard_normal((2, n, 1, hd)).astype(np.float16))
+    starts = np.concatenate([[0], np.cumsum(rows)]).astype(np.int32)
+    q = rng.standard_normal((starts[-1] + 40, group, hd)).astype(np.float16)
+    c, pt, pn, ps = pool.cache(dev(pool.k), dev(pool.v)), dev(pool.table), dev(np.array(n_kv, np.int32)), dev(starts)
+    out = np.zeros(q.shape, np.float32)
+
+    def run(q):
+        po = dev(out)
+        be.paged_attention(B.paged_attention_desc(c, B.paged_batch(ps, pn, pt, 3, len(q), pool.table.shape[1]), dev(q), po, group, out_type=B.FP32))
+        return dev.back(po, out).view(np.uint32)
+
+    def leave(size):                                         # full tiles of 128 rows with scores of all sizes, in every CTA and buffer
+        big = np.full((4096, 4, hd), size, np.float16) * rng.choice([-1, 1], (4096, 4, hd)).astype(np.float16)
+        b = B.paged_batch(dev(np.array([0, 4096], np.int32)), dev(np.array([900], np.int32)), pt, 1, 4096, pool.table.shape[1])
+        be.paged_attention(B.paged_attention_desc(c, b, dev(big), dev(np.zeros(big.shape, np.float16)), 4, causal=False))
+
+    leave(0.0)
+    first = run(q)
+    for size in (1.0, 30.0, 3000.0):
+        leave(size)
+        assert np.array_equal(run(q)[:starts[-1]], first[:starts[-1]]), size
+    for size in (0.0, 30.0, 3000.0):
+        other = q.copy()
+        other[starts[1]:] = size * rng.standard_normal(other[starts[1]:].shape)
+        assert np.array_equal(run(other)[:starts[1]], first[:starts[1]]), size
+        other[starts[2]:] = q[starts[2]:]
+        other[starts[3]:] = size
+        assert np.array_equal(run(other)[starts[2]:starts[3]], first[starts[2]:starts[3]]), size
