@@ -127,6 +127,7 @@ def lib():
         "spyb_paged_append": (i32, [vp, C.POINTER(PagedAppendDesc)]),
         "spyb_paged_attention": (i32, [vp, C.POINTER(PagedAttentionDesc)]),
         "spyb_sample": (i32, [vp, C.POINTER(SampleDesc)]),
+        "spyb_paged_selftest_late": (i32, [vp, i32, u64, C.POINTER(i32)]),
         "spyb_paged_append_check": (i32, [C.POINTER(PagedAppendDesc), C.c_char_p, i32]),
         "spyb_paged_attention_check": (i32, [C.POINTER(PagedAttentionDesc), C.c_char_p, i32]),
         "spyb_sample_check": (i32, [C.POINTER(SampleDesc), C.c_char_p, i32]),
@@ -354,6 +355,12 @@ class B200Backend:
         st = self._paged_attention(self.h, C.byref(desc))
         if st != SUCCESS:
             self._check(st)
+
+    def paged_selftest_late(self, who: int, limit_ns: int) -> int:
+        """Runs attention over pages with one role of its kernel late (1: the warps that check values, within the limit); returns the error code of the waits."""
+        code = C.c_int32(0)
+        self._check(self._l.spyb_paged_selftest_late(self.h, who, limit_ns, C.byref(code)))
+        return int(code.value)
 
     def sample(self, desc: SampleDesc) -> None:
         """The next token of every row of logits."""

@@ -4,6 +4,7 @@
 #include <algorithm>
 #include <climits>
 #include <cmath>
+#include <cstring>
 #include <vector>
 
 #include <math_constants.h>
@@ -718,6 +719,39 @@ int paged_cut_selftest() {
 
 using namespace spyb;
 
+// The public call, and with a role that is late the self-checks'
+static spyb_status paged_attention(spyb_backend *be, const spyb_paged_attention_desc &desc, int late, uint64_t wait_limit) {
+    const spyb_paged_attention_desc *d = &desc;
+    Refusal no;
+    if (check_attention(no, *d) != SPYB_SUCCESS) { be->set_error("%s", no.text); return SPYB_UNSUPPORTED; }
+    if (d->batch.n_seq == 0 || d->batch.n_rows == 0) { return SPYB_SUCCESS; }
+    use_device(be->config.device_id);
+    if (!be->paged_workspace()) { return SPYB_FAIL; }
+    const int hd = d->cache.head_dim;
+    PagedAttention p;
+    p.view = view_of(d->cache, d->batch);
+    p.q = static_cast<const __half *>(d->q); p.out = d->out;
+    p.k = static_cast<const __half *>(d->cache.k); p.v = static_cast<const __half *>(d->cache.v);
+    p.q_stride = d->q_stride; p.out_stride = d->out_stride; p.n_head_kv = d->cache.n_head_kv; p.group = d->n_head / d->cache.n_head_kv;
+    p.causal = d->causal != 0; p.window = paged_window(d->window); p.out_f32 = d->out_type == SPYB_FP32;
+    const float scale = d->scale == 0.f ? 1.0f / std::sqrt((float)hd) : d->scale;
+    p.scale_log2 = (float)((double)scale * 1.4426950408889634073599);
+    p.late = late; p.partial = be->paged_partial; p.arrived = be->paged_arrived;
+    const int64_t most = (int64_t)(d->batch.max_rows > 0 ? std::min(d->batch.max_rows, d->batch.n_rows) : d->batch.n_rows) * p.group;
+    const LaunchCfg cfg = be->launch_cfg(be->config.use_pdl != 0);
+    p.few_rows = 1 << 30;
+    if (most > PA_FEW_ROWS && scale >= 0.f) {
+        cudaError_t err = cudaSuccess;
+        p.few_rows = p.view.n_seq == 1 ? 0 : PA_FEW_ROWS;
+        if (!launch_paged_attention_tc(p, hd, d->n_head, be->num_sms_total, cfg, wait_limit, &err)) { p.few_rows = 1 << 30; }
+        SPYB_CUDA(be, err);
+    }
+    const int row_tiles = std::min<int64_t>(most, p.few_rows) <= 16 ? 1 : 2;
+    p.tile_rows = 16 * row_tiles;
+    if (p.few_rows > 0) { SPYB_CUDA(be, launch_paged_attention_rows(p, hd, row_tiles, be->num_sms_total, cfg)); }
+    return SPYB_SUCCESS;
+}
+
 extern "C" {
 
 spyb_status spyb_paged_append_check(const spyb_paged_append_desc *d, char *message, int32_t size) {
@@ -756,34 +790,56 @@ spyb_status spyb_paged_append(spyb_backend *be, const spyb_paged_append_desc *d)
 }
 
 spyb_status spyb_paged_attention(spyb_backend *be, const spyb_paged_attention_desc *d) {
-    if (be == nullptr || d == nullptr) { return SPYB_FAIL; }
-    Refusal no;
-    if (check_attention(no, *d) != SPYB_SUCCESS) { be->set_error("%s", no.text); return SPYB_UNSUPPORTED; }
-    if (d->batch.n_seq == 0 || d->batch.n_rows == 0) { return SPYB_SUCCESS; }
+    return be == nullptr || d == nullptr ? SPYB_FAIL : paged_attention(be, *d, PA_ON_TIME, be->wait_limit_ns);
+}
+
+// Self-check of the tensor-memory kernel's hand-overs: a chunk at the end of a long conversation and a short one, on time and with one of its roles late. A role that is late within
+// the limit of the waits changes nothing.
+spyb_status spyb_paged_selftest_late(spyb_backend *be, int32_t who, uint64_t limit_ns, int32_t *error_code_out) {
+    if (be == nullptr || limit_ns == 0 || who != PA_LATE_CHECKS) { return SPYB_FAIL; }
     use_device(be->config.device_id);
-    if (!be->paged_workspace()) { return SPYB_FAIL; }
-    const int hd = d->cache.head_dim;
-    PagedAttention p;
-    p.view = view_of(d->cache, d->batch);
-    p.q = static_cast<const __half *>(d->q); p.out = d->out;
-    p.k = static_cast<const __half *>(d->cache.k); p.v = static_cast<const __half *>(d->cache.v);
-    p.q_stride = d->q_stride; p.out_stride = d->out_stride; p.n_head_kv = d->cache.n_head_kv; p.group = d->n_head / d->cache.n_head_kv;
-    p.causal = d->causal != 0; p.window = paged_window(d->window); p.out_f32 = d->out_type == SPYB_FP32;
-    const float scale = d->scale == 0.f ? 1.0f / std::sqrt((float)hd) : d->scale;
-    p.scale_log2 = (float)((double)scale * 1.4426950408889634073599);
-    p.partial = be->paged_partial; p.arrived = be->paged_arrived;
-    const int64_t most = (int64_t)(d->batch.max_rows > 0 ? std::min(d->batch.max_rows, d->batch.n_rows) : d->batch.n_rows) * p.group;
-    const LaunchCfg cfg = be->launch_cfg(be->config.use_pdl != 0);
-    p.few_rows = 1 << 30;
-    if (most > PA_FEW_ROWS && scale >= 0.f) {
-        cudaError_t err = cudaSuccess;
-        p.few_rows = p.view.n_seq == 1 ? 0 : PA_FEW_ROWS;
-        if (!launch_paged_attention_tc(p, hd, d->n_head, be->num_sms_total, cfg, be->wait_limit_ns, &err)) { p.few_rows = 1 << 30; }
+    SPYB_CUDA(be, cudaStreamSynchronize(be->stream));
+    if (be->device_error()) { return SPYB_FAIL; }
+    constexpr int heads = 2, group = 3, page = 16, pages = 1300, rows[2] = {300, 70}, kv[2] = {20000, 70}, n_rows = rows[0] + rows[1];
+    const int32_t words[5] = {0, rows[0], n_rows, kv[0], kv[1]};
+    std::vector<int32_t> table(2 * pages);
+    for (int i = 0; i < 2 * pages; ++i) { table[i] = i % pages; }
+    int code = 0;
+    for (const int hd : {64, 128}) {
+        const size_t n_pool = (size_t)pages * page * heads * hd, n_q = (size_t)n_rows * heads * group * hd;
+        std::vector<uint16_t> host(2 * n_pool + n_q);
+        uint32_t seed = 1;
+        for (uint16_t &x : host) { seed = seed * 1664525u + 1013904223u; x = (uint16_t)(0x3000 + (seed >> 18) % 0x0c00 + (seed & 0x80000000u ? 0x8000 : 0)); }   // 0.125 to 1, either sign
+        std::vector<float> want(n_q), got(n_q);
+        uint8_t *mem = nullptr;
+        const size_t at_out = host.size() * 2, at_words = at_out + n_q * 4, at_table = at_words + sizeof words, size = at_table + table.size() * 4;
+        SPYB_CUDA(be, cudaMalloc(&mem, size));
+        spyb_paged_attention_desc d = {};
+        d.cache.k = mem; d.cache.v = mem + n_pool * 2; d.cache.number_type = SPYB_FP16; d.cache.n_pages = pages; d.cache.page_size = page; d.cache.n_head_kv = heads; d.cache.head_dim = hd;
+        d.cache.page_stride = page * heads * hd; d.cache.token_stride = heads * hd; d.cache.head_stride = hd;
+        d.batch.row_start = reinterpret_cast<int32_t *>(mem + at_words); d.batch.n_kv = d.batch.row_start + 3; d.batch.page_table = reinterpret_cast<int32_t *>(mem + at_table);
+        d.batch.n_seq = 2; d.batch.n_rows = n_rows; d.batch.table_stride = pages;
+        d.q = mem + n_pool * 4; d.out = mem + at_out; d.q_stride = d.out_stride = heads * group * hd; d.n_head = heads * group; d.out_type = SPYB_FP32; d.causal = 1;
+        cudaError_t err = upload(mem, host.data(), host.size() * 2);
+        if (err == cudaSuccess) { err = upload(mem + at_words, words, sizeof words); }
+        if (err == cudaSuccess) { err = upload(mem + at_table, table.data(), table.size() * 4); }
+        spyb_status st = SPYB_SUCCESS;
+        auto run = [&](int late, uint64_t limit, std::vector<float> &to) {
+            if (err == cudaSuccess) { err = cudaMemsetAsync(d.out, 0xff, n_q * 4, be->stream); }
+            if (err == cudaSuccess && st == SPYB_SUCCESS) { st = paged_attention(be, d, late, limit); }
+            if (err == cudaSuccess) { err = cudaMemcpyAsync(to.data(), d.out, n_q * 4, cudaMemcpyDeviceToHost, be->stream); }
+            if (err == cudaSuccess) { err = cudaStreamSynchronize(be->stream); }   // returns: the kernels ended by themselves
+            return be->clear_device_error();
+        };
+        const int before = run(PA_ON_TIME, be->wait_limit_ns, want);
+        if (before == 0) { code = run(who, limit_ns, got); }
+        cudaFree(mem);
         SPYB_CUDA(be, err);
+        if (st != SPYB_SUCCESS) { return st; }
+        if (error_code_out != nullptr) { *error_code_out = before != 0 ? before : code; }
+        if (before != 0 || code != 0) { be->set_error("paged selftest: heads of %d: a wait gave up (code %d)", hd, before != 0 ? before : code); return SPYB_FAIL; }
+        if (std::memcmp(want.data(), got.data(), n_q * 4) != 0) { be->set_error("paged selftest: heads of %d: a late role changed the output", hd); return SPYB_FAIL; }
     }
-    const int row_tiles = std::min<int64_t>(most, p.few_rows) <= 16 ? 1 : 2;
-    p.tile_rows = 16 * row_tiles;
-    if (p.few_rows > 0) { SPYB_CUDA(be, launch_paged_attention_rows(p, hd, row_tiles, be->num_sms_total, cfg)); }
     return SPYB_SUCCESS;
 }
 

@@ -21,6 +21,7 @@ struct PagedAppend {
     int          n_head = 0, n_head_kv = 0, head_dim = 0, rot = 0, halves = 0;
     double       turns[128] = {};         // pair i turns by this share of a full circle a position
 };
+enum PagedLate { PA_ON_TIME = 0, PA_LATE_CHECKS = 1 };   // the warps that check V stay a few microseconds behind everything else
 struct PagedAttention {
     PagedView    view;
     const __half *q = nullptr, *k = nullptr, *v = nullptr;
@@ -34,6 +35,7 @@ struct PagedAttention {
     int          few_rows = 0;            // sequences of up to so many rows (of all query heads of a K/V head) are the small kernel's
     float       *partial = nullptr;       // [CTAs][2][rows of a tile][head_dim + 2]
     unsigned    *arrived = nullptr;       // [CTAs], zero between launches
+    int          late = PA_ON_TIME;       // self-checks of the tensor-memory kernel
 };
 int         paged_cut_selftest();   // host-only: 0 when the CTAs' pieces cover every item once, on any lengths
 cudaError_t launch_paged_append(const PagedAppend &p, int in_type, int q_out_type, int sms, const LaunchCfg &cfg);

@@ -64,7 +64,7 @@ struct Entry {
 constexpr uint64_t PT_LANDING_NS = 1000000000;       // when a wait gave up: what is on its way has this long to land (whatever the limit of the waits)
 constexpr int PT_ENTRIES = 4, PT_READERS = 11;       // stretches known ahead; warps that read them: eight for probabilities, one for MMAs, two for Q and V
 struct TcShared {
-    uint64_t full[8], empty[8];                          // a slot's copies have landed; its last MMA is done
+    uint64_t full[8], empty[8];                          // a slot's copies have landed; its last MMA is done, and both warps that check V have seen its phase
     uint64_t clean[8];                                   // of the last V tiles: what nobody sees is cleared
     uint64_t q_ready[2][2], q_free[2][2];                // of the two tiles and their buffers, in stretches in which they see anything
     uint64_t s_ready[2], s_free[2], p_ready[2][2], p_free[2], o_ready[2];   // (P ready) of the first 96 positions and the rest; (free) where P lies apart
@@ -160,7 +160,13 @@ struct Walker {                                      // the copying warp's place
     }
 };
 
-template <int HD>
+__device__ __noinline__ void stand_still(uint64_t ns) {
+    const uint64_t t0 = global_timer_ns();
+    for (int i = 0; i < (1 << 22) && global_timer_ns() - t0 < ns; ++i) { __nanosleep(200); }
+}
+
+// LATE: the self-checks' kernels (p.late)
+template <int HD, bool LATE>
 __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_constant__ PagedAttention p, const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
                                                                   const int box, int *error_flag, const uint64_t wait_limit) {
     using Shape = TcShape<HD>;
@@ -173,7 +179,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
     const uint32_t q_ready = smem_u32(sh.q_ready), q_free = smem_u32(sh.q_free), s_ready = smem_u32(sh.s_ready), s_free = smem_u32(sh.s_free), p_ready = smem_u32(sh.p_ready),
                    o_ready = smem_u32(sh.o_ready), p_free = smem_u32(sh.p_free);
     if (tid == 0) {
-        for (int i = 0; i < 8; ++i) { mbar_init(full + 8 * i, 1); mbar_init(empty + 8 * i, 1); mbar_init(clean + 8 * i, 2); sh.poison[i] = 0; }
+        for (int i = 0; i < 8; ++i) { mbar_init(full + 8 * i, 1); mbar_init(empty + 8 * i, 3); mbar_init(clean + 8 * i, 2); sh.poison[i] = 0; }
         for (int i = 0; i < 4; ++i) { mbar_init(q_ready + 8 * i, 1); mbar_init(q_free + 8 * i, 1); mbar_init(p_ready + 8 * i, 4); }
         for (int t = 0; t < 2; ++t) { mbar_init(s_ready + 8 * t, 1); mbar_init(s_free + 8 * t, 4); mbar_init(o_ready + 8 * t, 1); mbar_init(p_free + 8 * t, 1); mbar_init(joined + 8 * t, 4); }
         mbar_init(smem_u32(&sh.over), 1);
@@ -548,8 +554,11 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
                     __syncwarp();
                 }
                 for (int step = en.begin; step < en.end; ++step) {
-                    // K as well, though nothing is done to it: copies land in any order, and a slot's phase that nobody waited for could be taken for the one after the next
+                    if (LATE && p.late == PA_LATE_CHECKS && tiles < 12) { stand_still(4000); }
+                    // K as well, though nothing is done to it: copies land in any order, and a slot's phase that nobody waited for could be taken for the one after the next.
+                    // A slot is not filled again before both warps have seen its phase, or they would wait for one that is over
                     wait_for(full + 8 * slot, phase, limit);
+                    if (lane == 0) { mbar_arrive(empty + 8 * slot); }
                     advance();
                     wait_for(full + 8 * slot, phase, limit);
                     if (!(en.whole(p, a, step) && (b.rows == 0 || en.whole(p, b, step)))) {
@@ -585,7 +594,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
                         fence_async_smem();
                     }
                     __syncwarp();
-                    if (lane == 0) { mbar_arrive(clean + 8 * (tiles & 7)); }
+                    if (lane == 0) { mbar_arrive(clean + 8 * (tiles & 7)); mbar_arrive(empty + 8 * slot); }
                     advance();
                     ++tiles;
                 }
@@ -731,21 +740,21 @@ bool query_map(CUtensorMap *map, const PagedAttention &p, int n_head, int head_d
     return tensor_map(map, p.q, 3, dims, strides, boxes);
 }
 // the warpgroups' registers after their split are what the block is launched with: fewer, and the split would wait for ever
-template <int HD> cudaError_t registers_suffice() {
+template <int HD, bool LATE> cudaError_t registers_suffice() {
     static const cudaError_t answer = [] {
         cudaFuncAttributes a;
-        const cudaError_t err = cudaFuncGetAttributes(&a, paged_tc_kernel<HD>);
+        const cudaError_t err = cudaFuncGetAttributes(&a, paged_tc_kernel<HD, LATE>);
         return err != cudaSuccess ? err : a.numRegs * PT_THREADS >= 256 * PT_REGS_SOFTMAX + 128 * PT_REGS_OTHERS ? cudaSuccess : cudaErrorInvalidConfiguration;
     }();
     return answer;
 }
-template <int HD>
+template <int HD, bool LATE>
 cudaError_t launch_tc(const PagedAttention &p, const CUtensorMap &q, const CUtensorMap &k, const CUtensorMap &v, int box, int sms, const LaunchCfg &cfg, uint64_t wait_limit) {
-    cudaError_t err = registers_suffice<HD>();
+    cudaError_t err = registers_suffice<HD, LATE>();
     if (err != cudaSuccess) { return err; }
-    err = allow_dynamic_smem(reinterpret_cast<const void *>(paged_tc_kernel<HD>), TcShape<HD>::SMEM);
+    err = allow_dynamic_smem(reinterpret_cast<const void *>(paged_tc_kernel<HD, LATE>), TcShape<HD>::SMEM);
     if (err != cudaSuccess) { return err; }
-    return launch_maybe_pdl(paged_tc_kernel<HD>, dim3(sms), PT_THREADS, TcShape<HD>::SMEM, cfg.stream, cfg.pdl, p, q, k, v, box, cfg.error_flag, wait_limit);
+    return launch_maybe_pdl(paged_tc_kernel<HD, LATE>, dim3(sms), PT_THREADS, TcShape<HD>::SMEM, cfg.stream, cfg.pdl, p, q, k, v, box, cfg.error_flag, wait_limit);
 }
 
 }  // namespace
@@ -765,7 +774,8 @@ bool launch_paged_attention_tc(const PagedAttention &given, int head_dim, int n_
     p.start_units = PA_START;
     CUtensorMap q, k, v;
     if (!query_map(&q, p, n_head, head_dim) || !page_map(&k, p.k, p.view, p.n_head_kv, head_dim, box) || !page_map(&v, p.v, p.view, p.n_head_kv, head_dim, box)) { return false; }
-    *err = head_dim == 128 ? launch_tc<128>(p, q, k, v, box, sms, cfg, wait_limit) : launch_tc<64>(p, q, k, v, box, sms, cfg, wait_limit);
+    const auto launch = p.late != PA_ON_TIME ? (head_dim == 128 ? launch_tc<128, true> : launch_tc<64, true>) : head_dim == 128 ? launch_tc<128, false> : launch_tc<64, false>;
+    *err = launch(p, q, k, v, box, sms, cfg, wait_limit);
     return true;
 }
 

@@ -924,3 +924,10 @@ def test_rows_of_nobody_decide_nothing(be, dev, hd, group):
         other[starts[2]:] = q[starts[2]:]
         other[starts[3]:] = size
         assert np.array_equal(run(other)[starts[2]:starts[3]], first[starts[2]:starts[3]]), size
+
+
+def test_warps_that_come_late_change_nothing():
+    """The warps that check V wait for phases of a ring that others drive: however late they come, none is over before they have seen it."""
+    b = B.B200Backend(0)
+    assert b.paged_selftest_late(1, 1_000_000_000) == 0
+    b.close()
