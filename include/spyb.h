@@ -321,7 +321,8 @@ typedef struct {
 spyb_status spyb_sample(spyb_backend *backend, const spyb_sample_desc *desc);
 
 /* Self-check of spyb_paged_attention's hand-overs, without a fault: the tensor-memory kernel on a small batch of its own with one of its roles late. who = 1: the warps that check values
- * stay microseconds behind; within `limit_ns` (the bound of every wait) the output has the same bits and error_code_out is 0. */
+ * stay microseconds behind; within `limit_ns` (the bound of every wait) the output has the same bits and error_code_out is 0. who = 2, 3: a copy of K and V, of Q comes three limits
+ * late: waits give up, the kernel returns by itself when the copy has landed, error_code_out is 7, the error is cleared and the next launch is right. */
 spyb_status spyb_paged_selftest_late(spyb_backend *backend, int32_t who, uint64_t limit_ns, int32_t *error_code_out);
 
 /* What the three calls above would answer to a descriptor, and why in `message` (up to `size` bytes with the closing 0; may be NULL with size 0): host

@@ -159,20 +159,22 @@ struct spyb_backend {
         const int code = *reinterpret_cast<volatile int *>(h_error_flag);
         *reinterpret_cast<volatile int *>(h_error_flag) = 0;
         if (pf_handoff != nullptr && cudaMemsetAsync(handoff_flags(), 0, handoff_flag_bytes(), stream) != cudaSuccess) { cudaGetLastError(); }
+        if (paged_arrived != nullptr && cudaMemsetAsync(paged_arrived, 0, paged_arrived_bytes(), stream) != cudaSuccess) { cudaGetLastError(); }
         return code;
     }
     void prefill_shared(spyb::PrefillGemm &g) const {   // what every prompt GEMM on this backend's stream has in common
         g.error_flag = d_error_flag; g.wait_limit_ns = wait_limit_ns;
         g.handoff = pf_handoff; g.handoff_flags = handoff_flags();
     }
+    size_t paged_arrived_bytes() const { return 4 * (size_t)num_sms_total * sizeof(unsigned); }
     // room for two pieces of 256 rows x 128 elements (with their maxima and sums) of every SM; the small kernel's pieces are less
     bool paged_workspace() {
         if (paged_arrived != nullptr) { return true; }
-        const size_t piece = 256 * (128 + 2) * sizeof(float), words = 4 * (size_t)num_sms_total;
+        const size_t piece = 256 * (128 + 2) * sizeof(float);
         void *raw = nullptr;
-        if (cudaMalloc(&raw, 2 * num_sms_total * piece + words * sizeof(unsigned)) != cudaSuccess) { cudaGetLastError(); set_error("paged_attention: out of device memory for its workspace"); return false; }
+        if (cudaMalloc(&raw, 2 * num_sms_total * piece + paged_arrived_bytes()) != cudaSuccess) { cudaGetLastError(); set_error("paged_attention: out of device memory for its workspace"); return false; }
         unsigned *arrived = reinterpret_cast<unsigned *>(static_cast<uint8_t *>(raw) + 2 * num_sms_total * piece);
-        if (cudaMemsetAsync(arrived, 0, words * sizeof(unsigned), stream) != cudaSuccess) { cudaGetLastError(); cudaFree(raw); set_error("paged_attention: its workspace cannot be cleared"); return false; }
+        if (cudaMemsetAsync(arrived, 0, paged_arrived_bytes(), stream) != cudaSuccess) { cudaGetLastError(); cudaFree(raw); set_error("paged_attention: its workspace cannot be cleared"); return false; }
         paged_partial = static_cast<float *>(raw); paged_arrived = arrived;
         return true;
     }

@@ -21,7 +21,8 @@ struct PagedAppend {
     int          n_head = 0, n_head_kv = 0, head_dim = 0, rot = 0, halves = 0;
     double       turns[128] = {};         // pair i turns by this share of a full circle a position
 };
-enum PagedLate { PA_ON_TIME = 0, PA_LATE_CHECKS = 1 };   // the warps that check V stay a few microseconds behind everything else
+// the warps that check V stay a few microseconds behind everything else; one copy of a CTA's K and V, or its first of Q, comes three limits of the waits late
+enum PagedLate { PA_ON_TIME = 0, PA_LATE_CHECKS = 1, PA_LATE_KV = 2, PA_LATE_Q = 3 };
 struct PagedAttention {
     PagedView    view;
     const __half *q = nullptr, *k = nullptr, *v = nullptr;

@@ -61,7 +61,10 @@ struct Entry {
         return j + PT_KEYS <= hi && (!p.causal || (j + PT_KEYS - 1 <= h.pos_first && (p.window <= 0 || j > h.pos_last - p.window)));
     }
 };
-constexpr uint64_t PT_LANDING_NS = 1000000000;       // when a wait gave up: what is on its way has this long to land (whatever the limit of the waits)
+// A lane whose wait has run out (its limit is 0 then) frees nothing any more: no slot that a copy may still be on its way to is filled again, no entry that somebody may
+// still read is written over. The other roles' waits run out in turn, so that every role ends by itself, and then who issued copies or products waits for their end, whoever
+// it was that gave up. (Waiting for it in every case, at the end of each role, cost 5 % of prompts of heads of 64.)
+constexpr uint64_t PT_LANDING_NS = 1000000000;       // what is on its way has this long to land (whatever the limit of the waits)
 constexpr int PT_ENTRIES = 4, PT_READERS = 11;       // stretches known ahead; warps that read them: eight for probabilities, one for MMAs, two for Q and V
 struct TcShared {
     uint64_t full[8], empty[8];                          // a slot's copies have landed; its last MMA is done, and both warps that check V have seen its phase
@@ -75,6 +78,7 @@ struct TcShared {
     uint32_t there[8];                                   // of the last tiles: which groups of eight positions are there
     int      poison[8];                                  // of the last stretches: a V tile that some rows see in part holds values that are not finite
     int      last[2];
+    int      gave_up;                                    // a wait of some warp has run out
     Entry    entry[PT_ENTRIES];
     PagedPlanShared plan;
 };
@@ -183,6 +187,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
         for (int i = 0; i < 4; ++i) { mbar_init(q_ready + 8 * i, 1); mbar_init(q_free + 8 * i, 1); mbar_init(p_ready + 8 * i, 4); }
         for (int t = 0; t < 2; ++t) { mbar_init(s_ready + 8 * t, 1); mbar_init(s_free + 8 * t, 4); mbar_init(o_ready + 8 * t, 1); mbar_init(p_free + 8 * t, 1); mbar_init(joined + 8 * t, 4); }
         mbar_init(smem_u32(&sh.over), 1);
+        sh.gave_up = 0;
         for (int i = 0; i < PT_ENTRIES; ++i) { mbar_init(known + 8 * i, 1); mbar_init(read + 8 * i, PT_READERS); }
         mbar_init_fence();
     }
@@ -199,17 +204,23 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
     const uint32_t tmem = sh.tmem;
     uint64_t limit = wait_limit;
     uint32_t stretch = 0;
+    auto gave_up = [&]() {                                // whether a wait of this warp has run out; all of its lanes' limits are 0 then
+        if (__all_sync(0xffffffffu, limit != 0)) { return false; }
+        limit = 0;
+        return true;
+    };
     // the next entry; false behind the last one, or when a wait gave up (the roles then end one after the other: nobody waits without a limit)
     auto next_entry = [&]() {
         wait_for(known + 8 * (stretch & (PT_ENTRIES - 1)), (stretch / PT_ENTRIES) & 1, limit);
-        if (!__all_sync(0xffffffffu, limit != 0)) { limit = 0; }
-        return limit != 0 && sh.entry[stretch & (PT_ENTRIES - 1)].todo != 0;
+        return !gave_up() && sh.entry[stretch & (PT_ENTRIES - 1)].todo != 0;
     };
     auto entry_read = [&](bool by_me) {
         if (by_me) { mbar_arrive(read + 8 * (stretch & (PT_ENTRIES - 1))); }
         ++stretch;
     };
 
+    // K and V tiles take slots in turn: K of step 0, V of step 0, K of step 1, ...
+    uint32_t slot = 0, phase = 0, issued = 0;             // (issued: tiles of K and V by the copying warp, of Q by those that check V)
     if (warp < 8) {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(PT_REGS_SOFTMAX));
         // ---------------------------------------------------------------------------------- probabilities, output
@@ -471,27 +482,26 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
         }
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PT_REGS_OTHERS));
-        // K and V tiles take slots in turn: K of step 0, V of step 0, K of step 1, ...
-        uint32_t slot = 0, phase = 0;
         auto advance = [&]() { if (++slot == SLOTS) { slot = 0; phase ^= 1; } };
         if (warp == 9) {
             // ------------------------------------------------------------------------------ the stretches, and their copies
             constexpr int halves = HD / 64;                                                 // a tile's boxes are 64 elements wide
             const int group = lane % 16 * 8, half = lane >> 4;                              // this lane's eight positions of a tile, and half
             const bool issues = (group & (box - 1)) == 0 && half < halves;
-            uint32_t copies = 0;
+            uint32_t &copies = issued;
             walk.seq = walk.at.seq; walk.head = walk.at.head; walk.tile = walk.at.tile; walk.off = walk.at.off;
             walk.q = paged_seq(p.view, walk.seq);
-            auto put = [&](const Entry &e) {
+            auto put = [&](const Entry &e) {                                                // false: somebody gave up
                 const uint32_t i = stretch & (PT_ENTRIES - 1);
                 wait_for(read + 8 * i, ((stretch / PT_ENTRIES) & 1) ^ 1, limit);
+                if (gave_up()) { return false; }
                 if (lane == 0) { sh.entry[i] = e; mbar_arrive(known + 8 * i); }
                 ++stretch;
+                return true;
             };
             for (;;) {
                 const Entry e = walk.entry(p);
-                put(e);
-                if (!__all_sync(0xffffffffu, limit != 0)) { limit = 0; break; }
+                if (!put(e)) { break; }
                 const int32_t *table = p.view.page_table + (int64_t)e.seq * p.view.table_stride;
                 auto page_of = [&](int step) {                                              // (one step ahead: the table's latency is hidden)
                     const int j = e.lo + step * PT_KEYS + group;
@@ -506,7 +516,8 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
 #pragma unroll
                     for (int kv = 0; kv < 2; ++kv) {
                         wait_for(empty + 8 * slot, phase ^ 1, limit);
-                        if (!__all_sync(0xffffffffu, limit != 0)) { limit = 0; break; }
+                        if (LATE && p.late == PA_LATE_KV && copies == 2) { stand_still(3 * wait_limit); }   // (issued all the same, with nobody waiting any more)
+                        else if (gave_up()) { break; }
                         const uint32_t bar = full + 8 * slot, dst = ring + slot * Shape::OPERAND;
                         if (lane == 0) {
                             if (kv == 0) { *reinterpret_cast<volatile uint32_t *>(&sh.there[copies / 2 & 7]) = there; }
@@ -520,21 +531,12 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
                     }
                     if (limit == 0) { break; }
                 }
-                if (!walk.next(p, e.todo)) { break; }
+                if (limit == 0 || !walk.next(p, e.todo)) { break; }
             }
-            Entry over = {};
-            put(over);
-            if (limit == 0) {   // something gave up: what is on its way lands before the CTA ends
-                uint64_t again = PT_LANDING_NS;
-                for (uint32_t i = 0; i < SLOTS && i < copies; ++i) {
-                    if (slot == 0) { slot = SLOTS; phase ^= 1; }
-                    --slot;
-                    wait_for(full + 8 * slot, phase, again);
-                }
-            }
+            if (limit != 0) { Entry over = {}; put(over); }
         } else if (warp >= 10) {
             // ------------------------------------------------------------------------------ Q of a tile each; V tiles that not all rows see whole, half of the rows each
-            uint32_t tiles = 0, q_count = 0;
+            uint32_t tiles = 0, &q_count = issued;
             const int t = warp - 10, v_row0 = t * (PT_KEYS / 2);
             while (next_entry()) {
                 const Entry &en = sh.entry[stretch & (PT_ENTRIES - 1)];
@@ -542,7 +544,8 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
                 if (t == 0 ? a.to > a.from : b.to > b.from) {
                     const uint32_t buffer = q_count % Shape::Q_BUFFERS, bar = 16 * t + 8 * buffer;
                     wait_for(q_free + bar, (q_count / Shape::Q_BUFFERS & 1) ^ 1, limit);
-                    if (!__all_sync(0xffffffffu, limit != 0)) { limit = 0; break; }
+                    if (LATE && p.late == PA_LATE_Q && q_count == 0) { stand_still(3 * wait_limit); }
+                    else if (gave_up()) { break; }
                     ++q_count;
                     // whole tokens, token by token their heads: what lies behind the sequence's rows is other sequences' or nothing, and goes nowhere
                     if (elect_one()) {
@@ -558,7 +561,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
                     // K as well, though nothing is done to it: copies land in any order, and a slot's phase that nobody waited for could be taken for the one after the next.
                     // A slot is not filled again before both warps have seen its phase, or they would wait for one that is over
                     wait_for(full + 8 * slot, phase, limit);
-                    if (lane == 0) { mbar_arrive(empty + 8 * slot); }
+                    if (lane == 0 && limit != 0) { mbar_arrive(empty + 8 * slot); }
                     advance();
                     wait_for(full + 8 * slot, phase, limit);
                     if (!(en.whole(p, a, step) && (b.rows == 0 || en.whole(p, b, step)))) {
@@ -594,24 +597,18 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
                         fence_async_smem();
                     }
                     __syncwarp();
-                    if (lane == 0) { mbar_arrive(clean + 8 * (tiles & 7)); mbar_arrive(empty + 8 * slot); }
+                    if (lane == 0 && limit != 0) { mbar_arrive(clean + 8 * (tiles & 7)); mbar_arrive(empty + 8 * slot); }
                     advance();
                     ++tiles;
                 }
                 __syncwarp();
                 entry_read(lane == 0);
             }
-            if (limit == 0 && q_count > 0) {   // (something gave up: what is on its way lands before the CTA ends)
-                for (uint32_t i = 1; i <= Shape::Q_BUFFERS && i <= q_count; ++i) {
-                    uint64_t again = PT_LANDING_NS;
-                    const uint32_t n = q_count - i;
-                    wait_for(q_ready + 16 * t + 8 * (n % Shape::Q_BUFFERS), n / Shape::Q_BUFFERS & 1, again);
-                }
-            }
         } else if (warp == 8) {
             // ------------------------------------------------------------------------------ MMAs
             constexpr uint32_t idesc_s = idesc_f16(PT_KEYS), idesc_o = idesc_f16(HD) | (1u << 16);   // (bit 16: B is MN-major)
             uint32_t q_count[2] = {0, 0}, s_count[2] = {0, 0}, p_phase[2] = {0, 0}, tiles = 0;
+            auto frees = [&]() { return elect_one() && limit != 0; };   // (the lane that issues has seen every wait's end for itself)
             auto scores = [&](int t, uint32_t k_slot, bool last) {
                 if (Shape::P_APART) { wait_for(s_free + 8 * t, (s_count[t] & 1) ^ 1, limit); tc_fence_after(); }   // (else P's products, in order, are what frees S)
                 ++s_count[t];
@@ -624,7 +621,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
                         mma_f16_ss(tmem + t * PT_KEYS, a + step, b + step, idesc_s, k != 0);
                     }
                     mma_commit(s_ready + 8 * t);
-                    if (last) { mma_commit(q_free + 16 * t + 8 * buffer); }
+                    if (last && limit != 0) { mma_commit(q_free + 16 * t + 8 * buffer); }
                 }
                 __syncwarp();
             };
@@ -645,7 +642,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
                         tc_fence_after();
 #pragma unroll
                         for (int t = 0; t < 2; ++t) { if (active(t, step)) { scores(t, slot, step + 1 == to[t]); } }
-                        if (elect_one()) { mma_commit(empty + 8 * slot); }
+                        if (frees()) { mma_commit(empty + 8 * slot); }
                         __syncwarp();
                         advance();
                     }
@@ -656,7 +653,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
                     if (Shape::P_APART && ahead) {
 #pragma unroll
                         for (int t = 0; t < 2; ++t) { if (active(t, step + 1)) { scores(t, slot, step + 2 == to[t]); } }
-                        if (elect_one()) { mma_commit(empty + 8 * slot); }
+                        if (frees()) { mma_commit(empty + 8 * slot); }
                         __syncwarp();
                     }
                     wait_for(full + 8 * v_slot, v_phase, limit);
@@ -684,7 +681,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
                         }
                         if (!Shape::P_APART && ahead && active(t, step + 1)) { scores(t, slot, step + 2 == to[t]); }
                     }
-                    if (elect_one()) {
+                    if (frees()) {
                         mma_commit(empty + 8 * v_slot);
                         if (!Shape::P_APART && ahead) { mma_commit(empty + 8 * slot); }
                     }
@@ -692,17 +689,32 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
                     if (ahead) { advance(); }
                 }
             }
-            if (limit == 0) {   // (something gave up: what was issued is done before the CTA ends)
-                if (elect_one()) { mma_commit(smem_u32(&sh.over)); }
-                __syncwarp();
-                uint64_t again = PT_LANDING_NS;
-                wait_for(smem_u32(&sh.over), 0, again);
-            }
         }
     }
-    if (limit == 0 && lane == 0) { pf_report(error_flag, 7); }
+    if (limit == 0 && lane == 0) { pf_report(error_flag, 7); *reinterpret_cast<volatile int *>(&sh.gave_up) = 1; }
     tc_fence_before();
     __syncthreads();
+    if (*reinterpret_cast<volatile int *>(&sh.gave_up)) {
+        uint64_t again = PT_LANDING_NS;
+        if (warp == 8) {
+            if (elect_one()) { mma_commit(smem_u32(&sh.over)); }
+            __syncwarp();
+            wait_for(smem_u32(&sh.over), 0, again);
+        } else if (warp == 9) {                           // each slot's last copy (the ones before it were waited for by whoever freed the slot)
+            for (uint32_t i = 0; i < SLOTS && i < issued; ++i) {
+                if (slot == 0) { slot = SLOTS; phase ^= 1; }
+                --slot;
+                wait_for(full + 8 * slot, phase, again);
+            }
+        } else if (warp >= 10) {
+            for (uint32_t i = 1; i <= Shape::Q_BUFFERS && i <= issued; ++i) {
+                const uint32_t n = issued - i;
+                wait_for(q_ready + 16 * (warp - 10) + 8 * (n % Shape::Q_BUFFERS), n / Shape::Q_BUFFERS & 1, again);
+            }
+        }
+        tc_fence_before();
+        __syncthreads();
+    }
     if (warp == 8) {
         tc_fence_after();
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");

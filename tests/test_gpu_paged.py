@@ -931,3 +931,17 @@ def test_warps_that_come_late_change_nothing():
     b = B.B200Backend(0)
     assert b.paged_selftest_late(1, 1_000_000_000) == 0
     b.close()
+
+
+@pytest.mark.parametrize("who", [2, 3])
+def test_copies_that_come_too_late_are_reported_and_leave_nothing(be, dev, who):
+    """Waits of 2 ms for a copy that comes after 6: they give up, the kernel ends by itself with the copy landed, the status says so, and later launches on the backend are right."""
+    b = B.B200Backend(0)
+    assert b.paged_selftest_late(who, 2_000_000) == 7
+    assert b.paged_selftest_late(1, 1_000_000_000) == 0
+    d = Device(b)
+    rng = np.random.default_rng(who)
+    check_attention(b, d, rng, [150, 1, 40], [700, 2000, 90], 4, 2, 128, 16)
+    check_attention(b, d, rng, [150, 1, 40], [700, 2000, 90], 6, 2, 64, 16)
+    d.free()
+    b.close()
