@@ -225,6 +225,7 @@ spyb_status spyb_create(const spyb_config *config, spyb_backend **out) {
     const size_t handoff = (size_t)be->num_sms_total * (PF_HANDOFF_BYTES + PF_HANDOFF_FLAGS * sizeof(unsigned));
     if (cudaMalloc(&be->pf_handoff, handoff) != cudaSuccess) { cudaGetLastError(); be->pf_handoff = nullptr; }   // (the GEMMs go without)
     else if (cudaMemsetAsync(be->pf_handoff, 0, handoff, be->stream) != cudaSuccess) { spyb_destroy(be); return SPYB_FAIL; }   // (in front of all that reads it)
+    if (!be->paged_workspace()) { be->set_error("%s", ""); }   // (a call that needs it asks again; a first call may come during a stream capture, which allows no allocation)
     be->cb_thread = std::thread(callback_worker, be);
     *out = be;
     return SPYB_SUCCESS;

@@ -104,7 +104,7 @@ struct spyb_backend {
     int         *h_error_flag = nullptr;   // mapped pinned word the kernels set when a bounded wait runs out
     int         *d_error_flag = nullptr;   // its device address
     void        *pf_handoff = nullptr;     // prompt GEMMs, one after the other on the stream: PrefillGemm::handoff, and behind it the flags
-    float       *paged_partial = nullptr;  // paged attention, one call after the other on the stream: what the CTAs of a cut item found (made at first use),
+    float       *paged_partial = nullptr;  // paged attention, one call after the other on the stream: what the CTAs of a cut item found (made with the backend),
     unsigned    *paged_arrived = nullptr;  // and how many of them are done, by their first CTA; zero between launches
     spyb::PagedTurns paged_turns;
     uint8_t     *noalloc_scratch = nullptr; // device address of the scratch array of spyb_matmul_noalloc (looked up once)

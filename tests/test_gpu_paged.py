@@ -945,3 +945,37 @@ def test_copies_that_come_too_late_are_reported_and_leave_nothing(be, dev, who):
     check_attention(b, d, rng, [150, 1, 40], [700, 2000, 90], 6, 2, 64, 16)
     d.free()
     b.close()
+
+
+def test_first_calls_beside_a_stream_capture(dev):
+    """A backend's first attention (both kernels) and sampling while another library captures a stream: nothing is allocated in the calls."""
+    import torch
+
+    rng = np.random.default_rng(41)
+    pool = Pool(rng, [700, 90], 2, 64, 16, fill=0.0)
+    for s, n in enumerate((700, 90)):
+        pool.put(s, *rng.standard_normal((2, n, 2, 64)).astype(np.float16))
+    q = rng.standard_normal((141, 4, 64)).astype(np.float16)
+    b = B.B200Backend(0)
+    d = Device(b)
+    cache = pool.cache(d(pool.k), d(pool.v))
+    many = B.paged_batch(d(np.array([0, 140, 141], np.int32)), d(np.array([700, 90], np.int32)), d(pool.table), 2, 141, pool.table.shape[1])
+    one = B.paged_batch(d(np.array([0, 1], np.int32)), d(np.array([700], np.int32)), d(pool.table), 1, 1, pool.table.shape[1])
+    pq, po, pi, out = d(q), d(np.zeros(q.shape, np.float32)), d(np.zeros(141, np.int32)), np.zeros(q.shape, np.float32)
+    x = torch.zeros(1000, device="cuda")
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = x + 1
+        b.paged_attention(B.paged_attention_desc(cache, many, pq, po, 4, out_type=B.FP32))
+        b.paged_attention(B.paged_attention_desc(cache, one, pq, po, 4, out_type=B.FP32))
+        b.sample(B.sample_desc(po, B.FP32, 141, 256, pi))
+    during = d.back(po, out)
+    b.paged_attention(B.paged_attention_desc(cache, many, pq, po, 4, out_type=B.FP32))
+    b.paged_attention(B.paged_attention_desc(cache, one, pq, po, 4, out_type=B.FP32))
+    assert during.any() and np.array_equal(during, d.back(po, out))
+    graph.replay()
+    torch.cuda.synchronize()
+    assert (y == 1).all()
+    d.free()
+    b.close()
