@@ -300,12 +300,14 @@ spyb_status spyb_paged_attention(spyb_backend *backend, const spyb_paged_attenti
 
 /* The next token of every row of logits [n_rows][n_vocab] (row_stride elements apart; SPYB_FP32 or SPYB_FP16): SamplerImpl<Greedy>::sample
  * (model/include/llm/sampler/greedy.h:20-25) with the usual settings, one of each a row; a NULL array leaves the setting out.
- *   w_i = exp((logit_i - largest) / temperature), in 64 bits; temperature NULL: 1; not above 0: the largest logit, the lowest index among equals
+ *   w_i = exp((logit_i - largest) / temperature); temperature NULL: 1; not above 0: the largest logit, the lowest index among equals
  *   top_k   (0 < top_k < n_vocab): the top_k largest logits stay, the lowest indices among equals
  *   top_p   (< 1): of these, in descending order, those in front of which less than top_p of their sum lies (never fewer than one)
- *   min_p   (> 0): of these, those with w_i >= min_p
+ *   min_p   (> 0): of these, those with w_i >= min_p (above 1 it reads as 1)
  *   the token is the first index, ascending, up to which the weights that stayed sum to more than uniform[row] (in [0, 1)) times their sum: at 0 the first
- *   whose weight is not 0 in 64 bits, however small
+ *   whose weight is not 0 in 64 bits, however small.
+ * Weights are held as integers, in units of 2^-45 of the largest (2^-42 for 2^20 tokens), each to 2^-31 of itself at most, 2^-34 as a rule, and cut to its unit; their sums are exact.
+ * top_p, min_p and the numbers are compared with these; numbers below 2^-20, and min_p beside them, with weights in floating point of 64 bits.
  * NaN and -inf are never drawn; where there is +inf, only +inf has weight, all the same. ids[row] = -1, probs[row] = 0 where there is nothing to draw.
  * probs (optional): the token's share of the weights that stayed. n_vocab at most 2^20. uniform NULL reads as zeros. */
 typedef struct {
@@ -319,6 +321,8 @@ typedef struct {
     float   *probs;
 } spyb_sample_desc;
 spyb_status spyb_sample(spyb_backend *backend, const spyb_sample_desc *desc);
+/* The weights of logits beside a largest one, as spyb_sample makes them for rows of n_vocab (host arrays; a check of their precision, synchronous). */
+spyb_status spyb_sample_weights(spyb_backend *backend, const float *logits_host, int32_t n, float largest, float temperature, int32_t n_vocab, uint64_t *weights_host);
 
 /* Self-check of spyb_paged_attention's hand-overs, without a fault: the tensor-memory kernel on a small batch of its own with one of its roles late. who = 1: the warps that check values
  * stay microseconds behind; within `limit_ns` (the bound of every wait) the output has the same bits and error_code_out is 0. who = 2, 3: a copy of K and V, of Q comes three limits

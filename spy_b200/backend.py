@@ -127,6 +127,7 @@ def lib():
         "spyb_paged_append": (i32, [vp, C.POINTER(PagedAppendDesc)]),
         "spyb_paged_attention": (i32, [vp, C.POINTER(PagedAttentionDesc)]),
         "spyb_sample": (i32, [vp, C.POINTER(SampleDesc)]),
+        "spyb_sample_weights": (i32, [vp, vp, i32, C.c_float, C.c_float, i32, vp]),
         "spyb_paged_selftest_late": (i32, [vp, i32, u64, C.POINTER(i32)]),
         "spyb_paged_append_check": (i32, [C.POINTER(PagedAppendDesc), C.c_char_p, i32]),
         "spyb_paged_attention_check": (i32, [C.POINTER(PagedAttentionDesc), C.c_char_p, i32]),
@@ -367,6 +368,13 @@ class B200Backend:
         st = self._sample(self.h, C.byref(desc))
         if st != SUCCESS:
             self._check(st)
+
+    def sample_weights(self, logits, largest: float, temperature: float, n_vocab: int) -> np.ndarray:
+        """The integers that sample weighs these logits by, beside a largest one, in rows of n_vocab: units of 2^-min(45, 62 - ceil(log2(n_vocab)))."""
+        x = np.ascontiguousarray(logits, dtype=np.float32)
+        w = np.empty(x.size, dtype=np.uint64)
+        self._check(self._l.spyb_sample_weights(self.h, _np_ptr(x), x.size, largest, temperature, n_vocab, _np_ptr(w)))
+        return w
 
     def submit_timed(self, descs, repeats: int) -> float:
         """Device time in ms of `repeats` submits that walk round-robin over the descriptors (measurement aid)."""

@@ -12,8 +12,9 @@ namespace spyb {
 namespace {
 
 // A cluster of CTAs has a row, each a slice of it in shared memory: the logits are read once, by bulk copies. Which token a number falls on must not depend on how
-// sums are rounded, so weights are integers: w = 2^S exp((x - largest) / T), S = 45 for up to 2^17 tokens. Their sums are exact in any order,
-// a histogram's too, and errors of 2^-34 of each weight, as often up as down, move a border of N weights' sums by some 2^-34 / sqrt(N) of the whole. An exponential to so many bits costs some 35
+// sums are rounded, so weights are integers: w = 2^S exp((x - largest) / T), S = 45 for up to 2^17 tokens (62 less the bits of their number for more). Their sums are exact in any
+// order, a histogram's too. A weight is off by some 2^-34 of itself, as often up as down, and is cut to whole units, half a unit down on average: a border of N weights' sums
+// moves by some 2^-34 / sqrt(N) of the whole and N / 2 units (2^-30 of the largest weight for 2^16 tokens). An exponential to so many bits costs some 35
 // instructions, so it is taken where it is needed only:
 //   greedy            none
 //   top-k             every CTA takes its share of k among its threads' own maxima (a histogram of their distances from its largest); the lowest such
@@ -98,11 +99,13 @@ struct SampleShared {
     int      found, found2;
 };
 
-// The weight of a logit as an integer, 2^S 2^-z with z = (largest - x) c, c = log2(e) / T, to 2^-34 of itself and a unit. (An operation in 64 bits takes eight clocks of a
+// The weight of a logit as an integer, 2^S 2^-z with z = (largest - x) c, c = log2(e) / T, to 2^-31.8 of itself at most and a unit (see below). (An operation in 64 bits takes eight clocks of a
 // quarter of an SM, one in f32 one: 192 rows of 128 000 at a temperature alone took 108 us with them, 100 like this.) z is taken apart as r / 1024 + f + e without an error that counts:
 //   p + p' = x c, by FMA; A = largest c in 64 bits, A = a + a' with a a multiple of 2^-14; r = round(1024 (a - p));
 //   f = (a - r / 1024) - p: the first difference is exact (multiples of 2^-14 below 2^10), the second too (|f| <= 2^-11); e = a' - p'.
-// 2^-(r / 1024) is a table's 2^46-fold and a shift, 2^-(f + e) = 1 + y with |y| < 2^-11.5, y to 2^-36 in f32.
+// 2^-(r / 1024) is a table's 2^46-fold and a shift, 2^-(f + e) = 1 + y with |y| < 2^-11.5. Of the weight: y's roundings 2^-34.2 (two steps and a constant, each half a step of
+// f32), the table's entry cut to 23 bits in its product with y 2^-33.5, that product rounded to 2^-33 of the largest entry, which is 2^-32 of the smallest, half of it 2^-33; p', a' and the
+// series' third term 2^-36 together.
 // Where |A| is too large for that (1000 and more: tiny temperatures, huge logits), or c itself for f32, the same in 64 bits.
 struct Weight {
     const uint64_t *table;      // 2^46 2^-(j / 1024)
@@ -111,6 +114,7 @@ struct Weight {
     bool   wide;                // in 64 bits
     double c, largest;
     int    shift;               // 46 - S
+    static __device__ __forceinline__ double factor(float temp) { return 1.4426950408889634073599 / (double)temp; }   // c (4e-39 to 1e45, or 0)
     __device__ __forceinline__ void set(const uint64_t *powers, float top, double scale, double edge, int bits) {   // edge: 56 / c (2^-56 is no unit: rounds to nothing)
         table = powers; c = scale; largest = top; shift = 46 - bits;
         const double a = largest * c, lowest = largest - edge;
@@ -395,7 +399,7 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(const __grid_cons
 
     *reinterpret_cast<uint4 *>(sh.table + 2 * tid) = powers;
     if (tid == SA_THREADS - 1) {
-        const double c = 1.4426950408889634073599 / (double)temp;      // (4e-39 to 1e45, or 0)
+        const double c = Weight::factor(temp);
         sh.c = c; sh.edge = 56 / c;
         sh.least = min_p > 0.f ? (uint64_t)max(1.0, ceil((double)fminf(min_p, 1.f) * __hiloint2double((1023 + p.frac_bits) << 20, 0))) : 1;
         sh.bin_scale = (float)fmin(c * (2 * SA_BINS / (double)(p.frac_bits + 1)), 3e38);   // of halves (cut: bins hold more than they should, and the slow search decides)
@@ -840,6 +844,18 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(const __grid_cons
     }
 }
 
+__global__ void weights_kernel(const uint64_t *powers, const float *logits, int n, float largest, float temp, int bits, uint64_t *weights) {
+    const double c = Weight::factor(temp);
+    Weight w;
+    w.set(powers, largest, c, 56 / c, bits);
+    for (int i = blockIdx.x * blockDim.x + threadIdx.x; i < n; i += gridDim.x * blockDim.x) { weights[i] = w(logits[i]); }
+}
+int weight_bits(int n_vocab) {
+    int log2_vocab = 0;
+    while ((1 << log2_vocab) < n_vocab) { ++log2_vocab; }
+    return std::min(45, 62 - log2_vocab);
+}
+
 template <class T, bool KEPT>
 cudaError_t launch_sample(SampleParams &p, int n_rows, int ctas, const LaunchCfg &cfg) {
     const size_t smem = sizeof(SampleShared) + (KEPT ? (size_t)p.per * 4 : 0);
@@ -898,12 +914,30 @@ extern "C" spyb_status spyb_sample(spyb_backend *be, const spyb_sample_desc *d) 
     use_device(be->config.device_id);
     SampleParams p;
     p.logits = d->logits; p.row_stride = d->row_stride; p.n_vocab = d->n_vocab;
-    int log2_vocab = 0;
-    while ((1 << log2_vocab) < d->n_vocab) { ++log2_vocab; }
-    p.frac_bits = std::min(45, 62 - log2_vocab);
+    p.frac_bits = weight_bits(d->n_vocab);
     p.temperature = d->temperature; p.top_k = d->top_k; p.top_p = d->top_p; p.min_p = d->min_p; p.uniform = d->uniform; p.ids = d->ids; p.probs = d->probs;
     p.powers = be->d_power_table; p.error_flag = be->d_error_flag; p.wait_limit = be->wait_limit_ns;
     const LaunchCfg cfg = be->launch_cfg(be->config.use_pdl != 0);
     SPYB_CUDA(be, d->number_type == SPYB_FP32 ? launch_sample<float>(p, d->n_rows, be->num_sms_total, cfg) : launch_sample<__half>(p, d->n_rows, be->num_sms_total, cfg));
+    return SPYB_SUCCESS;
+}
+
+// The weights as the sampler's kernels make them: in units of 2^-S of the largest, S as for n_vocab logits. Host arrays.
+extern "C" spyb_status spyb_sample_weights(spyb_backend *be, const float *logits_host, int32_t n, float largest, float temperature, int32_t n_vocab, uint64_t *weights_host) {
+    if (be == nullptr || logits_host == nullptr || weights_host == nullptr || n < 1 || n_vocab < 1 || n_vocab > (1 << SA_INDEX_BITS) || !(temperature > 0.f)) { return SPYB_FAIL; }
+    use_device(be->config.device_id);
+    uint8_t *mem = nullptr;
+    SPYB_CUDA(be, cudaMalloc(&mem, (size_t)n * 12));
+    uint64_t *weights = reinterpret_cast<uint64_t *>(mem);
+    float    *logits  = reinterpret_cast<float *>(weights + n);
+    cudaError_t err = upload(logits, logits_host, (size_t)n * 4);
+    if (err == cudaSuccess) {
+        weights_kernel<<<64, 256, 0, be->stream>>>(be->d_power_table, logits, n, largest, temperature, weight_bits(n_vocab), weights);
+        err = cudaGetLastError();
+    }
+    if (err == cudaSuccess) { err = cudaMemcpyAsync(weights_host, weights, (size_t)n * 8, cudaMemcpyDeviceToHost, be->stream); }
+    if (err == cudaSuccess) { err = cudaStreamSynchronize(be->stream); }
+    cudaFree(mem);
+    SPYB_CUDA(be, err);
     return SPYB_SUCCESS;
 }

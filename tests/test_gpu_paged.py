@@ -979,3 +979,22 @@ def test_first_calls_beside_a_stream_capture(dev):
     assert (y == 1).all()
     d.free()
     b.close()
+
+
+@pytest.mark.parametrize("vocab", [1000, 1 << 17, (1 << 17) + 1, 1 << 20])
+@pytest.mark.parametrize("c_largest", [0.0, 1.0, -30.0, 640.0, 959.9, -959.9, 960.1, -960.1, 5000.0, -3e5])
+def test_weights_of_the_sampler(be, vocab, c_largest):
+    """2^S exp((x - largest) / T): to 2^-31.8 of itself (as derived beside the code) and a unit, on both sides of the switch to 64 bits at largest / T log2(e) = 960."""
+    bits = min(45, 62 - int(np.ceil(np.log2(vocab))))
+    rng = np.random.default_rng(int(abs(c_largest)) + vocab)
+    for t in (1.0, 0.37, 1e-3, 2.5e4, 1e-35, 1e33):
+        t = np.float32(t)
+        largest = np.float32(c_largest * np.log(2.0) * float(t))
+        x = (float(largest) - float(t) * np.concatenate([np.linspace(0, 45, 20000), 36 * rng.random(100000), [0, 1e-8, 60, 1e4]])).astype(np.float32)
+        x = np.append(np.minimum(x, largest), -np.inf).astype(np.float32)
+        w = be.sample_weights(x, largest, t, vocab)
+        z = (x.astype(np.longdouble) - np.longdouble(largest)) / np.longdouble(t)
+        want = np.exp(z) * np.longdouble(2.0) ** bits
+        err = np.abs(w.astype(np.longdouble) - want)
+        assert (err <= want * np.longdouble(2.0) ** -31.8 + 1).all(), (t, float((np.maximum(err - 1, 0) / np.maximum(want, 1)).max()))
+        assert w[x == largest].min() == w.max() == 2 ** bits and w[-1] == 0
