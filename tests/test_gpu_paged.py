@@ -998,3 +998,98 @@ def test_weights_of_the_sampler(be, vocab, c_largest):
         err = np.abs(w.astype(np.longdouble) - want)
         assert (err <= want * np.longdouble(2.0) ** -31.8 + 1).all(), (t, float((np.maximum(err - 1, 0) / np.maximum(want, 1)).max()))
         assert w[x == largest].min() == w.max() == 2 ** bits and w[-1] == 0
+
+
+# ---------------------------------------------------------------------------------------------- every position, by counting
+def check_counts(be, dev, rng, rows, n_kv, h, h_kv, hd, page, causal=True, window=0, max_rows=0, q_pad=0, out_pad=0, out=np.float32):
+    """All keys 0: a row's output is the mean of the values that it sees. Values are small whole numbers, so that every sum on the way (below 2^24) is exact and the output is one
+    quotient, rounded to f32 twice (the reciprocal and the product: 2^-23 of it): a position that is left out, seen twice or another head's shows by at least one part in its number."""
+    n_kv = [max(r, n) for r, n in zip(rows, n_kv)]
+    pool = Pool(rng, n_kv, h_kv, hd, page, fill=0.0)
+    starts = np.concatenate([[0], np.cumsum(rows)]).astype(np.int32)
+    n_rows = int(starts[-1])
+    q_stride, out_stride = h * hd + q_pad, h * hd + out_pad
+    q = np.full((n_rows, q_stride), np.nan, np.float16)
+    q[:, :h * hd] = rng.standard_normal((n_rows, h * hd))
+    out0 = np.full((n_rows, out_stride), 7.5, out)
+    sums = []
+    for s, n in enumerate(n_kv):
+        v = rng.integers(-9, 10, (n, h_kv, hd))
+        pool.put(s, np.zeros(v.shape, np.float16), v.astype(np.float16))
+        sums.append(np.concatenate([np.zeros((1, h_kv, hd), np.int64), np.cumsum(v, axis=0)]))
+        assert np.abs(sums[-1]).max() + 9 * n < 2 ** 24
+    po = dev(out0)
+    batch = B.paged_batch(dev(starts), dev(np.array(n_kv, np.int32)), dev(pool.table), len(rows), n_rows, pool.table.shape[1], max_rows)
+    be.paged_attention(B.paged_attention_desc(pool.cache(dev(pool.k), dev(pool.v)), batch, dev(q), po, h, out_type=B.FP32 if out == np.float32 else B.FP16, causal=causal, window=window,
+                                              q_stride=q_stride, out_stride=out_stride))
+    got = dev.back(po, out0)
+    assert (got[:, h * hd:] == 7.5).all()                    # between the rows
+    got = got[:, :h * hd].reshape(n_rows, h, hd).astype(np.float64)
+    heads = np.arange(h) // (h // h_kv)
+    for s, n in enumerate(n_kv):
+        pos = np.arange(n - rows[s], n)
+        hi = pos + 1 if causal else np.full(rows[s], n)
+        lo = np.maximum(0, hi - window) if window else np.zeros(rows[s], int)
+        total, count = (sums[s][hi] - sums[s][lo])[:, heads], (hi - lo)[:, None, None]
+        want = total / count
+        tol = np.abs(want) * 2.0 ** -23 if out == np.float32 else np.abs(want) * (2.0 ** -11 + 2.0 ** -23) + 2.0 ** -25
+        assert (np.abs(got[starts[s]:starts[s + 1]] - want) <= tol).all(), s
+        if out == np.float32 and rows[s]:                    # sixteen positions less, anywhere, would show
+            at = rng.integers(0, max(1, n - 16), 20)
+            for a in at:
+                less = total[-1] - (sums[s][np.minimum(a + 16, hi[-1])] - sums[s][np.minimum(a, hi[-1])])[heads]
+                assert lo[-1] > a or (np.abs(less / count[-1] - want[-1]) > tol[-1]).any()
+
+
+@pytest.mark.parametrize("hd", [32, 64, 96, 128])
+def test_every_position_of_long_contexts(be, dev, hd):
+    """Items that all CTAs have a piece of: one K/V head, one row to a few."""
+    rng = np.random.default_rng(hd)
+    check_counts(be, dev, rng, [1], [40000], 2, 1, hd, 64, max_rows=1)
+    check_counts(be, dev, rng, [1], [65537], 1, 1, hd, 24, max_rows=1)
+    check_counts(be, dev, rng, [3, 1], [50001, 20011], 4, 1, hd, 16)
+    check_counts(be, dev, rng, [7, 1, 30], [30000, 11, 9001], 5, 1, hd, 32)
+    check_counts(be, dev, rng, [40], [9000], 2, 1, hd, 64)
+
+
+@pytest.mark.parametrize("hd", [64, 96, 128])
+@pytest.mark.parametrize("n_seq", [1, 2, 4, 5, 12, 13, 128, 129, 384, 385, 800])
+def test_every_position_of_many_sequences(be, dev, n_seq, hd):
+    """As many sequences as warps, as threads, and more than either; of no rows, single rows, a few and many."""
+    rng = np.random.default_rng(n_seq)
+    rows = rng.choice([0, 1, 1, 2, 5, 40], n_seq)
+    rows[0] = 3
+    if n_seq <= 13:
+        rows[-1] = 300
+    n_kv = [int(x) for x in rng.integers(1, 400 if n_seq > 20 else 4000, n_seq)]
+    check_counts(be, dev, rng, rows.tolist(), n_kv, 6, 2, hd, 16)
+    check_counts(be, dev, rng, np.minimum(rows, 1).tolist(), n_kv, 6, 2, hd, 16, max_rows=1)
+    check_counts(be, dev, rng, rows.tolist(), n_kv, 2, 1, hd, 8, window=90)
+
+
+@pytest.mark.parametrize("hd", [32, 64, 96, 128])
+def test_every_position_of_sequences_with_many_tiles(be, dev, hd):
+    """More than 32 tiles of rows a sequence, which a CTA finds its place among in several rounds."""
+    rng = np.random.default_rng(hd)
+    check_counts(be, dev, rng, [1300, 2, 1100], [1400, 900, 1100], 2, 2, hd, 16)
+    check_counts(be, dev, rng, [9000], [9100], 1, 1, hd, 64, window=700)
+    check_counts(be, dev, rng, [2300, 700], [2300, 900], 8, 1, hd, 3)
+    check_counts(be, dev, rng, [1200], [2000], 2, 1, hd, 16, causal=False)
+
+
+@pytest.mark.parametrize("hd", [32, 64, 96, 128])
+@pytest.mark.parametrize("out", [np.float32, np.float16])
+def test_rows_with_room_between_them(be, dev, hd, out):
+    """Row strides of Q and of the output that are not the heads' width."""
+    rng = np.random.default_rng(hd)
+    for rows, n_kv in (([1, 1, 3], [300, 41, 90]), ([200, 1, 33], [900, 41, 33]), ([20], [6000])):
+        check_counts(be, dev, rng, rows, n_kv, 4, 2, hd, 16, q_pad=8, out_pad=hd, out=out)
+        check_counts(be, dev, rng, rows, n_kv, 3, 1, hd, 16, q_pad=2 * hd + 24, out_pad=8, out=out)
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+def test_more_query_heads_than_a_tile_has_rows(be, dev, hd):
+    rng = np.random.default_rng(hd)
+    for group in (127, 128, 129, 300):
+        check_counts(be, dev, rng, [1, 5, 20], [300, 41, 700], group, 1, hd, 16)
+        check_attention(be, dev, rng, [1, 3], [130, 41], group, 1, hd, 16)
