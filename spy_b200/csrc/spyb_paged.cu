@@ -36,7 +36,6 @@ __device__ __forceinline__ int sequence_of(const PagedView &v, int row) {   // t
     const int c = __popc(__ballot_sync(0xffffffffu, lane < n && v.row_start[min(lo + lane, v.n_seq)] <= row));
     return lo + c - 1;
 }
-template <class T> struct Eight { float v[8]; };
 __device__ __forceinline__ void load4(const float *p, float *v) { const float4 x = __ldcs(reinterpret_cast<const float4 *>(p)); v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w; }
 __device__ __forceinline__ void load4(const __half *p, float *v) {
     const uint2 x = __ldcs(reinterpret_cast<const uint2 *>(p));
@@ -631,8 +630,19 @@ PagedView view_of(const spyb_paged_cache &c, const spyb_paged_batch &b) {
 
 }  // namespace
 
+// unit `rest` of a sequence whose K/V heads have `one` units each, one tile after the other (paged_plan looks at 32 at a time)
+template <int UNIT, int ALIGN> static void paged_find(const PagedAttention &p, const PagedSeq &q, int64_t one, int64_t rest, int &head, int &tile, int &off) {
+    head = (int)paged_div(rest, one); rest -= head * one;
+    for (tile = 0;; ++tile) {
+        const int u = paged_item<UNIT, ALIGN>(p, q, tile).units + p.start_units;
+        if (rest < u) { break; }
+        rest -= u;
+    }
+    off = (int)rest;                                      // (of the item with its beginning)
+}
 // Host check of how the work is cut: on any lengths, also ones that make no sense, the CTAs' pieces cover every unit of every item once, and every CTA of an item has a place of
-// its own for what it finds. 0 = passed.
+// its own for what it finds. (Items, shares, cuts and places are the kernels' own functions; where a CTA begins is searched here one by one, by the kernels with all threads.)
+// 0 = passed.
 template <int UNIT, int ALIGN> static int cut_selftest(uint32_t seed, int tile_rows) {
     auto rnd = [&](int n) { seed = seed * 1664525u + 1013904223u; return (int)((seed >> 8) % (uint32_t)n); };
     for (int turn = 0; turn < 400; ++turn) {

@@ -96,18 +96,6 @@ __host__ __device__ __forceinline__ int64_t paged_seq_units(const PagedAttention
 __host__ __device__ __forceinline__ int64_t paged_div(int64_t a, int64_t b) {   // (a division of 64 bits costs some 100 instructions)
     return ((a | b) >> 32) == 0 ? (int64_t)((uint32_t)a / (uint32_t)b) : a / b;
 }
-// unit `rest` of a sequence whose K/V heads have `one` units each
-template <int UNIT, int ALIGN>
-__host__ __device__ __forceinline__ void paged_find(const PagedAttention &p, const PagedSeq &q, int64_t one, int64_t rest, int &head, int &tile, int &off) {
-    head = (int)paged_div(rest, one); rest -= head * one;
-    for (tile = 0;; ++tile) {
-        const int u = paged_item<UNIT, ALIGN>(p, q, tile).units + p.start_units;
-        if (rest < u) { break; }
-        rest -= u;
-    }
-    off = (int)rest;                                      // (of the item with its beginning)
-}
-
 // All units cut into `ctas` stretches, the first `longer` of them one longer than the others
 struct PagedShare { int64_t total, each; int ctas, longer; };
 __host__ __device__ __forceinline__ PagedShare paged_share(int64_t total, int ctas) {
