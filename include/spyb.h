@@ -24,7 +24,7 @@ typedef enum { SPYB_SUCCESS = 0, SPYB_FAIL = 1, SPYB_UNSUPPORTED = 2 } spyb_stat
 
 /* NumberType, orchestration/include/number/number_impl/type.h:12-45 (GGML numbering) */
 enum {
-    SPYB_FP32 = 0, SPYB_FP16 = 1, SPYB_Q4_0 = 2, SPYB_Q8_0 = 8, SPYB_Q4_K = 12, SPYB_Q6_K = 14, SPYB_INT32 = 26
+    SPYB_FP32 = 0, SPYB_FP16 = 1, SPYB_Q4_0 = 2, SPYB_Q8_0 = 8, SPYB_Q4_K = 12, SPYB_Q6_K = 14, SPYB_INT8 = 24, SPYB_INT32 = 26
 };
 
 /* OperatorType, orchestration/include/operator/type.h:38-52 (order matters) */
@@ -298,6 +298,67 @@ typedef struct {
 } spyb_paged_attention_desc;
 spyb_status spyb_paged_attention(spyb_backend *backend, const spyb_paged_attention_desc *desc);
 
+/* ---- caches of 8 bits, normalised queries and keys, batches that share a beginning: the two operators above with more to describe.
+ *
+ * A cache of type SPYB_INT8 keeps a byte an element and a scale for each head of each position: an element stands for byte * scale. Strides of its spyb_paged_cache are multiples of 16
+ * elements. `pairs` are fp16 pairs (K's scale, V's); the pair of (page, position in the page, head) lies at page * page_stride + position * token_stride + head * head_stride, in
+ * pairs (4-byte aligned). The scale of a head is the smallest fp16 that is not below its largest magnitude / 127, and its bytes are its elements / scale to the nearest even: off by half
+ * a scale at most. A head of zeros has scale 0. One that holds an infinity, NaN or a magnitude above 65468 (127 of the scale 515.5) has scale NaN: all of it reads as NaN. (Scales that a
+ * caller writes are to be 0 .. 515.5: more than fp16 holds may read as infinities.) */
+typedef struct {
+    void   *pairs;
+    int64_t page_stride, token_stride, head_stride;
+} spyb_paged_scales;
+
+/* spyb_paged_append with a norm of every head of Q and K in front of the rotation, into a cache of SPYB_FP16 or SPYB_INT8: x -> x / sqrt(mean of x^2 + norm_eps) * weight (NormRMS and Mul,
+ * orchestration/include/operator/non-linear.h:117, over a head's elements). q_norm, k_norm: f32 [head_dim], the same for all heads; NULL leaves a norm out. norm_eps: not negative.
+ * Everything is held in f32 (angles in 64 bits) and rounded once. `scales` is of SPYB_INT8 caches, and not read otherwise. The rest is spyb_paged_append's. */
+typedef struct {
+    spyb_paged_append_desc append;
+    spyb_paged_scales scales;
+    const float *q_norm, *k_norm;
+    float   norm_eps;
+    int32_t reserved;
+} spyb_paged_store_desc;
+spyb_status spyb_paged_store(spyb_backend *backend, const spyb_paged_store_desc *desc);
+
+/* K and V of the batch's rows out of the pages, as values: row r of k and v, [n_rows][n_head_kv][head_dim] in out_type SPYB_FP16 or SPYB_FP32 (strides of rows in elements, multiples of 16
+ * bytes; 16-byte aligned), is what the row's position holds. Rows that count a whole sequence give all of it. A position that is "not there" gives zeros, rows of nobody are left as they were. k or v may
+ * be NULL. Cache types, scales and head_dim as spyb_paged_store's. */
+typedef struct {
+    spyb_paged_cache cache;
+    spyb_paged_batch batch;
+    spyb_paged_scales scales;
+    void   *k, *v;
+    int64_t k_stride, v_stride;
+    int32_t out_type, reserved;
+} spyb_paged_load_desc;
+spyb_status spyb_paged_load(spyb_backend *backend, const spyb_paged_load_desc *desc);
+
+/* Which sequences hold the same K and V in their first positions (one system prompt, a document, the trunk of several answers): sequences group_start[g] .. group_start[g+1]-1 (ascending) the same in
+ * their first n_shared[g] ones, usually because their tables name the same pages. Device arrays, read when the kernels run; sequences in no group share nothing. That is a promise about values, and nothing else:
+ * which positions a row sees does not change, and what is shared is read, once for all, from the pages of the group's first sequence that has rows. (It is cut to whole 128 positions that all rows
+ * of the group see, so a window leaves nothing of it.) n_group = 0: nothing is shared, the rest is not read. `workspace`: device memory, 16-byte aligned, of spyb_paged_attend_workspace bytes, this call's until the
+ * backend's stream has passed it; it needs no clearing, and calls that follow one another on a backend may have one. */
+typedef struct {
+    const int32_t *group_start;   /* [n_group + 1] */
+    const int32_t *n_shared;      /* [n_group] */
+    int32_t  n_group, reserved;
+    void    *workspace;
+    uint64_t workspace_bytes;
+} spyb_paged_shared;
+
+/* spyb_paged_attention over a cache of SPYB_FP16 or SPYB_INT8, with what sequences share read once for all of them. For SPYB_INT8 the kernel for many rows rounds byte * scale to fp16 in front of
+ * its products, the one for few rows multiplies scores and probabilities by the scales in f32. A row that sees nothing is zeros; what is not seen has no influence, scales of any value included. */
+typedef struct {
+    spyb_paged_attention_desc attention;
+    spyb_paged_scales scales;
+    spyb_paged_shared shared;
+} spyb_paged_attend_desc;
+spyb_status spyb_paged_attend(spyb_backend *backend, const spyb_paged_attend_desc *desc);
+/* Bytes of workspace that a call with groups of sequences asks for (host arithmetic; 0 where a size makes no sense). */
+uint64_t spyb_paged_attend_workspace(int32_t n_seq, int32_t n_rows, int32_t n_head, int32_t head_dim);
+
 /* The next token of every row of logits [n_rows][n_vocab] (row_stride elements apart; SPYB_FP32 or SPYB_FP16): SamplerImpl<Greedy>::sample
  * (model/include/llm/sampler/greedy.h:20-25) with the usual settings, one of each a row; a NULL array leaves the setting out.
  *   w_i = exp((logit_i - largest) / temperature); temperature NULL: 1; not above 0: the largest logit, the lowest index among equals
@@ -329,10 +390,13 @@ spyb_status spyb_sample_weights(spyb_backend *backend, const float *logits_host,
  * late: waits give up, the kernel returns by itself when the copy has landed, error_code_out is 7, the error is cleared and the next launch is right. */
 spyb_status spyb_paged_selftest_late(spyb_backend *backend, int32_t who, uint64_t limit_ns, int32_t *error_code_out);
 
-/* What the three calls above would answer to a descriptor, and why in `message` (up to `size` bytes with the closing 0; may be NULL with size 0): host
+/* What the calls above would answer to a descriptor, and why in `message` (up to `size` bytes with the closing 0; may be NULL with size 0): host
  * arithmetic only, no GPU needed. */
 spyb_status spyb_paged_append_check(const spyb_paged_append_desc *desc, char *message, int32_t size);
 spyb_status spyb_paged_attention_check(const spyb_paged_attention_desc *desc, char *message, int32_t size);
+spyb_status spyb_paged_store_check(const spyb_paged_store_desc *desc, char *message, int32_t size);
+spyb_status spyb_paged_load_check(const spyb_paged_load_desc *desc, char *message, int32_t size);
+spyb_status spyb_paged_attend_check(const spyb_paged_attend_desc *desc, char *message, int32_t size);
 spyb_status spyb_sample_check(const spyb_sample_desc *desc, char *message, int32_t size);
 
 /* ---- whole-model path: the graph LLAMAModel::build_graph emits (model/src/llm/model/llama.cpp:86-264)

@@ -18,7 +18,7 @@ _PKG = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_PKG, "libspyb200.so")
 
 SUCCESS, FAIL, UNSUPPORTED = 0, 1, 2
-FP32, FP16, Q4_0, Q8_0, Q4_K, Q6_K, INT32 = 0, 1, 2, 8, 12, 14, 26
+FP32, FP16, Q4_0, Q8_0, Q4_K, Q6_K, INT8, INT32 = 0, 1, 2, 8, 12, 14, 24, 26
 OP = dict(Input=0, Nop=1, Dup=2, Copy=3, View=4, Reshape=5, GetRow=8, Transpose=9, Permute=10, Contiguous=11, Silu=13,
           Softmax=17, Add=18, Mul=20, MatMul=23, NormRMS=26, Rope=27)
 NODE_CONSTANT, NODE_IO, NODE_CACHE, NODE_DYNAMIC = 0, 1, 2, 6
@@ -82,6 +82,27 @@ class PagedAttentionDesc(C.Structure):
                 ("out_type", C.c_int32), ("causal", C.c_int32), ("window", C.c_int32), ("scale", C.c_float), ("reserved", C.c_int32)]
 
 
+class PagedScales(C.Structure):
+    _fields_ = [("pairs", C.c_void_p), ("page_stride", C.c_int64), ("token_stride", C.c_int64), ("head_stride", C.c_int64)]
+
+
+class PagedShared(C.Structure):
+    _fields_ = [("group_start", C.c_void_p), ("n_shared", C.c_void_p), ("n_group", C.c_int32), ("reserved", C.c_int32), ("workspace", C.c_void_p), ("workspace_bytes", C.c_uint64)]
+
+
+class PagedStoreDesc(C.Structure):
+    _fields_ = [("append", PagedAppendDesc), ("scales", PagedScales), ("q_norm", C.c_void_p), ("k_norm", C.c_void_p), ("norm_eps", C.c_float), ("reserved", C.c_int32)]
+
+
+class PagedLoadDesc(C.Structure):
+    _fields_ = [("cache", PagedCache), ("batch", PagedBatch), ("scales", PagedScales), ("k", C.c_void_p), ("v", C.c_void_p), ("k_stride", C.c_int64), ("v_stride", C.c_int64),
+                ("out_type", C.c_int32), ("reserved", C.c_int32)]
+
+
+class PagedAttendDesc(C.Structure):
+    _fields_ = [("attention", PagedAttentionDesc), ("scales", PagedScales), ("shared", PagedShared)]
+
+
 class SampleDesc(C.Structure):
     _fields_ = [("logits", C.c_void_p), ("row_stride", C.c_int64), ("number_type", C.c_int32), ("n_rows", C.c_int32), ("n_vocab", C.c_int32), ("reserved", C.c_int32),
                 ("temperature", C.c_void_p), ("top_k", C.c_void_p), ("top_p", C.c_void_p), ("min_p", C.c_void_p), ("uniform", C.c_void_p), ("ids", C.c_void_p), ("probs", C.c_void_p)]
@@ -126,11 +147,18 @@ def lib():
         "spyb_attention": (i32, [vp, vp, vp, vp, vp, i32, i32, i32, i32, i32, i32]),
         "spyb_paged_append": (i32, [vp, C.POINTER(PagedAppendDesc)]),
         "spyb_paged_attention": (i32, [vp, C.POINTER(PagedAttentionDesc)]),
+        "spyb_paged_store": (i32, [vp, C.POINTER(PagedStoreDesc)]),
+        "spyb_paged_load": (i32, [vp, C.POINTER(PagedLoadDesc)]),
+        "spyb_paged_attend": (i32, [vp, C.POINTER(PagedAttendDesc)]),
+        "spyb_paged_attend_workspace": (u64, [i32, i32, i32, i32]),
         "spyb_sample": (i32, [vp, C.POINTER(SampleDesc)]),
         "spyb_sample_weights": (i32, [vp, vp, i32, C.c_float, C.c_float, i32, vp]),
         "spyb_paged_selftest_late": (i32, [vp, i32, u64, C.POINTER(i32)]),
         "spyb_paged_append_check": (i32, [C.POINTER(PagedAppendDesc), C.c_char_p, i32]),
         "spyb_paged_attention_check": (i32, [C.POINTER(PagedAttentionDesc), C.c_char_p, i32]),
+        "spyb_paged_store_check": (i32, [C.POINTER(PagedStoreDesc), C.c_char_p, i32]),
+        "spyb_paged_load_check": (i32, [C.POINTER(PagedLoadDesc), C.c_char_p, i32]),
+        "spyb_paged_attend_check": (i32, [C.POINTER(PagedAttendDesc), C.c_char_p, i32]),
         "spyb_sample_check": (i32, [C.POINTER(SampleDesc), C.c_char_p, i32]),
         "spyb_model_read_activation": (i32, [vp, i32, vp, u64]),
         "spyb_model_bench_kernel": (C.c_float, [vp, i32, i32, C.POINTER(u64)]),
@@ -206,14 +234,22 @@ def make_tensor(data_ptr, number_type: int, ne, nb=None, node_type: int = NODE_D
     return t
 
 
-def paged_cache(k_ptr, v_ptr, n_pages: int, page_size: int, n_head_kv: int, head_dim: int, token_major: bool = False, strides=None) -> PagedCache:
-    """fp16 keys and values in pages: [page][head][position][element], or [page][position][head][element] (token_major), or with the given strides
-    (page, position, head) in elements."""
-    c = PagedCache(k_ptr, v_ptr, FP16, n_pages, page_size, n_head_kv, head_dim, 0)
+def paged_cache(k_ptr, v_ptr, n_pages: int, page_size: int, n_head_kv: int, head_dim: int, token_major: bool = False, strides=None, number_type: int = FP16) -> PagedCache:
+    """Keys and values in pages, fp16 or (for paged_store, paged_load and paged_attend) INT8: [page][head][position][element], or [page][position][head][element]
+    (token_major), or with the given strides (page, position, head) in elements."""
+    c = PagedCache(k_ptr, v_ptr, number_type, n_pages, page_size, n_head_kv, head_dim, 0)
     if strides is None:
         strides = (page_size * n_head_kv * head_dim, n_head_kv * head_dim, head_dim) if token_major else (page_size * n_head_kv * head_dim, head_dim, page_size * head_dim)
     c.page_stride, c.token_stride, c.head_stride = strides
     return c
+
+
+def paged_scales(pairs_ptr, page_size: int, n_head_kv: int, token_major: bool = False, strides=None) -> PagedScales:
+    """Scales of an INT8 cache, fp16 pairs (K's, V's): [page][head][position][2], or [page][position][head][2] (token_major), or with the given strides (page, position,
+    head) in pairs."""
+    if strides is None:
+        strides = (page_size * n_head_kv, n_head_kv, 1) if token_major else (page_size * n_head_kv, 1, page_size)
+    return PagedScales(pairs_ptr, *strides)
 
 
 def paged_batch(row_start_ptr, n_kv_ptr, page_table_ptr, n_seq: int, n_rows: int, table_stride: int, max_rows: int = 0) -> PagedBatch:
@@ -239,6 +275,29 @@ def paged_attention_desc(cache: PagedCache, batch: PagedBatch, q, out, n_head: i
                               scale, 0)
 
 
+def paged_store_desc(append: PagedAppendDesc, scales: PagedScales | None = None, q_norm=None, k_norm=None, norm_eps: float = 0.0) -> PagedStoreDesc:
+    """An append with norms of Q's and K's heads in front of the rotation (device arrays of head_dim f32; None leaves one out) and, for an INT8 cache, its scales."""
+    return PagedStoreDesc(append, scales or PagedScales(), q_norm, k_norm, norm_eps, 0)
+
+
+def paged_load_desc(cache: PagedCache, batch: PagedBatch, k, v, scales: PagedScales | None = None, out_type: int = FP16, k_stride=None, v_stride=None) -> PagedLoadDesc:
+    """k, v: [rows][n_head_kv][head_dim] in out_type, what the rows' positions hold (None leaves one out)."""
+    width = cache.n_head_kv * cache.head_dim
+    return PagedLoadDesc(cache, batch, scales or PagedScales(), k, v, width if k_stride is None else k_stride, width if v_stride is None else v_stride, out_type, 0)
+
+
+def paged_attend_workspace(n_seq: int, n_rows: int, n_head: int, head_dim: int) -> int:
+    """Bytes of device memory that paged_attend wants for a batch with groups of sequences that share their beginning."""
+    return lib().spyb_paged_attend_workspace(n_seq, n_rows, n_head, head_dim)
+
+
+def paged_attend_desc(attention: PagedAttentionDesc, scales: PagedScales | None = None, group_start=None, n_shared=None, n_group: int = 0, workspace=None,
+                      workspace_bytes: int = 0) -> PagedAttendDesc:
+    """Attention over an fp16 cache or an INT8 one with its scales; group_start [n_group + 1], n_shared [n_group]: int32 device arrays, sequences group_start[g] ..
+    group_start[g+1]-1 hold the same K and V in their first n_shared[g] positions."""
+    return PagedAttendDesc(attention, scales or PagedScales(), PagedShared(group_start, n_shared, n_group, 0, workspace, workspace_bytes))
+
+
 def sample_desc(logits, number_type: int, n_rows: int, n_vocab: int, ids, uniform=None, temperature=None, top_k=None, top_p=None, min_p=None, probs=None,
                 row_stride=None) -> SampleDesc:
     """logits [n_rows][n_vocab]; settings and uniform numbers: device arrays with one value a row, None leaves a setting out; ids int32, probs f32 (optional)."""
@@ -246,8 +305,9 @@ def sample_desc(logits, number_type: int, n_rows: int, n_vocab: int, ids, unifor
 
 
 def refusal(desc) -> str:
-    """Why paged_append, paged_attention or sample would not take this descriptor ("" if they would); no GPU needed."""
-    check = {PagedAppendDesc: lib().spyb_paged_append_check, PagedAttentionDesc: lib().spyb_paged_attention_check, SampleDesc: lib().spyb_sample_check}[type(desc)]
+    """Why the operator that a descriptor of paged pages or of sampling is for would not take it ("" if it would); no GPU needed."""
+    check = {PagedAppendDesc: lib().spyb_paged_append_check, PagedAttentionDesc: lib().spyb_paged_attention_check, PagedStoreDesc: lib().spyb_paged_store_check,
+             PagedLoadDesc: lib().spyb_paged_load_check, PagedAttendDesc: lib().spyb_paged_attend_check, SampleDesc: lib().spyb_sample_check}[type(desc)]
     buf = C.create_string_buffer(256)
     return "" if check(C.byref(desc), buf, len(buf)) == SUCCESS else buf.value.decode()
 
@@ -268,6 +328,7 @@ class B200Backend:
                  use_graph: bool = True, arena_bytes: int = 0):
         self._l = lib()
         self._submit = self._l.spyb_submit
+        self._paged_store, self._paged_load, self._paged_attend = self._l.spyb_paged_store, self._l.spyb_paged_load, self._l.spyb_paged_attend
         self._paged_append, self._paged_attention, self._sample = self._l.spyb_paged_append, self._l.spyb_paged_attention, self._l.spyb_sample
         cfg = Config(device_id, tp_size, tp_rank, int(use_pdl), int(use_graph), 0, arena_bytes)
         h = C.c_void_p()
@@ -354,6 +415,24 @@ class B200Backend:
     def paged_attention(self, desc: PagedAttentionDesc) -> None:
         """Attention of the rows over their sequences' pages."""
         st = self._paged_attention(self.h, C.byref(desc))
+        if st != SUCCESS:
+            self._check(st)
+
+    def paged_store(self, desc: PagedStoreDesc) -> None:
+        """paged_append with norms of Q's and K's heads, into fp16 or 8-bit pages."""
+        st = self._paged_store(self.h, C.byref(desc))
+        if st != SUCCESS:
+            self._check(st)
+
+    def paged_load(self, desc: PagedLoadDesc) -> None:
+        """K and V of the rows' positions, out of the pages, as values."""
+        st = self._paged_load(self.h, C.byref(desc))
+        if st != SUCCESS:
+            self._check(st)
+
+    def paged_attend(self, desc: PagedAttendDesc) -> None:
+        """paged_attention over fp16 or 8-bit pages, with what sequences share read once for all of them."""
+        st = self._paged_attend(self.h, C.byref(desc))
         if st != SUCCESS:
             self._check(st)
 

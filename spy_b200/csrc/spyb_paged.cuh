@@ -3,11 +3,13 @@
 
 #include "spyb_common.cuh"
 #include "spyb_kernels.h"
+#include "../../include/spyb.h"
 
 namespace spyb {
 
 struct PagedView {                        // a spyb_paged_cache and a spyb_paged_batch as the kernels read them
-    const int32_t *row_start = nullptr, *n_kv = nullptr, *page_table = nullptr;
+    const int32_t *row_start = nullptr, *row_end = nullptr, *n_kv = nullptr, *page_table = nullptr;   // (row_end: row_start + 1, or an array of its own)
+    const int32_t *from = nullptr;        // positions in front of it (a multiple of PA_SHARED) are not this pass's; nullptr: all are
     int            n_seq = 0, n_rows = 0, table_stride = 0, n_pages = 0, page_size = 1;
     int            n_kv_most = 0;         // positions that a row of the table can name
     int64_t        page_stride = 0, token_stride = 0, head_stride = 0;
@@ -23,6 +25,9 @@ struct PagedAppend {
 };
 // the warps that check V stay a few microseconds behind everything else; one copy of a CTA's K and V, or its first of Q, comes three limits of the waits late
 enum PagedLate { PA_ON_TIME = 0, PA_LATE_CHECKS = 1, PA_LATE_KV = 2, PA_LATE_Q = 3 };
+// What a kernel of attention is built for: an fp16 cache whose sequences have nothing in common; one of the two passes where they have; bytes with scales, in passes or not
+enum PagedKind { PK_PLAIN = 0, PK_SHARED = 1, PK_INT8 = 2 };
+struct PagedScales { const uint32_t *pairs = nullptr; int64_t page_stride = 0, token_stride = 0, head_stride = 0; };   // fp16 pairs: K's scale below, V's above
 struct PagedAttention {
     PagedView    view;
     const __half *q = nullptr, *k = nullptr, *v = nullptr;
@@ -37,16 +42,53 @@ struct PagedAttention {
     float       *partial = nullptr;       // [CTAs][2][rows of a tile][head_dim + 2]
     unsigned    *arrived = nullptr;       // [CTAs], zero between launches
     int          late = PA_ON_TIME;       // self-checks of the tensor-memory kernel
+    PagedScales  scales;                  // of an 8-bit cache
+    float2      *stats = nullptr;         // first pass of two, over what sequences share: every row's maximum and sum go here, its accumulators as they are to `out` (f32), both [row][head]
+    const float2 *with_stats = nullptr;   // second pass: these are joined with what is found
+    const float  *with_out = nullptr;
+    __host__ __device__ int kind() const { return scales.pairs != nullptr ? PK_INT8 : stats != nullptr || with_stats != nullptr ? PK_SHARED : PK_PLAIN; }
 };
+struct PagedStore {
+    PagedAppend   append;
+    const float  *q_norm = nullptr, *k_norm = nullptr;
+    float         eps = 0.f;
+    uint8_t      *k8 = nullptr, *v8 = nullptr;       // an 8-bit cache, in place of append's
+    PagedScales   scales;                            // (written)
+};
+struct PagedLoad {
+    PagedView    view;
+    const void  *k = nullptr, *v = nullptr;
+    PagedScales  scales;
+    void        *k_out = nullptr, *v_out = nullptr;
+    int64_t      k_stride = 0, v_stride = 0;
+    int          n_head_kv = 0, head_dim = 0;
+};
+struct PagedShared {                      // which sequences share what, and what becomes of it (PA_SHARED)
+    PagedView      view;
+    const int32_t *group_start = nullptr, *n_shared = nullptr;
+    int            n_group = 0, causal = 1;
+    int32_t       *from = nullptr, *row_end = nullptr, *kv = nullptr;   // [n_seq] each: where a sequence's own positions begin; rows and positions of the first pass's sequences
+};
+constexpr int PA_SHARED = 128;            // what is shared is cut to a multiple of so many positions: both kernels' blocks begin at such ones
 int         paged_cut_selftest();   // host-only: 0 when the CTAs' pieces cover every item once, on any lengths
+cudaError_t launch_paged_store(const PagedStore &p, int in_type, int q_out_type, int sms, const LaunchCfg &cfg);
+cudaError_t launch_paged_load(const PagedLoad &p, int out_type, int sms, const LaunchCfg &cfg);
+cudaError_t launch_paged_shared(const PagedShared &p, const LaunchCfg &cfg);
 cudaError_t launch_paged_append(const PagedAppend &p, int in_type, int q_out_type, int sms, const LaunchCfg &cfg);
 cudaError_t launch_paged_attention_rows(const PagedAttention &p, int head_dim, int row_tiles, int sms, const LaunchCfg &cfg);
+cudaError_t launch_paged_attend_rows(const PagedAttention &p, int head_dim, int row_tiles, int sms, const LaunchCfg &cfg);   // (kinds other than PK_PLAIN)
 // the kernel on tensor memory; false where it does not take these pages, heads or strides (nothing is launched then)
 bool        launch_paged_attention_tc(const PagedAttention &p, int head_dim, int n_head, int sms, const LaunchCfg &cfg, uint64_t wait_limit, cudaError_t *err);
 // Sequences of up to so many rows (times query heads of a K/V head) are the small kernel's, whose tile of 16 rows costs them nothing but the memory's time; a second tile
 // doubles its instructions. 24 sequences of up to 9000 positions, four query heads a K/V head: 3 and 4 rows (12 and 16 in all) 95 and 98 us there against
 // 118 and 118 on tensor memory, 5 and 8 rows (20 and 32) 144 and 156 against 118 and 118.
 constexpr int PA_FEW_ROWS = 16;
+
+// What every operator asks of the cache and the batch; `scales`: those that may come with bytes (nullptr: an fp16 cache alone)
+struct Refusal;
+spyb_status paged_check_view(Refusal &no, const char *what, const spyb_paged_cache &c, const spyb_paged_batch &b, const spyb_paged_scales *scales = nullptr);
+PagedView   paged_view(const spyb_paged_cache &c, const spyb_paged_batch &b);
+PagedScales paged_scales_of(const spyb_paged_cache &c, const spyb_paged_scales &s);
 
 // ---------------------------------------------------------------------------------------------- cutting the work
 // The rows of a sequence that share a K/V head - token by token, its query heads side by side - are cut into tiles; a tile and a K/V head are an item, and the
@@ -58,7 +100,7 @@ constexpr int PA_FEW_ROWS = 16;
 // Tensor memory, of 128: 24 x 5 rows of up to 9000 117.5 / 109.7 / 110.6 / 113.2, 512 rows at 3968 54.7 / 53.1 / 52.2 / 52.4, prompts of 6 under a window
 // 225.8 / 209.0 / 211.3 / 218.9, 512 at 1024 34.5 / 27.3 / 28.4 / 30.0.
 constexpr int PA_START = 2;
-struct PagedSeq { int row0, rows, first, kv; };   // first row and number of rows, position of the first row, positions that are there
+struct PagedSeq { int row0, rows, first, kv, from; };   // first row and number of rows, position of the first row, positions that are there, and the first of them that this pass reads
 struct PagedItem { int lo, hi, units; };          // positions [lo, hi) that some row of the tile sees (lo a multiple of ALIGN)
 
 __host__ __device__ __forceinline__ int pmin(int a, int b) { return a < b ? a : b; }
@@ -66,9 +108,9 @@ __host__ __device__ __forceinline__ int pmax(int a, int b) { return a < b ? b : 
 // Positions are below 2^30: a window of as many hides nothing, and a position minus a window stays in 32 bits also for rows in front of position 0
 inline int paged_window(int window) { return pmin(window, 1 << 30); }
 __host__ __device__ __forceinline__ PagedSeq paged_seq(const PagedView &v, int s) {
-    const int a = pmax(0, pmin(v.row_start[s], v.n_rows)), end = pmax(a, pmin(v.row_start[s + 1], 1 << 24)), b = pmin(end, v.n_rows);
+    const int a = pmax(0, pmin(v.row_start[s], v.n_rows)), end = pmax(a, pmin(v.row_end[s], 1 << 24)), b = pmin(end, v.n_rows);
     const int kv = pmin(pmax(0, v.n_kv[s]), 1 << 30);
-    return {a, b - a, kv - (end - a), pmin(kv, v.n_kv_most)};
+    return {a, b - a, kv - (end - a), pmin(kv, v.n_kv_most), v.from != nullptr ? v.from[s] : 0};
 }
 template <int UNIT, int ALIGN>
 __host__ __device__ __forceinline__ PagedItem paged_item(const PagedAttention &p, const PagedSeq &q, int tile) {
@@ -76,7 +118,7 @@ __host__ __device__ __forceinline__ PagedItem paged_item(const PagedAttention &p
     const int i0 = (int)((unsigned)(tile * p.tile_rows) / (unsigned)p.group), i1 = (int)((unsigned)last / (unsigned)p.group);
     PagedItem t;
     t.hi = p.causal ? pmin(q.kv, q.first + i1 + 1) : q.kv;
-    t.lo = p.causal && p.window > 0 ? pmax(0, q.first + i0 - p.window + 1) / ALIGN * ALIGN : 0;
+    t.lo = p.causal && p.window > 0 ? pmax(0, q.first + i0 - p.window + 1) / ALIGN * ALIGN : q.from;   // (a window leaves nothing to share)
     t.units = pmax(1, (t.hi - t.lo + UNIT - 1) / UNIT);   // (an item without positions still has its zeros to write)
     return t;
 }
@@ -214,5 +256,56 @@ __host__ __device__ __forceinline__ PagedCut paged_cut(const PagedPlace &at, int
     return {a, b - a + 1};
 }
 __host__ __device__ __forceinline__ int64_t paged_slot(int c, int c0) { return 2 * (int64_t)c + (c == c0 ? 1 : 0); }
+
+// What the first pass found for four elements of a row, into what the second one did (maxima in powers of two)
+__device__ __forceinline__ void paged_join_pass(float4 &v, float &l, float m, float2 with, float4 u) {
+    const float top = fmaxf(m, with.x), base = top == -INFINITY ? 0.f : top, f = exp2f(m - base), w = exp2f(with.x - base);
+    v = make_float4(f * v.x + w * u.x, f * v.y + w * u.y, f * v.z + w * u.z, f * v.w + w * u.w);
+    l = f * l + w * with.y;
+}
+
+// ---------------------------------------------------------------------------------------------- bytes
+// Four signed bytes as fp16 numbers, without an error: the byte plus 128 is the low half of the mantissa of 1024 + it, and 1152 is taken off.
+__device__ __forceinline__ uint32_t sub_1152(uint32_t h2) {
+    uint32_t r;
+    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(h2), "r"(0x64806480u));
+    return r;
+}
+__device__ __forceinline__ void halves_of(uint32_t w, uint32_t &lo, uint32_t &hi) {
+    w ^= 0x80808080u;
+    lo = sub_1152(__byte_perm(w, 0x64646464u, 0x4140)); hi = sub_1152(__byte_perm(w, 0x64646464u, 0x4342));
+}
+// of two words, the pairs of bytes that have the same place
+__device__ __forceinline__ void pairs_of(uint32_t a, uint32_t b, uint32_t (&h2)[4]) {
+    a ^= 0x80808080u; b ^= 0x80808080u;
+    const uint32_t lo = __byte_perm(a, b, 0x5140), hi = __byte_perm(a, b, 0x7362);
+    h2[0] = sub_1152(__byte_perm(lo, 0x64646464u, 0x4140)); h2[1] = sub_1152(__byte_perm(lo, 0x64646464u, 0x4342));
+    h2[2] = sub_1152(__byte_perm(hi, 0x64646464u, 0x4140)); h2[3] = sub_1152(__byte_perm(hi, 0x64646464u, 0x4342));
+}
+__device__ __forceinline__ float2 half2_bits(uint32_t x) { return __half22float2(*reinterpret_cast<const __half2 *>(&x)); }
+
+// ---------------------------------------------------------------------------------------------- rows and elements
+__device__ __forceinline__ int sequence_of(const PagedView &v, int row) {   // the last s with row_start[s] <= row, by a whole warp; -1 and n_seq: nobody's
+    const int lane = threadIdx.x & 31;
+    int lo = 0, n = v.n_seq + 1;
+    while (n > 32) {
+        const int step = (n + 31) / 32, i = lo + lane * step;
+        const int c = __popc(__ballot_sync(0xffffffffu, lane * step < n && v.row_start[min(i, v.n_seq)] <= row));
+        if (c == 0) { return -1; }
+        lo += (c - 1) * step;
+        n = min(step, v.n_seq + 1 - lo);
+    }
+    const int c = __popc(__ballot_sync(0xffffffffu, lane < n && v.row_start[min(lo + lane, v.n_seq)] <= row));
+    return lo + c - 1;
+}
+__device__ __forceinline__ void load4(const float *p, float *v) { const float4 x = __ldcs(reinterpret_cast<const float4 *>(p)); v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w; }
+__device__ __forceinline__ void load4(const __half *p, float *v) {
+    const uint2 x = __ldcs(reinterpret_cast<const uint2 *>(p));
+    const float2 a = __half22float2(*reinterpret_cast<const __half2 *>(&x.x)), b = __half22float2(*reinterpret_cast<const __half2 *>(&x.y));
+    v[0] = a.x; v[1] = a.y; v[2] = b.x; v[3] = b.y;
+}
+__device__ __forceinline__ uint32_t pack2(float a, float b) { const __half2 h = __floats2half2_rn(a, b); return *reinterpret_cast<const uint32_t *>(&h); }
+__device__ __forceinline__ void store4(float *p, const float *v) { *reinterpret_cast<float4 *>(p) = make_float4(v[0], v[1], v[2], v[3]); }
+__device__ __forceinline__ void store4(__half *p, const float *v) { *reinterpret_cast<uint2 *>(p) = make_uint2(pack2(v[0], v[1]), pack2(v[2], v[3])); }
 
 }  // namespace spyb

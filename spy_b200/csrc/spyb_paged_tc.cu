@@ -779,6 +779,7 @@ static int paged_tc_box(int page_size) {   // positions of a box: the largest po
 bool launch_paged_attention_tc(const PagedAttention &given, int head_dim, int n_head, int sms, const LaunchCfg &cfg, uint64_t wait_limit, cudaError_t *err) {
     const int box = paged_tc_box(given.view.page_size);
     const PagedView &view = given.view;
+    if (given.kind() != PK_PLAIN) { return false; }
     const int64_t most = std::max({view.token_stride, view.head_stride, view.page_stride, given.q_stride}), least = std::min({view.token_stride, view.head_stride, view.page_stride, given.q_stride});
     if ((head_dim != 64 && head_dim != 128) || box < 8 || given.group > PT_ROWS || least <= 0 || most >= (1ll << 38)) { return false; }
     PagedAttention p = given;
