@@ -34,11 +34,14 @@ constexpr int PT_THREADS = 384, PT_ROWS = 128, PT_KEYS = 128;
 constexpr int PT_REGS_SOFTMAX = 208, PT_REGS_OTHERS = 88;   // 256 x 208 + 128 x 88 = 384 x 168, what the block is launched with
 constexpr uint32_t PT_HALF = PT_KEYS * 128;              // bytes of 128 rows x 64 elements
 
-template <int HD> struct TcShape {
+template <int HD, int KIND> struct TcShape {
     static constexpr uint32_t OPERAND = PT_KEYS * HD * 2;                      // a tile of Q, K or V
-    static constexpr int SLOTS = HD == 128 ? 5 : 8;                            // K and V tiles in flight
+    static constexpr bool BYTES = KIND == PK_INT8;
+    static constexpr int SLOTS = BYTES ? (HD == 128 ? 3 : 4) : HD == 128 ? 5 : 8;   // K and V tiles in flight; of bytes: made into operands ahead
+    static constexpr int BYTE_SLOTS = BYTES ? (HD == 128 ? 4 : 6) : 0;         // tiles of bytes in flight
+    static constexpr uint32_t BYTE_TILE = PT_KEYS * HD;
     static constexpr int Q_BUFFERS = HD == 128 ? 1 : 2;                        // (heads of 64: the next stretch's Q comes while this one's is in use; there is room for it)
-    static constexpr uint32_t SMEM = (2 * Q_BUFFERS + SLOTS) * OPERAND + 1024; // (+ alignment)
+    static constexpr uint32_t SMEM = (2 * Q_BUFFERS + SLOTS) * OPERAND + BYTE_SLOTS * BYTE_TILE + 1024; // (+ alignment)
     // tensor memory: S of both tiles, then O of both; P over S, or for heads of 64, whose O leaves room, beside it: the next S is made while P is
     static constexpr bool P_APART = HD == 64;
     static constexpr uint32_t P_COLUMN = P_APART ? 256 : 0, P_STEP = P_APART ? 64 : 128, O_COLUMN = P_APART ? 384 : 256;
@@ -69,6 +72,7 @@ constexpr int PT_ENTRIES = 4, PT_READERS = 11;       // stretches known ahead; w
 struct TcShared {
     uint64_t full[8], empty[8];                          // a slot's copies have landed; its last MMA is done, and both warps that check V have seen its phase
     uint64_t clean[8];                                   // of the last V tiles: what nobody sees is cleared
+    uint64_t byte_full[8], byte_empty[8];                // 8-bit caches: a tile of bytes has landed; both warps have made its operand (`full` is that operand's, `empty` its last MMA's)
     uint64_t q_ready[2][2], q_free[2][2];                // of the two tiles and their buffers, in stretches in which they see anything
     uint64_t s_ready[2], s_free[2], p_ready[2][2], p_free[2], o_ready[2];   // (P ready) of the first 96 positions and the rest; (free) where P lies apart
     uint64_t known[PT_ENTRIES], read[PT_ENTRIES];        // an entry is there; all have read it
@@ -170,10 +174,43 @@ __device__ __noinline__ void stand_still(uint64_t ns) {
 }
 
 // LATE: the self-checks' kernels (p.late)
-template <int HD, bool LATE>
+// Bytes of 64 positions (row0 on) of a tile as an operand: byte x scale, rounded to fp16. A lane has 16 bytes at a time, a quarter of a warp one row or two; `pairs`: the scales of positions
+// row0 + lane and row0 + 32 + lane, K's below and V's above. (Lanes of the operand's second half write their two pieces the other way round: eight lanes, eight places in the banks.)
+template <int HD> __device__ __forceinline__ void make_operand(uint32_t bytes, uint32_t operand, int row0, uint32_t scale0, uint32_t scale1, bool is_v) {
+    constexpr int PER = HD / 16, AT_ONCE = 32 / PER, LOOPS = 64 / AT_ONCE;
+    const int lane = threadIdx.x & 31, c = lane % PER, r0 = lane / PER;
+    const uint32_t sel = is_v ? 0x3232 : 0x1010;
+    const int swap = HD == 128 ? c >> 2 : 0;
+    const uint32_t src = bytes + (row0 + r0) * HD + c * 16, half = operand + (c >> 2) * PT_HALF;
+#pragma unroll 4
+    for (int i = 0; i < LOOPS; ++i) {
+        const int r = i * AT_ONCE + r0;                                // (of the 64)
+        const uint4 w = lds128(src + i * (AT_ONCE * HD));
+        const uint32_t pair = __shfl_sync(0xffffffffu, i * AT_ONCE < 32 ? scale0 : scale1, r & 31);
+        const uint32_t d = __byte_perm(pair, 0, sel);
+        uint32_t h[8];
+        halves_of(w.x, h[0], h[1]); halves_of(w.y, h[2], h[3]); halves_of(w.z, h[4], h[5]); halves_of(w.w, h[6], h[7]);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) { asm("mul.rn.f16x2 %0, %0, %1;" : "+r"(h[e]) : "r"(d)); }
+        const uint32_t row = half + (row0 + r) * 128;
+        const int first = (2 * (c & 3) + swap) ^ (r & 7);              // (row0 is a multiple of 8)
+        sts128(row + first * 16, swap ? make_uint4(h[4], h[5], h[6], h[7]) : make_uint4(h[0], h[1], h[2], h[3]));
+        sts128(row + (first ^ 1) * 16, swap ? make_uint4(h[0], h[1], h[2], h[3]) : make_uint4(h[4], h[5], h[6], h[7]));
+    }
+}
+// a scale beyond what bytes of fp16 values have is an infinity, as its elements may be
+__device__ __forceinline__ bool large_scale(uint32_t h) { return (h & 0x7fffu) > 0x6007u; }   // 515.5
+__device__ __forceinline__ uint32_t no_large_scale(uint32_t pair) {
+    if (large_scale(pair) && (pair & 0x7fffu) <= 0x7c00u) { pair = (pair & 0xffff8000u) | 0x7c00u; }
+    if (large_scale(pair >> 16) && (pair >> 16 & 0x7fffu) <= 0x7c00u) { pair = (pair & 0x8000ffffu) | 0x7c000000u; }
+    return pair;
+}
+
+template <int HD, bool LATE, int KIND>
 __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_constant__ PagedAttention p, const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
                                                                   const int box, int *error_flag, const uint64_t wait_limit) {
-    using Shape = TcShape<HD>;
+    using Shape = TcShape<HD, KIND>;
+    constexpr bool BYTES = Shape::BYTES;
     constexpr int SLOTS = Shape::SLOTS;
     extern __shared__ uint8_t raw[];
     __shared__ TcShared sh;
@@ -182,8 +219,10 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
     const uint32_t full = smem_u32(sh.full), empty = smem_u32(sh.empty), clean = smem_u32(sh.clean), known = smem_u32(sh.known), read = smem_u32(sh.read), joined = smem_u32(sh.joined);
     const uint32_t q_ready = smem_u32(sh.q_ready), q_free = smem_u32(sh.q_free), s_ready = smem_u32(sh.s_ready), s_free = smem_u32(sh.s_free), p_ready = smem_u32(sh.p_ready),
                    o_ready = smem_u32(sh.o_ready), p_free = smem_u32(sh.p_free);
+    const uint32_t byte_full = smem_u32(sh.byte_full), byte_empty = smem_u32(sh.byte_empty), byte_ring = ring + SLOTS * Shape::OPERAND;
     if (tid == 0) {
-        for (int i = 0; i < 8; ++i) { mbar_init(full + 8 * i, 1); mbar_init(empty + 8 * i, 3); mbar_init(clean + 8 * i, 2); sh.poison[i] = 0; }
+        for (int i = 0; i < 8; ++i) { mbar_init(full + 8 * i, BYTES ? 2 : 1); mbar_init(empty + 8 * i, BYTES ? 1 : 3); mbar_init(clean + 8 * i, 2); sh.poison[i] = 0; }
+        if (BYTES) { for (int i = 0; i < 8; ++i) { mbar_init(byte_full + 8 * i, 1); mbar_init(byte_empty + 8 * i, 2); } }
         for (int i = 0; i < 4; ++i) { mbar_init(q_ready + 8 * i, 1); mbar_init(q_free + 8 * i, 1); mbar_init(p_ready + 8 * i, 4); }
         for (int t = 0; t < 2; ++t) { mbar_init(s_ready + 8 * t, 1); mbar_init(s_free + 8 * t, 4); mbar_init(o_ready + 8 * t, 1); mbar_init(p_free + 8 * t, 1); mbar_init(joined + 8 * t, 4); }
         mbar_init(smem_u32(&sh.over), 1);
@@ -342,7 +381,18 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
             const int  parts = en.parts, c0 = en.c0;
             if (any) { wait_for(o_ready + 8 * t, o_phase, limit); o_phase ^= 1; tc_fence_after(); }
             float4 *part = reinterpret_cast<float4 *>(p.partial) + (paged_slot(blockIdx.x, c0) * 2 + t) * (PT_ROWS * (HD + 2) / 4);     // [HD / 4][128] x 4, [128], [128]
-            const float inv = parts > 1 ? 1.f : l == 0.f ? 0.f : 1.f / l;
+            const int64_t cell = KIND == PK_PLAIN ? 0 : (int64_t)(en.row0 + token) * (p.n_head_kv * p.group) + en.head * p.group + g;   // (of rows that are there) in what the two passes exchange
+            const bool whole_item = parts == 1, with = KIND != PK_PLAIN && p.with_stats != nullptr && en.lo > 0;
+            float factor = 1.f, other = 0.f, all = l;         // the row is (o factor + what the first pass found x other) / all
+            if (KIND != PK_PLAIN && whole_item && mine) {
+                if (p.stats != nullptr) { p.stats[cell] = make_float2(m, l); all = 1.f; }
+                else if (with) {
+                    const float2 w = p.with_stats[cell];
+                    const float top = fmaxf(m, w.x), ref = top == -CUDART_INF_F ? 0.f : top;
+                    factor = exp2f(m - ref); other = exp2f(w.x - ref); all = factor * l + other * w.y;
+                }
+            }
+            const float inv = !whole_item ? 1.f : all == 0.f ? 0.f : 1.f / all;
             const bool poisoned = any && *reinterpret_cast<volatile int *>(&sh.poison[stretch & 7]) == (int)stretch + 1;
             const int64_t to_row = (int64_t)(en.row0 + token) * p.out_stride + (en.head * p.group + g) * HD;
 #pragma unroll 1
@@ -363,13 +413,33 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
                         for (int j = ja; j < jb; ++j) {
                             const int page = p.view.page_table[(int64_t)en.seq * p.view.table_stride + j / p.view.page_size];
                             if (page < 0 || page >= p.view.n_pages) { continue; }
-                            const __half *v = p.v + page * p.view.page_stride + (j % p.view.page_size) * p.view.token_stride + en.head * p.view.head_stride + 32 * i;
+                            const int64_t at = page * p.view.page_stride + (j % p.view.page_size) * p.view.token_stride + en.head * p.view.head_stride + 32 * i;
+                            if constexpr (BYTES) {
+                                const uint32_t pair = p.scales.pairs[page * p.scales.page_stride + (j % p.view.page_size) * p.scales.token_stride + en.head * p.scales.head_stride];
+                                if (!large_scale(pair >> 16)) { continue; }
+                                const float scale = half2_bits(no_large_scale(pair)).y;
+                                const int8_t *v = reinterpret_cast<const int8_t *>(p.v) + at;
 #pragma unroll
-                            for (int c = 0; c < 32; ++c) {
-                                const float y = __half2float(v[c]);
-                                if (!isfinite(y)) { o[c] = __float_as_uint(__uint_as_float(o[c]) + y); }
+                                for (int c = 0; c < 32; ++c) { o[c] = __float_as_uint(__uint_as_float(o[c]) + (float)v[c] * scale); }
+                            } else {
+                                const __half *v = p.v + at;
+#pragma unroll
+                                for (int c = 0; c < 32; ++c) {
+                                    const float y = __half2float(v[c]);
+                                    if (!isfinite(y)) { o[c] = __float_as_uint(__uint_as_float(o[c]) + y); }
+                                }
                             }
                         }
+                    }
+                }
+                if (KIND != PK_PLAIN && whole_item && mine && with) {
+                    const float4 *u = reinterpret_cast<const float4 *>(p.with_out + cell * HD + 32 * i);
+#pragma unroll
+                    for (int c = 0; c < 8; ++c) {
+                        const float4 x = u[c];
+                        const float y[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) { o[4 * c + e] = __float_as_uint(__uint_as_float(o[4 * c + e]) * factor + y[e] * other); }
                     }
                 }
                 if (parts > 1 && mine) {
@@ -454,6 +524,24 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
                                     for (int c = 0; c < FOURS; ++c) { v[c].x += f * u[j][c].x; v[c].y += f * u[j][c].y; v[c].z += f * u[j][c].z; v[c].w += f * u[j][c].w; }
                                 }
                             }
+                            if constexpr (KIND != PK_PLAIN) {
+                                const int64_t its = (int64_t)(en.row0 + (2 * en.tile + t) * half_tokens + token_in) * (p.n_head_kv * p.group) + en.head * p.group + r - token_in * p.group;
+                                if (p.stats != nullptr) {
+                                    if (q4 == 0) { p.stats[its] = make_float2(top, sum); }
+                                    sum = 1.f;
+                                } else if (with) {
+                                    const float2 w = p.with_stats[its];
+                                    const float both = fmaxf(top, w.x), at = both == -CUDART_INF_F ? 0.f : both, f = exp2f(top - at), h = exp2f(w.x - at);
+                                    sum = f * sum + h * w.y;
+                                    const float4 *from = reinterpret_cast<const float4 *>(p.with_out + its * HD);
+#pragma unroll
+                                    for (int c = 0; c < FOURS; ++c) {
+                                        if (q4 + c * share >= HD / 4) { break; }
+                                        const float4 x = from[q4 + c * share];
+                                        v[c] = make_float4(f * v[c].x + h * x.x, f * v[c].y + h * x.y, f * v[c].z + h * x.z, f * v[c].w + h * x.w);
+                                    }
+                                }
+                            }
                             const float inv_all = sum == 0.f ? 0.f : 1.f / sum;
 #pragma unroll
                             for (int c = 0; c < FOURS; ++c) { v[c] = make_float4(v[c].x * inv_all, v[c].y * inv_all, v[c].z * inv_all, v[c].w * inv_all); }
@@ -485,7 +573,9 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
         auto advance = [&]() { if (++slot == SLOTS) { slot = 0; phase ^= 1; } };
         if (warp == 9) {
             // ------------------------------------------------------------------------------ the stretches, and their copies
-            constexpr int halves = HD / 64;                                                 // a tile's boxes are 64 elements wide
+            constexpr int halves = BYTES ? 1 : HD / 64;                                     // a tile's boxes are 64 elements wide, of bytes all of a head
+            constexpr int COPY_SLOTS = BYTES ? Shape::BYTE_SLOTS : SLOTS;
+            const uint32_t landed = BYTES ? byte_full : full, free_again = BYTES ? byte_empty : empty;
             const int group = lane % 16 * 8, half = lane >> 4;                              // this lane's eight positions of a tile, and half
             const bool issues = (group & (box - 1)) == 0 && half < halves;
             uint32_t &copies = issued;
@@ -515,18 +605,19 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
                     named = page_of(step + 1);
 #pragma unroll
                     for (int kv = 0; kv < 2; ++kv) {
-                        wait_for(empty + 8 * slot, phase ^ 1, limit);
+                        wait_for(free_again + 8 * slot, phase ^ 1, limit);
                         if (LATE && p.late == PA_LATE_KV && copies == 2) { stand_still(3 * wait_limit); }   // (issued all the same, with nobody waiting any more)
                         else if (gave_up()) { break; }
-                        const uint32_t bar = full + 8 * slot, dst = ring + slot * Shape::OPERAND;
+                        const uint32_t bar = landed + 8 * slot, dst = BYTES ? byte_ring + slot * Shape::BYTE_TILE : ring + slot * Shape::OPERAND;
                         if (lane == 0) {
                             if (kv == 0) { *reinterpret_cast<volatile uint32_t *>(&sh.there[copies / 2 & 7]) = there; }
-                            mbar_expect_tx(bar, Shape::OPERAND);
+                            mbar_expect_tx(bar, BYTES ? Shape::BYTE_TILE : Shape::OPERAND);
                         }
                         __syncwarp();
-                        if (issues) { tma_load(dst + half * PT_HALF + group * 128, kv == 0 ? &k_map : &v_map, bar, half * 64, token, e.head, page); }
+                        if (issues) { tma_load(BYTES ? dst + group * HD : dst + half * PT_HALF + group * 128, kv == 0 ? &k_map : &v_map, bar, half * 64, token, e.head, page); }
                         __syncwarp();
-                        advance();
+                        if (BYTES) { if (++slot == COPY_SLOTS) { slot = 0; phase ^= 1; } }
+                        else { advance(); }
                         ++copies;
                     }
                     if (limit == 0) { break; }
@@ -536,7 +627,8 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
             if (limit != 0) { Entry over = {}; put(over); }
         } else if (warp >= 10) {
             // ------------------------------------------------------------------------------ Q of a tile each; V tiles that not all rows see whole, half of the rows each
-            uint32_t tiles = 0, &q_count = issued;
+            // (8-bit caches: operands of all K and V tiles, half of the rows each)
+            uint32_t tiles = 0, &q_count = issued, byte_slot = 0, byte_phase = 0;
             const int t = warp - 10, v_row0 = t * (PT_KEYS / 2);
             while (next_entry()) {
                 const Entry &en = sh.entry[stretch & (PT_ENTRIES - 1)];
@@ -556,50 +648,106 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
                     }
                     __syncwarp();
                 }
-                for (int step = en.begin; step < en.end; ++step) {
-                    if (LATE && p.late == PA_LATE_CHECKS && tiles < 12) { stand_still(4000); }
-                    // K as well, though nothing is done to it: copies land in any order, and a slot's phase that nobody waited for could be taken for the one after the next.
-                    // A slot is not filled again before both warps have seen its phase, or they would wait for one that is over
-                    wait_for(full + 8 * slot, phase, limit);
-                    if (lane == 0 && limit != 0) { mbar_arrive(empty + 8 * slot); }
-                    advance();
-                    wait_for(full + 8 * slot, phase, limit);
-                    if (!(en.whole(p, a, step) && (b.rows == 0 || en.whole(p, b, step)))) {
-                        const int j0 = en.lo + step * PT_KEYS;
-                        const int first = p.causal && p.window > 0 ? max(0, a.pos_first - p.window + 1) - j0 : 0, end = en.hi - j0;   // rows that some query sees
-                        const uint32_t v_addr = ring + slot * Shape::OPERAND;
-                        uint32_t bad = 0;
-                        auto piece = [&](int i) {                                            // (half, row, piece of the row)
-                            const int at = i * 32 + lane;
-                            return (at >> 9) * PT_HALF + v_row0 * 128 + (at & 511) * 16;
-                        };
-#pragma unroll 8
-                        for (int i = 0; i < PT_KEYS / 2 * HD / 8 / 32; ++i) {
-                            const int r = v_row0 + (((i * 32 + lane) & 511) >> 3);
-                            const uint4 v = lds128(v_addr + piece(i));
-                            if (r >= end || r < first) { sts128(v_addr + piece(i), make_uint4(0, 0, 0, 0)); }
-                            else { bad |= not_finite(v.x) | not_finite(v.y) | not_finite(v.z) | not_finite(v.w); }
-                        }
-                        if (__any_sync(0xffffffffu, bad)) {
-#pragma unroll 1
-                            for (int i = 0; i < PT_KEYS / 2 * HD / 8 / 32; ++i) {
-                                const uint4 v = lds128(v_addr + piece(i));
-                                uint32_t w[4] = {v.x, v.y, v.z, v.w};
+                if constexpr (BYTES) {
+                    // the scales of this lane's two positions of a step are read a step ahead, their pages two
+                    const int32_t *table = p.view.page_table + (int64_t)en.seq * p.view.table_stride;
+                    const int seen_from = p.causal && p.window > 0 ? max(0, a.pos_first - p.window + 1) : 0, hi = en.hi, lo = en.lo, end = en.end;
+                    const int64_t head_at = en.head * p.scales.head_stride;
+                    int page[2];
+                    uint32_t pair[2], next_pair[2];
+                    auto position = [&](int step, int i) { return lo + step * PT_KEYS + v_row0 + 32 * i + lane; };
+                    auto find = [&](int step) {
 #pragma unroll
-                                for (int e = 0; e < 4; ++e) {
-                                    if ((w[e] & 0x7c00u) == 0x7c00u) { w[e] &= 0xffff0000u; }
-                                    if ((w[e] & 0x7c000000u) == 0x7c000000u) { w[e] &= 0xffffu; }
-                                }
-                                sts128(v_addr + piece(i), make_uint4(w[0], w[1], w[2], w[3]));
-                            }
-                            if (lane == 0) { *reinterpret_cast<volatile int *>(&sh.poison[stretch & 7]) = (int)stretch + 1; }
+                        for (int i = 0; i < 2; ++i) {
+                            const int j = position(step, i);
+                            page[i] = step < end && j >= seen_from && j < hi ? table[(unsigned)j / (unsigned)p.view.page_size] : -1;   // (what nobody sees is 0)
                         }
-                        fence_async_smem();
+                    };
+                    auto fetch = [&](int step) {
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            next_pair[i] = 0;
+                            if (page[i] >= 0 && page[i] < p.view.n_pages) {
+                                next_pair[i] = p.scales.pairs[page[i] * p.scales.page_stride + (unsigned)position(step, i) % (unsigned)p.view.page_size * p.scales.token_stride + head_at];
+                            }
+                        }
+                    };
+                    find(en.begin); fetch(en.begin); find(en.begin + 1);
+                    for (int step = en.begin; step < end; ++step) {
+                        if (LATE && p.late == PA_LATE_CHECKS && tiles < 12) { stand_still(4000); }
+                        pair[0] = no_large_scale(next_pair[0]); pair[1] = no_large_scale(next_pair[1]);
+                        fetch(step + 1); find(step + 2);
+#pragma unroll 1
+                        for (int kv = 0; kv < 2; ++kv) {
+                            if (kv == 1 && !(en.whole(p, a, step) && (b.rows == 0 || en.whole(p, b, step)))) {
+                                // 0 x inf: positions that some rows see and others do not. They are taken out, and given back to the rows that see them
+                                const bool bad0 = large_scale(pair[0] >> 16), bad1 = large_scale(pair[1] >> 16);
+                                if (__any_sync(0xffffffffu, bad0 || bad1)) {
+                                    if (bad0) { pair[0] &= 0xffffu; }
+                                    if (bad1) { pair[1] &= 0xffffu; }
+                                    if (lane == 0) { *reinterpret_cast<volatile int *>(&sh.poison[stretch & 7]) = (int)stretch + 1; }
+                                }
+                            }
+                            wait_for(byte_full + 8 * byte_slot, byte_phase, limit);
+                            wait_for(empty + 8 * slot, phase ^ 1, limit);
+                            if (gave_up()) { break; }
+                            make_operand<HD>(byte_ring + byte_slot * Shape::BYTE_TILE, ring + slot * Shape::OPERAND, v_row0, pair[0], pair[1], kv == 1);
+                            fence_async_smem();
+                            __syncwarp();
+                            if (lane == 0) { mbar_arrive(byte_empty + 8 * byte_slot); mbar_arrive(full + 8 * slot); }
+                            if (++byte_slot == Shape::BYTE_SLOTS) { byte_slot = 0; byte_phase ^= 1; }
+                            advance();
+                        }
+                        if (limit == 0) { break; }
+                        ++tiles;
                     }
-                    __syncwarp();
-                    if (lane == 0 && limit != 0) { mbar_arrive(clean + 8 * (tiles & 7)); mbar_arrive(empty + 8 * slot); }
-                    advance();
-                    ++tiles;
+                    if (limit == 0) { break; }
+                } else {
+                    for (int step = en.begin; step < en.end; ++step) {
+                        if (LATE && p.late == PA_LATE_CHECKS && tiles < 12) { stand_still(4000); }
+                        // K as well, though nothing is done to it: copies land in any order, and a slot's phase that nobody waited for could be taken for the one after the next.
+                        // A slot is not filled again before both warps have seen its phase, or they would wait for one that is over
+                        wait_for(full + 8 * slot, phase, limit);
+                        if (lane == 0 && limit != 0) { mbar_arrive(empty + 8 * slot); }
+                        advance();
+                        wait_for(full + 8 * slot, phase, limit);
+                        if (!(en.whole(p, a, step) && (b.rows == 0 || en.whole(p, b, step)))) {
+                            const int j0 = en.lo + step * PT_KEYS;
+                            const int first = p.causal && p.window > 0 ? max(0, a.pos_first - p.window + 1) - j0 : 0, end = en.hi - j0;   // rows that some query sees
+                            const uint32_t v_addr = ring + slot * Shape::OPERAND;
+                            uint32_t bad = 0;
+                            auto piece = [&](int i) {                                            // (half, row, piece of the row)
+                                const int at = i * 32 + lane;
+                                return (at >> 9) * PT_HALF + v_row0 * 128 + (at & 511) * 16;
+                            };
+    #pragma unroll 8
+                            for (int i = 0; i < PT_KEYS / 2 * HD / 8 / 32; ++i) {
+                                const int r = v_row0 + (((i * 32 + lane) & 511) >> 3);
+                                const uint4 v = lds128(v_addr + piece(i));
+                                if (r >= end || r < first) { sts128(v_addr + piece(i), make_uint4(0, 0, 0, 0)); }
+                                else { bad |= not_finite(v.x) | not_finite(v.y) | not_finite(v.z) | not_finite(v.w); }
+                            }
+                            if (__any_sync(0xffffffffu, bad)) {
+    #pragma unroll 1
+                                for (int i = 0; i < PT_KEYS / 2 * HD / 8 / 32; ++i) {
+                                    const uint4 v = lds128(v_addr + piece(i));
+                                    uint32_t w[4] = {v.x, v.y, v.z, v.w};
+    #pragma unroll
+                                    for (int e = 0; e < 4; ++e) {
+                                        if ((w[e] & 0x7c00u) == 0x7c00u) { w[e] &= 0xffff0000u; }
+                                        if ((w[e] & 0x7c000000u) == 0x7c000000u) { w[e] &= 0xffffu; }
+                                    }
+                                    sts128(v_addr + piece(i), make_uint4(w[0], w[1], w[2], w[3]));
+                                }
+                                if (lane == 0) { *reinterpret_cast<volatile int *>(&sh.poison[stretch & 7]) = (int)stretch + 1; }
+                            }
+                            fence_async_smem();
+                        }
+                        __syncwarp();
+                        if (lane == 0 && limit != 0) { mbar_arrive(clean + 8 * (tiles & 7)); mbar_arrive(empty + 8 * slot); }
+                        advance();
+                        ++tiles;
+                    }
                 }
                 __syncwarp();
                 entry_read(lane == 0);
@@ -657,7 +805,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
                         __syncwarp();
                     }
                     wait_for(full + 8 * v_slot, v_phase, limit);
-                    wait_for(clean + 8 * (tiles & 7), (tiles >> 3) & 1, limit);
+                    if (!BYTES) { wait_for(clean + 8 * (tiles & 7), (tiles >> 3) & 1, limit); }   // (an operand is made of what is seen alone)
                     ++tiles;
 #pragma unroll
                     for (int t = 0; t < 2; ++t) {
@@ -701,10 +849,11 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
             __syncwarp();
             wait_for(smem_u32(&sh.over), 0, again);
         } else if (warp == 9) {                           // each slot's last copy (the ones before it were waited for by whoever freed the slot)
-            for (uint32_t i = 0; i < SLOTS && i < issued; ++i) {
-                if (slot == 0) { slot = SLOTS; phase ^= 1; }
+            constexpr uint32_t COPY_SLOTS = BYTES ? Shape::BYTE_SLOTS : SLOTS;
+            for (uint32_t i = 0; i < COPY_SLOTS && i < issued; ++i) {
+                if (slot == 0) { slot = COPY_SLOTS; phase ^= 1; }
                 --slot;
-                wait_for(full + 8 * slot, phase, again);
+                wait_for((BYTES ? byte_full : full) + 8 * slot, phase, again);
             }
         } else if (warp >= 10) {
             for (uint32_t i = 1; i <= Shape::Q_BUFFERS && i <= issued; ++i) {
@@ -733,17 +882,18 @@ EncodeTiled encoder() {
     }();
     return fn;
 }
-bool tensor_map(CUtensorMap *map, const __half *data, int n, const cuuint64_t *dims, const cuuint64_t *strides, const cuuint32_t *box) {
+bool tensor_map(CUtensorMap *map, const __half *data, int n, const cuuint64_t *dims, const cuuint64_t *strides, const cuuint32_t *box, bool bytes = false) {
     const cuuint32_t ones[4] = {1, 1, 1, 1};
-    return encoder() != nullptr && encoder()(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, n, const_cast<__half *>(data), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                                             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+    return encoder() != nullptr && encoder()(map, bytes ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, n, const_cast<__half *>(data), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                                             bytes ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
-// pages of one pool: [page][head][position][element] whatever the order of the strides; boxes of `box` positions x 64 elements
-bool page_map(CUtensorMap *map, const __half *pool, const PagedView &v, int heads, int head_dim, int box) {
+// pages of one pool: [page][head][position][element] whatever the order of the strides; boxes of `box` positions x 64 elements, or x all bytes of a head
+bool page_map(CUtensorMap *map, const __half *pool, const PagedView &v, int heads, int head_dim, int box, bool bytes) {
+    const cuuint64_t size = bytes ? 1 : 2;
     const cuuint64_t dims[4] = {(cuuint64_t)head_dim, (cuuint64_t)v.page_size, (cuuint64_t)heads, (cuuint64_t)v.n_pages};
-    const cuuint64_t strides[3] = {(cuuint64_t)v.token_stride * 2, (cuuint64_t)v.head_stride * 2, (cuuint64_t)v.page_stride * 2};
-    const cuuint32_t boxes[4] = {64, (cuuint32_t)box, 1, 1};
-    return tensor_map(map, pool, 4, dims, strides, boxes);
+    const cuuint64_t strides[3] = {(cuuint64_t)v.token_stride * size, (cuuint64_t)v.head_stride * size, (cuuint64_t)v.page_stride * size};
+    const cuuint32_t boxes[4] = {bytes ? (cuuint32_t)head_dim : 64, (cuuint32_t)box, 1, 1};
+    return tensor_map(map, pool, 4, dims, strides, boxes, bytes);
 }
 // Q: [row][head][element], boxes of whole tokens of a group of heads
 bool query_map(CUtensorMap *map, const PagedAttention &p, int n_head, int head_dim) {
@@ -752,21 +902,26 @@ bool query_map(CUtensorMap *map, const PagedAttention &p, int n_head, int head_d
     return tensor_map(map, p.q, 3, dims, strides, boxes);
 }
 // the warpgroups' registers after their split are what the block is launched with: fewer, and the split would wait for ever
-template <int HD, bool LATE> cudaError_t registers_suffice() {
+template <int HD, bool LATE, int KIND> cudaError_t registers_suffice() {
     static const cudaError_t answer = [] {
         cudaFuncAttributes a;
-        const cudaError_t err = cudaFuncGetAttributes(&a, paged_tc_kernel<HD, LATE>);
+        const cudaError_t err = cudaFuncGetAttributes(&a, paged_tc_kernel<HD, LATE, KIND>);
         return err != cudaSuccess ? err : a.numRegs * PT_THREADS >= 256 * PT_REGS_SOFTMAX + 128 * PT_REGS_OTHERS ? cudaSuccess : cudaErrorInvalidConfiguration;
     }();
     return answer;
 }
-template <int HD, bool LATE>
+template <int HD, bool LATE, int KIND>
 cudaError_t launch_tc(const PagedAttention &p, const CUtensorMap &q, const CUtensorMap &k, const CUtensorMap &v, int box, int sms, const LaunchCfg &cfg, uint64_t wait_limit) {
-    cudaError_t err = registers_suffice<HD, LATE>();
+    cudaError_t err = registers_suffice<HD, LATE, KIND>();
     if (err != cudaSuccess) { return err; }
-    err = allow_dynamic_smem(reinterpret_cast<const void *>(paged_tc_kernel<HD, LATE>), TcShape<HD>::SMEM);
+    err = allow_dynamic_smem(reinterpret_cast<const void *>(paged_tc_kernel<HD, LATE, KIND>), TcShape<HD, KIND>::SMEM);
     if (err != cudaSuccess) { return err; }
-    return launch_maybe_pdl(paged_tc_kernel<HD, LATE>, dim3(sms), PT_THREADS, TcShape<HD>::SMEM, cfg.stream, cfg.pdl, p, q, k, v, box, cfg.error_flag, wait_limit);
+    return launch_maybe_pdl(paged_tc_kernel<HD, LATE, KIND>, dim3(sms), PT_THREADS, TcShape<HD, KIND>::SMEM, cfg.stream, cfg.pdl, p, q, k, v, box, cfg.error_flag, wait_limit);
+}
+
+template <bool LATE, int KIND>
+cudaError_t launch_tc(const PagedAttention &p, int head_dim, const CUtensorMap &q, const CUtensorMap &k, const CUtensorMap &v, int box, int sms, const LaunchCfg &cfg, uint64_t wait_limit) {
+    return head_dim == 128 ? launch_tc<128, LATE, KIND>(p, q, k, v, box, sms, cfg, wait_limit) : launch_tc<64, LATE, KIND>(p, q, k, v, box, sms, cfg, wait_limit);
 }
 
 }  // namespace
@@ -779,16 +934,18 @@ static int paged_tc_box(int page_size) {   // positions of a box: the largest po
 bool launch_paged_attention_tc(const PagedAttention &given, int head_dim, int n_head, int sms, const LaunchCfg &cfg, uint64_t wait_limit, cudaError_t *err) {
     const int box = paged_tc_box(given.view.page_size);
     const PagedView &view = given.view;
-    if (given.kind() != PK_PLAIN) { return false; }
     const int64_t most = std::max({view.token_stride, view.head_stride, view.page_stride, given.q_stride}), least = std::min({view.token_stride, view.head_stride, view.page_stride, given.q_stride});
     if ((head_dim != 64 && head_dim != 128) || box < 8 || given.group > PT_ROWS || least <= 0 || most >= (1ll << 38)) { return false; }
     PagedAttention p = given;
     p.tile_rows = 2 * (PT_ROWS / p.group) * p.group;
     p.start_units = PA_START;
     CUtensorMap q, k, v;
-    if (!query_map(&q, p, n_head, head_dim) || !page_map(&k, p.k, p.view, p.n_head_kv, head_dim, box) || !page_map(&v, p.v, p.view, p.n_head_kv, head_dim, box)) { return false; }
-    const auto launch = p.late != PA_ON_TIME ? (head_dim == 128 ? launch_tc<128, true> : launch_tc<64, true>) : head_dim == 128 ? launch_tc<128, false> : launch_tc<64, false>;
-    *err = launch(p, q, k, v, box, sms, cfg, wait_limit);
+    const int kind = p.kind();
+    const bool bytes = kind == PK_INT8;
+    if (!query_map(&q, p, n_head, head_dim) || !page_map(&k, p.k, p.view, p.n_head_kv, head_dim, box, bytes) || !page_map(&v, p.v, p.view, p.n_head_kv, head_dim, box, bytes)) { return false; }
+    const auto launch = kind == PK_SHARED ? launch_tc<false, PK_SHARED> : bytes ? (p.late != PA_ON_TIME ? launch_tc<true, PK_INT8> : launch_tc<false, PK_INT8>)
+                                          : p.late != PA_ON_TIME ? launch_tc<true, PK_PLAIN> : launch_tc<false, PK_PLAIN>;
+    *err = launch(p, head_dim, q, k, v, box, sms, cfg, wait_limit);
     return true;
 }
 
