@@ -358,11 +358,13 @@ static spyb_status attention_pass(spyb_backend *be, PagedAttention p, int head_d
         if (!launch_paged_attention_tc(p, head_dim, n_head, be->num_sms_total, cfg, wait_limit, &err)) { p.few_rows = 1 << 30; }
         SPYB_CUDA(be, err);
     }
-    const int row_tiles = std::min<int64_t>(most, p.few_rows) <= 16 ? 1 : 2;
-    p.tile_rows = 16 * row_tiles;
-    if (p.few_rows > 0) {
-        SPYB_CUDA(be, p.kind() == PK_PLAIN ? launch_paged_attention_rows(p, head_dim, row_tiles, be->num_sms_total, cfg) : launch_paged_attend_rows(p, head_dim, row_tiles, be->num_sms_total, cfg));
-    }
+    if (p.few_rows == 0) { return SPYB_SUCCESS; }
+    const int64_t rows = std::min<int64_t>(most, p.few_rows);
+    const int row_tiles = rows <= 16 ? 1 : 2;
+    p.tile_rows = p.kind() == PK_INT8 && rows <= 8 ? 8 : 16 * row_tiles;
+    SPYB_CUDA(be, p.kind() == PK_INT8 ? launch_paged_attention_bytes(p, head_dim, be->num_sms_total, cfg)
+                  : p.kind() == PK_SHARED ? launch_paged_shared_rows(p, head_dim, row_tiles, be->num_sms_total, cfg)
+                                          : launch_paged_attention_rows(p, head_dim, row_tiles, be->num_sms_total, cfg));
     return SPYB_SUCCESS;
 }
 // The public calls (`scales`, `shared`: spyb_paged_attend's), and with a role that is late the self-checks'. The descriptors have been checked.

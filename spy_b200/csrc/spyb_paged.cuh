@@ -76,7 +76,8 @@ cudaError_t launch_paged_load(const PagedLoad &p, int out_type, int sms, const L
 cudaError_t launch_paged_shared(const PagedShared &p, const LaunchCfg &cfg);
 cudaError_t launch_paged_append(const PagedAppend &p, int in_type, int q_out_type, int sms, const LaunchCfg &cfg);
 cudaError_t launch_paged_attention_rows(const PagedAttention &p, int head_dim, int row_tiles, int sms, const LaunchCfg &cfg);
-cudaError_t launch_paged_attend_rows(const PagedAttention &p, int head_dim, int row_tiles, int sms, const LaunchCfg &cfg);   // (kinds other than PK_PLAIN)
+cudaError_t launch_paged_shared_rows(const PagedAttention &p, int head_dim, int row_tiles, int sms, const LaunchCfg &cfg);   // (PK_SHARED)
+cudaError_t launch_paged_attention_bytes(const PagedAttention &p, int head_dim, int sms, const LaunchCfg &cfg);               // (PK_INT8; tiles of 8, 16 or 32 rows)
 // the kernel on tensor memory; false where it does not take these pages, heads or strides (nothing is launched then)
 bool        launch_paged_attention_tc(const PagedAttention &p, int head_dim, int n_head, int sms, const LaunchCfg &cfg, uint64_t wait_limit, cudaError_t *err);
 // Sequences of up to so many rows (times query heads of a K/V head) are the small kernel's, whose tile of 16 rows costs them nothing but the memory's time; a second tile

@@ -258,8 +258,6 @@ cudaError_t launch_paged_load(const PagedLoad &p, int out_type, int, const Launc
 cudaError_t launch_paged_shared(const PagedShared &p, const LaunchCfg &cfg) {
     return launch_maybe_pdl(paged_shared_kernel, dim3((p.view.n_seq + SH_WARPS - 1) / SH_WARPS), SH_WARPS * 32, 0, cfg.stream, cfg.pdl, p);
 }
-cudaError_t launch_paged_attend_rows(const PagedAttention &p, int head_dim, int row_tiles, int sms, const LaunchCfg &cfg) {
-    return p.kind() == PK_INT8 ? launch_rows_kind<PK_INT8>(p, head_dim, row_tiles, sms, cfg) : launch_rows_kind<PK_SHARED>(p, head_dim, row_tiles, sms, cfg);
-}
+cudaError_t launch_paged_shared_rows(const PagedAttention &p, int head_dim, int row_tiles, int sms, const LaunchCfg &cfg) { return launch_rows_kind<PK_SHARED>(p, head_dim, row_tiles, sms, cfg); }
 
 }  // namespace spyb

@@ -1,4 +1,4 @@
-// Attention of few rows a sequence over caches in pages: the kernel.
+// Attention of few rows a sequence over caches in pages: the kernel for fp16 ones, and what it shares with the one for bytes.
 #pragma once
 
 #include <math_constants.h>
@@ -32,67 +32,122 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, bool there) {   // zeros where it is not
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
 }
-__device__ __forceinline__ void cp_async4(uint32_t dst, const void *src, bool there) {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(there ? 4 : 0) : "memory");
-}
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 __device__ __forceinline__ float ex2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
 __device__ __forceinline__ bool not_finite2(uint32_t h2) { return (h2 & 0x7c00u) == 0x7c00u || (h2 & 0x7c000000u) == 0x7c000000u; }
 
-template <int HD, int KIND> struct RowsShape {
-    static constexpr bool BYTES = KIND == PK_INT8;
-    static constexpr int ROW = BYTES ? (HD == 96 ? 128 : HD) : HD <= 64 ? 128 : 256;   // bytes of a position in shared memory (16-byte pieces swizzled within eight)
-    static constexpr int STAGE = 2 * PR_BLOCK * ROW + (BYTES ? PR_BLOCK * 4 : 0);      // (bytes: and the positions' scales)
-    static constexpr int STAGES = BYTES ? 3 : ROW == 128 ? 4 : 3;    // (short positions: three CTAs an SM; a warp's time a block is what their instructions wait for one another)
-    static constexpr int RING = PR_WARPS * STAGES * STAGE;
-    static constexpr int PIECES = BYTES ? HD / 16 : HD / 8;          // 16-byte pieces of a position
-    // where byte 16 c of position r lies: bytes so that what a quarter of a warp reads at a time - two positions side by side, or every second one - lies in other banks
-    static __device__ __forceinline__ int place(int r, int c) {
-        if (!BYTES || HD > 64) { return r * ROW + ((c ^ (r & 7)) << 4); }
-        if (HD == 64) { return (r >> 1) * 128 + ((((r ^ (r >> 2)) & 1) * 4 + (c ^ (r & 2))) << 4); }
-        return r * ROW + (c << 4);
+struct RowsDone { int rows, tile, row0, head, from; };   // an item's rows that this tile holds, its tile, the sequence's first row, K/V head, and where its own positions begin
+// What the warps of a CTA found for an item ([warp][room][HD], maxima, sums), joined and put where it goes: to the output, or where other CTAs have pieces of the item to the workspace, and by the
+// last of these, in their order, to the output. All threads, behind a barrier.
+template <int HD, int TILE, int KIND>
+__device__ __forceinline__ void rows_finish(const PagedAttention &p, const PagedCut &cut, const RowsDone &what, const float *mo, const float *mm, const float *ml, int room, int &last_one) {
+    constexpr int PART = TILE * (HD + 2), NT = PR_WARPS * 32;
+    const int tid = threadIdx.x, done = what.rows;
+    float *part = p.partial + paged_slot(blockIdx.x, cut.c0) * PART;
+    auto put = [&](int r, int c, float4 v, float m, float l) {   // four elements of a row, its maximum and sum
+        const int pr = what.tile * TILE + r, token = (int)((unsigned)pr / (unsigned)p.group), g = pr - token * p.group;
+        const int64_t o2 = (int64_t)(what.row0 + token) * p.out_stride + (what.head * p.group + g) * HD + c;
+        if constexpr (KIND != PK_PLAIN) {
+            const int64_t cell = (int64_t)(what.row0 + token) * (p.n_head_kv * p.group) + what.head * p.group + g;
+            if (p.stats != nullptr) {
+                if (c == 0) { p.stats[cell] = make_float2(m, l); }
+                *reinterpret_cast<float4 *>(static_cast<float *>(p.out) + o2) = v;
+                return;
+            }
+            if (p.with_stats != nullptr && what.from > 0) { paged_join_pass(v, l, m, p.with_stats[cell], *reinterpret_cast<const float4 *>(p.with_out + cell * HD + c)); }
+        }
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        const float w[4] = {v.x * inv, v.y * inv, v.z * inv, v.w * inv};
+        if (p.out_f32) { store4(static_cast<float *>(p.out) + o2, w); } else { store4(static_cast<__half *>(p.out) + o2, w); }
+    };
+    for (int x = tid; x < done * (HD / 4); x += NT) {
+        const int r = x / (HD / 4), c = (x - r * (HD / 4)) * 4;
+        float m = -CUDART_INF_F;
+#pragma unroll
+        for (int w = 0; w < PR_WARPS; ++w) { m = fmaxf(m, mm[w * room + r]); }
+        const float base = m == -CUDART_INF_F ? 0.f : m;
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        float l = 0.f;
+#pragma unroll
+        for (int w = 0; w < PR_WARPS; ++w) {
+            const float f = ex2(mm[w * room + r] - base);
+            const float4 u = *reinterpret_cast<const float4 *>(mo + (w * room + r) * HD + c);
+            v.x += f * u.x; v.y += f * u.y; v.z += f * u.z; v.w += f * u.w;
+            l += f * ml[w * room + r];
+        }
+        if (cut.parts == 1) { put(r, c, v, m, l); }
+        else {
+            *reinterpret_cast<float4 *>(part + r * HD + c) = v;
+            if (c == 0) { part[TILE * HD + r] = m; part[TILE * HD + TILE + r] = l; }
+        }
     }
-};
-// N bytes of position r from byte N i on, as words
-template <class Shape, int N> __device__ __forceinline__ void lds_row(uint32_t addr, int r, int i, uint32_t (&w)[N / 4]) {
-    if constexpr (N % 16 == 0) {
-#pragma unroll
-        for (int k = 0; k < N / 16; ++k) {
-            const uint4 x = lds128(addr + Shape::place(r, i * (N / 16) + k));
-            w[4 * k] = x.x; w[4 * k + 1] = x.y; w[4 * k + 2] = x.z; w[4 * k + 3] = x.w;
+    if (cut.parts > 1) {
+        __syncthreads();
+        if (tid == 0) {
+            __threadfence();
+            const unsigned n = atomicAdd(p.arrived + cut.c0, 1u);
+            last_one = n == (unsigned)cut.parts - 1;
+            if (last_one) { p.arrived[cut.c0] = 0; __threadfence(); }
         }
-    } else if constexpr (N % 8 == 0) {
+        __syncthreads();
+        if (last_one) {
+            for (int x = tid; x < done * (HD / 4); x += NT) {
+                const int r = x / (HD / 4), c = (x - r * (HD / 4)) * 4;
+                float m = -CUDART_INF_F, l = 0.f;
+                float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+                // eight CTAs' findings are in flight together; what came before is scaled to the new maximum
+#pragma unroll 1
+                for (int i0 = 0; i0 < cut.parts; i0 += 8) {
+                    float  pm[8], pl[8], top = m;
+                    float4 u[8];
 #pragma unroll
-        for (int k = 0; k < N / 8; ++k) {
-            const int at = i * (N / 8) + k;
-            const uint2 x = lds64(addr + Shape::place(r, at >> 1) + (at & 1) * 8);
-            w[2 * k] = x.x; w[2 * k + 1] = x.y;
+                    for (int j = 0; j < 8; ++j) {
+                        const bool is = i0 + j < cut.parts;
+                        const float *from = p.partial + paged_slot(cut.c0 + (is ? i0 + j : 0), cut.c0) * PART;
+                        pm[j] = is ? __ldcg(from + TILE * HD + r) : -CUDART_INF_F;
+                        pl[j] = is ? __ldcg(from + TILE * HD + TILE + r) : 0.f;
+                        u[j] = is ? __ldcg(reinterpret_cast<const float4 *>(from + r * HD + c)) : make_float4(0.f, 0.f, 0.f, 0.f);
+                    }
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) { top = fmaxf(top, pm[j]); }
+                    const float base = top == -CUDART_INF_F ? 0.f : top, before = ex2(m - base);
+                    m = top; l *= before;
+                    v = make_float4(v.x * before, v.y * before, v.z * before, v.w * before);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        const float f = ex2(pm[j] - base);
+                        v.x += f * u[j].x; v.y += f * u[j].y; v.z += f * u[j].z; v.w += f * u[j].w;
+                        l += f * pl[j];
+                    }
+                }
+                put(r, c, v, m, l);
+            }
         }
-    } else {
-#pragma unroll
-        for (int k = 0; k < N / 4; ++k) { const int at = i * (N / 4) + k; w[k] = lds32(addr + Shape::place(r, at >> 2) + (at & 3) * 4); }
     }
 }
-template <int HD, int MT, int KIND> struct RowsSmem {       // the ring; what the warps found: beside it for up to EARLY rows, in its place for more; the masks of the ring's stages
-    using Shape = RowsShape<HD, KIND>;
-    static constexpr int EARLY = MT == 1 ? 8 : 0, FOUND = PR_WARPS * 16 * MT * (HD + 2) * 4, RING = Shape::RING > FOUND ? Shape::RING : FOUND;
-    static constexpr int CTAS = MT == 1 && (HD <= 64 || KIND == PK_INT8) ? 3 : 2;         // of an SM (64 single tokens, heads of 64, before the cut counted items' beginnings: 65 us with three, 79 with two; longer heads' rings leave room for two)
-    static constexpr int MASKS = RING + PR_WARPS * EARLY * (HD + 2) * 4, BYTES = MASKS + PR_WARPS * Shape::STAGES * 4;
+
+template <int HD> struct RowsShape {
+    static constexpr int ROW = HD <= 64 ? 128 : 256;                 // bytes of a position in shared memory (16-byte pieces swizzled within eight)
+    static constexpr int STAGE = 2 * PR_BLOCK * ROW;
+    static constexpr int STAGES = ROW == 128 ? 4 : 3;                // (short positions: three CTAs an SM; a warp's time a block is what their instructions wait for one another)
+    static constexpr int RING = PR_WARPS * STAGES * STAGE;
+};
+template <int HD, int MT> struct RowsSmem {       // the ring; what the warps found: beside it for up to EARLY rows, in its place for more; the masks of the ring's stages
+    static constexpr int EARLY = MT == 1 ? 8 : 0, FOUND = PR_WARPS * 16 * MT * (HD + 2) * 4, RING = RowsShape<HD>::RING > FOUND ? RowsShape<HD>::RING : FOUND;
+    static constexpr int CTAS = MT == 1 && HD <= 64 ? 3 : 2;         // of an SM (64 single tokens, heads of 64, before the cut counted items' beginnings: 65 us with three, 79 with two; longer heads' rings leave room for two)
+    static constexpr int MASKS = RING + PR_WARPS * EARLY * (HD + 2) * 4, BYTES = MASKS + PR_WARPS * RowsShape<HD>::STAGES * 4;
 };
 // IN_PAGE: a block's positions lie in one page (pages of a multiple of 16), heads of up to 64: 64 single tokens 64.8 us against 66.6. (Longer heads' blocks take longer than
 // the table's latency: 103.2 us against 102.8, they go without.)
 template <int HD, int MT, bool IN_PAGE, int KIND>
 __global__ void __launch_bounds__(PR_WARPS * 32) paged_rows_kernel(const __grid_constant__ PagedAttention p) {
-    using Shape = RowsShape<HD, KIND>;
-    using Smem = RowsSmem<HD, MT, KIND>;
-    constexpr bool BYTES = KIND == PK_INT8;
-    constexpr int PR_STAGES = Shape::STAGES, TILE = 16 * MT, ROW = Shape::ROW, STAGE = Shape::STAGE, NT = PR_WARPS * 32;
+    constexpr int PR_STAGES = RowsShape<HD>::STAGES, TILE = 16 * MT, ROW = RowsShape<HD>::ROW, STAGE = RowsShape<HD>::STAGE, NT = PR_WARPS * 32;
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ PagedPlanShared plan;
     __shared__ int last_one;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    uint32_t *there = reinterpret_cast<uint32_t *>(smem + Smem::MASKS) + warp * PR_STAGES;
+    uint32_t *there = reinterpret_cast<uint32_t *>(smem + RowsSmem<HD, MT>::MASKS) + warp * PR_STAGES;
     const uint32_t ring = smem_u32(smem) + warp * PR_STAGES * STAGE;
     pdl_launch_dependents();
     pdl_wait();
@@ -103,8 +158,7 @@ __global__ void __launch_bounds__(PR_WARPS * 32) paged_rows_kernel(const __grid_
     PagedItem it;
     int todo, ka, kb, n_block, packed;        // of the item that comes next: units of this CTA, positions [ka, kb), blocks of them; rows of the tile
     const int32_t *table;
-    using Kept = std::conditional_t<BYTES, uint8_t, __half>;
-    const Kept *kbase, *vbase;
+    const __half *kbase, *vbase;
     auto describe = [&]() {
         it = paged_item<PR_UNIT, PR_BLOCK>(p, q, tile);
         todo = (int)min((int64_t)(it.units - off), at.end - at.unit);
@@ -112,7 +166,7 @@ __global__ void __launch_bounds__(PR_WARPS * 32) paged_rows_kernel(const __grid_
         n_block = kb > ka ? (kb - ka + PR_BLOCK - 1) / PR_BLOCK : 0;
         packed = min(TILE, q.rows * p.group - tile * TILE);
         table = p.view.page_table + (int64_t)seq * p.view.table_stride;
-        kbase = reinterpret_cast<const Kept *>(p.k) + head * p.view.head_stride; vbase = reinterpret_cast<const Kept *>(p.v) + head * p.view.head_stride;
+        kbase = p.k + head * p.view.head_stride; vbase = p.v + head * p.view.head_stride;
     };
         auto page_of = [&](int b) {          // page of block b, or (lanes 0..15 and 16..31 alike) of this lane's position in it; -1: none
             const int j = ka + b * PR_BLOCK + (IN_PAGE ? 0 : lane & 15);
@@ -125,24 +179,18 @@ __global__ void __launch_bounds__(PR_WARPS * 32) paged_rows_kernel(const __grid_
             const int64_t cell = ok ? page * p.view.page_stride + in_page * p.view.token_stride : 0;
             const unsigned mask = IN_PAGE ? (ok ? (kb - j >= PR_BLOCK ? 0xffffu : (1u << (kb - j)) - 1) : 0u) : __ballot_sync(0xffffffffu, ok) & 0xffffu;
             const uint32_t dst = ring + stage * STAGE;
-            constexpr int PIECES = Shape::PIECES, WIDE = 16 / sizeof(Kept);
-            if constexpr (BYTES) {
-                const int r = lane & 15;                      // (lanes 0..15: the scales of a position each)
-                const int64_t o = p.scales.page_stride * page + p.scales.token_stride * (in_page + (IN_PAGE ? r : 0)) + p.scales.head_stride * head;
-                const bool in = (mask >> r) & 1;
-                if (lane < 16) { cp_async4(dst + 2 * PR_BLOCK * ROW + r * 4, p.scales.pairs + (in ? o : 0), in); }
-            }
+            constexpr int PIECES = HD / 8;
             if constexpr (IN_PAGE) {
                 static_assert(32 % PIECES == 0, "a row's pieces are lanes side by side");
                 constexpr int AT_ONCE = 32 / PIECES;
                 const int r0 = lane / PIECES, c = lane % PIECES;
-                int64_t o = cell + r0 * p.view.token_stride + c * WIDE;
+                int64_t o = cell + r0 * p.view.token_stride + c * 8;
                 const int64_t more = AT_ONCE * p.view.token_stride;
 #pragma unroll
                 for (int i = 0; i < PIECES / 2; ++i) {
                     const int r = i * AT_ONCE + r0;
                     const bool in = (mask >> r) & 1;
-                    const uint32_t d = dst + Shape::place(r, c);
+                    const uint32_t d = dst + r * ROW + ((c ^ (r & 7)) << 4);
                     const int64_t at = in ? o : 0;
                     cp_async16(d, kbase + at, in);
                     cp_async16(d + PR_BLOCK * ROW, vbase + at, in);
@@ -153,8 +201,8 @@ __global__ void __launch_bounds__(PR_WARPS * 32) paged_rows_kernel(const __grid_
                 for (int i = 0; i < PIECES / 2; ++i) {
                     const int x = i * 32 + lane, r = x / PIECES, c = x - r * PIECES;
                     const bool in = (mask >> r) & 1;
-                    const int64_t row = __shfl_sync(0xffffffffu, cell, r), o = in ? row + c * WIDE : 0;
-                    const uint32_t d = dst + Shape::place(r, c);
+                    const int64_t row = __shfl_sync(0xffffffffu, cell, r), o = in ? row + c * 8 : 0;
+                    const uint32_t d = dst + r * ROW + ((c ^ (r & 7)) << 4);
                     cp_async16(d, kbase + o, in);
                     cp_async16(d + PR_BLOCK * ROW, vbase + o, in);
                 }
@@ -191,13 +239,11 @@ __global__ void __launch_bounds__(PR_WARPS * 32) paged_rows_kernel(const __grid_
                 const int r = m * 16 + hf * 8 + (lane >> 2), pr = tile * TILE + min(r, packed - 1);
                 const int token = (int)((unsigned)pr / (unsigned)p.group), g = pr - token * p.group;
                 pos[m][hf] = q.first + token;
-                // (bytes: a lane's elements are HD / 4 side by side, four a product, so that it reads K's the same way)
-                const uint32_t *src = reinterpret_cast<const uint32_t *>(p.q + (int64_t)(q.row0 + token) * p.q_stride + (head * p.group + g) * HD) + (lane & 3) * (BYTES ? HD / 8 : 1);
-                constexpr int STEP = BYTES ? 2 : 8, SECOND = BYTES ? 1 : 4;
+                const uint32_t *src = reinterpret_cast<const uint32_t *>(p.q + (int64_t)(q.row0 + token) * p.q_stride + (head * p.group + g) * HD) + (lane & 3);
 #pragma unroll
                 for (int ks = 0; ks < HD / 16; ++ks) {
-                    qf[m][ks][hf] = r < packed ? src[ks * STEP] : 0u;
-                    qf[m][ks][2 + hf] = r < packed ? src[ks * STEP + SECOND] : 0u;
+                    qf[m][ks][hf] = r < packed ? src[ks * 8] : 0u;
+                    qf[m][ks][2 + hf] = r < packed ? src[ks * 8 + 4] : 0u;
                 }
             }
         }
@@ -206,7 +252,6 @@ __global__ void __launch_bounds__(PR_WARPS * 32) paged_rows_kernel(const __grid_
     start();
     for (;;) {
         const int pos_first = q.first + (int)((unsigned)(tile * TILE) / (unsigned)p.group), pos_last = q.first + (int)((unsigned)(tile * TILE + packed - 1) / (unsigned)p.group);
-        float unit = ldexpf(1.f, 40);             // bytes: V's scales are taken against the largest so far, rounded up to a power of two; this is one over it
         float o[MT][HD / 8][4], mx[MT][2], sum[MT][2], base[MT][2], over[MT][2];   // (base: the maximum, or 0 for none; over: scores beyond it move the maximum)
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
@@ -235,37 +280,13 @@ __global__ void __launch_bounds__(PR_WARPS * 32) paged_rows_kernel(const __grid_
 #pragma unroll
                 for (int n = 0; n < 2; ++n) { sc[m][n][0] = sc[m][n][1] = sc[m][n][2] = sc[m][n][3] = 0.f; }
             }
-            float k_scale[2][2], v_scale[2][2];           // bytes: of this lane's four positions, K's with what scores are scaled by anyway
-            if constexpr (BYTES) {
 #pragma unroll
-                for (int n = 0; n < 2; ++n) {
-                    const uint2 s = lds64(vs_addr + PR_BLOCK * ROW + (n * 8 + (lane & 3) * 2) * 4);
-                    const float2 a = half2_bits(s.x), c = half2_bits(s.y);
-                    k_scale[n][0] = fmaf(a.x, 0.f, a.x * p.scale_log2); k_scale[n][1] = fmaf(c.x, 0.f, c.x * p.scale_log2);   // (an infinite one is NaN: its elements' infinities do not add up to one)
-                    v_scale[n][0] = a.y; v_scale[n][1] = c.y;
-                }
-                uint32_t kw[2][HD / 16];
+            for (int ks = 0; ks < HD / 16; ++ks) {
+                uint32_t kf[4];
+                const int r = (lane & 7) + ((lane >> 4) << 3), c = 2 * ks + ((lane >> 3) & 1);
+                ldsm4(ks_addr + r * ROW + ((c ^ (r & 7)) << 4), kf);
 #pragma unroll
-                for (int n = 0; n < 2; ++n) { lds_row<Shape, HD / 4>(ks_addr, n * 8 + (lane >> 2), lane & 3, kw[n]); }
-#pragma unroll
-                for (int ks = 0; ks < HD / 16; ++ks) {
-#pragma unroll
-                    for (int n = 0; n < 2; ++n) {
-                        uint32_t b0, b1;
-                        halves_of(kw[n][ks], b0, b1);
-#pragma unroll
-                        for (int m = 0; m < MT; ++m) { mma16816(sc[m][n], qf[m][ks], b0, b1); }
-                    }
-                }
-            } else {
-#pragma unroll
-                for (int ks = 0; ks < HD / 16; ++ks) {
-                    uint32_t kf[4];
-                    const int r = (lane & 7) + ((lane >> 4) << 3), c = 2 * ks + ((lane >> 3) & 1);
-                    ldsm4(ks_addr + r * ROW + ((c ^ (r & 7)) << 4), kf);
-#pragma unroll
-                    for (int m = 0; m < MT; ++m) { mma16816(sc[m][0], qf[m][ks], kf[0], kf[1]); mma16816(sc[m][1], qf[m][ks], kf[2], kf[3]); }
-                }
+                for (int m = 0; m < MT; ++m) { mma16816(sc[m][0], qf[m][ks], kf[0], kf[1]); mma16816(sc[m][1], qf[m][ks], kf[2], kf[3]); }
             }
             // scores against the maximum, in powers of two
             bool above = false;
@@ -276,43 +297,13 @@ __global__ void __launch_bounds__(PR_WARPS * 32) paged_rows_kernel(const __grid_
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         float &x = sc[m][n][e];
-                        x = fmaf(x, BYTES ? k_scale[n][e & 1] : p.scale_log2, -base[m][e >> 1]);
+                        x = fmaf(x, p.scale_log2, -base[m][e >> 1]);
                         if (!whole) {
                             const int jj = n * 8 + (lane & 3) * 2 + (e & 1), d = pos[m][e >> 1] - (j0 + jj);
                             const bool seen = ((mask >> jj) & 1) && (!p.causal || (d >= 0 && (p.window <= 0 || d < p.window)));
                             x = seen ? x : -CUDART_INF_F;
                         }
                         above |= x > over[m][e >> 1];
-                    }
-                }
-            }
-            bool odd = false;                             // bytes: a scale of V is not finite
-            if constexpr (BYTES) {
-                bool more_of_v = false;
-#pragma unroll
-                for (int n = 0; n < 2; ++n) {
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) { v_scale[n][e] *= unit; more_of_v |= !(fabsf(v_scale[n][e]) <= 1.f); }
-                }
-                if (__any_sync(0xffffffffu, more_of_v)) {
-                    float most = 1.f / unit;
-#pragma unroll
-                    for (int n = 0; n < 2; ++n) {
-#pragma unroll
-                        for (int e = 0; e < 2; ++e) { const bool fine = fabsf(v_scale[n][e]) < CUDART_INF_F; most = fmaxf(most, fine ? fabsf(v_scale[n][e]) / unit : 0.f); odd |= !fine; }
-                    }
-                    odd = __any_sync(0xffffffffu, odd);
-                    most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
-                    most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
-                    const uint32_t up = (__float_as_uint(most) + 0x7fffffu) & 0x7f800000u;   // (2^-24 at least, 2^16 at most)
-                    const float to = __uint_as_float(0x7f000000u - up), f = to / unit;
-                    unit = to;
-#pragma unroll
-                    for (int n = 0; n < 2; ++n) { v_scale[n][0] *= f; v_scale[n][1] *= f; }
-#pragma unroll
-                    for (int m = 0; m < MT; ++m) {
-#pragma unroll
-                        for (int n = 0; n < HD / 8; ++n) { o[m][n][0] *= f; o[m][n][1] *= f; o[m][n][2] *= f; o[m][n][3] *= f; }
                     }
                 }
             }
@@ -345,31 +336,10 @@ __global__ void __launch_bounds__(PR_WARPS * 32) paged_rows_kernel(const __grid_
                     for (int n = 0; n < 2; ++n) {
                         const float a = ex2(sc[m][n][2 * hf]), c = ex2(sc[m][n][2 * hf + 1]);
                         sum[m][hf] += a + c;
-                        if (!BYTES) { pf[m][2 * n + hf] = pack2(a, c); }
-                        else if (!odd) { pf[m][2 * n + hf] = pack2(a * v_scale[n][0], c * v_scale[n][1]); }
-                        else {                                // (what is not seen is 0 whatever its scale is)
-                            pf[m][2 * n + hf] = pack2(sc[m][n][2 * hf] == -CUDART_INF_F ? 0.f : a * v_scale[n][0], sc[m][n][2 * hf + 1] == -CUDART_INF_F ? 0.f : c * v_scale[n][1]);
-                        }
+                        pf[m][2 * n + hf] = pack2(a, c);
                     }
                 }
             }
-            if constexpr (BYTES) {
-                // a lane has the same HD / 8 elements of its four positions: column g of the n-th product is element g HD / 8 + n
-                uint32_t vw[4][HD / 32];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) { lds_row<Shape, HD / 8>(vs_addr, (i >> 1) * 8 + (lane & 3) * 2 + (i & 1), lane >> 2, vw[i]); }
-#pragma unroll
-                for (int w = 0; w < HD / 32; ++w) {
-                    uint32_t b0[4], b1[4];
-                    pairs_of(vw[0][w], vw[1][w], b0);
-                    pairs_of(vw[2][w], vw[3][w], b1);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-#pragma unroll
-                        for (int m = 0; m < MT; ++m) { mma16816(o[m][4 * w + e], pf[m], b0[e], b1[e]); }
-                    }
-                }
-            } else {
             uint32_t bad = 0;
 #pragma unroll
             for (int d = 0; d < HD / 16; ++d) {
@@ -412,22 +382,22 @@ __global__ void __launch_bounds__(PR_WARPS * 32) paged_rows_kernel(const __grid_
                     }
                 }
             }
-            }
             stage = stage == PR_STAGES - 1 ? 0 : stage + 1;
         }
         cp_wait<0>();
         __syncwarp();
         // What is known of this item; the next one's copies start before its findings are joined, where these have a place of their own
-        const int done = packed, done_tile = tile, done_row0 = q.row0, done_head = head, done_from = q.from;
+        const RowsDone what = {packed, tile, q.row0, head, q.from};
+        const int done = packed;
         const PagedCut cut = paged_cut(at, at.unit - off, it.units);
         at.unit += todo + p.start_units;
         off = 0;
-        const bool more = at.unit < at.end && paged_next(p, true, q, seq, head, tile), early = done <= Smem::EARLY;
+        const bool more = at.unit < at.end && paged_next(p, true, q, seq, head, tile), early = done <= RowsSmem<HD, MT>::EARLY;
         if (more) { describe(); }
         if (more && early) { start(); }
         if (!early) { __syncthreads(); }
-        const int room = early ? Smem::EARLY : TILE;              // rows of a warp's findings
-        float *mo = reinterpret_cast<float *>(smem + (early ? Smem::RING : 0)), *mm = mo + PR_WARPS * room * HD, *ml = mm + PR_WARPS * room;
+        const int room = early ? RowsSmem<HD, MT>::EARLY : TILE;              // rows of a warp's findings
+        float *mo = reinterpret_cast<float *>(smem + (early ? RowsSmem<HD, MT>::RING : 0)), *mm = mo + PR_WARPS * room * HD, *ml = mm + PR_WARPS * room;
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
 #pragma unroll
@@ -437,107 +407,15 @@ __global__ void __launch_bounds__(PR_WARPS * 32) paged_rows_kernel(const __grid_
                 l += __shfl_xor_sync(0xffffffffu, l, 2);
                 const int r = m * 16 + hf * 8 + (lane >> 2);
                 if (r < done) {
-                    float *dst = mo + (warp * room + r) * HD + (lane & 3) * (BYTES ? HD / 4 : 2);
-                    if constexpr (BYTES) {
-                        const float f = 1.f / unit;
+                    float *dst = mo + (warp * room + r) * HD + (lane & 3) * 2;
 #pragma unroll
-                        for (int e = 0; e < 2; ++e) {
-#pragma unroll
-                            for (int n = 0; n < HD / 8; n += 4) {
-                                *reinterpret_cast<float4 *>(dst + e * (HD / 8) + n) = make_float4(o[m][n][2 * hf + e] * f, o[m][n + 1][2 * hf + e] * f, o[m][n + 2][2 * hf + e] * f, o[m][n + 3][2 * hf + e] * f);
-                            }
-                        }
-                    } else {
-#pragma unroll
-                        for (int n = 0; n < HD / 8; ++n) { *reinterpret_cast<float2 *>(dst + n * 8) = make_float2(o[m][n][2 * hf], o[m][n][2 * hf + 1]); }
-                    }
+                    for (int n = 0; n < HD / 8; ++n) { *reinterpret_cast<float2 *>(dst + n * 8) = make_float2(o[m][n][2 * hf], o[m][n][2 * hf + 1]); }
                     if ((lane & 3) == 0) { mm[warp * room + r] = mx[m][hf]; ml[warp * room + r] = l; }
                 }
             }
         }
         __syncthreads();
-        constexpr int PART = TILE * (HD + 2);
-        float *part = p.partial + paged_slot(blockIdx.x, cut.c0) * PART;
-        auto put = [&](int r, int c, float4 v, float m, float l) {   // four elements of a row, its maximum and sum
-            const int pr = done_tile * TILE + r, token = (int)((unsigned)pr / (unsigned)p.group), g = pr - token * p.group;
-            const int64_t o2 = (int64_t)(done_row0 + token) * p.out_stride + (done_head * p.group + g) * HD + c;
-            if constexpr (KIND != PK_PLAIN) {
-                const int64_t cell = (int64_t)(done_row0 + token) * (p.n_head_kv * p.group) + done_head * p.group + g;
-                if (p.stats != nullptr) {
-                    if (c == 0) { p.stats[cell] = make_float2(m, l); }
-                    *reinterpret_cast<float4 *>(static_cast<float *>(p.out) + o2) = v;
-                    return;
-                }
-                if (p.with_stats != nullptr && done_from > 0) { paged_join_pass(v, l, m, p.with_stats[cell], *reinterpret_cast<const float4 *>(p.with_out + cell * HD + c)); }
-            }
-            const float inv = l == 0.f ? 0.f : 1.f / l;
-            const float w[4] = {v.x * inv, v.y * inv, v.z * inv, v.w * inv};
-            if (p.out_f32) { store4(static_cast<float *>(p.out) + o2, w); } else { store4(static_cast<__half *>(p.out) + o2, w); }
-        };
-        for (int x = tid; x < done * (HD / 4); x += NT) {
-            const int r = x / (HD / 4), c = (x - r * (HD / 4)) * 4;
-            float m = -CUDART_INF_F;
-#pragma unroll
-            for (int w = 0; w < PR_WARPS; ++w) { m = fmaxf(m, mm[w * room + r]); }
-            const float base = m == -CUDART_INF_F ? 0.f : m;
-            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-            float l = 0.f;
-#pragma unroll
-            for (int w = 0; w < PR_WARPS; ++w) {
-                const float f = ex2(mm[w * room + r] - base);
-                const float4 u = *reinterpret_cast<const float4 *>(mo + (w * room + r) * HD + c);
-                v.x += f * u.x; v.y += f * u.y; v.z += f * u.z; v.w += f * u.w;
-                l += f * ml[w * room + r];
-            }
-            if (cut.parts == 1) { put(r, c, v, m, l); }
-            else {
-                *reinterpret_cast<float4 *>(part + r * HD + c) = v;
-                if (c == 0) { part[TILE * HD + r] = m; part[TILE * HD + TILE + r] = l; }
-            }
-        }
-        if (cut.parts > 1) {
-            __syncthreads();
-            if (tid == 0) {
-                __threadfence();
-                const unsigned n = atomicAdd(p.arrived + cut.c0, 1u);
-                last_one = n == (unsigned)cut.parts - 1;
-                if (last_one) { p.arrived[cut.c0] = 0; __threadfence(); }
-            }
-            __syncthreads();
-            if (last_one) {
-                for (int x = tid; x < done * (HD / 4); x += NT) {
-                    const int r = x / (HD / 4), c = (x - r * (HD / 4)) * 4;
-                    float m = -CUDART_INF_F, l = 0.f;
-                    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-                    // eight CTAs' findings are in flight together; what came before is scaled to the new maximum
-#pragma unroll 1
-                    for (int i0 = 0; i0 < cut.parts; i0 += 8) {
-                        float  pm[8], pl[8], top = m;
-                        float4 u[8];
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) {
-                            const bool is = i0 + j < cut.parts;
-                            const float *from = p.partial + paged_slot(cut.c0 + (is ? i0 + j : 0), cut.c0) * PART;
-                            pm[j] = is ? __ldcg(from + TILE * HD + r) : -CUDART_INF_F;
-                            pl[j] = is ? __ldcg(from + TILE * HD + TILE + r) : 0.f;
-                            u[j] = is ? __ldcg(reinterpret_cast<const float4 *>(from + r * HD + c)) : make_float4(0.f, 0.f, 0.f, 0.f);
-                        }
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) { top = fmaxf(top, pm[j]); }
-                        const float base = top == -CUDART_INF_F ? 0.f : top, before = ex2(m - base);
-                        m = top; l *= before;
-                        v = make_float4(v.x * before, v.y * before, v.z * before, v.w * before);
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) {
-                            const float f = ex2(pm[j] - base);
-                            v.x += f * u[j].x; v.y += f * u[j].y; v.z += f * u[j].z; v.w += f * u[j].w;
-                            l += f * pl[j];
-                        }
-                    }
-                    put(r, c, v, m, l);
-                }
-            }
-        }
+        rows_finish<HD, TILE, KIND>(p, cut, what, mo, mm, ml, room, last_one);
         if (!more) { return; }
         __syncthreads();                      // (the findings' place is free again)
         if (!early) { start(); }
@@ -546,22 +424,22 @@ __global__ void __launch_bounds__(PR_WARPS * 32) paged_rows_kernel(const __grid_
 
 template <int HD, int MT, bool IN_PAGE, int KIND>
 cudaError_t launch_rows_as(const PagedAttention &p, int sms, const LaunchCfg &cfg) {
-    using Smem = RowsSmem<HD, MT, KIND>;
     const void *kernel = reinterpret_cast<const void *>(paged_rows_kernel<HD, MT, IN_PAGE, KIND>);
-    const cudaError_t err = allow_dynamic_smem(kernel, (size_t)Smem::BYTES);
+    const cudaError_t err = allow_dynamic_smem(kernel, (size_t)RowsSmem<HD, MT>::BYTES);
     if (err != cudaSuccess) { return err; }
-    return launch_maybe_pdl(paged_rows_kernel<HD, MT, IN_PAGE, KIND>, dim3(Smem::CTAS * sms), PR_WARPS * 32, (size_t)Smem::BYTES, cfg.stream, cfg.pdl, p);
+    return launch_maybe_pdl(paged_rows_kernel<HD, MT, IN_PAGE, KIND>, dim3(RowsSmem<HD, MT>::CTAS * sms), PR_WARPS * 32, (size_t)RowsSmem<HD, MT>::BYTES, cfg.stream, cfg.pdl, p);
 }
 template <int HD, int MT, int KIND>
 cudaError_t launch_rows(PagedAttention p, int sms, const LaunchCfg &cfg) {
     const int page = p.view.page_size;
     p.page_shift = -1; p.start_units = PA_START;
     for (int s = 0; s < 31; ++s) { if (page == 1 << s) { p.page_shift = s; } }
-    if constexpr (HD <= 64 || (KIND == PK_INT8 && HD == 128)) {
+    if constexpr (HD <= 64) {
         if (page % PR_BLOCK == 0) { return launch_rows_as<HD, MT, true, KIND>(p, sms, cfg); }
     }
     return launch_rows_as<HD, MT, false, KIND>(p, sms, cfg);
 }
+
 template <int KIND>
 cudaError_t launch_rows_kind(const PagedAttention &p, int head_dim, int row_tiles, int sms, const LaunchCfg &cfg) {
     switch (head_dim * 2 + row_tiles - 1) {
@@ -576,6 +454,5 @@ cudaError_t launch_rows_kind(const PagedAttention &p, int head_dim, int row_tile
     default: return cudaErrorInvalidValue;
     }
 }
-
 }  // namespace
 }  // namespace spyb

@@ -7,7 +7,8 @@
 // products run. K and V come page by page through tensor maps, in pieces of as many positions as divide the page size, into the 128-byte
 // swizzle of the operands: K row by row (K-major), V as it lies (its positions are the product's inner dimension: MN-major), no transposition anywhere.
 //   warps 0-3, 4-7   probabilities of tile 0 / 1, rescaling, output          warp 8   issues the MMAs
-//   warp 9           copies                                                   warps 10, 11  clear and check the V tiles that not all rows see whole
+//   warp 9           copies                                                   warps 10, 11  Q; clear and check the V tiles that not all rows see whole
+//   warps 12-15      (8-bit caches) make the operands of K and V: bytes land in a ring of their own, byte x scale is rounded to fp16
 // Probabilities are taken against a maximum that follows the true one when that is 2^8 above it: O is rescaled in the first steps and hardly ever after.
 // Measured (heads of 128): 8192 tokens of a prompt, 32 heads, 570 us, 965 TFLOP/s of the 1640 of a matrix product; 512 tokens at 32 768 positions 281 us, 970;
 // 1500 at 9111, 40 heads, 247 us, 1040; 512 at 3968 52 to 55 us, 595; five tokens of 24 sequences of up to 9000, 111 us, 4.2 TB/s. Heads of 64 have half the
@@ -30,13 +31,14 @@
 namespace spyb {
 namespace {
 
-constexpr int PT_THREADS = 384, PT_ROWS = 128, PT_KEYS = 128;
-constexpr int PT_REGS_SOFTMAX = 208, PT_REGS_OTHERS = 88;   // 256 x 208 + 128 x 88 = 384 x 168, what the block is launched with
+constexpr int PT_ROWS = 128, PT_KEYS = 128;
 constexpr uint32_t PT_HALF = PT_KEYS * 128;              // bytes of 128 rows x 64 elements
 
 template <int HD, int KIND> struct TcShape {
     static constexpr uint32_t OPERAND = PT_KEYS * HD * 2;                      // a tile of Q, K or V
     static constexpr bool BYTES = KIND == PK_INT8;
+    static constexpr int THREADS = BYTES ? 512 : 384, READERS = BYTES ? 15 : 11;   // (readers of an entry: eight warps for probabilities, one for MMAs, two for Q and V, four for bytes)
+    static constexpr int REGS_SOFTMAX = BYTES ? 184 : 208, REGS_OTHERS = BYTES ? 72 : 88;   // 256 x 208 + 128 x 88 = 384 x 168, 256 x 184 + 256 x 72 = 512 x 128: what the block is launched with
     static constexpr int SLOTS = BYTES ? (HD == 128 ? 3 : 4) : HD == 128 ? 5 : 8;   // K and V tiles in flight; of bytes: made into operands ahead
     static constexpr int BYTE_SLOTS = BYTES ? (HD == 128 ? 4 : 6) : 0;         // tiles of bytes in flight
     static constexpr uint32_t BYTE_TILE = PT_KEYS * HD;
@@ -68,11 +70,11 @@ struct Entry {
 // still read is written over. The other roles' waits run out in turn, so that every role ends by itself, and then who issued copies or products waits for their end, whoever
 // it was that gave up. (Waiting for it in every case, at the end of each role, cost 5 % of prompts of heads of 64.)
 constexpr uint64_t PT_LANDING_NS = 1000000000;       // what is on its way has this long to land (whatever the limit of the waits)
-constexpr int PT_ENTRIES = 4, PT_READERS = 11;       // stretches known ahead; warps that read them: eight for probabilities, one for MMAs, two for Q and V
+constexpr int PT_ENTRIES = 4;                        // stretches known ahead
 struct TcShared {
     uint64_t full[8], empty[8];                          // a slot's copies have landed; its last MMA is done, and both warps that check V have seen its phase
     uint64_t clean[8];                                   // of the last V tiles: what nobody sees is cleared
-    uint64_t byte_full[8], byte_empty[8];                // 8-bit caches: a tile of bytes has landed; both warps have made its operand (`full` is that operand's, `empty` its last MMA's)
+    uint64_t byte_full[8], byte_empty[8];                // 8-bit caches: a tile of bytes has landed; its operand is made (`full` is that operand's, `empty` its last MMA's)
     uint64_t q_ready[2][2], q_free[2][2];                // of the two tiles and their buffers, in stretches in which they see anything
     uint64_t s_ready[2], s_free[2], p_ready[2][2], p_free[2], o_ready[2];   // (P ready) of the first 96 positions and the rest; (free) where P lies apart
     uint64_t known[PT_ENTRIES], read[PT_ENTRIES];        // an entry is there; all have read it
@@ -174,28 +176,32 @@ __device__ __noinline__ void stand_still(uint64_t ns) {
 }
 
 // LATE: the self-checks' kernels (p.late)
-// Bytes of 64 positions (row0 on) of a tile as an operand: byte x scale, rounded to fp16. A lane has 16 bytes at a time, a quarter of a warp one row or two; `pairs`: the scales of positions
-// row0 + lane and row0 + 32 + lane, K's below and V's above. (Lanes of the operand's second half write their two pieces the other way round: eight lanes, eight places in the banks.)
-template <int HD> __device__ __forceinline__ void make_operand(uint32_t bytes, uint32_t operand, int row0, uint32_t scale0, uint32_t scale1, bool is_v) {
-    constexpr int PER = HD / 16, AT_ONCE = 32 / PER, LOOPS = 64 / AT_ONCE;
+// Bytes of 32 positions (row0 on) of a tile as an operand: byte x scale, rounded to fp16. A lane has 16 bytes at a time, a quarter of a warp one row or two; `scales`: of position row0 + lane, K's
+// below and V's above. (Lanes of the operand's second half write their two pieces the other way round: eight lanes, eight places in the banks.)
+template <int HD> __device__ __forceinline__ void make_operand(uint32_t bytes, uint32_t operand, int row0, uint32_t scales, bool is_v) {
+    constexpr int PER = HD / 16, AT_ONCE = 32 / PER, LOOPS = 32 / AT_ONCE;
     const int lane = threadIdx.x & 31, c = lane % PER, r0 = lane / PER;
-    const uint32_t sel = is_v ? 0x3232 : 0x1010;
+    const uint32_t both = __byte_perm(scales, 0, is_v ? 0x3232 : 0x1010);
     const int swap = HD == 128 ? c >> 2 : 0;
-    const uint32_t src = bytes + (row0 + r0) * HD + c * 16, half = operand + (c >> 2) * PT_HALF;
-#pragma unroll 4
-    for (int i = 0; i < LOOPS; ++i) {
-        const int r = i * AT_ONCE + r0;                                // (of the 64)
-        const uint4 w = lds128(src + i * (AT_ONCE * HD));
-        const uint32_t pair = __shfl_sync(0xffffffffu, i * AT_ONCE < 32 ? scale0 : scale1, r & 31);
-        const uint32_t d = __byte_perm(pair, 0, sel);
-        uint32_t h[8];
-        halves_of(w.x, h[0], h[1]); halves_of(w.y, h[2], h[3]); halves_of(w.z, h[4], h[5]); halves_of(w.w, h[6], h[7]);
+    const uint32_t src = bytes + (row0 + r0) * HD + c * 16, half = operand + (c >> 2) * PT_HALF + (row0 + r0) * 128;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) { asm("mul.rn.f16x2 %0, %0, %1;" : "+r"(h[e]) : "r"(d)); }
-        const uint32_t row = half + (row0 + r) * 128;
-        const int first = (2 * (c & 3) + swap) ^ (r & 7);              // (row0 is a multiple of 8)
-        sts128(row + first * 16, swap ? make_uint4(h[4], h[5], h[6], h[7]) : make_uint4(h[0], h[1], h[2], h[3]));
-        sts128(row + (first ^ 1) * 16, swap ? make_uint4(h[0], h[1], h[2], h[3]) : make_uint4(h[4], h[5], h[6], h[7]));
+    for (int i0 = 0; i0 < LOOPS; i0 += 4) {
+        uint4 w[4];                                                    // (reads in flight)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) { w[i] = lds128(src + (i0 + i) * (AT_ONCE * HD)); }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int r = (i0 + i) * AT_ONCE + r0;
+            const uint32_t d = __shfl_sync(0xffffffffu, both, r);
+            uint32_t h[8];
+            halves_of(w[i].x, h[0], h[1]); halves_of(w[i].y, h[2], h[3]); halves_of(w[i].z, h[4], h[5]); halves_of(w[i].w, h[6], h[7]);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) { asm("mul.rn.f16x2 %0, %0, %1;" : "+r"(h[e]) : "r"(d)); }
+            const uint32_t row = half + (i0 + i) * (AT_ONCE * 128);
+            const int first = (2 * (c & 3) + swap) ^ (r & 7);          // (row0 is a multiple of 8)
+            sts128(row + first * 16, swap ? make_uint4(h[4], h[5], h[6], h[7]) : make_uint4(h[0], h[1], h[2], h[3]));
+            sts128(row + (first ^ 1) * 16, swap ? make_uint4(h[0], h[1], h[2], h[3]) : make_uint4(h[4], h[5], h[6], h[7]));
+        }
     }
 }
 // a scale beyond what bytes of fp16 values have is an infinity, as its elements may be
@@ -207,7 +213,7 @@ __device__ __forceinline__ uint32_t no_large_scale(uint32_t pair) {
 }
 
 template <int HD, bool LATE, int KIND>
-__global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_constant__ PagedAttention p, const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
+__global__ void __launch_bounds__(TcShape<HD, KIND>::THREADS, 1) paged_tc_kernel(const __grid_constant__ PagedAttention p, const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
                                                                   const int box, int *error_flag, const uint64_t wait_limit) {
     using Shape = TcShape<HD, KIND>;
     constexpr bool BYTES = Shape::BYTES;
@@ -221,20 +227,20 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
                    o_ready = smem_u32(sh.o_ready), p_free = smem_u32(sh.p_free);
     const uint32_t byte_full = smem_u32(sh.byte_full), byte_empty = smem_u32(sh.byte_empty), byte_ring = ring + SLOTS * Shape::OPERAND;
     if (tid == 0) {
-        for (int i = 0; i < 8; ++i) { mbar_init(full + 8 * i, BYTES ? 2 : 1); mbar_init(empty + 8 * i, BYTES ? 1 : 3); mbar_init(clean + 8 * i, 2); sh.poison[i] = 0; }
-        if (BYTES) { for (int i = 0; i < 8; ++i) { mbar_init(byte_full + 8 * i, 1); mbar_init(byte_empty + 8 * i, 2); } }
+        for (int i = 0; i < 8; ++i) { mbar_init(full + 8 * i, BYTES ? 4 : 1); mbar_init(empty + 8 * i, BYTES ? 1 : 3); mbar_init(clean + 8 * i, 2); sh.poison[i] = 0; }
+        if (BYTES) { for (int i = 0; i < 8; ++i) { mbar_init(byte_full + 8 * i, 1); mbar_init(byte_empty + 8 * i, 4); } }
         for (int i = 0; i < 4; ++i) { mbar_init(q_ready + 8 * i, 1); mbar_init(q_free + 8 * i, 1); mbar_init(p_ready + 8 * i, 4); }
         for (int t = 0; t < 2; ++t) { mbar_init(s_ready + 8 * t, 1); mbar_init(s_free + 8 * t, 4); mbar_init(o_ready + 8 * t, 1); mbar_init(p_free + 8 * t, 1); mbar_init(joined + 8 * t, 4); }
         mbar_init(smem_u32(&sh.over), 1);
         sh.gave_up = 0;
-        for (int i = 0; i < PT_ENTRIES; ++i) { mbar_init(known + 8 * i, 1); mbar_init(read + 8 * i, PT_READERS); }
+        for (int i = 0; i < PT_ENTRIES; ++i) { mbar_init(known + 8 * i, 1); mbar_init(read + 8 * i, Shape::READERS); }
         mbar_init_fence();
     }
     pdl_launch_dependents();
     pdl_wait();
     Walker walk;
     // (at least four units a CTA, items' beginnings among them: 512 tokens at 512 positions 20.8 us, 23.8 from two on; 4 x 20 rows at 700 positions 24.5 and 22.8)
-    walk.at = paged_plan<PT_THREADS, PT_KEYS, PT_KEYS>(p, false, 4, sh.plan);
+    walk.at = paged_plan<Shape::THREADS, PT_KEYS, PT_KEYS>(p, false, 4, sh.plan);
     if (walk.at.unit >= walk.at.end) { return; }
     if (warp == 8) { asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&sh.tmem)) : "memory"); }
     tc_fence_before();
@@ -261,7 +267,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
     // K and V tiles take slots in turn: K of step 0, V of step 0, K of step 1, ...
     uint32_t slot = 0, phase = 0, issued = 0;             // (issued: tiles of K and V by the copying warp, of Q by those that check V)
     if (warp < 8) {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(PT_REGS_SOFTMAX));
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Shape::REGS_SOFTMAX));
         // ---------------------------------------------------------------------------------- probabilities, output
         const int t = warp >> 2, row = tid & 127;
         const uint32_t lanes = (uint32_t)(warp & 3) << 21;                                   // (32 lanes a warp, in the address's upper half)
@@ -569,7 +575,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
             entry_read(lane == 0);
         }
     } else {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PT_REGS_OTHERS));
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Shape::REGS_OTHERS));
         auto advance = [&]() { if (++slot == SLOTS) { slot = 0; phase ^= 1; } };
         if (warp == 9) {
             // ------------------------------------------------------------------------------ the stretches, and their copies
@@ -625,10 +631,10 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
                 if (limit == 0 || !walk.next(p, e.todo)) { break; }
             }
             if (limit != 0) { Entry over = {}; put(over); }
-        } else if (warp >= 10) {
+        } else if (warp == 10 || warp == 11) {
             // ------------------------------------------------------------------------------ Q of a tile each; V tiles that not all rows see whole, half of the rows each
-            // (8-bit caches: operands of all K and V tiles, half of the rows each)
-            uint32_t tiles = 0, &q_count = issued, byte_slot = 0, byte_phase = 0;
+            // (of 8-bit caches Q alone)
+            uint32_t tiles = 0, &q_count = issued;
             const int t = warp - 10, v_row0 = t * (PT_KEYS / 2);
             while (next_entry()) {
                 const Entry &en = sh.entry[stretch & (PT_ENTRIES - 1)];
@@ -648,61 +654,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
                     }
                     __syncwarp();
                 }
-                if constexpr (BYTES) {
-                    // the scales of this lane's two positions of a step are read a step ahead, their pages two
-                    const int32_t *table = p.view.page_table + (int64_t)en.seq * p.view.table_stride;
-                    const int seen_from = p.causal && p.window > 0 ? max(0, a.pos_first - p.window + 1) : 0, hi = en.hi, lo = en.lo, end = en.end;
-                    const int64_t head_at = en.head * p.scales.head_stride;
-                    int page[2];
-                    uint32_t pair[2], next_pair[2];
-                    auto position = [&](int step, int i) { return lo + step * PT_KEYS + v_row0 + 32 * i + lane; };
-                    auto find = [&](int step) {
-#pragma unroll
-                        for (int i = 0; i < 2; ++i) {
-                            const int j = position(step, i);
-                            page[i] = step < end && j >= seen_from && j < hi ? table[(unsigned)j / (unsigned)p.view.page_size] : -1;   // (what nobody sees is 0)
-                        }
-                    };
-                    auto fetch = [&](int step) {
-#pragma unroll
-                        for (int i = 0; i < 2; ++i) {
-                            next_pair[i] = 0;
-                            if (page[i] >= 0 && page[i] < p.view.n_pages) {
-                                next_pair[i] = p.scales.pairs[page[i] * p.scales.page_stride + (unsigned)position(step, i) % (unsigned)p.view.page_size * p.scales.token_stride + head_at];
-                            }
-                        }
-                    };
-                    find(en.begin); fetch(en.begin); find(en.begin + 1);
-                    for (int step = en.begin; step < end; ++step) {
-                        if (LATE && p.late == PA_LATE_CHECKS && tiles < 12) { stand_still(4000); }
-                        pair[0] = no_large_scale(next_pair[0]); pair[1] = no_large_scale(next_pair[1]);
-                        fetch(step + 1); find(step + 2);
-#pragma unroll 1
-                        for (int kv = 0; kv < 2; ++kv) {
-                            if (kv == 1 && !(en.whole(p, a, step) && (b.rows == 0 || en.whole(p, b, step)))) {
-                                // 0 x inf: positions that some rows see and others do not. They are taken out, and given back to the rows that see them
-                                const bool bad0 = large_scale(pair[0] >> 16), bad1 = large_scale(pair[1] >> 16);
-                                if (__any_sync(0xffffffffu, bad0 || bad1)) {
-                                    if (bad0) { pair[0] &= 0xffffu; }
-                                    if (bad1) { pair[1] &= 0xffffu; }
-                                    if (lane == 0) { *reinterpret_cast<volatile int *>(&sh.poison[stretch & 7]) = (int)stretch + 1; }
-                                }
-                            }
-                            wait_for(byte_full + 8 * byte_slot, byte_phase, limit);
-                            wait_for(empty + 8 * slot, phase ^ 1, limit);
-                            if (gave_up()) { break; }
-                            make_operand<HD>(byte_ring + byte_slot * Shape::BYTE_TILE, ring + slot * Shape::OPERAND, v_row0, pair[0], pair[1], kv == 1);
-                            fence_async_smem();
-                            __syncwarp();
-                            if (lane == 0) { mbar_arrive(byte_empty + 8 * byte_slot); mbar_arrive(full + 8 * slot); }
-                            if (++byte_slot == Shape::BYTE_SLOTS) { byte_slot = 0; byte_phase ^= 1; }
-                            advance();
-                        }
-                        if (limit == 0) { break; }
-                        ++tiles;
-                    }
-                    if (limit == 0) { break; }
-                } else {
+                if constexpr (!BYTES) {
                     for (int step = en.begin; step < en.end; ++step) {
                         if (LATE && p.late == PA_LATE_CHECKS && tiles < 12) { stand_still(4000); }
                         // K as well, though nothing is done to it: copies land in any order, and a slot's phase that nobody waited for could be taken for the one after the next.
@@ -751,6 +703,66 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
                 }
                 __syncwarp();
                 entry_read(lane == 0);
+            }
+        } else if (warp >= 12) {
+            // ------------------------------------------------------------------------------ operands of bytes and scales: 32 rows of every K and V tile each
+            if constexpr (BYTES) {
+                uint32_t tiles = 0, byte_slot = 0, byte_phase = 0;
+                const int row0 = (warp - 12) * 32;
+                const unsigned page_size = p.view.page_size;
+                while (next_entry()) {
+                    const Entry &en = sh.entry[stretch & (PT_ENTRIES - 1)];
+                    const Tile a = en.half[0], b = en.half[1];
+                    // The scales of this lane's position of a step are read a step ahead, its page two. (Loads without branches around them, or each is waited for where it stands: what is not
+                    // there reads something that is, and counts as 0.)
+                    const int32_t *table = p.view.page_table + (int64_t)en.seq * p.view.table_stride;
+                    const uint32_t *pairs = p.scales.pairs + en.head * p.scales.head_stride;
+                    const int seen_from = p.causal && p.window > 0 ? max(0, a.pos_first - p.window + 1) : 0, hi = en.hi, lo = en.lo, end = en.end;
+                    int page = 0, at = 0;
+                    bool ok = false, next_ok = false;
+                    uint32_t next_pair = 0;
+                    auto find = [&](int step) {
+                        const int j = lo + step * PT_KEYS + row0 + lane;
+                        ok = step < end && j >= seen_from && j < hi;                                 // (what nobody sees is not there)
+                        const unsigned in = ok ? j : 0, which = in / page_size;
+                        page = table[which]; at = in - which * page_size;
+                    };
+                    auto fetch = [&]() {                                                             // of the step that was found last
+                        next_ok = ok && page >= 0 && page < p.view.n_pages;
+                        next_pair = pairs[(next_ok ? page : 0) * p.scales.page_stride + at * p.scales.token_stride];
+                    };
+                    if (en.begin < end) { find(en.begin); fetch(); find(en.begin + 1); }
+                    for (int step = en.begin; step < end; ++step) {
+                        if (LATE && p.late == PA_LATE_CHECKS && tiles < 12) { stand_still(4000); }
+                        uint32_t pair = next_ok ? no_large_scale(next_pair) : 0u;
+                        fetch(); find(step + 2);
+#pragma unroll 1
+                        for (int kv = 0; kv < 2; ++kv) {
+                            if (kv == 1 && !(en.whole(p, a, step) && (b.rows == 0 || en.whole(p, b, step)))) {
+                                // 0 x inf: positions that some rows see and others do not. They are taken out, and given back to the rows that see them
+                                const bool bad = large_scale(pair >> 16);
+                                if (__any_sync(0xffffffffu, bad)) {
+                                    if (bad) { pair &= 0xffffu; }
+                                    if (lane == 0) { *reinterpret_cast<volatile int *>(&sh.poison[stretch & 7]) = (int)stretch + 1; }
+                                }
+                            }
+                            wait_for(byte_full + 8 * byte_slot, byte_phase, limit);
+                            wait_for(empty + 8 * slot, phase ^ 1, limit);
+                            if (gave_up()) { break; }
+                            make_operand<HD>(byte_ring + byte_slot * Shape::BYTE_TILE, ring + slot * Shape::OPERAND, row0, pair, kv == 1);
+                            fence_async_smem();
+                            __syncwarp();
+                            if (lane == 0) { mbar_arrive(byte_empty + 8 * byte_slot); mbar_arrive(full + 8 * slot); }
+                            if (++byte_slot == Shape::BYTE_SLOTS) { byte_slot = 0; byte_phase ^= 1; }
+                            advance();
+                        }
+                        if (limit == 0) { break; }
+                        ++tiles;
+                    }
+                    if (limit == 0) { break; }
+                    __syncwarp();
+                    entry_read(lane == 0);
+                }
             }
         } else if (warp == 8) {
             // ------------------------------------------------------------------------------ MMAs
@@ -855,7 +867,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
                 --slot;
                 wait_for((BYTES ? byte_full : full) + 8 * slot, phase, again);
             }
-        } else if (warp >= 10) {
+        } else if (warp == 10 || warp == 11) {
             for (uint32_t i = 1; i <= Shape::Q_BUFFERS && i <= issued; ++i) {
                 const uint32_t n = issued - i;
                 wait_for(q_ready + 16 * (warp - 10) + 8 * (n % Shape::Q_BUFFERS), n / Shape::Q_BUFFERS & 1, again);
@@ -906,7 +918,7 @@ template <int HD, bool LATE, int KIND> cudaError_t registers_suffice() {
     static const cudaError_t answer = [] {
         cudaFuncAttributes a;
         const cudaError_t err = cudaFuncGetAttributes(&a, paged_tc_kernel<HD, LATE, KIND>);
-        return err != cudaSuccess ? err : a.numRegs * PT_THREADS >= 256 * PT_REGS_SOFTMAX + 128 * PT_REGS_OTHERS ? cudaSuccess : cudaErrorInvalidConfiguration;
+        return err != cudaSuccess ? err : a.numRegs * TcShape<HD, KIND>::THREADS >= 256 * TcShape<HD, KIND>::REGS_SOFTMAX + (TcShape<HD, KIND>::THREADS - 256) * TcShape<HD, KIND>::REGS_OTHERS ? cudaSuccess : cudaErrorInvalidConfiguration;
     }();
     return answer;
 }
@@ -916,7 +928,7 @@ cudaError_t launch_tc(const PagedAttention &p, const CUtensorMap &q, const CUten
     if (err != cudaSuccess) { return err; }
     err = allow_dynamic_smem(reinterpret_cast<const void *>(paged_tc_kernel<HD, LATE, KIND>), TcShape<HD, KIND>::SMEM);
     if (err != cudaSuccess) { return err; }
-    return launch_maybe_pdl(paged_tc_kernel<HD, LATE, KIND>, dim3(sms), PT_THREADS, TcShape<HD, KIND>::SMEM, cfg.stream, cfg.pdl, p, q, k, v, box, cfg.error_flag, wait_limit);
+    return launch_maybe_pdl(paged_tc_kernel<HD, LATE, KIND>, dim3(sms), TcShape<HD, KIND>::THREADS, TcShape<HD, KIND>::SMEM, cfg.stream, cfg.pdl, p, q, k, v, box, cfg.error_flag, wait_limit);
 }
 
 template <bool LATE, int KIND>
