@@ -320,6 +320,7 @@ template <int UNIT, int ALIGN> static int cut_selftest(uint32_t seed, int tile_r
 int paged_cut_selftest() {
     int bad = cut_selftest<64, 16>(1, 16);
     if (bad == 0) { bad = cut_selftest<64, 16>(2, 32); }
+    if (bad == 0) { bad = cut_selftest<64, 64>(4, 8); }
     if (bad == 0) { bad = cut_selftest<128, 128>(3, 0); }
     return bad == 0 ? 0 : 100 + bad;
 }
@@ -351,18 +352,20 @@ static PagedAppend append_of(spyb_backend *be, const spyb_paged_append_desc &giv
 // One pass over pages: sequences of many rows on tensor memory, the others on the kernel for few
 static spyb_status attention_pass(spyb_backend *be, PagedAttention p, int head_dim, int n_head, int64_t most, uint64_t wait_limit) {
     const LaunchCfg cfg = be->launch_cfg(be->config.use_pdl != 0);
+    const bool bytes = p.kind() == PK_INT8;
     p.few_rows = 1 << 30;
-    if (most > PA_FEW_ROWS && p.scale_log2 >= 0.f) {
+    if (most > (bytes ? PB_FEW_ROWS : PA_FEW_ROWS) && p.scale_log2 >= 0.f) {
         cudaError_t err = cudaSuccess;
-        p.few_rows = p.view.n_seq == 1 ? 0 : PA_FEW_ROWS;
+        // what single tokens beside the many rows have is the small kernel's in its narrowest tile
+        p.few_rows = p.view.n_seq == 1 ? 0 : !bytes ? PA_FEW_ROWS : p.group > PB_FEW_ROWS ? 0 : (p.group + 7) / 8 * 8;
         if (!launch_paged_attention_tc(p, head_dim, n_head, be->num_sms_total, cfg, wait_limit, &err)) { p.few_rows = 1 << 30; }
         SPYB_CUDA(be, err);
     }
     if (p.few_rows == 0) { return SPYB_SUCCESS; }
     const int64_t rows = std::min<int64_t>(most, p.few_rows);
     const int row_tiles = rows <= 16 ? 1 : 2;
-    p.tile_rows = p.kind() == PK_INT8 && rows <= 8 ? 8 : 16 * row_tiles;
-    SPYB_CUDA(be, p.kind() == PK_INT8 ? launch_paged_attention_bytes(p, head_dim, be->num_sms_total, cfg)
+    p.tile_rows = bytes ? (rows <= 8 ? 8 : rows <= 16 ? 16 : 24) : 16 * row_tiles;
+    SPYB_CUDA(be, bytes ? launch_paged_attention_bytes(p, head_dim, be->num_sms_total, cfg, wait_limit)
                   : p.kind() == PK_SHARED ? launch_paged_shared_rows(p, head_dim, row_tiles, be->num_sms_total, cfg)
                                           : launch_paged_attention_rows(p, head_dim, row_tiles, be->num_sms_total, cfg));
     return SPYB_SUCCESS;

@@ -77,13 +77,16 @@ cudaError_t launch_paged_shared(const PagedShared &p, const LaunchCfg &cfg);
 cudaError_t launch_paged_append(const PagedAppend &p, int in_type, int q_out_type, int sms, const LaunchCfg &cfg);
 cudaError_t launch_paged_attention_rows(const PagedAttention &p, int head_dim, int row_tiles, int sms, const LaunchCfg &cfg);
 cudaError_t launch_paged_shared_rows(const PagedAttention &p, int head_dim, int row_tiles, int sms, const LaunchCfg &cfg);   // (PK_SHARED)
-cudaError_t launch_paged_attention_bytes(const PagedAttention &p, int head_dim, int sms, const LaunchCfg &cfg);               // (PK_INT8; tiles of 8, 16 or 32 rows)
+cudaError_t launch_paged_attention_bytes(const PagedAttention &p, int head_dim, int sms, const LaunchCfg &cfg, uint64_t wait_limit);   // (PK_INT8; tiles of 8, 16 or 24 rows)
 // the kernel on tensor memory; false where it does not take these pages, heads or strides (nothing is launched then)
 bool        launch_paged_attention_tc(const PagedAttention &p, int head_dim, int n_head, int sms, const LaunchCfg &cfg, uint64_t wait_limit, cudaError_t *err);
 // Sequences of up to so many rows (times query heads of a K/V head) are the small kernel's, whose tile of 16 rows costs them nothing but the memory's time; a second tile
 // doubles its instructions. 24 sequences of up to 9000 positions, four query heads a K/V head: 3 and 4 rows (12 and 16 in all) 95 and 98 us there against
 // 118 and 118 on tensor memory, 5 and 8 rows (20 and 32) 144 and 156 against 118 and 118.
 constexpr int PA_FEW_ROWS = 16;
+// The same of the small kernel for bytes, whose tiles have 8, 16 or 24 rows: the 24 sequences at 3 and 4 rows (12 and 16 in all) 82 and 87 us, at 5 and 6 (20 and 24) 124 and 130, on tensor memory 146
+// for any of these, 149 at 8 rows (32), where two small tiles take 221.
+constexpr int PB_FEW_ROWS = 24;
 
 // What every operator asks of the cache and the batch; `scales`: those that may come with bytes (nullptr: an fp16 cache alone)
 struct Refusal;

@@ -8,31 +8,35 @@
 //   Scales stay out of the products' operands: K's multiply scores (where scale and log2 e are a product anyway), V's the probabilities, in f32. So that no probability leaves fp16's range,
 //   V's scales are taken against the largest so far, rounded up to a power of two; like the maximum of the scores it moves a few times at the start and hardly ever after.
 
+#include <cuda.h>
+
 #include "spyb_internal.h"
 #include "spyb_paged.cuh"
+#include "spyb_paged_maps.h"
 #include "spyb_paged_rows.cuh"
+#include "spyb_tc.cuh"
 
 namespace spyb {
 namespace {
 
+constexpr int PB_THREADS = (PR_WARPS + 1) * 32, PB_STAGE = PR_WARPS * PR_BLOCK;   // four warps that compute and one that copies; positions of a stage of the ring, 16 a warp
 template <int HD> struct BytesShape {
-    static constexpr int ROW = HD == 96 ? 128 : HD;                  // bytes of a position in shared memory
-    static constexpr int SCALES = 2 * PR_BLOCK * ROW, STAGE = SCALES + PR_BLOCK * 4;
-    static constexpr int STAGES = HD <= 64 ? 4 : 3;
-    static constexpr int RING = PR_WARPS * STAGES * STAGE;
+    static constexpr int ROW = HD == 96 ? 128 : HD, TILE = PR_BLOCK * ROW;   // bytes of a position in shared memory, of 16
+    static constexpr int V_AT = PB_STAGE * ROW, STAGE = 2 * V_AT;
     static constexpr int PIECES = HD / 16;                           // 16-byte pieces of a position
-    // where byte 16 c of position r lies: what a quarter of a warp reads at a time - two positions side by side, or every second one - lies in other banks
+    // where byte 16 c of position r lies: the tensor maps' swizzles of 128 and 64 bytes
     static __device__ __forceinline__ int place(int r, int c) {
-        if (HD > 64) { return r * ROW + ((c ^ (r & 7)) << 4); }
-        if (HD == 64) { return (r >> 1) * 128 + ((((r ^ (r >> 2)) & 1) * 4 + (c ^ (r & 2))) << 4); }
-        return r * ROW + (c << 4);
+        return HD > 64 ? r * ROW + ((c ^ (r & 7)) << 4) : HD == 64 ? r * ROW + ((c ^ (r >> 1 & 3)) << 4) : r * ROW + (c << 4);
     }
 };
-template <int HD, int NT> struct BytesSmem {       // the ring; what the warps found: beside it for up to EARLY rows, in its place for more; the masks of the ring's stages
+// the ring, what the warps found, scales of the ring's stages
+template <int HD, int NT> struct BytesSmem {
     using Shape = BytesShape<HD>;
-    static constexpr int CTAS = NT == 1 ? 4 : NT == 2 ? 3 : 2;        // of an SM
-    static constexpr int EARLY = NT == 1 && HD <= 64 ? 8 : 0, FOUND = PR_WARPS * 8 * NT * (HD + 2) * 4, RING = Shape::RING > FOUND ? Shape::RING : FOUND;
-    static constexpr int MASKS = RING + PR_WARPS * EARLY * (HD + 2) * 4, BYTES = MASKS + PR_WARPS * Shape::STAGES * 4;
+    static constexpr int CTAS = NT == 1 ? 3 : 2;                     // of an SM
+    static constexpr int STAGES = 3;
+    static constexpr bool Q_SHARED = NT > 2;                         // Q's operands in shared memory, all warps' (they would not leave room for the sums in registers)
+    static constexpr int FOUND = STAGES * Shape::STAGE, QUERY = FOUND + PR_WARPS * 8 * NT * (HD + 2) * 4, SCALES = QUERY + (Q_SHARED ? NT * HD * 16 : 0);
+    static constexpr int BYTES = SCALES + STAGES * PB_STAGE * 4 + 1024;   // (+ alignment)
 };
 // N bytes of position r from byte N i on, as words
 template <class Shape, int N> __device__ __forceinline__ void lds_row(uint32_t addr, int r, int i, uint32_t (&w)[N / 4]) {
@@ -57,9 +61,13 @@ template <class Shape, int N> __device__ __forceinline__ void lds_row(uint32_t a
 __device__ __forceinline__ void cp_async4(uint32_t dst, const void *src, bool there) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(there ? 4 : 0) : "memory");
 }
+__device__ __forceinline__ void mma_f(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {   // (not volatile: the compiler may move it)
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
 __device__ __forceinline__ uint32_t transposed(uint32_t x) {   // of an 8 x 8 matrix, two elements a lane
     uint32_t y;
-    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
     return y;
 }
 __device__ __forceinline__ float over_groups(float v, bool largest) {   // over the lanes that have the same query rows
@@ -68,127 +76,196 @@ __device__ __forceinline__ float over_groups(float v, bool largest) {   // over 
     return v;
 }
 
-// IN_PAGE: a block's positions lie in one page (pages of a multiple of 16, but for heads of 96)
-template <int HD, int NT, bool IN_PAGE>
-__global__ void __launch_bounds__(PR_WARPS * 32, BytesSmem<HD, NT>::CTAS) paged_bytes_kernel(const __grid_constant__ PagedAttention p) {
+__device__ __forceinline__ void sts64(uint32_t addr, uint2 v) { asm volatile("st.shared.v2.u32 [%0], {%1,%2};" ::"r"(addr), "r"(v.x), "r"(v.y) : "memory"); }
+__device__ __forceinline__ void tma_pages(uint32_t dst, const CUtensorMap *map, uint32_t bar, int token, int head, int page) {
+    asm volatile("cp.async.bulk.tensor.4d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3,%4,%5,%6}], [%2];"
+                 ::"r"(dst), "l"(map), "r"(bar), "r"(0), "r"(token), "r"(head), "r"(page) : "memory");
+}
+__device__ __forceinline__ void arrive_when_copied(uint32_t bar) { asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory"); }   // of this lane's copies so far
+// A CTA's part of an item, found by the copying warp for all: rows of the tile, stages of the ring, positions [ka, kb); rows 0: behind the last one
+struct BytesEntry { int rows, n_stage, ka, kb, tile, head, row0, first, from, c0, parts; };
+constexpr int PB_ENTRIES = 4;                 // known ahead
+
+// One warp copies for four that compute (with each its own copies a block's took a third of the warp's time on it: some hundred instructions of addresses).
+// MAPS: K and V come by tensor maps, boxes of `box` positions that lie in one page (pages of a multiple of 16, heads of 64 and 128); otherwise by 16 bytes a lane.
+template <int HD, int NT, bool MAPS>
+__global__ void __launch_bounds__(PB_THREADS, BytesSmem<HD, NT>::CTAS) paged_bytes_kernel(const __grid_constant__ PagedAttention p, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
+                                                                                          const int box, int *error_flag, const uint64_t wait_limit) {
     using Shape = BytesShape<HD>;
     using Smem = BytesSmem<HD, NT>;
-    constexpr int STAGES = Shape::STAGES, TILE = 8 * NT, STAGE = Shape::STAGE, V_AT = PR_BLOCK * Shape::ROW, PIECES = Shape::PIECES;
-    extern __shared__ __align__(128) uint8_t smem[];
+    constexpr int STAGES = Smem::STAGES, ROWS = 8 * NT, TILE = Shape::TILE, V_AT = Shape::V_AT, PIECES = Shape::PIECES;
+    extern __shared__ uint8_t raw[];
     __shared__ PagedPlanShared plan;
     __shared__ int last_one;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-    uint32_t *there = reinterpret_cast<uint32_t *>(smem + Smem::MASKS) + warp * STAGES;
-    const uint32_t ring = smem_u32(smem) + warp * STAGES * STAGE;
+    __shared__ uint64_t full_bars[STAGES], empty_bars[STAGES], known_bars[PB_ENTRIES], read_bars[PB_ENTRIES], joined_bar;
+    __shared__ BytesEntry entries[PB_ENTRIES];
+    __shared__ __align__(8) uint16_t there[STAGES][PR_WARPS];   // which positions of a stage are there
+    uint8_t *const smem = raw + (-smem_u32(raw) & 1023);
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const uint32_t ring = smem_u32(smem), scales = ring + Smem::SCALES, full = smem_u32(full_bars), empty = smem_u32(empty_bars), known = smem_u32(known_bars), read = smem_u32(read_bars);
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < STAGES; ++i) { mbar_init(full + 8 * i, 33); mbar_init(empty + 8 * i, PR_WARPS); }
+        mbar_init(smem_u32(&joined_bar), PR_WARPS);
+        for (int i = 0; i < PB_ENTRIES; ++i) { mbar_init(known + 8 * i, 1); mbar_init(read + 8 * i, PR_WARPS); }
+        mbar_init_fence();
+    }
+    if (MAPS && threadIdx.x == PR_WARPS * 32) {
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&k_map) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&v_map) : "memory");
+    }
     pdl_launch_dependents();
     pdl_wait();
-    PagedPlace at = paged_plan<PR_WARPS * 32, PR_UNIT, PR_BLOCK>(p, true, 1, plan);
+    PagedPlace at = paged_plan<PB_THREADS, PB_STAGE, PB_STAGE>(p, true, 1, plan);
     if (at.unit >= at.end) { return; }
-    PagedSeq q = paged_seq(p.view, at.seq);
-    int seq = at.seq, head = at.head, tile = at.tile, off = at.off;
-    PagedItem it;
-    int todo, ka, kb, n_block, packed;        // of the item that comes next: units of this CTA, positions [ka, kb), blocks of them; rows of the tile
-    const int32_t *table;
-    const uint8_t *kbase, *vbase;
-    const uint32_t *sbase;
-    auto describe = [&]() {
-        it = paged_item<PR_UNIT, PR_BLOCK>(p, q, tile);
-        todo = (int)min((int64_t)(it.units - off), at.end - at.unit);
-        ka = it.lo + off * PR_UNIT; kb = min(it.hi, ka + todo * PR_UNIT);
-        n_block = kb > ka ? (kb - ka + PR_BLOCK - 1) / PR_BLOCK : 0;
-        packed = min(TILE, q.rows * p.group - tile * TILE);
-        table = p.view.page_table + (int64_t)seq * p.view.table_stride;
-        kbase = reinterpret_cast<const uint8_t *>(p.k) + head * p.view.head_stride; vbase = reinterpret_cast<const uint8_t *>(p.v) + head * p.view.head_stride;
-        sbase = p.scales.pairs + head * p.scales.head_stride;
-    };
-    auto page_of = [&](int b) {              // page of block b, or (lanes 0..15 and 16..31 alike) of this lane's position in it; -1: none
-        const int j = ka + b * PR_BLOCK + (IN_PAGE ? 0 : lane & 15);
-        return b < n_block && j < kb ? table[p.page_shift >= 0 ? j >> p.page_shift : j / p.view.page_size] : -1;
-    };
-    auto issue = [&](int b, int stage, int page) {
-        const int j = ka + b * PR_BLOCK + (IN_PAGE ? 0 : lane & 15);
-        const bool ok = page >= 0 && page < p.view.n_pages;
-        const int in_page = p.page_shift >= 0 ? j & (p.view.page_size - 1) : j % p.view.page_size;
-        const int64_t cell = ok ? page * p.view.page_stride + in_page * p.view.token_stride : 0;
-        const unsigned mask = IN_PAGE ? (ok ? (kb - j >= PR_BLOCK ? 0xffffu : (1u << (kb - j)) - 1) : 0u) : __ballot_sync(0xffffffffu, ok) & 0xffffu;
-        const uint32_t dst = ring + stage * STAGE;
-        {
-            const int r = lane & 15;                          // (lanes 0..15: the scales of a position each)
-            const bool in = (mask >> r) & 1;
-            const int64_t o = in ? p.scales.page_stride * page + p.scales.token_stride * (in_page + (IN_PAGE ? r : 0)) : 0;
-            if (lane < 16) { cp_async4(dst + Shape::SCALES + r * 4, sbase + o, in); }
-        }
-        if constexpr (IN_PAGE) {
-            constexpr int AT_ONCE = 32 / PIECES;              // (a row's pieces are lanes side by side)
-            const int r0 = lane / PIECES, c = lane % PIECES;
-            int64_t o = cell + r0 * p.view.token_stride + c * 16;
-            const int64_t more = AT_ONCE * p.view.token_stride;
+    uint64_t limit = wait_limit;              // (0: a wait of this warp has run out. It frees nothing and copies nothing any more, so the others' run out in turn)
+    uint32_t stage = 0, phase = 0;
+    auto advance = [&]() { if (++stage == STAGES) { stage = 0; phase ^= 1; } };
+    if (warp == PR_WARPS) {
+        // ---------------------------------------------------------------------------------- copies
+        uint32_t issued = 0, entry = 0;
+        PagedSeq q = paged_seq(p.view, at.seq);
+        int seq = at.seq, head = at.head, tile = at.tile, off = at.off;
+        auto put = [&](const BytesEntry &e) {                 // false: a wait has run out
+            const uint32_t i = entry & (PB_ENTRIES - 1);
+            mbar_wait_lean(read + 8 * i, ((entry / PB_ENTRIES) & 1) ^ 1, limit);
+            if (!__all_sync(0xffffffffu, limit != 0)) { limit = 0; return false; }
+            if (lane == 0) { entries[i] = e; mbar_arrive(known + 8 * i); }
+            ++entry;
+            return true;
+        };
+        for (bool more = true; more;) {
+            const PagedItem it = paged_item<PB_STAGE, PB_STAGE>(p, q, tile);   // (stages begin where boxes do)
+            const int todo = (int)min((int64_t)(it.units - off), at.end - at.unit), ka = it.lo + off * PB_STAGE, kb = min(it.hi, ka + todo * PB_STAGE), n_stage = kb > ka ? (kb - ka + PB_STAGE - 1) / PB_STAGE : 0;
+            const PagedCut cut = paged_cut(at, at.unit - off, it.units);
+            const BytesEntry e = {min(ROWS, q.rows * p.group - tile * ROWS), n_stage, ka, kb, tile, head, q.row0, q.first, q.from, cut.c0, cut.parts};
+            if (!put(e)) { break; }
+            const int32_t *table = p.view.page_table + (int64_t)seq * p.view.table_stride;
+            const uint32_t *pairs = p.scales.pairs + head * p.scales.head_stride;
+            int page[2];                                      // of this lane's two positions of a stage, read a stage ahead. (No branch around the loads, or they are waited for where they stand)
+            auto find = [&](int s) {
 #pragma unroll
-            for (int i = 0; i < PIECES / 2; ++i) {
-                const int r = i * AT_ONCE + r0;
-                const bool in = (mask >> r) & 1;
-                const uint32_t d = dst + Shape::place(r, c);
-                const int64_t from = in ? o : 0;
-                cp_async16(d, kbase + from, in);
-                cp_async16(d + V_AT, vbase + from, in);
-                o += more;
-            }
-        } else {
+                for (int i = 0; i < 2; ++i) {
+                    const int j = min(ka + s * PB_STAGE + 32 * i + lane, kb - 1);
+                    page[i] = table[p.page_shift >= 0 ? j >> p.page_shift : j / p.view.page_size];
+                }
+            };
+            if (n_stage > 0) { find(0); }
+            for (int s = 0; s < n_stage; ++s) {
+                mbar_wait_lean(empty + 8 * stage, phase ^ 1, limit);
+                if (!__all_sync(0xffffffffu, limit != 0)) { limit = 0; break; }
+                const uint32_t bar = full + 8 * stage, dst = ring + stage * Shape::STAGE;
+                int in[2], at[2];
+                bool ok[2];
+                unsigned mask[2];
 #pragma unroll
-            for (int i = 0; i < PIECES / 2; ++i) {
-                const int x = i * 32 + lane, r = x / PIECES, c = x - r * PIECES;
-                const bool in = (mask >> r) & 1;
-                const int64_t row = __shfl_sync(0xffffffffu, cell, r), o = in ? row + c * 16 : 0;
-                const uint32_t d = dst + Shape::place(r, c);
-                cp_async16(d, kbase + o, in);
-                cp_async16(d + V_AT, vbase + o, in);
+                for (int i = 0; i < 2; ++i) {
+                    const int j = ka + s * PB_STAGE + 32 * i + lane;
+                    in[i] = p.page_shift >= 0 ? j & (p.view.page_size - 1) : j % p.view.page_size;
+                    at[i] = page[i];
+                    ok[i] = j < kb && at[i] >= 0 && at[i] < p.view.n_pages;
+                    mask[i] = __ballot_sync(0xffffffffu, ok[i]);
+                }
+                if (s + 1 < n_stage) { find(s + 1); }
+                if (lane == 0) {
+                    *reinterpret_cast<uint2 *>(there[stage]) = make_uint2(mask[0], mask[1]);
+                    if (MAPS) { mbar_expect_tx(bar, Shape::STAGE); } else { mbar_arrive(bar); }
+                }
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    cp_async4(scales + (stage * PB_STAGE + 32 * i + lane) * 4, pairs + (ok[i] ? at[i] * p.scales.page_stride + in[i] * p.scales.token_stride : 0), ok[i]);
+                }
+                if constexpr (MAPS) {
+                    __syncwarp();
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const int r = 32 * i + lane;
+                        if ((r & (box - 1)) == 0) {           // (a box that is not there: a page behind the last one, which reads as zeros; positions behind kb are read, and masked)
+                            const int from = ok[i] ? at[i] : p.view.n_pages, token = ok[i] ? in[i] : 0;
+                            tma_pages(dst + r * Shape::ROW, &k_map, bar, token, head, from);
+                            tma_pages(dst + V_AT + r * Shape::ROW, &v_map, bar, token, head, from);
+                        }
+                        __syncwarp();
+                    }
+                } else {
+                    const uint8_t *kbase = reinterpret_cast<const uint8_t *>(p.k) + head * p.view.head_stride, *vbase = reinterpret_cast<const uint8_t *>(p.v) + head * p.view.head_stride;
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const int64_t cell = ok[h] ? at[h] * p.view.page_stride + in[h] * p.view.token_stride : 0;
+#pragma unroll 2
+                        for (int i = 0; i < PIECES; ++i) {
+                            const int x = i * 32 + lane, r = x / PIECES, c = x - r * PIECES;
+                            const bool is = (mask[h] >> r) & 1;
+                            const int64_t from = __shfl_sync(0xffffffffu, cell, r), o = is ? from + c * 16 : 0;
+                            const uint32_t d = dst + h * 32 * Shape::ROW + Shape::place(r, c);
+                            cp_async16(d, kbase + o, is);
+                            cp_async16(d + V_AT, vbase + o, is);
+                        }
+                    }
+                }
+                arrive_when_copied(bar);
+                advance();
+                ++issued;
+            }
+            if (limit == 0) { break; }
+            at.unit += todo + p.start_units;
+            off = 0;
+            more = at.unit < at.end && paged_next(p, true, q, seq, head, tile);
+        }
+        if (limit != 0) { const BytesEntry over = {}; put(over); }
+        if (limit == 0) {                     // what is still on its way lands before the CTA ends
+            if (lane == 0) { pf_report(error_flag, 7); }
+            uint64_t again = 1000000000;
+            for (uint32_t i = 0; i < STAGES && i < issued; ++i) {
+                if (stage == 0) { stage = STAGES; phase ^= 1; }
+                --stage;
+                mbar_wait_lean(full + 8 * stage, phase, again);
             }
         }
-        if (lane == 0) { there[stage] = mask; }
-        cp_commit();
-    };
-
-    // IN_PAGE: a lane has the page of every 32nd block of this warp, the next 32 are read while these are in use; a block's is told by its lane
-    int page = -1, ids = -1, ids_next = -1, issued = 0;   // (page: of the block that is issued next)
-    auto next_page = [&](int b) {             // of block b, the `issued`-th of this warp
-        if (!IN_PAGE) { return page_of(b); }
-        const int l = issued & 31;
-        if (l == 0) { ids = ids_next; ids_next = page_of(warp + (issued + 32 + lane) * PR_WARPS); }
-        ++issued;
-        return __shfl_sync(0xffffffffu, ids, l);
-    };
-    uint32_t qf[NT][HD / 16][2];              // row g of each tile of eight, elements t HD / 4 on, four a product
+        return;
+    }
+    // -------------------------------------------------------------------------------------- scores, probabilities, sums
+    const int g = lane >> 2, t = lane & 3;
+    uint2 qf[Smem::Q_SHARED ? 1 : NT][HD / 16];   // row g of each tile of eight, elements t HD / 4 on, four a product
+    const uint32_t q_at = ring + Smem::QUERY + lane * 8;   // or [tile][product][lane]
     int pos[NT][2];                           // of rows 2 t, 2 t + 1
-    auto start = [&]() {                      // the item's first blocks are on their way while its Q comes
-        issued = 0;
-        if (IN_PAGE) { ids_next = page_of(warp + lane * PR_WARPS); }
-        page = next_page(warp);
-#pragma unroll
-        for (int i = 0; i < STAGES - 1; ++i) {
-            const int next = next_page(warp + (i + 1) * PR_WARPS);
-            if (warp + i * PR_WARPS < n_block) { issue(warp + i * PR_WARPS, i, page); } else { cp_commit(); }
-            page = next;
-        }
+    uint32_t entry = 0, joined_phase = 0;
+    auto meet = [&]() {                       // the four warps (a barrier whose wait ends: one of them may have given up)
+        __syncwarp();
+        if (lane == 0) { mbar_arrive(smem_u32(&joined_bar)); }
+        mbar_wait_lean(smem_u32(&joined_bar), joined_phase, limit);
+        if (!__all_sync(0xffffffffu, limit != 0)) { limit = 0; }
+        joined_phase ^= 1;
+    };
+    BytesEntry e;
+    auto next = [&]() {                       // the next item and its Q; false behind the last one, or when a wait has run out
+        const uint32_t i = entry & (PB_ENTRIES - 1);
+        mbar_wait_lean(known + 8 * i, (entry / PB_ENTRIES) & 1, limit);
+        if (!__all_sync(0xffffffffu, limit != 0)) { limit = 0; return false; }
+        e = entries[i];
+        ++entry;
+        __syncwarp();
+        if (lane == 0) { mbar_arrive(read + 8 * i); }
+        if (e.rows == 0) { return false; }
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-            {
-                const int r = n * 8 + g, pr = tile * TILE + min(r, packed - 1);
+            if (!Smem::Q_SHARED || n % PR_WARPS == warp) {
+                const int r = n * 8 + g, pr = e.tile * ROWS + min(r, e.rows - 1);
                 const int token = (int)((unsigned)pr / (unsigned)p.group), h = pr - token * p.group;
-                const uint2 *src = reinterpret_cast<const uint2 *>(p.q + (int64_t)(q.row0 + token) * p.q_stride + (head * p.group + h) * HD) + t * (HD / 16);
+                const uint2 *src = reinterpret_cast<const uint2 *>(p.q + (int64_t)(e.row0 + token) * p.q_stride + (e.head * p.group + h) * HD) + t * (HD / 16);
 #pragma unroll
                 for (int ks = 0; ks < HD / 16; ++ks) {
-                    const uint2 x = r < packed ? src[ks] : make_uint2(0, 0);
-                    qf[n][ks][0] = x.x; qf[n][ks][1] = x.y;
+                    const uint2 x = r < e.rows ? src[ks] : make_uint2(0, 0);
+                    if (Smem::Q_SHARED) { sts64(q_at + (n * (HD / 16) + ks) * 256, x); } else { qf[Smem::Q_SHARED ? 0 : n][ks] = x; }
                 }
             }
 #pragma unroll
-            for (int e = 0; e < 2; ++e) { pos[n][e] = q.first + (int)((unsigned)(tile * TILE + min(n * 8 + 2 * t + e, packed - 1)) / (unsigned)p.group); }
+            for (int i = 0; i < 2; ++i) { pos[n][i] = e.first + (int)((unsigned)(e.tile * ROWS + min(n * 8 + 2 * t + i, e.rows - 1)) / (unsigned)p.group); }
         }
+        if (Smem::Q_SHARED) { meet(); }
+        return true;
     };
-    describe();
-    start();
-    for (;;) {
-        const int pos_first = q.first + (int)((unsigned)(tile * TILE) / (unsigned)p.group), pos_last = q.first + (int)((unsigned)(tile * TILE + packed - 1) / (unsigned)p.group);
+    while (next()) {
+        const int first_row = e.tile * ROWS, pos_first = e.first + (int)((unsigned)first_row / (unsigned)p.group), pos_last = e.first + (int)((unsigned)(first_row + e.rows - 1) / (unsigned)p.group);
         float o[NT][HD / 16][4], mx[NT][2], sum[NT][2], base[NT][2], over[NT][2];   // (base: the maximum, or 0 for none; over: scores beyond it move the maximum)
         float unit = 1099511627776.f;             // one over the power of two that V's scales are taken against: 2^-40 at first, below the least scale
 #pragma unroll
@@ -197,30 +274,22 @@ __global__ void __launch_bounds__(PR_WARPS * 32, BytesSmem<HD, NT>::CTAS) paged_
 #pragma unroll
             for (int i = 0; i < HD / 16; ++i) { o[n][i][0] = o[n][i][1] = o[n][i][2] = o[n][i][3] = 0.f; }
         }
-        int stage = 0;
-        for (int b = warp; b < n_block; b += PR_WARPS) {
-            {
-                const int ahead = b + (STAGES - 1) * PR_WARPS, next = next_page(ahead + PR_WARPS);
-                const int to = stage == 0 ? STAGES - 1 : stage - 1;
-                __syncwarp();
-                if (ahead < n_block) { issue(ahead, to, page); } else { cp_commit(); }
-                page = next;
-            }
-            cp_wait<STAGES - 1>();
-            __syncwarp();
-            const uint32_t k_addr = ring + stage * STAGE, v_addr = k_addr + V_AT;
-            const uint32_t mask = there[stage];
-            const int j0 = ka + b * PR_BLOCK;
+        for (int s = 0; s < e.n_stage; ++s) {
+            mbar_wait_lean(full + 8 * stage, phase, limit);
+            if (!__all_sync(0xffffffffu, limit != 0)) { limit = 0; break; }
+            const uint32_t k_addr = ring + stage * Shape::STAGE + warp * TILE, v_addr = k_addr + V_AT, s_addr = scales + (stage * PB_STAGE + warp * PR_BLOCK) * 4;
+            const uint32_t mask = there[stage][warp];
+            const int j0 = e.ka + s * PB_STAGE + warp * PR_BLOCK;
             const bool whole = mask == 0xffffu && (!p.causal || (j0 + PR_BLOCK - 1 <= pos_first && (p.window <= 0 || j0 > pos_last - p.window)));
             // scores of positions g and g + 8
             float sc[NT][4], v_scale[2], k_scale[2];
-#pragma unroll
-            for (int n = 0; n < NT; ++n) { sc[n][0] = sc[n][1] = sc[n][2] = sc[n][3] = 0.f; }
             {
+#pragma unroll
+                for (int n = 0; n < NT; ++n) { sc[n][0] = sc[n][1] = sc[n][2] = sc[n][3] = 0.f; }
                 uint32_t w0[HD / 16], w1[HD / 16];
                 lds_row<Shape, HD / 4>(k_addr, g, t, w0);
                 lds_row<Shape, HD / 4>(k_addr, g + 8, t, w1);
-                const float2 s0 = half2_bits(lds32(k_addr + Shape::SCALES + g * 4)), s1 = half2_bits(lds32(k_addr + Shape::SCALES + g * 4 + 32));
+                const float2 s0 = half2_bits(lds32(s_addr + g * 4)), s1 = half2_bits(lds32(s_addr + (g + 8) * 4));
                 k_scale[0] = fmaf(s0.x, 0.f, s0.x * p.scale_log2); k_scale[1] = fmaf(s1.x, 0.f, s1.x * p.scale_log2);   // (an infinite one is NaN: its elements' infinities do not add up to one)
                 v_scale[0] = s0.y; v_scale[1] = s1.y;
 #pragma unroll
@@ -229,151 +298,158 @@ __global__ void __launch_bounds__(PR_WARPS * 32, BytesSmem<HD, NT>::CTAS) paged_
                     halves_of(w0[ks], a[0], a[2]);
                     halves_of(w1[ks], a[1], a[3]);
 #pragma unroll
-                    for (int n = 0; n < NT; ++n) { mma16816(sc[n], a, qf[n][ks][0], qf[n][ks][1]); }
+                    for (int n = 0; n < NT; ++n) {
+                        const uint2 b = Smem::Q_SHARED ? lds64(q_at + (n * (HD / 16) + ks) * 256) : qf[Smem::Q_SHARED ? 0 : n][ks];
+                        mma_f(sc[n], a, b.x, b.y);
+                    }
                 }
             }
             // against the maximum, in powers of two
             bool above = false, odd = false;                  // (odd: a scale of V is not finite)
+            {
 #pragma unroll
-            for (int n = 0; n < NT; ++n) {
+                for (int n = 0; n < NT; ++n) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    float &x = sc[n][e];
-                    x = fmaf(x, k_scale[e >> 1], -base[n][e & 1]);
-                    if (!whole) {
-                        const int jj = g + (e >> 1) * 8, d = pos[n][e & 1] - (j0 + jj);
-                        const bool seen = ((mask >> jj) & 1) && (!p.causal || (d >= 0 && (p.window <= 0 || d < p.window)));
-                        x = seen ? x : -CUDART_INF_F;
+                    for (int e = 0; e < 4; ++e) {
+                        float &x = sc[n][e];
+                        x = fmaf(x, k_scale[e >> 1], -base[n][e & 1]);
+                        if (!whole) {
+                            const int jj = g + (e >> 1) * 8, d = pos[n][e & 1] - (j0 + jj);
+                            const bool seen = ((mask >> jj) & 1) && (!p.causal || (d >= 0 && (p.window <= 0 || d < p.window)));
+                            x = seen ? x : -CUDART_INF_F;
+                        }
+                        above |= x > over[n][e & 1];
                     }
-                    above |= x > over[n][e & 1];
                 }
+#pragma unroll
+                for (int e = 0; e < 2; ++e) { v_scale[e] *= unit; above |= !(fabsf(v_scale[e]) <= 1.f); }
             }
-            v_scale[0] *= unit; v_scale[1] *= unit;
-            if (__any_sync(0xffffffffu, above || !(fmaxf(fabsf(v_scale[0]), fabsf(v_scale[1])) <= 1.f) || v_scale[0] != v_scale[0] || v_scale[1] != v_scale[1])) {
-                const bool fine0 = fabsf(v_scale[0]) < CUDART_INF_F, fine1 = fabsf(v_scale[1]) < CUDART_INF_F;
-                odd = __any_sync(0xffffffffu, !fine0 || !fine1);
-                const float most = over_groups(fmaxf(fmaxf(fine0 ? fabsf(v_scale[0]) : 0.f, fine1 ? fabsf(v_scale[1]) : 0.f), 1.f), true);
+            if (__any_sync(0xffffffffu, above)) {
+                float most = 1.f;
+                bool  fine = true;
+                {
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) { const bool is = fabsf(v_scale[e]) < CUDART_INF_F; fine &= is; most = fmaxf(most, is ? fabsf(v_scale[e]) : 1.f); }
+                }
+                odd = !__all_sync(0xffffffffu, fine);
+                most = over_groups(most, true);
                 const uint32_t up = (__float_as_uint(most) + 0x7fffffu) & 0x7f800000u;      // the next power of two, 2^56 at most
                 const float f_scale = __uint_as_float(0x7f000000u - up);                    // one over it
-                unit *= f_scale; v_scale[0] *= f_scale; v_scale[1] *= f_scale;
+                unit *= f_scale;
+                { v_scale[0] *= f_scale; v_scale[1] *= f_scale; }
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
-                        const float v = over_groups(fmaxf(sc[n][e], sc[n][2 + e]), true);
-                        const bool  moves = v > over[n][e];
-                        const float to = moves ? fmaxf(mx[n][e], base[n][e] + v) : mx[n][e], f = to == mx[n][e] ? 1.f : ex2(mx[n][e] - to);   // (2^-inf = 0 at the first)
+                        float v = fmaxf(sc[n][e], sc[n][2 + e]);
+                        v = over_groups(v, true);
+                        const float to = v > over[n][e] ? fmaxf(mx[n][e], base[n][e] + v) : mx[n][e], f = to == mx[n][e] ? 1.f : ex2(mx[n][e] - to);   // (2^-inf = 0 at the first)
                         const float from = base[n][e], f_o = f * f_scale;
                         mx[n][e] = to; sum[n][e] *= f;
                         base[n][e] = to == -CUDART_INF_F ? 0.f : to;
                         over[n][e] = to == -CUDART_INF_F ? to : 8.f;
-                        sc[n][e] += from - base[n][e]; sc[n][2 + e] += from - base[n][e];
+                        { sc[n][e] += from - base[n][e]; sc[n][2 + e] += from - base[n][e]; }
 #pragma unroll
                         for (int i = 0; i < HD / 16; ++i) { o[n][i][e] *= f_o; o[n][i][2 + e] *= f_o; }
                     }
                 }
             }
-            uint32_t pf[NT][2];
+            {
+                uint32_t pf[NT][2];
 #pragma unroll
-            for (int n = 0; n < NT; ++n) {
+                for (int n = 0; n < NT; ++n) {
 #pragma unroll
-                for (int hf = 0; hf < 2; ++hf) {
-                    const float a = ex2(sc[n][2 * hf]), c = ex2(sc[n][2 * hf + 1]);
-                    sum[n][0] += a; sum[n][1] += c;
-                    float u = a * v_scale[hf], w = c * v_scale[hf];
-                    if (odd) {                                // what is not seen is 0 whatever its scale is
-                        u = sc[n][2 * hf] == -CUDART_INF_F ? 0.f : u;
-                        w = sc[n][2 * hf + 1] == -CUDART_INF_F ? 0.f : w;
+                    for (int hf = 0; hf < 2; ++hf) {
+                        const float a = ex2(sc[n][2 * hf]), c = ex2(sc[n][2 * hf + 1]);
+                        sum[n][0] += a; sum[n][1] += c;
+                        float x = a * v_scale[hf], y = c * v_scale[hf];
+                        if (odd) {                            // what is not seen is 0 whatever its scale is
+                            x = sc[n][2 * hf] == -CUDART_INF_F ? 0.f : x;
+                            y = sc[n][2 * hf + 1] == -CUDART_INF_F ? 0.f : y;
+                        }
+                        pf[n][hf] = transposed(pack2(x, y));
                     }
-                    pf[n][hf] = transposed(pack2(u, w));
+                }
+                // a lane has elements g HD / 8 on of positions 2 t, 2 t + 1, 2 t + 8, 2 t + 9: the i-th product's rows g and g + 8 are elements 2 i and 2 i + 1 of these
+                uint32_t vw[4][HD / 32];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) { lds_row<Shape, HD / 8>(v_addr, (i >> 1) * 8 + t * 2 + (i & 1), g, vw[i]); }
+                __syncwarp();
+                if (lane == 0) { mbar_arrive(empty + 8 * stage); }
+#pragma unroll
+                for (int w = 0; w < HD / 32; ++w) {
+                    uint32_t b0[4], b1[4];
+                    pairs_of(vw[0][w], vw[1][w], b0);
+                    pairs_of(vw[2][w], vw[3][w], b1);
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const uint32_t a[4] = {b0[2 * i], b0[2 * i + 1], b1[2 * i], b1[2 * i + 1]};
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) { mma_f(o[n][2 * w + i], a, pf[n][0], pf[n][1]); }
+                    }
                 }
             }
-            // a lane has elements g HD / 8 on of positions 2 t, 2 t + 1, 2 t + 8, 2 t + 9: the i-th product's rows g and g + 8 are elements 2 i and 2 i + 1 of these
-            uint32_t vw[4][HD / 32];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) { lds_row<Shape, HD / 8>(v_addr, (i >> 1) * 8 + t * 2 + (i & 1), g, vw[i]); }
-#pragma unroll
-            for (int w = 0; w < HD / 32; ++w) {
-                uint32_t b0[4], b1[4];
-                pairs_of(vw[0][w], vw[1][w], b0);
-                pairs_of(vw[2][w], vw[3][w], b1);
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const uint32_t a[4] = {b0[2 * i], b0[2 * i + 1], b1[2 * i], b1[2 * i + 1]};
-#pragma unroll
-                    for (int n = 0; n < NT; ++n) { mma16816(o[n][2 * w + i], a, pf[n][0], pf[n][1]); }
-                }
-            }
-            stage = stage == STAGES - 1 ? 0 : stage + 1;
+            advance();
         }
-        cp_wait<0>();
-        __syncwarp();
-        // What is known of this item; the next one's copies start before its findings are joined, where these have a place of their own
-        const RowsDone what = {packed, tile, q.row0, head, q.from};
-        const PagedCut cut = paged_cut(at, at.unit - off, it.units);
-        at.unit += todo + p.start_units;
-        off = 0;
-        const bool more = at.unit < at.end && paged_next(p, true, q, seq, head, tile), early = what.rows <= Smem::EARLY;
-        if (more) { describe(); }
-        if (more && early) { start(); }
-        if (!early) { __syncthreads(); }
-        const int room = early ? Smem::EARLY : TILE;              // rows of a warp's findings
-        float *mo = reinterpret_cast<float *>(smem + (early ? Smem::RING : 0)), *mm = mo + PR_WARPS * room * HD, *ml = mm + PR_WARPS * room;
+        // This warp's findings (the next item's copies are on their way)
+        float *mo = reinterpret_cast<float *>(smem + Smem::FOUND), *mm = mo + PR_WARPS * ROWS * HD, *ml = mm + PR_WARPS * ROWS;
         const float f = 1.f / unit;
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const float l = over_groups(sum[n][e], false);
-                const int r = n * 8 + 2 * t + e;
-                if (r < what.rows) {
-                    float *dst = mo + (warp * room + r) * HD + g * (HD / 8);
+            for (int i = 0; i < 2; ++i) {
+                const float l = over_groups(sum[n][i], false);
+                const int r = n * 8 + 2 * t + i;
+                if (r < e.rows) {
+                    float *dst = mo + (warp * ROWS + r) * HD + g * (HD / 8);
 #pragma unroll
-                    for (int i = 0; i < HD / 16; i += 2) { *reinterpret_cast<float4 *>(dst + 2 * i) = make_float4(o[n][i][e] * f, o[n][i][2 + e] * f, o[n][i + 1][e] * f, o[n][i + 1][2 + e] * f); }
-                    if (g == 0) { mm[warp * room + r] = mx[n][e]; ml[warp * room + r] = l; }
+                    for (int k = 0; k < HD / 16; k += 2) { *reinterpret_cast<float4 *>(dst + 2 * k) = make_float4(o[n][k][i] * f, o[n][k][2 + i] * f, o[n][k + 1][i] * f, o[n][k + 1][2 + i] * f); }
+                    if (g == 0) { mm[warp * ROWS + r] = mx[n][i]; ml[warp * ROWS + r] = l; }
                 }
             }
         }
-        __syncthreads();
-        rows_finish<HD, TILE, PK_INT8>(p, cut, what, mo, mm, ml, room, last_one);
-        if (!more) { return; }
-        __syncthreads();                      // (the findings' place is free again)
-        if (!early) { start(); }
+        meet();
+        const RowsDone what = {e.rows, e.tile, e.row0, e.head, e.from};
+        rows_finish<HD, ROWS, PK_INT8, PR_WARPS>(p, PagedCut{e.c0, e.parts}, what, mo, mm, ml, ROWS, last_one, meet);
+        meet();                 // (the findings' place is free again)
     }
+    if (limit == 0 && lane == 0) { pf_report(error_flag, 7); }
 }
 
-template <int HD, int NT, bool IN_PAGE>
-cudaError_t launch_bytes_as(const PagedAttention &p, int sms, const LaunchCfg &cfg) {
+template <int HD, int NT, bool MAPS>
+cudaError_t launch_bytes_as(const PagedAttention &p, const CUtensorMap &k, const CUtensorMap &v, int box, int sms, const LaunchCfg &cfg, uint64_t wait_limit) {
     using Smem = BytesSmem<HD, NT>;
-    const cudaError_t err = allow_dynamic_smem(reinterpret_cast<const void *>(paged_bytes_kernel<HD, NT, IN_PAGE>), (size_t)Smem::BYTES);
+    const cudaError_t err = allow_dynamic_smem(reinterpret_cast<const void *>(paged_bytes_kernel<HD, NT, MAPS>), (size_t)Smem::BYTES);
     if (err != cudaSuccess) { return err; }
-    return launch_maybe_pdl(paged_bytes_kernel<HD, NT, IN_PAGE>, dim3(Smem::CTAS * sms), PR_WARPS * 32, (size_t)Smem::BYTES, cfg.stream, cfg.pdl, p);
+    return launch_maybe_pdl(paged_bytes_kernel<HD, NT, MAPS>, dim3(Smem::CTAS * sms), PB_THREADS, (size_t)Smem::BYTES, cfg.stream, cfg.pdl, p, k, v, box, cfg.error_flag, wait_limit);
 }
 template <int HD, int NT>
-cudaError_t launch_bytes(PagedAttention p, int sms, const LaunchCfg &cfg) {
+cudaError_t launch_bytes(PagedAttention p, int sms, const LaunchCfg &cfg, uint64_t wait_limit) {
     const int page = p.view.page_size;
     p.page_shift = -1; p.start_units = PA_START;
     for (int s = 0; s < 31; ++s) { if (page == 1 << s) { p.page_shift = s; } }
-    if constexpr (HD != 96) {
-        if (page % PR_BLOCK == 0) { return launch_bytes_as<HD, NT, true>(p, sms, cfg); }
+    CUtensorMap k = {}, v = {};
+    if constexpr (HD == 64 || HD == 128) {
+        const int box = page % 64 == 0 ? 64 : page % 32 == 0 ? 32 : 16;
+        if (page % 16 == 0 && paged_byte_map(&k, p.k, p.view, p.n_head_kv, HD, box) && paged_byte_map(&v, p.v, p.view, p.n_head_kv, HD, box)) { return launch_bytes_as<HD, NT, true>(p, k, v, box, sms, cfg, wait_limit); }
     }
-    return launch_bytes_as<HD, NT, false>(p, sms, cfg);
+    return launch_bytes_as<HD, NT, false>(p, k, v, 0, sms, cfg, wait_limit);
 }
 template <int NT>
-cudaError_t launch_bytes(const PagedAttention &p, int head_dim, int sms, const LaunchCfg &cfg) {
+cudaError_t launch_bytes(const PagedAttention &p, int head_dim, int sms, const LaunchCfg &cfg, uint64_t wait_limit) {
     switch (head_dim) {
-    case 32: return launch_bytes<32, NT>(p, sms, cfg);
-    case 64: return launch_bytes<64, NT>(p, sms, cfg);
-    case 96: return launch_bytes<96, NT>(p, sms, cfg);
-    case 128: return launch_bytes<128, NT>(p, sms, cfg);
+    case 32: return launch_bytes<32, NT>(p, sms, cfg, wait_limit);
+    case 64: return launch_bytes<64, NT>(p, sms, cfg, wait_limit);
+    case 96: return launch_bytes<96, NT>(p, sms, cfg, wait_limit);
+    case 128: return launch_bytes<128, NT>(p, sms, cfg, wait_limit);
     default: return cudaErrorInvalidValue;
     }
 }
 
 }  // namespace
 
-cudaError_t launch_paged_attention_bytes(const PagedAttention &p, int head_dim, int sms, const LaunchCfg &cfg) {
-    return p.tile_rows == 8 ? launch_bytes<1>(p, head_dim, sms, cfg) : p.tile_rows == 16 ? launch_bytes<2>(p, head_dim, sms, cfg) : launch_bytes<4>(p, head_dim, sms, cfg);
+cudaError_t launch_paged_attention_bytes(const PagedAttention &p, int head_dim, int sms, const LaunchCfg &cfg, uint64_t wait_limit) {
+    return p.tile_rows == 8 ? launch_bytes<1>(p, head_dim, sms, cfg, wait_limit) : p.tile_rows == 16 ? launch_bytes<2>(p, head_dim, sms, cfg, wait_limit) : launch_bytes<3>(p, head_dim, sms, cfg, wait_limit);
 }
 
 }  // namespace spyb

@@ -38,10 +38,10 @@ __device__ __forceinline__ float ex2(float x) { float y; asm("ex2.approx.ftz.f32
 __device__ __forceinline__ bool not_finite2(uint32_t h2) { return (h2 & 0x7c00u) == 0x7c00u || (h2 & 0x7c000000u) == 0x7c000000u; }
 
 struct RowsDone { int rows, tile, row0, head, from; };   // an item's rows that this tile holds, its tile, the sequence's first row, K/V head, and where its own positions begin
-// What the warps of a CTA found for an item ([warp][room][HD], maxima, sums), joined and put where it goes: to the output, or where other CTAs have pieces of the item to the workspace, and by the
+// What WARPS warps of a CTA found for an item ([warp][room][HD], maxima, sums), joined and put where it goes: to the output, or where other CTAs have pieces of the item to the workspace, and by the
 // last of these, in their order, to the output. All threads, behind a barrier.
-template <int HD, int TILE, int KIND>
-__device__ __forceinline__ void rows_finish(const PagedAttention &p, const PagedCut &cut, const RowsDone &what, const float *mo, const float *mm, const float *ml, int room, int &last_one) {
+template <int HD, int TILE, int KIND, int WARPS, class Meet>
+__device__ __forceinline__ void rows_finish(const PagedAttention &p, const PagedCut &cut, const RowsDone &what, const float *mo, const float *mm, const float *ml, int room, int &last_one, const Meet &meet) {
     constexpr int PART = TILE * (HD + 2), NT = PR_WARPS * 32;
     const int tid = threadIdx.x, done = what.rows;
     float *part = p.partial + paged_slot(blockIdx.x, cut.c0) * PART;
@@ -65,12 +65,12 @@ __device__ __forceinline__ void rows_finish(const PagedAttention &p, const Paged
         const int r = x / (HD / 4), c = (x - r * (HD / 4)) * 4;
         float m = -CUDART_INF_F;
 #pragma unroll
-        for (int w = 0; w < PR_WARPS; ++w) { m = fmaxf(m, mm[w * room + r]); }
+        for (int w = 0; w < WARPS; ++w) { m = fmaxf(m, mm[w * room + r]); }
         const float base = m == -CUDART_INF_F ? 0.f : m;
         float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
         float l = 0.f;
 #pragma unroll
-        for (int w = 0; w < PR_WARPS; ++w) {
+        for (int w = 0; w < WARPS; ++w) {
             const float f = ex2(mm[w * room + r] - base);
             const float4 u = *reinterpret_cast<const float4 *>(mo + (w * room + r) * HD + c);
             v.x += f * u.x; v.y += f * u.y; v.z += f * u.z; v.w += f * u.w;
@@ -83,14 +83,14 @@ __device__ __forceinline__ void rows_finish(const PagedAttention &p, const Paged
         }
     }
     if (cut.parts > 1) {
-        __syncthreads();
+        meet();
         if (tid == 0) {
             __threadfence();
             const unsigned n = atomicAdd(p.arrived + cut.c0, 1u);
             last_one = n == (unsigned)cut.parts - 1;
             if (last_one) { p.arrived[cut.c0] = 0; __threadfence(); }
         }
-        __syncthreads();
+        meet();
         if (last_one) {
             for (int x = tid; x < done * (HD / 4); x += NT) {
                 const int r = x / (HD / 4), c = (x - r * (HD / 4)) * 4;
@@ -415,7 +415,7 @@ __global__ void __launch_bounds__(PR_WARPS * 32) paged_rows_kernel(const __grid_
             }
         }
         __syncthreads();
-        rows_finish<HD, TILE, KIND>(p, cut, what, mo, mm, ml, room, last_one);
+        rows_finish<HD, TILE, KIND, PR_WARPS>(p, cut, what, mo, mm, ml, room, last_one, [] { __syncthreads(); });
         if (!more) { return; }
         __syncthreads();                      // (the findings' place is free again)
         if (!early) { start(); }

@@ -26,6 +26,7 @@
 
 #include "spyb_internal.h"
 #include "spyb_paged.cuh"
+#include "spyb_paged_maps.h"
 #include "spyb_tc.cuh"
 
 namespace spyb {
@@ -894,18 +895,19 @@ EncodeTiled encoder() {
     }();
     return fn;
 }
-bool tensor_map(CUtensorMap *map, const __half *data, int n, const cuuint64_t *dims, const cuuint64_t *strides, const cuuint32_t *box, bool bytes = false) {
+// (Bytes of a position are 128 or fewer: where positions lie apart, more than these would be another head's. Three of 100 000 by token, 8 heads: 121 us with 256, 115 with 128.)
+bool tensor_map(CUtensorMap *map, const __half *data, int n, const cuuint64_t *dims, const cuuint64_t *strides, const cuuint32_t *box, bool bytes = false, CUtensorMapSwizzle swizzle = CU_TENSOR_MAP_SWIZZLE_128B) {
     const cuuint32_t ones[4] = {1, 1, 1, 1};
     return encoder() != nullptr && encoder()(map, bytes ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, n, const_cast<__half *>(data), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                                             bytes ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+                                             swizzle, bytes ? CU_TENSOR_MAP_L2_PROMOTION_L2_128B : CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 // pages of one pool: [page][head][position][element] whatever the order of the strides; boxes of `box` positions x 64 elements, or x all bytes of a head
-bool page_map(CUtensorMap *map, const __half *pool, const PagedView &v, int heads, int head_dim, int box, bool bytes) {
+bool page_map(CUtensorMap *map, const __half *pool, const PagedView &v, int heads, int head_dim, int box, bool bytes, CUtensorMapSwizzle swizzle) {
     const cuuint64_t size = bytes ? 1 : 2;
     const cuuint64_t dims[4] = {(cuuint64_t)head_dim, (cuuint64_t)v.page_size, (cuuint64_t)heads, (cuuint64_t)v.n_pages};
     const cuuint64_t strides[3] = {(cuuint64_t)v.token_stride * size, (cuuint64_t)v.head_stride * size, (cuuint64_t)v.page_stride * size};
     const cuuint32_t boxes[4] = {bytes ? (cuuint32_t)head_dim : 64, (cuuint32_t)box, 1, 1};
-    return tensor_map(map, pool, 4, dims, strides, boxes, bytes);
+    return tensor_map(map, pool, 4, dims, strides, boxes, bytes, swizzle);
 }
 // Q: [row][head][element], boxes of whole tokens of a group of heads
 bool query_map(CUtensorMap *map, const PagedAttention &p, int n_head, int head_dim) {
@@ -938,6 +940,10 @@ cudaError_t launch_tc(const PagedAttention &p, int head_dim, const CUtensorMap &
 
 }  // namespace
 
+bool paged_byte_map(CUtensorMap *map, const void *pool, const PagedView &v, int heads, int head_dim, int box) {
+    const int64_t most = std::max({v.token_stride, v.head_stride, v.page_stride}), least = std::min({v.token_stride, v.head_stride, v.page_stride});
+    return least > 0 && most < (1ll << 38) && page_map(map, static_cast<const __half *>(pool), v, heads, head_dim, box, true, head_dim == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B);
+}
 static int paged_tc_box(int page_size) {   // positions of a box: the largest power of two up to 128 that divides the page size
     int box = 1;
     while (box < PT_KEYS && page_size % (2 * box) == 0) { box *= 2; }
@@ -954,7 +960,8 @@ bool launch_paged_attention_tc(const PagedAttention &given, int head_dim, int n_
     CUtensorMap q, k, v;
     const int kind = p.kind();
     const bool bytes = kind == PK_INT8;
-    if (!query_map(&q, p, n_head, head_dim) || !page_map(&k, p.k, p.view, p.n_head_kv, head_dim, box, bytes) || !page_map(&v, p.v, p.view, p.n_head_kv, head_dim, box, bytes)) { return false; }
+    const CUtensorMapSwizzle swizzle = bytes ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B;
+    if (!query_map(&q, p, n_head, head_dim) || !page_map(&k, p.k, p.view, p.n_head_kv, head_dim, box, bytes, swizzle) || !page_map(&v, p.v, p.view, p.n_head_kv, head_dim, box, bytes, swizzle)) { return false; }
     const auto launch = kind == PK_SHARED ? launch_tc<false, PK_SHARED> : bytes ? (p.late != PA_ON_TIME ? launch_tc<true, PK_INT8> : launch_tc<false, PK_INT8>)
                                           : p.late != PA_ON_TIME ? launch_tc<true, PK_PLAIN> : launch_tc<false, PK_PLAIN>;
     *err = launch(p, head_dim, q, k, v, box, sms, cfg, wait_limit);

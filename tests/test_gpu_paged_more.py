@@ -390,6 +390,8 @@ def test_bytes_short_and_empty(be, dev, rows, n_kv, hd):
 def test_bytes_windows(be, dev, window, rows, hd):
     rng = np.random.default_rng(window)
     check_attend(be, dev, rng, [rows, 1, rows], [700, 90, rows], 6, 2, hd, 16, window=window)
+    for page in (32, 64, 192):                               # (a window that begins in the middle of a page)
+        check_attend(be, dev, rng, [1, 2, 1, 1], [700, 590, 333, 64], 6, 2, hd, page, window=window)
 
 
 @pytest.mark.parametrize("hd", [32, 64, 96, 128])
