@@ -204,13 +204,12 @@ spyb_status check_load(Refusal &no, const spyb_paged_load_desc &d) {
     return SPYB_SUCCESS;
 }
 // What a call with groups keeps in its workspace: accumulators and statistics of the first pass, and who shares what
-struct SharedRoom { uint64_t out, stats, words, bytes; };
+struct SharedRoom { uint64_t out, stats, cuts, words, bytes; };
 SharedRoom shared_room(int64_t n_seq, int64_t n_rows, int64_t n_head, int64_t head_dim) {
     SharedRoom r;
     const uint64_t cells = (uint64_t)n_rows * n_head;
-    r.out = 0; r.stats = cells * head_dim * sizeof(float); r.words = r.stats + cells * sizeof(float2);
-    r.words = (r.words + 15) & ~15ull;
-    r.bytes = (r.words + 3 * (uint64_t)n_seq * sizeof(int32_t) + 15) & ~15ull;
+    r.out = 0; r.stats = cells * head_dim * sizeof(float); r.cuts = r.stats + cells * sizeof(float2); r.words = r.cuts + cells * sizeof(int2);
+    r.bytes = (r.words + 4 * (uint64_t)n_seq * sizeof(int32_t) + 15) & ~15ull;
     return r;
 }
 spyb_status check_attend(Refusal &no, const spyb_paged_attend_desc &d) {
@@ -350,15 +349,17 @@ static PagedAppend append_of(spyb_backend *be, const spyb_paged_append_desc &giv
     return p;
 }
 // One pass over pages: sequences of many rows on tensor memory, the others on the kernel for few
-static spyb_status attention_pass(spyb_backend *be, PagedAttention p, int head_dim, int n_head, int64_t most, uint64_t wait_limit) {
+static spyb_status attention_pass(spyb_backend *be, PagedAttention p, int head_dim, int n_head, int64_t most, uint64_t wait_limit, bool *on_tensor_memory = nullptr) {
     const LaunchCfg cfg = be->launch_cfg(be->config.use_pdl != 0);
     const bool bytes = p.kind() == PK_INT8;
     p.few_rows = 1 << 30;
     if (most > (bytes ? PB_FEW_ROWS : PA_FEW_ROWS) && p.scale_log2 >= 0.f) {
         cudaError_t err = cudaSuccess;
         // what single tokens beside the many rows have is the small kernel's in its narrowest tile
-        p.few_rows = p.view.n_seq == 1 ? 0 : !bytes ? PA_FEW_ROWS : p.group > PB_FEW_ROWS ? 0 : (p.group + 7) / 8 * 8;
-        if (!launch_paged_attention_tc(p, head_dim, n_head, be->num_sms_total, cfg, wait_limit, &err)) { p.few_rows = 1 << 30; }
+        p.few_rows = p.view.n_seq == 1 || p.stats != nullptr ? 0 : !bytes ? PA_FEW_ROWS : p.group > PB_FEW_ROWS ? 0 : (p.group + 7) / 8 * 8;
+        const bool taken = launch_paged_attention_tc(p, head_dim, n_head, be->num_sms_total, cfg, wait_limit, &err);
+        if (!taken) { p.few_rows = 1 << 30; }
+        if (on_tensor_memory != nullptr) { *on_tensor_memory = taken; }
         SPYB_CUDA(be, err);
     }
     if (p.few_rows == 0) { return SPYB_SUCCESS; }
@@ -393,13 +394,20 @@ static spyb_status paged_attention(spyb_backend *be, const spyb_paged_attention_
         uint8_t *const mem = static_cast<uint8_t *>(shared->workspace);
         PagedShared g;
         g.view = p.view; g.group_start = shared->group_start; g.n_shared = shared->n_shared; g.n_group = shared->n_group; g.causal = p.causal;
-        g.from = reinterpret_cast<int32_t *>(mem + room.words); g.row_end = g.from + d.batch.n_seq; g.kv = g.row_end + d.batch.n_seq;
+        g.from = reinterpret_cast<int32_t *>(mem + room.words); g.row_end = g.from + d.batch.n_seq; g.kv = g.row_end + d.batch.n_seq; g.lead = g.kv + d.batch.n_seq;
         SPYB_CUDA(be, launch_paged_shared(g, be->launch_cfg(be->config.use_pdl != 0)));
         PagedAttention first = p;
         first.view.row_end = g.row_end; first.view.n_kv = g.kv; first.causal = 0;
-        first.out = mem + room.out; first.out_f32 = 1; first.out_stride = (int64_t)d.n_head * hd; first.stats = reinterpret_cast<float2 *>(mem + room.stats);
-        const spyb_status st = attention_pass(be, first, hd, d.n_head, (int64_t)d.batch.n_rows * p.group, wait_limit);
+        first.out = mem + room.out; first.out_f32 = 1; first.out_stride = (int64_t)d.n_head * hd; first.stats = reinterpret_cast<float2 *>(mem + room.stats); first.cuts = reinterpret_cast<int2 *>(mem + room.cuts);
+        bool on_tensor_memory = false;
+        const spyb_status st = attention_pass(be, first, hd, d.n_head, (int64_t)d.batch.n_rows * p.group, wait_limit, &on_tensor_memory);
         if (st != SPYB_SUCCESS) { return st; }
+        if (on_tensor_memory) {
+            PagedSharedJoin j;
+            j.view = p.view; j.from = g.from; j.lead = g.lead; j.cuts = first.cuts; j.partial = be->paged_partial; j.out = static_cast<float *>(first.out); j.stats = first.stats;
+            j.n_head_kv = p.n_head_kv; j.group = p.group;
+            SPYB_CUDA(be, launch_paged_shared_join(j, hd, be->launch_cfg(be->config.use_pdl != 0)));
+        }
         p.view.from = g.from; p.with_stats = first.stats; p.with_out = static_cast<const float *>(first.out);
     }
     return attention_pass(be, p, hd, d.n_head, most, wait_limit);

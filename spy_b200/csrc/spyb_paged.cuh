@@ -44,6 +44,7 @@ struct PagedAttention {
     int          late = PA_ON_TIME;       // self-checks of the tensor-memory kernel
     PagedScales  scales;                  // of an 8-bit cache
     float2      *stats = nullptr;         // first pass of two, over what sequences share: every row's maximum and sum go here, its accumulators as they are to `out` (f32), both [row][head]
+    int2        *cuts = nullptr;          // of the first pass on tensor memory, by K/V head and first row of a tile: first CTA and number of CTAs of its item. Several leave their findings where they are
     const float2 *with_stats = nullptr;   // second pass: these are joined with what is found
     const float  *with_out = nullptr;
     __host__ __device__ int kind() const { return scales.pairs != nullptr ? PK_INT8 : stats != nullptr || with_stats != nullptr ? PK_SHARED : PK_PLAIN; }
@@ -67,13 +68,23 @@ struct PagedShared {                      // which sequences share what, and wha
     PagedView      view;
     const int32_t *group_start = nullptr, *n_shared = nullptr;
     int            n_group = 0, causal = 1;
-    int32_t       *from = nullptr, *row_end = nullptr, *kv = nullptr;   // [n_seq] each: where a sequence's own positions begin; rows and positions of the first pass's sequences
+    int32_t       *from = nullptr, *row_end = nullptr, *kv = nullptr, *lead = nullptr;   // [n_seq] each: where a sequence's own positions begin; rows and positions of the first pass's sequences; first row of the group
+};
+struct PagedSharedJoin {                  // cut items of the first pass on tensor memory
+    PagedView      view;
+    const int32_t *from = nullptr, *lead = nullptr;
+    const int2    *cuts = nullptr;
+    const float   *partial = nullptr;
+    float         *out = nullptr;
+    float2        *stats = nullptr;
+    int            n_head_kv = 0, group = 1;
 };
 constexpr int PA_SHARED = 128;            // what is shared is cut to a multiple of so many positions: both kernels' blocks begin at such ones
 int         paged_cut_selftest();   // host-only: 0 when the CTAs' pieces cover every item once, on any lengths
 cudaError_t launch_paged_store(const PagedStore &p, int in_type, int q_out_type, int sms, const LaunchCfg &cfg);
 cudaError_t launch_paged_load(const PagedLoad &p, int out_type, int sms, const LaunchCfg &cfg);
 cudaError_t launch_paged_shared(const PagedShared &p, const LaunchCfg &cfg);
+cudaError_t launch_paged_shared_join(const PagedSharedJoin &p, int head_dim, const LaunchCfg &cfg);
 cudaError_t launch_paged_append(const PagedAppend &p, int in_type, int q_out_type, int sms, const LaunchCfg &cfg);
 cudaError_t launch_paged_attention_rows(const PagedAttention &p, int head_dim, int row_tiles, int sms, const LaunchCfg &cfg);
 cudaError_t launch_paged_shared_rows(const PagedAttention &p, int head_dim, int row_tiles, int sms, const LaunchCfg &cfg);   // (PK_SHARED)

@@ -224,7 +224,58 @@ __global__ void __launch_bounds__(SH_WARPS * 32) paged_shared_kernel(const __gri
         p.from[s] = common;
         p.kv[s] = common;
         p.row_end[s] = s == leader && common > 0 ? p.view.row_start[group_end] : begin;
+        p.lead[s] = common > 0 ? p.view.row_start[leader] : begin;
     }
+}
+
+// A row of a query head a warp: the pieces of its tile that the first pass's CTAs left, joined in their order. (In the first pass itself one CTA would have to read them all, 18 pieces of 64 KB where 64 requests
+// share 6000 positions: 35 us of its 51.)
+constexpr int SJ_WARPS = 8, SJ_TILE = 128;    // (rows of a tile of the tensor-memory kernel)
+template <int HD>
+__global__ void __launch_bounds__(SJ_WARPS * 32) paged_shared_join_kernel(const __grid_constant__ PagedSharedJoin p) {
+    pdl_launch_dependents();
+    pdl_wait();
+    const int lane = threadIdx.x & 31, n_head = p.n_head_kv * p.group;
+    const int64_t cell = (int64_t)blockIdx.x * SJ_WARPS + (threadIdx.x >> 5);
+    const int row = (int)(cell / n_head), head = (int)(cell - (int64_t)row * n_head), kv = (int)((unsigned)head / (unsigned)p.group);
+    if (row >= p.view.n_rows) { return; }
+    const int s = sequence_of(p.view, row);
+    if (s < 0 || s >= p.view.n_seq || row >= p.view.row_end[s] || p.from[s] == 0) { return; }
+    const int lead = max(0, p.lead[s]), tokens = SJ_TILE / p.group, half = (int)((unsigned)(row - lead) / (unsigned)tokens), first = lead + half * tokens;
+    if (row < lead) { return; }                                     // (no group that makes sense)
+    const int2 cut = p.cuts[(int64_t)kv * p.view.n_rows + first];
+    if (cut.y < 2) { return; }
+    const int r = (row - first) * p.group + head - kv * p.group;
+    constexpr int PIECE = SJ_TILE * (HD + 2);
+    auto piece = [&](int i) { return p.partial + (paged_slot(cut.x + i, cut.x) * 2 + (half & 1)) * PIECE; };
+    float  m = -INFINITY, l = 0.f;
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+    for (int i0 = 0; i0 < cut.y; i0 += 8) {                         // eight pieces are in flight together; what came before is scaled to the new maximum
+        float  pm[8], pl[8], top = m;
+        float4 u[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const bool is = i0 + j < cut.y;
+            const float *from = piece(is ? i0 + j : 0);
+            pm[j] = is ? __ldcg(from + SJ_TILE * HD + r) : -INFINITY;
+            pl[j] = is ? __ldcg(from + SJ_TILE * HD + SJ_TILE + r) : 0.f;
+            u[j] = is && lane < HD / 4 ? __ldcg(reinterpret_cast<const float4 *>(from) + lane * SJ_TILE + r) : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) { top = fmaxf(top, pm[j]); }
+        const float base = top == -INFINITY ? 0.f : top, before = exp2f(m - base);
+        m = top; l *= before;
+        v = make_float4(v.x * before, v.y * before, v.z * before, v.w * before);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const float f = exp2f(pm[j] - base);
+            v.x += f * u[j].x; v.y += f * u[j].y; v.z += f * u[j].z; v.w += f * u[j].w;
+            l += f * pl[j];
+        }
+    }
+    if (lane < HD / 4) { reinterpret_cast<float4 *>(p.out + cell * HD)[lane] = v; }
+    if (lane == 0) { p.stats[cell] = make_float2(m, l); }
 }
 
 template <class TIn, class TQ, bool EIGHT>
@@ -257,6 +308,10 @@ cudaError_t launch_paged_load(const PagedLoad &p, int out_type, int, const Launc
 }
 cudaError_t launch_paged_shared(const PagedShared &p, const LaunchCfg &cfg) {
     return launch_maybe_pdl(paged_shared_kernel, dim3((p.view.n_seq + SH_WARPS - 1) / SH_WARPS), SH_WARPS * 32, 0, cfg.stream, cfg.pdl, p);
+}
+cudaError_t launch_paged_shared_join(const PagedSharedJoin &p, int head_dim, const LaunchCfg &cfg) {
+    const int64_t cells = (int64_t)p.view.n_rows * p.n_head_kv * p.group;
+    return launch_maybe_pdl(head_dim == 128 ? paged_shared_join_kernel<128> : paged_shared_join_kernel<64>, dim3((unsigned)((cells + SJ_WARPS - 1) / SJ_WARPS)), SJ_WARPS * 32, 0, cfg.stream, cfg.pdl, p);
 }
 cudaError_t launch_paged_shared_rows(const PagedAttention &p, int head_dim, int row_tiles, int sms, const LaunchCfg &cfg) { return launch_rows_kind<PK_SHARED>(p, head_dim, row_tiles, sms, cfg); }
 

@@ -477,6 +477,10 @@ __global__ void __launch_bounds__(TcShape<HD, KIND>::THREADS, 1) paged_tc_kernel
             if (parts > 1 && own.rows > 0) {
                 float *stats = reinterpret_cast<float *>(part + PT_ROWS * HD / 4);
                 stats[row] = m; stats[PT_ROWS + row] = l;
+            }
+            if (KIND != PK_PLAIN && p.cuts != nullptr) {      // (joined by the next kernel, by all SMs: an item's rows are few and its CTAs many)
+                if (row == 0 && own.rows > 0 && (whole_item || c0 == (int)blockIdx.x)) { p.cuts[(int64_t)en.head * p.view.n_rows + en.row0 + (2 * en.tile + t) * half_tokens] = make_int2(c0, parts); }
+            } else if (parts > 1 && own.rows > 0) {
                 __threadfence();
                 all_of_tile();
                 if (row == 0) {

@@ -91,9 +91,9 @@ def test_the_fp16_operators_take_no_bytes():
 
 
 def test_room_for_two_passes():
-    """Accumulators, two statistics a row and head, three words a sequence; nothing where a size makes no sense."""
+    """Accumulators, two statistics and two words of who has them a row and head, four words a sequence; nothing where a size makes no sense."""
     n = B.paged_attend_workspace(3, 7, 4, 64)
-    assert 7 * 4 * (64 * 4 + 8) + 3 * 3 * 4 <= n <= 7 * 4 * (64 * 4 + 8) + 3 * 3 * 4 + 32
+    assert 7 * 4 * (64 * 4 + 16) + 4 * 3 * 4 <= n <= 7 * 4 * (64 * 4 + 16) + 4 * 3 * 4 + 32
     assert B.paged_attend_workspace(-1, 7, 4, 64) == B.paged_attend_workspace(1, 1 << 24, 4, 64) == B.paged_attend_workspace(1, 7, -4, 64) == 0
     assert B.paged_attend_workspace(1, (1 << 24) - 1, 128, 128) > 1 << 40
 
