@@ -10,149 +10,167 @@
 namespace spyb {
 namespace {
 
-// ---------------------------------------------------------------------------------------------- store
-// Memory bound, as append: an element is read once (4 or 2 bytes) and written once (2, or 1 and a 64th of a scale). A CTA has one row; a head's threads, eight elements each, lie side by side in
-// a warp (as many as the next power of two), so that the mean of squares and the largest magnitude are shuffles. An element is rounded once: norm, rotation and scale are f32, angles 64 bits.
-constexpr int ST_THREADS = 256;
+struct RowPlace { int64_t cell, pair; int pos; bool mine; };        // of a row: where its position lies (cell -1: not there) and its scales; mine: a sequence's
+__device__ __forceinline__ RowPlace row_place(const PagedView &v, const PagedScales &scales, int row) {   // by one thread
+    RowPlace a = {-1, 0, -1, false};
+    if (row >= v.n_rows) { return a; }
+    int q = -1, n = v.n_seq + 1;                                    // the last one that begins at the row or in front of it
+    for (int lo = 0; n > 0;) {
+        const int half = n / 2;
+        if (v.row_start[lo + half] <= row) { q = lo + half; lo += half + 1; n -= half + 1; } else { n = half; }
+    }
+    if (q < 0 || q >= v.n_seq) { return a; }
+    const int end = v.row_start[q + 1];
+    a.pos = v.n_kv[q] - end + row; a.mine = row < end;
+    if (a.mine && a.pos >= 0 && a.pos < v.n_kv_most) {
+        const int page = v.page_table[(int64_t)q * v.table_stride + a.pos / v.page_size], at = a.pos % v.page_size;
+        if (page >= 0 && page < v.n_pages) { a.cell = page * v.page_stride + at * v.token_stride; a.pair = page * scales.page_stride + at * scales.token_stride; }
+    }
+    return a;
+}
+__device__ __forceinline__ void store8(float *p, const float *v) { store4(p, v); store4(p + 4, v + 4); }
+__device__ __forceinline__ void store8(__half *p, const float *v) { *reinterpret_cast<uint4 *>(p) = make_uint4(pack2(v[0], v[1]), pack2(v[2], v[3]), pack2(v[4], v[5]), pack2(v[6], v[7])); }
 
-template <class TIn, class TQ, bool EIGHT, bool AHEAD>
-__global__ void __launch_bounds__(ST_THREADS) paged_store_kernel(const __grid_constant__ PagedStore s, const int width) {
+// ---------------------------------------------------------------------------------------------- store
+// An element is read once (4 or 2 bytes) and written once (2, or 1 and a 64th of a scale); beside that the instructions count, some 100 for eight elements, so all that can be done once is: a CTA has up to
+// ST_ROWS rows, whose places a lane each finds; their cosines and sines are made a pair a thread and go through shared memory; a thread has eight elements of a head in all of these rows, so that kinds of heads, weights and
+// addresses are found once a head. A head's threads lie side by side in a warp (as many as the next power of two): the mean of squares and the largest magnitude are shuffles.
+// An element is rounded once: norm, rotation and scale are f32, angles 64 bits.
+constexpr int ST_THREADS = 256, ST_ROWS = 8;
+struct StorePlace { int pos; int64_t cell, pair; };                 // pos -1: nobody's row, or one in front of position 0; cell -1: its page is not there
+__device__ __forceinline__ float larger(float a, float b) { float r; asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b)); return r; }
+__device__ __forceinline__ float one_over(float x) { float r; asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x)); return r; }   // (off by a step at most)
+
+template <class TIn, class TQ, bool EIGHT, bool HALVES>
+__global__ void __launch_bounds__(ST_THREADS, 4) paged_store_kernel(const __grid_constant__ PagedStore s, const int width, const int rows_each) {
     const PagedAppend &p = s.append;
+    __shared__ __align__(16) float2 turn[ST_ROWS][128];             // cosine and sine of a pair
+    __shared__ StorePlace places[ST_ROWS];
     pdl_launch_dependents();
     pdl_wait();
-    const int row = blockIdx.x;
+    const int row0 = blockIdx.x * rows_each, rows = min(rows_each, p.view.n_rows - row0);
     const int per = p.head_dim / 8, slots = ST_THREADS / width;     // threads of a head that have elements, heads at a time
-    const int slot = threadIdx.x / width, item = threadIdx.x & (width - 1), total = p.n_head + 2 * p.n_head_kv;
+    const int slot = threadIdx.x / width, item = threadIdx.x & (width - 1), total = p.n_head + 2 * p.n_head_kv, keys_end = p.n_head + p.n_head_kv;
     const bool turned = item < p.rot / 8;
-    const int  e0 = turned && p.halves ? 4 * item : 8 * item, e1 = turned && p.halves ? e0 + p.rot / 2 : e0 + 4;
-    const int  step = slots * gridDim.y;
-    auto fetch = [&](int head, float (&x)[8]) {
-        const bool is_q = head < p.n_head, is_k = !is_q && head < p.n_head + p.n_head_kv;
-        const int  hh = is_q ? head : is_k ? head - p.n_head : head - p.n_head - p.n_head_kv;
-        const TIn *src = static_cast<const TIn *>(is_q ? p.q : is_k ? p.k : p.v) + row * (is_q ? p.q_stride : is_k ? p.k_stride : p.v_stride) + (int64_t)hh * p.head_dim;
-        load4(src + e0, x);
-        load4(src + e1, x + 4);
+    const int  e0 = HALVES && turned ? 4 * item : 8 * item, e1 = HALVES && turned ? e0 + p.rot / 2 : e0 + 4;
+    struct Head { const TIn *src; int64_t stride; bool is_q, is_k, mine; int hh; };
+    auto head_of = [&](int h) {
+        Head a;
+        a.is_q = h < p.n_head; a.is_k = !a.is_q && h < keys_end; a.mine = item < per && h < total;
+        a.hh = a.is_q ? h : a.is_k ? h - p.n_head : h - keys_end;
+        a.stride = a.is_q ? p.q_stride : a.is_k ? p.k_stride : p.v_stride;
+        a.src = static_cast<const TIn *>(a.is_q ? p.q : a.is_k ? p.k : p.v) + row0 * a.stride + (int64_t)a.hh * p.head_dim;
+        return a;
     };
-    auto works = [&](int h) { return item < per && h < total; };
-    // (the first head's elements are on their way while the row's place is found)
-    int   h0 = blockIdx.y * slots;                                  // (the same for all threads: they meet in shuffles)
-    float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, q_weight[8], k_weight[8];
-    if (works(h0 + slot)) { fetch(h0 + slot, x); }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) { q_weight[i] = k_weight[i] = 1.f; }
-    if (item < per && s.q_norm != nullptr) { load4(s.q_norm + e0, q_weight); load4(s.q_norm + e1, q_weight + 4); }
-    if (item < per && s.k_norm != nullptr) { load4(s.k_norm + e0, k_weight); load4(s.k_norm + e1, k_weight + 4); }
-    const int q = sequence_of(p.view, row);
-    if (q < 0 || q >= p.view.n_seq) { return; }
-    const int end = p.view.row_start[q + 1];
-    const int pos = p.view.n_kv[q] - end + row;
-    if (row >= end || pos < 0) { return; }
-    int64_t cell = -1, pair = 0;
-    if (pos < p.view.n_kv_most) {
-        const int page = p.view.page_table[(int64_t)q * p.view.table_stride + pos / p.view.page_size], at = pos % p.view.page_size;
-        if (page >= 0 && page < p.view.n_pages) {
-            cell = page * p.view.page_stride + at * p.view.token_stride;
-            pair = page * s.scales.page_stride + at * s.scales.token_stride;
-        }
+    auto fetch = [&](const Head &a, int r, float (&x)[8]) {
+        if (a.mine && r < rows) { load4(a.src + r * a.stride + e0, x); load4(a.src + r * a.stride + e1, x + 4); }
+    };
+    // (the first head's elements are on their way while the rows' places are found)
+    int  h0 = blockIdx.y * slots;                                   // (the same for all threads: they meet in shuffles)
+    Head head = head_of(h0 + slot);
+    float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    fetch(head, 0, x);
+    if (threadIdx.x < rows) {
+        const RowPlace at = row_place(p.view, s.scales, row0 + threadIdx.x);
+        places[threadIdx.x] = {at.mine ? at.pos : -1, at.cell, at.pair};
     }
-    float co[4], si[4];
-    if (turned) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const double t = (double)pos * p.turns[4 * item + i];
-            sincospif(2.0f * (float)(t - rint(t)), &si[i], &co[i]);
-        }
+    __syncthreads();
+    for (int i = threadIdx.x; i < rows * (p.rot / 2); i += ST_THREADS) {
+        const int r = i / (p.rot / 2), k = i - r * (p.rot / 2);
+        const double t = (double)places[r].pos * p.turns[k];
+        sincospif(2.0f * (float)(t - rint(t)), &turn[r][k].y, &turn[r][k].x);
     }
+    __syncthreads();
     const float mean = 1.f / (float)p.head_dim;
     for (;;) {
-        const int  h = h0 + slot, next = h0 + step;
-        const bool is_q = h < p.n_head, is_k = !is_q && h < p.n_head + p.n_head_kv, mine = works(h);
-        const int  hh = is_q ? h : is_k ? h - p.n_head : h - p.n_head - p.n_head_kv;
-        float ahead[8];
-        if (AHEAD && works(next + slot)) { fetch(next + slot, ahead); }
-        if (is_q ? s.q_norm != nullptr : is_k && s.k_norm != nullptr) {
-            float sum = 0.f;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) { sum = fmaf(x[i], x[i], sum); }
-            const unsigned all = width == 32 ? 0xffffffffu : ((1u << width) - 1) << (threadIdx.x & 31 & ~(width - 1));   // a head's threads: others may have another kind of head
-            for (int o = width / 2; o > 0; o >>= 1) { sum += __shfl_xor_sync(all, sum, o); }
-            const float f = rsqrtf(fmaf(sum, mean, s.eps));
-#pragma unroll
-            for (int i = 0; i < 8; ++i) { x[i] = x[i] * f * (is_q ? q_weight[i] : k_weight[i]); }
+        const float *weight = head.is_q ? s.q_norm : head.is_k ? s.k_norm : nullptr;
+        const bool some_norm = (h0 < p.n_head && s.q_norm != nullptr) || (h0 < keys_end && h0 + slots > p.n_head && s.k_norm != nullptr), some_cache = h0 + slots > p.n_head;   // of the CTA's heads
+        float w[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        if (weight != nullptr && head.mine) {
+            const float4 a = __ldg(reinterpret_cast<const float4 *>(weight + e0)), c = __ldg(reinterpret_cast<const float4 *>(weight + e1));
+            w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w; w[4] = c.x; w[5] = c.y; w[6] = c.z; w[7] = c.w;
         }
-        if (turned && (is_q || is_k)) {
+        const int64_t to = head.is_q ? (int64_t)row0 * p.q_out_stride + (int64_t)head.hh * p.head_dim : head.hh * p.view.head_stride;
+        for (int r = 0; r < rows; ++r) {
+            float ahead[8];
+            fetch(head, r + 1, ahead);
+            const StorePlace at = places[r];
+            if (some_norm) {
+                float sum = 0.f;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int a = p.halves ? i : 2 * i, b = p.halves ? i + 4 : 2 * i + 1;
-                const float u = x[a], w = x[b];
-                x[a] = u * co[i] - w * si[i];
-                x[b] = u * si[i] + w * co[i];
-            }
-        }
-        if (is_q) {
-            if (mine) {
-                TQ *dst = static_cast<TQ *>(p.q_out) + row * p.q_out_stride + (int64_t)hh * p.head_dim;
-                store4(dst + e0, x); store4(dst + e1, x + 4);
-            }
-        } else if constexpr (EIGHT) {
-            uint32_t most = 0;                                      // (as bits: NaN is above everything)
+                for (int i = 0; i < 8; ++i) { sum = fmaf(x[i], x[i], sum); }
 #pragma unroll
-            for (int i = 0; i < 8; ++i) { most = max(most, __float_as_uint(x[i]) & 0x7fffffffu); }
-            const unsigned all = width == 32 ? 0xffffffffu : ((1u << width) - 1) << (threadIdx.x & 31 & ~(width - 1));
-            for (int o = width / 2; o > 0; o >>= 1) { most = max(most, __shfl_xor_sync(all, most, o)); }
-            const bool   fine = most <= __float_as_uint(65468.f);
-            const __half scale = fine ? __float2half_ru(__fdiv_rn(__uint_as_float(most), 127.f)) : __ushort_as_half(0x7fff);
-            if (mine && cell >= 0) {
-                const float per_one = fine && most > 0 ? 1.f / __half2float(scale) : 0.f;
-                uint8_t *dst = (is_k ? s.k8 : s.v8) + cell + hh * p.view.head_stride;
-                uint32_t b[8];
+                for (int o = 16; o > 0; o >>= 1) { if (o < width) { sum += __shfl_xor_sync(0xffffffffu, sum, o); } }
+                if (weight != nullptr) {
+                    const float f = rsqrtf(fmaf(sum, mean, s.eps));
 #pragma unroll
-                for (int i = 0; i < 8; ++i) { b[i] = fine ? __float_as_uint(fmaf(x[i], per_one, 12582912.f)) : 0u; }   // (1.5 x 2^23: the integer is the low byte)
-                *reinterpret_cast<uint32_t *>(dst + e0) = __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
-                *reinterpret_cast<uint32_t *>(dst + e1) = __byte_perm(__byte_perm(b[4], b[5], 0x0040), __byte_perm(b[6], b[7], 0x0040), 0x5410);
-                if (item == 0) { reinterpret_cast<__half *>(const_cast<uint32_t *>(s.scales.pairs))[2 * (pair + hh * s.scales.head_stride) + (is_k ? 0 : 1)] = scale; }
+                    for (int i = 0; i < 8; ++i) { x[i] = x[i] * f * w[i]; }
+                }
             }
-        } else if (mine && cell >= 0) {
-            __half *dst = (is_k ? p.k_cache : p.v_cache) + cell + hh * p.view.head_stride;
-            store4(dst + e0, x); store4(dst + e1, x + 4);
-        }
-        if (next >= total) { break; }
-        h0 = next;
-        if (AHEAD) {
+            if (turned && (head.is_q || head.is_k)) {
+                const float4 c0 = *reinterpret_cast<const float4 *>(&turn[r][4 * item]), c1 = *reinterpret_cast<const float4 *>(&turn[r][4 * item + 2]);
+                const float co[4] = {c0.x, c0.z, c1.x, c1.z}, si[4] = {c0.y, c0.w, c1.y, c1.w};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    constexpr int STEP = HALVES ? 1 : 2, SECOND = HALVES ? 4 : 1;
+                    const float u = x[STEP * i], v = x[STEP * i + SECOND];
+                    x[STEP * i] = u * co[i] - v * si[i];
+                    x[STEP * i + SECOND] = u * si[i] + v * co[i];
+                }
+            }
+            float most = 0.f;
+            if (EIGHT && some_cache) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) { most = larger(most, fabsf(x[i])); }
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) { if (o < width) { most = larger(most, __shfl_xor_sync(0xffffffffu, most, o)); } }
+            }
+            if (head.is_q) {
+                if (head.mine && at.pos >= 0) {
+                    TQ *dst = static_cast<TQ *>(p.q_out) + r * p.q_out_stride + to;
+                    store4(dst + e0, x); store4(dst + e1, x + 4);
+                }
+            } else if (head.mine && at.pos >= 0 && at.cell >= 0) {
+                if constexpr (EIGHT) {
+                    const bool   fine = most <= 65468.f;
+                    const __half scale = fine ? __float2half_ru(__fdiv_rn(most, 127.f)) : __ushort_as_half(0x7fff);
+                    const float  per_one = fine && most > 0.f ? one_over(__half2float(scale)) : 0.f;
+                    uint8_t *dst = (head.is_k ? s.k8 : s.v8) + at.cell + to;
+                    uint32_t b[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) { b[i] = __float_as_uint(fmaf(x[i], per_one, 12582912.f)); }   // (1.5 x 2^23: the integer is the low byte. Beside a scale that is NaN the bytes are any)
+                    *reinterpret_cast<uint32_t *>(dst + e0) = __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
+                    *reinterpret_cast<uint32_t *>(dst + e1) = __byte_perm(__byte_perm(b[4], b[5], 0x0040), __byte_perm(b[6], b[7], 0x0040), 0x5410);
+                    if (item == 0) { reinterpret_cast<__half *>(const_cast<uint32_t *>(s.scales.pairs))[2 * (at.pair + head.hh * s.scales.head_stride) + (head.is_k ? 0 : 1)] = scale; }
+                } else {
+                    __half *dst = (head.is_k ? p.k_cache : p.v_cache) + at.cell + to;
+                    store4(dst + e0, x); store4(dst + e1, x + 4);
+                }
+            }
 #pragma unroll
             for (int i = 0; i < 8; ++i) { x[i] = ahead[i]; }
-        } else if (works(h0 + slot)) { fetch(h0 + slot, x); }
+        }
+        h0 += slots * gridDim.y;
+        if (h0 >= total) { break; }
+        head = head_of(h0 + slot);
+        fetch(head, 0, x);
     }
 }
 
 // ---------------------------------------------------------------------------------------------- load
-// Memory bound: a byte (or two) read and two (or four) written an element. A CTA has eight rows, whose places its warps find, one each; a thread has eight elements of one head in all of them.
-constexpr int LD_THREADS = 256, LD_ROWS = 8;
+// Memory bound: a byte (or two) read and two (or four) written an element. A CTA has 32 rows, whose places the lanes of its first warp find, one each (four dependent loads, which as many rows share); a thread
+// has eight elements of one head in all of them.
+constexpr int LD_THREADS = 256;
 
-template <class T, bool EIGHT>
+template <class T, bool EIGHT, int LD_ROWS>
 __global__ void __launch_bounds__(LD_THREADS) paged_load_kernel(const __grid_constant__ PagedLoad p) {
     __shared__ int64_t cells[LD_ROWS], pairs[LD_ROWS];             // -1: nothing there; -2: nobody's row
     pdl_launch_dependents();
     pdl_wait();
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, row0 = blockIdx.x * LD_ROWS;
-    {
-        const int row = row0 + warp;
-        int64_t cell = -2, pair = 0;
-        const int q = row < p.view.n_rows ? sequence_of(p.view, row) : -1;
-        if (q >= 0 && q < p.view.n_seq) {
-            const int end = p.view.row_start[q + 1], pos = p.view.n_kv[q] - end + row;
-            if (row < end) {
-                cell = -1;
-                if (pos >= 0 && pos < p.view.n_kv_most) {
-                    const int page = p.view.page_table[(int64_t)q * p.view.table_stride + pos / p.view.page_size], at = pos % p.view.page_size;
-                    if (page >= 0 && page < p.view.n_pages) {
-                        cell = page * p.view.page_stride + at * p.view.token_stride;
-                        pair = page * p.scales.page_stride + at * p.scales.token_stride;
-                    }
-                }
-            }
-        }
-        if (lane == 0) { cells[warp] = cell; pairs[warp] = pair; }
+    const int row0 = blockIdx.x * LD_ROWS;
+    if (threadIdx.x < LD_ROWS) {
+        const RowPlace at = row_place(p.view, p.scales, row0 + threadIdx.x);
+        cells[threadIdx.x] = at.mine ? at.cell : -2; pairs[threadIdx.x] = at.pair;
     }
     __syncthreads();
     const int per = p.head_dim / 8, each = p.n_head_kv * per, first = p.k_out != nullptr ? 0 : each, items = (p.v_out != nullptr ? 2 * each : each) - first;
@@ -163,25 +181,40 @@ __global__ void __launch_bounds__(LD_THREADS) paged_load_kernel(const __grid_con
         const int64_t in = head * p.view.head_stride + e, out = head * p.head_dim + e, stride = is_v ? p.v_stride : p.k_stride;
         T *dst = static_cast<T *>(is_v ? p.v_out : p.k_out) + (int64_t)row0 * stride + out;
         const int64_t of_pair = head * p.scales.head_stride;
-#pragma unroll 4
-        for (int r = sub; r < LD_ROWS; r += rows_at_once) {
-            const int64_t cell = cells[r];
-            float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-            if (cell >= 0) {
-                if constexpr (EIGHT) {
-                    const uint2 w = __ldcs(reinterpret_cast<const uint2 *>(static_cast<const uint8_t *>(is_v ? p.v : p.k) + cell + in));
-                    const float2 s = half2_bits(p.scales.pairs[pairs[r] + of_pair]);
-                    const float scale = is_v ? s.y : s.x;
-                    uint32_t h[4];
-                    halves_of(w.x, h[0], h[1]); halves_of(w.y, h[2], h[3]);
+        constexpr int TOGETHER = 4;                                 // rows whose bytes are on their way at a time
+        for (int r0 = sub; r0 < LD_ROWS; r0 += TOGETHER * rows_at_once) {
+            uint4    w[TOGETHER];
+            uint32_t pair[TOGETHER];
+            int64_t  cell[TOGETHER];
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) { const float2 u = half2_bits(h[k]); x[2 * k] = u.x * scale; x[2 * k + 1] = u.y * scale; }
-                } else {
-                    const __half *src = static_cast<const __half *>(is_v ? p.v : p.k) + cell + in;
-                    load4(src, x); load4(src + 4, x + 4);
+            for (int k = 0; k < TOGETHER; ++k) {
+                const int r = r0 + k * rows_at_once;
+                cell[k] = r < LD_ROWS ? cells[r] : -2;
+                if (cell[k] >= 0) {
+                    if constexpr (EIGHT) {
+                        const uint2 y = __ldcs(reinterpret_cast<const uint2 *>(static_cast<const uint8_t *>(is_v ? p.v : p.k) + cell[k] + in));
+                        w[k].x = y.x; w[k].y = y.y;
+                        pair[k] = __ldg(p.scales.pairs + pairs[r] + of_pair);
+                    } else { w[k] = __ldcs(reinterpret_cast<const uint4 *>(static_cast<const __half *>(is_v ? p.v : p.k) + cell[k] + in)); }
                 }
             }
-            if (cell != -2) { store4(dst + r * stride, x); store4(dst + r * stride + 4, x + 4); }
+#pragma unroll
+            for (int k = 0; k < TOGETHER; ++k) {
+                const int r = r0 + k * rows_at_once;
+                float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+                if (cell[k] >= 0) {
+                    uint32_t h[4] = {w[k].x, w[k].y, w[k].z, w[k].w};
+                    float scale = 1.f;
+                    if constexpr (EIGHT) {
+                        const float2 s = half2_bits(pair[k]);
+                        scale = is_v ? s.y : s.x;
+                        halves_of(w[k].x, h[0], h[1]); halves_of(w[k].y, h[2], h[3]);
+                    }
+#pragma unroll
+                    for (int i4 = 0; i4 < 4; ++i4) { const float2 u = half2_bits(h[i4]); x[2 * i4] = EIGHT ? u.x * scale : u.x; x[2 * i4 + 1] = EIGHT ? u.y * scale : u.y; }
+                }
+                if (cell[k] != -2) { store8(dst + r * stride, x); }
+            }
         }
     }
 }
@@ -278,16 +311,21 @@ __global__ void __launch_bounds__(SJ_WARPS * 32) paged_shared_join_kernel(const 
     if (lane == 0) { p.stats[cell] = make_float2(m, l); }
 }
 
+template <int ROWS>
+cudaError_t launch_load(const PagedLoad &p, int out_type, const LaunchCfg &cfg) {
+    const auto kernel = p.scales.pairs != nullptr ? (out_type == SPYB_FP32 ? paged_load_kernel<float, true, ROWS> : paged_load_kernel<__half, true, ROWS>)
+                                                  : out_type == SPYB_FP32 ? paged_load_kernel<float, false, ROWS> : paged_load_kernel<__half, false, ROWS>;
+    return launch_maybe_pdl(kernel, dim3((p.view.n_rows + ROWS - 1) / ROWS), LD_THREADS, 0, cfg.stream, cfg.pdl, p);
+}
 template <class TIn, class TQ, bool EIGHT>
 cudaError_t launch_store(const PagedStore &p, int sms, const LaunchCfg &cfg) {
     int width = 1;
     while (width < p.append.head_dim / 8) { width *= 2; }
     const int total = p.append.n_head + 2 * p.append.n_head_kv, slots = ST_THREADS / width, loops = (total + slots - 1) / slots;
-    // few rows: a row's heads are spread over CTAs
-    const int  split = std::max(1, std::min(loops, 2 * sms / std::max(1, p.append.view.n_rows)));
-    const dim3 grid(p.append.view.n_rows, split);
-    return (int64_t)p.append.view.n_rows * split <= 4 * sms ? launch_maybe_pdl(paged_store_kernel<TIn, TQ, EIGHT, true>, grid, ST_THREADS, 0, cfg.stream, cfg.pdl, p, width)
-                                                            : launch_maybe_pdl(paged_store_kernel<TIn, TQ, EIGHT, false>, grid, ST_THREADS, 0, cfg.stream, cfg.pdl, p, width);
+    // few rows: a row's heads are spread over CTAs; many: several rows a CTA, as long as there are CTAs for four an SM
+    const int n_rows = p.append.view.n_rows, each = std::max(1, std::min(ST_ROWS, n_rows / (4 * sms))), split = std::max(1, std::min(loops, 2 * sms / std::max(1, n_rows)));
+    const auto kernel = p.append.halves ? paged_store_kernel<TIn, TQ, EIGHT, true> : paged_store_kernel<TIn, TQ, EIGHT, false>;
+    return launch_maybe_pdl(kernel, dim3((n_rows + each - 1) / each, split), ST_THREADS, 0, cfg.stream, cfg.pdl, p, width, each);
 }
 template <class TIn, class TQ>
 cudaError_t launch_store(const PagedStore &p, int sms, const LaunchCfg &cfg) {
@@ -300,11 +338,9 @@ cudaError_t launch_paged_store(const PagedStore &p, int in_type, int q_out_type,
     if (in_type == SPYB_FP32) { return q_out_type == SPYB_FP32 ? launch_store<float, float>(p, sms, cfg) : launch_store<float, __half>(p, sms, cfg); }
     return q_out_type == SPYB_FP32 ? launch_store<__half, float>(p, sms, cfg) : launch_store<__half, __half>(p, sms, cfg);
 }
-cudaError_t launch_paged_load(const PagedLoad &p, int out_type, int, const LaunchCfg &cfg) {
-    const dim3 grid((p.view.n_rows + LD_ROWS - 1) / LD_ROWS);
-    const auto kernel = p.scales.pairs != nullptr ? (out_type == SPYB_FP32 ? paged_load_kernel<float, true> : paged_load_kernel<__half, true>)
-                                                  : out_type == SPYB_FP32 ? paged_load_kernel<float, false> : paged_load_kernel<__half, false>;
-    return launch_maybe_pdl(kernel, grid, LD_THREADS, 0, cfg.stream, cfg.pdl, p);
+cudaError_t launch_paged_load(const PagedLoad &p, int out_type, int sms, const LaunchCfg &cfg) {
+    // (few rows: on as many CTAs as there are, 1 of 300: 5.2 us with eight rows each, 8.6 with 32)
+    return p.view.n_rows >= 32 * 4 * sms ? launch_load<32>(p, out_type, cfg) : launch_load<8>(p, out_type, cfg);
 }
 cudaError_t launch_paged_shared(const PagedShared &p, const LaunchCfg &cfg) {
     return launch_maybe_pdl(paged_shared_kernel, dim3((p.view.n_seq + SH_WARPS - 1) / SH_WARPS), SH_WARPS * 32, 0, cfg.stream, cfg.pdl, p);
