@@ -85,10 +85,17 @@ __device__ __forceinline__ void rows_finish(const PagedAttention &p, const Paged
     if (cut.parts > 1) {
         meet();
         if (tid == 0) {
-            __threadfence();
-            const unsigned n = atomicAdd(p.arrived + cut.c0, 1u);
-            last_one = n == (unsigned)cut.parts - 1;
-            if (last_one) { p.arrived[cut.c0] = 0; __threadfence(); }
+            if (KIND == PK_INT8) {            // (one instruction orders what the CTA wrote before it and what the last one reads after it; 64 single tokens of up to 4096 positions: 59.7 us, 60.1 with two fences)
+                unsigned n;
+                asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], %2;" : "=r"(n) : "l"(p.arrived + cut.c0), "r"(1u) : "memory");
+                last_one = n == (unsigned)cut.parts - 1;
+                if (last_one) { p.arrived[cut.c0] = 0; }
+            } else {
+                __threadfence();
+                const unsigned n = atomicAdd(p.arrived + cut.c0, 1u);
+                last_one = n == (unsigned)cut.parts - 1;
+                if (last_one) { p.arrived[cut.c0] = 0; __threadfence(); }
+            }
         }
         meet();
         if (last_one) {

@@ -177,31 +177,42 @@ __device__ __noinline__ void stand_still(uint64_t ns) {
 }
 
 // LATE: the self-checks' kernels (p.late)
-// Bytes of 32 positions (row0 on) of a tile as an operand: byte x scale, rounded to fp16. A lane has 16 bytes at a time, a quarter of a warp one row or two; `scales`: of position row0 + lane, K's
-// below and V's above. (Lanes of the operand's second half write their two pieces the other way round: eight lanes, eight places in the banks.)
+// Bytes of 32 positions (row0 on) of a tile as an operand: byte x scale, rounded to fp16. `scales`: of position row0 + lane, K's below and V's above. A lane has 16 bytes at a time, four lanes 64 bytes
+// of a row: eight lanes, whose reads and writes are one turn of the banks each, have two rows that both the bytes' swizzle and the operand's send to different banks (heads of 128: r and r ^ 5).
+// Places do not change from one group of eight rows to the next, so that they are made once a tile.
 template <int HD> __device__ __forceinline__ void make_operand(uint32_t bytes, uint32_t operand, int row0, uint32_t scales, bool is_v) {
-    constexpr int PER = HD / 16, AT_ONCE = 32 / PER, LOOPS = 32 / AT_ONCE;
-    const int lane = threadIdx.x & 31, c = lane % PER, r0 = lane / PER;
+    constexpr int STEPS = HD == 128 ? 2 : 1;                           // a warp's turns for eight rows
+    const int lane = threadIdx.x & 31, c = lane & 3;
     const uint32_t both = __byte_perm(scales, 0, is_v ? 0x3232 : 0x1010);
-    const int swap = HD == 128 ? c >> 2 : 0;
-    const uint32_t src = bytes + (row0 + r0) * HD + c * 16, half = operand + (c >> 2) * PT_HALF + (row0 + r0) * 128;
+    uint32_t src[STEPS], dst[STEPS];
+    int row[STEPS];
 #pragma unroll
-    for (int i0 = 0; i0 < LOOPS; i0 += 4) {
-        uint4 w[4];                                                    // (reads in flight)
+    for (int e = 0; e < STEPS; ++e) {
+        const int first = HD == 128 ? 2 * e + (lane >> 4) : lane >> 2, half = HD == 128 ? lane >> 3 & 1 : 0;
+        row[e] = HD == 128 && (lane & 4) ? first ^ 5 : first;
+        src[e] = bytes + (row0 + row[e]) * HD + (HD == 128 ? ((4 * half + c) ^ row[e]) << 4 : c << 4);
+        dst[e] = operand + half * PT_HALF + (row0 + row[e]) * 128 + (((2 * c) ^ row[e]) << 4);
+    }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) { w[i] = lds128(src + (i0 + i) * (AT_ONCE * HD)); }
+    for (int i0 = 0; i0 < 4; i0 += 2) {                                // groups of eight rows, two at a time
+        uint4 w[2][STEPS];                                             // (reads in flight)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int r = (i0 + i) * AT_ONCE + r0;
-            const uint32_t d = __shfl_sync(0xffffffffu, both, r);
-            uint32_t h[8];
-            halves_of(w[i].x, h[0], h[1]); halves_of(w[i].y, h[2], h[3]); halves_of(w[i].z, h[4], h[5]); halves_of(w[i].w, h[6], h[7]);
+        for (int i = 0; i < 2; ++i) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) { asm("mul.rn.f16x2 %0, %0, %1;" : "+r"(h[e]) : "r"(d)); }
-            const uint32_t row = half + (i0 + i) * (AT_ONCE * 128);
-            const int first = (2 * (c & 3) + swap) ^ (r & 7);          // (row0 is a multiple of 8)
-            sts128(row + first * 16, swap ? make_uint4(h[4], h[5], h[6], h[7]) : make_uint4(h[0], h[1], h[2], h[3]));
-            sts128(row + (first ^ 1) * 16, swap ? make_uint4(h[0], h[1], h[2], h[3]) : make_uint4(h[4], h[5], h[6], h[7]));
+            for (int e = 0; e < STEPS; ++e) { w[i][e] = lds128(src[e] + (i0 + i) * 8 * HD); }
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+#pragma unroll
+            for (int e = 0; e < STEPS; ++e) {
+                const uint32_t d = __shfl_sync(0xffffffffu, both, (i0 + i) * 8 + row[e]);
+                uint32_t h[8];
+                halves_of(w[i][e].x, h[0], h[1]); halves_of(w[i][e].y, h[2], h[3]); halves_of(w[i][e].z, h[4], h[5]); halves_of(w[i][e].w, h[6], h[7]);
+#pragma unroll
+                for (int k = 0; k < 8; ++k) { asm("mul.rn.f16x2 %0, %0, %1;" : "+r"(h[k]) : "r"(d)); }
+                sts128(dst[e] + (i0 + i) * 1024, make_uint4(h[0], h[1], h[2], h[3]));
+                sts128((dst[e] ^ 16) + (i0 + i) * 1024, make_uint4(h[4], h[5], h[6], h[7]));
+            }
         }
     }
 }
@@ -964,7 +975,7 @@ bool launch_paged_attention_tc(const PagedAttention &given, int head_dim, int n_
     CUtensorMap q, k, v;
     const int kind = p.kind();
     const bool bytes = kind == PK_INT8;
-    const CUtensorMapSwizzle swizzle = bytes ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B;
+    const CUtensorMapSwizzle swizzle = bytes && head_dim == 64 ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B;   // (see make_operand)
     if (!query_map(&q, p, n_head, head_dim) || !page_map(&k, p.k, p.view, p.n_head_kv, head_dim, box, bytes, swizzle) || !page_map(&v, p.v, p.view, p.n_head_kv, head_dim, box, bytes, swizzle)) { return false; }
     const auto launch = kind == PK_SHARED ? launch_tc<false, PK_SHARED> : bytes ? (p.late != PA_ON_TIME ? launch_tc<true, PK_INT8> : launch_tc<false, PK_INT8>)
                                           : p.late != PA_ON_TIME ? launch_tc<true, PK_PLAIN> : launch_tc<false, PK_PLAIN>;
