@@ -261,54 +261,64 @@ __global__ void __launch_bounds__(SH_WARPS * 32) paged_shared_kernel(const __gri
     }
 }
 
-// A row of a query head a warp: the pieces of its tile that the first pass's CTAs left, joined in their order. (In the first pass itself one CTA would have to read them all, 18 pieces of 64 KB where 64 requests
-// share 6000 positions: 35 us of its 51.)
+// Rows of two query heads a warp: the pieces of their tiles that the first pass's CTAs left, joined in their order. (In the first pass itself one CTA would have to read them all, 18 pieces of 64 KB where 64 requests
+// share 6000 positions: 25 us of its 51.) A piece has its rows side by side, four elements of each: two rows are what a sector of memory holds.
 constexpr int SJ_WARPS = 8, SJ_TILE = 128;    // (rows of a tile of the tensor-memory kernel)
 template <int HD>
 __global__ void __launch_bounds__(SJ_WARPS * 32) paged_shared_join_kernel(const __grid_constant__ PagedSharedJoin p) {
     pdl_launch_dependents();
     pdl_wait();
     const int lane = threadIdx.x & 31, n_head = p.n_head_kv * p.group;
-    const int64_t cell = (int64_t)blockIdx.x * SJ_WARPS + (threadIdx.x >> 5);
+    const int64_t cell = ((int64_t)blockIdx.x * SJ_WARPS + (threadIdx.x >> 5)) * 2 + (lane & 1);
     const int row = (int)(cell / n_head), head = (int)(cell - (int64_t)row * n_head), kv = (int)((unsigned)head / (unsigned)p.group);
     if (row >= p.view.n_rows) { return; }
-    const int s = sequence_of(p.view, row);
+    int s = -1, n = p.view.n_seq + 1;                               // the last one that begins at the row or in front of it
+    for (int lo = 0; n > 0;) {
+        const int half = n / 2;
+        if (p.view.row_start[lo + half] <= row) { s = lo + half; lo += half + 1; n -= half + 1; } else { n = half; }
+    }
     if (s < 0 || s >= p.view.n_seq || row >= p.view.row_end[s] || p.from[s] == 0) { return; }
     const int lead = max(0, p.lead[s]), tokens = SJ_TILE / p.group, half = (int)((unsigned)(row - lead) / (unsigned)tokens), first = lead + half * tokens;
     if (row < lead) { return; }                                     // (no group that makes sense)
     const int2 cut = p.cuts[(int64_t)kv * p.view.n_rows + first];
     if (cut.y < 2) { return; }
     const int r = (row - first) * p.group + head - kv * p.group;
-    constexpr int PIECE = SJ_TILE * (HD + 2);
-    auto piece = [&](int i) { return p.partial + (paged_slot(cut.x + i, cut.x) * 2 + (half & 1)) * PIECE; };
+    constexpr int PIECE = SJ_TILE * (HD + 2), FOURS = HD / 64;      // of a lane: four elements, 64 apart
+    const float *const place = p.partial + (half & 1) * PIECE;
     float  m = -INFINITY, l = 0.f;
-    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    float4 v[FOURS];
+#pragma unroll
+    for (int c = 0; c < FOURS; ++c) { v[c] = make_float4(0.f, 0.f, 0.f, 0.f); }
 #pragma unroll 1
     for (int i0 = 0; i0 < cut.y; i0 += 8) {                         // eight pieces are in flight together; what came before is scaled to the new maximum
         float  pm[8], pl[8], top = m;
-        float4 u[8];
+        float4 u[8][FOURS];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             const bool is = i0 + j < cut.y;
-            const float *from = piece(is ? i0 + j : 0);
+            const float *from = place + paged_slot(cut.x + (is ? i0 + j : 0), cut.x) * 2 * PIECE;
             pm[j] = is ? __ldcg(from + SJ_TILE * HD + r) : -INFINITY;
             pl[j] = is ? __ldcg(from + SJ_TILE * HD + SJ_TILE + r) : 0.f;
-            u[j] = is && lane < HD / 4 ? __ldcg(reinterpret_cast<const float4 *>(from) + lane * SJ_TILE + r) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int c = 0; c < FOURS; ++c) { u[j][c] = is ? __ldcg(reinterpret_cast<const float4 *>(from) + (16 * c + lane / 2) * SJ_TILE + r) : make_float4(0.f, 0.f, 0.f, 0.f); }
         }
 #pragma unroll
         for (int j = 0; j < 8; ++j) { top = fmaxf(top, pm[j]); }
         const float base = top == -INFINITY ? 0.f : top, before = exp2f(m - base);
         m = top; l *= before;
-        v = make_float4(v.x * before, v.y * before, v.z * before, v.w * before);
+#pragma unroll
+        for (int c = 0; c < FOURS; ++c) { v[c] = make_float4(v[c].x * before, v[c].y * before, v[c].z * before, v[c].w * before); }
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             const float f = exp2f(pm[j] - base);
-            v.x += f * u[j].x; v.y += f * u[j].y; v.z += f * u[j].z; v.w += f * u[j].w;
             l += f * pl[j];
+#pragma unroll
+            for (int c = 0; c < FOURS; ++c) { v[c].x += f * u[j][c].x; v[c].y += f * u[j][c].y; v[c].z += f * u[j][c].z; v[c].w += f * u[j][c].w; }
         }
     }
-    if (lane < HD / 4) { reinterpret_cast<float4 *>(p.out + cell * HD)[lane] = v; }
-    if (lane == 0) { p.stats[cell] = make_float2(m, l); }
+#pragma unroll
+    for (int c = 0; c < FOURS; ++c) { reinterpret_cast<float4 *>(p.out + cell * HD)[16 * c + lane / 2] = v[c]; }
+    if (lane < 2) { p.stats[cell] = make_float2(m, l); }
 }
 
 template <int ROWS>
@@ -347,7 +357,7 @@ cudaError_t launch_paged_shared(const PagedShared &p, const LaunchCfg &cfg) {
 }
 cudaError_t launch_paged_shared_join(const PagedSharedJoin &p, int head_dim, const LaunchCfg &cfg) {
     const int64_t cells = (int64_t)p.view.n_rows * p.n_head_kv * p.group;
-    return launch_maybe_pdl(head_dim == 128 ? paged_shared_join_kernel<128> : paged_shared_join_kernel<64>, dim3((unsigned)((cells + SJ_WARPS - 1) / SJ_WARPS)), SJ_WARPS * 32, 0, cfg.stream, cfg.pdl, p);
+    return launch_maybe_pdl(head_dim == 128 ? paged_shared_join_kernel<128> : paged_shared_join_kernel<64>, dim3((unsigned)((cells + 2 * SJ_WARPS - 1) / (2 * SJ_WARPS))), SJ_WARPS * 32, 0, cfg.stream, cfg.pdl, p);
 }
 cudaError_t launch_paged_shared_rows(const PagedAttention &p, int head_dim, int row_tiles, int sms, const LaunchCfg &cfg) { return launch_rows_kind<PK_SHARED>(p, head_dim, row_tiles, sms, cfg); }
 

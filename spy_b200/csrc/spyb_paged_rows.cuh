@@ -45,7 +45,20 @@ __device__ __forceinline__ void rows_finish(const PagedAttention &p, const Paged
     constexpr int PART = TILE * (HD + 2), NT = PR_WARPS * 32;
     const int tid = threadIdx.x, done = what.rows;
     float *part = p.partial + paged_slot(blockIdx.x, cut.c0) * PART;
-    auto put = [&](int r, int c, float4 v, float m, float l) {   // four elements of a row, its maximum and sum
+    // what the first pass found for four elements is read one turn ahead
+    const bool with = KIND != PK_PLAIN && p.with_stats != nullptr && what.from > 0;
+    struct First { float2 stats; float4 sums; };
+    auto first_pass = [&](int x) {
+        First f = {make_float2(-CUDART_INF_F, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
+        if (KIND != PK_PLAIN && with && x < done * (HD / 4)) {
+            const int r = x / (HD / 4), pr = what.tile * TILE + r, token = (int)((unsigned)pr / (unsigned)p.group);
+            const int64_t cell = (int64_t)(what.row0 + token) * (p.n_head_kv * p.group) + what.head * p.group + pr - token * p.group;
+            f.stats = p.with_stats[cell]; f.sums = *reinterpret_cast<const float4 *>(p.with_out + cell * HD + (x - r * (HD / 4)) * 4);
+        }
+        return f;
+    };
+    First next = first_pass(tid);
+    auto put = [&](int r, int c, float4 v, float m, float l, const First &f) {   // four elements of a row, its maximum and sum
         const int pr = what.tile * TILE + r, token = (int)((unsigned)pr / (unsigned)p.group), g = pr - token * p.group;
         const int64_t o2 = (int64_t)(what.row0 + token) * p.out_stride + (what.head * p.group + g) * HD + c;
         if constexpr (KIND != PK_PLAIN) {
@@ -55,7 +68,7 @@ __device__ __forceinline__ void rows_finish(const PagedAttention &p, const Paged
                 *reinterpret_cast<float4 *>(static_cast<float *>(p.out) + o2) = v;
                 return;
             }
-            if (p.with_stats != nullptr && what.from > 0) { paged_join_pass(v, l, m, p.with_stats[cell], *reinterpret_cast<const float4 *>(p.with_out + cell * HD + c)); }
+            if (with) { paged_join_pass(v, l, m, f.stats, f.sums); }
         }
         const float inv = l == 0.f ? 0.f : 1.f / l;
         const float w[4] = {v.x * inv, v.y * inv, v.z * inv, v.w * inv};
@@ -63,6 +76,8 @@ __device__ __forceinline__ void rows_finish(const PagedAttention &p, const Paged
     };
     for (int x = tid; x < done * (HD / 4); x += NT) {
         const int r = x / (HD / 4), c = (x - r * (HD / 4)) * 4;
+        const First found = next;
+        if (cut.parts == 1) { next = first_pass(x + NT); }
         float m = -CUDART_INF_F;
 #pragma unroll
         for (int w = 0; w < WARPS; ++w) { m = fmaxf(m, mm[w * room + r]); }
@@ -76,7 +91,7 @@ __device__ __forceinline__ void rows_finish(const PagedAttention &p, const Paged
             v.x += f * u.x; v.y += f * u.y; v.z += f * u.z; v.w += f * u.w;
             l += f * ml[w * room + r];
         }
-        if (cut.parts == 1) { put(r, c, v, m, l); }
+        if (cut.parts == 1) { put(r, c, v, m, l, found); }
         else {
             *reinterpret_cast<float4 *>(part + r * HD + c) = v;
             if (c == 0) { part[TILE * HD + r] = m; part[TILE * HD + TILE + r] = l; }
@@ -101,6 +116,8 @@ __device__ __forceinline__ void rows_finish(const PagedAttention &p, const Paged
         if (last_one) {
             for (int x = tid; x < done * (HD / 4); x += NT) {
                 const int r = x / (HD / 4), c = (x - r * (HD / 4)) * 4;
+                const First found = next;
+                next = first_pass(x + NT);
                 float m = -CUDART_INF_F, l = 0.f;
                 float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
                 // eight CTAs' findings are in flight together; what came before is scaled to the new maximum
@@ -128,7 +145,7 @@ __device__ __forceinline__ void rows_finish(const PagedAttention &p, const Paged
                         l += f * pl[j];
                     }
                 }
-                put(r, c, v, m, l);
+                put(r, c, v, m, l, found);
             }
         }
     }
