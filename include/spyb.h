@@ -337,8 +337,8 @@ spyb_status spyb_paged_load(spyb_backend *backend, const spyb_paged_load_desc *d
 
 /* Which sequences hold the same K and V in their first positions (one system prompt, a document, the trunk of several answers): sequences group_start[g] .. group_start[g+1]-1 (ascending) the same in
  * their first n_shared[g] ones, usually because their tables name the same pages. Device arrays, read when the kernels run; sequences in no group share nothing. That is a promise about values, and nothing else:
- * which positions a row sees does not change, and what is shared is read, once for all, from the pages of the group's first sequence that has rows. (It is cut to whole 128 positions that all rows
- * of the group see, so a window leaves nothing of it.) n_group = 0: nothing is shared, the rest is not read. `workspace`: device memory, 16-byte aligned, of spyb_paged_attend_workspace bytes, this call's until the
+ * which positions a row sees does not change, and what is shared is read, once for all, from the pages of the group's first sequence that has rows. (It is cut to what all rows of the group see, in whole pages or so, so a
+ * window leaves nothing of it, and below 128 positions to nothing.) n_group = 0: nothing is shared, the rest is not read. `workspace`: device memory, 16-byte aligned, of spyb_paged_attend_workspace bytes, this call's until the
  * backend's stream has passed it; it needs no clearing, and calls that follow one another on a backend may have one. */
 typedef struct {
     const int32_t *group_start;   /* [n_group + 1] */

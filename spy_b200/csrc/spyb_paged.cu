@@ -393,7 +393,7 @@ static spyb_status paged_attention(spyb_backend *be, const spyb_paged_attention_
         const SharedRoom room = shared_room(d.batch.n_seq, d.batch.n_rows, d.n_head, hd);
         uint8_t *const mem = static_cast<uint8_t *>(shared->workspace);
         PagedShared g;
-        g.view = p.view; g.group_start = shared->group_start; g.n_shared = shared->n_shared; g.n_group = shared->n_group; g.causal = p.causal;
+        g.view = p.view; g.group_start = shared->group_start; g.n_shared = shared->n_shared; g.n_group = shared->n_group; g.causal = p.causal; g.align = paged_shared_align(d.cache.page_size);
         g.from = reinterpret_cast<int32_t *>(mem + room.words); g.row_end = g.from + d.batch.n_seq; g.kv = g.row_end + d.batch.n_seq; g.lead = g.kv + d.batch.n_seq;
         SPYB_CUDA(be, launch_paged_shared(g, be->launch_cfg(be->config.use_pdl != 0)));
         PagedAttention first = p;

@@ -9,7 +9,7 @@ namespace spyb {
 
 struct PagedView {                        // a spyb_paged_cache and a spyb_paged_batch as the kernels read them
     const int32_t *row_start = nullptr, *row_end = nullptr, *n_kv = nullptr, *page_table = nullptr;   // (row_end: row_start + 1, or an array of its own)
-    const int32_t *from = nullptr;        // positions in front of it (a multiple of PA_SHARED) are not this pass's; nullptr: all are
+    const int32_t *from = nullptr;        // positions in front of it (paged_shared_align) are not this pass's; nullptr: all are
     int            n_seq = 0, n_rows = 0, table_stride = 0, n_pages = 0, page_size = 1;
     int            n_kv_most = 0;         // positions that a row of the table can name
     int64_t        page_stride = 0, token_stride = 0, head_stride = 0;
@@ -64,10 +64,10 @@ struct PagedLoad {
     int64_t      k_stride = 0, v_stride = 0;
     int          n_head_kv = 0, head_dim = 0;
 };
-struct PagedShared {                      // which sequences share what, and what becomes of it (PA_SHARED)
+struct PagedShared {                      // which sequences share what, and what becomes of it
     PagedView      view;
     const int32_t *group_start = nullptr, *n_shared = nullptr;
-    int            n_group = 0, causal = 1;
+    int            n_group = 0, causal = 1, align = 128;                 // align: what is shared is cut to a multiple of so many positions
     int32_t       *from = nullptr, *row_end = nullptr, *kv = nullptr, *lead = nullptr;   // [n_seq] each: where a sequence's own positions begin; rows and positions of the first pass's sequences; first row of the group
 };
 struct PagedSharedJoin {                  // cut items of the first pass on tensor memory
@@ -79,7 +79,9 @@ struct PagedSharedJoin {                  // cut items of the first pass on tens
     float2        *stats = nullptr;
     int            n_head_kv = 0, group = 1;
 };
-constexpr int PA_SHARED = 128;            // what is shared is cut to a multiple of so many positions: both kernels' blocks begin at such ones
+constexpr int PA_SHARED = 128;            // fewer positions than that are not shared
+// A sequence's own positions begin where a box of the kernels' tensor maps and a block of 16 do: at a multiple of the largest power of two that divides the page size, 16 to 128
+inline int paged_shared_align(int page_size) { int a = 128; while (a > 16 && page_size % a != 0) { a /= 2; } return a; }
 int         paged_cut_selftest();   // host-only: 0 when the CTAs' pieces cover every item once, on any lengths
 cudaError_t launch_paged_store(const PagedStore &p, int in_type, int q_out_type, int sms, const LaunchCfg &cfg);
 cudaError_t launch_paged_load(const PagedLoad &p, int out_type, int sms, const LaunchCfg &cfg);

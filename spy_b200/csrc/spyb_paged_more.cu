@@ -250,7 +250,7 @@ __global__ void __launch_bounds__(SH_WARPS * 32) paged_shared_kernel(const __gri
             leader = min(leader, __shfl_xor_sync(0xffffffffu, leader, o));
             with_rows += __shfl_xor_sync(0xffffffffu, with_rows, o);
         }
-        common = with_rows > 1 ? common / PA_SHARED * PA_SHARED : 0;
+        common = with_rows > 1 && common >= PA_SHARED ? common / p.align * p.align : 0;
     }
     if (lane == 0) {
         const int begin = p.view.row_start[s];
