@@ -303,8 +303,7 @@ spyb_status spyb_paged_attention(spyb_backend *backend, const spyb_paged_attenti
  * A cache of type SPYB_INT8 keeps a byte an element and a scale for each head of each position: an element stands for byte * scale. Strides of its spyb_paged_cache are multiples of 16
  * elements. `pairs` are fp16 pairs (K's scale, V's); the pair of (page, position in the page, head) lies at page * page_stride + position * token_stride + head * head_stride, in
  * pairs (4-byte aligned). The scale of a head is the smallest fp16 that is not below its largest magnitude / 127, and its bytes are its elements / scale to the nearest even: off by half
- * a scale at most. A head of zeros has scale 0. One that holds an infinity, NaN or a magnitude above 65468 (127 of the scale 515.5) has scale NaN: all of it reads as NaN. (Scales that a
- * caller writes are to be 0 .. 515.5: more than fp16 holds may read as infinities.) */
+ * a scale at most. A head of zeros has scale 0. One that holds an infinity, NaN or a magnitude above 65468 (127 of the scale 515.5) has scale NaN: all of it reads as NaN. */
 typedef struct {
     void   *pairs;
     int64_t page_stride, token_stride, head_stride;
@@ -348,8 +347,8 @@ typedef struct {
     uint64_t workspace_bytes;
 } spyb_paged_shared;
 
-/* spyb_paged_attention over a cache of SPYB_FP16 or SPYB_INT8, with what sequences share read once for all of them. For SPYB_INT8 the kernel for many rows rounds byte * scale to fp16 in front of
- * its products, the one for few rows multiplies scores and probabilities by the scales in f32. A row that sees nothing is zeros; what is not seen has no influence, scales of any value included. */
+/* spyb_paged_attention over a cache of SPYB_FP16 or SPYB_INT8, with what sequences share read once for all of them. For SPYB_INT8 scores are
+ * multiplied by K's scales and probabilities by V's in f32; a probability times a scale is rounded to fp16 in front of the second product, against the largest scale met. A row that sees nothing is zeros; what is not seen has no influence, scales of any value included. */
 typedef struct {
     spyb_paged_attention_desc attention;
     spyb_paged_scales scales;

@@ -8,7 +8,7 @@
 // swizzle of the operands: K row by row (K-major), V as it lies (its positions are the product's inner dimension: MN-major), no transposition anywhere.
 //   warps 0-3, 4-7   probabilities of tile 0 / 1, rescaling, output          warp 8   issues the MMAs
 //   warp 9           copies                                                   warps 10, 11  Q; clear and check the V tiles that not all rows see whole
-//   warps 12-15      (8-bit caches) make the operands of K and V: bytes land in a ring of their own, byte x scale is rounded to fp16
+//   warps 12-15      (8-bit caches) make the operands of K and V: bytes land in a ring of their own, as whole numbers in fp16
 // Probabilities are taken against a maximum that follows the true one when that is 2^8 above it: O is rescaled in the first steps and hardly ever after.
 // Measured (heads of 128): 8192 tokens of a prompt, 32 heads, 570 us, 965 TFLOP/s of the 1640 of a matrix product; 512 tokens at 32 768 positions 281 us, 970;
 // 1500 at 9111, 40 heads, 247 us, 1040; 512 at 3968 52 to 55 us, 595; five tokens of 24 sequences of up to 9000, 111 us, 4.2 TB/s. Heads of 64 have half the
@@ -39,9 +39,9 @@ template <int HD, int KIND> struct TcShape {
     static constexpr uint32_t OPERAND = PT_KEYS * HD * 2;                      // a tile of Q, K or V
     static constexpr bool BYTES = KIND == PK_INT8;
     static constexpr int THREADS = BYTES ? 512 : 384, READERS = BYTES ? 15 : 11;   // (readers of an entry: eight warps for probabilities, one for MMAs, two for Q and V, four for bytes)
-    static constexpr int REGS_SOFTMAX = BYTES ? 184 : 208, REGS_OTHERS = BYTES ? 72 : 88;   // 256 x 208 + 128 x 88 = 384 x 168, 256 x 184 + 256 x 72 = 512 x 128: what the block is launched with
+    static constexpr int REGS_SOFTMAX = BYTES ? 192 : 208, REGS_OTHERS = BYTES ? 64 : 88;   // 256 x 208 + 128 x 88 = 384 x 168, 256 x 192 + 256 x 64 = 512 x 128: what the block is launched with
     static constexpr int SLOTS = BYTES ? (HD == 128 ? 3 : 4) : HD == 128 ? 5 : 8;   // K and V tiles in flight; of bytes: made into operands ahead
-    static constexpr int BYTE_SLOTS = BYTES ? (HD == 128 ? 4 : 6) : 0;         // tiles of bytes in flight
+    static constexpr int BYTE_SLOTS = BYTES ? (HD == 128 ? 3 : 6) : 0;         // tiles of bytes in flight
     static constexpr uint32_t BYTE_TILE = PT_KEYS * HD;
     static constexpr int Q_BUFFERS = HD == 128 ? 1 : 2;                        // (heads of 64: the next stretch's Q comes while this one's is in use; there is room for it)
     static constexpr uint32_t SMEM = (2 * Q_BUFFERS + SLOTS) * OPERAND + BYTE_SLOTS * BYTE_TILE + 1024; // (+ alignment)
@@ -72,9 +72,13 @@ struct Entry {
 // it was that gave up. (Waiting for it in every case, at the end of each role, cost 5 % of prompts of heads of 64.)
 constexpr uint64_t PT_LANDING_NS = 1000000000;       // what is on its way has this long to land (whatever the limit of the waits)
 constexpr int PT_ENTRIES = 4;                        // stretches known ahead
-struct TcShared {
+// 8-bit caches, of the last four steps: K's scales with what scores are scaled by anyway, V's, and the exponents of powers of two that V's are not above, by the warps that read them
+template <int KIND> struct ByteScales {};
+template <> struct __align__(16) ByteScales<PK_INT8> { float k[4][PT_KEYS], v[4][PT_KEYS], v_top[4][4]; };
+template <int KIND> struct TcShared {
     uint64_t full[8], empty[8];                          // a slot's copies have landed; its last MMA is done, and both warps that check V have seen its phase
     uint64_t clean[8];                                   // of the last V tiles: what nobody sees is cleared
+    ByteScales<KIND> scale;
     uint64_t byte_full[8], byte_empty[8];                // 8-bit caches: a tile of bytes has landed; its operand is made (`full` is that operand's, `empty` its last MMA's)
     uint64_t q_ready[2][2], q_free[2][2];                // of the two tiles and their buffers, in stretches in which they see anything
     uint64_t s_ready[2], s_free[2], p_ready[2][2], p_free[2], o_ready[2];   // (P ready) of the first 96 positions and the rest; (free) where P lies apart
@@ -177,21 +181,18 @@ __device__ __noinline__ void stand_still(uint64_t ns) {
 }
 
 // LATE: the self-checks' kernels (p.late)
-// Bytes of 32 positions (row0 on) of a tile as an operand: byte x scale, rounded to fp16. `scales`: of position row0 + lane, K's below and V's above. A lane has 16 bytes at a time, four lanes 64 bytes
-// of a row: eight lanes, whose reads and writes are one turn of the banks each, have two rows that both the bytes' swizzle and the operand's send to different banks (heads of 128: r and r ^ 5).
-// Places do not change from one group of eight rows to the next, so that they are made once a tile.
-template <int HD> __device__ __forceinline__ void make_operand(uint32_t bytes, uint32_t operand, int row0, uint32_t scales, bool is_v) {
+// Bytes of 32 positions (row0 on) of a tile as an operand: whole numbers, without an error (scales are for scores and probabilities, in f32: rounded products of both would cost a score some 2^-12 of
+// its terms, three times the error of the whole). A lane has 16 bytes at a time, four lanes 64 bytes of a row: eight lanes, whose reads and writes are one turn of the banks each, have two rows that both
+// the bytes' swizzle and the operand's send to different banks (heads of 128: r and r ^ 5). Places do not change from one group of eight rows to the next, so that they are made once a tile.
+template <int HD> __device__ __forceinline__ void make_operand(uint32_t bytes, uint32_t operand, int row0) {
     constexpr int STEPS = HD == 128 ? 2 : 1;                           // a warp's turns for eight rows
     const int lane = threadIdx.x & 31, c = lane & 3;
-    const uint32_t both = __byte_perm(scales, 0, is_v ? 0x3232 : 0x1010);
     uint32_t src[STEPS], dst[STEPS];
-    int row[STEPS];
 #pragma unroll
     for (int e = 0; e < STEPS; ++e) {
-        const int first = HD == 128 ? 2 * e + (lane >> 4) : lane >> 2, half = HD == 128 ? lane >> 3 & 1 : 0;
-        row[e] = HD == 128 && (lane & 4) ? first ^ 5 : first;
-        src[e] = bytes + (row0 + row[e]) * HD + (HD == 128 ? ((4 * half + c) ^ row[e]) << 4 : c << 4);
-        dst[e] = operand + half * PT_HALF + (row0 + row[e]) * 128 + (((2 * c) ^ row[e]) << 4);
+        const int first = HD == 128 ? 2 * e + (lane >> 4) : lane >> 2, half = HD == 128 ? lane >> 3 & 1 : 0, row = HD == 128 && (lane & 4) ? first ^ 5 : first;
+        src[e] = bytes + (row0 + row) * HD + (HD == 128 ? ((4 * half + c) ^ row) << 4 : c << 4);
+        dst[e] = operand + half * PT_HALF + (row0 + row) * 128 + (((2 * c) ^ row) << 4);
     }
 #pragma unroll
     for (int i0 = 0; i0 < 4; i0 += 2) {                                // groups of eight rows, two at a time
@@ -205,24 +206,15 @@ template <int HD> __device__ __forceinline__ void make_operand(uint32_t bytes, u
         for (int i = 0; i < 2; ++i) {
 #pragma unroll
             for (int e = 0; e < STEPS; ++e) {
-                const uint32_t d = __shfl_sync(0xffffffffu, both, (i0 + i) * 8 + row[e]);
                 uint32_t h[8];
                 halves_of(w[i][e].x, h[0], h[1]); halves_of(w[i][e].y, h[2], h[3]); halves_of(w[i][e].z, h[4], h[5]); halves_of(w[i][e].w, h[6], h[7]);
-#pragma unroll
-                for (int k = 0; k < 8; ++k) { asm("mul.rn.f16x2 %0, %0, %1;" : "+r"(h[k]) : "r"(d)); }
                 sts128(dst[e] + (i0 + i) * 1024, make_uint4(h[0], h[1], h[2], h[3]));
                 sts128((dst[e] ^ 16) + (i0 + i) * 1024, make_uint4(h[4], h[5], h[6], h[7]));
             }
         }
     }
 }
-// a scale beyond what bytes of fp16 values have is an infinity, as its elements may be
-__device__ __forceinline__ bool large_scale(uint32_t h) { return (h & 0x7fffu) > 0x6007u; }   // 515.5
-__device__ __forceinline__ uint32_t no_large_scale(uint32_t pair) {
-    if (large_scale(pair) && (pair & 0x7fffu) <= 0x7c00u) { pair = (pair & 0xffff8000u) | 0x7c00u; }
-    if (large_scale(pair >> 16) && (pair >> 16 & 0x7fffu) <= 0x7c00u) { pair = (pair & 0x8000ffffu) | 0x7c000000u; }
-    return pair;
-}
+__device__ __forceinline__ bool infinite_or_nan(uint32_t h) { return (h & 0x7c00u) == 0x7c00u; }
 
 template <int HD, bool LATE, int KIND>
 __global__ void __launch_bounds__(TcShape<HD, KIND>::THREADS, 1) paged_tc_kernel(const __grid_constant__ PagedAttention p, const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
@@ -231,7 +223,7 @@ __global__ void __launch_bounds__(TcShape<HD, KIND>::THREADS, 1) paged_tc_kernel
     constexpr bool BYTES = Shape::BYTES;
     constexpr int SLOTS = Shape::SLOTS;
     extern __shared__ uint8_t raw[];
-    __shared__ TcShared sh;
+    __shared__ TcShared<KIND> sh;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const uint32_t base = (smem_u32(raw) + 1023) & ~1023u, q_addr = base, ring = base + 2 * Shape::Q_BUFFERS * Shape::OPERAND;
     const uint32_t full = smem_u32(sh.full), empty = smem_u32(sh.empty), clean = smem_u32(sh.clean), known = smem_u32(sh.known), read = smem_u32(sh.read), joined = smem_u32(sh.joined);
@@ -310,10 +302,35 @@ __global__ void __launch_bounds__(TcShape<HD, KIND>::THREADS, 1) paged_tc_kernel
                 tmem_ld_wait();
 #pragma unroll
                 for (int i = 1; i < 4; ++i) { tmem_ld32(s_tmem + 32 * i, s + 32 * i); }
+                // bytes: scores by K's scales, so that they are in powers of two already
+                const float4 *k_scale = nullptr, *v_scale = nullptr;
+                float v_top = 0.f;
+                if constexpr (BYTES) {
+                    const int at = (tiles + step - en.begin) & 3;
+                    k_scale = reinterpret_cast<const float4 *>(sh.scale.k[at]); v_scale = reinterpret_cast<const float4 *>(sh.scale.v[at]);
+                    const float4 e = *reinterpret_cast<const float4 *>(sh.scale.v_top[at]);
+                    v_top = fmaxf(fmaxf(e.x, e.y), fmaxf(e.z, e.w));
+                }
+                auto by_scales = [&](int from, int to) {
+                    if constexpr (BYTES) {
+#pragma unroll
+                        for (int c = 0; c < 128; c += 4) {
+                            if (c < from || c >= to) { continue; }
+                            const float4 k = k_scale[c / 4];
+                            float a, b;
+                            f2_unpack(f2_mul(f2_pack_bits(s[c], s[c + 1]), f2_pack(k.x, k.y)), a, b);
+                            s[c] = __float_as_uint(a); s[c + 1] = __float_as_uint(b);
+                            f2_unpack(f2_mul(f2_pack_bits(s[c + 2], s[c + 3]), f2_pack(k.z, k.w)), a, b);
+                            s[c + 2] = __float_as_uint(a); s[c + 3] = __float_as_uint(b);
+                        }
+                    }
+                };
+                if (plain) { by_scales(0, 32); }
                 if (!plain) {
                     const int j0 = en.lo + step * PT_KEYS;
                     const int c1 = (p.causal ? min(en.hi, pos + 1) : en.hi) - j0, c0 = p.causal && p.window > 0 ? pos - p.window + 1 - j0 : 0;
                     tmem_ld_wait();
+                    by_scales(0, 128);
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         const int a = min(max(c0 - 32 * i, 0), 32), b = min(max(c1 - 32 * i, 0), 32);
@@ -331,9 +348,15 @@ __global__ void __launch_bounds__(TcShape<HD, KIND>::THREADS, 1) paged_tc_kernel
 #pragma unroll
                     for (int c = 0; c < 16; ++c) {
                         float a, b;
-                        f2_unpack(f2_fma(f2_pack_bits(s[32 * i + 2 * c], s[32 * i + 2 * c + 1]), scale2, neg2), a, b);
+                        const uint64_t x = f2_pack_bits(s[32 * i + 2 * c], s[32 * i + 2 * c + 1]);
+                        f2_unpack(BYTES ? f2_add(x, neg2) : f2_fma(x, scale2, neg2), a, b);
                         a = exp2_fast(a); b = exp2_fast(b);
-                        sum[c & 1] = f2_add(sum[c & 1], f2_pack(a, b));
+                        const uint64_t power = f2_pack(a, b);
+                        sum[c & 1] = f2_add(sum[c & 1], power);
+                        if constexpr (BYTES) {                // (V's scales beside the probabilities)
+                            const float2 v = reinterpret_cast<const float2 *>(v_scale)[16 * i + c];
+                            f2_unpack(f2_mul(power, f2_pack(v.x, v.y)), a, b);
+                        }
                         h[c] = pack_f16(a, b);
                     }
                     tmem_st16(p_tmem + 16 * i, h);
@@ -346,13 +369,14 @@ __global__ void __launch_bounds__(TcShape<HD, KIND>::THREADS, 1) paged_tc_kernel
                 };
                 if (Shape::P_APART) { wait_for(p_free + 8 * t, p_phase, limit); p_phase ^= 1; tc_fence_after(); }   // (P's products of the step before; else S is made behind them)
                 // Powers against the maximum of the steps before, which nearly always does; whether it did shows beside them. (Not the stretch's first time round.)
-                bool fresh = step == own.from;
+                bool fresh = step == own.from, scaled = false;
                 for (;;) {
                     const float neg = m == -CUDART_INF_F ? 0.f : -m;
                     neg2 = f2_pack(neg, neg);
                     sum[0] = sum[1] = 0;
                     if (!fresh) { powers(0); }
                     tmem_ld_wait();
+                    if (BYTES && plain && !scaled) { by_scales(32, 128); scaled = true; }
                     if (!fresh) { powers(1); }
                     float tops[4];
 #pragma unroll
@@ -362,7 +386,8 @@ __global__ void __launch_bounds__(TcShape<HD, KIND>::THREADS, 1) paged_tc_kernel
 #pragma unroll
                         for (int e = 0; e < 4; ++e) { tops[e] = max3(tops[e], __uint_as_float(s[c + 2 * e]), __uint_as_float(s[c + 2 * e + 1])); }
                     }
-                    const float top = fmaxf(max3(tops[0], tops[1], tops[2]), tops[3]) * scale;
+                    // (bytes: the largest weight is at most a probability of 1 by the largest of V's scales; sums of probabilities are against the same)
+                    const float most = fmaxf(max3(tops[0], tops[1], tops[2]), tops[3]), top = BYTES ? most + v_top : most * scale;
                     if (__any_sync(0xffffffffu, mine && top > m + 8.f)) {
                         const float to = fmaxf(m, top), f = to == m ? 1.f : exp2_fast(m - to);
                         m = to; l *= f;
@@ -434,8 +459,8 @@ __global__ void __launch_bounds__(TcShape<HD, KIND>::THREADS, 1) paged_tc_kernel
                             const int64_t at = page * p.view.page_stride + (j % p.view.page_size) * p.view.token_stride + en.head * p.view.head_stride + 32 * i;
                             if constexpr (BYTES) {
                                 const uint32_t pair = p.scales.pairs[page * p.scales.page_stride + (j % p.view.page_size) * p.scales.token_stride + en.head * p.scales.head_stride];
-                                if (!large_scale(pair >> 16)) { continue; }
-                                const float scale = half2_bits(no_large_scale(pair)).y;
+                                if (!infinite_or_nan(pair >> 16)) { continue; }
+                                const float scale = half2_bits(pair).y;
                                 const int8_t *v = reinterpret_cast<const int8_t *>(p.v) + at;
 #pragma unroll
                                 for (int c = 0; c < 32; ++c) { o[c] = __float_as_uint(__uint_as_float(o[c]) + (float)v[c] * scale); }
@@ -750,22 +775,29 @@ __global__ void __launch_bounds__(TcShape<HD, KIND>::THREADS, 1) paged_tc_kernel
                     if (en.begin < end) { find(en.begin); fetch(); find(en.begin + 1); }
                     for (int step = en.begin; step < end; ++step) {
                         if (LATE && p.late == PA_LATE_CHECKS && tiles < 12) { stand_still(4000); }
-                        uint32_t pair = next_ok ? no_large_scale(next_pair) : 0u;
+                        uint32_t pair = next_ok ? next_pair : 0u;
                         fetch(); find(step + 2);
+                        if (!(en.whole(p, a, step) && (b.rows == 0 || en.whole(p, b, step)))) {
+                            // 0 x inf: positions that some rows see and others do not. They are taken out, and given back to the rows that see them
+                            const bool bad = infinite_or_nan(pair >> 16);
+                            if (__any_sync(0xffffffffu, bad)) {
+                                if (bad) { pair &= 0xffffu; }
+                                if (lane == 0) { *reinterpret_cast<volatile int *>(&sh.poison[stretch & 7]) = (int)stretch + 1; }
+                            }
+                        }
+                        const float2 scale = half2_bits(pair);
+                        const unsigned top = __reduce_max_sync(0xffffffffu, infinite_or_nan(pair >> 16) ? 0u : __float_as_uint(fabsf(scale.y)));
 #pragma unroll 1
                         for (int kv = 0; kv < 2; ++kv) {
-                            if (kv == 1 && !(en.whole(p, a, step) && (b.rows == 0 || en.whole(p, b, step)))) {
-                                // 0 x inf: positions that some rows see and others do not. They are taken out, and given back to the rows that see them
-                                const bool bad = large_scale(pair >> 16);
-                                if (__any_sync(0xffffffffu, bad)) {
-                                    if (bad) { pair &= 0xffffu; }
-                                    if (lane == 0) { *reinterpret_cast<volatile int *>(&sh.poison[stretch & 7]) = (int)stretch + 1; }
-                                }
-                            }
                             wait_for(byte_full + 8 * byte_slot, byte_phase, limit);
                             wait_for(empty + 8 * slot, phase ^ 1, limit);
                             if (gave_up()) { break; }
-                            make_operand<HD>(byte_ring + byte_slot * Shape::BYTE_TILE, ring + slot * Shape::OPERAND, row0, pair, kv == 1);
+                            if (kv == 0) {                // (a slot for K is free: what the step four before this one had is read)
+                                sh.scale.k[tiles & 3][row0 + lane] = fmaf(scale.x, 0.f, scale.x * p.scale_log2);   // (an infinite one is NaN: its elements' infinities do not add up to one)
+                                sh.scale.v[tiles & 3][row0 + lane] = scale.y;
+                                if (lane == 0) { sh.scale.v_top[tiles & 3][warp - 12] = top == 0 ? -24.f : (float)((int)(top >> 23) - 126); }
+                            }
+                            make_operand<HD>(byte_ring + byte_slot * Shape::BYTE_TILE, ring + slot * Shape::OPERAND, row0);
                             fence_async_smem();
                             __syncwarp();
                             if (lane == 0) { mbar_arrive(byte_empty + 8 * byte_slot); mbar_arrive(full + 8 * slot); }
