@@ -384,9 +384,10 @@ spyb_status spyb_sample(spyb_backend *backend, const spyb_sample_desc *desc);
 /* The weights of logits beside a largest one, as spyb_sample makes them for rows of n_vocab (host arrays; a check of their precision, synchronous). */
 spyb_status spyb_sample_weights(spyb_backend *backend, const float *logits_host, int32_t n, float largest, float temperature, int32_t n_vocab, uint64_t *weights_host);
 
-/* Self-check of spyb_paged_attention's hand-overs, without a fault: the tensor-memory kernel on a small batch of its own with one of its roles late. who = 1: the warps that check values
- * stay microseconds behind; within `limit_ns` (the bound of every wait) the output has the same bits and error_code_out is 0. who = 2, 3: a copy of K and V, of Q comes three limits
- * late: waits give up, the kernel returns by itself when the copy has landed, error_code_out is 7, the error is cleared and the next launch is right. */
+/* Self-check of the hand-overs of spyb_paged_attention and spyb_paged_attend, without a fault: the tensor-memory kernel on a small batch of its own, over fp16 pages and over bytes, with one of its roles
+ * late. who = 1: the warps that check values (that make operands of bytes) stay microseconds behind; within `limit_ns` (the bound of every wait) the output has the same bits and error_code_out is 0.
+ * who = 2, 3: a copy of K and V, of Q comes three limits late: waits give up, the kernel returns by itself when the copy has landed, error_code_out is 7, the error is cleared and the next launch is
+ * right. who = 4: the same of a copy of K and V in the kernel for few rows of bytes. */
 spyb_status spyb_paged_selftest_late(spyb_backend *backend, int32_t who, uint64_t limit_ns, int32_t *error_code_out);
 
 /* What the calls above would answer to a descriptor, and why in `message` (up to `size` bytes with the closing 0; may be NULL with size 0): host

@@ -437,7 +437,7 @@ class B200Backend:
             self._check(st)
 
     def paged_selftest_late(self, who: int, limit_ns: int) -> int:
-        """Runs attention over pages with one role of its kernel late (1: the warps that check values, within the limit; 2, 3: a copy of K and V, of Q, beyond it); returns the error code of the waits."""
+        """Runs attention over pages with one role of its kernel late (1: the warps that check values or make operands of bytes, within the limit; 2, 3: a copy of K and V, of Q, beyond it; 4: a copy of the kernel for few rows of bytes); returns the error code of the waits."""
         code = C.c_int32(0)
         self._check(self._l.spyb_paged_selftest_late(self.h, who, limit_ns, C.byref(code)))
         return int(code.value)

@@ -495,20 +495,26 @@ uint64_t spyb_paged_attend_workspace(int32_t n_seq, int32_t n_rows, int32_t n_he
 // the limit of the waits changes nothing; copies that come three limits late make waits give up: the kernel ends by itself, when they have landed, says so, and leaves nothing for
 // the next launch.
 spyb_status spyb_paged_selftest_late(spyb_backend *be, int32_t who, uint64_t limit_ns, int32_t *error_code_out) {
-    if (be == nullptr || limit_ns == 0 || who < PA_LATE_CHECKS || who > PA_LATE_Q) { return SPYB_FAIL; }
+    if (be == nullptr || limit_ns == 0 || who < PA_LATE_CHECKS || who > PA_LATE_FEW) { return SPYB_FAIL; }
     use_device(be->config.device_id);
     SPYB_CUDA(be, cudaStreamSynchronize(be->stream));
     if (be->device_error()) { return SPYB_FAIL; }
-    constexpr int heads = 2, group = 3, page = 16, pages = 1300, rows[2] = {300, 70}, kv[2] = {20000, 70}, n_rows = rows[0] + rows[1];
+    // (few rows: of the kernel for bytes)
+    const bool few = who == PA_LATE_FEW;
+    constexpr int heads = 2, group = 3, page = 16, pages = 1300, kv[2] = {20000, 70};
+    const int rows[2] = {few ? 2 : 300, few ? 1 : 70}, n_rows = rows[0] + rows[1];
     const int32_t words[5] = {0, rows[0], n_rows, kv[0], kv[1]};
     std::vector<int32_t> table(2 * pages);
     for (int i = 0; i < 2 * pages; ++i) { table[i] = i % pages; }
     int code = 0;
-    for (const int hd : {64, 128}) {
+    for (const int which : {0, 1, 2, 3}) {
+        const int  hd = which & 1 ? 128 : 64;
+        const bool bytes = which >= 2;
+        if (few && !bytes) { continue; }
         const size_t n_pool = (size_t)pages * page * heads * hd, n_q = (size_t)n_rows * heads * group * hd;
         std::vector<uint16_t> host(2 * n_pool + n_q);
         uint32_t seed = 1;
-        for (uint16_t &x : host) { seed = seed * 1664525u + 1013904223u; x = (uint16_t)(0x3000 + (seed >> 18) % 0x0c00 + (seed & 0x80000000u ? 0x8000 : 0)); }   // 0.125 to 1, either sign
+        for (uint16_t &x : host) { seed = seed * 1664525u + 1013904223u; x = (uint16_t)(0x3000 + (seed >> 18) % 0x0c00 + (seed & 0x80000000u ? 0x8000 : 0)); }   // 0.125 to 1, either sign (bytes: any, and these numbers as their scales)
         std::vector<float> want(n_q), got(n_q);
         uint8_t *mem = nullptr;
         const size_t at_out = host.size() * 2, at_words = at_out + n_q * 4, at_table = at_words + sizeof words, size = at_table + table.size() * 4;
@@ -516,6 +522,11 @@ spyb_status spyb_paged_selftest_late(spyb_backend *be, int32_t who, uint64_t lim
         spyb_paged_attention_desc d = {};
         d.cache.k = mem; d.cache.v = mem + n_pool * 2; d.cache.number_type = SPYB_FP16; d.cache.n_pages = pages; d.cache.page_size = page; d.cache.n_head_kv = heads; d.cache.head_dim = hd;
         d.cache.page_stride = page * heads * hd; d.cache.token_stride = heads * hd; d.cache.head_stride = hd;
+        spyb_paged_scales scales = {};
+        if (bytes) {                                          // (both pools of bytes in the place of the one of K in fp16, scales in V's)
+            d.cache.number_type = SPYB_INT8; d.cache.v = mem + n_pool;
+            scales.pairs = mem + n_pool * 2; scales.page_stride = page * heads; scales.token_stride = heads; scales.head_stride = 1;
+        }
         d.batch.row_start = reinterpret_cast<int32_t *>(mem + at_words); d.batch.n_kv = d.batch.row_start + 3; d.batch.page_table = reinterpret_cast<int32_t *>(mem + at_table);
         d.batch.n_seq = 2; d.batch.n_rows = n_rows; d.batch.table_stride = pages;
         d.q = mem + n_pool * 4; d.out = mem + at_out; d.q_stride = d.out_stride = heads * group * hd; d.n_head = heads * group; d.out_type = SPYB_FP32; d.causal = 1;
@@ -525,7 +536,7 @@ spyb_status spyb_paged_selftest_late(spyb_backend *be, int32_t who, uint64_t lim
         spyb_status st = SPYB_SUCCESS;
         auto run = [&](int late, uint64_t limit, std::vector<float> &to) {
             if (err == cudaSuccess) { err = cudaMemsetAsync(d.out, 0xff, n_q * 4, be->stream); }
-            if (err == cudaSuccess && st == SPYB_SUCCESS) { st = paged_attention(be, d, late, limit); }
+            if (err == cudaSuccess && st == SPYB_SUCCESS) { st = paged_attention(be, d, late, limit, bytes ? &scales : nullptr); }
             if (err == cudaSuccess) { err = cudaMemcpyAsync(to.data(), d.out, n_q * 4, cudaMemcpyDeviceToHost, be->stream); }
             if (err == cudaSuccess) { err = cudaStreamSynchronize(be->stream); }   // returns: the kernels ended by themselves
             return be->clear_device_error();
@@ -538,8 +549,8 @@ spyb_status spyb_paged_selftest_late(spyb_backend *be, int32_t who, uint64_t lim
         SPYB_CUDA(be, err);
         if (st != SPYB_SUCCESS) { return st; }
         if (error_code_out != nullptr) { *error_code_out = code; }
-        if (before != 0 || code != expected || after != 0) { be->set_error("paged selftest: heads of %d: codes %d, %d, %d where 0, %d, 0 were expected", hd, before, code, after, expected); return SPYB_FAIL; }
-        if (std::memcmp(want.data(), got.data(), n_q * 4) != 0) { be->set_error("paged selftest: heads of %d: a late role changed the output, its own or the next launch's", hd); return SPYB_FAIL; }
+        if (before != 0 || code != expected || after != 0) { be->set_error("paged selftest: heads of %d%s: codes %d, %d, %d where 0, %d, 0 were expected", hd, bytes ? " in bytes" : "", before, code, after, expected); return SPYB_FAIL; }
+        if (std::memcmp(want.data(), got.data(), n_q * 4) != 0) { be->set_error("paged selftest: heads of %d%s: a late role changed the output, its own or the next launch's", hd, bytes ? " in bytes" : ""); return SPYB_FAIL; }
     }
     return SPYB_SUCCESS;
 }

@@ -23,8 +23,9 @@ struct PagedAppend {
     int          n_head = 0, n_head_kv = 0, head_dim = 0, rot = 0, halves = 0;
     double       turns[128] = {};         // pair i turns by this share of a full circle a position
 };
-// the warps that check V stay a few microseconds behind everything else; one copy of a CTA's K and V, or its first of Q, comes three limits of the waits late
-enum PagedLate { PA_ON_TIME = 0, PA_LATE_CHECKS = 1, PA_LATE_KV = 2, PA_LATE_Q = 3 };
+// the warps that check V (that make operands of bytes) stay a few microseconds behind everything else; one copy of a CTA's K and V, or its first of Q, comes three limits of the waits late; the same of a
+// copy of K and V in the kernel for few rows of bytes
+enum PagedLate { PA_ON_TIME = 0, PA_LATE_CHECKS = 1, PA_LATE_KV = 2, PA_LATE_Q = 3, PA_LATE_FEW = 4 };
 // What a kernel of attention is built for: an fp16 cache whose sequences have nothing in common; one of the two passes where they have; bytes with scales, in passes or not
 enum PagedKind { PK_PLAIN = 0, PK_SHARED = 1, PK_INT8 = 2 };
 struct PagedScales { const uint32_t *pairs = nullptr; int64_t page_stride = 0, token_stride = 0, head_stride = 0; };   // fp16 pairs: K's scale below, V's above
@@ -41,7 +42,7 @@ struct PagedAttention {
     int          few_rows = 0;            // sequences of up to so many rows (of all query heads of a K/V head) are the small kernel's
     float       *partial = nullptr;       // [CTAs][2][rows of a tile][head_dim + 2]
     unsigned    *arrived = nullptr;       // [CTAs], zero between launches
-    int          late = PA_ON_TIME;       // self-checks of the tensor-memory kernel
+    int          late = PA_ON_TIME;       // self-checks of the tensor-memory kernel and of the one for few rows of bytes
     PagedScales  scales;                  // of an 8-bit cache
     float2      *stats = nullptr;         // first pass of two, over what sequences share: every row's maximum and sum go here, its accumulators as they are to `out` (f32), both [row][head]
     int2        *cuts = nullptr;          // of the first pass on tensor memory, by K/V head and first row of a tile: first CTA and number of CTAs of its item. Several leave their findings where they are

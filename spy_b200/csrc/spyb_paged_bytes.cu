@@ -77,6 +77,11 @@ __device__ __forceinline__ float over_groups(float v, bool largest) {   // over 
 }
 
 __device__ __forceinline__ void sts64(uint32_t addr, uint2 v) { asm volatile("st.shared.v2.u32 [%0], {%1,%2};" ::"r"(addr), "r"(v.x), "r"(v.y) : "memory"); }
+constexpr uint64_t PB_LANDING_NS = 1000000000;      // copies have this long to land (whatever the limit of the waits)
+__device__ __noinline__ void stand_still(uint64_t ns) {
+    const uint64_t t0 = global_timer_ns();
+    for (int i = 0; i < (1 << 22) && global_timer_ns() - t0 < ns; ++i) { __nanosleep(200); }
+}
 __device__ __forceinline__ void tma_pages(uint32_t dst, const CUtensorMap *map, uint32_t bar, int token, int head, int page) {
     asm volatile("cp.async.bulk.tensor.4d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3,%4,%5,%6}], [%2];"
                  ::"r"(dst), "l"(map), "r"(bar), "r"(0), "r"(token), "r"(head), "r"(page) : "memory");
@@ -153,6 +158,7 @@ __global__ void __launch_bounds__(PB_THREADS, BytesSmem<HD, NT>::CTAS) paged_byt
             for (int s = 0; s < n_stage; ++s) {
                 mbar_wait_lean(empty + 8 * stage, phase ^ 1, limit);
                 if (!__all_sync(0xffffffffu, limit != 0)) { limit = 0; break; }
+                if (p.late == PA_LATE_FEW && issued == 2) { stand_still(3 * wait_limit); }   // (the self-check's: issued all the same, with nobody waiting any more)
                 const uint32_t bar = full + 8 * stage, dst = ring + stage * Shape::STAGE;
                 int in[2], at[2];
                 bool ok[2];
@@ -212,14 +218,13 @@ __global__ void __launch_bounds__(PB_THREADS, BytesSmem<HD, NT>::CTAS) paged_byt
             more = at.unit < at.end && paged_next(p, true, q, seq, head, tile);
         }
         if (limit != 0) { const BytesEntry over = {}; put(over); }
-        if (limit == 0) {                     // what is still on its way lands before the CTA ends
-            if (lane == 0) { pf_report(error_flag, 7); }
-            uint64_t again = 1000000000;
-            for (uint32_t i = 0; i < STAGES && i < issued; ++i) {
-                if (stage == 0) { stage = STAGES; phase ^= 1; }
-                --stage;
-                mbar_wait_lean(full + 8 * stage, phase, again);
-            }
+        // What is on its way lands before the CTA ends, also where those who waited for it have given up
+        if (limit == 0 && lane == 0) { pf_report(error_flag, 7); }
+        uint64_t again = PB_LANDING_NS;
+        for (uint32_t i = 0; i < STAGES && i < issued; ++i) {
+            if (stage == 0) { stage = STAGES; phase ^= 1; }
+            --stage;
+            mbar_wait_lean(full + 8 * stage, phase, again);
         }
         return;
     }
