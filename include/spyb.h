@@ -310,7 +310,7 @@ typedef struct {
 } spyb_paged_scales;
 
 /* spyb_paged_append with a norm of every head of Q and K in front of the rotation, into a cache of SPYB_FP16 or SPYB_INT8: x -> x / sqrt(mean of x^2 + norm_eps) * weight (NormRMS and Mul,
- * orchestration/include/operator/non-linear.h:117, over a head's elements). q_norm, k_norm: f32 [head_dim], the same for all heads; NULL leaves a norm out. norm_eps: not negative.
+ * orchestration/include/operator/non-linear.h:117, over a head's elements). q_norm, k_norm: f32 [head_dim], 16-byte aligned, the same for all heads; NULL leaves a norm out. norm_eps: not negative.
  * Everything is held in f32 (angles in 64 bits) and rounded once. `scales` is of SPYB_INT8 caches, and not read otherwise. The rest is spyb_paged_append's. */
 typedef struct {
     spyb_paged_append_desc append;

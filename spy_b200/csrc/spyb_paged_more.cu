@@ -92,7 +92,7 @@ __global__ void __launch_bounds__(ST_THREADS, 4) paged_store_kernel(const __grid
         }
         const int64_t to = head.is_q ? (int64_t)row0 * p.q_out_stride + (int64_t)head.hh * p.head_dim : head.hh * p.view.head_stride;
         for (int r = 0; r < rows; ++r) {
-            float ahead[8];
+            float ahead[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};   // (a lane without elements takes part in its head's sum and maximum with zeros)
             fetch(head, r + 1, ahead);
             const StorePlace at = places[r];
             if (some_norm) {
@@ -153,6 +153,8 @@ __global__ void __launch_bounds__(ST_THREADS, 4) paged_store_kernel(const __grid
         h0 += slots * gridDim.y;
         if (h0 >= total) { break; }
         head = head_of(h0 + slot);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) { x[i] = 0.f; }
         fetch(head, 0, x);
     }
 }
@@ -194,7 +196,7 @@ __global__ void __launch_bounds__(LD_THREADS) paged_load_kernel(const __grid_con
                     if constexpr (EIGHT) {
                         const uint2 y = __ldcs(reinterpret_cast<const uint2 *>(static_cast<const uint8_t *>(is_v ? p.v : p.k) + cell[k] + in));
                         w[k].x = y.x; w[k].y = y.y;
-                        pair[k] = __ldg(p.scales.pairs + pairs[r] + of_pair);
+                        pair[k] = p.scales.pairs[pairs[r] + of_pair];
                     } else { w[k] = __ldcs(reinterpret_cast<const uint4 *>(static_cast<const __half *>(is_v ? p.v : p.k) + cell[k] + in)); }
                 }
             }
@@ -349,7 +351,7 @@ cudaError_t launch_paged_store(const PagedStore &p, int in_type, int q_out_type,
     return q_out_type == SPYB_FP32 ? launch_store<__half, float>(p, sms, cfg) : launch_store<__half, __half>(p, sms, cfg);
 }
 cudaError_t launch_paged_load(const PagedLoad &p, int out_type, int sms, const LaunchCfg &cfg) {
-    // (few rows: on as many CTAs as there are, 1 of 300: 5.2 us with eight rows each, 8.6 with 32)
+    // (few rows: on as many CTAs as there are. 1 of 300, before the loads were made together: 5.2 us with eight rows each, 8.6 with 32; 4.1 now)
     return p.view.n_rows >= 32 * 4 * sms ? launch_load<32>(p, out_type, cfg) : launch_load<8>(p, out_type, cfg);
 }
 cudaError_t launch_paged_shared(const PagedShared &p, const LaunchCfg &cfg) {

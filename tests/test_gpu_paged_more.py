@@ -181,6 +181,16 @@ def test_store_many_sequences_and_other_strides(be, dev):
     check_store(be, dev, rng, [7, 50], [100, 50], 4, 2, 64, 16, True, strides=(16 * 2 * 96 + 48, 80 + 80, 80), scale_strides=(16 * 7 + 3, 7, 3))
 
 
+@pytest.mark.parametrize("hd", [24, 40, 96, 200])
+@pytest.mark.parametrize("eight", [False, True])
+def test_store_heads_that_fill_no_power_of_two_in_several_rows_of_a_block(be, dev, hd, eight):
+    rng = np.random.default_rng(hd)
+    one = (hd + 15) // 16 * 16                                                              # (strides of bytes are multiples of 16)
+    strides = lambda n: (16 * n * one, n * one, one) if eight else None  # noqa: E731
+    check_store(be, dev, rng, [1300, 0, 1], [1350, 0, 9], 5, 2, hd, 16, eight, mode=B.ROPE_PAIRS, strides=strides(2))
+    check_store(be, dev, rng, [900], [900], 30, 12, hd, 16, eight, mode=B.ROPE_HALVES, strides=strides(12))      # (several turns of heads, the last one of few)
+
+
 def test_store_heads_of_all_kinds(be, dev):
     """Zeros, one value, the smallest numbers, the largest that bytes take and the next, infinities and NaN; what is read back, and what is kept."""
     hd = 64
