@@ -7,6 +7,11 @@
 //   16-byte pieces: the products' inner order is the lane's own, the same for Q, whose elements it reads alike, and V's elements are where the accumulators' rows are.
 //   Scales stay out of the products' operands: K's multiply scores (where scale and log2 e are a product anyway), V's the probabilities, in f32. So that no probability leaves fp16's range,
 //   V's scales are taken against the largest so far, rounded up to a power of two; like the maximum of the scores it moves a few times at the start and hardly ever after.
+// Measured (heads of 128): 64 single tokens of up to 4096 positions, 32 query heads on 8 (277 MB), 60 us, 4.6 TB/s (heads of 64 51 us); three of 100 000, 40 on 8, 115 us, 5.3 TB/s, by head 106; one of 4000, 32 on 32 (33 MB),
+// 15 us. Single tokens' loop runs at the memory's rate; beside it 7 us until the first stage is there (lengths, the plan, page table, bytes, one after the other) and 4 us for every item that is done, joins among them.
+// Five rows of 24 sequences of up to 9000 (tiles of 24 rows) 118 us: 1.7 us a stage of 64 positions, a warp's chain of products and conversions with eight warps an SM (168 registers), and 5 us for a join.
+// Slower: K by mma.sync on bytes, with Q as two bytes of a 16-bit number; bytes as 2^-24 times themselves with their 128 taken off the sums (8 %); 32 positions a warp at a time; two chains of scores; rings of four stages;
+// what the warps found added up one after the other (61 -> 68 us); joins of two and four pieces of four elements at once (the same, and 2 %).
 
 #include <cuda.h>
 
@@ -89,6 +94,8 @@ __device__ __forceinline__ void tma_pages(uint32_t dst, const CUtensorMap *map, 
 __device__ __forceinline__ void arrive_when_copied(uint32_t bar) { asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory"); }   // of this lane's copies so far
 // A CTA's part of an item, found by the copying warp for all: rows of the tile, stages of the ring, positions [ka, kb); rows 0: behind the last one
 struct BytesEntry { int rows, n_stage, ka, kb, tile, head, row0, first, from, c0, parts; };
+// What probabilities and V's scales are taken against follows when a score is 2^PB_SLACK above it, a scale PB_SLACK_SCALE times it: products up to 2^15 are as exact in fp16 as those below 1
+constexpr float PB_SLACK = 11.f, PB_SLACK_SCALE = 16.f;
 constexpr int PB_ENTRIES = 4;                 // known ahead
 
 // One warp copies for four that compute (with each its own copies a block's took a third of the warp's time on it: some hundred instructions of addresses).
@@ -315,47 +322,45 @@ __global__ void __launch_bounds__(PB_THREADS, BytesSmem<HD, NT>::CTAS) paged_byt
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        float &x = sc[n][e];
-                        x = fmaf(x, k_scale[e >> 1], -base[n][e & 1]);
+                    for (int i = 0; i < 4; ++i) {
+                        float &x = sc[n][i];
+                        x = fmaf(x, k_scale[i >> 1], -base[n][i & 1]);
                         if (!whole) {
-                            const int jj = g + (e >> 1) * 8, d = pos[n][e & 1] - (j0 + jj);
+                            const int jj = g + (i >> 1) * 8, d = pos[n][i & 1] - (j0 + jj);
                             const bool seen = ((mask >> jj) & 1) && (!p.causal || (d >= 0 && (p.window <= 0 || d < p.window)));
                             x = seen ? x : -CUDART_INF_F;
                         }
-                        above |= x > over[n][e & 1];
+                        above |= x > over[n][i & 1];
                     }
                 }
 #pragma unroll
-                for (int e = 0; e < 2; ++e) { v_scale[e] *= unit; above |= !(fabsf(v_scale[e]) <= 1.f); }
+                for (int i = 0; i < 2; ++i) { v_scale[i] *= unit; above |= !(fabsf(v_scale[i]) <= PB_SLACK_SCALE); }
             }
             if (__any_sync(0xffffffffu, above)) {
                 float most = 1.f;
                 bool  fine = true;
-                {
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) { const bool is = fabsf(v_scale[e]) < CUDART_INF_F; fine &= is; most = fmaxf(most, is ? fabsf(v_scale[e]) : 1.f); }
-                }
+                for (int i = 0; i < 2; ++i) { const bool is = fabsf(v_scale[i]) < CUDART_INF_F; fine &= is; most = fmaxf(most, is ? fabsf(v_scale[i]) : 1.f); }
                 odd = !__all_sync(0xffffffffu, fine);
                 most = over_groups(most, true);
                 const uint32_t up = (__float_as_uint(most) + 0x7fffffu) & 0x7f800000u;      // the next power of two, 2^56 at most
                 const float f_scale = __uint_as_float(0x7f000000u - up);                    // one over it
                 unit *= f_scale;
-                { v_scale[0] *= f_scale; v_scale[1] *= f_scale; }
+                v_scale[0] *= f_scale; v_scale[1] *= f_scale;
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        float v = fmaxf(sc[n][e], sc[n][2 + e]);
+                    for (int i = 0; i < 2; ++i) {
+                        float v = fmaxf(sc[n][i], sc[n][2 + i]);
                         v = over_groups(v, true);
-                        const float to = v > over[n][e] ? fmaxf(mx[n][e], base[n][e] + v) : mx[n][e], f = to == mx[n][e] ? 1.f : ex2(mx[n][e] - to);   // (2^-inf = 0 at the first)
-                        const float from = base[n][e], f_o = f * f_scale;
-                        mx[n][e] = to; sum[n][e] *= f;
-                        base[n][e] = to == -CUDART_INF_F ? 0.f : to;
-                        over[n][e] = to == -CUDART_INF_F ? to : 8.f;
-                        { sc[n][e] += from - base[n][e]; sc[n][2 + e] += from - base[n][e]; }
+                        const float to = v > over[n][i] ? fmaxf(mx[n][i], base[n][i] + v) : mx[n][i], f = to == mx[n][i] ? 1.f : ex2(mx[n][i] - to);   // (2^-inf = 0 at the first)
+                        const float from = base[n][i], f_o = f * f_scale;
+                        mx[n][i] = to; sum[n][i] *= f;
+                        base[n][i] = to == -CUDART_INF_F ? 0.f : to;
+                        over[n][i] = to == -CUDART_INF_F ? to : PB_SLACK;
+                        sc[n][i] += from - base[n][i]; sc[n][2 + i] += from - base[n][i];
 #pragma unroll
-                        for (int i = 0; i < HD / 16; ++i) { o[n][i][e] *= f_o; o[n][i][2 + e] *= f_o; }
+                        for (int k = 0; k < HD / 16; ++k) { o[n][k][i] *= f_o; o[n][k][2 + i] *= f_o; }
                     }
                 }
             }
@@ -416,7 +421,7 @@ __global__ void __launch_bounds__(PB_THREADS, BytesSmem<HD, NT>::CTAS) paged_byt
         meet();
         const RowsDone what = {e.rows, e.tile, e.row0, e.head, e.from};
         rows_finish<HD, ROWS, PK_INT8, PR_WARPS>(p, PagedCut{e.c0, e.parts}, what, mo, mm, ml, ROWS, last_one, meet);
-        meet();                 // (the findings' place is free again)
+        meet();                               // (the findings' place is free again)
     }
     if (limit == 0 && lane == 0) { pf_report(error_flag, 7); }
 }
