@@ -348,7 +348,8 @@ typedef struct {
 } spyb_paged_shared;
 
 /* spyb_paged_attention over a cache of SPYB_FP16 or SPYB_INT8, with what sequences share read once for all of them. For SPYB_INT8 scores are
- * multiplied by K's scales and probabilities by V's in f32; a probability times a scale is rounded to fp16 in front of the second product, against the largest scale met. A row that sees nothing is zeros; what is not seen has no influence, scales of any value included. */
+ * multiplied by K's scales and probabilities by V's in f32; a probability times a scale is rounded to fp16 in front of the second product, against the largest scale met, which is that of
+ * all rows of a sequence that are read together. A row that sees nothing is zeros; what is not seen has no influence but by that, infinite and NaN scales none at all. */
 typedef struct {
     spyb_paged_attention_desc attention;
     spyb_paged_scales scales;

@@ -153,6 +153,7 @@ __global__ void __launch_bounds__(PB_THREADS, BytesSmem<HD, NT>::CTAS) paged_byt
             if (!put(e)) { break; }
             const int32_t *table = p.view.page_table + (int64_t)seq * p.view.table_stride;
             const uint32_t *pairs = p.scales.pairs + head * p.scales.head_stride;
+            const int seen_from = p.causal && p.window > 0 ? q.first + (int)((unsigned)(tile * ROWS) / (unsigned)p.group) - p.window + 1 : 0;   // what nobody sees is not there, its scales neither
             int page[2];                                      // of this lane's two positions of a stage, read a stage ahead. (No branch around the loads, or they are waited for where they stand)
             auto find = [&](int s) {
 #pragma unroll
@@ -168,7 +169,7 @@ __global__ void __launch_bounds__(PB_THREADS, BytesSmem<HD, NT>::CTAS) paged_byt
                 if (p.late == PA_LATE_FEW && issued == 2) { stand_still(3 * wait_limit); }   // (the self-check's: issued all the same, with nobody waiting any more)
                 const uint32_t bar = full + 8 * stage, dst = ring + stage * Shape::STAGE;
                 int in[2], at[2];
-                bool ok[2];
+                bool ok[2], seen[2];
                 unsigned mask[2];
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
@@ -176,7 +177,8 @@ __global__ void __launch_bounds__(PB_THREADS, BytesSmem<HD, NT>::CTAS) paged_byt
                     in[i] = p.page_shift >= 0 ? j & (p.view.page_size - 1) : j % p.view.page_size;
                     at[i] = page[i];
                     ok[i] = j < kb && at[i] >= 0 && at[i] < p.view.n_pages;
-                    mask[i] = __ballot_sync(0xffffffffu, ok[i]);
+                    seen[i] = ok[i] && j >= seen_from;
+                    mask[i] = __ballot_sync(0xffffffffu, seen[i]);
                 }
                 if (s + 1 < n_stage) { find(s + 1); }
                 if (lane == 0) {
@@ -185,7 +187,7 @@ __global__ void __launch_bounds__(PB_THREADS, BytesSmem<HD, NT>::CTAS) paged_byt
                 }
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
-                    cp_async4(scales + (stage * PB_STAGE + 32 * i + lane) * 4, pairs + (ok[i] ? at[i] * p.scales.page_stride + in[i] * p.scales.token_stride : 0), ok[i]);
+                    cp_async4(scales + (stage * PB_STAGE + 32 * i + lane) * 4, pairs + (seen[i] ? at[i] * p.scales.page_stride + in[i] * p.scales.token_stride : 0), seen[i]);
                 }
                 if constexpr (MAPS) {
                     __syncwarp();

@@ -458,6 +458,21 @@ def test_bytes_scales_that_are_not_finite_reach_only_who_sees_them(be, dev, rows
     assert not np.isfinite(got[sees_v][:, :2]).all(axis=2).any() and not np.isfinite(got[sees_k][:, 2:]).all(axis=2).any()
 
 
+@pytest.mark.parametrize("rows", [1, 2, 6, 100])
+@pytest.mark.parametrize("hd", [32, 64, 128])
+def test_bytes_the_largest_scale_in_front_of_the_window_has_no_influence(be, dev, rows, hd):
+    rng = np.random.default_rng(rows + hd)
+    n, h, h_kv, window = 230 + rows, 4, 2, 90
+    pool = BytePool(rng, [n], h_kv, hd, 16)
+    k, v = pool.put(0, *rng.standard_normal((2, n, h_kv, hd)))
+    q = rng.standard_normal((rows, h, hd)).astype(np.float16)
+    out0 = np.zeros(q.shape, dtype=np.float32)
+    before = attend(be, dev, pool, [0, rows], q, out0, window=window)
+    for j in range(n - rows - window + 1):
+        pool.scale_view()[pool.table[0, j // 16], j % 16] = 65504
+    assert np.array_equal(before, attend(be, dev, pool, [0, rows], q, out0, window=window))
+
+
 def test_bytes_whole_chip_on_one_head_and_cut_items(be, dev):
     rng = np.random.default_rng(5)
     check_attend(be, dev, rng, [1], [40000], 2, 1, 64, 64, max_rows=1)
