@@ -405,7 +405,7 @@ static spyb_status paged_attention(spyb_backend *be, const spyb_paged_attention_
         if (on_tensor_memory) {
             PagedSharedJoin j;
             j.view = p.view; j.from = g.from; j.lead = g.lead; j.cuts = first.cuts; j.partial = be->paged_partial; j.out = static_cast<float *>(first.out); j.stats = first.stats;
-            j.n_head_kv = p.n_head_kv; j.group = p.group;
+            j.n_head_kv = p.n_head_kv; j.group = p.group; j.ctas = be->num_sms_total;
             SPYB_CUDA(be, launch_paged_shared_join(j, hd, be->launch_cfg(be->config.use_pdl != 0)));
         }
         p.view.from = g.from; p.with_stats = first.stats; p.with_out = static_cast<const float *>(first.out);

@@ -78,7 +78,7 @@ struct PagedSharedJoin {                  // cut items of the first pass on tens
     const float   *partial = nullptr;
     float         *out = nullptr;
     float2        *stats = nullptr;
-    int            n_head_kv = 0, group = 1;
+    int            n_head_kv = 0, group = 1, ctas = 0;               // ctas: of the first pass
 };
 constexpr int PA_SHARED = 128;            // fewer positions than that are not shared
 // A sequence's own positions begin where a box of the kernels' tensor maps and a block of 16 do: at a multiple of the largest power of two that divides the page size, 16 to 128

@@ -223,6 +223,8 @@ __global__ void __launch_bounds__(LD_THREADS) paged_load_kernel(const __grid_con
 
 // ---------------------------------------------------------------------------------------------- who shares what
 // A warp for each sequence: its group, what all of the group's sequences that have rows see whole, and the first of these, which stands for all in the first pass.
+// Groups and beginnings of rows are the caller's, on the device: where they are not ascending, a sequence may find a group that its first sequence is not in, or have rows that are not among that one's in the
+// first pass. Such a sequence shares nothing, so that a row whose sequence has a `from` is a row of the first pass.
 constexpr int SH_WARPS = 8;
 __global__ void __launch_bounds__(SH_WARPS * 32) paged_shared_kernel(const __grid_constant__ PagedShared p) {
     pdl_launch_dependents();
@@ -253,6 +255,11 @@ __global__ void __launch_bounds__(SH_WARPS * 32) paged_shared_kernel(const __gri
             with_rows += __shfl_xor_sync(0xffffffffu, with_rows, o);
         }
         common = with_rows > 1 && common >= PA_SHARED ? common / p.align * p.align : 0;
+        if (common > 0) {                                           // (the same for all lanes)
+            const int32_t *start = p.view.row_start;
+            const int end = start[group_end];
+            if (sequence_of(groups, leader) != g || start[leader + 1] > end || start[s] < start[leader] || start[s + 1] > end) { common = 0; }
+        }
     }
     if (lane == 0) {
         const int begin = p.view.row_start[s];
@@ -283,7 +290,7 @@ __global__ void __launch_bounds__(SJ_WARPS * 32) paged_shared_join_kernel(const 
     const int lead = max(0, p.lead[s]), tokens = SJ_TILE / p.group, half = (int)((unsigned)(row - lead) / (unsigned)tokens), first = lead + half * tokens;
     if (row < lead) { return; }                                     // (no group that makes sense)
     const int2 cut = p.cuts[(int64_t)kv * p.view.n_rows + first];
-    if (cut.y < 2) { return; }
+    if (cut.y < 2 || cut.x < 0 || cut.x > p.ctas - cut.y) { return; }   // (a pass that gave up may have left any word there; pieces are read from places of CTAs alone)
     const int r = (row - first) * p.group + head - kv * p.group;
     constexpr int PIECE = SJ_TILE * (HD + 2), FOURS = HD / 64;      // of a lane: four elements, 64 apart
     const float *const place = p.partial + (half & 1) * PIECE;

@@ -1,0 +1,155 @@
+"""GPU: the operators over 8-bit pages and shared beginnings under bounds that scale with what each row sees, and at the inputs where their roundings go wrong first.
+
+Tolerances of attention (`close_attention`): what is rounded to fp16 in front of the second product are the weights w_j = 2^(s_j - m) v_scale_j (fp16 pages: v_scale = 1), m at most the largest
+s_j + log2(v_scale_j) of the positions that the row sees; a rounding is off by 2^-11 of the weight, and by 2^-25 among fp16's smallest numbers, that is 2^-25 of the row's largest contribution."""
+import numpy as np
+import pytest
+
+from spy_b200 import backend as B
+from test_gpu_paged import Device, Pool, be, dev  # noqa: F401
+from test_gpu_paged_more import BytePool, attend
+
+pytestmark = pytest.mark.gpu
+
+
+def close_attention(q, kb, vb, sk, sv, first, scale, causal, window, there):
+    """q [rows][heads][e]; kb, vb [positions][kv heads][e] and their scales [positions][kv heads], f64. The output, and how far the kernels may be from it (without the output's own rounding)."""
+    rows, h, hd = q.shape
+    n, h_kv, _ = kb.shape
+    out, off = np.zeros(q.shape), np.zeros(q.shape)
+    per = scale / np.log(2)
+    for g in range(h_kv):
+        heads = np.arange(g * (h // h_kv), (g + 1) * (h // h_kv))
+        s_all = np.einsum("rhe,ne->rhn", q[:, heads], kb[:, g]) * (sk[:, g] * per)
+        a_all = np.einsum("rhe,ne->rhn", np.abs(q[:, heads]), np.abs(kb[:, g])) * np.abs(sk[:, g] * per)
+        for i in range(rows):
+            j = np.arange(n)
+            seen = there.copy()
+            if causal:
+                seen &= j <= first + i
+                if window:
+                    seen &= j > first + i - window
+            if not seen.any():
+                continue
+            v, v_scale = vb[seen, g], np.abs(sv[seen, g])
+            for x, head in enumerate(heads):
+                s, a = s_all[i, x, seen], a_all[i, x, seen]
+                p = np.exp2(s - s.max())
+                w = p * v_scale
+                top = (p * np.maximum(v_scale, 2.0 ** -24)).max()
+                # an exponent: head_dim exact products summed in f32 (a truncation each: 2^-23 of the sum of magnitudes), by a scale that is rounded three times, beside a maximum that is moved up a few times
+                d = np.log(2) * (hd * 2.0 ** -23 * a + 8 * 2.0 ** -24 * (np.abs(s) + np.abs(s).max() + 40))
+                # weights to fp16; powers of two and joins; f32 sums, 16 terms a step
+                rel = 2.0 ** -11 + 2.0 ** -20 + (len(s) / 16 + 60) * 2.0 ** -23
+                out[i, head] = (p * sv[seen, g]) @ v / p.sum()
+                off[i, head] = ((rel + d) * w) @ np.abs(v) + 2.0 ** -25 * top * np.abs(v).sum(0) + np.abs(out[i, head]) * (d @ p + rel * p.sum())
+                off[i, head] /= p.sum()
+    return out, off
+
+
+def held(pool, s, n):
+    """What pages hold of a sequence: whole numbers (or values) and scales of K and V, and which positions are there."""
+    pos = np.arange(n)
+    pages = pool.table[s, pos // pool.page]
+    there = (pages >= 0) & (pages < pool.n_pages)
+    at = (np.where(there, pages, 0), pos % pool.page)
+    k, v = (np.where(there[:, None, None], pool.view(x)[at], 0).astype(np.float64) for x in (pool.k, pool.v))
+    if not isinstance(pool, BytePool):
+        return k, v, np.ones(k.shape[:2]), np.ones(k.shape[:2]), there
+    sc = np.where(there[:, None, None], pool.scale_view()[at], 0).astype(np.float64)
+    return k, v, sc[..., 0], sc[..., 1], there
+
+
+def check_close(got, pool, starts, rows, q, scale=None, causal=True, window=0, room=None, show=None):
+    """All rows of all sequences; `room`: the largest share of a typical output that the bound may be, so that it says something."""
+    hd = q.shape[2]
+    for s, n in enumerate(pool.n_kv):
+        a, b = starts[s], starts[s + 1]
+        if b == a:
+            continue
+        want, off = close_attention(q[a:b].astype(np.float64), *held(pool, s, n)[:4], n - rows[s], hd ** -0.5 if scale is None else scale, causal, window, held(pool, s, n)[4])
+        if room is not None:
+            assert np.median(off) <= room * np.sqrt((want ** 2).mean()), (float(np.median(off)), float(np.sqrt((want ** 2).mean())))
+        tol = off + (np.abs(want) * 2.0 ** -11 + 2.0 ** -25 if got.dtype == np.float16 else np.abs(want) * 2.0 ** -24)
+        err = np.abs(got[a:b].astype(np.float64) - want)
+        assert (err <= tol).all(), (s, float((err / np.maximum(tol, 1e-300)).max()), np.unravel_index(np.argmax(err / np.maximum(tol, 1e-300)), err.shape))
+
+
+def make_pool(rng, n_kv, h_kv, hd, page, eight=True, sizes=0.5, token_major=False, groups=None):
+    pool = BytePool(rng, n_kv, h_kv, hd, page, token_major) if eight else Pool(rng, n_kv, h_kv, hd, page, token_major)
+    x = [rng.standard_normal((2, n, h_kv, hd)) * np.exp(sizes * rng.standard_normal((2, n, h_kv, 1))) for n in n_kv]
+    for g, n in enumerate(groups[1] if groups else []):
+        a, b = groups[0][g], groups[0][g + 1]
+        longest = max(range(a, b), key=lambda i: n_kv[i])
+        for i in range(a, b):
+            m = min(n, n_kv[i])
+            x[i][:, :m] = x[longest][:, :m]
+            pool.table[i, :m // page] = pool.table[longest, :m // page]
+    for s in range(len(n_kv)):
+        pool.put(s, *(x[s].astype(np.float16)))
+    return pool
+
+
+# ---------------------------------------------------------------------------------------------- shared beginnings
+@pytest.mark.parametrize("eight", [False, True])
+@pytest.mark.parametrize("shared", [128, 290, 299, 300, 500, 100000])
+@pytest.mark.parametrize("rows", [1, 2, 12])
+def test_what_is_shared_is_cut_to_what_all_rows_see(be, dev, eight, shared, rows):
+    """The shortest sequence of three has 300 positions in front of its rows: of more than that only these are shared, whatever the caller says."""
+    rng = np.random.default_rng(shared + rows)
+    for hd, page, causal in ((64, 16, True), (128, 24, True), (96, 16, True), (128, 32, False)):
+        n_kv, starts = [900 + rows, 300 + rows, 640 + rows], [0, rows, 2 * rows, 3 * rows]
+        pool = make_pool(rng, n_kv, 2, hd, page, eight, groups=([0, 3], [min(shared, 900)]))
+        q = rng.standard_normal((3 * rows, 4, hd)).astype(np.float16)
+        got = attend(be, dev, pool, starts, q, np.zeros(q.shape, dtype=np.float32), ([0, 3], [shared]), causal=causal)
+        check_close(got, pool, starts, [rows] * 3, q, causal=causal, room=0.05)
+
+
+@pytest.mark.parametrize("eight", [False, True])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_groups_of_any_order_give_what_no_groups_give(be, dev, eight, hd):
+    """Rows enough for the kernel on tensor memory in the first pass, sequences whose first 304 positions are all the same, and groups that are not ascending, overlap or leave the batch: whatever is
+    made of them, what a row sees does not change, and nothing outside the described buffers is touched."""
+    rng = np.random.default_rng(hd)
+    n_seq, rows, h, h_kv, common = 6, 9, 4, 2, 304
+    n_kv = [common + rows + 50 * i for i in range(n_seq)]
+    pool = make_pool(rng, n_kv, h_kv, hd, 16, eight, groups=([0, n_seq], [common]))
+    starts = np.arange(n_seq + 1) * rows
+    q = rng.standard_normal((n_seq * rows, h, hd)).astype(np.float16)
+    size = B.paged_attend_workspace(n_seq, n_seq * rows, h, hd)
+    margin = np.full((3 * n_seq * rows, h, hd), 3.0, dtype=np.float32)
+    po = dev(margin)
+    b = B.paged_batch(dev(starts.astype(np.int32)), dev(np.array(n_kv, np.int32)), dev(pool.table), n_seq, n_seq * rows, pool.table.shape[1])
+    a = B.paged_attention_desc(pool.cache(dev(pool.k), dev(pool.v)), b, dev(q), po + n_seq * rows * h * hd * 4, h, out_type=B.FP32)
+    sc = pool.of_scales(dev(pool.scales)) if eight else None
+    kinds = [[2, 0, 6], [0, 2, 1, 6], [0, 4, 2, 6], [5, 1, 3], [-7, 3, 2, 90], [6, 5, 4, 3, 2, 1, 0], [0, 0, 6, 6], [1, 6, 0, 4, 2, 9], [0, 1 << 30], [0, 6]] + [rng.integers(-2, 9, 5).tolist() for _ in range(12)]
+    for start in kinds:
+        for fill in (0x33, 0xff, 0x7f):
+            room = dev(np.full(size + 64, fill, np.uint8))
+            be.paged_attend(B.paged_attend_desc(a, sc, group_start=dev(np.array(start, np.int64).astype(np.int32)), n_shared=dev(np.full(len(start) - 1, common, np.int32)), n_group=len(start) - 1, workspace=room,
+                                                workspace_bytes=size))
+            got = dev.back(po, margin)
+            assert (got[:n_seq * rows] == 3).all() and (got[2 * n_seq * rows:] == 3).all()
+            assert (dev.back(room, np.zeros(size + 64, np.uint8))[size:] == fill).all()
+            check_close(got[n_seq * rows:2 * n_seq * rows], pool, starts, [rows] * n_seq, q, room=0.05)
+
+
+@pytest.mark.parametrize("eight", [False, True])
+def test_groups_over_rows_that_make_no_sense_touch_nothing_else(be, dev, eight):
+    """Rows' beginnings that are not ascending, negative or behind the last row, under one group: answered inside the described buffers."""
+    rng = np.random.default_rng(3)
+    n_seq, n_rows, h, hd, common = 5, 60, 4, 64, 304
+    n_kv = [common + 60] * n_seq
+    pool = make_pool(rng, n_kv, 2, hd, 16, eight, groups=([0, n_seq], [common]))
+    q = rng.standard_normal((n_rows, h, hd)).astype(np.float16)
+    size = B.paged_attend_workspace(n_seq, n_rows, h, hd)
+    margin = np.full((3 * n_rows, h, hd), 3.0, dtype=np.float32)
+    po, c, pq, pn, pt = dev(margin), pool.cache(dev(pool.k), dev(pool.v)), dev(q), dev(np.array(n_kv, np.int32)), dev(pool.table)
+    sc = pool.of_scales(dev(pool.scales)) if eight else None
+    for start in ([0, 20, 10, 40, 30, 60], [50, 40, 30, 20, 10, 0], [-9, 5, 70, 20, 65, 1 << 20], [0, 60, 0, 60, 0, 60], [10, 30, 5, 50, 2, 40], [0, 30, 12, 13, 14, 20]):
+        room = dev(np.full(size + 64, 0x33, np.uint8))
+        a = B.paged_attention_desc(c, B.paged_batch(dev(np.array(start, np.int32)), pn, pt, n_seq, n_rows, pool.table.shape[1]), pq, po + n_rows * h * hd * 4, h, out_type=B.FP32)
+        be.paged_attend(B.paged_attend_desc(a, sc, group_start=dev(np.array([0, n_seq], np.int32)), n_shared=dev(np.array([common], np.int32)), n_group=1, workspace=room, workspace_bytes=size))
+        got = dev.back(po, margin)
+        assert (got[:n_rows] == 3).all() and (got[2 * n_rows:] == 3).all()
+        assert (dev.back(room, np.zeros(size + 64, np.uint8))[size:] == 0x33).all()
