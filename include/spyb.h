@@ -348,8 +348,8 @@ typedef struct {
 } spyb_paged_shared;
 
 /* spyb_paged_attention over a cache of SPYB_FP16 or SPYB_INT8, with what sequences share read once for all of them. For SPYB_INT8 scores are
- * multiplied by K's scales and probabilities by V's in f32; a probability times a scale is rounded to fp16 in front of the second product, against the largest scale met, which is that of
- * all rows of a sequence that are read together. A row that sees nothing is zeros; what is not seen has no influence but by that, infinite and NaN scales none at all. */
+ * multiplied by K's scales and probabilities by V's in f32; their products, the weights of the row's positions, are rounded to fp16 in front of the second product, against the row's largest one (scales below 2^-24
+ * counting as that). A row that sees nothing is zeros; what is not seen has no influence, scales of any size, infinite and NaN ones included. */
 typedef struct {
     spyb_paged_attention_desc attention;
     spyb_paged_scales scales;

@@ -5,8 +5,8 @@
 //   costs half the products, scores and accumulators of one that has query rows in the 16.
 //   Bytes become fp16 numbers without an error in registers (five instructions for four of K, six of V). A lane reads HD / 4 bytes of two positions of K and HD / 8 of four of V in
 //   16-byte pieces: the products' inner order is the lane's own, the same for Q, whose elements it reads alike, and V's elements are where the accumulators' rows are.
-//   Scales stay out of the products' operands: K's multiply scores (where scale and log2 e are a product anyway), V's the probabilities, in f32. So that no probability leaves fp16's range,
-//   V's scales are taken against the largest so far, rounded up to a power of two; like the maximum of the scores it moves a few times at the start and hardly ever after.
+//   Scales stay out of the products' operands: K's multiply scores (where scale and log2 e are a product anyway), V's the probabilities, in f32. What is rounded to fp16 is their product, the weight of a position: a
+//   row's maximum is that of its scores plus log2 of V's scales, over what it sees, so that weights are rounded against the row's largest one, whatever the scales of other positions and other rows' are.
 // Measured (heads of 128): 64 single tokens of up to 4096 positions, 32 query heads on 8 (277 MB), 60 us, 4.6 TB/s (heads of 64 51 us); three of 100 000, 40 on 8, 115 us, 5.3 TB/s, by head 106; one of 4000, 32 on 32 (33 MB),
 // 15 us. Single tokens' loop runs at the memory's rate; beside it 7 us until the first stage is there (lengths, the plan, page table, bytes, one after the other) and 4 us for every item that is done, joins among them.
 // Five rows of 24 sequences of up to 9000 (tiles of 24 rows) 118 us: 1.7 us a stage of 64 positions, a warp's chain of products and conversions with eight warps an SM (168 registers), and 5 us for a join.
@@ -81,6 +81,7 @@ __device__ __forceinline__ float over_groups(float v, bool largest) {   // over 
     return v;
 }
 
+__device__ __forceinline__ float lg2(float x) { float y; asm("lg2.approx.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
 __device__ __forceinline__ void sts64(uint32_t addr, uint2 v) { asm volatile("st.shared.v2.u32 [%0], {%1,%2};" ::"r"(addr), "r"(v.x), "r"(v.y) : "memory"); }
 constexpr uint64_t PB_LANDING_NS = 1000000000;      // copies have this long to land (whatever the limit of the waits)
 __device__ __noinline__ void stand_still(uint64_t ns) {
@@ -94,8 +95,9 @@ __device__ __forceinline__ void tma_pages(uint32_t dst, const CUtensorMap *map, 
 __device__ __forceinline__ void arrive_when_copied(uint32_t bar) { asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory"); }   // of this lane's copies so far
 // A CTA's part of an item, found by the copying warp for all: rows of the tile, stages of the ring, positions [ka, kb); rows 0: behind the last one
 struct BytesEntry { int rows, n_stage, ka, kb, tile, head, row0, first, from, c0, parts; };
-// What probabilities and V's scales are taken against follows when a score is 2^PB_SLACK above it, a scale PB_SLACK_SCALE times it: products up to 2^15 are as exact in fp16 as those below 1
-constexpr float PB_SLACK = 11.f, PB_SLACK_SCALE = 16.f;
+// What weights are taken against follows when one is 2^PB_SLACK times that: weights up to 2^15 are as exact in fp16 as those below 1
+constexpr float PB_SLACK = 15.f;
+constexpr float PB_LEAST = -24.f;             // log2 of the least scale; a scale of 0, or one that is not finite, counts as it (so that scores have a maximum, and sums of probabilities stay below 2^40 each)
 constexpr int PB_ENTRIES = 4;                 // known ahead
 
 // One warp copies for four that compute (with each its own copies a block's took a third of the warp's time on it: some hundred instructions of addresses).
@@ -280,8 +282,7 @@ __global__ void __launch_bounds__(PB_THREADS, BytesSmem<HD, NT>::CTAS) paged_byt
     };
     while (next()) {
         const int first_row = e.tile * ROWS, pos_first = e.first + (int)((unsigned)first_row / (unsigned)p.group), pos_last = e.first + (int)((unsigned)(first_row + e.rows - 1) / (unsigned)p.group);
-        float o[NT][HD / 16][4], mx[NT][2], sum[NT][2], base[NT][2], over[NT][2];   // (base: the maximum, or 0 for none; over: scores beyond it move the maximum)
-        float unit = 1099511627776.f;             // one over the power of two that V's scales are taken against: 2^-40 at first, below the least scale
+        float o[NT][HD / 16][4], mx[NT][2], sum[NT][2], base[NT][2], over[NT][2];   // (mx: of the weights, in powers of two; base: that, or 0 for none; over: weights beyond it move the maximum)
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
             mx[n][0] = mx[n][1] = over[n][0] = over[n][1] = -CUDART_INF_F; sum[n][0] = sum[n][1] = base[n][0] = base[n][1] = 0.f;
@@ -296,7 +297,7 @@ __global__ void __launch_bounds__(PB_THREADS, BytesSmem<HD, NT>::CTAS) paged_byt
             const int j0 = e.ka + s * PB_STAGE + warp * PR_BLOCK;
             const bool whole = mask == 0xffffu && (!p.causal || (j0 + PR_BLOCK - 1 <= pos_first && (p.window <= 0 || j0 > pos_last - p.window)));
             // scores of positions g and g + 8
-            float sc[NT][4], v_scale[2], k_scale[2];
+            float sc[NT][4], v_scale[2], v_log[2], k_scale[2];
             {
 #pragma unroll
                 for (int n = 0; n < NT; ++n) { sc[n][0] = sc[n][1] = sc[n][2] = sc[n][3] = 0.f; }
@@ -322,6 +323,13 @@ __global__ void __launch_bounds__(PB_THREADS, BytesSmem<HD, NT>::CTAS) paged_byt
             bool above = false, odd = false;                  // (odd: a scale of V is not finite)
             {
 #pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const float size = fabsf(v_scale[i]);
+                    const bool is = size < CUDART_INF_F;
+                    v_log[i] = is ? fmaxf(lg2(size), PB_LEAST) : PB_LEAST;
+                    above |= !is;
+                }
+#pragma unroll
                 for (int n = 0; n < NT; ++n) {
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
@@ -332,37 +340,26 @@ __global__ void __launch_bounds__(PB_THREADS, BytesSmem<HD, NT>::CTAS) paged_byt
                             const bool seen = ((mask >> jj) & 1) && (!p.causal || (d >= 0 && (p.window <= 0 || d < p.window)));
                             x = seen ? x : -CUDART_INF_F;
                         }
-                        above |= x > over[n][i & 1];
+                        above |= x + v_log[i >> 1] > over[n][i & 1];
                     }
                 }
-#pragma unroll
-                for (int i = 0; i < 2; ++i) { v_scale[i] *= unit; above |= !(fabsf(v_scale[i]) <= PB_SLACK_SCALE); }
             }
             if (__any_sync(0xffffffffu, above)) {
-                float most = 1.f;
-                bool  fine = true;
-#pragma unroll
-                for (int i = 0; i < 2; ++i) { const bool is = fabsf(v_scale[i]) < CUDART_INF_F; fine &= is; most = fmaxf(most, is ? fabsf(v_scale[i]) : 1.f); }
-                odd = !__all_sync(0xffffffffu, fine);
-                most = over_groups(most, true);
-                const uint32_t up = (__float_as_uint(most) + 0x7fffffu) & 0x7f800000u;      // the next power of two, 2^56 at most
-                const float f_scale = __uint_as_float(0x7f000000u - up);                    // one over it
-                unit *= f_scale;
-                v_scale[0] *= f_scale; v_scale[1] *= f_scale;
+                odd = !__all_sync(0xffffffffu, fabsf(v_scale[0]) < CUDART_INF_F && fabsf(v_scale[1]) < CUDART_INF_F);
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
-                        float v = fmaxf(sc[n][i], sc[n][2 + i]);
+                        float v = fmaxf(sc[n][i] + v_log[0], sc[n][2 + i] + v_log[1]);
                         v = over_groups(v, true);
                         const float to = v > over[n][i] ? fmaxf(mx[n][i], base[n][i] + v) : mx[n][i], f = to == mx[n][i] ? 1.f : ex2(mx[n][i] - to);   // (2^-inf = 0 at the first)
-                        const float from = base[n][i], f_o = f * f_scale;
+                        const float from = base[n][i];
                         mx[n][i] = to; sum[n][i] *= f;
                         base[n][i] = to == -CUDART_INF_F ? 0.f : to;
                         over[n][i] = to == -CUDART_INF_F ? to : PB_SLACK;
                         sc[n][i] += from - base[n][i]; sc[n][2 + i] += from - base[n][i];
 #pragma unroll
-                        for (int k = 0; k < HD / 16; ++k) { o[n][k][i] *= f_o; o[n][k][2 + i] *= f_o; }
+                        for (int k = 0; k < HD / 16; ++k) { o[n][k][i] *= f; o[n][k][2 + i] *= f; }
                     }
                 }
             }
@@ -405,7 +402,6 @@ __global__ void __launch_bounds__(PB_THREADS, BytesSmem<HD, NT>::CTAS) paged_byt
         }
         // This warp's findings (the next item's copies are on their way)
         float *mo = reinterpret_cast<float *>(smem + Smem::FOUND), *mm = mo + PR_WARPS * ROWS * HD, *ml = mm + PR_WARPS * ROWS;
-        const float f = 1.f / unit;
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
 #pragma unroll
@@ -415,7 +411,7 @@ __global__ void __launch_bounds__(PB_THREADS, BytesSmem<HD, NT>::CTAS) paged_byt
                 if (r < e.rows) {
                     float *dst = mo + (warp * ROWS + r) * HD + g * (HD / 8);
 #pragma unroll
-                    for (int k = 0; k < HD / 16; k += 2) { *reinterpret_cast<float4 *>(dst + 2 * k) = make_float4(o[n][k][i] * f, o[n][k][2 + i] * f, o[n][k + 1][i] * f, o[n][k + 1][2 + i] * f); }
+                    for (int k = 0; k < HD / 16; k += 2) { *reinterpret_cast<float4 *>(dst + 2 * k) = make_float4(o[n][k][i], o[n][k][2 + i], o[n][k + 1][i], o[n][k + 1][2 + i]); }
                     if (g == 0) { mm[warp * ROWS + r] = mx[n][i]; ml[warp * ROWS + r] = l; }
                 }
             }

@@ -90,6 +90,82 @@ def make_pool(rng, n_kv, h_kv, hd, page, eight=True, sizes=0.5, token_major=Fals
     return pool
 
 
+# ---------------------------------------------------------------------------------------------- V's scales
+@pytest.mark.parametrize("rows", [1, 2, 6, 100])
+@pytest.mark.parametrize("hd", [32, 64, 128])
+@pytest.mark.parametrize("large", [32.0, 515.5, 65504.0])
+def test_a_position_of_no_weight_and_a_large_scale_takes_nothing_from_the_others(be, dev, rows, hd, large):
+    """4000 positions of scale 0.03 and, at the start, in the middle and near the end, one whose score is some 40 below theirs and whose V is thousands of times larger."""
+    rng = np.random.default_rng(rows + hd)
+    n, h, h_kv = 4000, 4, 2
+    pool = make_pool(rng, [n], h_kv, hd, 16, sizes=0.1)
+    q = (1 + 0.1 * rng.standard_normal((rows, h, hd))).astype(np.float16)
+    at = lambda j: (pool.table[0, j // 16], j % 16)  # noqa: E731
+    pool.scale_view()[(pool.table[0, np.arange(n) // 16], np.arange(n) % 16)] = (0.03 / 16, 0.03)
+    for j in (3, 2222, n - rows - 5):
+        pool.view(pool.k)[at(j)] = -100
+        pool.scale_view()[at(j)] = (40 / 100 * hd ** -0.5, large)
+    got = attend(be, dev, pool, [0, rows], q, np.zeros(q.shape, dtype=np.float32))
+    check_close(got, pool, [0, rows], [rows], q, room=0.15)
+
+
+@pytest.mark.parametrize("rows", [2, 6, 100])
+@pytest.mark.parametrize("hd", [32, 64, 128])
+def test_scales_of_positions_that_a_row_does_not_see_take_nothing_from_it(be, dev, rows, hd):
+    """The last row's position has K and V of any scale: the rows in front of it are as near as without it, and in the kernel for few rows, where a row's maximum is its own alone, the same bits."""
+    rng = np.random.default_rng(rows + hd)
+    n, h, h_kv = 500 + rows, 6, 2
+    pool = make_pool(rng, [n], h_kv, hd, 16)
+    q, out0, last = rng.standard_normal((rows, h, hd)).astype(np.float16), np.zeros((rows, h, hd), dtype=np.float32), (pool.table[0, (n - 1) // 16], (n - 1) % 16)
+    got = []
+    for pair in ((1e-3, 1e-3), (5.0, 515.5), (65504.0, 65504.0), (0.0, 2.0 ** -24)):
+        pool.scale_view()[last] = pair
+        got.append(attend(be, dev, pool, [0, rows], q, out0)[:rows - 1])
+        pool.scale_view()[last] = 1
+        front = pool.n_kv
+        pool.n_kv = [n - 1]
+        check_close(got[-1], pool, [0, rows - 1], [rows - 1], q[:rows - 1], room=0.05)
+        pool.n_kv = front
+    assert rows == 100 or all(np.array_equal(got[0].view(np.uint32), x.view(np.uint32)) for x in got[1:])
+
+
+@pytest.mark.parametrize("rows", [1, 5, 40])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_scales_that_are_zero_negative_or_the_smallest(be, dev, rows, hd):
+    rng = np.random.default_rng(rows * hd)
+    n, h, h_kv = 600, 4, 2
+    for kind in range(4):
+        pool = make_pool(rng, [n], h_kv, hd, 16)
+        where = (pool.table[0, np.arange(n) // 16], np.arange(n) % 16, slice(None), 1)
+        v = pool.scale_view()[where].copy()
+        pool.scale_view()[where] = (0 * v, np.where(rng.random(v.shape) < 0.5, -v, v), 0 * v + 2.0 ** -24, np.where(rng.random(v.shape) < 0.5, 0, v))[kind]
+        q = (2 * rng.standard_normal((rows, h, hd))).astype(np.float16)
+        check_close(attend(be, dev, pool, [0, rows], q, np.zeros(q.shape, dtype=np.float32)), pool, [0, rows], [rows], q)
+
+
+# ---------------------------------------------------------------------------------------------- long contexts, scores and scales of all sizes
+@pytest.mark.parametrize("rows,n_kv,h,h_kv,hd,page", [([1], [40000], 2, 1, 64, 64), ([1], [30011], 4, 2, 128, 24), ([3], [30000], 4, 1, 128, 16), ([40], [9000], 2, 1, 128, 64), ([33], [12000], 3, 1, 64, 16),
+                                                      ([5, 1], [20000, 700], 4, 2, 96, 16), ([1, 6], [9000, 12001], 4, 4, 32, 32)])
+@pytest.mark.parametrize("spread,sizes", [(0.05, 0.2), (1.0, 0.5), (1.0, 2.0)])
+def test_cut_items_of_all_scores_and_scales(be, dev, rows, n_kv, h, h_kv, hd, page, spread, sizes):
+    """Items that many CTAs share, whose pieces have maxima and scales of their own."""
+    rng = np.random.default_rng(n_kv[0] + hd)
+    pool = make_pool(rng, n_kv, h_kv, hd, page, sizes=sizes)
+    starts = np.concatenate([[0], np.cumsum(rows)])
+    q = (spread * rng.standard_normal((starts[-1], h, hd))).astype(np.float16)
+    check_close(attend(be, dev, pool, starts, q, np.zeros(q.shape, dtype=np.float32)), pool, starts, rows, q, room=0.3)
+
+
+@pytest.mark.parametrize("rows", [1, 4, 33, 300])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_sharp_rows_and_scales_of_all_sizes_by_what_each_row_sees(be, dev, rows, hd):
+    rng = np.random.default_rng(rows)
+    for spread, sizes in ((2.0, 0.2), (0.05, 2.5)):
+        pool = make_pool(rng, [900, rows], 2, hd, 16, sizes=sizes)
+        q = (spread * rng.standard_normal((2 * rows, 8, hd))).astype(np.float16)
+        check_close(attend(be, dev, pool, [0, rows, 2 * rows], q, np.zeros(q.shape, dtype=np.float32)), pool, [0, rows, 2 * rows], [rows, rows], q, room=0.3)
+
+
 # ---------------------------------------------------------------------------------------------- shared beginnings
 @pytest.mark.parametrize("eight", [False, True])
 @pytest.mark.parametrize("shared", [128, 290, 299, 300, 500, 100000])
