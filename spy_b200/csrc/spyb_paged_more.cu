@@ -40,6 +40,13 @@ constexpr int ST_THREADS = 256, ST_ROWS = 8;
 struct StorePlace { int pos; int64_t cell, pair; };                 // pos -1: nobody's row, or one in front of position 0; cell -1: its page is not there
 __device__ __forceinline__ float larger(float a, float b) { float r; asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b)); return r; }
 __device__ __forceinline__ float one_over(float x) { float r; asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x)); return r; }   // (off by a step at most)
+// x / scale to the nearest whole number, a half to the even one. A product with the reciprocal may be wrong beside a half; what is left over of x then says which it is, without an error: x - q scale, at most
+// half a scale or a bit more, is a multiple of x's last place or of the scale's (11 bits), which 24 bits hold
+__device__ __forceinline__ float nearest_byte(float x, float scale, float per_one) {
+    const float q = rintf(x * per_one), left = fmaf(-q, scale, x), twice = 2.f * fabsf(left);
+    const bool odd = ((int)q & 1) != 0;
+    return twice > scale || (twice == scale && odd) ? q + copysignf(1.f, left) : q;
+}
 
 template <class TIn, class TQ, bool EIGHT, bool HALVES>
 __global__ void __launch_bounds__(ST_THREADS, 4) paged_store_kernel(const __grid_constant__ PagedStore s, const int width, const int rows_each) {
@@ -135,10 +142,16 @@ __global__ void __launch_bounds__(ST_THREADS, 4) paged_store_kernel(const __grid
                     const bool   fine = most <= 65468.f;
                     const __half scale = fine ? __float2half_ru(__fdiv_rn(most, 127.f)) : __ushort_as_half(0x7fff);
                     const float  per_one = fine && most > 0.f ? one_over(__half2float(scale)) : 0.f;
+                    // (two products, 2^-21 to either side: where they agree, which is nearly always, that is the nearest. 1.5 x 2^23: the integer is the low byte. Beside a scale that is NaN the bytes are any)
+                    const float  more = per_one * (1.f + 0x1p-21f), less = per_one * (1.f - 0x1p-21f), ones = 12582912.f;
                     uint8_t *dst = (head.is_k ? s.k8 : s.v8) + at.cell + to;
-                    uint32_t b[8];
+                    uint32_t b[8], differ = 0;
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) { b[i] = __float_as_uint(fmaf(x[i], per_one, 12582912.f)); }   // (1.5 x 2^23: the integer is the low byte. Beside a scale that is NaN the bytes are any)
+                    for (int i = 0; i < 8; ++i) { b[i] = __float_as_uint(fmaf(x[i], more, ones)); differ |= b[i] ^ __float_as_uint(fmaf(x[i], less, ones)); }
+                    if (differ != 0) {
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) { b[i] = __float_as_uint(nearest_byte(x[i], __half2float(scale), per_one) + ones); }
+                    }
                     *reinterpret_cast<uint32_t *>(dst + e0) = __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
                     *reinterpret_cast<uint32_t *>(dst + e1) = __byte_perm(__byte_perm(b[4], b[5], 0x0040), __byte_perm(b[6], b[7], 0x0040), 0x5410);
                     if (item == 0) { reinterpret_cast<__half *>(const_cast<uint32_t *>(s.scales.pairs))[2 * (at.pair + head.hh * s.scales.head_stride) + (head.is_k ? 0 : 1)] = scale; }

@@ -7,7 +7,7 @@ import pytest
 
 from spy_b200 import backend as B
 from test_gpu_paged import Device, Pool, be, dev  # noqa: F401
-from test_gpu_paged_more import BytePool, attend
+from test_gpu_paged_more import TYPES, BytePool, attend, scale_above
 
 pytestmark = pytest.mark.gpu
 
@@ -229,3 +229,57 @@ def test_groups_over_rows_that_make_no_sense_touch_nothing_else(be, dev, eight):
         got = dev.back(po, margin)
         assert (got[:n_rows] == 3).all() and (got[2 * n_rows:] == 3).all()
         assert (dev.back(room, np.zeros(size + 64, np.uint8))[size:] == 0x33).all()
+
+
+# ---------------------------------------------------------------------------------------------- store
+def store_values(be, dev, values, dtype=np.float32, **norms):
+    """K and V (the same values, [rows][head_dim]) into 8-bit pages, without rotation: bytes and scales of V, of K."""
+    n, hd = values.shape
+    pool = BytePool(np.random.default_rng(0), [n], 1, hd, 16)
+    pk, pv, ps, px = dev(pool.k), dev(pool.v), dev(pool.scales), dev(values.astype(dtype))
+    batch = B.paged_batch(dev(np.array([0, n], np.int32)), dev(np.array([n], np.int32)), dev(pool.table), 1, n, pool.table.shape[1])
+    be.paged_store(B.paged_store_desc(B.paged_append_desc(pool.cache(pk, pv), batch, None, px, px, None, 0, in_type=TYPES[dtype], rope_mode=B.ROPE_NONE), pool.of_scales(ps), **norms))
+    at = (pool.table[0, np.arange(n) // 16], np.arange(n) % 16)
+    k, v, sc = dev.back(pk, pool.k), dev.back(pv, pool.v), pool.scale_view(dev.back(ps, pool.scales))[at][:, 0]
+    return (pool.view(v)[at][:, 0], sc[:, 1]), (pool.view(k)[at][:, 0], sc[:, 0])
+
+
+def nearest_even(x, scale):
+    """x / scale to the nearest whole number, a half to the even one, without an error on the way: twice the quotient is compared as whole numbers of 2^-200."""
+    from fractions import Fraction
+    got = np.zeros(x.shape, np.int64)
+    for i, row in enumerate(x):
+        unit = Fraction(float(scale[i]))
+        got[i] = [round(Fraction(float(e)) / unit) if unit else 0 for e in row]      # (Python rounds a half to the even one)
+    return got
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+def test_bytes_are_the_nearest_and_a_half_goes_to_the_even_one(be, dev, hd):
+    """Elements that are k + 1/2 scales to the last bit, or a bit beside it, for scales of all mantissas: K and V the same bytes, which are the nearest."""
+    rng = np.random.default_rng(hd)
+    n = 700
+    scale = (1 + rng.integers(0, 1024, n) / 1024) * 2.0 ** rng.integers(-14, 8, n)                    # (of 11 bits, as fp16's)
+    k = rng.integers(-126, 126, (n, hd))
+    x = (scale[:, None] * (k + 0.5)).astype(np.float32)                                               # exact: 11 bits by 8
+    beside = rng.integers(0, 3, (n, hd))
+    x = np.where(beside == 0, x, np.nextafter(x, np.where(beside == 1, np.float32(np.inf), np.float32(-np.inf)))).astype(np.float32)
+    x[:, 5] = (127 * scale).astype(np.float32)                                                        # exact: the largest magnitude
+    for bytes_, got in store_values(be, dev, x):
+        assert np.array_equal(got.astype(np.float64), scale)
+        assert np.array_equal(bytes_.astype(np.int64), nearest_even(x, scale))
+
+
+def test_a_scale_is_not_below_its_largest_magnitude_by_127(be, dev):
+    """Largest magnitudes a bit above 127 fp16 numbers: their quotients lie between f32 numbers beside these."""
+    rng = np.random.default_rng(11)
+    n, hd = 900, 64
+    h = (1 + rng.integers(0, 1024, n) / 1024) * 2.0 ** rng.integers(-14, 8, n)
+    most = np.nextafter((127 * h).astype(np.float32), np.float32(np.inf))
+    x = (rng.uniform(-1, 1, (n, hd)) * most[:, None]).astype(np.float32)
+    x[np.arange(n), rng.integers(0, hd, n)] = most
+    want = scale_above(most.astype(np.float64) / 127)
+    assert (want > h).all()
+    for bytes_, got in store_values(be, dev, x):
+        assert np.array_equal(got, want)
+        assert np.array_equal(bytes_.astype(np.int64), nearest_even(x, got.astype(np.float64)))
