@@ -311,7 +311,9 @@ typedef struct {
 
 /* spyb_paged_append with a norm of every head of Q and K in front of the rotation, into a cache of SPYB_FP16 or SPYB_INT8: x -> x / sqrt(mean of x^2 + norm_eps) * weight (NormRMS and Mul,
  * orchestration/include/operator/non-linear.h:117, over a head's elements). q_norm, k_norm: f32 [head_dim], 16-byte aligned, the same for all heads; NULL leaves a norm out. norm_eps: not negative.
- * Everything is held in f32 (angles in 64 bits) and rounded once. `scales` is of SPYB_INT8 caches, and not read otherwise. The rest is spyb_paged_append's. */
+ * Everything is held in f32 (angles in 64 bits) and rounded once; squares too, so that a norm is right for heads whose largest magnitude is at most 10^18 and, where norm_eps is below 10^-30, at least 10^-15 (beyond, squares
+ * leave f32: zeros come out of the largest). `scales` is of SPYB_INT8 caches, and not read otherwise. The rest is spyb_paged_append's; of two rows of one call that share a page and a position in it, a head of an SPYB_INT8
+ * cache may get one row's bytes and the other's scale. */
 typedef struct {
     spyb_paged_append_desc append;
     spyb_paged_scales scales;
@@ -336,8 +338,8 @@ spyb_status spyb_paged_load(spyb_backend *backend, const spyb_paged_load_desc *d
 
 /* Which sequences hold the same K and V in their first positions (one system prompt, a document, the trunk of several answers): sequences group_start[g] .. group_start[g+1]-1 (ascending) the same in
  * their first n_shared[g] ones, usually because their tables name the same pages. Device arrays, read when the kernels run; sequences in no group share nothing. That is a promise about values, and nothing else:
- * which positions a row sees does not change, and what is shared is read, once for all, from the pages of the group's first sequence that has rows. (It is cut to what all rows of the group see, in whole pages or so, so a
- * window leaves nothing of it, and below 128 positions to nothing.) n_group = 0: nothing is shared, the rest is not read. `workspace`: device memory, 16-byte aligned, of spyb_paged_attend_workspace bytes, this call's until the
+ * which positions a row sees does not change, and what is shared is read, once for all, from the pages of the group's first sequence that has rows. (It is cut to what all rows of the group see, to a multiple of the largest
+ * power of two from 16 to 128 that divides the page size, or of 16; a window leaves nothing of it, nor do fewer than 128 positions.) n_group = 0: nothing is shared, the rest is not read. `workspace`: device memory, 16-byte aligned, of spyb_paged_attend_workspace bytes, this call's until the
  * backend's stream has passed it; it needs no clearing, and calls that follow one another on a backend may have one. */
 typedef struct {
     const int32_t *group_start;   /* [n_group + 1] */

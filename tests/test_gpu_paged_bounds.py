@@ -7,7 +7,7 @@ import pytest
 
 from spy_b200 import backend as B
 from test_gpu_paged import Device, Pool, be, dev  # noqa: F401
-from test_gpu_paged_more import TYPES, BytePool, attend, scale_above
+from test_gpu_paged_more import TYPES, BytePool, attend, plain_norm, scale_above
 
 pytestmark = pytest.mark.gpu
 
@@ -283,3 +283,27 @@ def test_a_scale_is_not_below_its_largest_magnitude_by_127(be, dev):
     for bytes_, got in store_values(be, dev, x):
         assert np.array_equal(got, want)
         assert np.array_equal(bytes_.astype(np.int64), nearest_even(x, got.astype(np.float64)))
+
+
+@pytest.mark.parametrize("eps", [0.0, 1e-30, 1e-6])
+@pytest.mark.parametrize("size", [1e18, 1e10, 1e-5, 1e-15])
+@pytest.mark.parametrize("hd", [24, 128, 256])
+def test_norms_of_very_large_and_very_small_heads(be, dev, eps, size, hd):
+    """Squares at either end of f32."""
+    rng = np.random.default_rng(hd)
+    n, h = 9, 3
+    x = (size * rng.uniform(-1, 1, (n, h, hd))).astype(np.float32)
+    x[:, 1] = rng.standard_normal((n, hd))                                                            # (an ordinary head beside them)
+    w = (1 + 0.3 * rng.standard_normal(hd)).astype(np.float32)
+    one = (hd + 15) // 16 * 16
+    pool = Pool(rng, [n], 1, hd, 16, strides=(16 * one, one, 16 * one), fill=0)
+    px, pq, q0 = dev(x), None, np.zeros((n, h, hd), np.float32)
+    pq = dev(q0)
+    batch = B.paged_batch(dev(np.array([0, n], np.int32)), dev(np.array([n], np.int32)), dev(pool.table), 1, n, pool.table.shape[1])
+    zeros = dev(np.zeros((n, hd), np.float32))
+    append = B.paged_append_desc(pool.cache(dev(pool.k), dev(pool.v)), batch, px, zeros, zeros, pq, h, q_out_type=B.FP32, rope_mode=B.ROPE_NONE)
+    be.paged_store(B.paged_store_desc(append, q_norm=dev(w), norm_eps=eps))
+    want = plain_norm(x.astype(np.float64), w.astype(np.float64), np.float64(np.float32(eps)))
+    err = np.abs(dev.back(pq, q0).astype(np.float64) - want)
+    # a sum of head_dim squares (half its relative error), a reciprocal square root of 2 steps, two products, each a bit among the smallest numbers
+    assert (err <= np.abs(want) * ((hd + 2) / 2 + 4 + 2) * 2.0 ** -24 + 3 * 2.0 ** -149).all(), float((err / np.maximum(np.abs(want), 1e-300)).max())
