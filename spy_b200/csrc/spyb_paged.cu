@@ -255,6 +255,11 @@ template <int UNIT, int ALIGN> static int cut_selftest(uint32_t seed, int tile_r
         p.start_units = rnd(2) * rnd(5);
         const bool all_seen = p.window > 0 && turn % 4 == 1;   // a window as long as an int can say is none
         if (all_seen) { p.window = paged_window(INT_MAX - rnd(3)); }
+        std::vector<int32_t> from(n_seq);        // own positions of the second of two passes; of nonsense too
+        if (turn % 2 == 1 && p.window == 0) {
+            for (int32_t &x : from) { x = 16 * rnd(1 + most_kv / (turn % 3 == 1 ? 8 : 24)); }
+            p.view.from = from.data();
+        }
         const int grid = 1 + rnd(300), least = 1 + rnd(4);
         for (int few = 0; few < 2; ++few) {
             PagedPlace at = {};
@@ -286,7 +291,7 @@ template <int UNIT, int ALIGN> static int cut_selftest(uint32_t seed, int tile_r
                     const PagedItem it = paged_item<UNIT, ALIGN>(p, q, tile);
                     if (q.row0 < 0 || q.rows < 1 || q.row0 + q.rows > p.view.n_rows || head >= p.n_head_kv || tile * p.tile_rows >= q.rows * p.group) { return 3; }
                     if (all_seen && it.lo != 0) { return 14; }
-                    if (it.lo < 0 || it.lo % ALIGN != 0 || it.hi > p.view.n_kv_most || off >= it.units || (int64_t)it.units * UNIT + it.lo < it.hi) { return 4; }
+                    if (it.lo < 0 || (p.view.from != nullptr ? it.lo != q.from || it.lo % 16 != 0 : it.lo % ALIGN != 0) || it.hi > p.view.n_kv_most || off >= it.units || (int64_t)it.units * UNIT + it.lo < it.hi) { return 4; }
                     const int todo = (int)std::min<int64_t>(it.units - off, at.end - at.unit);
                     const PagedCut cut = paged_cut(at, at.unit - off, it.units);
                     if ((cut.parts == 1) != (todo == it.units) || cut.c0 < 0 || cut.c0 + cut.parts > ctas || c < cut.c0 || c >= cut.c0 + cut.parts) { return 5; }
@@ -319,7 +324,7 @@ template <int UNIT, int ALIGN> static int cut_selftest(uint32_t seed, int tile_r
 int paged_cut_selftest() {
     int bad = cut_selftest<64, 16>(1, 16);
     if (bad == 0) { bad = cut_selftest<64, 16>(2, 32); }
-    if (bad == 0) { bad = cut_selftest<64, 64>(4, 8); }
+    for (const int tile : {8, 16, 24}) { if (bad == 0) { bad = cut_selftest<64, 64>(4 + tile, tile); } }
     if (bad == 0) { bad = cut_selftest<128, 128>(3, 0); }
     return bad == 0 ? 0 : 100 + bad;
 }

@@ -119,7 +119,7 @@ PagedScales paged_scales_of(const spyb_paged_cache &c, const spyb_paged_scales &
 // 225.8 / 209.0 / 211.3 / 218.9, 512 at 1024 34.5 / 27.3 / 28.4 / 30.0.
 constexpr int PA_START = 2;
 struct PagedSeq { int row0, rows, first, kv, from; };   // first row and number of rows, position of the first row, positions that are there, and the first of them that this pass reads
-struct PagedItem { int lo, hi, units; };          // positions [lo, hi) that some row of the tile sees (lo a multiple of ALIGN)
+struct PagedItem { int lo, hi, units; };          // positions [lo, hi) that some row of the tile sees (lo a multiple of ALIGN, or where own positions begin: of paged_shared_align, 16 to 128)
 
 __host__ __device__ __forceinline__ int pmin(int a, int b) { return a < b ? a : b; }
 __host__ __device__ __forceinline__ int pmax(int a, int b) { return a < b ? b : a; }
