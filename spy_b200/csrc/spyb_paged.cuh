@@ -98,8 +98,8 @@ bool        launch_paged_attention_tc(const PagedAttention &p, int head_dim, int
 // doubles its instructions. 24 sequences of up to 9000 positions, four query heads a K/V head: 3 and 4 rows (12 and 16 in all) 95 and 98 us there against
 // 118 and 118 on tensor memory, 5 and 8 rows (20 and 32) 144 and 156 against 118 and 118.
 constexpr int PA_FEW_ROWS = 16;
-// The same of the small kernel for bytes, whose tiles have 8, 16 or 24 rows: the 24 sequences at 3 and 4 rows (12 and 16 in all) 79 and 85 us, at 5 and 6 (20 and 24) 118 and 123, on tensor memory 163 to 167
-// for any of these, 169 at 8 rows (32), where two small tiles take 218.
+// The same of the small kernel for bytes, whose tiles have 8, 16 or 24 rows: the 24 sequences at 3 and 4 rows (12 and 16 in all) 80 and 85 us, at 5 and 6 (20 and 24) 117 and 122, on tensor memory 155 to 159
+// for any of these, 160 at 8 rows (32), where two small tiles take 208. 5 rows of 6 sequences of up to 600 18 us and 26, of 64 47 and 78, of one of 60 000 77 and 92 (3 rows 52 and 87).
 constexpr int PB_FEW_ROWS = 24;
 
 // What every operator asks of the cache and the batch; `scales`: those that may come with bytes (nullptr: an fp16 cache alone)

@@ -7,9 +7,9 @@
 //   16-byte pieces: the products' inner order is the lane's own, the same for Q, whose elements it reads alike, and V's elements are where the accumulators' rows are.
 //   Scales stay out of the products' operands: K's multiply scores (where scale and log2 e are a product anyway), V's the probabilities, in f32. What is rounded to fp16 is their product, the weight of a position: a
 //   row's maximum is that of its scores plus log2 of V's scales, over what it sees, so that weights are rounded against the row's largest one, whatever the scales of other positions and other rows' are.
-// Measured (heads of 128): 64 single tokens of up to 4096 positions, 32 query heads on 8 (277 MB), 60 us, 4.6 TB/s (heads of 64 51 us); three of 100 000, 40 on 8, 115 us, 5.3 TB/s, by head 106; one of 4000, 32 on 32 (33 MB),
+// Measured (heads of 128): 64 single tokens of up to 4096 positions, 32 query heads on 8 (277 MB), 61 us, 4.5 TB/s (heads of 64 52 us, 96 71, 32 41); three of 100 000, 40 on 8, 115 us, 5.3 TB/s, by head 108; one of 4000, 32 on 32 (33 MB),
 // 15 us. Single tokens' loop runs at the memory's rate; beside it 7 us until the first stage is there (lengths, the plan, page table, bytes, one after the other) and 4 us for every item that is done, joins among them.
-// Five rows of 24 sequences of up to 9000 (tiles of 24 rows) 118 us: 1.7 us a stage of 64 positions, a warp's chain of products and conversions with eight warps an SM (168 registers), and 5 us for a join.
+// Five rows of 24 sequences of up to 9000 (tiles of 24 rows) 117 us: 1.7 us a stage of 64 positions, a warp's chain of products and conversions with eight warps an SM (168 registers), and 5 us for a join.
 // Slower: K by mma.sync on bytes, with Q as two bytes of a 16-bit number; bytes as 2^-24 times themselves with their 128 taken off the sums (8 %); 32 positions a warp at a time; two chains of scores; rings of four stages;
 // what the warps found added up one after the other (61 -> 68 us); joins of two and four pieces of four elements at once (the same, and 2 %).
 

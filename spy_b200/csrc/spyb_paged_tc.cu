@@ -15,7 +15,7 @@
 // products for as many powers: 8192 tokens 524 us, 524 TFLOP/s. A step of 256 rows and 128 positions takes 2.4 us, in which 16 powers a clock alone take 1.1; the chain of
 // a tile - S, reading it, maximum, powers, P, product - is what bounds it, two tiles hide each other's. Beside the steps: 7 us until the first (lengths, the plan, page
 // table, Q and K), 5 us from one stretch to the next and 6 for the join of an item on a cut, which is what holds short contexts back (512 tokens at 1024: 28 us).
-// Bytes: 1500 tokens at 9111 399 us, 645 TFLOP/s; 512 at 32 768 421; five tokens of 24 sequences 166. Shared memory has more to do: operands are read as bytes and written as halves, and every row reads every position's two scales;
+// Bytes: 1500 tokens at 9111 392 us, 657 TFLOP/s; 512 at 32 768 408; heads of 64, 4096 tokens 222; five tokens of 24 sequences 158. Shared memory has more to do: operands are read as bytes and written as halves, and every row reads every position's two scales;
 // the probabilities' warps have 192 registers in place of 208. (Operands that are rounded products byte x scale: 331 us, and three times the error.)
 // Tried and left out: powers by polynomials on the FMA units for some of the columns (slower: their instructions are what is short), the two tiles taking turns by
 // barriers (no gain), both tiles on one tile's rows by every second step where only one has rows (24 x 5 rows 122 us against 119: memory bounds those steps).
@@ -396,7 +396,7 @@ __global__ void __launch_bounds__(TcShape<HD, KIND>::THREADS, 1) paged_tc_kernel
                     const bool above = !(BYTES && moved) && __any_sync(0xffffffffu, mine && top > m + Shape::SLACK);
                     if constexpr (BYTES) {
                         // That is a bound: the largest score and the largest scale need not be one position's, nor need the row see both. Where it is far above some row's maximum, rows go on to their own
-                        // largest weights: what a row does not see, or has no weight, takes nothing from its other weights. (Only rows that are far above going on: 434 us in place of 399 for 1500 tokens
+                        // largest weights: what a row does not see, or has no weight, takes nothing from its other weights. (Only rows that are far above going on: 434 us in place of 392 for 1500 tokens
                         // at 9111, for there are more such turns.)
                         if (above) {
                             float own_top[2] = {-CUDART_INF_F, -CUDART_INF_F};
